@@ -1,0 +1,295 @@
+// Pieces the paged-cache kernels share: kernel arguments, safe reads of a
+// request's device metadata, element conversions and the division of the
+// attention's work among the thread blocks.
+#pragma once
+
+#include <cuda_bf16.h>
+
+#include "ops.cuh"
+
+namespace etb {
+namespace paged {
+
+// The arithmetic on a request's metadata also runs on the host (its tests).
+#define ETB_HD __host__ __device__ __forceinline__
+template <typename I> ETB_HD I least_of(I a, I b) { return a < b ? a : b; }
+template <typename I> ETB_HD I most_of(I a, I b) { return a > b ? a : b; }
+
+struct Pools {
+  int64_t pages, page_stride, head_stride, token_stride;
+  int page_size, kv_heads, head_dim;
+};
+struct Batch {
+  const int64_t* offsets;
+  const int64_t* lengths;
+  const int32_t* table;
+  int* status;
+  int64_t tokens, columns;
+  int batch, capacity;  // capacity = columns * page_size
+};
+struct Rope {
+  const float* cos;
+  const float* sin;
+  int64_t rows;
+};
+
+__device__ __forceinline__ void report(int* status, int bit) {
+  if (status != nullptr) atomicOr(status, bit);
+}
+
+// A request's new tokens (rows first .. first + n - 1 of the tensors) and its
+// length, clamped to the tensors and the page table; `bad` holds the status
+// bits of what had to be clamped.
+struct Request {
+  int64_t first;
+  int n, len, bad;
+};
+ETB_HD Request load_request(const Batch& B, int b) {
+  const int64_t o0 = B.offsets[b], o1 = B.offsets[b + 1], l = B.lengths[b];
+  const int64_t a = least_of(most_of(o0, (int64_t)0), B.tokens);
+  const int64_t e = least_of(most_of(o1, a), B.tokens);
+  const int64_t len = least_of(most_of(l, (int64_t)0), (int64_t)B.capacity);
+  return Request{a, (int)(e - a), (int)len,
+                 ((a != o0 || e != o1) ? ET_B200_PAGED_BAD_OFFSET : 0) |
+                     (len != l ? ET_B200_PAGED_BAD_LENGTH : 0)};
+}
+
+// Element offset of slot 0 dims of `key` (0 <= key < capacity) of request b
+// in the pools for head h; -1 for a page outside the pool.
+ETB_HD int64_t key_offset(const Pools& P, const Batch& B, int b, int h,
+                                              int key) {
+  const int column = key / P.page_size, slot = key - column * P.page_size;
+  const int64_t page = B.table[(int64_t)b * B.columns + column];
+  if (page < 0 || page >= P.pages) return -1;
+  return page * P.page_stride + h * P.head_stride + slot * P.token_stride;
+}
+
+// ---- element types ------------------------------------------------------------------
+
+template <typename T> __device__ __forceinline__ float to_f32(T x);
+template <> __device__ __forceinline__ float to_f32<float>(float x) { return x; }
+template <> __device__ __forceinline__ float to_f32<__half>(__half x) { return __half2float(x); }
+template <> __device__ __forceinline__ float to_f32<__nv_bfloat16>(__nv_bfloat16 x) {
+  return __bfloat162float(x);
+}
+template <typename T> __device__ __forceinline__ T from_f32(float x);
+template <> __device__ __forceinline__ float from_f32<float>(float x) { return x; }
+template <> __device__ __forceinline__ __half from_f32<__half>(float x) {
+  return __float2half_rn(x);
+}
+template <> __device__ __forceinline__ __nv_bfloat16 from_f32<__nv_bfloat16>(float x) {
+  return __float2bfloat16_rn(x);
+}
+
+// RoPE of the pair (x0, x1) in the reference's rounding order
+// (native/a2_attention_provider.c:792-935).
+__device__ __forceinline__ void rotate(float& x0, float& x1, float c, float s) {
+  const float a = rn_mul(x0, c), b = rn_mul(x1, s), d = rn_mul(x0, s), e = rn_mul(x1, c);
+  x0 = rn_sub(a, b);
+  x1 = rn_add(d, e);
+}
+// The table row of a position: the last one for positions beyond the tables.
+__device__ __forceinline__ int64_t rope_row(const Rope& R, int64_t pos, int* status) {
+  if (pos >= R.rows) {
+    report(status, ET_B200_PAGED_BAD_ROPE);
+    return R.rows - 1;
+  }
+  return pos;
+}
+
+// ---- division of the attention's work -------------------------------------------------
+//
+// The rows of one (request, kv head) are its new tokens times the group of
+// query heads, token-major (row r: token r / group, head r % group), cut into
+// tiles of `rows`; a tile walks the keys its last token sees in blocks of
+// `keys`.  A unit is one (tile, block); the units of all requests, ordered by
+// request, head, tile, block, are divided evenly among the thread blocks
+// whatever the lengths are.  A tile cut by such a border leaves partial sums,
+// which a second kernel joins.
+struct Tiling {
+  int rows, keys, group, kv_heads;
+};
+ETB_HD int tile_count(const Tiling& t, const Request& r) {
+  return (int)(((int64_t)r.n * t.group + t.rows - 1) / t.rows);
+}
+// Keys that the last row of a tile sees (0 when it stands before position 0).
+ETB_HD int tile_visible(const Tiling& t, const Request& r, int tile) {
+  const int64_t last = least_of((int64_t)(tile + 1) * t.rows, (int64_t)r.n * t.group) - 1;
+  return most_of(0, r.len - r.n + (int)(last / t.group) + 1);
+}
+ETB_HD int tile_units(const Tiling& t, const Request& r, int tile) {
+  return most_of(1, (tile_visible(t, r, tile) + t.keys - 1) / t.keys);
+}
+ETB_HD int64_t head_units(const Tiling& t, const Request& r) {
+  const int tiles = tile_count(t, r);
+  int64_t s = 0;
+  for (int i = 0; i < tiles; i++) s += tile_units(t, r, i);
+  return s;
+}
+
+// Where a thread block stands: block `blk` of `nblk` of a tile.
+struct Place {
+  Request r;
+  int b, h, tile, tiles, blk, nblk;
+};
+ETB_HD void enter_tile(const Tiling& t, Place& p) {
+  p.blk = 0;
+  p.nblk = tile_units(t, p.r, p.tile);
+}
+// The next unit; past the last one of the batch b == B.batch.
+ETB_HD void advance(const Tiling& t, const Batch& B, Place& p) {
+  if (++p.blk < p.nblk) return;
+  if (++p.tile == p.tiles) {
+    p.tile = 0;
+    if (++p.h == t.kv_heads) {
+      p.h = 0;
+      do {
+        if (++p.b >= B.batch) return;
+        p.r = load_request(B, p.b);
+      } while (p.r.n == 0);
+      p.tiles = tile_count(t, p.r);
+    }
+  }
+  enter_tile(t, p);
+}
+
+struct Share {
+  int64_t units;  // of this thread block
+  int64_t per;    // of every thread block but the last
+};
+// This block's share of the units and where it begins; every thread of the
+// NT-thread block calls it and gets the same.
+template <int NT>
+__device__ Share divide(const Tiling& t, const Batch& B, int64_t least, Place& p) {
+  __shared__ int64_t warp_sum_s[NT / 32];
+  __shared__ int64_t found_s[2];
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  auto units_of = [&](int b) -> int64_t {
+    if (b >= B.batch) return 0;
+    const Request r = load_request(B, b);
+    if (r.bad != 0 && blockIdx.x == 0) report(B.status, r.bad);
+    return head_units(t, r) * t.kv_heads;
+  };
+  // inclusive scan over the block; *all receives the block's sum
+  auto scan = [&](int64_t v, int64_t* all) -> int64_t {
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const int64_t u = __shfl_up_sync(0xffffffffu, v, o);
+      if (lane >= o) v += u;
+    }
+    __syncthreads();
+    if (lane == 31) warp_sum_s[warp] = v;
+    __syncthreads();
+    int64_t before = 0, sum = 0;
+#pragma unroll
+    for (int w = 0; w < NT / 32; w++) {
+      if (w < warp) before += warp_sum_s[w];
+      sum += warp_sum_s[w];
+    }
+    *all = sum;
+    return v + before;
+  };
+  int64_t total = 0, mine = 0, incl = 0;
+  for (int base = 0; base < B.batch; base += NT) {
+    int64_t all;
+    mine = units_of(base + tid);
+    incl = scan(mine, &all);
+    total += all;
+  }
+  Share s;
+  s.per = max(least, (total + gridDim.x - 1) / gridDim.x);
+  const int64_t u0 = (int64_t)blockIdx.x * s.per;
+  s.units = max((int64_t)0, min(total - u0, s.per));
+  p.b = B.batch;
+  if (s.units == 0) return s;
+  int64_t before = 0;
+  for (int base = 0; base < B.batch; base += NT) {
+    int64_t all;
+    if (B.batch > NT) {
+      mine = units_of(base + tid);
+      incl = scan(mine, &all);
+    } else {
+      all = total;
+    }
+    const int64_t from = before + incl - mine;
+    if (from <= u0 && u0 < from + mine) {
+      found_s[0] = base + tid;
+      found_s[1] = u0 - from;
+    }
+    before += all;
+    if (u0 < before) break;
+  }
+  __syncthreads();
+  p.b = (int)found_s[0];
+  int64_t rest = found_s[1];
+  p.r = load_request(B, p.b);
+  p.tiles = tile_count(t, p.r);
+  const int64_t each = head_units(t, p.r);
+  p.h = (int)(rest / each);
+  rest -= p.h * each;
+  p.tile = 0;
+  enter_tile(t, p);
+  while (rest >= p.nblk) {
+    rest -= p.nblk;
+    p.tile++;
+    enter_tile(t, p);
+  }
+  p.blk = (int)rest;
+  return s;
+}
+
+// ---- joining of cut tiles --------------------------------------------------------------
+//
+// Workspace: per thread block a Cut (the tile it began and did not finish,
+// parts == 0 for none), then two slots of partial results: slot 0 for the
+// tile it continued, slot 1 for the tile it began.  A slot holds the
+// unnormalised sums [rows][dim] relative to the row's maximum, the maxima
+// (base 2) and the sums of exponentials.
+struct Cut {
+  int64_t first;
+  int n, h, tile, parts;
+};
+struct Joint {
+  Cut* cuts;
+  float* sums;   // [blocks][2][rows][dim]
+  float* stats;  // [blocks][2][2][rows]: maxima, sums of exponentials
+};
+constexpr size_t kCutBytes = 64;
+__host__ __device__ inline size_t joint_bytes(int blocks, int rows, int dim) {
+  return (size_t)blocks * (kCutBytes + 2 * sizeof(float) * (size_t)rows * (dim + 2));
+}
+inline Joint joint_of(void* ws, int blocks, int rows, int dim) {
+  Joint j;
+  j.cuts = static_cast<Cut*>(ws);
+  j.sums = reinterpret_cast<float*>(static_cast<char*>(ws) + (size_t)blocks * kCutBytes);
+  j.stats = j.sums + (size_t)blocks * 2 * rows * dim;
+  return j;
+}
+
+struct AttendArgs {
+  Pools pools;
+  Batch batch;
+  Rope rope;
+  Tiling tiling;
+  Joint joint;
+  const void* keys;
+  const void* values;
+  const void* q;
+  void* o;
+  float* lse;
+  int64_t q_stride, o_stride, least;
+  int q_heads;
+  float scale_log2;  // log2(e) / sqrt(head_dim)
+};
+
+// Host pieces of the entry points.
+int32_t check_cache(const et_b200_paged_cache_v1* c, et_kernel_error* e, const char* op);
+int32_t check_batch(const et_b200_paged_batch_v1* b, const et_b200_paged_cache_v1* c,
+                    et_kernel_error* e, const char* op);
+int32_t check_rope(const et_b200_paged_rope_v1* r, et_kernel_error* e, const char* op);
+Pools pools_of(const et_b200_paged_cache_v1* c);
+Batch batch_of(const et_b200_paged_batch_v1* b, const et_b200_paged_cache_v1* c);
+Rope rope_of(const et_b200_paged_rope_v1* r);
+
+}  // namespace paged
+}  // namespace etb

@@ -1,0 +1,650 @@
+// Causal attention of new tokens over a paged cache
+// (et_b200_paged_attention_v1): the kernel for any page size, head_dim and
+// type, and the joining of cut tiles.
+//
+// o = sum_j p_j v_j / sum_j p_j, p_j = 2^(s_j - m), s_j = log2(e) scale q'.k_j,
+// m the running maximum.  A thread block takes its share of the (tile, block)
+// units (paged.cuh): tiles of 16 WM rows, blocks of BK keys.  K and V arrive
+// by 16-byte cp.async in a ring of STAGES blocks (rows XOR-swizzled by 16-byte
+// pieces, so ldmatrix and the f32 reads of V are free of bank conflicts); the
+// key addresses of a block are looked up one block ahead of its copies.  Warp
+// (wm, wk) takes 16 rows and BK / WK keys of each block with its own maxima,
+// sums and accumulators (mma.sync m16n8k16, or for f32 m16n8k8 as 3xTF32:
+// hi hi + hi lo + lo hi of operands rounded to TF32 pairs), which are joined
+// where a tile ends.  With few rows (a decoding step) reading the cache
+// bounds it: one tile of 16 rows, warps split along the keys.
+#include <math.h>
+
+#include <type_traits>
+
+#include "attention_tc.cuh"
+#include "paged.cuh"
+
+namespace etb {
+namespace {
+
+using namespace paged;
+
+// ---- warp matrix pieces -----------------------------------------------------------------
+
+__device__ __forceinline__ void ldsm4(uint32_t (&r)[4], uint32_t addr) {
+  asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0,%1,%2,%3}, [%4];"
+               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
+               : "r"(addr)
+               : "memory");
+}
+__device__ __forceinline__ void ldsm4t(uint32_t (&r)[4], uint32_t addr) {
+  asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0,%1,%2,%3}, [%4];"
+               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
+               : "r"(addr)
+               : "memory");
+}
+__device__ __forceinline__ uint32_t lds32(uint32_t addr) {
+  uint32_t v;
+  asm volatile("ld.shared.b32 %0, [%1];" : "=r"(v) : "r"(addr) : "memory");
+  return v;
+}
+template <typename T>
+__device__ __forceinline__ void mma16(float (&d)[4], const uint32_t (&a)[4], uint32_t b0,
+                                      uint32_t b1) {
+  if constexpr (std::is_same_v<T, __half>)
+    asm volatile(
+        "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, "
+        "{%8,%9}, {%0,%1,%2,%3};"
+        : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+        : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+  else
+    asm volatile(
+        "mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, "
+        "{%8,%9}, {%0,%1,%2,%3};"
+        : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+        : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+__device__ __forceinline__ void mma_tf32(float (&d)[4], const uint32_t (&a)[4], uint32_t b0,
+                                         uint32_t b1) {
+  asm volatile(
+      "mma.sync.aligned.m16n8k8.row.col.f32.tf32.tf32.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, "
+      "{%8,%9}, {%0,%1,%2,%3};"
+      : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+      : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+// x = hi + lo + r with hi, lo TF32 values, |r| <= 2^-22 |x|
+__device__ __forceinline__ void pair_tf32(uint32_t x, uint32_t& hi, uint32_t& lo) {
+  asm("cvt.rna.tf32.f32 %0, %1;" : "=r"(hi) : "f"(__uint_as_float(x)));
+  const float rest = __uint_as_float(x) - __uint_as_float(hi);
+  asm("cvt.rna.tf32.f32 %0, %1;" : "=r"(lo) : "f"(rest));
+}
+template <typename T>
+__device__ __forceinline__ uint32_t pack2(float a, float b) {
+  if constexpr (std::is_same_v<T, __half>) {
+    const __half2 h = __floats2half2_rn(a, b);
+    return *reinterpret_cast<const uint32_t*>(&h);
+  } else {
+    const __nv_bfloat162 h = __floats2bfloat162_rn(a, b);
+    return *reinterpret_cast<const uint32_t*>(&h);
+  }
+}
+__device__ __forceinline__ void cp16(uint32_t dst, const void* src, bool full) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src),
+               "r"(full ? 16 : 0)
+               : "memory");
+}
+__device__ __forceinline__ void cp_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int N>
+__device__ __forceinline__ void cp_wait() {
+  asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
+}
+
+// Two neighbouring outputs; one store where the address allows it.
+template <typename T>
+__device__ __forceinline__ void store2(T* dst, float a, float b) {
+  if ((reinterpret_cast<uintptr_t>(dst) & (2 * sizeof(T) - 1)) == 0) {
+    if constexpr (sizeof(T) == 4)
+      *reinterpret_cast<float2*>(dst) = make_float2(a, b);
+    else
+      *reinterpret_cast<uint32_t*>(dst) = pack2<T>(a, b);
+  } else {
+    dst[0] = from_f32<T>(a);
+    dst[1] = from_f32<T>(b);
+  }
+}
+
+// ---- the kernel -------------------------------------------------------------------------
+
+template <typename T, int DH_, int WM_, int WK_, int BK_, int STAGES_>
+struct Shape {
+  static constexpr int DH = DH_, WM = WM_, WK = WK_, BK = BK_, STAGES = STAGES_;
+  static constexpr int NT = 32 * WM * WK, BM = 16 * WM, KW = BK / WK;
+  static constexpr int ROW = DH * (int)sizeof(T), PIECES = ROW / 16;  // of one key
+  static constexpr int TILE = BK * ROW, STAGE = 2 * TILE;
+  static constexpr int Q_BYTES = BM * ROW;
+  static constexpr int MERGE = (WK - 1) * BM * DH * 4;
+  static constexpr int KOFF = STAGES * STAGE + Q_BYTES;
+  static constexpr int SMEM = KOFF + 2 * BK * 8 + WK * BM * 8;
+  static_assert(KW % 16 == 0 && BK <= NT * 2, "keys per warp");
+  static_assert(MERGE <= STAGE, "the joining of warps reuses a stage");
+  static_assert(SMEM <= 232448, "shared memory");
+  // byte of 16-byte piece c of a row
+  __device__ static uint32_t at(int row, int c) {
+    const int x = PIECES >= 8 ? (row & 7) : ((row >> 1) & 3);
+    return (uint32_t)(row * ROW + ((c ^ x) << 4));
+  }
+};
+
+template <typename T, typename S>
+__global__ void __launch_bounds__(S::NT)
+paged_attention_kernel(AttendArgs a) {
+  constexpr int DH = S::DH, BM = S::BM, BK = S::BK, KW = S::KW, NT = S::NT, WK = S::WK;
+  constexpr bool F32 = sizeof(T) == 4;
+  constexpr int KSTEP = F32 ? 8 : 16;  // dims (or keys) per matrix instruction
+  extern __shared__ __align__(128) uint8_t smem[];
+  int64_t* koff = reinterpret_cast<int64_t*>(smem + S::KOFF);
+  float* join_m = reinterpret_cast<float*>(smem + S::KOFF + 2 * BK * 8);
+  float* join_l = join_m + WK * BM;
+  const uint32_t base = smem_u32(smem);
+  const uint32_t qs = base + S::STAGES * S::STAGE;
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  const int wm = warp / WK, wk = warp % WK;
+  const int dim = a.pools.head_dim, group = a.tiling.group;
+  const T* keys = static_cast<const T*>(a.keys);
+  const T* values = static_cast<const T*>(a.values);
+  // lets the joining kernel start its launch; it waits for this one's results
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+
+  Place p;
+  const Share share = divide<NT>(a.tiling, a.batch, a.least, p);
+  Cut cut{0, 0, 0, 0, 0};
+  if (share.units > 0) {
+    const int units = (int)share.units;
+    Place kp = p;        // the block whose key addresses are looked up next
+    int looked = 0;
+    auto look_up = [&]() {  // addresses of block `looked` into slot looked & 1
+      if (looked < units) {
+        const int visible = tile_visible(a.tiling, kp.r, kp.tile);
+        for (int i = tid; i < BK; i += NT) {
+          const int key = kp.blk * BK + i;
+          int64_t off = -1;
+          if (key < visible) {
+            off = key_offset(a.pools, a.batch, kp.b, kp.h, key);
+            if (off < 0) report(a.batch.status, ET_B200_PAGED_BAD_PAGE);
+          }
+          koff[(looked & 1) * BK + i] = off;
+        }
+        advance(a.tiling, a.batch, kp);
+      }
+      looked++;
+    };
+    auto issue = [&](int u) {  // copies of unit u into stage u % STAGES
+      if (u < units) {
+        const uint32_t st = base + (uint32_t)(u % S::STAGES) * S::STAGE;
+        for (int i = tid; i < BK * S::PIECES; i += NT) {
+          const int row = i / S::PIECES, c = i % S::PIECES;
+          const int64_t off = koff[(u & 1) * BK + row];
+          const bool full = off >= 0 && c * (16 / (int)sizeof(T)) < dim;
+          const int64_t e = full ? off + c * (16 / (int)sizeof(T)) : 0;
+          const uint32_t dst = st + S::at(row, c);
+          cp16(dst, keys + e, full);
+          cp16(dst + S::TILE, values + e, full);
+        }
+      }
+      cp_commit();
+    };
+    look_up();
+    __syncthreads();
+#pragma unroll
+    for (int s = 0; s < S::STAGES - 1; s++) {
+      issue(s);
+      look_up();
+      __syncthreads();
+    }
+
+    float o[DH / 8][4];
+    float m[2], l[2];
+    int vis[2], vis_min = 0;
+    bool whole = false;  // this block began the tile
+    for (int u = 0; u < units; u++) {
+      cp_wait<S::STAGES - 2>();
+      __syncthreads();  // stage u is complete; stage u - 1 and its addresses are free
+      issue(u + S::STAGES - 1);
+      look_up();
+      const bool first = u == 0 || p.blk == 0;
+      if (first) {  // a new tile: its queries, rotated
+        whole = p.blk == 0;
+        const int rows = (int)min((int64_t)BM, (int64_t)p.r.n * group - (int64_t)p.tile * BM);
+        for (int i = tid; i < BM * DH / 2; i += NT) {
+          const int r = i / (DH / 2), d = 2 * (i % (DH / 2));
+          float x0 = 0.0f, x1 = 0.0f;
+          if (r < rows && d < dim) {
+            const int64_t g = (int64_t)p.tile * BM + r;
+            const int t = (int)(g / group), j = (int)(g % group);
+            const T* src = static_cast<const T*>(a.q) + (p.r.first + t) * a.q_stride +
+                           (int64_t)(p.h * group + j) * dim + d;
+            x0 = to_f32<T>(src[0]);
+            x1 = to_f32<T>(src[1]);
+            const int pos = p.r.len - p.r.n + t;
+            if (a.rope.cos != nullptr && pos >= 0) {
+              const int64_t at = rope_row(a.rope, pos, a.batch.status) * (dim / 2) + d / 2;
+              rotate(x0, x1, a.rope.cos[at], a.rope.sin[at]);
+            }
+          }
+          T* dst = reinterpret_cast<T*>(smem + S::STAGES * S::STAGE + S::at(r, d * (int)sizeof(T) / 16)) +
+                   d % (16 / (int)sizeof(T));
+          dst[0] = from_f32<T>(x0);
+          dst[1] = from_f32<T>(x1);
+        }
+#pragma unroll
+        for (int i = 0; i < DH / 8; i++) o[i][0] = o[i][1] = o[i][2] = o[i][3] = 0.0f;
+#pragma unroll
+        for (int i = 0; i < 2; i++) {
+          m[i] = -INFINITY;
+          l[i] = 0.0f;
+          const int r = wm * 16 + lane / 4 + 8 * i;
+          const int64_t g = (int64_t)p.tile * BM + r;
+          vis[i] = r < rows ? max(0, p.r.len - p.r.n + (int)(g / group) + 1) : 0;
+        }
+        vis_min = rows == BM ? max(0, p.r.len - p.r.n + (int)((int64_t)p.tile * BM / group) + 1) : 0;
+        __syncthreads();
+      }
+      const uint32_t kt = base + (uint32_t)(u % S::STAGES) * S::STAGE, vt = kt + S::TILE;
+
+      // scores of this warp's KW keys
+      float s[KW / 8][4];
+#pragma unroll
+      for (int i = 0; i < KW / 8; i++) s[i][0] = s[i][1] = s[i][2] = s[i][3] = 0.0f;
+#pragma unroll
+      for (int ks = 0; ks < DH / KSTEP; ks++) {
+        uint32_t qa[4];
+        ldsm4(qa, qs + S::at(wm * 16 + (lane & 15), 2 * ks + (lane >> 4)));
+        uint32_t qh[4], ql[4];
+        if constexpr (F32) {
+#pragma unroll
+          for (int i = 0; i < 4; i++) pair_tf32(qa[i], qh[i], ql[i]);
+        }
+#pragma unroll
+        for (int n = 0; n < KW / 16; n++) {
+          uint32_t kb[4];
+          ldsm4(kb, kt + S::at(wk * KW + 16 * n + ((lane >> 4) << 3) + (lane & 7),
+                               2 * ks + ((lane >> 3) & 1)));
+          if constexpr (F32) {
+            uint32_t kh[4], kl[4];
+#pragma unroll
+            for (int i = 0; i < 4; i++) pair_tf32(kb[i], kh[i], kl[i]);
+#pragma unroll
+            for (int i = 0; i < 2; i++) {
+              mma_tf32(s[2 * n + i], ql, kh[2 * i], kh[2 * i + 1]);
+              mma_tf32(s[2 * n + i], qh, kl[2 * i], kl[2 * i + 1]);
+              mma_tf32(s[2 * n + i], qh, kh[2 * i], kh[2 * i + 1]);
+            }
+          } else {
+            mma16<T>(s[2 * n], qa, kb[0], kb[1]);
+            mma16<T>(s[2 * n + 1], qa, kb[2], kb[3]);
+          }
+        }
+      }
+      // running maxima, probabilities (rows lane / 4 and lane / 4 + 8)
+      const int key0 = p.blk * BK + wk * KW;
+      const bool full = key0 + KW <= vis_min;
+      float top[2] = {-INFINITY, -INFINITY};
+#pragma unroll
+      for (int i = 0; i < KW / 8; i++)
+#pragma unroll
+        for (int e = 0; e < 4; e++) {
+          const int key = key0 + 8 * i + 2 * (lane & 3) + (e & 1);
+          s[i][e] = full || key < vis[e >> 1] ? s[i][e] * a.scale_log2 : -INFINITY;
+          top[e >> 1] = fmaxf(top[e >> 1], s[i][e]);
+        }
+      float factor[2], from[2];
+#pragma unroll
+      for (int i = 0; i < 2; i++) {
+        top[i] = fmaxf(top[i], __shfl_xor_sync(0xffffffffu, top[i], 1));
+        top[i] = fmaxf(top[i], __shfl_xor_sync(0xffffffffu, top[i], 2));
+        const float now = fmaxf(m[i], top[i]);
+        from[i] = now == -INFINITY ? 0.0f : now;
+        factor[i] = ex2(m[i] - from[i]);
+        m[i] = now;
+        l[i] *= factor[i];
+      }
+#pragma unroll
+      for (int i = 0; i < KW / 8; i++)
+#pragma unroll
+        for (int e = 0; e < 4; e++) {
+          s[i][e] = ex2(s[i][e] - from[e >> 1]);
+          l[e >> 1] += s[i][e];
+        }
+      if (__any_sync(0xffffffffu, factor[0] != 1.0f || factor[1] != 1.0f)) {
+#pragma unroll
+        for (int i = 0; i < DH / 8; i++) {
+          o[i][0] *= factor[0];
+          o[i][1] *= factor[0];
+          o[i][2] *= factor[1];
+          o[i][3] *= factor[1];
+        }
+      }
+      // o += P V
+      if constexpr (F32) {
+        // key 2 (lane % 4) + {0, 1} of each 8 stands at matrix k lane % 4 + {0, 4},
+        // so the score registers are the A operand as they lie
+#pragma unroll
+        for (int kk = 0; kk < KW / 8; kk++) {
+          uint32_t ph[4], pl[4];
+#pragma unroll
+          for (int i = 0; i < 4; i++)
+            pair_tf32(__float_as_uint(s[kk][((i & 1) << 1) | (i >> 1)]), ph[i], pl[i]);
+          const int row = wk * KW + 8 * kk + 2 * (lane & 3);
+#pragma unroll
+          for (int n = 0; n < DH / 8; n++) {
+            const int d = 8 * n + lane / 4;
+            uint32_t vh[2], vl[2];
+#pragma unroll
+            for (int i = 0; i < 2; i++)
+              pair_tf32(lds32(vt + S::at(row + i, d / 4) + 4 * (d & 3)), vh[i], vl[i]);
+            mma_tf32(o[n], pl, vh[0], vh[1]);
+            mma_tf32(o[n], ph, vl[0], vl[1]);
+            mma_tf32(o[n], ph, vh[0], vh[1]);
+          }
+        }
+      } else {
+#pragma unroll
+        for (int kk = 0; kk < KW / 16; kk++) {
+          uint32_t pa[4];
+#pragma unroll
+          for (int i = 0; i < 4; i++)
+            pa[i] = pack2<T>(s[2 * kk + (i >> 1)][2 * (i & 1)], s[2 * kk + (i >> 1)][2 * (i & 1) + 1]);
+#pragma unroll
+          for (int n = 0; n < DH / 16; n++) {
+            uint32_t vb[4];
+            ldsm4t(vb, vt + S::at(wk * KW + 16 * kk + (lane & 15), 2 * n + (lane >> 4)));
+            mma16<T>(o[2 * n], pa, vb[0], vb[1]);
+            mma16<T>(o[2 * n + 1], pa, vb[2], vb[3]);
+          }
+        }
+      }
+
+      const bool tile_ends = p.blk + 1 == p.nblk;
+      if (tile_ends || u + 1 == units) {
+#pragma unroll
+        for (int i = 0; i < 2; i++) {
+          l[i] += __shfl_xor_sync(0xffffffffu, l[i], 1);
+          l[i] += __shfl_xor_sync(0xffffffffu, l[i], 2);
+        }
+        const int r0 = wm * 16 + lane / 4;
+        if constexpr (WK > 1) {
+          __syncthreads();  // every warp is done with the stage
+          float* merge = reinterpret_cast<float*>(smem + (u % S::STAGES) * S::STAGE);
+          if ((lane & 3) == 0) {
+#pragma unroll
+            for (int i = 0; i < 2; i++) {
+              join_m[wk * BM + r0 + 8 * i] = m[i];
+              join_l[wk * BM + r0 + 8 * i] = l[i];
+            }
+          }
+          if (wk > 0) {
+            float* mine = merge + ((wk - 1) * S::WM + wm) * 16 * DH + lane * 4;
+#pragma unroll
+            for (int n = 0; n < DH / 8; n++)
+              *reinterpret_cast<float4*>(mine + n * 128) = make_float4(o[n][0], o[n][1], o[n][2], o[n][3]);
+          }
+          __syncthreads();
+          if (wk == 0) {
+            float f[WK][2];
+#pragma unroll
+            for (int i = 0; i < 2; i++) {
+              float all = m[i];
+#pragma unroll
+              for (int w = 1; w < WK; w++) all = fmaxf(all, join_m[w * BM + r0 + 8 * i]);
+              const float ref = all == -INFINITY ? 0.0f : all;
+              f[0][i] = ex2(m[i] - ref);
+              l[i] *= f[0][i];
+#pragma unroll
+              for (int w = 1; w < WK; w++) {
+                f[w][i] = ex2(join_m[w * BM + r0 + 8 * i] - ref);
+                l[i] += f[w][i] * join_l[w * BM + r0 + 8 * i];
+              }
+              m[i] = all;
+            }
+#pragma unroll
+            for (int n = 0; n < DH / 8; n++) {
+#pragma unroll
+              for (int e = 0; e < 4; e++) o[n][e] *= f[0][e >> 1];
+#pragma unroll
+              for (int w = 1; w < WK; w++) {
+                const float4 x = *reinterpret_cast<const float4*>(
+                    merge + ((w - 1) * S::WM + wm) * 16 * DH + n * 128 + lane * 4);
+                o[n][0] += f[w][0] * x.x;
+                o[n][1] += f[w][0] * x.y;
+                o[n][2] += f[w][1] * x.z;
+                o[n][3] += f[w][1] * x.w;
+              }
+            }
+          }
+        }
+        const bool done = whole && tile_ends;
+        if (wk == 0) {
+          const int slot = 2 * (int)blockIdx.x + (whole ? 1 : 0);
+#pragma unroll
+          for (int i = 0; i < 2; i++) {
+            const int r = r0 + 8 * i;
+            const int64_t g = (int64_t)p.tile * BM + r;
+            if (done) {
+              if (g < (int64_t)p.r.n * group) {
+                const int64_t t = p.r.first + g / group;
+                const int h = p.h * group + (int)(g % group);
+                const float inv = l[i] > 0.0f ? 1.0f / l[i] : 0.0f;
+                T* dst = static_cast<T*>(a.o) + t * a.o_stride + (int64_t)h * dim;
+#pragma unroll
+                for (int n = 0; n < DH / 8; n++) {
+                  const int d = 8 * n + 2 * (lane & 3);
+                  if (d < dim) store2<T>(dst + d, o[n][2 * i] * inv, o[n][2 * i + 1] * inv);
+                }
+                if (a.lse != nullptr && (lane & 3) == 0)
+                  a.lse[t * a.q_heads + h] = l[i] > 0.0f ? m[i] * kLn2 + logf(l[i]) : -INFINITY;
+              }
+            } else {
+              float* dst = a.joint.sums + ((int64_t)slot * BM + r) * DH;
+#pragma unroll
+              for (int n = 0; n < DH / 8; n++)
+                *reinterpret_cast<float2*>(dst + 8 * n + 2 * (lane & 3)) =
+                    make_float2(o[n][2 * i], o[n][2 * i + 1]);
+              if ((lane & 3) == 0) {
+                a.joint.stats[(int64_t)slot * 2 * BM + r] = m[i];
+                a.joint.stats[((int64_t)slot * 2 + 1) * BM + r] = l[i];
+              }
+            }
+          }
+        }
+        if (whole && !tile_ends) {
+          const int64_t rest = p.nblk - p.blk - 1;
+          cut = Cut{p.r.first, p.r.n, p.h, p.tile, 1 + (int)((rest + share.per - 1) / share.per)};
+        }
+      }
+      advance(a.tiling, a.batch, p);
+    }
+    cp_wait<0>();
+  }
+  if (tid == 0) a.joint.cuts[blockIdx.x] = cut;
+}
+
+// Joins the parts of the tile that thread block blockIdx.x of the attention
+// began and did not finish; blockIdx.y takes rows y, y + gridDim.y, ...
+template <typename T>
+__global__ void __launch_bounds__(128) paged_join_kernel(AttendArgs a, int dim_padded) {
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+  const int c = blockIdx.x, rows = a.tiling.rows, group = a.tiling.group;
+  const Cut cut = a.joint.cuts[c];
+  if (cut.parts == 0) return;
+  const int dim = a.pools.head_dim;
+  auto slot_of = [&](int part) { return part == 0 ? 2 * c + 1 : 2 * (c + part); };
+  for (int r = blockIdx.y; r < rows; r += gridDim.y) {
+    const int64_t g = (int64_t)cut.tile * rows + r;
+    if (g >= (int64_t)cut.n * group) return;
+    float m = -INFINITY;
+    for (int i = 0; i < cut.parts; i++)
+      m = fmaxf(m, a.joint.stats[(int64_t)slot_of(i) * 2 * rows + r]);
+    const float ref = m == -INFINITY ? 0.0f : m;
+    float l = 0.0f, x0 = 0.0f, x1 = 0.0f;
+    const int d = 2 * threadIdx.x;
+    for (int i = 0; i < cut.parts; i++) {
+      const int64_t s = slot_of(i);
+      const float f = ex2(a.joint.stats[s * 2 * rows + r] - ref);
+      l += f * a.joint.stats[(s * 2 + 1) * rows + r];
+      if (d < dim) {
+        const float2 x = *reinterpret_cast<const float2*>(a.joint.sums + (s * rows + r) * dim_padded + d);
+        x0 += f * x.x;
+        x1 += f * x.y;
+      }
+    }
+    const int64_t t = cut.first + g / group;
+    const int h = cut.h * group + (int)(g % group);
+    const float inv = l > 0.0f ? 1.0f / l : 0.0f;
+    if (d < dim) store2<T>(static_cast<T*>(a.o) + t * a.o_stride + (int64_t)h * dim + d, x0 * inv, x1 * inv);
+    if (a.lse != nullptr && threadIdx.x == 0)
+      a.lse[t * a.q_heads + h] = l > 0.0f ? m * kLn2 + logf(l) : -INFINITY;
+  }
+}
+
+// ---- launching --------------------------------------------------------------------------
+
+// Padded head_dim of the kernels: 32, 64, 128 or 256.
+int padded(int64_t dim) { return dim <= 32 ? 32 : dim <= 64 ? 64 : dim <= 128 ? 128 : 256; }
+
+constexpr int kMostPerSm = 2;  // resident thread blocks per SM that the workspace allows for
+
+// Resident thread blocks of a kernel per SM (at most kMostPerSm), per device
+// (the attribute that admits its shared memory is set on the way).
+template <auto Kernel>
+int resident_blocks(int threads, int smem) {
+  static std::atomic<int> known[64];
+  int dev = 0;
+  cudaGetDevice(&dev);
+  if (dev >= 0 && dev < 64) {
+    const int n = known[dev].load(std::memory_order_relaxed);
+    if (n > 0) return n;
+  }
+  cudaFuncSetAttribute(Kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+  int n = 0;
+  cudaOccupancyMaxActiveBlocksPerMultiprocessor(&n, Kernel, threads, smem);
+  n = n < 1 ? 1 : n > kMostPerSm ? kMostPerSm : n;
+  if (dev >= 0 && dev < 64) known[dev].store(n, std::memory_order_relaxed);
+  return n;
+}
+
+template <typename T, typename S>
+bool launch_shape(AttendArgs& a, void* ws, cudaStream_t stream) {
+  const int resident = resident_blocks<paged_attention_kernel<T, S>>(S::NT, S::SMEM);
+  const int blocks = resident * sm_count();
+  a.tiling.rows = S::BM;
+  a.tiling.keys = S::BK;
+  a.least = 4;
+  a.joint = joint_of(ws, blocks, S::BM, S::DH);
+  paged_attention_kernel<T, S><<<blocks, S::NT, S::SMEM, stream>>>(a);
+  cudaLaunchConfig_t cfg{};
+  cfg.gridDim = dim3(blocks, S::BM < 16 ? S::BM : 16);
+  cfg.blockDim = dim3(128);
+  cfg.stream = stream;
+  cudaLaunchAttribute attr{};
+  attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr.val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = &attr;
+  cfg.numAttrs = 1;
+  cudaLaunchKernelEx(&cfg, paged_join_kernel<T>, a, (int)S::DH);
+  count_launch(2);
+  return true;
+}
+
+template <typename T, int DH>
+void launch_dim(AttendArgs& a, int64_t max_new, void* ws, cudaStream_t stream) {
+  constexpr bool F32 = sizeof(T) == 4;
+  // up to 16 rows per kv head: one row tile, warps along the keys; more: 64-row
+  // tiles, every warp walks all keys
+  if (max_new * a.tiling.group <= 16) {
+    if constexpr (F32 && DH == 256) launch_shape<T, Shape<T, DH, 1, 2, 32, 3>>(a, ws, stream);
+    else launch_shape<T, Shape<T, DH, 1, 4, 64, 3>>(a, ws, stream);
+  } else {
+    if constexpr (F32 && DH == 256) launch_shape<T, Shape<T, DH, 4, 1, 32, 2>>(a, ws, stream);
+    else launch_shape<T, Shape<T, DH, 4, 1, 64, 2>>(a, ws, stream);
+  }
+}
+
+template <typename T>
+void launch_type(AttendArgs& a, int64_t max_new, void* ws, cudaStream_t stream) {
+  switch (padded(a.pools.head_dim)) {
+    case 32: return launch_dim<T, 32>(a, max_new, ws, stream);
+    case 64: return launch_dim<T, 64>(a, max_new, ws, stream);
+    case 128: return launch_dim<T, 128>(a, max_new, ws, stream);
+    default: return launch_dim<T, 256>(a, max_new, ws, stream);
+  }
+}
+
+}  // namespace
+}  // namespace etb
+
+using namespace etb;
+using namespace etb::paged;
+
+extern "C" {
+
+size_t et_b200_paged_attention_workspace_bytes_v1(const et_b200_paged_cache_v1* c,
+                                                  int64_t q_heads) {
+  if (check_cache(c, nullptr, "paged-attention-workspace") || q_heads < 1 ||
+      q_heads % c->kv_heads != 0)
+    return 0;
+  return joint_bytes(kMostPerSm * sm_count(), 64, padded(c->head_dim));
+}
+
+int32_t et_b200_paged_attention_v1(const et_b200_paged_cache_v1* c,
+                                   const et_b200_paged_batch_v1* b,
+                                   const et_b200_paged_rope_v1* rope, int64_t q_heads,
+                                   const void* q, int64_t q_stride, void* o, int64_t o_stride,
+                                   float* lse, void* workspace, size_t workspace_bytes,
+                                   void* stream, et_kernel_error* e) {
+  const char* op = "paged-attention";
+  if (int32_t r = check_cache(c, e, op)) return r;
+  if (int32_t r = check_batch(b, c, e, op)) return r;
+  if (int32_t r = check_rope(rope, e, op)) return r;
+  if (q_heads < 1 || q_heads > 65536 || q_heads % c->kv_heads != 0)
+    return set_error(e, ET_KERNEL_ERROR_SHAPE_MISMATCH, ET_KERNEL_CODE_INVALID_SHAPE, op,
+                     "q_heads must be a multiple of the cache's kv_heads");
+  if (b->tokens > 0 && b->batch > 0) {
+    const int64_t row = q_heads * c->head_dim, size = c->dtype == ET_B200_DTYPE_F32 ? 4 : 2;
+    if (q == nullptr || o == nullptr)
+      return set_error(e, ET_KERNEL_ERROR_INVALID_ARGUMENT, ET_KERNEL_CODE_NULL_ARGUMENT, op,
+                       "q and o are required");
+    if (q_stride < row || o_stride < row || q_stride > (int64_t)1 << 31 ||
+        o_stride > (int64_t)1 << 31)
+      return set_error(e, ET_KERNEL_ERROR_NONCONTIGUOUS, ET_KERNEL_CODE_INVALID_BUFFER, op,
+                       "rows of q or o overlap or lie too far apart");
+    if ((reinterpret_cast<uintptr_t>(q) | reinterpret_cast<uintptr_t>(o)) % size != 0)
+      return set_error(e, ET_KERNEL_ERROR_INVALID_ARGUMENT, ET_KERNEL_CODE_INVALID_BUFFER, op,
+                       "q and o must be aligned to their elements");
+    if (workspace == nullptr || (reinterpret_cast<uintptr_t>(workspace) & 255) != 0 ||
+        workspace_bytes < et_b200_paged_attention_workspace_bytes_v1(c, q_heads))
+      return set_error(e, ET_KERNEL_ERROR_INVALID_ARGUMENT, ET_KERNEL_CODE_BUFFER_TOO_SMALL, op,
+                       "workspace is smaller than et_b200_paged_attention_workspace_bytes_v1 or "
+                       "not 256-byte aligned");
+    AttendArgs a{};
+    a.pools = pools_of(c);
+    a.batch = batch_of(b, c);
+    a.rope = rope_of(rope);
+    a.tiling.group = (int)(q_heads / c->kv_heads);
+    a.tiling.kv_heads = (int)c->kv_heads;
+    a.keys = c->keys;
+    a.values = c->values;
+    a.q = q;
+    a.o = o;
+    a.lse = lse;
+    a.q_stride = q_stride;
+    a.o_stride = o_stride;
+    a.q_heads = (int)q_heads;
+    a.scale_log2 = kLog2e / sqrtf((float)c->head_dim);
+    auto st = static_cast<cudaStream_t>(stream);
+    if (c->dtype == ET_B200_DTYPE_F32) launch_type<float>(a, b->max_new, workspace, st);
+    else if (c->dtype == ET_B200_DTYPE_F16) launch_type<__half>(a, b->max_new, workspace, st);
+    else launch_type<__nv_bfloat16>(a, b->max_new, workspace, st);
+    const cudaError_t status = cudaGetLastError();
+    if (status != cudaSuccess) return cuda_error(e, status, op);
+  }
+  if (e) memset(e, 0, sizeof(*e));
+  return 0;
+}
+
+}  // extern "C"

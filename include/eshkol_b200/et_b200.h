@@ -150,6 +150,138 @@ int32_t et_b200_attention_backward_v1(
     size_t workspace_bytes, int32_t workspace_from_forward, void *stream,
     et_kernel_error *error);
 
+/* ------------------------------------------------------------ serving
+ * Decoding for many requests at once on device tensors: appending keys and
+ * values to a paged cache (the keys' RoPE applied on the way), causal
+ * attention of the new tokens over it, and sampling the next token from
+ * logits.  No reference counterpart: the reference caches one dense
+ * [batch, kv_heads, capacity, head_dim] block per layer (the A2 KV cache
+ * below) and leaves sampling to its host.  The arithmetic is the A2
+ * provider's (native/a2_attention_provider.c:669-716, rope :792-935).
+ * All calls enqueue on `stream` (a cudaStream_t, NULL = the legacy default
+ * stream) of the current device, return without synchronising, allocate
+ * nothing, keep nothing between calls and can be captured in a CUDA graph.
+ * Pointers are device memory of the current device unless said otherwise. */
+enum { ET_B200_DTYPE_F32 = 0, ET_B200_DTYPE_F16 = 1, ET_B200_DTYPE_BF16 = 2 };
+
+/* Two pools of pages, one layer's keys and values, both addressed as element
+ * page * page_stride + head * head_stride + slot * token_stride + d.  Any
+ * page_size >= 1; head_dim a multiple of 8 up to 256; pools 16-byte aligned
+ * and strides multiples of 16 bytes. */
+typedef struct et_b200_paged_cache_v1 {
+  size_t struct_size;
+  void *keys;
+  void *values;
+  int64_t pages, page_size, kv_heads, head_dim;
+  int64_t page_stride, head_stride, token_stride;
+  uint32_t dtype; /* ET_B200_DTYPE_*, of the pools and of q, k, v and o */
+  uint32_t reserved;
+} et_b200_paged_cache_v1;
+
+/* One step's requests.  Request b brings the rows offsets[b] .. offsets[b + 1]
+ * - 1 of the token-major tensors as its last new tokens; lengths[b] counts
+ * its tokens with them, so its token i of n stands at position lengths[b] - n
+ * + i, in slot position % page_size of page page_table[b][position /
+ * page_size].  A request may bring no token; a token at a negative position
+ * is not stored and sees no key.  Rows of no request are neither read nor
+ * written.  max_new and max_length (the host's idea of the largest request)
+ * only pick the kernel.  The arrays are device memory, read when the kernels
+ * run; what in them leads outside the pools or tensors is not followed but
+ * recorded in *status (never cleared here): */
+enum {
+  ET_B200_PAGED_BAD_PAGE = 1,   /* a page outside the pool: reads as zeros,
+                                   writes are dropped */
+  ET_B200_PAGED_BAD_LENGTH = 2, /* a length below 0 or beyond the table's
+                                   columns: clamped */
+  ET_B200_PAGED_BAD_OFFSET = 4, /* offsets that fall or leave the tensors:
+                                   clamped */
+  ET_B200_PAGED_BAD_ROPE = 8    /* a position beyond the RoPE tables: the last
+                                   row is used */
+};
+typedef struct et_b200_paged_batch_v1 {
+  size_t struct_size;
+  int64_t batch, tokens, table_columns;
+  int64_t max_new, max_length;
+  const int64_t *offsets;    /* [batch + 1], ascending from 0 */
+  const int64_t *lengths;    /* [batch] */
+  const int32_t *page_table; /* [batch, table_columns] */
+  int32_t *status;           /* one word, or NULL */
+} et_b200_paged_batch_v1;
+
+/* RoPE tables as et_b200_rope_tables_v1 lays them out: device f32 [rows,
+ * head_dim / 2], indexed by position; both NULL = no rotation. */
+typedef struct et_b200_paged_rope_v1 {
+  const float *cos;
+  const float *sin;
+  int64_t rows;
+} et_b200_paged_rope_v1;
+
+/* Stores the step's keys (rotated) and values into their pages.  k and v:
+ * [tokens, kv_heads, head_dim], heads dense, rows k_stride / v_stride elements
+ * apart.  The rotation is computed in f32 and rounded once to the pools' type.
+ * Two requests that own the same slot race. */
+int32_t et_b200_paged_append_v1(const et_b200_paged_cache_v1 *cache,
+                                const et_b200_paged_batch_v1 *batch,
+                                const et_b200_paged_rope_v1 *rope,
+                                const void *k, int64_t k_stride, const void *v,
+                                int64_t v_stride, void *stream,
+                                et_kernel_error *error);
+
+/* o = softmax(q' k^T / sqrt(head_dim)) v over the keys at positions up to the
+ * query's own (the new tokens' keys are in the cache already), q' = q rotated
+ * in f32.  q and o: [tokens, q_heads, head_dim], heads dense, rows q_stride /
+ * o_stride elements apart; q_heads a multiple of kv_heads, query head h reads
+ * key head h / (q_heads / kv_heads).  A query that sees no key gets zeros.
+ * lse (f32 [tokens, q_heads], or NULL) receives ln(sum of exp of the scaled
+ * scores), -inf without keys.  Scores, statistics and sums are f32; q' and the
+ * probabilities are rounded to the pools' type for the tensor cores at f16
+ * and bf16, and carried as TF32 pairs (about 22 bits) at f32.  Keys and
+ * values of positions below a request's length must be finite; slots behind
+ * may hold anything.  The workspace (any contents, overwritten; its size does
+ * not depend on the batch) serves one call at a time: calls that may overlap,
+ * and graphs that may, need one each. */
+size_t et_b200_paged_attention_workspace_bytes_v1(
+    const et_b200_paged_cache_v1 *cache, int64_t q_heads);
+int32_t et_b200_paged_attention_v1(const et_b200_paged_cache_v1 *cache,
+                                   const et_b200_paged_batch_v1 *batch,
+                                   const et_b200_paged_rope_v1 *rope,
+                                   int64_t q_heads, const void *q,
+                                   int64_t q_stride, void *o, int64_t o_stride,
+                                   float *lse, void *workspace,
+                                   size_t workspace_bytes, void *stream,
+                                   et_kernel_error *error);
+
+/* Draws one token per row of logits [rows, vocabulary] (row_stride elements
+ * apart) by inversion: with the weights w = exp((x - max x) / temperature) of
+ * the tokens that the filters keep, ids[r] is the first token, in vocabulary
+ * order, whose running sum of w exceeds uniform[r] times their total, and
+ * logprobs[r] (or NULL) is ln(w / total) of it.  Filters, in this order, each
+ * off where its array is NULL or its row's value says so; equal logits rank
+ * by index, the most likely token is always kept:
+ *   top_k  (<= 0: off)  the top_k most likely tokens;
+ *   top_p  (>= 1: off)  tokens with less than top_p of the mass that top_k
+ *                       left ranked before them;
+ *   min_p  (<= 0: off)  w >= min_p (w of the most likely token is 1).
+ * temperature NULL means 1; a row whose temperature is not above 2^-100 takes
+ * the most likely token, with log-probability 0.  Weights are 2^-40 fixed
+ * point, so results depend on no order of summation.  -inf and NaN logits are
+ * never drawn; a row without others gets id -1 and log-probability -inf;
+ * +inf logits share all weight.  vocabulary <= 2^22.  uniform is meant in
+ * [0, 1); other values act as the nearest end. */
+typedef struct et_b200_sampling_v1 {
+  size_t struct_size;
+  int64_t rows, vocabulary, row_stride;
+  uint32_t dtype; /* ET_B200_DTYPE_* of the logits */
+  uint32_t reserved;
+  const float *temperature; /* [rows] */
+  const int64_t *top_k;     /* [rows] */
+  const float *top_p;       /* [rows] */
+  const float *min_p;       /* [rows] */
+} et_b200_sampling_v1;
+int32_t et_b200_sample_v1(const et_b200_sampling_v1 *shape, const void *logits,
+                          const float *uniform, int64_t *ids, float *logprobs,
+                          void *stream, et_kernel_error *error);
+
 /* ------------------------------------------------------------ synthetic data
  * Seeded inputs shared with the tests: value i of (seed, stream) is a pure
  * function of (seed, stream, i).  Host-only; no device is needed. */

@@ -1,0 +1,547 @@
+"""The serving operators (paged append, paged attention, sampling) against
+float64 forms of the same formulas, alone and run together.
+
+Tolerances.  A rounding to a type is off by at most u = eps / 2 of the value.
+Append: f32 rotation x0 c - x1 s, three roundings of 2^-24 of at most
+|x0| + |x1|, then u |k'|; values are copied.  Attention at f16 / bf16: q' is
+rounded (u), so a score is off by at most delta = (u + DIM 2^-23) scale
+sum |q'||k| + 2^-22 |score| (f32 accumulation, the base-2 exponential); a
+weight by exp(2 delta) - 1 relative, plus u for its own rounding in the
+numerator, so o is off by at most (exp(2 delta) - 1 + u + KEYS 2^-23) sum p|v|
++ u |o|.  At f32 the bar of the framework's other f32-grade attention tests:
+2e-5 absolute plus relative.
+"""
+import math
+
+import numpy as np
+import pytest
+import torch
+
+from eshkol_transformer_b200 import paged, sampling
+from serving_f64 import attention, ragged, rope_tables, sample, turn
+
+pytestmark = pytest.mark.gpu
+
+F32, F16, BF16 = torch.float32, torch.float16, torch.bfloat16
+U = {F32: 2.0 ** -24, F16: 2.0 ** -11, BF16: 2.0 ** -8}
+
+
+class Step:
+    """A cache and one step's tensors.  The pools hold NaN wherever no request
+    keeps a key, and `spare` rows follow the last request's."""
+
+    def __init__(self, requests, q_heads, heads, dim, page, dtype, seed=1, layout="heads",
+                 spare=2, strided=False):
+        g = torch.Generator(device="cuda").manual_seed(seed)
+        rand = lambda *s: torch.randn(*s, device="cuda", generator=g)
+        self.requests, self.dtype, self.page = requests, dtype, page
+        offsets, lengths = ragged(requests)
+        self.offsets = torch.tensor(offsets, device="cuda")
+        self.lengths = torch.tensor(lengths, device="cuda")
+        self.used, self.tokens = offsets[-1], offsets[-1] + spare
+        longest = max(lengths + [1])
+        columns = -(-longest // page)
+        batch = len(requests)
+        pages = batch * columns + 2
+        self.table = torch.randperm(pages, device="cuda", generator=g)[:batch * columns]
+        self.table = self.table.reshape(batch, columns).int()
+        shape = (pages, heads, page, dim) if layout == "heads" else (pages, page, heads, dim)
+        pools = [torch.full(shape, math.nan, device="cuda", dtype=dtype) for _ in range(2)]
+        self.keys, self.values = [p if layout == "heads" else p.transpose(1, 2) for p in pools]
+        # every key and value of the requests, [length, heads, dim] each
+        self.k = [rand(m, heads, dim).to(dtype) for _, m in requests]
+        self.v = [rand(m, heads, dim).to(dtype) for _, m in requests]
+        for b in range(batch):
+            self.store(b, self.k[b], self.v[b])
+        width = q_heads * dim + (3 if strided else 0)
+        self.q = rand(self.tokens, width).to(dtype)[:, width - q_heads * dim:]
+        self.q = self.q.unflatten(1, (q_heads, dim))
+        self.o = torch.full((self.tokens, width), 7.0, device="cuda", dtype=dtype)
+        self.o = self.o[:, width - q_heads * dim:].unflatten(1, (q_heads, dim))
+        self.lse = torch.full((self.tokens, q_heads), 7.0, device="cuda")
+        self.status = torch.zeros(1, dtype=torch.int32, device="cuda")
+        self.cos, self.sin = [t.cuda() for t in rope_tables(longest, dim)]
+        self.cache = paged.PagedCache(self.keys, self.values)
+        self.q_heads = q_heads
+
+    def batch(self, **kw):
+        return paged.PagedBatch(self.offsets, self.lengths, self.table, self.tokens,
+                                max((n for n, _ in self.requests), default=0), None, self.status,
+                                **kw)
+
+    def slots(self, b, first, last):
+        at = torch.arange(first, last, device="cuda")
+        return self.table[b].long()[at // self.page], at % self.page
+
+    def store(self, b, k, v):
+        where, slot = self.slots(b, 0, k.shape[0])
+        self.keys[where, :, slot] = k
+        self.values[where, :, slot] = v
+
+    def attend(self, rope=True, stream=0, attention_object=None):
+        a = attention_object or paged.PagedAttention(self.cache, self.q_heads)
+        a.forward(self.batch(), self.q, self.o, (self.cos, self.sin) if rope else None, self.lse,
+                  stream)
+
+    def check(self, rope=True):
+        torch.cuda.synchronize()
+        assert int(self.status) == 0
+        first = 0
+        for b, (n, m) in enumerate(self.requests):
+            rows = slice(first, first + n)
+            first += n
+            if n == 0:
+                continue
+            at = torch.arange(m - n, m, device="cuda").clamp_min(0)
+            q = self.q[rows].double()
+            if rope and m > 0:
+                q = turn(q, self.cos[at], self.sin[at])
+            o, lse, weighted, spread = attention(q, self.k[b].double(), self.v[b].double(), m - n)
+            got, u, dim = self.o[rows].double(), U[self.dtype], q.shape[-1]
+            if self.dtype == F32:
+                bound = 2e-5 + 2e-5 * o.abs()
+                lse_bound = 2e-5 + 2e-5 * lse.abs()
+            else:
+                delta = (u + dim * 2.0 ** -23) * spread + 2.0 ** -22 * spread
+                wide = (2 * delta).expm1() + u + (m + 16) * 2.0 ** -23
+                bound = wide[..., None] * weighted + u * o.abs() + 1e-30
+                lse_bound = delta + 2e-5 * (1 + lse.abs())
+            empty = torch.isinf(lse)
+            assert torch.equal(torch.isinf(self.lse[rows]), empty)
+            assert (got[empty] == 0).all()
+            assert ((got - o).abs() <= bound).all(), (b, float(((got - o).abs() - bound).max()))
+            assert ((self.lse[rows].double() - lse).abs() <= lse_bound)[~empty].all()
+        # rows of no request stay as they were
+        assert (self.o[self.used:] == 7.0).all() and (self.lse[self.used:] == 7.0).all()
+
+
+DECODE = [(1, 1), (1, 17), (0, 40), (1, 64), (1, 65), (1, 300)]
+CHUNKS = [(5, 5), (0, 0), (1, 200), (33, 97), (7, 3), (70, 130), (3, 64)]
+
+
+@pytest.mark.parametrize("dtype", [F32, F16, BF16])
+@pytest.mark.parametrize("q_heads,heads,dim,page", [(4, 4, 64, 16), (8, 2, 128, 16), (3, 1, 32, 1),
+                                                    (2, 2, 80, 24), (5, 1, 256, 8), (8, 1, 8, 128),
+                                                    (6, 2, 40, 7), (32, 2, 64, 64)])
+@pytest.mark.parametrize("requests", [DECODE, CHUNKS], ids=["decode", "chunks"])
+def test_attention_vs_float64(lib, cuda, requests, q_heads, heads, dim, page, dtype):
+    s = Step(requests, q_heads, heads, dim, page, dtype, seed=dim + page)
+    s.attend()
+    s.check()
+
+
+@pytest.mark.parametrize("dtype", [F32, F16, BF16])
+@pytest.mark.parametrize("requests,q_heads,heads,dim", [
+    ([(1, 20011)], 8, 1, 64),                          # one tile over all thread blocks
+    ([(1, 5000), (1, 3), (1, 9001)], 4, 2, 128),
+    ([(300, 1500)], 4, 1, 64),                         # tiles that straddle the shares
+    ([(1 + b % 3, 1 + 7 * b % 130) for b in range(300)], 2, 2, 64),  # more requests than threads
+    ([(257, 600), (1, 2000), (129, 129), (16, 16)], 8, 2, 128),
+    ([(200, 1000)], 3, 1, 64),                         # a group that straddles tiles
+], ids=["long", "ragged", "chunk", "many", "mixed", "odd group"])
+def test_attention_divided_work(lib, cuda, requests, q_heads, heads, dim, dtype):
+    s = Step(requests, q_heads, heads, dim, 32, dtype, seed=len(requests))
+    s.attend()
+    s.check()
+
+
+@pytest.mark.parametrize("dtype", [F32, F16])
+@pytest.mark.parametrize("requests", [DECODE, CHUNKS], ids=["decode", "chunks"])
+def test_attention_strides_and_no_rotation(lib, cuda, requests, dtype):
+    s = Step(requests, 4, 2, 64, 16, dtype, layout="slots", strided=True)
+    s.attend(rope=False)
+    s.check(rope=False)
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
+def test_attention_large_scores(lib, cuda, dtype):
+    """Scores in the hundreds: the running maximum carries the softmax."""
+    s = Step([(1, 500), (40, 300)], 2, 1, 64, 16, dtype, seed=3)
+    s.q *= 40.0
+    s.attend()
+    torch.cuda.synchronize()
+    assert torch.isfinite(s.o[:s.used].float()).all() and torch.isfinite(s.lse[:s.used]).all()
+    if dtype != F32:  # at f32 the scores' own rounding exceeds the fixed bar
+        s.check()
+
+
+def test_attention_kernels_agree_whatever_the_hint(lib, cuda):
+    """max_new only picks the kernel."""
+    s = Step([(3, 200), (1, 70)], 4, 2, 64, 16, F16)
+    a = paged.PagedAttention(s.cache, 4)
+    for hint in (0, 1, 4, 1000):
+        s.o.fill_(7.0)
+        s.lse.fill_(7.0)
+        b = paged.PagedBatch(s.offsets, s.lengths, s.table, s.tokens, hint, 0, s.status)
+        a.forward(b, s.q, s.o, (s.cos, s.sin), s.lse)
+        s.check()
+
+
+@pytest.mark.parametrize("dtype", [F32, F16, BF16])
+@pytest.mark.parametrize("heads,dim,page,layout,shift", [
+    (1, 8, 1, "heads", 0), (2, 64, 16, "heads", 0), (8, 128, 24, "slots", 0),
+    (3, 80, 7, "heads", 1), (16, 64, 128, "slots", 3), (4, 256, 16, "heads", 2)])
+def test_append_vs_float64(lib, cuda, dtype, heads, dim, page, layout, shift):
+    requests = [(1, 1), (0, 9), (4, 40), (1, 17), (6, 4), (33, 33)]
+    s = Step(requests, heads, heads, dim, page, dtype, layout=layout)
+    # k and v as parts of a wider row, off their vector alignment by `shift` elements
+    wide = torch.randn(s.tokens, 2 * heads * dim + 2 * shift, device="cuda").to(dtype)
+    k = wide[:, shift:shift + heads * dim].unflatten(1, (heads, dim))
+    v = wide[:, shift + heads * dim:2 * heads * dim + shift].unflatten(1, (heads, dim))
+    keys, values = s.keys.clone(), s.values.clone()
+    s.cache.append(s.batch(), k, v, rope=(s.cos, s.sin))
+    torch.cuda.synchronize()
+    assert int(s.status) == 0
+    same = torch.ones(s.keys.shape[0], page, dtype=torch.bool, device="cuda")
+    first = 0
+    for b, (n, m) in enumerate(requests):
+        skip = max(0, n - m)  # tokens before position 0 are not stored
+        rows = slice(first + skip, first + n)
+        first += n
+        where, slot = s.slots(b, m - n + skip, m)
+        want = turn(k[rows], s.cos[m - n + skip:m], s.sin[m - n + skip:m])
+        x = k[rows].double().abs().unflatten(2, (dim // 2, 2)).sum(3, keepdim=True)
+        bound = 3 * 2.0 ** -24 * x.expand(-1, -1, -1, 2).flatten(2) + U[dtype] * want.abs()
+        # below the type's normal range roundings are absolute
+        bound += torch.finfo(dtype).smallest_normal * torch.finfo(dtype).eps
+        assert ((s.keys[where, :, slot].double() - want).abs() <= 1.01 * bound).all()
+        assert torch.equal(s.values[where, :, slot], v[rows])
+        same[where, slot] = False
+    for now, before in ((s.keys, keys), (s.values, values)):
+        now, before = now.transpose(1, 2)[same], before.transpose(1, 2)[same]
+        assert torch.equal(now.isnan(), before.isnan())
+        assert torch.equal(now.nan_to_num(), before.nan_to_num())
+
+
+def test_append_without_rotation_copies(lib, cuda):
+    s = Step([(2, 30), (1, 5)], 2, 2, 64, 16, BF16)
+    k, v = torch.randn(2, s.tokens, 2, 64, device="cuda").bfloat16()
+    s.cache.append(s.batch(), k, v)
+    for b, rows, (n, m) in ((0, slice(0, 2), (2, 30)), (1, slice(2, 3), (1, 5))):
+        where, slot = s.slots(b, m - n, m)
+        assert torch.equal(s.keys[where, :, slot], k[rows])
+        assert torch.equal(s.values[where, :, slot], v[rows])
+
+
+def test_bad_metadata_is_recorded_and_not_followed(lib, cuda):
+    """Pages outside the pool read as zeros and drop writes; lengths, offsets
+    and positions beyond the tables are clamped."""
+    s = Step([(1, 40), (2, 40), (1, 20)], 2, 1, 64, 16, F16)
+    k, v = torch.randn(2, s.tokens, 1, 64, device="cuda").half()
+    bits = {"page": paged.BAD_PAGE, "length": paged.BAD_LENGTH, "offset": paged.BAD_OFFSET,
+            "rope": paged.BAD_ROPE}
+    for what, bit in bits.items():
+        s.status.zero_()
+        keep = [t.clone() for t in (s.table, s.lengths, s.offsets, s.cos, s.keys, s.values)]
+        rope = (s.cos, s.sin)
+        if what == "page":
+            s.table[0, 2], s.table[1, 2], s.table[2, 1] = -1, s.keys.shape[0], 2 ** 31 - 1
+        elif what == "length":
+            s.lengths[0], s.lengths[1] = -(2 ** 40), 2 ** 40
+        elif what == "offset":
+            s.offsets[1], s.offsets[3] = 2 ** 40, -9
+        else:
+            rope = (s.cos[:3].contiguous(), s.sin[:3].contiguous())
+        s.keys.nan_to_num_()
+        s.values.nan_to_num_()
+        before = s.keys.clone()
+        s.cache.append(s.batch(), k, v, rope=rope)
+        torch.cuda.synchronize()
+        assert int(s.status) & bit, what
+        if what == "page":  # every write of the step went to a bad page
+            assert torch.equal(s.keys, before)
+        for hint in (1, 100):
+            s.status.zero_()
+            b = paged.PagedBatch(s.offsets, s.lengths, s.table, s.tokens, hint, None, s.status)
+            paged.PagedAttention(s.cache, 2).forward(b, s.q, s.o, rope, s.lse)
+            torch.cuda.synchronize()
+            assert int(s.status) & bit, what
+            assert torch.isfinite(s.o.float()).all()
+        for t, old in zip((s.table, s.lengths, s.offsets, s.cos, s.keys, s.values), keep):
+            t.copy_(old)
+
+
+def test_far_pages(lib, cuda):
+    """A pool whose elements pass 2^32: offsets are 64-bit."""
+    pages, heads, page, dim = 2 ** 32 // (2 * 16 * 64) + 64, 2, 16, 64
+    keys = torch.zeros(pages, heads, page, dim, dtype=F16, device="cuda")
+    values = torch.zeros_like(keys)
+    table = torch.tensor([[pages - 1, 0, pages - 2]], dtype=torch.int32, device="cuda")
+    offsets, lengths = torch.tensor([0, 40], device="cuda"), torch.tensor([40], device="cuda")
+    k, v = torch.randn(2, 40, heads, dim, device="cuda").half()
+    cache = paged.PagedCache(keys, values)
+    for hint in (1, 40):
+        batch = paged.PagedBatch(offsets, lengths, table, 40, hint)
+        cache.append(batch, k, v)
+        assert torch.equal(keys[pages - 1], k[:16].transpose(0, 1))
+        assert torch.equal(values[pages - 2, :, :8], v[32:].transpose(0, 1))
+        o = torch.empty(40, 2, dim, dtype=F16, device="cuda")
+        paged.PagedAttention(cache, 2).forward(batch, k, o)
+        want, _, weighted, spread = attention(k.double(), k.double(), v.double(), 0)
+        delta = (U[F16] + 2.0 ** -16) * spread
+        bound = ((2 * delta).expm1() + U[F16] + 2.0 ** -17)[..., None] * weighted
+        assert ((o.double() - want).abs() <= bound + U[F16] * want.abs()).all()
+
+
+def test_streams_graphs_and_workspaces(lib, cuda):
+    """A captured step follows the buffers it was captured over, two graphs
+    with their own workspaces replay side by side, and results do not change
+    from run to run."""
+    steps = [Step([(1, 700), (1, 90), (1, 4000)], 4, 2, 64, 16, BF16, seed=i) for i in range(2)]
+    objects = [paged.PagedAttention(s.cache, 4) for s in steps]
+    graphs, streams = [], [torch.cuda.Stream() for _ in steps]
+    batches = [s.batch() for s in steps]
+    for s, a, b, stream in zip(steps, objects, batches, streams):
+        s.attend(attention_object=a)
+        s.check()
+        s.first = s.o.clone()
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph, stream=stream):
+            a.forward(b, s.q, s.o, (s.cos, s.sin), s.lse, stream=stream.cuda_stream)
+        graphs.append(graph)
+    for s in steps:
+        s.o.fill_(7.0)
+    torch.cuda.synchronize()
+    for _ in range(5):
+        for graph, stream in zip(graphs, streams):
+            with torch.cuda.stream(stream):
+                graph.replay()
+    torch.cuda.synchronize()
+    for s in steps:
+        assert torch.equal(s.o, s.first)
+        s.check()
+    # other requests in the same buffers
+    s = steps[0]
+    s.lengths.copy_(torch.tensor([650, 1, 3999], device="cuda"))
+    s.requests = [(1, 650), (1, 1), (1, 3999)]
+    for b, (_, m) in enumerate(s.requests):
+        s.k[b], s.v[b] = s.k[b][:m], s.v[b][:m]
+    torch.cuda.synchronize()
+    graphs[0].replay()
+    s.check()
+
+
+def test_python_refusals(lib, cuda):
+    s = Step([(1, 20)], 2, 1, 64, 16, F16, spare=0)
+    good = s.q
+    a = paged.PagedAttention(s.cache, 2)
+    for bad in (good.float(), good[:, :1], good.transpose(0, 1), good.cpu(),
+                torch.zeros(1, 2, 128, dtype=F16, device="cuda")[..., ::2]):
+        with pytest.raises(ValueError):
+            a.forward(s.batch(), bad, s.o)
+    with pytest.raises(ValueError):
+        a.forward(s.batch(), good, s.o, rope=(s.cos, s.sin[:3]))
+    with pytest.raises(ValueError):
+        a.forward(s.batch(), good, s.o, lse=torch.zeros(1, 1, device="cuda"))
+    with pytest.raises(ValueError):
+        paged.PagedAttention(s.cache, 0)
+    with pytest.raises(ValueError):
+        paged.PagedCache(s.keys, s.values[:1])
+    with pytest.raises(ValueError):
+        paged.PagedCache(s.keys.int(), s.values.int())
+    with pytest.raises(ValueError):
+        paged.PagedBatch(s.offsets.int(), s.lengths, s.table, 1)
+    with pytest.raises(ValueError):
+        paged.PagedBatch(s.offsets, s.lengths, s.table.long(), 1)
+    with pytest.raises(ValueError):
+        paged.PagedBatch(s.offsets[:1], s.lengths, s.table, 1)
+    sampler = sampling.Sampler(2, 10)
+    x, u, ids = torch.zeros(2, 10, device="cuda"), torch.zeros(2, device="cuda"), \
+        torch.zeros(2, dtype=torch.int64, device="cuda")
+    for args in ((x[:1], u, ids), (x.double(), u, ids), (x, u.double(), ids), (x, u, ids.int()),
+                 (x, u[:1], ids), (x.t().contiguous().t(), u, ids)):
+        with pytest.raises(ValueError):
+            sampler.sample(*args)
+    with pytest.raises(ValueError):
+        sampler.sample(x, u, ids, top_k=torch.zeros(2, device="cuda"))
+
+
+# ---- sampling ------------------------------------------------------------------------------
+
+def draw(x, u, temperature=None, top_k=None, top_p=None, min_p=None):
+    rows = x.shape[0]
+    dev = lambda a, t: None if a is None else torch.as_tensor(np.broadcast_to(a, rows).copy(),
+                                                              dtype=t, device="cuda")
+    ids = torch.full((rows,), -7, dtype=torch.int64, device="cuda")
+    logprobs = torch.full((rows,), 7.0, device="cuda")
+    args = dict(temperature=dev(temperature, F32), top_k=dev(top_k, torch.int64),
+                top_p=dev(top_p, F32), min_p=dev(min_p, F32))
+    sampling.Sampler(rows, x.shape[1]).sample(x, dev(u, F32), ids, logprobs, **args)
+    return ids.cpu().numpy(), logprobs.cpu().numpy()
+
+
+def check_draw(x, u, temperature=None, top_k=None, top_p=None, min_p=None, margin=2.5e-7, least=0.5):
+    """Drawn ids equal the float64 form's wherever the draw is not within
+    `margin` of a border: a weight is off by at most 1e-7 relative, so a
+    running sum and its total each by 1e-7 of the total.  (Of 50,000 kept tokens
+    one draw in 40 is that close to a border.)  A log-probability is then off
+    by 2e-7 plus its own rounding."""
+    ids, logprobs = draw(x, u, temperature, top_k, top_p, min_p)
+    xs, rows = x.double().cpu().numpy(), x.shape[0]
+    at = lambda a, r, off: off if a is None else float(np.float32(np.broadcast_to(a, rows)[r]))
+    checked = 0
+    for r in range(rows):
+        i, lp, room = sample(xs[r], at(u, r, 0.0), at(temperature, r, 1.0), int(at(top_k, r, 0)),
+                             at(top_p, r, 1.0), at(min_p, r, 0.0))
+        if room <= margin:
+            continue
+        checked += 1
+        assert ids[r] == i, (r, ids[r], i)
+        if np.isfinite(lp):
+            assert abs(logprobs[r] - lp) <= 1e-6 + 2.0 ** -23 * abs(lp), (r, logprobs[r], lp)
+        else:
+            assert logprobs[r] == lp
+    assert checked >= least * rows  # the margins leave most rows
+
+
+def logits_of(rows, vocab, dtype, seed, sigma=2.0):
+    g = torch.Generator(device="cuda").manual_seed(seed)
+    x = torch.randn(rows, vocab, device="cuda", generator=g) * sigma
+    if vocab > 50:
+        x[:, vocab - vocab // 50:] = -math.inf
+        x[:, :24] += 9.0 - 0.3 * torch.arange(24, device="cuda")
+        x = x[:, torch.randperm(vocab, device="cuda", generator=g)].contiguous()
+    return x.to(dtype)
+
+
+@pytest.mark.parametrize("dtype", [F32, F16, BF16])
+@pytest.mark.parametrize("vocab", [1, 2, 33, 1000, 4099, 32768, 50257])
+@pytest.mark.parametrize("kw", [dict(), dict(top_k=40), dict(top_p=0.9), dict(min_p=0.05),
+                                dict(top_k=50, top_p=0.8, min_p=0.02), dict(top_k=3000),
+                                dict(top_k=1), dict(top_p=0.0), dict(min_p=1.0),
+                                dict(top_p=0.99999, top_k=2000)], ids=str)
+def test_sampling_vs_float64(lib, cuda, vocab, dtype, kw):
+    rows = 12
+    u = np.random.default_rng(vocab).random(rows).astype(np.float32)
+    t = np.linspace(0.3, 1.7, rows).astype(np.float32)
+    t[5] = 0.0
+    check_draw(logits_of(rows, vocab, dtype, vocab), u, t, **kw)
+
+
+@pytest.mark.parametrize("vocab", [5, 1024, 30011])
+def test_sampling_ties_go_by_index(lib, cuda, vocab):
+    """Equal logits: the draw is floor(u n) and cuts keep the lowest indexes."""
+    u = (np.arange(64) / 64).astype(np.float32)
+    x = torch.zeros(64, vocab, device="cuda")
+    assert np.array_equal(draw(x, u)[0], np.floor(u.astype(np.float64) * vocab))
+    assert np.array_equal(draw(x, u, top_k=4)[0], np.floor(u * 4))
+    # a quarter of the mass: the first ceil(n / 4)
+    assert np.array_equal(draw(x, u, top_p=0.25)[0],
+                          np.floor(u.astype(np.float64) * math.ceil(vocab / 4)))
+    x = torch.randint(0, 3, (64, vocab), device="cuda").to(BF16)
+    for kw in (dict(top_k=3), dict(top_p=0.5), dict(top_k=4, top_p=0.6), dict(top_k=vocab // 2)):
+        check_draw(x, (u + 1 / 256).astype(np.float32), **kw, margin=1e-7)
+
+
+def test_sampling_special_values(lib, cuda):
+    inf, nan = math.inf, math.nan
+    rows = torch.tensor([
+        [-inf, -inf, -inf, -inf],   # nothing to draw
+        [nan, nan, -inf, nan],
+        [nan, -inf, 3.0, nan],      # one token
+        [1.0, inf, -inf, inf],      # +inf shares all weight
+        [-3e38, 3e38, 0.0, nan],
+        [0.0, -0.0, -inf, nan],     # -0 equals +0
+        [-65504.0, -65504.0, -65504.0, -65504.0],
+    ], device="cuda")
+    lo, hi = np.zeros(7, np.float32), np.full(7, 0.999, np.float32)
+    for kw in (dict(), dict(top_k=2), dict(top_p=0.999), dict(min_p=0.5)):
+        ids, lp = draw(rows, lo, **kw)
+        assert ids.tolist() == [-1, -1, 2, 1, 1, 0, 0], kw
+        assert lp[0] == lp[1] == -inf and lp[2] == lp[4] == 0.0
+        assert np.allclose(lp[[3, 5]], math.log(0.5), atol=1e-6)
+        ids, _ = draw(rows, hi, **kw)
+        assert ids.tolist() == [-1, -1, 2, 3, 1, 1, 1 if kw.get("top_k") else 3], kw
+    assert draw(rows, hi, temperature=0.0)[0].tolist() == [-1, -1, 2, 1, 1, 0, 0]
+    # uniform numbers outside [0, 1) act as the nearest end
+    x = torch.zeros(4, 6, device="cuda")
+    assert draw(x, np.array([-1.0, 1.0, 5.0, nan], np.float32))[0].tolist() == [0, 5, 5, 0]
+    assert draw(x, 0.5, temperature=nan)[0].tolist() == [0] * 4
+
+
+def test_sampling_strides_and_large_vocabulary(lib, cuda):
+    x = logits_of(3, 200001, BF16, 5)
+    wide = torch.zeros(3, 200100, dtype=BF16, device="cuda")
+    wide[:, 3:200004] = x
+    u = np.array([0.1, 0.5, 0.9], np.float32)
+    for kw in (dict(), dict(top_p=0.9), dict(top_k=64, top_p=0.9)):
+        a, b = draw(x, u, **kw), draw(wide[:, 3:200004], u, **kw)
+        assert np.array_equal(a[0], b[0]) and np.array_equal(a[1], b[1])
+        # borders lie some 1e-6 apart here, so the margins may leave no row
+        check_draw(x, u, **kw, least=0.0)
+
+
+# ---- together ------------------------------------------------------------------------------
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
+def test_decoding_loop(lib, cuda, dtype):
+    """Prompts, then single tokens: append, attend, project, sample, the next
+    token's keys from the drawn ids, all on the device and (the single-token
+    step) from a captured graph, against the same loop in float64."""
+    torch.manual_seed(5)
+    vocab, heads, q_heads, dim, page = 500, 2, 4, 64, 16
+    prompts = [37, 1, 64]
+    emb = torch.randn(vocab, q_heads + 2 * heads, dim, device="cuda")
+    head = torch.randn(q_heads * dim, vocab, device="cuda") * 0.2
+    steps = 4
+    columns = -(-(max(prompts) + steps) // page)
+    pools = torch.zeros(2, 3 * columns, heads, page, dim, dtype=dtype, device="cuda")
+    cache = paged.PagedCache(pools[0], pools[1])
+    table = torch.randperm(3 * columns, device="cuda").reshape(3, columns).int()
+    rope = tuple(t.cuda() for t in rope_tables(max(prompts) + steps, dim))
+    attend, sampler = paged.PagedAttention(cache, q_heads), sampling.Sampler(3, vocab)
+    tokens = [torch.randint(vocab, (n,), device="cuda") for n in prompts]
+    uniforms = torch.rand(steps, 3, device="cuda")
+    lengths = torch.tensor(prompts, device="cuda")
+    ids = torch.empty(3, dtype=torch.int64, device="cuda")
+    logits = torch.empty(3, vocab, device="cuda")
+    u = torch.empty(3, device="cuda")
+
+    def step(batch, flat, last, stream):
+        x = emb[flat].to(dtype)
+        cache.append(batch, x[:, q_heads:q_heads + heads], x[:, q_heads + heads:], rope, stream)
+        o = torch.empty(flat.shape[0], q_heads, dim, dtype=dtype, device="cuda")
+        attend.forward(batch, x[:, :q_heads], o, rope, stream=stream)
+        torch.matmul(o[last].flatten(1).float(), head, out=logits)
+        sampler.sample(logits, u, ids, top_k=torch.full((3,), 40, device="cuda"), stream=stream)
+
+    flat = torch.cat(tokens)
+    offsets = torch.tensor([0] + list(np.cumsum(prompts)), device="cuda")
+    u.copy_(uniforms[0])
+    step(paged.PagedBatch(offsets, lengths, table, flat.shape[0], 64, 80), flat, offsets[1:] - 1, 0)
+    drawn, seen = [ids.clone()], [logits.clone()]
+    one = paged.PagedBatch(torch.arange(4, device="cuda"), lengths, table, 3, 1, 80)
+    last = torch.arange(3, device="cuda")
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.stream(side):
+        torch.matmul(torch.zeros(3, q_heads * dim, device="cuda"), head)  # library set-up
+    torch.cuda.synchronize()
+    with torch.cuda.graph(graph, stream=side):
+        lengths += 1
+        step(one, ids, last, side.cuda_stream)
+    for t in range(1, steps):
+        u.copy_(uniforms[t])
+        graph.replay()
+        torch.cuda.synchronize()
+        drawn.append(ids.clone())
+        seen.append(logits.clone())
+    # the same in float64, on the drawn tokens
+    for b in range(3):
+        text = torch.cat([tokens[b]] + [d[b:b + 1] for d in drawn[:-1]])
+        x = emb[text].to(dtype)
+        n = text.shape[0]
+        q, k = (turn(p, rope[0][:n], rope[1][:n]) for p in (x[:, :q_heads],
+                                                           x[:, q_heads:q_heads + heads]))
+        o, _, weighted, spread = attention(q, k.to(dtype).double(), x[:, q_heads + heads:].double(), 0)
+        unit = U[dtype]
+        delta = (2 * unit + dim * 2.0 ** -22) * spread  # k' rounded in the cache may round apart
+        bound = ((2 * delta).expm1() + unit + 2.0 ** -14)[..., None] * weighted + unit * o.abs()
+        for t in range(steps):
+            at = prompts[b] - 1 + t
+            want = o[at].flatten() @ head.double()
+            room = bound[at].flatten() @ head.double().abs() + 1e-4
+            assert ((seen[t][b].double() - want).abs() <= room).all()
+            i, _, margin = sample(seen[t][b].cpu().numpy(), float(uniforms[t, b]), 1.0, 40)
+            assert margin <= 2.5e-7 or i == int(drawn[t][b])
