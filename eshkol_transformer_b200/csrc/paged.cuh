@@ -290,6 +290,10 @@ int32_t check_rope(const et_b200_paged_rope_v1* r, et_kernel_error* e, const cha
 Pools pools_of(const et_b200_paged_cache_v1* c);
 Batch batch_of(const et_b200_paged_batch_v1* b, const et_b200_paged_cache_v1* c);
 Rope rope_of(const et_b200_paged_rope_v1* r);
+// The tcgen05 kernel (paged_attention_tc.cu): launches it and returns its
+// thread blocks, 0 where it does not take the cache (nothing is launched).
+size_t attend_tc_workspace(int dim_padded);
+int attend_tc(const et_b200_paged_cache_v1* c, AttendArgs& a, void* ws, cudaStream_t stream);
 
 }  // namespace paged
 }  // namespace etb

@@ -528,17 +528,10 @@ int resident_blocks(int threads, int smem) {
   return n;
 }
 
-template <typename T, typename S>
-bool launch_shape(AttendArgs& a, void* ws, cudaStream_t stream) {
-  const int resident = resident_blocks<paged_attention_kernel<T, S>>(S::NT, S::SMEM);
-  const int blocks = resident * sm_count();
-  a.tiling.rows = S::BM;
-  a.tiling.keys = S::BK;
-  a.least = 4;
-  a.joint = joint_of(ws, blocks, S::BM, S::DH);
-  paged_attention_kernel<T, S><<<blocks, S::NT, S::SMEM, stream>>>(a);
+template <typename T>
+void launch_join(const AttendArgs& a, int blocks, int dim_padded, cudaStream_t stream) {
   cudaLaunchConfig_t cfg{};
-  cfg.gridDim = dim3(blocks, S::BM < 16 ? S::BM : 16);
+  cfg.gridDim = dim3(blocks, 16);
   cfg.blockDim = dim3(128);
   cfg.stream = stream;
   cudaLaunchAttribute attr{};
@@ -546,9 +539,20 @@ bool launch_shape(AttendArgs& a, void* ws, cudaStream_t stream) {
   attr.val.programmaticStreamSerializationAllowed = 1;
   cfg.attrs = &attr;
   cfg.numAttrs = 1;
-  cudaLaunchKernelEx(&cfg, paged_join_kernel<T>, a, (int)S::DH);
-  count_launch(2);
-  return true;
+  cudaLaunchKernelEx(&cfg, paged_join_kernel<T>, a, dim_padded);
+  count_launch();
+}
+
+template <typename T, typename S>
+void launch_shape(AttendArgs& a, void* ws, cudaStream_t stream) {
+  const int blocks = resident_blocks<paged_attention_kernel<T, S>>(S::NT, S::SMEM) * sm_count();
+  a.tiling.rows = S::BM;
+  a.tiling.keys = S::BK;
+  a.least = 4;
+  a.joint = joint_of(ws, blocks, S::BM, S::DH);
+  paged_attention_kernel<T, S><<<blocks, S::NT, S::SMEM, stream>>>(a);
+  count_launch();
+  launch_join<T>(a, blocks, S::DH, stream);
 }
 
 template <typename T, int DH>
@@ -566,7 +570,14 @@ void launch_dim(AttendArgs& a, int64_t max_new, void* ws, cudaStream_t stream) {
 }
 
 template <typename T>
-void launch_type(AttendArgs& a, int64_t max_new, void* ws, cudaStream_t stream) {
+void launch_type(const et_b200_paged_cache_v1* c, AttendArgs& a, int64_t max_new, void* ws,
+                 cudaStream_t stream) {
+  if constexpr (sizeof(T) == 2) {
+    if (max_new * a.tiling.group > 16) {
+      if (const int blocks = attend_tc(c, a, ws, stream))
+        return launch_join<T>(a, blocks, c->head_dim <= 64 ? 64 : 128, stream);
+    }
+  }
   switch (padded(a.pools.head_dim)) {
     case 32: return launch_dim<T, 32>(a, max_new, ws, stream);
     case 64: return launch_dim<T, 64>(a, max_new, ws, stream);
@@ -588,7 +599,9 @@ size_t et_b200_paged_attention_workspace_bytes_v1(const et_b200_paged_cache_v1* 
   if (check_cache(c, nullptr, "paged-attention-workspace") || q_heads < 1 ||
       q_heads % c->kv_heads != 0)
     return 0;
-  return joint_bytes(kMostPerSm * sm_count(), 64, padded(c->head_dim));
+  const size_t plain = joint_bytes(kMostPerSm * sm_count(), 64, padded(c->head_dim));
+  const size_t tc = attend_tc_workspace(padded(c->head_dim));
+  return plain > tc ? plain : tc;
 }
 
 int32_t et_b200_paged_attention_v1(const et_b200_paged_cache_v1* c,
@@ -637,9 +650,9 @@ int32_t et_b200_paged_attention_v1(const et_b200_paged_cache_v1* c,
     a.q_heads = (int)q_heads;
     a.scale_log2 = kLog2e / sqrtf((float)c->head_dim);
     auto st = static_cast<cudaStream_t>(stream);
-    if (c->dtype == ET_B200_DTYPE_F32) launch_type<float>(a, b->max_new, workspace, st);
-    else if (c->dtype == ET_B200_DTYPE_F16) launch_type<__half>(a, b->max_new, workspace, st);
-    else launch_type<__nv_bfloat16>(a, b->max_new, workspace, st);
+    if (c->dtype == ET_B200_DTYPE_F32) launch_type<float>(c, a, b->max_new, workspace, st);
+    else if (c->dtype == ET_B200_DTYPE_F16) launch_type<__half>(c, a, b->max_new, workspace, st);
+    else launch_type<__nv_bfloat16>(c, a, b->max_new, workspace, st);
     const cudaError_t status = cudaGetLastError();
     if (status != cudaSuccess) return cuda_error(e, status, op);
   }

@@ -1,0 +1,488 @@
+// Attention of chunks of new tokens over a paged cache on tcgen05: f16 / bf16,
+// head_dim up to 128, pages of a power of two of at least 8 slots.
+//
+// The mathematics and the division of the work are those of
+// paged_attention.cu.  A tile is 256 rows (row: token x query head of the
+// group) as two halves of 128 TMEM lanes, a block 128 keys.  K and V blocks
+// arrive page by page through 4-D TMA maps of the pools (dim, slot, head,
+// page) into a ring of slots that both halves read, which halves the L2
+// traffic per product.  One thread issues, per block, P V and the next Q K^T
+// of half 0, then those of half 1: while the tensor pipe works on one half,
+// the other half's four warps (one row per thread, no exchange between
+// threads) turn scores into probabilities, written over the scores in TMEM as
+// the A operand of P V.  The row maximum stands until a block exceeds it by
+// 2^8 (the sums stay far inside f32), so O is rescaled in TMEM only then.
+// Waits are bounded; one that runs out raises a CTA-wide abort, copies and
+// products in flight are waited for and TMEM is released.
+#include <math.h>
+
+#include <type_traits>
+
+#include "attention_f16.cuh"
+#include "paged.cuh"
+
+namespace etb {
+namespace {
+
+using namespace paged;
+using namespace f16att;
+
+constexpr int HALF = 128, BK = 128;
+// warps 0-7 probabilities; 8 products, 9 copies (10, 11 fill the warpgroup, whose
+// registers above kLeanRegs go to the other two: 256 x 208 + 128 x 88 = 384 x 168)
+constexpr int MMA_WARP = 8, LOAD_WARP = 9, THREADS = 384;
+constexpr int kWideRegs = 208, kLeanRegs = 88;
+static_assert(256 * kWideRegs + 128 * kLeanRegs <= THREADS * 168, "registers at launch");
+constexpr float kJump = 8.0f;  // log2 of the largest P the standing maximum allows
+
+__device__ int g_wait_error;  // bounded waits that gave up (the status word tells the caller)
+
+__device__ __forceinline__ void tma_load_4d(uint32_t dst, const CUtensorMap* map, uint32_t bar,
+                                            int x, int y, int z, int w) {
+  asm volatile(
+      "cp.async.bulk.tensor.4d.shared::cluster.global.tile.mbarrier::complete_tx::bytes"
+      " [%0], [%1, {%3, %4, %5, %6}], [%2];" ::"r"(dst),
+      "l"(reinterpret_cast<uint64_t>(map)), "r"(bar), "r"(x), "r"(y), "r"(z), "r"(w)
+      : "memory");
+}
+
+template <typename T>
+__device__ __forceinline__ uint32_t pack2(float a, float b) {
+  if constexpr (std::is_same_v<T, __half>) {
+    const __half2 h = __floats2half2_rn(a, b);
+    return *reinterpret_cast<const uint32_t*>(&h);
+  } else {
+    const __nv_bfloat162 h = __floats2bfloat162_rn(a, b);
+    return *reinterpret_cast<const uint32_t*>(&h);
+  }
+}
+
+template <int DH>
+struct Layout {
+  static constexpr int SLOT = BK * DH * 2;           // one block of K or V
+  static constexpr int SLOTS = DH == 128 ? 5 : 8;
+  static constexpr int Q = SLOTS * SLOT;              // two halves of 128 rows
+  static constexpr int BARS = Q + 2 * HALF * DH * 2;
+  static constexpr int SMEM = BARS + 512 + 1024;
+  // TMEM: scores of the halves (P over the first 64 columns), outputs
+  static constexpr uint32_t S0 = 0, O0 = 256, COLS = 512;
+  static_assert(O0 + 2 * DH <= COLS && SMEM <= 232448, "TMEM and shared memory");
+};
+
+template <typename T, int DH>
+__global__ void __launch_bounds__(THREADS, 1)
+paged_attention_tc_kernel(const __grid_constant__ CUtensorMap k_map,
+                          const __grid_constant__ CUtensorMap v_map, AttendArgs a, int box_rows) {
+  using L = Layout<DH>;
+  constexpr int SLOTS = L::SLOTS;
+  constexpr uint32_t kType = std::is_same_v<T, __nv_bfloat16> ? (1u << 7) | (1u << 10) : 0u;
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) &
+                                             ~(uintptr_t)1023);
+  uint64_t* bars = reinterpret_cast<uint64_t*>(smem + L::BARS);
+  enum { FULL = 0, EMPTY = 8, SFULL = 16, PREADY = 18, QREADY = 20, ODONE = 22, DRAIN = 24, NBARS };
+  const uint32_t bar0 = smem_u32(bars);
+  auto B_ = [&](int i) { return bar0 + 8u * (uint32_t)i; };
+  uint32_t* tslot = reinterpret_cast<uint32_t*>(bars + NBARS);
+  volatile int* abort = reinterpret_cast<volatile int*>(tslot + 1);
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  const uint32_t base = smem_u32(smem);
+  const int group = a.tiling.group, dim = a.pools.head_dim;
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+
+  if (tid == 0) {
+    for (int i = 0; i < NBARS; i++)
+      mbar_init(B_(i), (i >= PREADY && i < ODONE) ? HALF : 1);
+    *abort = 0;
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+  }
+  if (warp == MMA_WARP) tmem_alloc(smem_u32(tslot), L::COLS);
+  Place p;
+  const Share share = divide<THREADS>(a.tiling, a.batch, a.least, p);
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = *tslot;
+  // blocks of the tile at p that fall into this share, and whether it has rows
+  // for the second half
+  int64_t left = share.units;
+  auto blocks_here = [&]() { return (int)min((int64_t)(p.nblk - p.blk), left); };
+  auto rows_here = [&]() {
+    return (int)min((int64_t)(2 * HALF), (int64_t)p.r.n * group - (int64_t)p.tile * 2 * HALF);
+  };
+  auto next_tile = [&](int done) {
+    left -= done;
+    p.blk += done - 1;
+    advance(a.tiling, a.batch, p);
+  };
+  auto wait = [&](int i, uint32_t parity) {
+    return role_wait(B_(i), parity & 1u, &g_wait_error, abort);
+  };
+
+  if (warp >= MMA_WARP) {
+  asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kLeanRegs));
+  if (warp == LOAD_WARP) {
+    // ---- K and V blocks, page by page
+    uint32_t count = 0;  // slots filled: K, V, K, V, ...
+    bool ok = true;
+    const int boxes_per_tile = DH / 64;
+    while (ok && left > 0) {
+      const int nb = blocks_here(), visible = tile_visible(a.tiling, p.r, p.tile);
+      for (int j = 0; ok && j < nb; j++) {
+        const int key0 = (p.blk + j) * BK;
+        const int boxes = (min(visible - key0, BK) + box_rows - 1) / box_rows;
+        // each lane looks up the boxes it will load (at most 16 pages of 8 keys)
+        const int mine = lane % 16;
+        int page = -1, slot = 0;
+        if (mine < boxes) {
+          const int key = key0 + mine * box_rows, column = key / a.pools.page_size;
+          slot = key - column * a.pools.page_size;
+          page = a.batch.table[(int64_t)p.b * a.batch.columns + column];
+          if (page < 0 || page >= a.pools.pages) {
+            report(a.batch.status, ET_B200_PAGED_BAD_PAGE);
+            page = -1;  // outside the map: filled with zeros
+          }
+        }
+#pragma unroll
+        for (int kv = 0; kv < 2; kv++) {
+          const uint32_t s = count % SLOTS, round = count / SLOTS;
+          if (round > 0) ok = wait(EMPTY + s, round - 1);
+          ok = __all_sync(0xffffffffu, ok);
+          if (!ok) break;
+          const uint32_t bar = B_(FULL + s), dst = base + s * L::SLOT;
+          if (lane == 0) mbar_expect_tx(bar, (uint32_t)(max(boxes, 0) * box_rows * DH * 2));
+          __syncwarp();
+          if (mine < boxes && lane / 16 < boxes_per_tile)
+            tma_load_4d(dst + (uint32_t)(lane / 16) * BK * 128u + (uint32_t)(mine * box_rows) * 128u,
+                        kv == 0 ? &k_map : &v_map, bar, 64 * (lane / 16), slot, p.h, page);
+          count++;
+        }
+      }
+      next_tile(nb);
+    }
+    // every copy has landed before the CTA releases its memory
+    if (lane == 0)
+      for (uint32_t c = count > SLOTS ? count - SLOTS : 0; c < count; c++)
+        mbar_wait(B_(FULL + c % SLOTS), (c / SLOTS) & 1u, &g_wait_error);
+  } else if (warp == MMA_WARP) {
+    // ---- products
+    constexpr uint32_t idesc_s = idesc_f16_m128(BK, 0) | kType;
+    constexpr uint32_t idesc_o = idesc_f16_m128(DH, 1) | kType;
+    uint32_t count = 0, items[2] = {0, 0}, steps[2] = {0, 0};
+    bool ok = true;
+    auto scores = [&](int t, uint32_t slot) {
+      const uint32_t q = base + L::Q + (uint32_t)t * (HALF * DH * 2), k = base + slot * L::SLOT;
+#pragma unroll
+      for (int i = 0; i < DH / 16; i++)
+        umma_f16(tmem + L::S0 + 128u * t, kdesc16<HALF>(q, i), kdesc16<BK>(k, i), idesc_s,
+                 i > 0 ? 1u : 0u);
+      umma_commit(B_(SFULL + t));
+    };
+    while (ok && left > 0) {
+      const int nb = blocks_here(), halves = rows_here() > HALF ? 2 : 1;
+      const int visible = tile_visible(a.tiling, p.r, p.tile);
+      uint32_t ks = count % SLOTS;
+      ok = wait(FULL + ks, count / SLOTS);
+      for (int t = 0; ok && t < halves; t++) {
+        ok = wait(QREADY + t, items[t]);
+        ok = __all_sync(0xffffffffu, ok);
+        if (!ok) break;
+        tc_fence_after();
+        if (lane == 0) scores(t, ks);
+      }
+      if (ok && lane == 0) umma_commit(B_(EMPTY + ks));
+      count++;
+      for (int j = 0; ok && j < nb; j++) {
+        const uint32_t vs = count % SLOTS, vt = base + vs * L::SLOT;
+        ok = wait(FULL + vs, count / SLOTS);
+        ok = __all_sync(0xffffffffu, ok);
+        if (!ok) break;
+        count++;
+        const int valid = visible - (p.blk + j) * BK;
+        if (valid < BK) {  // slots behind the visible keys may hold anything
+          for (int i = max(valid, 0) * 8 + lane; i < BK * 8; i += 32)
+#pragma unroll
+            for (int c = 0; c < DH / 64; c++)
+              sts128(vt + (uint32_t)c * BK * 128u + (uint32_t)i * 16u, make_float4(0.f, 0.f, 0.f, 0.f));
+          fence_async_smem();
+          __syncwarp();
+        }
+        const bool more = j + 1 < nb;
+        if (more) {
+          ks = count % SLOTS;
+          ok = wait(FULL + ks, count / SLOTS);
+          count++;
+        }
+        for (int t = 0; ok && t < halves; t++) {
+          ok = wait(PREADY + t, steps[t]);
+          ok = __all_sync(0xffffffffu, ok);
+          if (!ok) break;
+          steps[t]++;
+          tc_fence_after();
+          if (lane == 0) {
+#pragma unroll
+            for (int i = 0; i < BK / 16; i++)
+              umma_f16_ts(tmem + L::O0 + (uint32_t)(DH * t), tmem + L::S0 + 128u * t + 8u * i,
+                          mdesc16<BK>(vt, i), idesc_o, (j > 0 || i > 0) ? 1u : 0u);
+            if (more) scores(t, ks);
+            else umma_commit(B_(ODONE + t));
+          }
+        }
+        if (ok && lane == 0) {
+          umma_commit(B_(EMPTY + vs));
+          if (more) umma_commit(B_(EMPTY + ks));
+        }
+      }
+      for (int t = 0; t < halves; t++) items[t]++;
+      next_tile(nb);
+    }
+    if (lane == 0) {
+      umma_commit(B_(DRAIN));
+      mbar_wait(B_(DRAIN), 0u, &g_wait_error);
+    }
+  }
+  } else {
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kWideRegs));
+    // ---- probabilities: half t, one row per thread
+    const int t = warp >> 2, row = tid & (HALF - 1);
+    const uint32_t lanes = tmem + ((uint32_t)((warp & 3) * 32) << 16);
+    const uint32_t s_at = lanes + L::S0 + 128u * t, o_at = lanes + L::O0 + (uint32_t)(DH * t);
+    const uint32_t q_row = base + L::Q + (uint32_t)t * (HALF * DH * 2) + (uint32_t)row * 128u;
+    const float scale = a.scale_log2;
+    const bool q_vec = ((reinterpret_cast<uintptr_t>(a.q) | (uintptr_t)(a.q_stride * 2)) & 15) == 0;
+    const bool o_vec = ((reinterpret_cast<uintptr_t>(a.o) | (uintptr_t)(a.o_stride * 2)) & 15) == 0;
+    uint32_t items = 0, steps = 0;
+    bool ok = true;
+    Cut cut{0, 0, 0, 0, 0};
+    while (ok && left > 0) {
+      const int nb = blocks_here(), rows = rows_here() - HALF * t;
+      const bool whole = p.blk == 0, ends = p.blk + nb == p.nblk;
+      if (whole && !ends) {
+        const int64_t rest = p.nblk - nb;
+        cut = Cut{p.r.first, p.r.n, p.h, p.tile, 1 + (int)((rest + share.per - 1) / share.per)};
+      }
+      if (rows > 0) {
+        const int64_t g = (int64_t)p.tile * 2 * HALF + HALF * t + row;
+        const bool valid = row < rows;
+        const int token = (int)(g / group), head = p.h * group + (int)(g % group);
+        const int pos = p.r.len - p.r.n + token;
+        const int vis = valid ? max(0, pos + 1) : 0;
+        // keys that every row of this warp sees (invalid rows follow the last valid one)
+        const int vis_warp = __shfl_sync(0xffffffffu, max(0, pos + 1), 0);
+        // ---- this row of Q, rotated, into the swizzled tile
+        {
+          const T* src = static_cast<const T*>(a.q) + (p.r.first + token) * a.q_stride + (int64_t)head * dim;
+          const float *ct = nullptr, *st = nullptr;
+          if (a.rope.cos != nullptr && valid && pos >= 0) {
+            const int64_t at = rope_row(a.rope, pos, a.batch.status) * (dim / 2);
+            ct = a.rope.cos + at;
+            st = a.rope.sin + at;
+          }
+#pragma unroll 4
+          for (int d = 0; d < DH; d += 8) {
+            union { uint4 v; T x[8]; } u;
+            u.v = make_uint4(0, 0, 0, 0);
+            if (valid && d < dim) {
+              if (q_vec) u.v = *reinterpret_cast<const uint4*>(src + d);
+              else
+#pragma unroll
+                for (int i = 0; i < 8; i++) u.x[i] = src[d + i];
+              if (ct != nullptr)
+#pragma unroll
+                for (int i = 0; i < 8; i += 2) {
+                  float x0 = to_f32<T>(u.x[i]), x1 = to_f32<T>(u.x[i + 1]);
+                  rotate(x0, x1, __ldg(ct + (d + i) / 2), __ldg(st + (d + i) / 2));
+                  u.x[i] = from_f32<T>(x0);
+                  u.x[i + 1] = from_f32<T>(x1);
+                }
+            }
+            const uint32_t piece = (uint32_t)(d >> 3) & 7u;
+            const float4 f = *reinterpret_cast<const float4*>(&u.v);
+            sts128(q_row + (uint32_t)(d >> 6) * HALF * 128u + ((piece ^ (uint32_t)(row & 7)) << 4), f);
+          }
+          fence_async_smem();
+          tc_fence_before();
+          mbar_arrive(B_(QREADY + t));
+        }
+        float m = -INFINITY, l = 0.0f;
+        for (int j = 0; ok && j < nb; j++) {
+          ok = __all_sync(0xffffffffu, wait(SFULL + t, steps));
+          if (!ok) break;
+          steps++;
+          tc_fence_after();
+          uint32_t r[4][32];
+#pragma unroll
+          for (int c = 0; c < 4; c++) tmem_ld32_nowait(s_at + 32 * c, r[c]);
+          tmem_wait_ld_pin<true>(r[0]);
+          tmem_wait_ld_pin<false>(r[1]);
+          tmem_wait_ld_pin<false>(r[2]);
+          tmem_wait_ld_pin<false>(r[3]);
+          const int key0 = (p.blk + j) * BK;
+          if (key0 + BK > vis_warp) {
+            const int seen = vis - key0;
+#pragma unroll
+            for (int c = 0; c < 4; c++)
+#pragma unroll
+              for (int i = 0; i < 32; i++)
+                if (32 * c + i >= seen) r[c][i] = 0xff800000u;  // -inf
+          }
+          float top[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+#pragma unroll
+          for (int c = 0; c < 4; c++)
+#pragma unroll
+            for (int i = 0; i < 32; i++) top[i & 3] = fmaxf(top[i & 3], __uint_as_float(r[c][i]));
+          const float bmax = fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3])) * scale;
+          const bool jump = bmax > m + kJump || (m == -INFINITY && bmax > -INFINITY);
+          if (__any_sync(0xffffffffu, jump)) {
+            const float factor = jump ? ex2(m - bmax) : 1.0f;  // 0 while m is -inf
+            if (jump) {
+              m = bmax;
+              l *= factor;
+            }
+            if (j > 0) {
+              // the scores' barrier also says that the last P V is complete
+#pragma unroll
+              for (int c = 0; c < DH / 32; c++) {
+                float o[32];
+                tmem_ld32(o_at + 32 * c, o);
+#pragma unroll
+                for (int i = 0; i < 32; i++) o[i] *= factor;
+                tmem_st32(o_at + 32 * c, o);
+              }
+            }
+          }
+          const float from = m == -INFINITY ? 0.0f : m;
+          float sum[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+          for (int c = 0; c < 4; c++) {
+            float w[16];
+#pragma unroll
+            for (int i = 0; i < 16; i++) {
+              const float x = ex2(fmaf(__uint_as_float(r[c][2 * i]), scale, -from));
+              const float y = ex2(fmaf(__uint_as_float(r[c][2 * i + 1]), scale, -from));
+              sum[(2 * i) & 3] += x;
+              sum[(2 * i + 1) & 3] += y;
+              w[i] = __uint_as_float(pack2<T>(x, y));
+            }
+            tmem_st16(s_at + 16 * c, w);
+          }
+          l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
+          tmem_wait_st();
+          tc_fence_before();
+          mbar_arrive(B_(PREADY + t));
+        }
+        if (ok) ok = __all_sync(0xffffffffu, wait(ODONE + t, items));
+        items++;
+        if (ok) {
+          tc_fence_after();
+          const bool done = whole && ends;
+          const float inv = l > 0.0f ? 1.0f / l : 0.0f;
+          T* dst = static_cast<T*>(a.o) + (p.r.first + token) * a.o_stride + (int64_t)head * dim;
+          const int slot = 2 * (int)blockIdx.x + (whole ? 1 : 0), r = HALF * t + row;
+          float* part = a.joint.sums + ((int64_t)slot * 2 * HALF + r) * DH;
+#pragma unroll
+          for (int c = 0; c < DH / 32; c++) {
+            float o[32];
+            tmem_ld32(o_at + 32 * c, o);
+            if (!valid) continue;
+            if (done) {
+#pragma unroll
+              for (int i = 0; i < 32; i += 8) {
+                const int d = 32 * c + i;
+                if (d >= dim) break;
+                union { uint4 v; uint32_t w[4]; T x[8]; } u;
+#pragma unroll
+                for (int k = 0; k < 4; k++) u.w[k] = pack2<T>(o[i + 2 * k] * inv, o[i + 2 * k + 1] * inv);
+                if (o_vec) *reinterpret_cast<uint4*>(dst + d) = u.v;
+                else
+#pragma unroll
+                  for (int k = 0; k < 8; k++) dst[d + k] = u.x[k];
+              }
+            } else {
+#pragma unroll
+              for (int i = 0; i < 32; i += 4)
+                *reinterpret_cast<float4*>(part + 32 * c + i) = make_float4(o[i], o[i + 1], o[i + 2], o[i + 3]);
+            }
+          }
+          if (valid) {
+            if (!done) {
+              a.joint.stats[(int64_t)slot * 4 * HALF + r] = m;
+              a.joint.stats[((int64_t)slot * 2 + 1) * 2 * HALF + r] = l;
+            } else if (a.lse != nullptr) {
+              a.lse[(p.r.first + token) * a.q_heads + head] = l > 0.0f ? m * kLn2 + logf(l) : -INFINITY;
+            }
+          }
+          tc_fence_before();  // O is read before the next tile's QREADY
+        }
+      }
+      next_tile(nb);
+    }
+    if (tid == 0) {
+      if (!ok) report(a.batch.status, ET_B200_PAGED_TIMEOUT);
+      a.joint.cuts[blockIdx.x] = cut;
+    }
+  }
+  tc_fence_before();
+  __syncthreads();
+  if (warp == MMA_WARP) {
+    tc_fence_after();
+    tmem_dealloc(tmem, L::COLS);
+  }
+}
+
+// Map of a pool: boxes of 64 dims x box_rows slots of one head of one page.
+bool pool_map(CUtensorMap* map, void* pool, const et_b200_paged_cache_v1* c, int box_rows) {
+  const cuuint64_t dims[4] = {(cuuint64_t)c->head_dim, (cuuint64_t)c->page_size,
+                              (cuuint64_t)c->kv_heads, (cuuint64_t)c->pages};
+  const cuuint64_t strides[3] = {(cuuint64_t)c->token_stride * 2, (cuuint64_t)c->head_stride * 2,
+                                 (cuuint64_t)c->page_stride * 2};
+  const cuuint32_t box[4] = {64, (cuuint32_t)box_rows, 1, 1}, one[4] = {1, 1, 1, 1};
+  return encode_fn()(map, c->dtype == ET_B200_DTYPE_F16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16
+                                                         : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16,
+                     4, pool, dims, strides, box, one, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                     CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                     CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
+template <typename T, int DH>
+int launch_tc(const et_b200_paged_cache_v1* c, AttendArgs& a, void* ws, cudaStream_t stream) {
+  using L = Layout<DH>;
+  const int box_rows = (int)(c->page_size < BK ? c->page_size : BK);
+  CUtensorMap k_map, v_map;
+  if (!pool_map(&k_map, c->keys, c, box_rows) || !pool_map(&v_map, c->values, c, box_rows)) return 0;
+  const int blocks = sm_count();
+  a.tiling.rows = 2 * HALF;
+  a.tiling.keys = BK;
+  a.least = 2;
+  a.joint = joint_of(ws, blocks, 2 * HALF, DH);
+  cudaFuncSetAttribute(paged_attention_tc_kernel<T, DH>,
+                       cudaFuncAttributeMaxDynamicSharedMemorySize, L::SMEM);
+  paged_attention_tc_kernel<T, DH><<<blocks, THREADS, L::SMEM, stream>>>(k_map, v_map, a, box_rows);
+  count_launch();
+  return blocks;
+}
+
+}  // namespace
+
+namespace paged {
+
+size_t attend_tc_workspace(int dim_padded) {
+  return dim_padded > 128 ? 0 : joint_bytes(sm_count(), 2 * HALF, dim_padded < 64 ? 64 : dim_padded);
+}
+
+int attend_tc(const et_b200_paged_cache_v1* c, AttendArgs& a, void* ws, cudaStream_t stream) {
+  const int64_t ps = c->page_size;
+  if (c->dtype == ET_B200_DTYPE_F32 || c->head_dim > 128 || ps < 8 || (ps & (ps - 1)) != 0 ||
+      encode_fn() == nullptr)
+    return 0;
+  // strides that a tensor map cannot hold
+  if (c->page_stride * 2 >= (int64_t)1 << 40 || c->head_stride * 2 >= (int64_t)1 << 40) return 0;
+  if (c->dtype == ET_B200_DTYPE_F16)
+    return c->head_dim <= 64 ? launch_tc<__half, 64>(c, a, ws, stream)
+                             : launch_tc<__half, 128>(c, a, ws, stream);
+  return c->head_dim <= 64 ? launch_tc<__nv_bfloat16, 64>(c, a, ws, stream)
+                           : launch_tc<__nv_bfloat16, 128>(c, a, ws, stream);
+}
+
+}  // namespace paged
+}  // namespace etb

@@ -26,6 +26,7 @@ BAD_PAGE = 1    # a page outside the pool: reads as zeros, writes are dropped
 BAD_LENGTH = 2  # a length below 0 or beyond the table's columns: clamped
 BAD_OFFSET = 4  # offsets that fall or leave the tensors: clamped
 BAD_ROPE = 8    # a position beyond the RoPE tables: the last row is used
+TIMEOUT = 16    # a kernel gave up waiting: o is not valid
 
 
 class CacheDescriptor(C.Structure):

@@ -195,8 +195,10 @@ enum {
                                    columns: clamped */
   ET_B200_PAGED_BAD_OFFSET = 4, /* offsets that fall or leave the tensors:
                                    clamped */
-  ET_B200_PAGED_BAD_ROPE = 8    /* a position beyond the RoPE tables: the last
+  ET_B200_PAGED_BAD_ROPE = 8,   /* a position beyond the RoPE tables: the last
                                    row is used */
+  ET_B200_PAGED_TIMEOUT = 16    /* a kernel gave up waiting for its own copies
+                                   or products: o is not valid */
 };
 typedef struct et_b200_paged_batch_v1 {
   size_t struct_size;
