@@ -3,11 +3,25 @@
 // Weights w(x) = exp((x - M) / temperature), M the row's maximum, as 2^-40
 // fixed point: integer sums are the same in every order, so cumulative sums,
 // cuts and draws are deterministic whatever the thread layout.  A cut (top-k,
-// top-p) is a pair (key, index): the tokens above a logit, and of those equal
-// to it the ones up to an index; it is found by radix selection on the
-// monotone integer image of the logits, counting tokens or adding their
-// weights per digit.  The draw inverts the running sum in vocabulary order.
+// top-p) is a pair (logit, index): the tokens above a logit, and of those
+// equal to it the ones up to an index.  The draw inverts the running sum in
+// vocabulary order.
+//
+// A row is read from memory once, into the shared memory of a cluster of
+// thread blocks (each a contiguous slice; as many as the slices need, more
+// when there are few rows), while its maximum is formed.  Then
+//  - a small top-k (or a small vocabulary) becomes a list: each slice keeps
+//    what reaches a lower bound of its k-th largest logit (from the maxima of
+//    its threads), one block sorts the gathered list, cuts it by all filters,
+//    sorts what is left by index and draws;
+//  - otherwise a cut is found from a histogram (tokens or weights) over
+//    1,024 steps of the logit, the border's step is gathered and sorted, and
+//    the draw adds the kept weights slice by slice, warp by warp.
+// Rows for which the list or the border's step overflows (thousands of equal
+// logits) or the slices do not fit are selected by radix from memory.
 #include <math.h>
+
+#include <cooperative_groups.h>
 
 #include <type_traits>
 
@@ -17,6 +31,7 @@ namespace etb {
 namespace {
 
 using paged::to_f32;
+namespace cg = cooperative_groups;
 
 constexpr int NT = 512, WARPS = NT / 32;
 constexpr int BINS = 2048;
@@ -30,25 +45,49 @@ __device__ __forceinline__ uint32_t key_of(float x) {
 }
 constexpr uint32_t kKeyMinusInf = 0x007fffffu;  // key_of(-inf)
 
+// log2(e) / temperature = hi + lo.  shift = M (hi + lo) = shift_hi + shift_lo
+// with shift_hi a multiple of 2^-8 below 2^15 (narrow), so that n + shift_hi
+// is exact for the integers n of the exponents.
 struct Scale {
-  float max, hi, lo;  // hi + lo = log2(e) / temperature
+  float max, hi, lo, shift, shift_hi, shift_lo;
+  bool narrow;
 };
+__device__ __forceinline__ Scale scale_of(float max, float temperature) {
+  Scale s;
+  const double per = 1.4426950408889634 / (double)temperature;
+  s.max = max;
+  s.hi = (float)per;
+  s.lo = (float)(per - (double)s.hi);
+  const double shift = (double)max * per;
+  s.narrow = fabs(shift) < 32000.0;
+  const double grid = rint(shift * 256.0) / 256.0;
+  s.shift = (float)shift;
+  s.shift_hi = (float)grid;
+  s.shift_lo = (float)(shift - grid);
+  return s;
+}
 
-// exp((x - max) / temperature) 2^40, rounded.  t = (x - max) (hi + lo) keeps
-// the rounding errors of the difference and the products, 2^t = 2^n 2^f with
-// 2^f - 1 by its series (|f| <= 1/2, terms up to f^7: 5e-9), so the relative
-// error stays near 3e-8 whatever the size of the logits.
+// exp((x - max) / temperature) 2^40, rounded: 2^t with t = (x - max) (hi +
+// lo) = n + f, f accurate to about 2^-25 because its one large difference is
+// formed by an fma whose other operand is exact; 2^f - 1 by its series (|f|
+// <= 1/2, terms up to f^7: 5e-9).  The relative error is near 3e-8 whatever
+// the size of the logits.
 __device__ __forceinline__ uint64_t weight_of(float x, const Scale& s) {
-  if (!(x > -INFINITY)) return 0;
-  if (s.max == INFINITY) return x == INFINITY ? 1ull << FRACTION : 0;
-  const float d = x - s.max;
-  const float t = d * s.hi;
-  if (!(t >= -(float)(FRACTION + 1))) return 0;
-  const float bb = d - x;
-  const float e = (x - (d - bb)) - (s.max + bb);
-  const float rest = fmaf(d, s.hi, -t) + fmaf(d, s.lo, e * s.hi);
-  const float n = rintf(t);
-  const float f = (t - n) + rest;
+  float n, f;
+  if (s.narrow) {
+    const float t = fmaf(x, s.hi, -s.shift);
+    if (!(t >= -(float)(FRACTION + 1))) return 0;
+    n = rintf(t);
+    f = fmaf(x, s.hi, -(n + s.shift_hi)) + fmaf(x, s.lo, -s.shift_lo);
+  } else {
+    if (!(x > -INFINITY)) return 0;
+    if (s.max == INFINITY) return x == INFINITY ? 1ull << FRACTION : 0;
+    const float d = x - s.max, t = d * s.hi;
+    if (!(t >= -(float)(FRACTION + 1))) return 0;
+    const float bb = d - x, e = (x - (d - bb)) - (s.max + bb);
+    n = rintf(t);
+    f = (t - n) + (fmaf(d, s.hi, -t) + fmaf(d, s.lo, e * s.hi));
+  }
   float y = 1.5252734e-5f;
   y = fmaf(y, f, 1.5403530e-4f);
   y = fmaf(y, f, 1.3333558e-3f);
@@ -57,10 +96,9 @@ __device__ __forceinline__ uint64_t weight_of(float x, const Scale& s) {
   y = fmaf(y, f, 2.4022651e-1f);
   y = fmaf(y, f, 6.9314718e-1f);
   y *= f;
-  const int k = FRACTION + (int)n;  // -1 .. 40
-  const float p = __uint_as_float((uint32_t)(127 + k) << 23);
-  const int64_t whole = k >= 0 ? (int64_t)1 << k : 0;
-  return (uint64_t)(k >= 0 ? whole + __float2ll_rn(y * p) : __float2ll_rn(fmaf(y, p, p)));
+  const int right = -(int)n;  // 0 .. 41
+  const uint64_t w = (uint64_t)(0x80000000u + (uint32_t)__float2int_rn(y * 0x1p31f)) << (FRACTION - 31);
+  return (w + ((1ull << right) >> 1)) >> right;
 }
 
 struct Shared {
@@ -227,76 +265,73 @@ __device__ __forceinline__ float value_of(uint32_t key) {
   return __uint_as_float((key & 0x80000000u) ? (key & 0x7fffffffu) : ~key);
 }
 
+struct Filters {
+  float temperature, top_p, min_p;
+  int64_t top_k;
+  double uniform;
+};
+struct Args {
+  const float* uniform;
+  const float* temperature;
+  const int64_t* top_k;
+  const float* top_p;
+  const float* min_p;
+  int64_t* ids;
+  float* logprobs;
+  int64_t row_stride;
+  int n, slice;  // tokens of a row, of a slice
+};
+__device__ __forceinline__ Filters filters_of(const Args& a, int64_t row) {
+  Filters f;
+  f.temperature = a.temperature != nullptr ? a.temperature[row] : 1.0f;
+  f.top_k = a.top_k != nullptr ? a.top_k[row] : 0;
+  f.top_p = a.top_p != nullptr ? a.top_p[row] : 1.0f;
+  f.min_p = a.min_p != nullptr ? a.min_p[row] : 0.0f;
+  f.uniform = (double)a.uniform[row];
+  return f;
+}
+// What the running sum has to reach: the first integer above u total, inside
+// [1, total].
+__device__ __forceinline__ uint64_t draw_aim(double u, uint64_t total) {
+  const double aim = u > 0.0 ? u * (double)total : 0.0;
+  return aim < (double)total ? min((uint64_t)aim + 1, total) : total;
+}
+// What the ranked weights have to reach for a share p of `total`.
+__device__ __forceinline__ uint64_t share_aim(float p, uint64_t total) {
+  const double aim = ceil((double)p * (double)total);
+  return aim > 1.0 ? (uint64_t)aim : 1ull;
+}
+// The least logit that min_p keeps (-inf: no limit).
+__device__ __forceinline__ float least_logit(const Filters& f, float max) {
+  if (!(f.min_p > 0.0f) || max == INFINITY) return -INFINITY;
+  const double least = (double)max + (double)f.temperature * log((double)fminf(f.min_p, 1.0f));
+  const float x = (float)least;
+  return (double)x < least ? nextafterf(x, INFINITY) : x;
+}
+__device__ __forceinline__ void answer(const Args& a, int64_t row, int id, float x,
+                                       const Filters& f, const Scale& sc, uint64_t total) {
+  a.ids[row] = id;
+  if (a.logprobs == nullptr) return;
+  const double d = sc.max == INFINITY ? 0.0 : (double)x - (double)sc.max;
+  a.logprobs[row] = (float)(d / (double)f.temperature -
+                            log((double)total / (double)weight_of(sc.max, sc)));
+}
+
+// One thread block draws for a row in global memory: radix selection.
 template <typename T>
-__global__ void __launch_bounds__(NT)
-sample_kernel(const T* __restrict__ logits, int64_t row_stride, int n,
-              const float* __restrict__ uniform, const float* __restrict__ temperature,
-              const int64_t* __restrict__ top_k, const float* __restrict__ top_p,
-              const float* __restrict__ min_p, int64_t* __restrict__ ids,
-              float* __restrict__ logprobs) {
-  __shared__ Shared sm;
-  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-  const int64_t row = blockIdx.x;
-  const T* x = logits + row * row_stride;
+__device__ void sample_row(const T* x, const Args& a, int64_t row, const Filters& flt,
+                           const Scale& sc, Shared& sm) {
+  const int n = a.n;
   auto key_at = [&](int i) { return key_of(to_f32<T>(x[i])); };
-
-  // the largest logit, of equal ones the first
-  uint64_t best = 0;
-  for (int i = tid; i < n; i += NT) {
-    const uint64_t v = ((uint64_t)key_at(i) << 32) | (0xffffffffu - (uint32_t)i);
-    best = max(best, v);
-  }
-#pragma unroll
-  for (int o = 16; o > 0; o >>= 1) best = max(best, (uint64_t)__shfl_xor_sync(0xffffffffu, best, o));
-  if (lane == 0) sm.warp[warp] = best;
-  __syncthreads();
-#pragma unroll
-  for (int w = 0; w < WARPS; w++) best = max(best, sm.warp[w]);
-  const uint32_t best_key = (uint32_t)(best >> 32);
-  const int64_t best_index = (int64_t)(0xffffffffu - (uint32_t)best);
-  if (best_key <= kKeyMinusInf) {
-    if (tid == 0) {
-      ids[row] = -1;
-      if (logprobs != nullptr) logprobs[row] = -INFINITY;
-    }
-    return;
-  }
-  const float temp = temperature != nullptr ? temperature[row] : 1.0f;
-  if (!(temp > 0x1p-100f)) {
-    if (tid == 0) {
-      ids[row] = best_index;
-      if (logprobs != nullptr) logprobs[row] = 0.0f;
-    }
-    return;
-  }
-  const double per = 1.4426950408889634 / (double)temp;
-  Scale sc;
-  sc.max = value_of(best_key);
-  sc.hi = (float)per;
-  sc.lo = (float)(per - (double)sc.hi);
-
   auto unit = [&](uint32_t key) { return weight_of(value_of(key), sc); };
   Cut cut{kKeyMinusInf, -1};
-  const int64_t k = top_k != nullptr ? top_k[row] : 0;
-  if (k > 0 && k < n)
+  if (flt.top_k > 0 && flt.top_k < n)
     select(n, sm, cut, key_at, [](uint32_t) -> uint64_t { return 1; },
-           [&](uint64_t all) { return (uint64_t)k < all ? (uint64_t)k : 0ull; });
-  const float share = top_p != nullptr ? top_p[row] : 1.0f;
-  if (share < 1.0f)
-    select(n, sm, cut, key_at, unit, [&](uint64_t all) {
-      const double aim = ceil((double)share * (double)all);
-      return aim > 1.0 ? (uint64_t)aim : 1ull;
-    });
-  const float low = min_p != nullptr ? min_p[row] : 0.0f;
-  if (low > 0.0f && sc.max < INFINITY) {
-    const double least = (double)sc.max + (double)temp * log((double)fminf(low, 1.0f));
-    float f = (float)least;
-    if ((double)f < least) f = nextafterf(f, INFINITY);
-    const uint32_t key = key_of(f);
-    if (key > cut.key) cut = Cut{key, INT64_MAX};
-  }
-
-  const double u = (double)uniform[row];
+           [&](uint64_t all) { return (uint64_t)flt.top_k < all ? (uint64_t)flt.top_k : 0ull; });
+  if (flt.top_p < 1.0f)
+    select(n, sm, cut, key_at, unit, [&](uint64_t all) { return share_aim(flt.top_p, all); });
+  const uint32_t least = key_of(least_logit(flt, sc.max));
+  if (least > cut.key) cut = Cut{least, INT64_MAX};
   uint64_t total = 0;
   const int id = in_order(
       n, sm,
@@ -306,16 +341,588 @@ sample_kernel(const T* __restrict__ logits, int64_t row_stride, int n,
       },
       [&](uint64_t all) {
         total = all;
-        const double aim = u > 0.0 ? u * (double)all : 0.0;
-        return aim < (double)all ? min((uint64_t)aim + 1, all) : all;
+        return draw_aim(flt.uniform, all);
       });
-  if (tid == 0) {
-    ids[row] = id;
-    if (logprobs != nullptr) {
-      const double d = sc.max == INFINITY ? 0.0 : (double)to_f32<T>(x[id]) - (double)sc.max;
-      logprobs[row] = (float)(d / (double)temp - log((double)total * 0x1p-40));
+  if (threadIdx.x == 0) answer(a, row, id, to_f32<T>(x[id]), flt, sc, total);
+}
+
+// ---- rows in the shared memory of a cluster ------------------------------------------------
+
+constexpr int LIST = 1024;       // entries of a list, steps of a histogram
+constexpr float kSteps = 24.0f;  // histogram steps per factor of 2 of a weight: 1,024 reach 2^-42
+
+__device__ __forceinline__ void cp16(uint32_t dst, const void* src) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
+}
+
+// A slice of n logits in shared memory, stored at their global address modulo
+// 16, so that whole 16-byte pieces copy and read as such.
+template <typename T>
+struct Slice {
+  static constexpr int N = 16 / sizeof(T);
+  const T* x;               // in shared memory
+  int n, head, pieces;      // tokens before the first whole piece, whole pieces
+  // f(i, value) for every token, in no particular order
+  template <typename F>
+  __device__ __forceinline__ void each(F f) const {
+    for (int p = threadIdx.x; p < pieces; p += NT) {
+      union { uint4 v; T x[N]; } u;
+      u.v = *reinterpret_cast<const uint4*>(x + head + p * N);
+#pragma unroll
+      for (int k = 0; k < N; k++) f(head + p * N + k, to_f32<T>(u.x[k]));
+    }
+    const int t = threadIdx.x, tail = head + pieces * N;
+    if (t < head) f(t, to_f32<T>(x[t]));
+    else if (t >= 32 && tail + t - 32 < n) f(tail + t - 32, to_f32<T>(x[tail + t - 32]));
+  }
+};
+
+// Sorts a[0 .. n), n a power of two, descending.
+__device__ void sort_descending(uint64_t* a, int n) {
+  for (int size = 2; size <= n; size <<= 1)
+    for (int step = size >> 1; step > 0; step >>= 1) {
+      __syncthreads();
+      for (int i = threadIdx.x; i < n / 2; i += NT) {
+        const int lo = 2 * i - (i & (step - 1)), hi = lo + step;
+        const uint64_t u = a[lo], v = a[hi];
+        if ((u < v) == ((lo & size) == 0)) {
+          a[lo] = v;
+          a[hi] = u;
+        }
+      }
+    }
+  __syncthreads();
+}
+// Pads a list of n entries with zeros to a power of two; that power.
+__device__ int pad_list(uint64_t* a, int n) {
+  int size = 32;
+  while (size < n) size <<= 1;
+  for (int i = n + threadIdx.x; i < size; i += NT) a[i] = 0;
+  return size;
+}
+__device__ __forceinline__ uint64_t entry_of(float x, int index) {
+  return ((uint64_t)key_of(x) << 32) | (0xffffffffu - (uint32_t)index);
+}
+__device__ __forceinline__ float entry_value(uint64_t e) { return value_of((uint32_t)(e >> 32)); }
+__device__ __forceinline__ int entry_index(uint64_t e) { return (int)(0xffffffffu - (uint32_t)e); }
+
+struct Border {
+  float value;  // tokens above it are kept,
+  int index;    // and those equal to it up to this index
+};
+__device__ __forceinline__ bool kept(const Border& b, float x, int i) {
+  return x > b.value || (x == b.value && i <= b.index);
+}
+
+struct Room {
+  union {
+    struct { uint64_t list[LIST], all[LIST]; };  // a block's list, the cluster's
+    struct { uint32_t low[LIST], high[LIST]; };  // a histogram
+    Shared radix;
+  };
+  uint64_t warp[WARPS];
+  uint64_t found[4];
+  float top;
+  int count, keep, step, before;
+  Border border;
+  uint64_t total;
+};
+
+// Inclusive sum over the block; *all: the block's.
+__device__ __forceinline__ uint64_t room_scan(uint64_t v, Room& rm, uint64_t* all) {
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  v = warp_scan(v);
+  __syncthreads();
+  if (lane == 31) rm.warp[warp] = v;
+  __syncthreads();
+  uint64_t before = 0, sum = 0;
+#pragma unroll
+  for (int w = 0; w < WARPS; w++) {
+    if (w < warp) before += rm.warp[w];
+    sum += rm.warp[w];
+  }
+  *all = sum;
+  return v + before;
+}
+
+// A value that at least k of the threads' maxima (`mine`, `top` the largest)
+// reach, so a lower bound of the k-th largest logit of the slice, and not many
+// more than 2 k: histograms of 256 steps over the maxima, each into the
+// border's step of the one before.  -inf where fewer than k are finite.
+__device__ float top_bound(float mine, float top, int k, Room& rm) {
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  uint32_t* bins = rm.low;
+  const bool some = mine > -INFINITY;
+  float low = some ? mine : INFINITY, bound = -INFINITY, high = top;
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) low = fminf(low, __shfl_xor_sync(0xffffffffu, low, o));
+  __syncthreads();
+  if (lane == 0) rm.warp[warp] = (uint64_t)__float_as_uint(low);
+  if (__syncthreads_count(some) < k) return -INFINITY;
+#pragma unroll
+  for (int w = 0; w < WARPS; w++) low = fminf(low, __uint_as_float((uint32_t)rm.warp[w]));
+  bound = low;  // all of them reach it
+  int above = 0;  // maxima over `high`
+  for (int round = 0; round < 4; round++) {
+    const float width = (high - low) * (1.0f / 256.0f), inv = 1.0f / width;
+    if (!(width > 0.0f) || !(width < INFINITY) || !(inv < INFINITY)) break;
+    if (tid < 256) bins[tid] = 0;
+    __syncthreads();
+    if (some && mine >= low && mine <= high) atomicAdd(&bins[min(255, (int)((high - mine) * inv))], 1u);
+    __syncthreads();
+    if (warp == 0) {
+      uint32_t c[8], sum = 0;
+#pragma unroll
+      for (int j = 0; j < 8; j++) sum += c[j] = bins[lane * 8 + j];
+      uint32_t run = (uint32_t)warp_scan(sum) - sum, before = 0;
+      int step = 255;
+#pragma unroll
+      for (int j = 0; j < 8; j++) {
+        if (step == 255 && above + (int)(run + c[j]) >= k) {
+          step = lane * 8 + j;
+          before = run;
+        }
+        run += c[j];
+      }
+      const int first = __reduce_min_sync(0xffffffffu, step);
+      if (step == first) rm.step = first, rm.before = (int)before;
+    }
+    __syncthreads();
+    const int step = rm.step, before = rm.before;
+    const float edge = high - ((float)step + 1.01f) * width;
+    const int reach = __syncthreads_count(some && mine >= edge);
+    if (reach < k) break;  // the steps are finer than the values' rounding
+    bound = fmaxf(bound, edge);
+    if (reach <= 2 * k + 32) break;
+    above += before;
+    high -= (float)step * width;
+    low = edge;
+  }
+  __syncthreads();
+  return bound;
+}
+
+// Gathers the blocks' lists (rm.list, rm.count) into rm.all of rank 0; the
+// number of entries, or -1 if they do not fit (every block gets the same).
+__device__ int gather_lists(cg::cluster_group& cluster, Room& rm, unsigned rank, unsigned blocks) {
+  cluster.sync();
+  int total = 0;
+  bool fits = true;
+  for (unsigned b = 0; b < blocks; b++) {
+    const int c = cluster.map_shared_rank(&rm, b)->count;
+    fits = fits && c <= LIST;
+    if (rank == 0 && fits && total + c <= LIST) {
+      const uint64_t* from = cluster.map_shared_rank(&rm, b)->list;
+      for (int i = threadIdx.x; i < c; i += NT) rm.all[total + i] = from[i];
+    }
+    total += c;
+    fits = fits && total <= LIST;
+  }
+  __syncthreads();
+  return fits ? total : -1;
+}
+
+// Rank 0: cuts the gathered list of n entries by all filters and draws.
+__device__ void draw_from_list(int n, const Args& a, int64_t row, const Filters& flt,
+                               const Scale& sc, Room& rm) {
+  constexpr int PER = LIST / NT;
+  const int tid = threadIdx.x;
+  const int size = pad_list(rm.all, n);
+  sort_descending(rm.all, size);
+  if (flt.top_k > 0 && flt.top_k < n) n = (int)flt.top_k;
+  uint64_t w[PER], mine = 0, all;
+#pragma unroll
+  for (int j = 0; j < PER; j++) {
+    const int i = tid * PER + j;
+    w[j] = i < n ? weight_of(entry_value(rm.all[i]), sc) : 0;
+    mine += w[j];
+  }
+  uint64_t run = room_scan(mine, rm, &all) - mine;
+  const uint64_t aim = flt.top_p < 1.0f ? share_aim(flt.top_p, all) : all;
+  const float least = least_logit(flt, sc.max);
+  if (tid == 0) rm.keep = 0;
+  __syncthreads();
+  int keep = 0;
+#pragma unroll
+  for (int j = 0; j < PER; j++) {
+    const int i = tid * PER + j;
+    if (i < n && (run < aim || i == 0) && entry_value(rm.all[i]) >= least) keep++;
+    run += w[j];
+  }
+  keep = __reduce_add_sync(0xffffffffu, keep);
+  if ((tid & 31) == 0 && keep) atomicAdd(&rm.keep, keep);
+  __syncthreads();
+  n = rm.keep;  // what is kept is a prefix of the ranking
+  __syncthreads();
+  // by index, ascending: entries (~index, logit bits), descending
+  for (int i = tid; i < n; i += NT) {
+    const uint64_t e = rm.all[i];
+    rm.all[i] = (e << 32) | (e >> 32);
+  }
+  sort_descending(rm.all, pad_list(rm.all, n));
+  mine = 0;
+#pragma unroll
+  for (int j = 0; j < PER; j++) {
+    const int i = tid * PER + j;
+    w[j] = i < n ? weight_of(value_of((uint32_t)rm.all[i]), sc) : 0;
+    mine += w[j];
+  }
+  run = room_scan(mine, rm, &all) - mine;
+  const uint64_t to = draw_aim(flt.uniform, all);
+#pragma unroll
+  for (int j = 0; j < PER; j++) {
+    if (run < to && to <= run + w[j]) {
+      const uint64_t e = rm.all[tid * PER + j];
+      answer(a, row, (int)(0xffffffffu - (uint32_t)(e >> 32)), value_of((uint32_t)e), flt, sc, all);
+    }
+    run += w[j];
+  }
+}
+
+// Lowers `border` to the shortest prefix of the ranking of the tokens it keeps
+// whose units reach aim(total) (0: unchanged); `per` histogram steps per unit
+// of the logit.  False (in every block of the
+// cluster) when the border's step holds more tokens than a list.
+template <typename T, typename Unit, typename Aim>
+__device__ bool cluster_cut(cg::cluster_group& cluster, Room& rm, unsigned rank, unsigned blocks,
+                            const Slice<T>& slice, int first, float max, float per, Border& border,
+                            Unit unit, Aim aim) {
+  constexpr int PER = LIST / NT;
+  const int tid = threadIdx.x;
+  // steps of 1 / per of the logit, falling; the last takes all below
+  auto step_of = [&](float x) {
+    const float t = (max - x) * per;
+    return t > 0.0f ? (int)fminf(t, (float)(LIST - 1)) : 0;
+  };
+  cluster.sync();  // nobody reads this block's room any more
+  for (int i = tid; i < LIST; i += NT) rm.low[i] = rm.high[i] = 0;
+  __syncthreads();
+  slice.each([&](int i, float x) {
+    if (!kept(border, x, first + i)) return;
+    const uint64_t w = unit(x);
+    if (w == 0) return;
+    const int step = step_of(x);
+    const uint32_t lo = (uint32_t)w, old = atomicAdd(&rm.low[step], lo);
+    const uint32_t hi = (uint32_t)(w >> 32) + (old + lo < old ? 1u : 0u);
+    if (hi != 0) atomicAdd(&rm.high[step], hi);
+  });
+  cluster.sync();
+  uint64_t bins[PER], mine = 0, all;
+#pragma unroll
+  for (int j = 0; j < PER; j++) {
+    const int i = tid * PER + j;
+    bins[j] = 0;
+    for (unsigned b = 0; b < blocks; b++) {
+      const Room* r = cluster.map_shared_rank(&rm, b);
+      bins[j] += ((uint64_t)r->high[i] << 32) | r->low[i];
+    }
+    mine += bins[j];
+  }
+  uint64_t run = room_scan(mine, rm, &all) - mine;
+  const uint64_t to = aim(all);
+  if (to == 0 || to > all) return true;
+#pragma unroll
+  for (int j = 0; j < PER; j++) {
+    if (run < to && to <= run + bins[j]) {
+      rm.found[0] = (uint64_t)(tid * PER + j);
+      rm.found[1] = to - run;
+    }
+    run += bins[j];
+  }
+  if (tid == 0) rm.count = 0;
+  cluster.sync();  // every block is done with the histograms: lists take their place
+  const int step = (int)rm.found[0];
+  const uint64_t rest = rm.found[1];
+  slice.each([&](int i, float x) {
+    if (!kept(border, x, first + i) || step_of(x) != step || unit(x) == 0) return;
+    const int at = atomicAdd(&rm.count, 1);
+    if (at < LIST) rm.list[at] = entry_of(x, first + i);
+  });
+  const int n = gather_lists(cluster, rm, rank, blocks);
+  if (n < 0) return false;
+  if (rank == 0) {
+    sort_descending(rm.all, pad_list(rm.all, n));
+    mine = 0;
+    uint64_t w[PER];
+#pragma unroll
+    for (int j = 0; j < PER; j++) {
+      const int i = tid * PER + j;
+      w[j] = i < n ? unit(entry_value(rm.all[i])) : 0;
+      mine += w[j];
+    }
+    run = room_scan(mine, rm, &all) - mine;
+#pragma unroll
+    for (int j = 0; j < PER; j++) {
+      if (run < rest && rest <= run + w[j]) {
+        const uint64_t e = rm.all[tid * PER + j];
+        rm.border = Border{entry_value(e), entry_index(e)};
+      }
+      run += w[j];
     }
   }
+  cluster.sync();
+  border = cluster.map_shared_rank(&rm, 0)->border;
+  return true;
+}
+
+template <typename T>
+__global__ void __launch_bounds__(NT, 2) sample_cluster_kernel(const T* __restrict__ logits, Args a) {
+  extern __shared__ __align__(16) uint8_t slice_smem[];
+  __shared__ Room rm;
+  cg::cluster_group cluster = cg::this_cluster();
+  const unsigned rank = cluster.block_rank(), blocks = cluster.num_blocks();
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  const int64_t row = blockIdx.x / blocks;
+  const T* x = logits + row * a.row_stride;
+  const Filters flt = filters_of(a, row);
+
+  // this block's slice, and its maximum while it arrives
+  const int first = min(a.n, (int)rank * a.slice);
+  Slice<T> slice;
+  slice.n = min(a.n, first + a.slice) - first;
+  const uintptr_t at = reinterpret_cast<uintptr_t>(x + first);
+  const int off = (int)(at & 15);
+  slice.head = min(slice.n, off == 0 ? 0 : (16 - off) / (int)sizeof(T));
+  slice.pieces = (slice.n - slice.head) / Slice<T>::N;
+  T* mine = reinterpret_cast<T*>(slice_smem + off);
+  slice.x = mine;
+  const uint32_t dst = (uint32_t)__cvta_generic_to_shared(mine + slice.head);
+  const T* src = x + first + slice.head;
+  constexpr int PARTS = 4;
+  const int part = (slice.pieces + PARTS - 1) / PARTS;
+#pragma unroll
+  for (int g = 0; g < PARTS; g++) {
+    const int end = min(slice.pieces, (g + 1) * part);
+    for (int p = g * part + tid; p < end; p += NT) cp16(dst + 16u * p, src + p * Slice<T>::N);
+    asm volatile("cp.async.commit_group;" ::: "memory");
+  }
+  float top = -INFINITY;
+  {
+    const int tail = slice.head + slice.pieces * Slice<T>::N;
+    if (tid < slice.head) {
+      mine[tid] = x[first + tid];
+      top = to_f32<T>(mine[tid]);
+    } else if (tid >= 32 && tail + tid - 32 < slice.n) {
+      mine[tail + tid - 32] = x[first + tail + tid - 32];
+      top = to_f32<T>(mine[tail + tid - 32]);
+    }
+    top = fmaxf(top, -INFINITY);  // NaN is no maximum
+  }
+#pragma unroll
+  for (int g = 0; g < PARTS; g++) {
+    if (g == 0) asm volatile("cp.async.wait_group 3;" ::: "memory");
+    if (g == 1) asm volatile("cp.async.wait_group 2;" ::: "memory");
+    if (g == 2) asm volatile("cp.async.wait_group 1;" ::: "memory");
+    if (g == 3) asm volatile("cp.async.wait_group 0;" ::: "memory");
+    const int end = min(slice.pieces, (g + 1) * part);
+    for (int p = g * part + tid; p < end; p += NT) {  // the pieces this thread copied
+      union { uint4 v; T x[Slice<T>::N]; } u;
+      u.v = *reinterpret_cast<const uint4*>(mine + slice.head + p * Slice<T>::N);
+#pragma unroll
+      for (int k = 0; k < Slice<T>::N; k++) top = fmaxf(top, to_f32<T>(u.x[k]));
+    }
+  }
+  const float thread_top = top;
+  top = warp_max(top);
+  if (lane == 0) rm.warp[warp] = (uint64_t)__float_as_uint(top);
+  if (tid == 0) rm.count = 0;
+  __syncthreads();
+  float block_top = -INFINITY;
+#pragma unroll
+  for (int w = 0; w < WARPS; w++) block_top = fmaxf(block_top, __uint_as_float((uint32_t)rm.warp[w]));
+  if (tid == 0) rm.top = block_top;
+  cluster.sync();
+  float max = -INFINITY;
+  for (unsigned b = 0; b < blocks; b++) max = fmaxf(max, cluster.map_shared_rank(&rm, b)->top);
+
+  // every path ends with a cluster.sync: no block leaves while another reads
+  // its shared memory
+  if (max == -INFINITY) {
+    if (rank == 0 && tid == 0) {
+      a.ids[row] = -1;
+      if (a.logprobs != nullptr) a.logprobs[row] = -INFINITY;
+    }
+    cluster.sync();
+    return;
+  }
+  if (!(flt.temperature > 0x1p-100f)) {  // the first of the largest
+    int best = INT32_MAX;
+    if (block_top == max)
+      slice.each([&](int i, float v) { if (v == max) best = min(best, first + i); });
+    best = __reduce_min_sync(0xffffffffu, best);
+    __syncthreads();
+    if (lane == 0) rm.warp[warp] = (uint64_t)best;
+    cluster.sync();
+    if (rank == 0 && warp == 0) {
+      for (unsigned i = lane; i < blocks * WARPS; i += 32)
+        best = min(best, (int)cluster.map_shared_rank(&rm, i / WARPS)->warp[i % WARPS]);
+      best = __reduce_min_sync(0xffffffffu, best);
+      if (lane == 0) {
+        a.ids[row] = best;
+        if (a.logprobs != nullptr) a.logprobs[row] = 0.0f;
+      }
+    }
+    cluster.sync();
+    return;
+  }
+  const Scale sc = scale_of(max, flt.temperature);
+  const bool top_k = flt.top_k > 0 && flt.top_k < a.n;
+
+  // ---- a list
+  bool listed = a.n <= LIST;
+  float bound = -INFINITY;
+  if (!listed && top_k && flt.top_k <= NT / 2) {
+    bound = top_bound(thread_top, block_top, (int)flt.top_k, rm);
+    listed = true;
+  }
+  if (listed) {
+    slice.each([&](int i, float v) {
+      if (v > -INFINITY && v >= bound) {
+        const int p = atomicAdd(&rm.count, 1);
+        if (p < LIST) rm.list[p] = entry_of(v, first + i);
+      }
+    });
+    const int n = gather_lists(cluster, rm, rank, blocks);
+    if (n >= 0) {
+      if (rank == 0) draw_from_list(n, a, row, flt, sc, rm);
+      cluster.sync();
+      return;
+    }
+  }
+
+  // ---- cuts from histograms
+  Border border{-INFINITY, -1};
+  bool good = true;
+  if (top_k)
+    good = cluster_cut<T>(cluster, rm, rank, blocks, slice, first, max, kSteps * 1.4427f, border,
+                          [](float) -> uint64_t { return 1; },
+                          [&](uint64_t all) { return (uint64_t)flt.top_k < all ? (uint64_t)flt.top_k : 0ull; });
+  if (good && flt.top_p < 1.0f)
+    good = cluster_cut<T>(cluster, rm, rank, blocks, slice, first, max, kSteps * sc.hi, border,
+                          [&](float v) { return weight_of(v, sc); },
+                          [&](uint64_t all) { return share_aim(flt.top_p, all); });
+  if (!good) {
+    cluster.sync();
+    if (rank == 0) sample_row<T>(x, a, row, flt, sc, rm.radix);
+    cluster.sync();
+    return;
+  }
+  const float least = least_logit(flt, sc.max);
+  if (least > border.value) border = Border{least, INT32_MAX};
+
+  // ---- the draw: running sums by block, warp, lane
+  auto weight_at = [&](int i) -> uint64_t {
+    const float v = to_f32<T>(slice.x[i]);
+    return kept(border, v, first + i) ? weight_of(v, sc) : 0;
+  };
+  const int span = (slice.n + WARPS - 1) / WARPS;
+  const int w0 = min(slice.n, warp * span), w1 = min(slice.n, w0 + span);
+  uint64_t sum = 0;
+  for (int i = w0 + lane; i < w1; i += 32) sum += weight_at(i);
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+  __syncthreads();
+  if (lane == 0) rm.warp[warp] = sum;
+  __syncthreads();
+  uint64_t here = 0;
+#pragma unroll
+  for (int w = 0; w < WARPS; w++) here += rm.warp[w];
+  if (tid == 0) rm.total = here;
+  cluster.sync();
+  uint64_t all = 0, before = 0;
+  for (unsigned b = 0; b < blocks; b++) {
+    const uint64_t t = cluster.map_shared_rank(&rm, b)->total;
+    if (b < rank) before += t;
+    all += t;
+  }
+  const uint64_t to = draw_aim(flt.uniform, all);
+  if (before < to && to <= before + here) {
+    uint64_t rest = to - before;
+    int w = 0;
+    while (w < WARPS - 1 && rest > rm.warp[w]) rest -= rm.warp[w++];
+    __syncthreads();
+    const int s0 = min(slice.n, w * span), s1 = min(slice.n, s0 + span);
+    const int each = (span + NT - 1) / NT;
+    const int t0 = min(s1, s0 + tid * each), t1 = min(s1, t0 + each);
+    uint64_t mine_sum = 0, unused;
+    for (int i = t0; i < t1; i++) mine_sum += weight_at(i);
+    uint64_t run = room_scan(mine_sum, rm, &unused) - mine_sum;
+    if (run < rest && rest <= run + mine_sum) {
+      int i = t0;
+      for (; i < t1; i++) {
+        run += weight_at(i);
+        if (run >= rest) break;
+      }
+      answer(a, row, first + i, to_f32<T>(slice.x[i]), flt, sc, all);
+    }
+  }
+  cluster.sync();
+}
+
+// Vocabularies beyond the shared memory of a cluster.
+template <typename T>
+__global__ void __launch_bounds__(NT) sample_kernel(const T* __restrict__ logits, Args a) {
+  __shared__ Shared sm;
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, n = a.n;
+  const int64_t row = blockIdx.x;
+  const T* x = logits + row * a.row_stride;
+  const Filters flt = filters_of(a, row);
+  // the largest logit, of equal ones the first
+  uint64_t best = 0;
+  for (int i = tid; i < n; i += NT)
+    best = max(best, ((uint64_t)key_of(to_f32<T>(x[i])) << 32) | (0xffffffffu - (uint32_t)i));
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) best = max(best, (uint64_t)__shfl_xor_sync(0xffffffffu, best, o));
+  if (lane == 0) sm.warp[warp] = best;
+  __syncthreads();
+#pragma unroll
+  for (int w = 0; w < WARPS; w++) best = max(best, sm.warp[w]);
+  const uint32_t best_key = (uint32_t)(best >> 32);
+  const bool none = best_key <= kKeyMinusInf;
+  if (none || !(flt.temperature > 0x1p-100f)) {
+    if (tid == 0) {
+      a.ids[row] = none ? -1 : (int64_t)(0xffffffffu - (uint32_t)best);
+      if (a.logprobs != nullptr) a.logprobs[row] = none ? -INFINITY : 0.0f;
+    }
+    return;
+  }
+  sample_row<T>(x, a, row, flt, scale_of(value_of(best_key), flt.temperature), sm);
+}
+
+// Clusters of as few thread blocks as hold a row (two of them per SM), and of
+// up to 8 while that leaves SMs idle and a slice keeps 4,096 logits.
+template <typename T>
+cudaError_t launch(const T* logits, Args a, int64_t rows, cudaStream_t stream) {
+  constexpr int kSliceBytes = 96 * 1024;
+  int blocks = 1;
+  auto slice_of = [&](int b) { return ((a.n + b - 1) / b + 15) / 16 * 16; };
+  while (blocks < 8 && (int64_t)slice_of(blocks) * (int)sizeof(T) > kSliceBytes) blocks *= 2;
+  if ((int64_t)slice_of(blocks) * (int)sizeof(T) > 208 * 1024 || rows * blocks > INT32_MAX) {
+    sample_kernel<T><<<(unsigned)rows, NT, 0, stream>>>(logits, a);
+    count_launch();
+    return cudaGetLastError();
+  }
+  while (blocks < 8 && rows * blocks * 2 <= 2 * sm_count() && slice_of(2 * blocks) >= 4096) blocks *= 2;
+  a.slice = slice_of(blocks);
+  const int smem = a.slice * (int)sizeof(T) + 32;
+  cudaError_t st = cudaFuncSetAttribute(sample_cluster_kernel<T>,
+                                        cudaFuncAttributeMaxDynamicSharedMemorySize, 209 * 1024);
+  if (st != cudaSuccess) return st;
+  cudaLaunchConfig_t cfg{};
+  cfg.gridDim = dim3((unsigned)(rows * blocks));
+  cfg.blockDim = dim3(NT);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = stream;
+  cudaLaunchAttribute attr{};
+  attr.id = cudaLaunchAttributeClusterDimension;
+  attr.val.clusterDim.x = blocks;
+  attr.val.clusterDim.y = 1;
+  attr.val.clusterDim.z = 1;
+  cfg.attrs = &attr;
+  cfg.numAttrs = 1;
+  st = cudaLaunchKernelEx(&cfg, sample_cluster_kernel<T>, logits, a);
+  count_launch();
+  return st;
 }
 
 }  // namespace
@@ -346,17 +953,15 @@ extern "C" int32_t et_b200_sample_v1(const et_b200_sampling_v1* s, const void* l
       return set_error(e, ET_KERNEL_ERROR_INVALID_ARGUMENT, ET_KERNEL_CODE_INVALID_BUFFER, op,
                        "logits must be aligned to their elements");
     auto st = static_cast<cudaStream_t>(stream);
-    auto go = [&](auto t) {
-      using T = decltype(t);
-      sample_kernel<T><<<(unsigned)s->rows, NT, 0, st>>>(
-          static_cast<const T*>(logits), s->row_stride, (int)s->vocabulary, uniform,
-          s->temperature, s->top_k, s->top_p, s->min_p, ids, logprobs);
-    };
-    if (s->dtype == ET_B200_DTYPE_F32) go(float{});
-    else if (s->dtype == ET_B200_DTYPE_F16) go(__half{});
-    else go(__nv_bfloat16{});
-    count_launch();
-    const cudaError_t status = cudaGetLastError();
+    const Args a{uniform, s->temperature, s->top_k, s->top_p, s->min_p, ids, logprobs,
+                 s->row_stride, (int)s->vocabulary, 0};
+    cudaError_t status;
+    if (s->dtype == ET_B200_DTYPE_F32)
+      status = launch(static_cast<const float*>(logits), a, s->rows, st);
+    else if (s->dtype == ET_B200_DTYPE_F16)
+      status = launch(static_cast<const __half*>(logits), a, s->rows, st);
+    else
+      status = launch(static_cast<const __nv_bfloat16*>(logits), a, s->rows, st);
     if (status != cudaSuccess) return cuda_error(e, status, op);
   }
   if (e) memset(e, 0, sizeof(*e));
