@@ -1,6 +1,6 @@
 // Sampling one token per row of logits (et_b200_sample_v1).
 //
-// Weights w(x) = exp((x - M) / temperature), M the row's maximum, as 2^-40
+// Weights w(x) = exp((x - M) / temperature), M the row's maximum, as 2^-35
 // fixed point: integer sums are the same in every order, so cumulative sums,
 // cuts and draws are deterministic whatever the thread layout.  A cut (top-k,
 // top-p) is a pair (logit, index): the tokens above a logit, and of those
@@ -35,7 +35,6 @@ namespace cg = cooperative_groups;
 
 constexpr int NT = 512, WARPS = NT / 32;
 constexpr int BINS = 2048;
-constexpr int FRACTION = 40;  // weights are multiples of 2^-40
 
 // Monotone integer image of a logit; NaN lowest, -0 equal to +0.
 __device__ __forceinline__ uint32_t key_of(float x) {
@@ -47,43 +46,44 @@ constexpr uint32_t kKeyMinusInf = 0x007fffffu;  // key_of(-inf)
 
 // log2(e) / temperature = hi + lo.  shift = M (hi + lo) = shift_hi + shift_lo
 // with shift_hi a multiple of 2^-8 below 2^15 (narrow), so that n + shift_hi
-// is exact for the integers n of the exponents.
+// is exact for the integers n of the exponents; low: logits below have weight
+// 0 whatever they are.
 struct Scale {
-  float max, hi, lo, shift, shift_hi, shift_lo;
+  float max, hi, lo, shift, shift_hi, shift_lo, low;
   bool narrow;
 };
-__device__ __forceinline__ Scale scale_of(float max, float temperature) {
+__device__ __forceinline__ Scale scale_of(float max, double per) {
   Scale s;
-  const double per = 1.4426950408889634 / (double)temperature;
   s.max = max;
   s.hi = (float)per;
   s.lo = (float)(per - (double)s.hi);
   const double shift = (double)max * per;
-  s.narrow = fabs(shift) < 32000.0;
+  s.narrow = fabs(shift) < 32000.0 && s.hi > 0x1p-60f;
   const double grid = rint(shift * 256.0) / 256.0;
   s.shift = (float)shift;
   s.shift_hi = (float)grid;
   s.shift_lo = (float)(shift - grid);
+  s.low = max - 64.0f / s.hi;
   return s;
 }
 
-// exp((x - max) / temperature) 2^40, rounded: 2^t with t = (x - max) (hi +
-// lo) = n + f, f accurate to about 2^-25 because its one large difference is
-// formed by an fma whose other operand is exact; 2^f - 1 by its series (|f|
-// <= 1/2, terms up to f^7: 5e-9).  The relative error is near 3e-8 whatever
-// the size of the logits.
-__device__ __forceinline__ uint64_t weight_of(float x, const Scale& s) {
+constexpr float kRound = 12582912.0f;  // 1.5 2^23: adding it rounds to an integer
+// 2^f = 1 + f (c1 + f (c2 + ...)), ck = ln(2)^k / k! to k = 7: |f| <= 1/2, error
+// 5e-9.  exp((x - max) / temperature) = 2^t, t = (x - max) (hi + lo) = n + f; f is
+// accurate to about 2^-25 because its one large difference is an fma whose
+// other operand is exact.  Relative error near 6e-8 whatever the size of the
+// logits.
+__device__ __forceinline__ float power_of(float x, const Scale& s) {
   float n, f;
   if (s.narrow) {
-    const float t = fmaf(x, s.hi, -s.shift);
-    if (!(t >= -(float)(FRACTION + 1))) return 0;
-    n = rintf(t);
-    f = fmaf(x, s.hi, -(n + s.shift_hi)) + fmaf(x, s.lo, -s.shift_lo);
+    x = fmaxf(x, s.low);  // NaN too
+    n = (fmaf(x, s.hi, -s.shift) + kRound) - kRound;
+    f = fmaf(x, s.hi, -n - s.shift_hi) + fmaf(x, s.lo, -s.shift_lo);
   } else {
-    if (!(x > -INFINITY)) return 0;
-    if (s.max == INFINITY) return x == INFINITY ? 1ull << FRACTION : 0;
+    if (!(x > -INFINITY)) return 0.0f;
+    if (s.max == INFINITY) return x == INFINITY ? 1.0f : 0.0f;
     const float d = x - s.max, t = d * s.hi;
-    if (!(t >= -(float)(FRACTION + 1))) return 0;
+    if (!(t >= -64.0f)) return 0.0f;
     const float bb = d - x, e = (x - (d - bb)) - (s.max + bb);
     n = rintf(t);
     f = (t - n) + (fmaf(d, s.hi, -t) + fmaf(d, s.lo, e * s.hi));
@@ -95,10 +95,76 @@ __device__ __forceinline__ uint64_t weight_of(float x, const Scale& s) {
   y = fmaf(y, f, 5.5504109e-2f);
   y = fmaf(y, f, 2.4022651e-1f);
   y = fmaf(y, f, 6.9314718e-1f);
-  y *= f;
-  const int right = -(int)n;  // 0 .. 41
-  const uint64_t w = (uint64_t)(0x80000000u + (uint32_t)__float2int_rn(y * 0x1p31f)) << (FRACTION - 31);
-  return (w + ((1ull << right) >> 1)) >> right;
+  y = fmaf(y, f, 1.0f);
+  return __int_as_float(__float_as_int(y) + ((int)n << 23));
+}
+// The weight in units of 2^-35.
+__device__ __forceinline__ uint64_t weight_of(float x, const Scale& s) {
+  return __float2ull_rn(power_of(x, s) * 0x1p35f);
+}
+
+// Sums of weights of up to 64 logits at a time, exact in f32: each is rounded
+// to multiples of 2^-17 (sums below 2^6) and the rest to multiples of 2^-35
+// (below 2^-12); both together round it as weight_of does.  Two logits per
+// packed instruction (narrow scales).
+struct Sum64 {
+  uint64_t coarse, fine;  // f32 pairs
+};
+__device__ __forceinline__ uint64_t pk(float a, float b) {
+  uint64_t r;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(a), "f"(b));
+  return r;
+}
+__device__ __forceinline__ float2 unpk(uint64_t v) {
+  float2 r;
+  asm("mov.b64 {%0, %1}, %2;" : "=f"(r.x), "=f"(r.y) : "l"(v));
+  return r;
+}
+__device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
+  uint64_t r;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+  return r;
+}
+__device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
+  uint64_t r;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+__device__ __forceinline__ uint64_t twice(float a) { return pk(a, a); }
+// power_of of two logits at once (narrow scales)
+__device__ __forceinline__ uint64_t powers_of(float a, float b, const Scale& s) {
+  const uint64_t x = pk(fmaxf(a, s.low), fmaxf(b, s.low)), hi = twice(s.hi), minus = twice(-1.0f);
+  const uint64_t m = add2(fma2(x, hi, twice(-s.shift)), twice(kRound));
+  const uint64_t n = add2(m, twice(-kRound));
+  const uint64_t f = add2(fma2(x, hi, fma2(n, minus, twice(-s.shift_hi))),
+                          fma2(x, twice(s.lo), twice(-s.shift_lo)));
+  uint64_t y = twice(1.5252734e-5f);
+  y = fma2(y, f, twice(1.5403530e-4f));
+  y = fma2(y, f, twice(1.3333558e-3f));
+  y = fma2(y, f, twice(9.6181291e-3f));
+  y = fma2(y, f, twice(5.5504109e-2f));
+  y = fma2(y, f, twice(2.4022651e-1f));
+  y = fma2(y, f, twice(6.9314718e-1f));
+  y = fma2(y, f, twice(1.0f));
+  // the integers n lie in the low bits of m
+  const float2 yy = unpk(y), mm = unpk(m);
+  return pk(__int_as_float(__float_as_int(yy.x) + (__float_as_int(mm.x) << 23)),
+            __int_as_float(__float_as_int(yy.y) + (__float_as_int(mm.y) << 23)));
+}
+__device__ __forceinline__ void add_weights(Sum64& sum, float a, float b, const Scale& s) {
+  const uint64_t w = powers_of(a, b, s), minus = twice(-1.0f);
+  const uint64_t q = add2(add2(w, twice(96.0f)), twice(-96.0f));
+  const uint64_t r = fma2(q, minus, w);
+  const uint64_t r2 = add2(add2(r, twice(0x1.8p-12f)), twice(-0x1.8p-12f));
+  sum.coarse = add2(sum.coarse, q);
+  sum.fine = add2(sum.fine, r2);
+}
+__device__ __forceinline__ uint64_t flush(Sum64& sum) {
+  const float2 c = unpk(sum.coarse), f = unpk(sum.fine);
+  const int64_t v = ((int64_t)__float2int_rn((c.x + c.y) * 0x1p17f) << 18) +
+                    (int64_t)__float2int_rn(f.x * 0x1p35f) + (int64_t)__float2int_rn(f.y * 0x1p35f);
+  sum.coarse = sum.fine = 0;
+  return (uint64_t)v;
 }
 
 struct Shared {
@@ -265,10 +331,12 @@ __device__ __forceinline__ float value_of(uint32_t key) {
   return __uint_as_float((key & 0x80000000u) ? (key & 0x7fffffffu) : ~key);
 }
 
+// A row's parameters, and what of them takes long double precision arithmetic
+// (formed while the logits arrive).
 struct Filters {
   float temperature, top_p, min_p;
   int64_t top_k;
-  double uniform;
+  double uniform, per, fall;  // log2(e) / temperature, temperature ln(min_p)
 };
 struct Args {
   const float* uniform;
@@ -288,6 +356,8 @@ __device__ __forceinline__ Filters filters_of(const Args& a, int64_t row) {
   f.top_p = a.top_p != nullptr ? a.top_p[row] : 1.0f;
   f.min_p = a.min_p != nullptr ? a.min_p[row] : 0.0f;
   f.uniform = (double)a.uniform[row];
+  f.per = 1.4426950408889634 / (double)f.temperature;
+  f.fall = f.min_p > 0.0f ? (double)f.temperature * log((double)fminf(f.min_p, 1.0f)) : 0.0;
   return f;
 }
 // What the running sum has to reach: the first integer above u total, inside
@@ -304,7 +374,7 @@ __device__ __forceinline__ uint64_t share_aim(float p, uint64_t total) {
 // The least logit that min_p keeps (-inf: no limit).
 __device__ __forceinline__ float least_logit(const Filters& f, float max) {
   if (!(f.min_p > 0.0f) || max == INFINITY) return -INFINITY;
-  const double least = (double)max + (double)f.temperature * log((double)fminf(f.min_p, 1.0f));
+  const double least = (double)max + f.fall;
   const float x = (float)least;
   return (double)x < least ? nextafterf(x, INFINITY) : x;
 }
@@ -313,7 +383,7 @@ __device__ __forceinline__ void answer(const Args& a, int64_t row, int id, float
   a.ids[row] = id;
   if (a.logprobs == nullptr) return;
   const double d = sc.max == INFINITY ? 0.0 : (double)x - (double)sc.max;
-  a.logprobs[row] = (float)(d / (double)f.temperature -
+  a.logprobs[row] = (float)(d * f.per * 0.6931471805599453 -
                             log((double)total / (double)weight_of(sc.max, sc)));
 }
 
@@ -349,10 +419,25 @@ __device__ void sample_row(const T* x, const Args& a, int64_t row, const Filters
 // ---- rows in the shared memory of a cluster ------------------------------------------------
 
 constexpr int LIST = 1024;       // entries of a list, steps of a histogram
-constexpr float kSteps = 24.0f;  // histogram steps per factor of 2 of a weight: 1,024 reach 2^-42
+constexpr float kTopSteps = 40.0f;  // steps per unit of the logit for a large top-k
 
 __device__ __forceinline__ void cp16(uint32_t dst, const void* src) {
   asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
+}
+
+// The largest value of a 16-byte piece; NaN only where all are.
+template <typename T>
+__device__ __forceinline__ float piece_max(const uint4& v) {
+  if constexpr (sizeof(T) == 4) {
+    return fmaxf(fmaxf(__uint_as_float(v.x), __uint_as_float(v.y)),
+                 fmaxf(__uint_as_float(v.z), __uint_as_float(v.w)));
+  } else {
+    using T2 = std::conditional_t<std::is_same_v<T, __half>, __half2, __nv_bfloat162>;
+    union { uint32_t w; T2 h; } a, b, c, d;
+    a.w = v.x; b.w = v.y; c.w = v.z; d.w = v.w;
+    const T2 m = __hmax2(__hmax2(a.h, b.h), __hmax2(c.h, d.h));
+    return fmaxf(to_f32<T>(m.x), to_f32<T>(m.y));
+  }
 }
 
 // A slice of n logits in shared memory, stored at their global address modulo
@@ -362,6 +447,44 @@ struct Slice {
   static constexpr int N = 16 / sizeof(T);
   const T* x;               // in shared memory
   int n, head, pieces;      // tokens before the first whole piece, whole pieces
+  // f(i, value) for every token that may reach `least`, in no particular order
+  // (16-byte pieces without one are skipped)
+  template <typename F>
+  __device__ __forceinline__ void each_from(float least, F f) const {
+    for (int p = threadIdx.x; p < pieces; p += NT) {
+      union { uint4 v; T x[N]; } u;
+      u.v = *reinterpret_cast<const uint4*>(x + head + p * N);
+      if (piece_max<T>(u.v) >= least)
+#pragma unroll
+        for (int k = 0; k < N; k++) f(head + p * N + k, to_f32<T>(u.x[k]));
+    }
+    const int t = threadIdx.x, tail = head + pieces * N;
+    if (t < head) f(t, to_f32<T>(x[t]));
+    else if (t >= 32 && tail + t - 32 < n) f(tail + t - 32, to_f32<T>(x[tail + t - 32]));
+  }
+  // f(i, values) for every piece of N tokens from i that may reach `least`;
+  // what is no whole piece comes with the rest of its values -inf
+  template <typename F>
+  __device__ __forceinline__ void each_piece(float least, F f) const {
+    for (int p = threadIdx.x; p < pieces + 2; p += NT) {
+      float v[N], top = -INFINITY;
+      int i = head + p * N;
+      if (p < pieces) {
+        union { uint4 v; T x[N]; } u;
+        u.v = *reinterpret_cast<const uint4*>(x + i);
+#pragma unroll
+        for (int k = 0; k < N; k++) v[k] = to_f32<T>(u.x[k]);
+      } else {
+        i = p == pieces ? 0 : head + pieces * N;
+        const int end = p == pieces ? head : n;
+#pragma unroll
+        for (int k = 0; k < N; k++) v[k] = i + k < end ? to_f32<T>(x[i + k]) : -INFINITY;
+      }
+#pragma unroll
+      for (int k = 0; k < N; k++) top = fmaxf(top, v[k]);
+      if (top >= least) f(i, v);
+    }
+  }
   // f(i, value) for every token, in no particular order
   template <typename F>
   __device__ __forceinline__ void each(F f) const {
@@ -422,7 +545,7 @@ struct Room {
   };
   uint64_t warp[WARPS];
   uint64_t found[4];
-  float top;
+  float top, bound;
   int count, keep, step, before;
   Border border;
   uint64_t total;
@@ -447,7 +570,7 @@ __device__ __forceinline__ uint64_t room_scan(uint64_t v, Room& rm, uint64_t* al
 
 // A value that at least k of the threads' maxima (`mine`, `top` the largest)
 // reach, so a lower bound of the k-th largest logit of the slice, and not many
-// more than 2 k: histograms of 256 steps over the maxima, each into the
+// more than 5 k / 4: histograms of 256 steps over the maxima, each into the
 // border's step of the one before.  -inf where fewer than k are finite.
 __device__ float top_bound(float mine, float top, int k, Room& rm) {
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
@@ -493,7 +616,7 @@ __device__ float top_bound(float mine, float top, int k, Room& rm) {
     const int reach = __syncthreads_count(some && mine >= edge);
     if (reach < k) break;  // the steps are finer than the values' rounding
     bound = fmaxf(bound, edge);
-    if (reach <= 2 * k + 32) break;
+    if (reach <= k + k / 4 + 16) break;
     above += before;
     high -= (float)step * width;
     low = edge;
@@ -502,29 +625,82 @@ __device__ float top_bound(float mine, float top, int k, Room& rm) {
   return bound;
 }
 
-// Gathers the blocks' lists (rm.list, rm.count) into rm.all of rank 0; the
-// number of entries, or -1 if they do not fit (every block gets the same).
-__device__ int gather_lists(cg::cluster_group& cluster, Room& rm, unsigned rank, unsigned blocks) {
-  cluster.sync();
-  int total = 0;
-  bool fits = true;
-  for (unsigned b = 0; b < blocks; b++) {
-    const int c = cluster.map_shared_rank(&rm, b)->count;
-    fits = fits && c <= LIST;
-    if (rank == 0 && fits && total + c <= LIST) {
-      const uint64_t* from = cluster.map_shared_rank(&rm, b)->list;
-      for (int i = threadIdx.x; i < c; i += NT) rm.all[total + i] = from[i];
-    }
-    total += c;
-    fits = fits && total <= LIST;
-  }
-  __syncthreads();
-  return fits ? total : -1;
+// Adds a token to the cluster's list in rank 0 (dropped when it is full).
+__device__ __forceinline__ void push(Room* to, uint64_t entry) {
+  const int at = atomicAdd(&to->count, 1);
+  if (at < LIST) to->all[at] = entry;
 }
 
-// Rank 0: cuts the gathered list of n entries by all filters and draws.
+// Ranks the n <= NT entries of rm.all, their weights in rm.list: every entry
+// is compared with all others, the NT threads sharing an entry's comparisons
+// in groups of `parts` neighbouring lanes.  That takes n^2 / NT steps without a
+// barrier, where sorting takes some log(n)^2 / 2 with one each.
+struct Ranking {
+  int parts;      // threads per entry
+  int entry;      // of this thread's group
+  bool mine;      // the entry exists
+};
+__device__ __forceinline__ Ranking ranking_of(int n) {
+  Ranking r;
+  r.parts = 1;
+  while (r.parts < 32 && r.parts * 2 * n <= NT) r.parts *= 2;
+  r.entry = threadIdx.x / r.parts;
+  r.mine = r.entry < n;
+  return r;
+}
+// The number and the weights of the entries for which `before(other)` holds.
+template <typename Before>
+__device__ __forceinline__ void count_before(const Ranking& r, int n, const Room& rm, Before before,
+                                             int* number, uint64_t* mass) {
+  int c = 0;
+  uint64_t m = 0;
+  if (r.mine)
+#pragma unroll 4
+    for (int j = threadIdx.x % r.parts; j < n; j += r.parts) {
+      const uint64_t other = rm.all[j], w = rm.list[j];
+      const bool b = before(other);
+      c += b ? 1 : 0;
+      m += b ? w : 0;
+    }
+  for (int o = 1; o < r.parts; o <<= 1) {
+    c += __shfl_xor_sync(0xffffffffu, c, o);
+    m += __shfl_xor_sync(0xffffffffu, m, o);
+  }
+  *number = c;
+  *mass = m;
+}
+
+// Rank 0: cuts the list of n entries by all filters and draws (n <= NT).
+__device__ void draw_from_short_list(int n, const Args& a, int64_t row, const Filters& flt,
+                                     const Scale& sc, Room& rm) {
+  const int tid = threadIdx.x;
+  rm.list[tid] = tid < n ? weight_of(entry_value(rm.all[tid]), sc) : 0;
+  __syncthreads();
+  const Ranking r = ranking_of(n);
+  const uint64_t e = r.mine ? rm.all[r.entry] : 0, w = r.mine ? rm.list[r.entry] : 0;
+  const float x = entry_value(e);
+  const bool first = r.mine && tid % r.parts == 0;  // speaks for its entry
+  int rank;
+  uint64_t before, all;
+  count_before(r, n, rm, [&](uint64_t other) { return other > e; }, &rank, &before);
+  const int k = flt.top_k > 0 && flt.top_k < n ? (int)flt.top_k : n;
+  room_scan(first && rank < k ? w : 0, rm, &all);
+  const uint64_t aim = flt.top_p < 1.0f ? share_aim(flt.top_p, all) : all;
+  const bool keep = first && rank < k && (before < aim || rank == 0) && x >= least_logit(flt, sc.max);
+  room_scan(keep ? w : 0, rm, &all);  // its barriers also end the reading of the weights
+  if (first && !keep) rm.list[r.entry] = 0;
+  __syncthreads();
+  const uint64_t to = draw_aim(flt.uniform, all);
+  int unused;
+  uint64_t run;  // indexes are stored inverted
+  count_before(r, n, rm, [&](uint64_t other) { return (uint32_t)other > (uint32_t)e; }, &unused, &run);
+  if (keep && run < to && to <= run + w) answer(a, row, entry_index(e), x, flt, sc, all);
+}
+
+// The same for any list, by sorting.
 __device__ void draw_from_list(int n, const Args& a, int64_t row, const Filters& flt,
                                const Scale& sc, Room& rm) {
+  if (n <= NT) return draw_from_short_list(n, a, row, flt, sc, rm);
   constexpr int PER = LIST / NT;
   const int tid = threadIdx.x;
   const int size = pad_list(rm.all, n);
@@ -579,14 +755,49 @@ __device__ void draw_from_list(int n, const Args& a, int64_t row, const Filters&
   }
 }
 
+// Sums over the blocks of a cluster of a value that each has in rm.total.
+__device__ __forceinline__ uint64_t cluster_total(cg::cluster_group& cluster, Room& rm,
+                                                  unsigned blocks) {
+  uint64_t all = 0;
+#pragma unroll
+  for (unsigned b = 0; b < 8; b++)
+    if (b < blocks) all += cluster.map_shared_rank(&rm, b)->total;
+  return all;
+}
+
+// What a cut adds up: tokens or weights.
+struct Tokens {
+  __device__ __forceinline__ uint64_t operator()(float x) const { return x > -INFINITY; }
+  __device__ __forceinline__ void both(float x, float y, uint64_t (&w)[2]) const {
+    w[0] = x > -INFINITY;
+    w[1] = y > -INFINITY;
+  }
+};
+struct Weights {
+  Scale sc;
+  __device__ __forceinline__ uint64_t operator()(float x) const { return weight_of(x, sc); }
+  __device__ __forceinline__ void both(float x, float y, uint64_t (&w)[2]) const {
+    if (sc.narrow) {
+      const float2 p = unpk(powers_of(x, y, sc));
+      w[0] = __float2ull_rn(p.x * 0x1p35f);
+      w[1] = __float2ull_rn(p.y * 0x1p35f);
+    } else {
+      w[0] = weight_of(x, sc);
+      w[1] = weight_of(y, sc);
+    }
+  }
+};
+
 // Lowers `border` to the shortest prefix of the ranking of the tokens it keeps
-// whose units reach aim(total) (0: unchanged); `per` histogram steps per unit
-// of the logit.  False (in every block of the
-// cluster) when the border's step holds more tokens than a list.
-template <typename T, typename Unit, typename Aim>
+// whose units reach `to` (at least 1, at most their sum); tokens under `least`
+// are known to lie behind it.  `per` histogram steps per unit of the logit.
+// False (in every block of the cluster) when the border's step holds more
+// tokens than a list or `least` was not low enough.
+template <typename T, typename Unit>
 __device__ bool cluster_cut(cg::cluster_group& cluster, Room& rm, unsigned rank, unsigned blocks,
-                            const Slice<T>& slice, int first, float max, float per, Border& border,
-                            Unit unit, Aim aim) {
+                            const Slice<T>& slice, int first, float max, float per, float least,
+                            Border& border, const Unit unit, uint64_t to) {
+  constexpr bool COUNT = std::is_same_v<Unit, Tokens>;
   constexpr int PER = LIST / NT;
   const int tid = threadIdx.x;
   // steps of 1 / per of the logit, falling; the last takes all below
@@ -594,33 +805,53 @@ __device__ bool cluster_cut(cg::cluster_group& cluster, Room& rm, unsigned rank,
     const float t = (max - x) * per;
     return t > 0.0f ? (int)fminf(t, (float)(LIST - 1)) : 0;
   };
+  least = fmaxf(least, border.value);
   cluster.sync();  // nobody reads this block's room any more
   for (int i = tid; i < LIST; i += NT) rm.low[i] = rm.high[i] = 0;
   __syncthreads();
-  slice.each([&](int i, float x) {
-    if (!kept(border, x, first + i)) return;
-    const uint64_t w = unit(x);
+  auto add = [&](float x, uint64_t w) {
     if (w == 0) return;
     const int step = step_of(x);
+    if (COUNT) {
+      atomicAdd(&rm.low[step], (uint32_t)w);
+      return;
+    }
     const uint32_t lo = (uint32_t)w, old = atomicAdd(&rm.low[step], lo);
     const uint32_t hi = (uint32_t)(w >> 32) + (old + lo < old ? 1u : 0u);
     if (hi != 0) atomicAdd(&rm.high[step], hi);
+  };
+  slice.each_piece(least, [&](int i, const float (&v)[Slice<T>::N]) {
+#pragma unroll
+    for (int k = 0; k < Slice<T>::N; k += 2) {
+      const bool a = v[k] >= least && kept(border, v[k], first + i + k);
+      const bool b = v[k + 1] >= least && kept(border, v[k + 1], first + i + k + 1);
+      if (a || b) {
+        uint64_t w[2];
+        unit.both(v[k], v[k + 1], w);
+        if (a) add(v[k], w[0]);
+        if (b) add(v[k + 1], w[1]);
+      }
+    }
   });
   cluster.sync();
-  uint64_t bins[PER], mine = 0, all;
+  static_assert(PER == 2, "two steps per thread");
+  uint64_t bins[PER] = {0, 0}, all;
 #pragma unroll
-  for (int j = 0; j < PER; j++) {
-    const int i = tid * PER + j;
-    bins[j] = 0;
-    for (unsigned b = 0; b < blocks; b++) {
+  for (unsigned b = 0; b < 8; b++)
+    if (b < blocks) {
       const Room* r = cluster.map_shared_rank(&rm, b);
-      bins[j] += ((uint64_t)r->high[i] << 32) | r->low[i];
+      const uint2 lo = *reinterpret_cast<const uint2*>(&r->low[2 * tid]);
+      bins[0] += lo.x;
+      bins[1] += lo.y;
+      if (!COUNT) {
+        const uint2 hi = *reinterpret_cast<const uint2*>(&r->high[2 * tid]);
+        bins[0] += (uint64_t)hi.x << 32;
+        bins[1] += (uint64_t)hi.y << 32;
+      }
     }
-    mine += bins[j];
-  }
-  uint64_t run = room_scan(mine, rm, &all) - mine;
-  const uint64_t to = aim(all);
-  if (to == 0 || to > all) return true;
+  uint64_t run = room_scan(bins[0] + bins[1], rm, &all) - bins[0] - bins[1];
+  if (tid == 0) rm.count = 0, rm.found[0] = LIST;
+  __syncthreads();
 #pragma unroll
   for (int j = 0; j < PER; j++) {
     if (run < to && to <= run + bins[j]) {
@@ -629,40 +860,133 @@ __device__ bool cluster_cut(cg::cluster_group& cluster, Room& rm, unsigned rank,
     }
     run += bins[j];
   }
-  if (tid == 0) rm.count = 0;
-  cluster.sync();  // every block is done with the histograms: lists take their place
+  cluster.sync();  // every block is done with the histograms: the list takes their place
   const int step = (int)rm.found[0];
   const uint64_t rest = rm.found[1];
-  slice.each([&](int i, float x) {
-    if (!kept(border, x, first + i) || step_of(x) != step || unit(x) == 0) return;
-    const int at = atomicAdd(&rm.count, 1);
-    if (at < LIST) rm.list[at] = entry_of(x, first + i);
+  if (step >= LIST) return false;
+  Room* head = cluster.map_shared_rank(&rm, 0);
+  // below the step's lower edge whatever step_of rounds
+  const float from = step == LIST - 1 ? least
+                                      : fmaxf(least, max - ((float)step + 1.01f) / per - fabsf(max) * 1e-6f);
+  slice.each_from(from, [&](int i, float x) {
+    if (x >= from && step_of(x) == step && kept(border, x, first + i)) push(head, entry_of(x, first + i));
   });
-  const int n = gather_lists(cluster, rm, rank, blocks);
-  if (n < 0) return false;
+  cluster.sync();
   if (rank == 0) {
-    sort_descending(rm.all, pad_list(rm.all, n));
-    mine = 0;
-    uint64_t w[PER];
-#pragma unroll
-    for (int j = 0; j < PER; j++) {
-      const int i = tid * PER + j;
-      w[j] = i < n ? unit(entry_value(rm.all[i])) : 0;
-      mine += w[j];
-    }
-    run = room_scan(mine, rm, &all) - mine;
-#pragma unroll
-    for (int j = 0; j < PER; j++) {
-      if (run < rest && rest <= run + w[j]) {
-        const uint64_t e = rm.all[tid * PER + j];
+    const int n = rm.count;
+    if (tid == 0) rm.border = Border{NAN, 0};
+    __syncthreads();
+    if (n <= NT) {
+      rm.list[tid] = tid < n ? unit(entry_value(rm.all[tid])) : 0;
+      __syncthreads();
+      const Ranking r = ranking_of(n);
+      const uint64_t e = r.mine ? rm.all[r.entry] : 0;
+      int unused;
+      uint64_t before;
+      count_before(r, n, rm, [&](uint64_t other) { return other > e; }, &unused, &before);
+      if (r.mine && before < rest && rest <= before + rm.list[r.entry])
         rm.border = Border{entry_value(e), entry_index(e)};
+    } else if (n <= LIST) {
+      sort_descending(rm.all, pad_list(rm.all, n));
+      uint64_t w[PER], mine = 0;
+#pragma unroll
+      for (int j = 0; j < PER; j++) {
+        const int i = tid * PER + j;
+        w[j] = i < n ? unit(entry_value(rm.all[i])) : 0;
+        mine += w[j];
       }
-      run += w[j];
+      run = room_scan(mine, rm, &all) - mine;
+#pragma unroll
+      for (int j = 0; j < PER; j++) {
+        if (run < rest && rest <= run + w[j]) {
+          const uint64_t e = rm.all[tid * PER + j];
+          rm.border = Border{entry_value(e), entry_index(e)};
+        }
+        run += w[j];
+      }
     }
   }
   cluster.sync();
-  border = cluster.map_shared_rank(&rm, 0)->border;
+  const Border found = head->border;
+  if (!(found.value == found.value)) return false;
+  border = found;
   return true;
+}
+
+// The block's weights that `border` keeps: their sum, the sums per warp in
+// rm.warp; warp w takes the tokens from span_of(w) to span_of(w + 1).
+template <typename T>
+__device__ __forceinline__ int span_of(const Slice<T>& s, int w) {
+  if (w == 0) return 0;
+  if (w >= WARPS) return s.n;
+  return s.head + min(s.pieces, w * ((s.pieces + WARPS - 1) / WARPS)) * Slice<T>::N;
+}
+template <typename T>
+__device__ uint64_t block_weights(const Slice<T>& s, int first, const Border& border,
+                                  const Scale& sc, Room& rm) {
+  constexpr int N = Slice<T>::N;
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const int each = (s.pieces + WARPS - 1) / WARPS;
+  const int p0 = min(s.pieces, warp * each), p1 = min(s.pieces, p0 + each);
+  auto weight_at = [&](int i) -> uint64_t {
+    const float v = to_f32<T>(s.x[i]);
+    return kept(border, v, first + i) ? weight_of(v, sc) : 0;
+  };
+  uint64_t sum = 0;
+  if (sc.narrow) {
+    const bool every = border.value == -INFINITY;
+    Sum64 part{0, 0};
+    int in = 0;
+    for (int p = p0 + lane; p < p1; p += 32) {
+      union { uint4 v; T x[N]; } u;
+      u.v = *reinterpret_cast<const uint4*>(s.x + s.head + p * N);
+      float v[N], top = -INFINITY;
+#pragma unroll
+      for (int k = 0; k < N; k++) {
+        v[k] = to_f32<T>(u.x[k]);
+        top = fmaxf(top, v[k]);
+      }
+      if (!every) {
+        if (!(top >= border.value)) continue;
+        const int i = first + s.head + p * N;
+#pragma unroll
+        for (int k = 0; k < N; k++) v[k] = kept(border, v[k], i + k) ? v[k] : -INFINITY;
+      }
+#pragma unroll
+      for (int k = 0; k < N; k += 2) add_weights(part, v[k], v[k + 1], sc);
+      if ((in += N) == 64) {
+        sum += flush(part);
+        in = 0;
+      }
+    }
+    sum += flush(part);
+  } else {
+    for (int p = p0 + lane; p < p1; p += 32) {
+      union { uint4 v; T x[N]; } u;
+      u.v = *reinterpret_cast<const uint4*>(s.x + s.head + p * N);
+      float top = to_f32<T>(u.x[0]);
+#pragma unroll
+      for (int k = 1; k < N; k++) top = fmaxf(top, to_f32<T>(u.x[k]));
+      if (top >= border.value)
+#pragma unroll
+        for (int k = 0; k < N; k++) {
+          const float v = to_f32<T>(u.x[k]);
+          if (kept(border, v, first + s.head + p * N + k)) sum += weight_of(v, sc);
+        }
+    }
+  }
+  if (warp == 0 && lane < s.head) sum += weight_at(lane);
+  const int tail = s.head + s.pieces * N;
+  if (warp == WARPS - 1 && tail + lane < s.n) sum += weight_at(tail + lane);
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+  __syncthreads();
+  if (lane == 0) rm.warp[warp] = sum;
+  __syncthreads();
+  uint64_t here = 0;
+#pragma unroll
+  for (int w = 0; w < WARPS; w++) here += rm.warp[w];
+  return here;
 }
 
 template <typename T>
@@ -718,8 +1042,7 @@ __global__ void __launch_bounds__(NT, 2) sample_cluster_kernel(const T* __restri
     for (int p = g * part + tid; p < end; p += NT) {  // the pieces this thread copied
       union { uint4 v; T x[Slice<T>::N]; } u;
       u.v = *reinterpret_cast<const uint4*>(mine + slice.head + p * Slice<T>::N);
-#pragma unroll
-      for (int k = 0; k < Slice<T>::N; k++) top = fmaxf(top, to_f32<T>(u.x[k]));
+      top = fmaxf(top, piece_max<T>(u.v));
     }
   }
   const float thread_top = top;
@@ -735,8 +1058,7 @@ __global__ void __launch_bounds__(NT, 2) sample_cluster_kernel(const T* __restri
   float max = -INFINITY;
   for (unsigned b = 0; b < blocks; b++) max = fmaxf(max, cluster.map_shared_rank(&rm, b)->top);
 
-  // every path ends with a cluster.sync: no block leaves while another reads
-  // its shared memory
+  // no block leaves while another may read or write its shared memory
   if (max == -INFINITY) {
     if (rank == 0 && tid == 0) {
       a.ids[row] = -1;
@@ -765,27 +1087,46 @@ __global__ void __launch_bounds__(NT, 2) sample_cluster_kernel(const T* __restri
     cluster.sync();
     return;
   }
-  const Scale sc = scale_of(max, flt.temperature);
+  const Scale sc = scale_of(max, flt.per);
   const bool top_k = flt.top_k > 0 && flt.top_k < a.n;
 
   // ---- a list
   bool listed = a.n <= LIST;
   float bound = -INFINITY;
   if (!listed && top_k && flt.top_k <= NT / 2) {
-    bound = top_bound(thread_top, block_top, (int)flt.top_k, rm);
+    // What k / blocks tokens of every slice reach, k tokens of the row reach;
+    // where a slice has fewer, what k tokens of one slice reach.
+    bound = top_bound(thread_top, block_top, ((int)flt.top_k + (int)blocks - 1) / (int)blocks, rm);
+    auto exchange = [&](bool least) {
+      if (tid == 0) rm.bound = bound;
+      cluster.sync();
+#pragma unroll
+      for (unsigned b = 0; b < 8; b++)
+        if (b < blocks) {
+          const float other = cluster.map_shared_rank(&rm, b)->bound;
+          bound = least ? fminf(bound, other) : fmaxf(bound, other);
+        }
+    };
+    exchange(true);
+    if (blocks > 1 && bound == -INFINITY) {
+      bound = top_bound(thread_top, block_top, (int)flt.top_k, rm);
+      cluster.sync();  // the first bounds are read
+      exchange(false);
+    }
     listed = true;
   }
   if (listed) {
-    slice.each([&](int i, float v) {
-      if (v > -INFINITY && v >= bound) {
-        const int p = atomicAdd(&rm.count, 1);
-        if (p < LIST) rm.list[p] = entry_of(v, first + i);
-      }
+    Room* head = cluster.map_shared_rank(&rm, 0);
+    slice.each_from(bound, [&](int i, float v) {
+      if (v > -INFINITY && v >= bound) push(head, entry_of(v, first + i));
     });
-    const int n = gather_lists(cluster, rm, rank, blocks);
-    if (n >= 0) {
-      if (rank == 0) draw_from_list(n, a, row, flt, sc, rm);
+    cluster.sync();
+    const int n = head->count;
+    if (n <= LIST) {
+      // only rank 0 has work left, in its own memory; it waits until the others
+      // have read its count
       cluster.sync();
+      if (rank == 0) draw_from_list(n, a, row, flt, sc, rm);
       return;
     }
   }
@@ -793,56 +1134,72 @@ __global__ void __launch_bounds__(NT, 2) sample_cluster_kernel(const T* __restri
   // ---- cuts from histograms
   Border border{-INFINITY, -1};
   bool good = true;
-  if (top_k)
-    good = cluster_cut<T>(cluster, rm, rank, blocks, slice, first, max, kSteps * 1.4427f, border,
-                          [](float) -> uint64_t { return 1; },
-                          [&](uint64_t all) { return (uint64_t)flt.top_k < all ? (uint64_t)flt.top_k : 0ull; });
-  if (good && flt.top_p < 1.0f)
-    good = cluster_cut<T>(cluster, rm, rank, blocks, slice, first, max, kSteps * sc.hi, border,
-                          [&](float v) { return weight_of(v, sc); },
-                          [&](uint64_t all) { return share_aim(flt.top_p, all); });
+  if (top_k) {
+    // how many there are to rank
+    int some = 0;
+    slice.each([&](int, float v) { some += v > -INFINITY; });
+    some = __reduce_add_sync(0xffffffffu, some);
+    __syncthreads();
+    if (lane == 0) rm.warp[warp] = (uint64_t)some;
+    __syncthreads();
+    if (tid == 0) {
+      uint64_t t = 0;
+      for (int w = 0; w < WARPS; w++) t += rm.warp[w];
+      rm.total = t;
+    }
+    cluster.sync();
+    if ((uint64_t)flt.top_k < cluster_total(cluster, rm, blocks))
+      good = cluster_cut<T>(cluster, rm, rank, blocks, slice, first, max, kTopSteps, -INFINITY, border,
+                            Tokens{}, (uint64_t)flt.top_k);
+    cluster.sync();
+  }
+  if (good && flt.top_p < 1.0f) {
+    const uint64_t here = block_weights(slice, first, border, sc, rm);
+    if (tid == 0) rm.total = here;
+    cluster.sync();
+    const uint64_t all = cluster_total(cluster, rm, blocks);
+    const uint64_t to = share_aim(flt.top_p, all);
+    // The tokens from the border down weigh more than the mass that may go, so
+    // the border's weight is over its share of a token; a little less, for the
+    // rounding of weights (half a unit) and logits.
+    const double gone = (double)(all - to) / (double)a.n;
+    float least = -INFINITY;
+    if (max < INFINITY)
+      least = (float)((double)max + (double)flt.temperature * log(fmax(gone - 0.51, 0.49) * (0.999 * 0x1p-35))) -
+              fabsf(max) * 1e-6f;
+    // all steps between the maximum and `least`
+    const float per = fminf((float)(LIST - 1) / fmaxf(max - least, 0.0f), 1e30f);
+    good = cluster_cut<T>(cluster, rm, rank, blocks, slice, first, max, per, least, border,
+                          Weights{sc}, to);
+    cluster.sync();
+  }
   if (!good) {
-    cluster.sync();
     if (rank == 0) sample_row<T>(x, a, row, flt, sc, rm.radix);
-    cluster.sync();
     return;
   }
   const float least = least_logit(flt, sc.max);
   if (least > border.value) border = Border{least, INT32_MAX};
 
   // ---- the draw: running sums by block, warp, lane
-  auto weight_at = [&](int i) -> uint64_t {
-    const float v = to_f32<T>(slice.x[i]);
-    return kept(border, v, first + i) ? weight_of(v, sc) : 0;
-  };
-  const int span = (slice.n + WARPS - 1) / WARPS;
-  const int w0 = min(slice.n, warp * span), w1 = min(slice.n, w0 + span);
-  uint64_t sum = 0;
-  for (int i = w0 + lane; i < w1; i += 32) sum += weight_at(i);
-#pragma unroll
-  for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
-  __syncthreads();
-  if (lane == 0) rm.warp[warp] = sum;
-  __syncthreads();
-  uint64_t here = 0;
-#pragma unroll
-  for (int w = 0; w < WARPS; w++) here += rm.warp[w];
+  const uint64_t here = block_weights(slice, first, border, sc, rm);
   if (tid == 0) rm.total = here;
   cluster.sync();
-  uint64_t all = 0, before = 0;
-  for (unsigned b = 0; b < blocks; b++) {
-    const uint64_t t = cluster.map_shared_rank(&rm, b)->total;
-    if (b < rank) before += t;
-    all += t;
-  }
+  const uint64_t all = cluster_total(cluster, rm, blocks);
+  uint64_t before = 0;
+  for (unsigned b = 0; b < rank; b++) before += cluster.map_shared_rank(&rm, b)->total;
+  cluster.sync();  // nothing of another block is read any more
   const uint64_t to = draw_aim(flt.uniform, all);
   if (before < to && to <= before + here) {
     uint64_t rest = to - before;
     int w = 0;
     while (w < WARPS - 1 && rest > rm.warp[w]) rest -= rm.warp[w++];
     __syncthreads();
-    const int s0 = min(slice.n, w * span), s1 = min(slice.n, s0 + span);
-    const int each = (span + NT - 1) / NT;
+    auto weight_at = [&](int i) -> uint64_t {
+      const float v = to_f32<T>(slice.x[i]);
+      return kept(border, v, first + i) ? weight_of(v, sc) : 0;
+    };
+    const int s0 = span_of(slice, w), s1 = span_of(slice, w + 1);
+    const int each = (s1 - s0 + NT - 1) / NT;
     const int t0 = min(s1, s0 + tid * each), t1 = min(s1, t0 + each);
     uint64_t mine_sum = 0, unused;
     for (int i = t0; i < t1; i++) mine_sum += weight_at(i);
@@ -856,7 +1213,6 @@ __global__ void __launch_bounds__(NT, 2) sample_cluster_kernel(const T* __restri
       answer(a, row, first + i, to_f32<T>(slice.x[i]), flt, sc, all);
     }
   }
-  cluster.sync();
 }
 
 // Vocabularies beyond the shared memory of a cluster.
@@ -886,7 +1242,7 @@ __global__ void __launch_bounds__(NT) sample_kernel(const T* __restrict__ logits
     }
     return;
   }
-  sample_row<T>(x, a, row, flt, scale_of(value_of(best_key), flt.temperature), sm);
+  sample_row<T>(x, a, row, flt, scale_of(value_of(best_key), flt.per), sm);
 }
 
 // Clusters of as few thread blocks as hold a row (two of them per SM), and of

@@ -73,14 +73,13 @@ class PagedCache:
         _need(strides[0] == strides[1], "both pools must have the same strides")
         self.lib = load()
         self.keys, self.values = keys, values
-        self.device, self.dtype = keys.device, keys.dtype
+        self.device, self.index, self.dtype = keys.device, keys.get_device(), keys.dtype
         self.pages, self.kv_heads, self.page_size, self.head_dim = keys.shape
         page, head, token = strides[0]
         self.descriptor = CacheDescriptor(
             C.sizeof(CacheDescriptor), keys.data_ptr(), values.data_ptr(), self.pages,
             self.page_size, self.kv_heads, self.head_dim, page, head, token, DTYPES[keys.dtype], 0)
         self._ref = C.byref(self.descriptor)
-        self._row = (self.kv_heads, self.head_dim)
 
     @staticmethod
     def _strides(t):
@@ -103,9 +102,11 @@ class PagedCache:
         err = k1.KernelError()
         k_stride = _rows(k, batch, self, self.kv_heads, "k")
         v_stride = _rows(v, batch, self, self.kv_heads, "v")
-        _check(self.lib.et_b200_paged_append_v1(
+        rc = self.lib.et_b200_paged_append_v1(
             self._ref, batch.bind(self), batch.rope(rope, self), k.data_ptr(), k_stride,
-            v.data_ptr(), v_stride, stream, C.byref(err)), err)
+            v.data_ptr(), v_stride, stream, C.byref(err))
+        if rc != 0:
+            _check(rc, err)
 
 
 class PagedBatch:
@@ -131,7 +132,7 @@ class PagedBatch:
         for t in tensors:
             _need(t.is_cuda and t.device == offsets.device and t.is_contiguous(),
                   "the batch's tensors must be dense CUDA tensors of one device")
-        self.tokens, self.device = int(tokens), offsets.device
+        self.tokens, self.index = int(tokens), offsets.get_device()
         self.keepalive = tensors
         columns = page_table.shape[1]
         self.descriptor = BatchDescriptor(
@@ -141,35 +142,38 @@ class PagedBatch:
             lengths.data_ptr(), page_table.data_ptr(),
             status.data_ptr() if status is not None else None)
         self._ref = C.byref(self.descriptor)
-        self._rope = RopeDescriptor()
-        self._rope_ref = C.byref(self._rope)
 
     def bind(self, cache: PagedCache):
-        _need(self.device == cache.device, "the batch and the cache are on different devices")
-        _need(torch.cuda.current_device() == cache.device.index,
-              "the cache's device is not the current one")
+        if self.index != cache.index:
+            raise ValueError("the batch and the cache are on different devices")
+        if torch.cuda.current_device() != cache.index:
+            raise ValueError("the cache's device is not the current one")
         return self._ref
 
     def rope(self, tables, cache: PagedCache):
         if tables is None:
             return None
         cos, sin = tables
-        _need(cos.shape == sin.shape and cos.dim() == 2 and cos.shape[1] * 2 == cache.head_dim and
-              cos.dtype == sin.dtype == torch.float32 and cos.is_contiguous() and
-              sin.is_contiguous() and cos.device == sin.device == cache.device,
-              "RoPE tables must be dense f32 [positions, head_dim / 2] on the cache's device")
-        self._rope.cos, self._rope.sin, self._rope.rows = cos.data_ptr(), sin.data_ptr(), cos.shape[0]
-        return self._rope_ref
+        shape = cos.shape
+        if (len(shape) != 2 or shape[1] * 2 != cache.head_dim or sin.shape != shape or
+                cos.dtype is not torch.float32 or sin.dtype is not torch.float32 or
+                not cos.is_contiguous() or not sin.is_contiguous() or
+                cos.get_device() != cache.index or sin.get_device() != cache.index):
+            raise ValueError("RoPE tables must be dense f32 [positions, head_dim / 2] on the "
+                             "cache's device")
+        return C.byref(RopeDescriptor(cos.data_ptr(), sin.data_ptr(), shape[0]))
 
 
 def _rows(t, batch: PagedBatch, cache: PagedCache, heads: int, name: str) -> int:
     """Checks a [tokens, heads, head_dim] tensor; its row stride."""
     dim = cache.head_dim
-    _need(t.shape == (batch.tokens, heads, dim), f"{name} must be [tokens, heads, head_dim]")
-    _need(t.dtype is cache.dtype and t.device == cache.device,
-          f"{name} must have the cache's type and device")
+    if t.shape != (batch.tokens, heads, dim):
+        raise ValueError(f"{name} must be [tokens, heads, head_dim]")
+    if t.dtype is not cache.dtype or t.get_device() != cache.index:
+        raise ValueError(f"{name} must have the cache's type and device")
     row, head, last = t.stride()
-    _need(last == 1 and (head == dim or heads == 1), f"the heads of {name} must be dense")
+    if last != 1 or (head != dim and heads != 1):
+        raise ValueError(f"the heads of {name} must be dense")
     return row if batch.tokens > 1 else max(row, heads * dim)
 
 

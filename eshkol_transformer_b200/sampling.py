@@ -6,7 +6,7 @@ import ctypes as C
 import torch
 
 from . import _check, k1, load
-from .paged import DTYPES, _need
+from .paged import DTYPES
 
 
 class SamplingDescriptor(C.Structure):
@@ -24,15 +24,14 @@ class Sampler:
 
     def __init__(self, rows: int, vocabulary: int):
         self.lib = load()
-        self.rows, self.vocabulary = rows, vocabulary
-        self.descriptor = SamplingDescriptor(C.sizeof(SamplingDescriptor), rows, vocabulary)
-        self._ref = C.byref(self.descriptor)
+        self.rows, self.vocabulary, self._shape = rows, vocabulary, (rows,)
 
     def _row_values(self, t, dtype, device, name: str):
         if t is None:
             return None
-        _need(t.shape == (self.rows,) and t.dtype is dtype and t.device == device and
-              t.is_contiguous(), f"{name} must be a dense {dtype} [rows] tensor on the logits' device")
+        if (t.shape != self._shape or t.dtype is not dtype or t.get_device() != device or
+                not t.is_contiguous()):
+            raise ValueError(f"{name} must be a dense {dtype} [rows] tensor on the logits' device")
         return t.data_ptr()
 
     def sample(self, logits, uniform, ids, logprobs=None, temperature=None, top_k=None, top_p=None,
@@ -41,23 +40,26 @@ class Sampler:
         drawn tokens and their log-probabilities; uniform f32 [rows] in
         [0, 1); temperature, top_p, min_p f32 [rows], top_k i64 [rows], or
         None."""
-        d, device = self.descriptor, logits.device
-        _need(logits.is_cuda and torch.cuda.current_device() == device.index,
-              "the logits must be on the current CUDA device")
-        _need(logits.shape == (self.rows, self.vocabulary) and logits.dtype in DTYPES and
-              (logits.stride(1) == 1 or self.vocabulary == 1),
-              "logits must be [rows, vocabulary] in f32, f16 or bf16 with dense rows")
-        d.row_stride = logits.stride(0) if self.rows > 1 else self.vocabulary
-        d.dtype = DTYPES[logits.dtype]
-        d.temperature = self._row_values(temperature, torch.float32, device, "temperature")
-        d.top_k = self._row_values(top_k, torch.int64, device, "top_k")
-        d.top_p = self._row_values(top_p, torch.float32, device, "top_p")
-        d.min_p = self._row_values(min_p, torch.float32, device, "min_p")
+        device = logits.get_device()
+        if device < 0 or torch.cuda.current_device() != device:
+            raise ValueError("the logits must be on the current CUDA device")
+        if (logits.shape != (self.rows, self.vocabulary) or logits.dtype not in DTYPES or
+                (logits.stride(1) != 1 and self.vocabulary != 1)):
+            raise ValueError("logits must be [rows, vocabulary] in f32, f16 or bf16 with dense rows")
+        if uniform is None or ids is None:
+            raise ValueError("uniform and ids are required")
+        f32 = torch.float32
+        d = SamplingDescriptor(
+            C.sizeof(SamplingDescriptor), self.rows, self.vocabulary,
+            logits.stride(0) if self.rows > 1 else self.vocabulary, DTYPES[logits.dtype], 0,
+            self._row_values(temperature, f32, device, "temperature"),
+            self._row_values(top_k, torch.int64, device, "top_k"),
+            self._row_values(top_p, f32, device, "top_p"),
+            self._row_values(min_p, f32, device, "min_p"))
         err = k1.KernelError()
-        _need(uniform is not None and ids is not None, "uniform and ids are required")
-        _check(self.lib.et_b200_sample_v1(
-            self._ref, logits.data_ptr(),
-            self._row_values(uniform, torch.float32, device, "uniform"),
+        rc = self.lib.et_b200_sample_v1(
+            C.byref(d), logits.data_ptr(), self._row_values(uniform, f32, device, "uniform"),
             self._row_values(ids, torch.int64, device, "ids"),
-            self._row_values(logprobs, torch.float32, device, "logprobs"), stream, C.byref(err)),
-            err)
+            self._row_values(logprobs, f32, device, "logprobs"), stream, C.byref(err))
+        if rc != 0:
+            _check(rc, err)

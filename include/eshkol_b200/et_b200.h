@@ -265,7 +265,7 @@ int32_t et_b200_paged_attention_v1(const et_b200_paged_cache_v1 *cache,
  *                       left ranked before them;
  *   min_p  (<= 0: off)  w >= min_p (w of the most likely token is 1).
  * temperature NULL means 1; a row whose temperature is not above 2^-100 takes
- * the most likely token, with log-probability 0.  Weights are 2^-40 fixed
+ * the most likely token, with log-probability 0.  Weights are 2^-35 fixed
  * point, so results depend on no order of summation.  -inf and NaN logits are
  * never drawn; a row without others gets id -1 and log-probability -inf;
  * +inf logits share all weight.  vocabulary <= 2^22.  uniform is meant in
