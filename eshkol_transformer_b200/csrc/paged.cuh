@@ -15,9 +15,28 @@ namespace paged {
 template <typename I> ETB_HD I least_of(I a, I b) { return a < b ? a : b; }
 template <typename I> ETB_HD I most_of(I a, I b) { return a > b ? a : b; }
 
+// Division by a fixed d: for 0 <= n < 2^31, n / d = n m >> (31 + l) with l =
+// ceil(log2 d) and m = ceil(2^(31 + l) / d) (Granlund & Montgomery, 1994: m
+// exceeds 2^(31 + l) / d by less than 2^l / d, which n < 2^31 cannot carry
+// into the quotient).
+struct Divisor {
+  uint32_t d, m;
+  int shift;  // l - 1, of the product's upper half
+};
+inline Divisor divisor_of(uint32_t d) {
+  int l = 0;
+  while (((uint64_t)1 << l) < d) l++;
+  if (l == 0) return Divisor{1, 0, 0};
+  return Divisor{d, (uint32_t)((((uint64_t)1 << (31 + l)) + d - 1) / d), l - 1};
+}
+ETB_HD int quotient(int n, const Divisor& v) {
+  return v.m == 0 ? n : (int)((uint32_t)(((uint64_t)(uint32_t)n * v.m) >> 32) >> v.shift);
+}
+
 struct Pools {
   int64_t pages, page_stride, head_stride, token_stride;
   int page_size, kv_heads, head_dim;
+  Divisor by_page;
 };
 struct Batch {
   const int64_t* offsets;
@@ -58,7 +77,7 @@ ETB_HD Request load_request(const Batch& B, int b) {
 // in the pools for head h; -1 for a page outside the pool.
 ETB_HD int64_t key_offset(const Pools& P, const Batch& B, int b, int h,
                                               int key) {
-  const int column = key / P.page_size, slot = key - column * P.page_size;
+  const int column = quotient(key, P.by_page), slot = key - column * P.page_size;
   const int64_t page = B.table[(int64_t)b * B.columns + column];
   if (page < 0 || page >= P.pages) return -1;
   return page * P.page_stride + h * P.head_stride + slot * P.token_stride;
@@ -101,24 +120,29 @@ __device__ __forceinline__ int64_t rope_row(const Rope& R, int64_t pos, int* sta
 //
 // The rows of one (request, kv head) are its new tokens times the group of
 // query heads, token-major (row r: token r / group, head r % group), cut into
-// tiles of `rows`; a tile walks the keys its last token sees in blocks of
-// `keys`.  A unit is one (tile, block); the units of all requests, ordered by
+// tiles of 2^row_bits; a tile walks the keys its last token sees in blocks of
+// 2^key_bits.  A unit is one (tile, block); the units of all requests, ordered by
 // request, head, tile, block, are divided evenly among the thread blocks
 // whatever the lengths are.  A tile cut by such a border leaves partial sums,
 // which a second kernel joins.
+// Rows and keys are powers of two; tokens times group stay below 2^31.
 struct Tiling {
-  int rows, keys, group, kv_heads;
+  int row_bits, key_bits, group, kv_heads;
+  Divisor by_group;
 };
+inline Tiling tiling_of(int row_bits, int key_bits, int group, int kv_heads) {
+  return Tiling{row_bits, key_bits, group, kv_heads, divisor_of((uint32_t)group)};
+}
 ETB_HD int tile_count(const Tiling& t, const Request& r) {
-  return (int)(((int64_t)r.n * t.group + t.rows - 1) / t.rows);
+  return (r.n * t.group + (1 << t.row_bits) - 1) >> t.row_bits;
 }
 // Keys that the last row of a tile sees (0 when it stands before position 0).
 ETB_HD int tile_visible(const Tiling& t, const Request& r, int tile) {
-  const int64_t last = least_of((int64_t)(tile + 1) * t.rows, (int64_t)r.n * t.group) - 1;
-  return most_of(0, r.len - r.n + (int)(last / t.group) + 1);
+  const int last = least_of((tile + 1) << t.row_bits, r.n * t.group) - 1;
+  return most_of(0, r.len - r.n + quotient(last, t.by_group) + 1);
 }
 ETB_HD int tile_units(const Tiling& t, const Request& r, int tile) {
-  return most_of(1, (tile_visible(t, r, tile) + t.keys - 1) / t.keys);
+  return most_of(1, (tile_visible(t, r, tile) + (1 << t.key_bits) - 1) >> t.key_bits);
 }
 ETB_HD int64_t head_units(const Tiling& t, const Request& r) {
   const int tiles = tile_count(t, r);
@@ -197,7 +221,9 @@ __device__ Share divide(const Tiling& t, const Batch& B, int64_t least, Place& p
     total += all;
   }
   Share s;
-  s.per = max(least, (total + gridDim.x - 1) / gridDim.x);
+  s.per = max(least, total < INT32_MAX - (int)gridDim.x
+                         ? (int64_t)(((uint32_t)total + gridDim.x - 1) / gridDim.x)
+                         : (total + gridDim.x - 1) / gridDim.x);
   const int64_t u0 = (int64_t)blockIdx.x * s.per;
   s.units = max((int64_t)0, min(total - u0, s.per));
   p.b = B.batch;
@@ -225,8 +251,8 @@ __device__ Share divide(const Tiling& t, const Batch& B, int64_t least, Place& p
   p.r = load_request(B, p.b);
   p.tiles = tile_count(t, p.r);
   const int64_t each = head_units(t, p.r);
-  p.h = (int)(rest / each);
-  rest -= p.h * each;
+  p.h = 0;
+  for (; rest >= each; rest -= each) p.h++;
   p.tile = 0;
   enter_tile(t, p);
   while (rest >= p.nblk) {

@@ -117,10 +117,15 @@ struct Shape {
   static constexpr int NT = 32 * WM * WK, BM = 16 * WM, KW = BK / WK;
   static constexpr int ROW = DH * (int)sizeof(T), PIECES = ROW / 16;  // of one key
   static constexpr int TILE = BK * ROW, STAGE = 2 * TILE;
-  static constexpr int Q_BYTES = BM * ROW;
+  static constexpr int TILE_Q = BM * ROW;
+  static constexpr int Q_BYTES = TILE_Q * (sizeof(T) == 4 ? 1 : 2);  // f16, bf16: with their residuals
   static constexpr int MERGE = (WK - 1) * BM * DH * 4;
+  static constexpr int RING = STAGES + 1;  // blocks with known key addresses
   static constexpr int KOFF = STAGES * STAGE + Q_BYTES;
-  static constexpr int SMEM = KOFF + 2 * BK * 8 + WK * BM * 8;
+  static constexpr int JOIN = KOFF + RING * BK * 8;
+  static constexpr int SMEM = JOIN + WK * BM * 8;
+  static constexpr int bits(int n) { return n <= 1 ? 0 : 1 + bits(n / 2); }
+  static_assert(1 << bits(BM) == BM && 1 << bits(BK) == BK, "powers of two");
   static_assert(KW % 16 == 0 && BK <= NT * 2, "keys per warp");
   static_assert(MERGE <= STAGE, "the joining of warps reuses a stage");
   static_assert(SMEM <= 232448, "shared memory");
@@ -139,7 +144,7 @@ paged_attention_kernel(AttendArgs a) {
   constexpr int KSTEP = F32 ? 8 : 16;  // dims (or keys) per matrix instruction
   extern __shared__ __align__(128) uint8_t smem[];
   int64_t* koff = reinterpret_cast<int64_t*>(smem + S::KOFF);
-  float* join_m = reinterpret_cast<float*>(smem + S::KOFF + 2 * BK * 8);
+  float* join_m = reinterpret_cast<float*>(smem + S::JOIN);
   float* join_l = join_m + WK * BM;
   const uint32_t base = smem_u32(smem);
   const uint32_t qs = base + S::STAGES * S::STAGE;
@@ -158,7 +163,7 @@ paged_attention_kernel(AttendArgs a) {
     const int units = (int)share.units;
     Place kp = p;        // the block whose key addresses are looked up next
     int looked = 0;
-    auto look_up = [&]() {  // addresses of block `looked` into slot looked & 1
+    auto look_up = [&]() {  // addresses of block `looked` into slot looked % RING
       if (looked < units) {
         const int visible = tile_visible(a.tiling, kp.r, kp.tile);
         for (int i = tid; i < BK; i += NT) {
@@ -168,7 +173,7 @@ paged_attention_kernel(AttendArgs a) {
             off = key_offset(a.pools, a.batch, kp.b, kp.h, key);
             if (off < 0) report(a.batch.status, ET_B200_PAGED_BAD_PAGE);
           }
-          koff[(looked & 1) * BK + i] = off;
+          koff[looked % S::RING * BK + i] = off;
         }
         advance(a.tiling, a.batch, kp);
       }
@@ -179,7 +184,7 @@ paged_attention_kernel(AttendArgs a) {
         const uint32_t st = base + (uint32_t)(u % S::STAGES) * S::STAGE;
         for (int i = tid; i < BK * S::PIECES; i += NT) {
           const int row = i / S::PIECES, c = i % S::PIECES;
-          const int64_t off = koff[(u & 1) * BK + row];
+          const int64_t off = koff[u % S::RING * BK + row];
           const bool full = off >= 0 && c * (16 / (int)sizeof(T)) < dim;
           const int64_t e = full ? off + c * (16 / (int)sizeof(T)) : 0;
           const uint32_t dst = st + S::at(row, c);
@@ -189,14 +194,42 @@ paged_attention_kernel(AttendArgs a) {
       }
       cp_commit();
     };
-    look_up();
+#pragma unroll
+    for (int s = 0; s < S::STAGES; s++) look_up();
     __syncthreads();
 #pragma unroll
-    for (int s = 0; s < S::STAGES - 1; s++) {
-      issue(s);
-      look_up();
-      __syncthreads();
-    }
+    for (int s = 0; s < S::STAGES - 1; s++) issue(s);
+
+    auto load_queries = [&]() {  // the rows of the tile at p, rotated
+      const int first_row = p.tile << a.tiling.row_bits, rows = min(BM, p.r.n * group - first_row);
+#pragma unroll 4
+      for (int i = tid; i < BM * DH / 2; i += NT) {
+        const int r = i / (DH / 2), d = 2 * (i % (DH / 2));
+        float x0 = 0.0f, x1 = 0.0f;
+        if (r < rows && d < dim) {
+          const int t = quotient(first_row + r, a.tiling.by_group), j = first_row + r - t * group;
+          const T* src = static_cast<const T*>(a.q) + (p.r.first + t) * a.q_stride +
+                         (int64_t)(p.h * group + j) * dim + d;
+          x0 = to_f32<T>(src[0]);
+          x1 = to_f32<T>(src[1]);
+          const int pos = p.r.len - p.r.n + t;
+          if (a.rope.cos != nullptr && pos >= 0) {
+            const int64_t at = rope_row(a.rope, pos, a.batch.status) * (dim / 2) + d / 2;
+            rotate(x0, x1, __ldg(a.rope.cos + at), __ldg(a.rope.sin + at));
+          }
+        }
+        const uint32_t at = S::at(r, d * (int)sizeof(T) / 16) + (d * (int)sizeof(T)) % 16;
+        T* dst = reinterpret_cast<T*>(smem + S::STAGES * S::STAGE + at);
+        dst[0] = from_f32<T>(x0);
+        dst[1] = from_f32<T>(x1);
+        if constexpr (!F32) {  // and what the rounding left
+          T* low = reinterpret_cast<T*>(smem + S::STAGES * S::STAGE + S::TILE_Q + at);
+          low[0] = from_f32<T>(x0 - to_f32<T>(dst[0]));
+          low[1] = from_f32<T>(x1 - to_f32<T>(dst[1]));
+        }
+      }
+    };
+    load_queries();
 
     float o[DH / 8][4];
     float m[2], l[2];
@@ -208,42 +241,23 @@ paged_attention_kernel(AttendArgs a) {
       issue(u + S::STAGES - 1);
       look_up();
       const bool first = u == 0 || p.blk == 0;
-      if (first) {  // a new tile: its queries, rotated
+      if (first) {  // a new tile
         whole = p.blk == 0;
-        const int rows = (int)min((int64_t)BM, (int64_t)p.r.n * group - (int64_t)p.tile * BM);
-        for (int i = tid; i < BM * DH / 2; i += NT) {
-          const int r = i / (DH / 2), d = 2 * (i % (DH / 2));
-          float x0 = 0.0f, x1 = 0.0f;
-          if (r < rows && d < dim) {
-            const int64_t g = (int64_t)p.tile * BM + r;
-            const int t = (int)(g / group), j = (int)(g % group);
-            const T* src = static_cast<const T*>(a.q) + (p.r.first + t) * a.q_stride +
-                           (int64_t)(p.h * group + j) * dim + d;
-            x0 = to_f32<T>(src[0]);
-            x1 = to_f32<T>(src[1]);
-            const int pos = p.r.len - p.r.n + t;
-            if (a.rope.cos != nullptr && pos >= 0) {
-              const int64_t at = rope_row(a.rope, pos, a.batch.status) * (dim / 2) + d / 2;
-              rotate(x0, x1, a.rope.cos[at], a.rope.sin[at]);
-            }
-          }
-          T* dst = reinterpret_cast<T*>(smem + S::STAGES * S::STAGE + S::at(r, d * (int)sizeof(T) / 16)) +
-                   d % (16 / (int)sizeof(T));
-          dst[0] = from_f32<T>(x0);
-          dst[1] = from_f32<T>(x1);
-        }
+        const int rows = min(BM, p.r.n * group - (p.tile << a.tiling.row_bits));
+        if (u > 0) load_queries();
 #pragma unroll
         for (int i = 0; i < DH / 8; i++) o[i][0] = o[i][1] = o[i][2] = o[i][3] = 0.0f;
 #pragma unroll
         for (int i = 0; i < 2; i++) {
           m[i] = -INFINITY;
           l[i] = 0.0f;
-          const int r = wm * 16 + lane / 4 + 8 * i;
-          const int64_t g = (int64_t)p.tile * BM + r;
-          vis[i] = r < rows ? max(0, p.r.len - p.r.n + (int)(g / group) + 1) : 0;
+          const int r = wm * 16 + lane / 4 + 8 * i, g = (p.tile << a.tiling.row_bits) + r;
+          vis[i] = r < rows ? max(0, p.r.len - p.r.n + quotient(g, a.tiling.by_group) + 1) : 0;
         }
-        vis_min = rows == BM ? max(0, p.r.len - p.r.n + (int)((int64_t)p.tile * BM / group) + 1) : 0;
-        __syncthreads();
+        vis_min = rows == BM ? max(0, p.r.len - p.r.n +
+                                          quotient(p.tile << a.tiling.row_bits, a.tiling.by_group) + 1)
+                             : 0;
+        if (u > 0) __syncthreads();
       }
       const uint32_t kt = base + (uint32_t)(u % S::STAGES) * S::STAGE, vt = kt + S::TILE;
 
@@ -259,6 +273,8 @@ paged_attention_kernel(AttendArgs a) {
         if constexpr (F32) {
 #pragma unroll
           for (int i = 0; i < 4; i++) pair_tf32(qa[i], qh[i], ql[i]);
+        } else {
+          ldsm4(ql, qs + S::TILE_Q + S::at(wm * 16 + (lane & 15), 2 * ks + (lane >> 4)));
         }
 #pragma unroll
         for (int n = 0; n < KW / 16; n++) {
@@ -276,6 +292,8 @@ paged_attention_kernel(AttendArgs a) {
               mma_tf32(s[2 * n + i], qh, kh[2 * i], kh[2 * i + 1]);
             }
           } else {
+            mma16<T>(s[2 * n], ql, kb[0], kb[1]);
+            mma16<T>(s[2 * n + 1], ql, kb[2], kb[3]);
             mma16<T>(s[2 * n], qa, kb[0], kb[1]);
             mma16<T>(s[2 * n + 1], qa, kb[2], kb[3]);
           }
@@ -338,9 +356,13 @@ paged_attention_kernel(AttendArgs a) {
 #pragma unroll
             for (int i = 0; i < 2; i++)
               pair_tf32(lds32(vt + S::at(row + i, d / 4) + 4 * (d & 3)), vh[i], vl[i]);
-            mma_tf32(o[n], pl, vh[0], vh[1]);
-            mma_tf32(o[n], ph, vl[0], vl[1]);
-            mma_tf32(o[n], ph, vh[0], vh[1]);
+            // the tensor pipe's accumulation truncates: eight keys at a time, added in f32
+            float part[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+            mma_tf32(part, pl, vh[0], vh[1]);
+            mma_tf32(part, ph, vl[0], vl[1]);
+            mma_tf32(part, ph, vh[0], vh[1]);
+#pragma unroll
+            for (int i = 0; i < 4; i++) o[n][i] += part[i];
           }
         }
       } else {
@@ -423,12 +445,11 @@ paged_attention_kernel(AttendArgs a) {
           const int slot = 2 * (int)blockIdx.x + (whole ? 1 : 0);
 #pragma unroll
           for (int i = 0; i < 2; i++) {
-            const int r = r0 + 8 * i;
-            const int64_t g = (int64_t)p.tile * BM + r;
+            const int r = r0 + 8 * i, g = (p.tile << a.tiling.row_bits) + r;
             if (done) {
-              if (g < (int64_t)p.r.n * group) {
-                const int64_t t = p.r.first + g / group;
-                const int h = p.h * group + (int)(g % group);
+              if (g < p.r.n * group) {
+                const int by = quotient(g, a.tiling.by_group), h = p.h * group + g - by * group;
+                const int64_t t = p.r.first + by;
                 const float inv = l[i] > 0.0f ? 1.0f / l[i] : 0.0f;
                 T* dst = static_cast<T*>(a.o) + t * a.o_stride + (int64_t)h * dim;
 #pragma unroll
@@ -465,40 +486,67 @@ paged_attention_kernel(AttendArgs a) {
 }
 
 // Joins the parts of the tile that thread block blockIdx.x of the attention
-// began and did not finish; blockIdx.y takes rows y, y + gridDim.y, ...
-template <typename T>
-__global__ void __launch_bounds__(128) paged_join_kernel(AttendArgs a, int dim_padded) {
+// began and did not finish; blockIdx.y takes rows y, y + gridDim.y, ...  The
+// warps take parts w, w + 8, ... of a row, 4 dims per lane, several parts' loads
+// in flight; shared memory adds the warps up in order.
+constexpr int JOIN_WARPS = 8;
+template <typename T, int DH>
+__global__ void __launch_bounds__(32 * JOIN_WARPS) paged_join_kernel(AttendArgs a) {
+  constexpr int V = DH >= 128 ? DH / 32 : 4, LANES = DH / V;  // dims per lane, lanes used
+  __shared__ float sums[JOIN_WARPS][DH];
+  __shared__ float totals[JOIN_WARPS];
   asm volatile("griddepcontrol.wait;" ::: "memory");
-  const int c = blockIdx.x, rows = a.tiling.rows, group = a.tiling.group;
+  const int c = blockIdx.x, rows = 1 << a.tiling.row_bits, group = a.tiling.group;
   const Cut cut = a.joint.cuts[c];
   if (cut.parts == 0) return;
-  const int dim = a.pools.head_dim;
+  const int dim = a.pools.head_dim, lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   auto slot_of = [&](int part) { return part == 0 ? 2 * c + 1 : 2 * (c + part); };
   for (int r = blockIdx.y; r < rows; r += gridDim.y) {
-    const int64_t g = (int64_t)cut.tile * rows + r;
-    if (g >= (int64_t)cut.n * group) return;
+    const int g = (cut.tile << a.tiling.row_bits) + r;
+    if (g >= cut.n * group) return;
     float m = -INFINITY;
-    for (int i = 0; i < cut.parts; i++)
+    for (int i = lane; i < cut.parts; i += 32)
       m = fmaxf(m, a.joint.stats[(int64_t)slot_of(i) * 2 * rows + r]);
+    m = warp_max(m);
     const float ref = m == -INFINITY ? 0.0f : m;
-    float l = 0.0f, x0 = 0.0f, x1 = 0.0f;
-    const int d = 2 * threadIdx.x;
-    for (int i = 0; i < cut.parts; i++) {
+    float l = 0.0f, x[V];
+#pragma unroll
+    for (int k = 0; k < V; k++) x[k] = 0.0f;
+#pragma unroll 4
+    for (int i = warp; i < cut.parts; i += JOIN_WARPS) {
       const int64_t s = slot_of(i);
       const float f = ex2(a.joint.stats[s * 2 * rows + r] - ref);
       l += f * a.joint.stats[(s * 2 + 1) * rows + r];
-      if (d < dim) {
-        const float2 x = *reinterpret_cast<const float2*>(a.joint.sums + (s * rows + r) * dim_padded + d);
-        x0 += f * x.x;
-        x1 += f * x.y;
+      if (lane < LANES) {
+        const float* src = a.joint.sums + (s * rows + r) * DH + lane * V;
+#pragma unroll
+        for (int k = 0; k < V; k += 4) {
+          const float4 y = *reinterpret_cast<const float4*>(src + k);
+          x[k] += f * y.x; x[k + 1] += f * y.y; x[k + 2] += f * y.z; x[k + 3] += f * y.w;
+        }
       }
     }
-    const int64_t t = cut.first + g / group;
-    const int h = cut.h * group + (int)(g % group);
-    const float inv = l > 0.0f ? 1.0f / l : 0.0f;
-    if (d < dim) store2<T>(static_cast<T*>(a.o) + t * a.o_stride + (int64_t)h * dim + d, x0 * inv, x1 * inv);
-    if (a.lse != nullptr && threadIdx.x == 0)
-      a.lse[t * a.q_heads + h] = l > 0.0f ? m * kLn2 + logf(l) : -INFINITY;
+    if (lane < LANES)
+#pragma unroll
+      for (int k = 0; k < V; k++) sums[warp][lane * V + k] = x[k];
+    if (lane == 0) totals[warp] = l;
+    __syncthreads();
+    const int d = 2 * threadIdx.x, by = quotient(g, a.tiling.by_group), h = cut.h * group + g - by * group;
+    const int64_t t = cut.first + by;
+    if (d < dim || threadIdx.x == 0) {
+      float total = 0.0f, y0 = 0.0f, y1 = 0.0f;
+#pragma unroll
+      for (int w = 0; w < JOIN_WARPS; w++) {
+        total += totals[w];
+        y0 += sums[w][d];
+        y1 += sums[w][d + 1];
+      }
+      const float inv = total > 0.0f ? 1.0f / total : 0.0f;
+      store2<T>(static_cast<T*>(a.o) + t * a.o_stride + (int64_t)h * dim + d, y0 * inv, y1 * inv);
+      if (a.lse != nullptr && threadIdx.x == 0)
+        a.lse[t * a.q_heads + h] = total > 0.0f ? m * kLn2 + logf(total) : -INFINITY;
+    }
+    __syncthreads();
   }
 }
 
@@ -528,31 +576,32 @@ int resident_blocks(int threads, int smem) {
   return n;
 }
 
-template <typename T>
-void launch_join(const AttendArgs& a, int blocks, int dim_padded, cudaStream_t stream) {
+template <typename T, int DH>
+void launch_join(const AttendArgs& a, int blocks, cudaStream_t stream) {
   cudaLaunchConfig_t cfg{};
-  cfg.gridDim = dim3(blocks, 16);
-  cfg.blockDim = dim3(128);
+  // a row per thread block up to 16 rows
+  const int rows = 1 << a.tiling.row_bits;
+  cfg.gridDim = dim3(blocks, rows < 16 ? rows : 16);
+  cfg.blockDim = dim3(32 * JOIN_WARPS);
   cfg.stream = stream;
   cudaLaunchAttribute attr{};
   attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
   attr.val.programmaticStreamSerializationAllowed = 1;
   cfg.attrs = &attr;
   cfg.numAttrs = 1;
-  cudaLaunchKernelEx(&cfg, paged_join_kernel<T>, a, dim_padded);
+  cudaLaunchKernelEx(&cfg, paged_join_kernel<T, DH>, a);
   count_launch();
 }
 
 template <typename T, typename S>
 void launch_shape(AttendArgs& a, void* ws, cudaStream_t stream) {
   const int blocks = resident_blocks<paged_attention_kernel<T, S>>(S::NT, S::SMEM) * sm_count();
-  a.tiling.rows = S::BM;
-  a.tiling.keys = S::BK;
-  a.least = 4;
+  a.tiling = tiling_of(S::bits(S::BM), S::bits(S::BK), a.tiling.group, a.pools.kv_heads);
+  a.least = 1;
   a.joint = joint_of(ws, blocks, S::BM, S::DH);
   paged_attention_kernel<T, S><<<blocks, S::NT, S::SMEM, stream>>>(a);
   count_launch();
-  launch_join<T>(a, blocks, S::DH, stream);
+  launch_join<T, S::DH>(a, blocks, stream);
 }
 
 template <typename T, int DH>
@@ -575,7 +624,8 @@ void launch_type(const et_b200_paged_cache_v1* c, AttendArgs& a, int64_t max_new
   if constexpr (sizeof(T) == 2) {
     if (max_new * a.tiling.group > 16) {
       if (const int blocks = attend_tc(c, a, ws, stream))
-        return launch_join<T>(a, blocks, c->head_dim <= 64 ? 64 : 128, stream);
+        return c->head_dim <= 64 ? launch_join<T, 64>(a, blocks, stream)
+                                 : launch_join<T, 128>(a, blocks, stream);
     }
   }
   switch (padded(a.pools.head_dim)) {
@@ -629,6 +679,9 @@ int32_t et_b200_paged_attention_v1(const et_b200_paged_cache_v1* c,
     if ((reinterpret_cast<uintptr_t>(q) | reinterpret_cast<uintptr_t>(o)) % size != 0)
       return set_error(e, ET_KERNEL_ERROR_INVALID_ARGUMENT, ET_KERNEL_CODE_INVALID_BUFFER, op,
                        "q and o must be aligned to their elements");
+    if (b->tokens * q_heads > INT32_MAX)
+      return set_error(e, ET_KERNEL_ERROR_SHAPE_MISMATCH, ET_KERNEL_CODE_INVALID_SHAPE, op,
+                       "tokens times q_heads must stay below 2^31");
     if (workspace == nullptr || (reinterpret_cast<uintptr_t>(workspace) & 255) != 0 ||
         workspace_bytes < et_b200_paged_attention_workspace_bytes_v1(c, q_heads))
       return set_error(e, ET_KERNEL_ERROR_INVALID_ARGUMENT, ET_KERNEL_CODE_BUFFER_TOO_SMALL, op,
@@ -639,7 +692,6 @@ int32_t et_b200_paged_attention_v1(const et_b200_paged_cache_v1* c,
     a.batch = batch_of(b, c);
     a.rope = rope_of(rope);
     a.tiling.group = (int)(q_heads / c->kv_heads);
-    a.tiling.kv_heads = (int)c->kv_heads;
     a.keys = c->keys;
     a.values = c->values;
     a.q = q;

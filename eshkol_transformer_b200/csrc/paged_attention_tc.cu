@@ -108,7 +108,7 @@ paged_attention_tc_kernel(const __grid_constant__ CUtensorMap k_map,
   int64_t left = share.units;
   auto blocks_here = [&]() { return (int)min((int64_t)(p.nblk - p.blk), left); };
   auto rows_here = [&]() {
-    return (int)min((int64_t)(2 * HALF), (int64_t)p.r.n * group - (int64_t)p.tile * 2 * HALF);
+    return min(2 * HALF, p.r.n * group - p.tile * 2 * HALF);
   };
   auto next_tile = [&](int done) {
     left -= done;
@@ -135,7 +135,7 @@ paged_attention_tc_kernel(const __grid_constant__ CUtensorMap k_map,
         const int mine = lane % 16;
         int page = -1, slot = 0;
         if (mine < boxes) {
-          const int key = key0 + mine * box_rows, column = key / a.pools.page_size;
+          const int key = key0 + mine * box_rows, column = quotient(key, a.pools.by_page);
           slot = key - column * a.pools.page_size;
           page = a.batch.table[(int64_t)p.b * a.batch.columns + column];
           if (page < 0 || page >= a.pools.pages) {
@@ -262,9 +262,9 @@ paged_attention_tc_kernel(const __grid_constant__ CUtensorMap k_map,
         cut = Cut{p.r.first, p.r.n, p.h, p.tile, 1 + (int)((rest + share.per - 1) / share.per)};
       }
       if (rows > 0) {
-        const int64_t g = (int64_t)p.tile * 2 * HALF + HALF * t + row;
+        const int g = p.tile * 2 * HALF + HALF * t + row;
         const bool valid = row < rows;
-        const int token = (int)(g / group), head = p.h * group + (int)(g % group);
+        const int token = quotient(g, a.tiling.by_group), head = p.h * group + g - token * group;
         const int pos = p.r.len - p.r.n + token;
         const int vis = valid ? max(0, pos + 1) : 0;
         // keys that every row of this warp sees (invalid rows follow the last valid one)
@@ -451,8 +451,8 @@ int launch_tc(const et_b200_paged_cache_v1* c, AttendArgs& a, void* ws, cudaStre
   CUtensorMap k_map, v_map;
   if (!pool_map(&k_map, c->keys, c, box_rows) || !pool_map(&v_map, c->values, c, box_rows)) return 0;
   const int blocks = sm_count();
-  a.tiling.rows = 2 * HALF;
-  a.tiling.keys = BK;
+  a.tiling = tiling_of(8, 7, a.tiling.group, a.pools.kv_heads);
+  static_assert(2 * HALF == 1 << 8 && BK == 1 << 7, "tiling");
   a.least = 2;
   a.joint = joint_of(ws, blocks, 2 * HALF, DH);
   cudaFuncSetAttribute(paged_attention_tc_kernel<T, DH>,

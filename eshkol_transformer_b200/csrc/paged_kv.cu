@@ -185,7 +185,7 @@ int32_t check_rope(const et_b200_paged_rope_v1* r, et_kernel_error* e, const cha
 
 Pools pools_of(const et_b200_paged_cache_v1* c) {
   return Pools{c->pages, c->page_stride, c->head_stride, c->token_stride, (int)c->page_size,
-               (int)c->kv_heads, (int)c->head_dim};
+               (int)c->kv_heads, (int)c->head_dim, divisor_of((uint32_t)c->page_size)};
 }
 Batch batch_of(const et_b200_paged_batch_v1* b, const et_b200_paged_cache_v1* c) {
   return Batch{b->offsets, b->lengths, b->page_table, b->status, b->tokens, b->table_columns,

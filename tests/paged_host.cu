@@ -35,9 +35,18 @@ int main() {
   CHECK(load_request(B, 5).bad == (ET_B200_PAGED_BAD_OFFSET | ET_B200_PAGED_BAD_LENGTH));
   CHECK(load_request(B, 6).bad == (ET_B200_PAGED_BAD_OFFSET | ET_B200_PAGED_BAD_LENGTH));
 
+  for (uint32_t d : {1u, 2u, 3u, 7u, 16u, 24u, 1000u, 65536u, (1u << 20) - 1, 1u << 20}) {
+    const Divisor v = divisor_of(d);
+    for (int64_t n = 0; n < (1ll << 31); n += 1 + n / 50) CHECK(quotient((int)n, v) == (int)(n / d));
+    for (int64_t k = 1; k * d < (1ll << 31); k += 1 + k / 20)
+      CHECK(quotient((int)(k * d), v) == k && quotient((int)(k * d) - 1, v) == k - 1);
+    CHECK(quotient(INT32_MAX, v) == (int)(INT32_MAX / d));
+  }
+
   Pools P{};
   P.pages = 10;
   P.page_size = 10;
+  P.by_page = divisor_of(10);
   P.kv_heads = 2;
   P.head_dim = 8;
   P.token_stride = 8;
@@ -70,8 +79,9 @@ int main() {
   W.batch = 7;
   W.capacity = 4096;
   for (int group : {1, 3, 8})
-    for (int rows : {16, 64, 128}) {
-      const Tiling t{rows, 64, group, 2};
+    for (int bits : {4, 6, 8}) {
+      const int rows = 1 << bits;
+      const Tiling t = tiling_of(bits, 6, group, 2);
       int64_t total = 0;
       for (int b = 0; b < 7; b++) total += head_units(t, load_request(W, b)) * 2;
       Place p{};
@@ -86,7 +96,7 @@ int main() {
         CHECK(p.blk == 0 || p.blk * 64 < tile_visible(t, p.r, p.tile));
         CHECK(p.blk + 1 < p.nblk || p.nblk * 64 >= tile_visible(t, p.r, p.tile));
         if (p.blk == 0)
-          rows_seen += least_of((int64_t)rows, (int64_t)p.r.n * group - (int64_t)p.tile * rows);
+          rows_seen += least_of(rows, p.r.n * group - p.tile * rows);
         CHECK(seen <= total);
       }
       CHECK(seen == total && rows_seen == 300 * group * 2);
