@@ -6,6 +6,7 @@
 #include <cuda_bf16.h>
 
 #include "ops.cuh"
+#include "tcgen05.cuh"
 
 namespace etb {
 namespace paged {
@@ -307,6 +308,23 @@ struct AttendArgs {
   int q_heads;
   float scale_log2;  // log2(e) / sqrt(head_dim)
 };
+
+// ---- TMA from the pools ---------------------------------------------------------------
+
+__device__ __forceinline__ void tma_load_4d(uint32_t dst, const CUtensorMap* map, uint32_t bar,
+                                            int x, int y, int z, int w) {
+  asm volatile(
+      "cp.async.bulk.tensor.4d.shared::cluster.global.tile.mbarrier::complete_tx::bytes"
+      " [%0], [%1, {%3, %4, %5, %6}], [%2];" ::"r"(dst),
+      "l"(reinterpret_cast<uint64_t>(map)), "r"(bar), "r"(x), "r"(y), "r"(z), "r"(w)
+      : "memory");
+}
+
+// Map of a pool for boxes of `wide` dims (64 or 128 bytes, swizzled as wide)
+// x box_rows slots of one head of one page; dims beyond head_dim and pages
+// outside the pool read as zeros.  False for pools it cannot describe (pages
+// that are no power of two of at least 8 slots, far strides).
+bool pool_map(CUtensorMap* map, void* pool, const et_b200_paged_cache_v1* c, int wide, int box_rows);
 
 // Host pieces of the entry points.
 int32_t check_cache(const et_b200_paged_cache_v1* c, et_kernel_error* e, const char* op);

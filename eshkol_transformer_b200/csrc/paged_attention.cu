@@ -5,9 +5,12 @@
 // o = sum_j p_j v_j / sum_j p_j, p_j = 2^(s_j - m), s_j = log2(e) scale q'.k_j,
 // m the running maximum.  A thread block takes its share of the (tile, block)
 // units (paged.cuh): tiles of 16 WM rows, blocks of BK keys.  K and V arrive
-// by 16-byte cp.async in a ring of STAGES blocks (rows XOR-swizzled by 16-byte
-// pieces, so ldmatrix and the f32 reads of V are free of bank conflicts); the
-// key addresses of a block are looked up one block ahead of its copies.  Warp
+// in a ring of STAGES blocks, rows XOR-swizzled by 16-byte pieces (so ldmatrix
+// and the f32 reads of V are free of bank conflicts): pages of a power of two
+// of at least 8 slots by TMA from a warp of its own, which keeps copies,
+// look-ups and block-wide barriers out of the arithmetic warps; any other page
+// size by 16-byte cp.async, the key addresses of a block looked up one block
+// ahead of its copies.  Warp
 // (wm, wk) takes 16 rows and BK / WK keys of each block with its own maxima,
 // sums and accumulators (mma.sync m16n8k16, or for f32 m16n8k8 as 3xTF32:
 // hi hi + hi lo + lo hi of operands rounded to TF32 pairs), which are joined
@@ -123,26 +126,38 @@ struct Shape {
   static constexpr int RING = STAGES + 1;  // blocks with known key addresses
   static constexpr int KOFF = STAGES * STAGE + Q_BYTES;
   static constexpr int JOIN = KOFF + RING * BK * 8;
-  static constexpr int SMEM = JOIN + WK * BM * 8;
+  static constexpr int BARS = JOIN + WK * BM * 8;
+  static constexpr int SMEM = BARS + 2 * STAGES * 8 + 16;
+  // a row in shared memory: chunks of 128 bytes (one of 64 at 4 pieces), each
+  // [BK] (or [BM]) rows with the TMA swizzle of that width
+  static constexpr int CHUNK = ROW < 128 ? ROW : 128, CHUNKS = ROW / CHUNK;
+  static constexpr int WIDE = CHUNK / (int)sizeof(T);  // elements of a chunk
+  static constexpr int PER_SM = 2 * (SMEM + 2048) <= 233472 ? 2 : 1;  // blocks the registers must allow
   static constexpr int bits(int n) { return n <= 1 ? 0 : 1 + bits(n / 2); }
   static_assert(1 << bits(BM) == BM && 1 << bits(BK) == BK, "powers of two");
   static_assert(KW % 16 == 0 && BK <= NT * 2, "keys per warp");
   static_assert(MERGE <= STAGE, "the joining of warps reuses a stage");
   static_assert(SMEM <= 232448, "shared memory");
-  // byte of 16-byte piece c of a row
+  // byte of 16-byte piece c of a row in a tile of R rows
+  template <int R>
   __device__ static uint32_t at(int row, int c) {
-    const int x = PIECES >= 8 ? (row & 7) : ((row >> 1) & 3);
-    return (uint32_t)(row * ROW + ((c ^ x) << 4));
+    if constexpr (PIECES >= 8)
+      return (uint32_t)((c >> 3) * R * 128 + row * 128 + (((c & 7) ^ (row & 7)) << 4));
+    else
+      return (uint32_t)(row * ROW + ((c ^ ((row >> 1) & 3)) << 4));
   }
 };
 
-template <typename T, typename S>
-__global__ void __launch_bounds__(S::NT)
-paged_attention_kernel(AttendArgs a) {
+__device__ int g_wait_error;  // bounded waits that gave up (the status word tells the caller)
+
+template <typename T, typename S, bool TMA>
+__global__ void __launch_bounds__(S::NT + (TMA ? 32 : 0), S::PER_SM)
+paged_attention_kernel(const __grid_constant__ CUtensorMap k_map,
+                       const __grid_constant__ CUtensorMap v_map, AttendArgs a, int box_bits) {
   constexpr int DH = S::DH, BM = S::BM, BK = S::BK, KW = S::KW, NT = S::NT, WK = S::WK;
   constexpr bool F32 = sizeof(T) == 4;
   constexpr int KSTEP = F32 ? 8 : 16;  // dims (or keys) per matrix instruction
-  extern __shared__ __align__(128) uint8_t smem[];
+  extern __shared__ __align__(1024) uint8_t smem[];
   int64_t* koff = reinterpret_cast<int64_t*>(smem + S::KOFF);
   float* join_m = reinterpret_cast<float*>(smem + S::JOIN);
   float* join_l = join_m + WK * BM;
@@ -156,8 +171,66 @@ paged_attention_kernel(AttendArgs a) {
   // lets the joining kernel start its launch; it waits for this one's results
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
 
+  // TMA: barriers of a stage (full, empty), 1 and one per arithmetic warp arrivals
+  const uint32_t bars = base + S::BARS;
+  auto full_bar = [&](int st) { return bars + 8u * (uint32_t)st; };
+  auto empty_bar = [&](int st) { return bars + 8u * (uint32_t)(S::STAGES + st); };
+  volatile int* abort = reinterpret_cast<volatile int*>(smem + S::BARS + 2 * S::STAGES * 8);
+  if (TMA && tid == 0) {
+    for (int i = 0; i < S::STAGES; i++) {
+      mbar_init(full_bar(i), 1);
+      mbar_init(empty_bar(i), NT / 32);
+    }
+    *abort = 0;
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+  }
+
   Place p;
-  const Share share = divide<NT>(a.tiling, a.batch, a.least, p);
+  const Share share = divide<NT + (TMA ? 32 : 0)>(a.tiling, a.batch, a.least, p);
+  __syncthreads();
+  if (TMA && warp == NT / 32) {
+    // ---- the copying warp
+    int fetched = 0;
+    const int per_block = BK >> box_bits, per_bits = S::bits(BK) - box_bits;
+    auto page_of = [&](const Place& k) {  // of this lane's box; -2 for none, -1 for a bad page
+      const int key = k.blk * BK + (lane << box_bits);
+      if (lane >= per_block || key >= tile_visible(a.tiling, k.r, k.tile)) return -2;
+      const int page = a.batch.table[(int64_t)k.b * a.batch.columns + quotient(key, a.pools.by_page)];
+      if (page >= 0 && page < a.pools.pages) return page;
+      report(a.batch.status, ET_B200_PAGED_BAD_PAGE);
+      return -1;  // outside the map: filled with zeros
+    };
+    int page = share.units > 0 ? page_of(p) : -2;
+    for (int u = 0; u < (int)share.units; u++) {
+      const int st = u % S::STAGES, key0 = p.blk * BK, h = p.h, now = page;
+      if (u >= S::STAGES && !__all_sync(0xffffffffu, role_wait(empty_bar(st), (uint32_t)((u / S::STAGES - 1) & 1),
+                                                               &g_wait_error, abort)))
+        break;
+      const int boxes = __popc(__ballot_sync(0xffffffffu, now != -2));
+      if (lane == 0) mbar_expect_tx(full_bar(st), (uint32_t)((boxes << box_bits) * S::ROW * 2));
+      __syncwarp();
+      const uint32_t dst = base + (uint32_t)st * S::STAGE;
+      for (int i0 = 0; i0 < per_block * S::CHUNKS * 2; i0 += 32) {
+        const int i = i0 + lane, box = i & (per_block - 1), c = i >> per_bits;  // K's chunks, then V's
+        const int from = __shfl_sync(0xffffffffu, now, box);
+        if (c < S::CHUNKS * 2 && from != -2) {
+          const int key = key0 + (box << box_bits), chunk = c % S::CHUNKS;
+          const int slot = key - quotient(key, a.pools.by_page) * a.pools.page_size;
+          tma_load_4d(dst + (uint32_t)(c / S::CHUNKS) * S::TILE + (uint32_t)chunk * BK * S::CHUNK +
+                          (uint32_t)(box << box_bits) * S::CHUNK,
+                      c < S::CHUNKS ? &k_map : &v_map, full_bar(st), chunk * S::WIDE, slot, h, from);
+        }
+        __syncwarp();
+      }
+      fetched = u + 1;
+      advance(a.tiling, a.batch, p);
+      if (u + 1 < (int)share.units) page = page_of(p);
+    }
+    // every copy has landed before the block releases its memory
+    for (int u = max(0, fetched - S::STAGES); u < fetched; u++)
+      mbar_wait(full_bar(u % S::STAGES), (uint32_t)((u / S::STAGES) & 1), &g_wait_error);
+    return;
+  }
   Cut cut{0, 0, 0, 0, 0};
   if (share.units > 0) {
     const int units = (int)share.units;
@@ -187,18 +260,20 @@ paged_attention_kernel(AttendArgs a) {
           const int64_t off = koff[u % S::RING * BK + row];
           const bool full = off >= 0 && c * (16 / (int)sizeof(T)) < dim;
           const int64_t e = full ? off + c * (16 / (int)sizeof(T)) : 0;
-          const uint32_t dst = st + S::at(row, c);
+          const uint32_t dst = st + S::template at<BK>(row, c);
           cp16(dst, keys + e, full);
           cp16(dst + S::TILE, values + e, full);
         }
       }
       cp_commit();
     };
+    if constexpr (!TMA) {
 #pragma unroll
-    for (int s = 0; s < S::STAGES; s++) look_up();
-    __syncthreads();
+      for (int s = 0; s < S::STAGES; s++) look_up();
+      __syncthreads();
 #pragma unroll
-    for (int s = 0; s < S::STAGES - 1; s++) issue(s);
+      for (int s = 0; s < S::STAGES - 1; s++) issue(s);
+    }
 
     auto load_queries = [&]() {  // the rows of the tile at p, rotated
       const int first_row = p.tile << a.tiling.row_bits, rows = min(BM, p.r.n * group - first_row);
@@ -218,7 +293,7 @@ paged_attention_kernel(AttendArgs a) {
             rotate(x0, x1, __ldg(a.rope.cos + at), __ldg(a.rope.sin + at));
           }
         }
-        const uint32_t at = S::at(r, d * (int)sizeof(T) / 16) + (d * (int)sizeof(T)) % 16;
+        const uint32_t at = S::template at<BM>(r, d * (int)sizeof(T) / 16) + (d * (int)sizeof(T)) % 16;
         T* dst = reinterpret_cast<T*>(smem + S::STAGES * S::STAGE + at);
         dst[0] = from_f32<T>(x0);
         dst[1] = from_f32<T>(x1);
@@ -230,21 +305,34 @@ paged_attention_kernel(AttendArgs a) {
       }
     };
     load_queries();
+    named_sync(1, NT);
 
     float o[DH / 8][4];
     float m[2], l[2];
     int vis[2], vis_min = 0;
     bool whole = false;  // this block began the tile
+    bool ok = true;
     for (int u = 0; u < units; u++) {
-      cp_wait<S::STAGES - 2>();
-      __syncthreads();  // stage u is complete; stage u - 1 and its addresses are free
-      issue(u + S::STAGES - 1);
-      look_up();
+      const int st = u % S::STAGES;
+      if constexpr (TMA) {
+        // after a wait that ran out the loop still ends, in step with the other warps
+        if (ok)
+          ok = __all_sync(0xffffffffu, role_wait(full_bar(st), (uint32_t)((u / S::STAGES) & 1),
+                                                 &g_wait_error, abort));
+      } else {
+        cp_wait<S::STAGES - 2>();
+        __syncthreads();  // stage u is complete; stage u - 1 and its addresses are free
+        issue(u + S::STAGES - 1);
+        look_up();
+      }
       const bool first = u == 0 || p.blk == 0;
       if (first) {  // a new tile
         whole = p.blk == 0;
         const int rows = min(BM, p.r.n * group - (p.tile << a.tiling.row_bits));
-        if (u > 0) load_queries();
+        if (u > 0) {
+          if (TMA) named_sync(1, NT);  // every warp is done with the last tile's queries
+          load_queries();
+        }
 #pragma unroll
         for (int i = 0; i < DH / 8; i++) o[i][0] = o[i][1] = o[i][2] = o[i][3] = 0.0f;
 #pragma unroll
@@ -257,9 +345,19 @@ paged_attention_kernel(AttendArgs a) {
         vis_min = rows == BM ? max(0, p.r.len - p.r.n +
                                           quotient(p.tile << a.tiling.row_bits, a.tiling.by_group) + 1)
                              : 0;
-        if (u > 0) __syncthreads();
+        if (u > 0) named_sync(1, NT);
       }
-      const uint32_t kt = base + (uint32_t)(u % S::STAGES) * S::STAGE, vt = kt + S::TILE;
+      const uint32_t kt = base + (uint32_t)st * S::STAGE, vt = kt + S::TILE;
+      if (TMA && p.blk + 1 == p.nblk) {
+        // slots behind the tile's keys may hold anything: this warp's rows of V
+        const int valid = tile_visible(a.tiling, p.r, p.tile) - p.blk * BK;
+        if (valid < (wk + 1) * KW) {
+          for (int row = max(valid, wk * KW); row < (wk + 1) * KW; row++)
+            for (int c = lane; c < S::PIECES; c += 32)
+              sts128(vt + S::template at<BK>(row, c), make_float4(0.f, 0.f, 0.f, 0.f));
+          __syncwarp();
+        }
+      }
 
       // scores of this warp's KW keys
       float s[KW / 8][4];
@@ -268,18 +366,18 @@ paged_attention_kernel(AttendArgs a) {
 #pragma unroll
       for (int ks = 0; ks < DH / KSTEP; ks++) {
         uint32_t qa[4];
-        ldsm4(qa, qs + S::at(wm * 16 + (lane & 15), 2 * ks + (lane >> 4)));
+        ldsm4(qa, qs + S::template at<BM>(wm * 16 + (lane & 15), 2 * ks + (lane >> 4)));
         uint32_t qh[4], ql[4];
         if constexpr (F32) {
 #pragma unroll
           for (int i = 0; i < 4; i++) pair_tf32(qa[i], qh[i], ql[i]);
         } else {
-          ldsm4(ql, qs + S::TILE_Q + S::at(wm * 16 + (lane & 15), 2 * ks + (lane >> 4)));
+          ldsm4(ql, qs + S::TILE_Q + S::template at<BM>(wm * 16 + (lane & 15), 2 * ks + (lane >> 4)));
         }
 #pragma unroll
         for (int n = 0; n < KW / 16; n++) {
           uint32_t kb[4];
-          ldsm4(kb, kt + S::at(wk * KW + 16 * n + ((lane >> 4) << 3) + (lane & 7),
+          ldsm4(kb, kt + S::template at<BK>(wk * KW + 16 * n + ((lane >> 4) << 3) + (lane & 7),
                                2 * ks + ((lane >> 3) & 1)));
           if constexpr (F32) {
             uint32_t kh[4], kl[4];
@@ -355,7 +453,7 @@ paged_attention_kernel(AttendArgs a) {
             uint32_t vh[2], vl[2];
 #pragma unroll
             for (int i = 0; i < 2; i++)
-              pair_tf32(lds32(vt + S::at(row + i, d / 4) + 4 * (d & 3)), vh[i], vl[i]);
+              pair_tf32(lds32(vt + S::template at<BK>(row + i, d / 4) + 4 * (d & 3)), vh[i], vl[i]);
             // the tensor pipe's accumulation truncates: eight keys at a time, added in f32
             float part[4] = {0.0f, 0.0f, 0.0f, 0.0f};
             mma_tf32(part, pl, vh[0], vh[1]);
@@ -375,7 +473,7 @@ paged_attention_kernel(AttendArgs a) {
 #pragma unroll
           for (int n = 0; n < DH / 16; n++) {
             uint32_t vb[4];
-            ldsm4t(vb, vt + S::at(wk * KW + 16 * kk + (lane & 15), 2 * n + (lane >> 4)));
+            ldsm4t(vb, vt + S::template at<BK>(wk * KW + 16 * kk + (lane & 15), 2 * n + (lane >> 4)));
             mma16<T>(o[2 * n], pa, vb[0], vb[1]);
             mma16<T>(o[2 * n + 1], pa, vb[2], vb[3]);
           }
@@ -391,8 +489,8 @@ paged_attention_kernel(AttendArgs a) {
         }
         const int r0 = wm * 16 + lane / 4;
         if constexpr (WK > 1) {
-          __syncthreads();  // every warp is done with the stage
-          float* merge = reinterpret_cast<float*>(smem + (u % S::STAGES) * S::STAGE);
+          named_sync(1, NT);  // every warp is done with the stage
+          float* merge = reinterpret_cast<float*>(smem + st * S::STAGE);
           if ((lane & 3) == 0) {
 #pragma unroll
             for (int i = 0; i < 2; i++) {
@@ -406,7 +504,7 @@ paged_attention_kernel(AttendArgs a) {
             for (int n = 0; n < DH / 8; n++)
               *reinterpret_cast<float4*>(mine + n * 128) = make_float4(o[n][0], o[n][1], o[n][2], o[n][3]);
           }
-          __syncthreads();
+          named_sync(1, NT);
           if (wk == 0) {
             float f[WK][2];
 #pragma unroll
@@ -478,9 +576,18 @@ paged_attention_kernel(AttendArgs a) {
           cut = Cut{p.r.first, p.r.n, p.h, p.tile, 1 + (int)((rest + share.per - 1) / share.per)};
         }
       }
+      if constexpr (TMA) {
+        if (tile_ends || u + 1 == units) fence_async_smem();  // plain writes before the next copy
+        __syncwarp();
+        if (lane == 0) mbar_arrive(empty_bar(st));
+      }
       advance(a.tiling, a.batch, p);
     }
-    cp_wait<0>();
+    if constexpr (TMA) {
+      if (!ok && tid == 0) report(a.batch.status, ET_B200_PAGED_TIMEOUT);
+    } else {
+      cp_wait<0>();
+    }
   }
   if (tid == 0) a.joint.cuts[blockIdx.x] = cut;
 }
@@ -555,7 +662,7 @@ __global__ void __launch_bounds__(32 * JOIN_WARPS) paged_join_kernel(AttendArgs 
 // Padded head_dim of the kernels: 32, 64, 128 or 256.
 int padded(int64_t dim) { return dim <= 32 ? 32 : dim <= 64 ? 64 : dim <= 128 ? 128 : 256; }
 
-constexpr int kMostPerSm = 2;  // resident thread blocks per SM that the workspace allows for
+constexpr int kMostPerSm = 4;  // resident thread blocks per SM that the workspace allows for
 
 // Resident thread blocks of a kernel per SM (at most kMostPerSm), per device
 // (the attribute that admits its shared memory is set on the way).
@@ -594,27 +701,38 @@ void launch_join(const AttendArgs& a, int blocks, cudaStream_t stream) {
 }
 
 template <typename T, typename S>
-void launch_shape(AttendArgs& a, void* ws, cudaStream_t stream) {
-  const int blocks = resident_blocks<paged_attention_kernel<T, S>>(S::NT, S::SMEM) * sm_count();
+void launch_shape(const et_b200_paged_cache_v1* c, AttendArgs& a, void* ws, cudaStream_t stream) {
+  int box_bits = 0;
+  while ((2 << box_bits) <= (c->page_size < S::BK ? c->page_size : S::BK)) box_bits++;
+  CUtensorMap k_map, v_map;
+  const bool tma = pool_map(&k_map, c->keys, c, S::WIDE, 1 << box_bits) &&
+                   pool_map(&v_map, c->values, c, S::WIDE, 1 << box_bits);
+  const int resident = tma ? resident_blocks<paged_attention_kernel<T, S, true>>(S::NT + 32, S::SMEM)
+                           : resident_blocks<paged_attention_kernel<T, S, false>>(S::NT, S::SMEM);
+  const int blocks = resident * sm_count();
   a.tiling = tiling_of(S::bits(S::BM), S::bits(S::BK), a.tiling.group, a.pools.kv_heads);
   a.least = 1;
   a.joint = joint_of(ws, blocks, S::BM, S::DH);
-  paged_attention_kernel<T, S><<<blocks, S::NT, S::SMEM, stream>>>(a);
+  if (tma)
+    paged_attention_kernel<T, S, true><<<blocks, S::NT + 32, S::SMEM, stream>>>(k_map, v_map, a, box_bits);
+  else
+    paged_attention_kernel<T, S, false><<<blocks, S::NT, S::SMEM, stream>>>(k_map, v_map, a, box_bits);
   count_launch();
   launch_join<T, S::DH>(a, blocks, stream);
 }
 
 template <typename T, int DH>
-void launch_dim(AttendArgs& a, int64_t max_new, void* ws, cudaStream_t stream) {
+void launch_dim(const et_b200_paged_cache_v1* c, AttendArgs& a, int64_t max_new, void* ws,
+                cudaStream_t stream) {
   constexpr bool F32 = sizeof(T) == 4;
   // up to 16 rows per kv head: one row tile, warps along the keys; more: 64-row
   // tiles, every warp walks all keys
   if (max_new * a.tiling.group <= 16) {
-    if constexpr (F32 && DH == 256) launch_shape<T, Shape<T, DH, 1, 2, 32, 3>>(a, ws, stream);
-    else launch_shape<T, Shape<T, DH, 1, 4, 64, 3>>(a, ws, stream);
+    if constexpr (F32 && DH == 256) launch_shape<T, Shape<T, DH, 1, 2, 32, 3>>(c, a, ws, stream);
+    else launch_shape<T, Shape<T, DH, 1, 4, 64, 3>>(c, a, ws, stream);
   } else {
-    if constexpr (F32 && DH == 256) launch_shape<T, Shape<T, DH, 4, 1, 32, 2>>(a, ws, stream);
-    else launch_shape<T, Shape<T, DH, 4, 1, 64, 2>>(a, ws, stream);
+    if constexpr (F32 && DH == 256) launch_shape<T, Shape<T, DH, 4, 1, 32, 2>>(c, a, ws, stream);
+    else launch_shape<T, Shape<T, DH, 4, 1, 64, 2>>(c, a, ws, stream);
   }
 }
 
@@ -629,10 +747,10 @@ void launch_type(const et_b200_paged_cache_v1* c, AttendArgs& a, int64_t max_new
     }
   }
   switch (padded(a.pools.head_dim)) {
-    case 32: return launch_dim<T, 32>(a, max_new, ws, stream);
-    case 64: return launch_dim<T, 64>(a, max_new, ws, stream);
-    case 128: return launch_dim<T, 128>(a, max_new, ws, stream);
-    default: return launch_dim<T, 256>(a, max_new, ws, stream);
+    case 32: return launch_dim<T, 32>(c, a, max_new, ws, stream);
+    case 64: return launch_dim<T, 64>(c, a, max_new, ws, stream);
+    case 128: return launch_dim<T, 128>(c, a, max_new, ws, stream);
+    default: return launch_dim<T, 256>(c, a, max_new, ws, stream);
   }
 }
 

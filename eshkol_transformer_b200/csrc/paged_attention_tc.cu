@@ -37,15 +37,6 @@ constexpr float kJump = 8.0f;  // log2 of the largest P the standing maximum all
 
 __device__ int g_wait_error;  // bounded waits that gave up (the status word tells the caller)
 
-__device__ __forceinline__ void tma_load_4d(uint32_t dst, const CUtensorMap* map, uint32_t bar,
-                                            int x, int y, int z, int w) {
-  asm volatile(
-      "cp.async.bulk.tensor.4d.shared::cluster.global.tile.mbarrier::complete_tx::bytes"
-      " [%0], [%1, {%3, %4, %5, %6}], [%2];" ::"r"(dst),
-      "l"(reinterpret_cast<uint64_t>(map)), "r"(bar), "r"(x), "r"(y), "r"(z), "r"(w)
-      : "memory");
-}
-
 template <typename T>
 __device__ __forceinline__ uint32_t pack2(float a, float b) {
   if constexpr (std::is_same_v<T, __half>) {
@@ -430,26 +421,13 @@ paged_attention_tc_kernel(const __grid_constant__ CUtensorMap k_map,
   }
 }
 
-// Map of a pool: boxes of 64 dims x box_rows slots of one head of one page.
-bool pool_map(CUtensorMap* map, void* pool, const et_b200_paged_cache_v1* c, int box_rows) {
-  const cuuint64_t dims[4] = {(cuuint64_t)c->head_dim, (cuuint64_t)c->page_size,
-                              (cuuint64_t)c->kv_heads, (cuuint64_t)c->pages};
-  const cuuint64_t strides[3] = {(cuuint64_t)c->token_stride * 2, (cuuint64_t)c->head_stride * 2,
-                                 (cuuint64_t)c->page_stride * 2};
-  const cuuint32_t box[4] = {64, (cuuint32_t)box_rows, 1, 1}, one[4] = {1, 1, 1, 1};
-  return encode_fn()(map, c->dtype == ET_B200_DTYPE_F16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16
-                                                         : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16,
-                     4, pool, dims, strides, box, one, CU_TENSOR_MAP_INTERLEAVE_NONE,
-                     CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
-                     CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
-}
-
 template <typename T, int DH>
 int launch_tc(const et_b200_paged_cache_v1* c, AttendArgs& a, void* ws, cudaStream_t stream) {
   using L = Layout<DH>;
   const int box_rows = (int)(c->page_size < BK ? c->page_size : BK);
   CUtensorMap k_map, v_map;
-  if (!pool_map(&k_map, c->keys, c, box_rows) || !pool_map(&v_map, c->values, c, box_rows)) return 0;
+  if (!pool_map(&k_map, c->keys, c, 64, box_rows) || !pool_map(&v_map, c->values, c, 64, box_rows))
+    return 0;
   const int blocks = sm_count();
   a.tiling = tiling_of(8, 7, a.tiling.group, a.pools.kv_heads);
   static_assert(2 * HALF == 1 << 8 && BK == 1 << 7, "tiling");
@@ -471,12 +449,7 @@ size_t attend_tc_workspace(int dim_padded) {
 }
 
 int attend_tc(const et_b200_paged_cache_v1* c, AttendArgs& a, void* ws, cudaStream_t stream) {
-  const int64_t ps = c->page_size;
-  if (c->dtype == ET_B200_DTYPE_F32 || c->head_dim > 128 || ps < 8 || (ps & (ps - 1)) != 0 ||
-      encode_fn() == nullptr)
-    return 0;
-  // strides that a tensor map cannot hold
-  if (c->page_stride * 2 >= (int64_t)1 << 40 || c->head_stride * 2 >= (int64_t)1 << 40) return 0;
+  if (c->dtype == ET_B200_DTYPE_F32 || c->head_dim > 128) return 0;
   if (c->dtype == ET_B200_DTYPE_F16)
     return c->head_dim <= 64 ? launch_tc<__half, 64>(c, a, ws, stream)
                              : launch_tc<__half, 128>(c, a, ws, stream);

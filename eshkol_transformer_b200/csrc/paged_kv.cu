@@ -183,6 +183,26 @@ int32_t check_rope(const et_b200_paged_rope_v1* r, et_kernel_error* e, const cha
   return 0;
 }
 
+bool pool_map(CUtensorMap* map, void* pool, const et_b200_paged_cache_v1* c, int wide, int box_rows) {
+  const int64_t rows = c->page_size, size = c->dtype == ET_B200_DTYPE_F32 ? 4 : 2;
+  if (rows < 8 || (rows & (rows - 1)) != 0 || encode_fn() == nullptr ||
+      c->page_stride * size >= (int64_t)1 << 40 || c->head_stride * size >= (int64_t)1 << 40)
+    return false;
+  const cuuint64_t dims[4] = {(cuuint64_t)c->head_dim, (cuuint64_t)c->page_size,
+                              (cuuint64_t)c->kv_heads, (cuuint64_t)c->pages};
+  const cuuint64_t strides[3] = {(cuuint64_t)(c->token_stride * size),
+                                 (cuuint64_t)(c->head_stride * size),
+                                 (cuuint64_t)(c->page_stride * size)};
+  const cuuint32_t box[4] = {(cuuint32_t)wide, (cuuint32_t)box_rows, 1, 1}, one[4] = {1, 1, 1, 1};
+  const auto type = c->dtype == ET_B200_DTYPE_F32   ? CU_TENSOR_MAP_DATA_TYPE_FLOAT32
+                    : c->dtype == ET_B200_DTYPE_F16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16
+                                                    : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16;
+  return encode_fn()(map, type, 4, pool, dims, strides, box, one, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                     wide * size == 64 ? CU_TENSOR_MAP_SWIZZLE_64B : CU_TENSOR_MAP_SWIZZLE_128B,
+                     CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                     CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
 Pools pools_of(const et_b200_paged_cache_v1* c) {
   return Pools{c->pages, c->page_stride, c->head_stride, c->token_stride, (int)c->page_size,
                (int)c->kv_heads, (int)c->head_dim, divisor_of((uint32_t)c->page_size)};
