@@ -101,6 +101,30 @@ template <> __device__ __forceinline__ __nv_bfloat16 from_f32<__nv_bfloat16>(flo
   return __float2bfloat16_rn(x);
 }
 
+// ---- pairs of f32 in one register pair: two operations per instruction ----------------
+
+__device__ __forceinline__ uint64_t pk(float a, float b) {
+  uint64_t r;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(a), "f"(b));
+  return r;
+}
+__device__ __forceinline__ float2 unpk(uint64_t v) {
+  float2 r;
+  asm("mov.b64 {%0, %1}, %2;" : "=f"(r.x), "=f"(r.y) : "l"(v));
+  return r;
+}
+__device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
+  uint64_t r;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+  return r;
+}
+__device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
+  uint64_t r;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+__device__ __forceinline__ uint64_t twice(float a) { return pk(a, a); }
+
 // RoPE of the pair (x0, x1) in the reference's rounding order
 // (native/a2_attention_provider.c:792-935).
 __device__ __forceinline__ void rotate(float& x0, float& x1, float c, float s) {
@@ -188,12 +212,15 @@ template <int NT>
 __device__ Share divide(const Tiling& t, const Batch& B, int64_t least, Place& p) {
   __shared__ int64_t warp_sum_s[NT / 32];
   __shared__ int64_t found_s[2];
+  __shared__ Request request_s;
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  Request mine_r{0, 0, 0, 0};
+  int64_t per_head = 0;
   auto units_of = [&](int b) -> int64_t {
     if (b >= B.batch) return 0;
-    const Request r = load_request(B, b);
-    if (r.bad != 0 && blockIdx.x == 0) report(B.status, r.bad);
-    return head_units(t, r) * t.kv_heads;
+    mine_r = load_request(B, b);
+    if (mine_r.bad != 0 && blockIdx.x == 0) report(B.status, mine_r.bad);
+    return (per_head = head_units(t, mine_r)) * t.kv_heads;
   };
   // inclusive scan over the block; *all receives the block's sum
   auto scan = [&](int64_t v, int64_t* all) -> int64_t {
@@ -241,19 +268,21 @@ __device__ Share divide(const Tiling& t, const Batch& B, int64_t least, Place& p
     const int64_t from = before + incl - mine;
     if (from <= u0 && u0 < from + mine) {
       found_s[0] = base + tid;
-      found_s[1] = u0 - from;
+      int64_t rest = u0 - from;
+      int h = 0;
+      for (; rest >= per_head; rest -= per_head) h++;
+      found_s[1] = ((int64_t)h << 48) | rest;  // units of a head stay below 2^45
+      request_s = mine_r;
     }
     before += all;
     if (u0 < before) break;
   }
   __syncthreads();
   p.b = (int)found_s[0];
-  int64_t rest = found_s[1];
-  p.r = load_request(B, p.b);
+  int64_t rest = found_s[1] & (((int64_t)1 << 48) - 1);
+  p.h = (int)(found_s[1] >> 48);
+  p.r = request_s;
   p.tiles = tile_count(t, p.r);
-  const int64_t each = head_units(t, p.r);
-  p.h = 0;
-  for (; rest >= each; rest -= each) p.h++;
   p.tile = 0;
   enter_tile(t, p);
   while (rest >= p.nblk) {
@@ -334,6 +363,12 @@ int32_t check_rope(const et_b200_paged_rope_v1* r, et_kernel_error* e, const cha
 Pools pools_of(const et_b200_paged_cache_v1* c);
 Batch batch_of(const et_b200_paged_batch_v1* b, const et_b200_paged_cache_v1* c);
 Rope rope_of(const et_b200_paged_rope_v1* r);
+// `most` thread blocks, or fewer where the host's sizes leave fewer units.
+inline int thread_blocks(const AttendArgs& a, int most, int rows, int keys) {
+  const int64_t tiles = (a.batch.tokens * a.tiling.group / rows + a.batch.batch) * a.pools.kv_heads;
+  const int64_t blocks = (a.batch.capacity + keys - 1) / keys;
+  return blocks < most && tiles * blocks < most ? (int)(tiles * blocks) : most;
+}
 // The tcgen05 kernel (paged_attention_tc.cu): launches it and returns its
 // thread blocks, 0 where it does not take the cache (nothing is launched).
 size_t attend_tc_workspace(int dim_padded);

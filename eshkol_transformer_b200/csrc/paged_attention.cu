@@ -277,30 +277,46 @@ paged_attention_kernel(const __grid_constant__ CUtensorMap k_map,
 
     auto load_queries = [&]() {  // the rows of the tile at p, rotated
       const int first_row = p.tile << a.tiling.row_bits, rows = min(BM, p.r.n * group - first_row);
-#pragma unroll 4
-      for (int i = tid; i < BM * DH / 2; i += NT) {
-        const int r = i / (DH / 2), d = 2 * (i % (DH / 2));
-        float x0 = 0.0f, x1 = 0.0f;
-        if (r < rows && d < dim) {
-          const int t = quotient(first_row + r, a.tiling.by_group), j = first_row + r - t * group;
-          const T* src = static_cast<const T*>(a.q) + (p.r.first + t) * a.q_stride +
-                         (int64_t)(p.h * group + j) * dim + d;
-          x0 = to_f32<T>(src[0]);
-          x1 = to_f32<T>(src[1]);
-          const int pos = p.r.len - p.r.n + t;
-          if (a.rope.cos != nullptr && pos >= 0) {
-            const int64_t at = rope_row(a.rope, pos, a.batch.status) * (dim / 2) + d / 2;
-            rotate(x0, x1, __ldg(a.rope.cos + at), __ldg(a.rope.sin + at));
+      constexpr int PAIRS = BM * DH / 2, AT_ONCE = S::WM == 1 ? 8 : 1;  // loads in flight per thread
+#pragma unroll(S::WM == 1 ? 1 : 4)
+      for (int i0 = tid; i0 < PAIRS; i0 += NT * AT_ONCE) {
+        T x[AT_ONCE][2];
+        float cs[AT_ONCE], sn[AT_ONCE];
+#pragma unroll
+        for (int k = 0; k < AT_ONCE; k++) {
+          const int i = i0 + k * NT, r = i / (DH / 2), d = 2 * (i % (DH / 2));
+          x[k][0] = x[k][1] = from_f32<T>(0.0f);
+          cs[k] = 1.0f;
+          sn[k] = 0.0f;
+          if (i < PAIRS && r < rows && d < dim) {
+            const int t = quotient(first_row + r, a.tiling.by_group), j = first_row + r - t * group;
+            const T* src = static_cast<const T*>(a.q) + (p.r.first + t) * a.q_stride +
+                           (int64_t)(p.h * group + j) * dim + d;
+            x[k][0] = src[0];
+            x[k][1] = src[1];
+            const int pos = p.r.len - p.r.n + t;
+            if (a.rope.cos != nullptr && pos >= 0) {
+              const int64_t at = rope_row(a.rope, pos, a.batch.status) * (dim / 2) + d / 2;
+              cs[k] = __ldg(a.rope.cos + at);
+              sn[k] = __ldg(a.rope.sin + at);
+            }
           }
         }
-        const uint32_t at = S::template at<BM>(r, d * (int)sizeof(T) / 16) + (d * (int)sizeof(T)) % 16;
-        T* dst = reinterpret_cast<T*>(smem + S::STAGES * S::STAGE + at);
-        dst[0] = from_f32<T>(x0);
-        dst[1] = from_f32<T>(x1);
-        if constexpr (!F32) {  // and what the rounding left
-          T* low = reinterpret_cast<T*>(smem + S::STAGES * S::STAGE + S::TILE_Q + at);
-          low[0] = from_f32<T>(x0 - to_f32<T>(dst[0]));
-          low[1] = from_f32<T>(x1 - to_f32<T>(dst[1]));
+#pragma unroll
+        for (int k = 0; k < AT_ONCE; k++) {
+          const int i = i0 + k * NT, r = i / (DH / 2), d = 2 * (i % (DH / 2));
+          if (i >= PAIRS) break;
+          float x0 = to_f32<T>(x[k][0]), x1 = to_f32<T>(x[k][1]);
+          if (a.rope.cos != nullptr) rotate(x0, x1, cs[k], sn[k]);
+          const uint32_t at = S::template at<BM>(r, d * (int)sizeof(T) / 16) + (d * (int)sizeof(T)) % 16;
+          T* dst = reinterpret_cast<T*>(smem + S::STAGES * S::STAGE + at);
+          dst[0] = from_f32<T>(x0);
+          dst[1] = from_f32<T>(x1);
+          if constexpr (!F32) {  // and what the rounding left
+            T* low = reinterpret_cast<T*>(smem + S::STAGES * S::STAGE + S::TILE_Q + at);
+            low[0] = from_f32<T>(x0 - to_f32<T>(dst[0]));
+            low[1] = from_f32<T>(x1 - to_f32<T>(dst[1]));
+          }
         }
       }
     };
@@ -592,68 +608,71 @@ paged_attention_kernel(const __grid_constant__ CUtensorMap k_map,
   if (tid == 0) a.joint.cuts[blockIdx.x] = cut;
 }
 
-// Joins the parts of the tile that thread block blockIdx.x of the attention
-// began and did not finish; blockIdx.y takes rows y, y + gridDim.y, ...  The
+// Joins the parts of the tiles that the thread blocks blockIdx.x, blockIdx.x +
+// gridDim.x, ... (of `blocks`) of the attention began and did not finish;
+// blockIdx.y takes rows y, y + gridDim.y, ...  The
 // warps take parts w, w + 8, ... of a row, 4 dims per lane, several parts' loads
 // in flight; shared memory adds the warps up in order.
 constexpr int JOIN_WARPS = 8;
 template <typename T, int DH>
-__global__ void __launch_bounds__(32 * JOIN_WARPS) paged_join_kernel(AttendArgs a) {
+__global__ void __launch_bounds__(32 * JOIN_WARPS) paged_join_kernel(AttendArgs a, int blocks) {
   constexpr int V = DH >= 128 ? DH / 32 : 4, LANES = DH / V;  // dims per lane, lanes used
   __shared__ float sums[JOIN_WARPS][DH];
   __shared__ float totals[JOIN_WARPS];
   asm volatile("griddepcontrol.wait;" ::: "memory");
-  const int c = blockIdx.x, rows = 1 << a.tiling.row_bits, group = a.tiling.group;
-  const Cut cut = a.joint.cuts[c];
-  if (cut.parts == 0) return;
+  const int rows = 1 << a.tiling.row_bits, group = a.tiling.group;
   const int dim = a.pools.head_dim, lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  auto slot_of = [&](int part) { return part == 0 ? 2 * c + 1 : 2 * (c + part); };
-  for (int r = blockIdx.y; r < rows; r += gridDim.y) {
-    const int g = (cut.tile << a.tiling.row_bits) + r;
-    if (g >= cut.n * group) return;
-    float m = -INFINITY;
-    for (int i = lane; i < cut.parts; i += 32)
-      m = fmaxf(m, a.joint.stats[(int64_t)slot_of(i) * 2 * rows + r]);
-    m = warp_max(m);
-    const float ref = m == -INFINITY ? 0.0f : m;
-    float l = 0.0f, x[V];
+  for (int c = blockIdx.x; c < blocks; c += gridDim.x) {
+    const Cut cut = a.joint.cuts[c];
+    if (cut.parts == 0) continue;
+    auto slot_of = [&](int part) { return part == 0 ? 2 * c + 1 : 2 * (c + part); };
+    for (int r = blockIdx.y; r < rows; r += gridDim.y) {
+      const int g = (cut.tile << a.tiling.row_bits) + r;
+      if (g >= cut.n * group) break;
+      float m = -INFINITY;
+      for (int i = lane; i < cut.parts; i += 32)
+        m = fmaxf(m, a.joint.stats[(int64_t)slot_of(i) * 2 * rows + r]);
+      m = warp_max(m);
+      const float ref = m == -INFINITY ? 0.0f : m;
+      float l = 0.0f, x[V];
 #pragma unroll
-    for (int k = 0; k < V; k++) x[k] = 0.0f;
+      for (int k = 0; k < V; k++) x[k] = 0.0f;
 #pragma unroll 4
-    for (int i = warp; i < cut.parts; i += JOIN_WARPS) {
-      const int64_t s = slot_of(i);
-      const float f = ex2(a.joint.stats[s * 2 * rows + r] - ref);
-      l += f * a.joint.stats[(s * 2 + 1) * rows + r];
-      if (lane < LANES) {
-        const float* src = a.joint.sums + (s * rows + r) * DH + lane * V;
+      for (int i = warp; i < cut.parts; i += JOIN_WARPS) {
+        const int64_t s = slot_of(i);
+        const float f = ex2(a.joint.stats[s * 2 * rows + r] - ref);
+        l += f * a.joint.stats[(s * 2 + 1) * rows + r];
+        if (lane < LANES) {
+          const float* src = a.joint.sums + (s * rows + r) * DH + lane * V;
 #pragma unroll
-        for (int k = 0; k < V; k += 4) {
-          const float4 y = *reinterpret_cast<const float4*>(src + k);
-          x[k] += f * y.x; x[k + 1] += f * y.y; x[k + 2] += f * y.z; x[k + 3] += f * y.w;
+          for (int k = 0; k < V; k += 4) {
+            const float4 y = *reinterpret_cast<const float4*>(src + k);
+            x[k] += f * y.x; x[k + 1] += f * y.y; x[k + 2] += f * y.z; x[k + 3] += f * y.w;
+          }
         }
       }
-    }
-    if (lane < LANES)
+      if (lane < LANES)
 #pragma unroll
-      for (int k = 0; k < V; k++) sums[warp][lane * V + k] = x[k];
-    if (lane == 0) totals[warp] = l;
-    __syncthreads();
-    const int d = 2 * threadIdx.x, by = quotient(g, a.tiling.by_group), h = cut.h * group + g - by * group;
-    const int64_t t = cut.first + by;
-    if (d < dim || threadIdx.x == 0) {
-      float total = 0.0f, y0 = 0.0f, y1 = 0.0f;
+        for (int k = 0; k < V; k++) sums[warp][lane * V + k] = x[k];
+      if (lane == 0) totals[warp] = l;
+      __syncthreads();
+      const int d = 2 * threadIdx.x, by = quotient(g, a.tiling.by_group), h = cut.h * group + g - by * group;
+      const int64_t t = cut.first + by;
+      if (d < dim || threadIdx.x == 0) {
+        float total = 0.0f, y0 = 0.0f, y1 = 0.0f;
 #pragma unroll
-      for (int w = 0; w < JOIN_WARPS; w++) {
-        total += totals[w];
-        y0 += sums[w][d];
-        y1 += sums[w][d + 1];
+        for (int w = 0; w < JOIN_WARPS; w++) {
+          total += totals[w];
+          y0 += sums[w][d];
+          y1 += sums[w][d + 1];
+        }
+        const float inv = total > 0.0f ? 1.0f / total : 0.0f;
+        store2<T>(static_cast<T*>(a.o) + t * a.o_stride + (int64_t)h * dim + d, y0 * inv, y1 * inv);
+        if (a.lse != nullptr && threadIdx.x == 0)
+          a.lse[t * a.q_heads + h] = total > 0.0f ? m * kLn2 + logf(total) : -INFINITY;
       }
-      const float inv = total > 0.0f ? 1.0f / total : 0.0f;
-      store2<T>(static_cast<T*>(a.o) + t * a.o_stride + (int64_t)h * dim + d, y0 * inv, y1 * inv);
-      if (a.lse != nullptr && threadIdx.x == 0)
-        a.lse[t * a.q_heads + h] = total > 0.0f ? m * kLn2 + logf(total) : -INFINITY;
+      __syncthreads();
     }
-    __syncthreads();
   }
 }
 
@@ -684,11 +703,11 @@ int resident_blocks(int threads, int smem) {
 }
 
 template <typename T, int DH>
-void launch_join(const AttendArgs& a, int blocks, cudaStream_t stream) {
+void launch_join(const AttendArgs& a, int blocks, int64_t rows, cudaStream_t stream) {
   cudaLaunchConfig_t cfg{};
-  // a row per thread block up to 16 rows
-  const int rows = 1 << a.tiling.row_bits;
-  cfg.gridDim = dim3(blocks, rows < 16 ? rows : 16);
+  // a row per thread block for as many rows as a tile is likely to have (the
+  // kernel walks any number)
+  cfg.gridDim = dim3(blocks < sm_count() ? blocks : sm_count(), rows < 1 ? 1 : rows < 16 ? rows : 16);
   cfg.blockDim = dim3(32 * JOIN_WARPS);
   cfg.stream = stream;
   cudaLaunchAttribute attr{};
@@ -696,12 +715,13 @@ void launch_join(const AttendArgs& a, int blocks, cudaStream_t stream) {
   attr.val.programmaticStreamSerializationAllowed = 1;
   cfg.attrs = &attr;
   cfg.numAttrs = 1;
-  cudaLaunchKernelEx(&cfg, paged_join_kernel<T, DH>, a);
+  cudaLaunchKernelEx(&cfg, paged_join_kernel<T, DH>, a, blocks);
   count_launch();
 }
 
 template <typename T, typename S>
-void launch_shape(const et_b200_paged_cache_v1* c, AttendArgs& a, void* ws, cudaStream_t stream) {
+void launch_shape(const et_b200_paged_cache_v1* c, AttendArgs& a, int64_t max_new, void* ws,
+                  cudaStream_t stream) {
   int box_bits = 0;
   while ((2 << box_bits) <= (c->page_size < S::BK ? c->page_size : S::BK)) box_bits++;
   CUtensorMap k_map, v_map;
@@ -709,7 +729,7 @@ void launch_shape(const et_b200_paged_cache_v1* c, AttendArgs& a, void* ws, cuda
                    pool_map(&v_map, c->values, c, S::WIDE, 1 << box_bits);
   const int resident = tma ? resident_blocks<paged_attention_kernel<T, S, true>>(S::NT + 32, S::SMEM)
                            : resident_blocks<paged_attention_kernel<T, S, false>>(S::NT, S::SMEM);
-  const int blocks = resident * sm_count();
+  const int blocks = thread_blocks(a, resident * sm_count(), S::BM, S::BK);
   a.tiling = tiling_of(S::bits(S::BM), S::bits(S::BK), a.tiling.group, a.pools.kv_heads);
   a.least = 1;
   a.joint = joint_of(ws, blocks, S::BM, S::DH);
@@ -718,7 +738,7 @@ void launch_shape(const et_b200_paged_cache_v1* c, AttendArgs& a, void* ws, cuda
   else
     paged_attention_kernel<T, S, false><<<blocks, S::NT, S::SMEM, stream>>>(k_map, v_map, a, box_bits);
   count_launch();
-  launch_join<T, S::DH>(a, blocks, stream);
+  launch_join<T, S::DH>(a, blocks, max_new * a.tiling.group, stream);
 }
 
 template <typename T, int DH>
@@ -728,11 +748,11 @@ void launch_dim(const et_b200_paged_cache_v1* c, AttendArgs& a, int64_t max_new,
   // up to 16 rows per kv head: one row tile, warps along the keys; more: 64-row
   // tiles, every warp walks all keys
   if (max_new * a.tiling.group <= 16) {
-    if constexpr (F32 && DH == 256) launch_shape<T, Shape<T, DH, 1, 2, 32, 3>>(c, a, ws, stream);
-    else launch_shape<T, Shape<T, DH, 1, 4, 64, 3>>(c, a, ws, stream);
+    if constexpr (F32 && DH == 256) launch_shape<T, Shape<T, DH, 1, 2, 32, 3>>(c, a, max_new, ws, stream);
+    else launch_shape<T, Shape<T, DH, 1, 4, 64, 3>>(c, a, max_new, ws, stream);
   } else {
-    if constexpr (F32 && DH == 256) launch_shape<T, Shape<T, DH, 4, 1, 32, 2>>(c, a, ws, stream);
-    else launch_shape<T, Shape<T, DH, 4, 1, 64, 2>>(c, a, ws, stream);
+    if constexpr (F32 && DH == 256) launch_shape<T, Shape<T, DH, 4, 1, 32, 2>>(c, a, max_new, ws, stream);
+    else launch_shape<T, Shape<T, DH, 4, 1, 64, 2>>(c, a, max_new, ws, stream);
   }
 }
 
@@ -742,8 +762,8 @@ void launch_type(const et_b200_paged_cache_v1* c, AttendArgs& a, int64_t max_new
   if constexpr (sizeof(T) == 2) {
     if (max_new * a.tiling.group > 16) {
       if (const int blocks = attend_tc(c, a, ws, stream))
-        return c->head_dim <= 64 ? launch_join<T, 64>(a, blocks, stream)
-                                 : launch_join<T, 128>(a, blocks, stream);
+        return c->head_dim <= 64 ? launch_join<T, 64>(a, blocks, 16, stream)
+                                 : launch_join<T, 128>(a, blocks, 16, stream);
     }
   }
   switch (padded(a.pools.head_dim)) {

@@ -6,9 +6,10 @@
 // group) as two halves of 128 TMEM lanes, a block 128 keys.  K and V blocks
 // arrive page by page through 4-D TMA maps of the pools (dim, slot, head,
 // page) into a ring of slots that both halves read, which halves the L2
-// traffic per product.  One thread issues, per block, P V and the next Q K^T
-// of half 0, then those of half 1: while the tensor pipe works on one half,
-// the other half's four warps (one row per thread, no exchange between
+// traffic per product.  Each half has a thread that issues P V of a block and
+// the next Q K^T behind it (one thread for both left the tensor pipe idle for
+// 1,100 of 3,950 cycles per pair of blocks between barriers); the two take
+// turns, which keeps the halves out of step: while the pipe works on one half, the other half's four warps (one row per thread, no exchange between
 // threads) turn scores into probabilities, written over the scores in TMEM as
 // the A operand of P V.  The row maximum stands until a block exceeds it by
 // 2^8 (the sums stay far inside f32), so O is rescaled in TMEM only then.
@@ -28,9 +29,9 @@ using namespace paged;
 using namespace f16att;
 
 constexpr int HALF = 128, BK = 128;
-// warps 0-7 probabilities; 8 products, 9 copies (10, 11 fill the warpgroup, whose
+// warps 0-7 probabilities; 8, 9 products, 10 copies (11 fills the warpgroup, whose
 // registers above kLeanRegs go to the other two: 256 x 208 + 128 x 88 = 384 x 168)
-constexpr int MMA_WARP = 8, LOAD_WARP = 9, THREADS = 384;
+constexpr int MMA_WARP = 8, LOAD_WARP = 10, THREADS = 384;
 constexpr int kWideRegs = 208, kLeanRegs = 88;
 static_assert(256 * kWideRegs + 128 * kLeanRegs <= THREADS * 168, "registers at launch");
 constexpr float kJump = 8.0f;  // log2 of the largest P the standing maximum allows
@@ -46,6 +47,24 @@ __device__ __forceinline__ uint32_t pack2(float a, float b) {
     const __nv_bfloat162 h = __floats2bfloat162_rn(a, b);
     return *reinterpret_cast<const uint32_t*>(&h);
   }
+}
+
+// 2^x of two finite values on the FMA pipe (x <= 8, under -126 as -126): x =
+// n + f with n rounded to nearest, 2^f by its polynomial of degree 4 of least
+// relative error on |f| <= 1/2 (2.7e-6), n added to the exponent.
+__device__ __forceinline__ uint64_t power2(uint64_t x) {
+  const float2 v = unpk(x);
+  x = pk(fmaxf(v.x, -126.0f), fmaxf(v.y, -126.0f));
+  const uint64_t m = add2(x, twice(12582912.0f));  // 1.5 2^23: n in the low bits
+  const uint64_t f = fma2(add2(m, twice(-12582912.0f)), twice(-1.0f), x);
+  uint64_t y = twice(9.5701013e-3f);
+  y = fma2(y, f, twice(5.5917859e-2f));
+  y = fma2(y, f, twice(2.4024744e-1f));
+  y = fma2(y, f, twice(6.9312179e-1f));
+  y = fma2(y, f, twice(9.9999928e-1f));
+  const float2 mm = unpk(m), yy = unpk(y);
+  return pk(__int_as_float(__float_as_int(yy.x) + (__float_as_int(mm.x) << 23)),
+            __int_as_float(__float_as_int(yy.y) + (__float_as_int(mm.y) << 23)));
 }
 
 template <int DH>
@@ -71,7 +90,7 @@ paged_attention_tc_kernel(const __grid_constant__ CUtensorMap k_map,
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) &
                                              ~(uintptr_t)1023);
   uint64_t* bars = reinterpret_cast<uint64_t*>(smem + L::BARS);
-  enum { FULL = 0, EMPTY = 8, SFULL = 16, PREADY = 18, QREADY = 20, ODONE = 22, DRAIN = 24, NBARS };
+  enum { FULL = 0, EMPTY = 8, SFULL = 16, PREADY = 18, QREADY = 20, ODONE = 22, DRAIN = 24, TURN = 26, NBARS = 28 };
   const uint32_t bar0 = smem_u32(bars);
   auto B_ = [&](int i) { return bar0 + 8u * (uint32_t)i; };
   uint32_t* tslot = reinterpret_cast<uint32_t*>(bars + NBARS);
@@ -83,7 +102,7 @@ paged_attention_tc_kernel(const __grid_constant__ CUtensorMap k_map,
 
   if (tid == 0) {
     for (int i = 0; i < NBARS; i++)
-      mbar_init(B_(i), (i >= PREADY && i < ODONE) ? HALF : 1);
+      mbar_init(B_(i), (i >= PREADY && i < ODONE) ? HALF : (i >= EMPTY && i < SFULL) ? 2 : 1);
     *abort = 0;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
@@ -155,42 +174,55 @@ paged_attention_tc_kernel(const __grid_constant__ CUtensorMap k_map,
     if (lane == 0)
       for (uint32_t c = count > SLOTS ? count - SLOTS : 0; c < count; c++)
         mbar_wait(B_(FULL + c % SLOTS), (c / SLOTS) & 1u, &g_wait_error);
-  } else if (warp == MMA_WARP) {
-    // ---- products
+  } else if (warp < LOAD_WARP) {
+    // ---- products of half t.  A half without rows goes along with the slots.
+    const int t = warp - MMA_WARP;
     constexpr uint32_t idesc_s = idesc_f16_m128(BK, 0) | kType;
     constexpr uint32_t idesc_o = idesc_f16_m128(DH, 1) | kType;
-    uint32_t count = 0, items[2] = {0, 0}, steps[2] = {0, 0};
+    const uint32_t q = base + L::Q + (uint32_t)t * (HALF * DH * 2);
+    const uint32_t s_at = tmem + L::S0 + 128u * t, o_at = tmem + L::O0 + (uint32_t)(DH * t);
+    uint32_t count = 0, items = 0, steps = 0, turns = 0;
     bool ok = true;
-    auto scores = [&](int t, uint32_t slot) {
-      const uint32_t q = base + L::Q + (uint32_t)t * (HALF * DH * 2), k = base + slot * L::SLOT;
+    // the halves' products go out in turns while both have rows
+    auto my_turn = [&](bool both) { return !both || (t == 0 && turns == 0) || wait(TURN + t, turns - 1 + t); };
+    auto pass_on = [&](bool both) {
+      if (both) {
+        mbar_arrive(B_(TURN + 1 - t));
+        turns++;
+      }
+    };
+    auto scores = [&](uint32_t slot) {
+      const uint32_t k = base + slot * L::SLOT;
 #pragma unroll
       for (int i = 0; i < DH / 16; i++)
-        umma_f16(tmem + L::S0 + 128u * t, kdesc16<HALF>(q, i), kdesc16<BK>(k, i), idesc_s,
-                 i > 0 ? 1u : 0u);
+        umma_f16(s_at, kdesc16<HALF>(q, i), kdesc16<BK>(k, i), idesc_s, i > 0 ? 1u : 0u);
       umma_commit(B_(SFULL + t));
     };
     while (ok && left > 0) {
-      const int nb = blocks_here(), halves = rows_here() > HALF ? 2 : 1;
+      const int nb = blocks_here();
+      const bool rows = rows_here() > HALF * t, both = rows_here() > HALF;
       const int visible = tile_visible(a.tiling, p.r, p.tile);
       uint32_t ks = count % SLOTS;
       ok = wait(FULL + ks, count / SLOTS);
-      for (int t = 0; ok && t < halves; t++) {
-        ok = wait(QREADY + t, items[t]);
-        ok = __all_sync(0xffffffffu, ok);
-        if (!ok) break;
-        tc_fence_after();
-        if (lane == 0) scores(t, ks);
-      }
-      if (ok && lane == 0) umma_commit(B_(EMPTY + ks));
       count++;
-      for (int j = 0; ok && j < nb; j++) {
+      if (ok && rows) ok = wait(QREADY + t, items);
+      if (ok) ok = my_turn(both);
+      ok = __all_sync(0xffffffffu, ok);
+      if (!ok) break;
+      tc_fence_after();
+      if (lane == 0) {
+        if (rows) scores(ks);
+        pass_on(both);
+        umma_commit(B_(EMPTY + ks));
+      }
+      turns = __shfl_sync(0xffffffffu, turns, 0);
+      for (int j = 0; j < nb; j++) {
         const uint32_t vs = count % SLOTS, vt = base + vs * L::SLOT;
-        ok = wait(FULL + vs, count / SLOTS);
-        ok = __all_sync(0xffffffffu, ok);
+        ok = __all_sync(0xffffffffu, wait(FULL + vs, count / SLOTS));
         if (!ok) break;
         count++;
         const int valid = visible - (p.blk + j) * BK;
-        if (valid < BK) {  // slots behind the visible keys may hold anything
+        if (valid < BK && rows) {  // slots behind the visible keys may hold anything
           for (int i = max(valid, 0) * 8 + lane; i < BK * 8; i += 32)
 #pragma unroll
             for (int c = 0; c < DH / 64; c++)
@@ -204,32 +236,32 @@ paged_attention_tc_kernel(const __grid_constant__ CUtensorMap k_map,
           ok = wait(FULL + ks, count / SLOTS);
           count++;
         }
-        for (int t = 0; ok && t < halves; t++) {
-          ok = wait(PREADY + t, steps[t]);
-          ok = __all_sync(0xffffffffu, ok);
-          if (!ok) break;
-          steps[t]++;
-          tc_fence_after();
-          if (lane == 0) {
+        if (ok && rows) ok = wait(PREADY + t, steps);
+        if (ok) ok = my_turn(both);
+        ok = __all_sync(0xffffffffu, ok);
+        if (!ok) break;
+        tc_fence_after();
+        if (lane == 0) {
+          if (rows) {
 #pragma unroll
             for (int i = 0; i < BK / 16; i++)
-              umma_f16_ts(tmem + L::O0 + (uint32_t)(DH * t), tmem + L::S0 + 128u * t + 8u * i,
-                          mdesc16<BK>(vt, i), idesc_o, (j > 0 || i > 0) ? 1u : 0u);
-            if (more) scores(t, ks);
+              umma_f16_ts(o_at, s_at + 8u * i, mdesc16<BK>(vt, i), idesc_o, (j > 0 || i > 0) ? 1u : 0u);
+            if (more) scores(ks);
             else umma_commit(B_(ODONE + t));
           }
-        }
-        if (ok && lane == 0) {
+          pass_on(both);
           umma_commit(B_(EMPTY + vs));
           if (more) umma_commit(B_(EMPTY + ks));
         }
+        turns = __shfl_sync(0xffffffffu, turns, 0);
+        steps += rows ? 1 : 0;
       }
-      for (int t = 0; t < halves; t++) items[t]++;
+      items += rows ? 1 : 0;
       next_tile(nb);
     }
     if (lane == 0) {
-      umma_commit(B_(DRAIN));
-      mbar_wait(B_(DRAIN), 0u, &g_wait_error);
+      umma_commit(B_(DRAIN + t));
+      mbar_wait(B_(DRAIN + t), 0u, &g_wait_error);
     }
   }
   } else {
@@ -309,7 +341,8 @@ paged_attention_tc_kernel(const __grid_constant__ CUtensorMap k_map,
           tmem_wait_ld_pin<false>(r[2]);
           tmem_wait_ld_pin<false>(r[3]);
           const int key0 = (p.blk + j) * BK;
-          if (key0 + BK > vis_warp) {
+          const bool masked = key0 + BK > vis_warp;
+          if (masked) {
             const int seen = vis - key0;
 #pragma unroll
             for (int c = 0; c < 4; c++)
@@ -343,21 +376,38 @@ paged_attention_tc_kernel(const __grid_constant__ CUtensorMap k_map,
             }
           }
           const float from = m == -INFINITY ? 0.0f : m;
-          float sum[4] = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-          for (int c = 0; c < 4; c++) {
+          // a quarter of the exponentials on the FMA pipe, the others on the special
+          // function unit (8 cycles per warp; the 4,096-token chunk: 783 us with all
+          // of them there, 757 with a quarter on the FMA pipe, 800 with half);
+          // blocks with masked scores (-inf) all on the latter
+          uint64_t sum[2] = {0, 0};
+          auto powers = [&](int c, auto some_masked) {
             float w[16];
 #pragma unroll
             for (int i = 0; i < 16; i++) {
-              const float x = ex2(fmaf(__uint_as_float(r[c][2 * i]), scale, -from));
-              const float y = ex2(fmaf(__uint_as_float(r[c][2 * i + 1]), scale, -from));
-              sum[(2 * i) & 3] += x;
-              sum[(2 * i + 1) & 3] += y;
-              w[i] = __uint_as_float(pack2<T>(x, y));
+              uint64_t x = fma2(pk(__uint_as_float(r[c][2 * i]), __uint_as_float(r[c][2 * i + 1])),
+                                twice(scale), twice(-from));
+              if (!decltype(some_masked)::value && (i & 3) == 3) {
+                x = power2(x);
+              } else {
+                const float2 v = unpk(x);
+                x = pk(ex2(v.x), ex2(v.y));
+              }
+              sum[i & 1] = add2(sum[i & 1], x);
+              const float2 v = unpk(x);
+              w[i] = __uint_as_float(pack2<T>(v.x, v.y));
             }
             tmem_st16(s_at + 16 * c, w);
+          };
+          if (masked) {
+#pragma unroll
+            for (int c = 0; c < 4; c++) powers(c, std::true_type{});
+          } else {
+#pragma unroll
+            for (int c = 0; c < 4; c++) powers(c, std::false_type{});
           }
-          l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
+          const float2 all = unpk(add2(sum[0], sum[1]));
+          l += all.x + all.y;
           tmem_wait_st();
           tc_fence_before();
           mbar_arrive(B_(PREADY + t));
@@ -428,7 +478,7 @@ int launch_tc(const et_b200_paged_cache_v1* c, AttendArgs& a, void* ws, cudaStre
   CUtensorMap k_map, v_map;
   if (!pool_map(&k_map, c->keys, c, 64, box_rows) || !pool_map(&v_map, c->values, c, 64, box_rows))
     return 0;
-  const int blocks = sm_count();
+  const int blocks = thread_blocks(a, sm_count(), 2 * HALF, BK);
   a.tiling = tiling_of(8, 7, a.tiling.group, a.pools.kv_heads);
   static_assert(2 * HALF == 1 << 8 && BK == 1 << 7, "tiling");
   a.least = 2;

@@ -30,7 +30,12 @@
 namespace etb {
 namespace {
 
+using paged::add2;
+using paged::fma2;
+using paged::pk;
 using paged::to_f32;
+using paged::twice;
+using paged::unpk;
 namespace cg = cooperative_groups;
 
 constexpr int NT = 512, WARPS = NT / 32;
@@ -110,27 +115,6 @@ __device__ __forceinline__ uint64_t weight_of(float x, const Scale& s) {
 struct Sum64 {
   uint64_t coarse, fine;  // f32 pairs
 };
-__device__ __forceinline__ uint64_t pk(float a, float b) {
-  uint64_t r;
-  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(a), "f"(b));
-  return r;
-}
-__device__ __forceinline__ float2 unpk(uint64_t v) {
-  float2 r;
-  asm("mov.b64 {%0, %1}, %2;" : "=f"(r.x), "=f"(r.y) : "l"(v));
-  return r;
-}
-__device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
-  uint64_t r;
-  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
-  return r;
-}
-__device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
-  uint64_t r;
-  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
-  return r;
-}
-__device__ __forceinline__ uint64_t twice(float a) { return pk(a, a); }
 // power_of of two logits at once (narrow scales)
 __device__ __forceinline__ uint64_t powers_of(float a, float b, const Scale& s) {
   const uint64_t x = pk(fmaxf(a, s.low), fmaxf(b, s.low)), hi = twice(s.hi), minus = twice(-1.0f);
