@@ -349,11 +349,12 @@ __device__ __forceinline__ void tma_load_4d(uint32_t dst, const CUtensorMap* map
       : "memory");
 }
 
-// Map of a pool for boxes of `wide` dims (64 or 128 bytes, swizzled as wide)
-// x box_rows slots of one head of one page; dims beyond head_dim and pages
+// Map of a pool for boxes of `wide` dims (swizzled: of 64 or 128 bytes, and as
+// wide as that) x box_rows slots of one head of one page; dims beyond head_dim and pages
 // outside the pool read as zeros.  False for pools it cannot describe (pages
 // that are no power of two of at least 8 slots, far strides).
-bool pool_map(CUtensorMap* map, void* pool, const et_b200_paged_cache_v1* c, int wide, int box_rows);
+bool pool_map(CUtensorMap* map, void* pool, const et_b200_paged_cache_v1* c, int wide, int box_rows,
+              bool swizzled = true);
 
 // Host pieces of the entry points.
 int32_t check_cache(const et_b200_paged_cache_v1* c, et_kernel_error* e, const char* op);
@@ -373,6 +374,9 @@ inline int thread_blocks(const AttendArgs& a, int most, int rows, int keys) {
 // thread blocks, 0 where it does not take the cache (nothing is launched).
 size_t attend_tc_workspace(int dim_padded);
 int attend_tc(const et_b200_paged_cache_v1* c, AttendArgs& a, void* ws, cudaStream_t stream);
+// The same for f32 caches (paged_attention_f32.cu); its workspace is within
+// attend_tc_workspace.
+int attend_f32(const et_b200_paged_cache_v1* c, AttendArgs& a, void* ws, cudaStream_t stream);
 
 }  // namespace paged
 }  // namespace etb

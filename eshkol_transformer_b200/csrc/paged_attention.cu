@@ -759,9 +759,10 @@ void launch_dim(const et_b200_paged_cache_v1* c, AttendArgs& a, int64_t max_new,
 template <typename T>
 void launch_type(const et_b200_paged_cache_v1* c, AttendArgs& a, int64_t max_new, void* ws,
                  cudaStream_t stream) {
-  if constexpr (sizeof(T) == 2) {
+  {
     if (max_new * a.tiling.group > 16) {
-      if (const int blocks = attend_tc(c, a, ws, stream))
+      const int blocks = sizeof(T) == 2 ? attend_tc(c, a, ws, stream) : attend_f32(c, a, ws, stream);
+      if (blocks > 0)
         return c->head_dim <= 64 ? launch_join<T, 64>(a, blocks, 16, stream)
                                  : launch_join<T, 128>(a, blocks, 16, stream);
     }

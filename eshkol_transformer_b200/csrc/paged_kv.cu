@@ -183,7 +183,8 @@ int32_t check_rope(const et_b200_paged_rope_v1* r, et_kernel_error* e, const cha
   return 0;
 }
 
-bool pool_map(CUtensorMap* map, void* pool, const et_b200_paged_cache_v1* c, int wide, int box_rows) {
+bool pool_map(CUtensorMap* map, void* pool, const et_b200_paged_cache_v1* c, int wide, int box_rows,
+              bool swizzled) {
   const int64_t rows = c->page_size, size = c->dtype == ET_B200_DTYPE_F32 ? 4 : 2;
   if (rows < 8 || (rows & (rows - 1)) != 0 || encode_fn() == nullptr ||
       c->page_stride * size >= (int64_t)1 << 40 || c->head_stride * size >= (int64_t)1 << 40)
@@ -198,7 +199,9 @@ bool pool_map(CUtensorMap* map, void* pool, const et_b200_paged_cache_v1* c, int
                     : c->dtype == ET_B200_DTYPE_F16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16
                                                     : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16;
   return encode_fn()(map, type, 4, pool, dims, strides, box, one, CU_TENSOR_MAP_INTERLEAVE_NONE,
-                     wide * size == 64 ? CU_TENSOR_MAP_SWIZZLE_64B : CU_TENSOR_MAP_SWIZZLE_128B,
+                     !swizzled            ? CU_TENSOR_MAP_SWIZZLE_NONE
+                     : wide * size == 64 ? CU_TENSOR_MAP_SWIZZLE_64B
+                                         : CU_TENSOR_MAP_SWIZZLE_128B,
                      CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
                      CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }

@@ -545,3 +545,28 @@ def test_decoding_loop(lib, cuda, dtype):
             assert ((seen[t][b].double() - want).abs() <= room).all()
             i, _, margin = sample(seen[t][b].cpu().numpy(), float(uniforms[t, b]), 1.0, 40)
             assert margin <= 2.5e-7 or i == int(drawn[t][b])
+
+
+@pytest.mark.parametrize("dim", [64, 128])
+def test_attention_f32_row_magnitudes(lib, cuda, dim):
+    """Keys and values whose rows differ by many powers of two, rows of zeros
+    among them (operand pairs carry an exponent per row): each output within
+    2e-5 of its row's weighted |v|, scores within 2e-5 of their own size."""
+    s = Step([(40, 700), (150, 150)], 4, 2, dim, 16, F32, seed=dim)
+    g = torch.Generator(device="cuda").manual_seed(dim)
+    for b in range(2):
+        m = s.k[b].shape[0]
+        for t, low, high in ((s.k[b], -12, 1), (s.v[b], -18, 18)):
+            t *= torch.exp2(torch.randint(low, high, (m, 2, 1), device="cuda", generator=g).float())
+            t[::7] = 0.0
+        s.store(b, s.k[b], s.v[b])
+    s.attend()
+    torch.cuda.synchronize()
+    first = 0
+    for b, (n, m) in enumerate(s.requests):
+        rows = slice(first, first + n)
+        first += n
+        q = turn(s.q[rows].double(), s.cos[m - n:m], s.sin[m - n:m])
+        o, lse, weighted, spread = attention(q, s.k[b].double(), s.v[b].double(), m - n)
+        assert ((s.o[rows].double() - o).abs() <= 2e-5 * weighted.amax(-1, keepdim=True)).all()
+        assert ((s.lse[rows].double() - lse).abs() <= 2e-5 * (1 + lse.abs())).all()
