@@ -225,31 +225,44 @@ paged_attention_f32_kernel(const __grid_constant__ CUtensorMap k_map,
           if (!ok) break;
           count++;
           const uint32_t raw = base + s * L::RAW, hi = conv + (uint32_t)kv * 2u * L::KT;
-#pragma unroll 4
-          for (int r0 = 0; r0 < BK; r0 += 4 * RW) {
-            const int row = r0 + (warp - CONVERT_WARP) * RW + sub;
-            float4 x = make_float4(0.f, 0.f, 0.f, 0.f);
-            if (row < valid) x = lds128(raw + (uint32_t)(row * DH + 4 * col) * 4u);
-            float m = abs_max4(0.0f, x);
+          // 8 rows of a lane group at once: loads, then maxima, then stores
+          constexpr int STEP = 4 * RW, AT_ONCE = 8;
 #pragma unroll
-            for (int o = LANES / 2; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
-            const int e = row_exponent(m);
-            const float sc = exp2_int(e);
-            float h0, l0, h1, l1;
-            pair2(x.x * sc, x.y * sc, h0, l0);
-            pair2(x.z * sc, x.w * sc, h1, l1);
-            const uint32_t piece = ((uint32_t)col & 15u) >> 1;
-            const uint32_t at = hi + (uint32_t)(col >> 4) * BK * 128u + (uint32_t)row * 128u +
-                                ((piece ^ (uint32_t)(row & 7)) << 4) + (uint32_t)(col & 1) * 8u;
-            asm volatile("st.shared.v2.f32 [%0], {%1, %2};" ::"r"(at), "f"(h0), "f"(h1) : "memory");
-            asm volatile("st.shared.v2.f32 [%0], {%1, %2};" ::"r"(at + L::KT), "f"(l0), "f"(l1)
-                         : "memory");
-            if (col == 0) {
-              if (kv == 0) {
-                f[row] = exp2_int(-e);
-              } else {
-                f[BK + row] = (float)-e;
-                f[2 * BK + row] = sc;
+          for (int r0 = 0; r0 < BK; r0 += AT_ONCE * STEP) {
+            const int row0 = r0 + (warp - CONVERT_WARP) * RW + sub;
+            float4 x[AT_ONCE];
+            float m[AT_ONCE];
+#pragma unroll
+            for (int k = 0; k < AT_ONCE; k++) {
+              const int row = row0 + k * STEP;
+              x[k] = make_float4(0.f, 0.f, 0.f, 0.f);
+              if (row < valid) x[k] = lds128(raw + (uint32_t)(row * DH + 4 * col) * 4u);
+              m[k] = abs_max4(0.0f, x[k]);
+            }
+#pragma unroll
+            for (int o = LANES / 2; o > 0; o >>= 1)
+#pragma unroll
+              for (int k = 0; k < AT_ONCE; k++) m[k] = fmaxf(m[k], __shfl_xor_sync(0xffffffffu, m[k], o));
+#pragma unroll
+            for (int k = 0; k < AT_ONCE; k++) {
+              const int row = row0 + k * STEP, e = row_exponent(m[k]);
+              const float sc = exp2_int(e);
+              float h0, l0, h1, l1;
+              pair2(x[k].x * sc, x[k].y * sc, h0, l0);
+              pair2(x[k].z * sc, x[k].w * sc, h1, l1);
+              const uint32_t piece = ((uint32_t)col & 15u) >> 1;
+              const uint32_t at = hi + (uint32_t)(col >> 4) * BK * 128u + (uint32_t)row * 128u +
+                                  ((piece ^ (uint32_t)(row & 7)) << 4) + (uint32_t)(col & 1) * 8u;
+              asm volatile("st.shared.v2.f32 [%0], {%1, %2};" ::"r"(at), "f"(h0), "f"(h1) : "memory");
+              asm volatile("st.shared.v2.f32 [%0], {%1, %2};" ::"r"(at + L::KT), "f"(l0), "f"(l1)
+                           : "memory");
+              if (col == 0) {
+                if (kv == 0) {
+                  f[row] = exp2_int(-e);
+                } else {
+                  f[BK + row] = (float)-e;
+                  f[2 * BK + row] = sc;
+                }
               }
             }
           }
@@ -284,50 +297,82 @@ paged_attention_f32_kernel(const __grid_constant__ CUtensorMap k_map,
       const int token = quotient(g, a.tiling.by_group), head = p.h * group + g - token * group;
       const int pos = p.r.len - p.r.n + token, vis = valid ? max(0, pos + 1) : 0;
       const int vis_warp = __shfl_sync(0xffffffffu, max(0, pos + 1), 0);
-      float cq;
-      // ---- this row of Q, rotated: hi into TMEM, lo into the swizzled tile
+      float cq = 0.0f;
+      // ---- the warp's rows of Q, rotated: 8 lanes a row, whole lines.  hi passes
+      // through the tile of lo on its way into TMEM (a row per lane), then lo takes
+      // the tile.
       {
-        const float* src = static_cast<const float*>(a.q) + (p.r.first + token) * a.q_stride + (int64_t)head * dim;
-        const float *ct = nullptr, *st = nullptr;
-        if (a.rope.cos != nullptr && valid && pos >= 0) {
-          const int64_t at = rope_row(a.rope, pos, a.batch.status) * (dim / 2);
-          ct = a.rope.cos + at;
-          st = a.rope.sin + at;
-        }
-        auto load4 = [&](int d) {
-          if (!valid || d >= dim) return make_float4(0.f, 0.f, 0.f, 0.f);
-          if (q_vec) return __ldg(reinterpret_cast<const float4*>(src + d));
-          return make_float4(__ldg(src + d), __ldg(src + d + 1), __ldg(src + d + 2), __ldg(src + d + 3));
-        };
-        float m = 0.0f;
-#pragma unroll 8
-        for (int d = 0; d < DH; d += 4) m = abs_max4(m, load4(d));
-        // a rotated pair is at most sqrt(2) times its larger element: below 2^14.5
-        const int e = row_exponent(m);
-        const float sc = exp2_int(e);
-        cq = a.scale_log2 * exp2_int(-e);
+        constexpr int P = DH / 32;  // 16-byte pieces of a lane
+        const uint32_t tile = base + L::QLO;
+#pragma unroll 1
+        for (int half = 0; half < 2; half++) {
+          for (int r0 = 0; r0 < 32; r0 += 8) {
+            float4 x[2][P], cs[2][P];
+            float sc[2];
 #pragma unroll
-        for (int c = 0; c < DH / 32; c++) {
-          float hi[16], lo[16];
+            for (int k = 0; k < 2; k++) {
+              const int r = warp * 32 + r0 + 4 * k + (lane >> 3), gr = p.tile * ROWS + r;
+              const int t = quotient(gr, a.tiling.by_group), at_pos = p.r.len - p.r.n + t;
+              const bool some = r < rows;
+              const float* src = static_cast<const float*>(a.q) + (p.r.first + t) * a.q_stride +
+                                 (int64_t)(p.h * group + gr - t * group) * dim;
+              const int64_t tab = some && a.rope.cos != nullptr && at_pos >= 0
+                                      ? rope_row(a.rope, at_pos, a.batch.status) * (dim / 2) : -1;
 #pragma unroll
-          for (int i = 0; i < 8; i++) {
-            const int d = 32 * c + 4 * i;
-            float4 x = load4(d);
-            if (ct != nullptr && d < dim) {
-              rotate(x.x, x.y, __ldg(ct + d / 2), __ldg(st + d / 2));
-              rotate(x.z, x.w, __ldg(ct + d / 2 + 1), __ldg(st + d / 2 + 1));
+              for (int i = 0; i < P; i++) {
+                const int d = 4 * ((lane & 7) + 8 * i);
+                x[k][i] = make_float4(0.f, 0.f, 0.f, 0.f);
+                cs[k][i] = make_float4(1.f, 0.f, 1.f, 0.f);
+                if (some && d < dim) {
+                  if (q_vec) x[k][i] = __ldg(reinterpret_cast<const float4*>(src + d));
+                  else x[k][i] = make_float4(__ldg(src + d), __ldg(src + d + 1), __ldg(src + d + 2), __ldg(src + d + 3));
+                  if (tab >= 0)
+                    cs[k][i] = make_float4(__ldg(a.rope.cos + tab + d / 2), __ldg(a.rope.sin + tab + d / 2),
+                                           __ldg(a.rope.cos + tab + d / 2 + 1), __ldg(a.rope.sin + tab + d / 2 + 1));
+                }
+              }
             }
-            pair2(x.x * sc, x.y * sc, hi[2 * i], lo[2 * i]);
-            pair2(x.z * sc, x.w * sc, hi[2 * i + 1], lo[2 * i + 1]);
-          }
-          tmem_st16(lanes + L::QH + 16u * c, hi);
-          const uint32_t q_row = base + L::QLO + (uint32_t)(c >> 1) * ROWS * 128u + (uint32_t)row * 128u;
 #pragma unroll
-          for (int i = 0; i < 4; i++)
-            sts128(q_row + ((((uint32_t)(c & 1) * 4u + (uint32_t)i) ^ (uint32_t)(row & 7)) << 4),
-                   make_float4(lo[4 * i], lo[4 * i + 1], lo[4 * i + 2], lo[4 * i + 3]));
+            for (int k = 0; k < 2; k++) {
+              float m = 0.0f;
+#pragma unroll
+              for (int i = 0; i < P; i++) m = abs_max4(m, x[k][i]);
+#pragma unroll
+              for (int o = 4; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
+              // a rotated pair is at most sqrt(2) times its larger element: below 2^14.5
+              const int e = row_exponent(m);
+              sc[k] = exp2_int(e);
+              const int mine = __shfl_sync(0xffffffffu, e, (lane & 3) * 8);
+              if ((lane >> 2) == (r0 >> 2) + k) cq = a.scale_log2 * exp2_int(-mine);
+            }
+#pragma unroll
+            for (int k = 0; k < 2; k++) {
+              const int r = warp * 32 + r0 + 4 * k + (lane >> 3);
+#pragma unroll
+              for (int i = 0; i < P; i++) {
+                float4 v = x[k][i];
+                if (a.rope.cos != nullptr) {
+                  rotate(v.x, v.y, cs[k][i].x, cs[k][i].y);
+                  rotate(v.z, v.w, cs[k][i].z, cs[k][i].w);
+                }
+                float h0, l0, h1, l1;
+                pair2(v.x * sc[k], v.y * sc[k], h0, l0);
+                pair2(v.z * sc[k], v.w * sc[k], h1, l1);
+                const int c = (lane & 7) + 8 * i;  // 8-byte unit of the row
+                const uint32_t at = tile + (uint32_t)(c >> 4) * ROWS * 128u + (uint32_t)r * 128u +
+                                    ((((uint32_t)c & 15u) >> 1 ^ (uint32_t)(r & 7)) << 4) + (uint32_t)(c & 1) * 8u;
+                asm volatile("st.shared.v2.f32 [%0], {%1, %2};" ::"r"(at), "f"(half ? l0 : h0),
+                             "f"(half ? l1 : h1) : "memory");
+              }
+            }
+          }
+          __syncwarp();
+          if (half == 0) {
+            tile_row16_to_tmem<DH>(tile, row, lanes, L::QH);
+            tmem_wait_st();
+            __syncwarp();
+          }
         }
-        tmem_wait_st();
         fence_async_smem();
         tc_fence_before();
         mbar_arrive(B_(QREADY));

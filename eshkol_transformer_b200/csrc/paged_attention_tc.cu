@@ -270,9 +270,9 @@ paged_attention_tc_kernel(const __grid_constant__ CUtensorMap k_map,
     const int t = warp >> 2, row = tid & (HALF - 1);
     const uint32_t lanes = tmem + ((uint32_t)((warp & 3) * 32) << 16);
     const uint32_t s_at = lanes + L::S0 + 128u * t, o_at = lanes + L::O0 + (uint32_t)(DH * t);
-    const uint32_t q_row = base + L::Q + (uint32_t)t * (HALF * DH * 2) + (uint32_t)row * 128u;
     const float scale = a.scale_log2;
     const bool q_vec = ((reinterpret_cast<uintptr_t>(a.q) | (uintptr_t)(a.q_stride * 2)) & 15) == 0;
+    const bool rope_vec = ((reinterpret_cast<uintptr_t>(a.rope.cos) | reinterpret_cast<uintptr_t>(a.rope.sin)) & 15) == 0;
     const bool o_vec = ((reinterpret_cast<uintptr_t>(a.o) | (uintptr_t)(a.o_stride * 2)) & 15) == 0;
     uint32_t items = 0, steps = 0;
     bool ok = true;
@@ -292,36 +292,71 @@ paged_attention_tc_kernel(const __grid_constant__ CUtensorMap k_map,
         const int vis = valid ? max(0, pos + 1) : 0;
         // keys that every row of this warp sees (invalid rows follow the last valid one)
         const int vis_warp = __shfl_sync(0xffffffffu, max(0, pos + 1), 0);
-        // ---- this row of Q, rotated, into the swizzled tile
+        // ---- the warp's rows of Q, rotated, into the swizzled tile: 8 lanes a row,
+        // whole lines, 8 rows' loads in flight
         {
-          const T* src = static_cast<const T*>(a.q) + (p.r.first + token) * a.q_stride + (int64_t)head * dim;
-          const float *ct = nullptr, *st = nullptr;
-          if (a.rope.cos != nullptr && valid && pos >= 0) {
-            const int64_t at = rope_row(a.rope, pos, a.batch.status) * (dim / 2);
-            ct = a.rope.cos + at;
-            st = a.rope.sin + at;
-          }
-#pragma unroll 4
-          for (int d = 0; d < DH; d += 8) {
-            union { uint4 v; T x[8]; } u;
-            u.v = make_uint4(0, 0, 0, 0);
-            if (valid && d < dim) {
-              if (q_vec) u.v = *reinterpret_cast<const uint4*>(src + d);
-              else
+          constexpr int P = DH / 64;  // 16-byte pieces of a lane
+          const int first_row = p.tile * 2 * HALF + HALF * t;
+          const uint32_t tile = base + L::Q + (uint32_t)t * (HALF * DH * 2);
+          for (int r0 = 0; r0 < 32; r0 += 8) {
+            union Piece { uint4 v; T x[8]; };
+            Piece u[2][P];
+            float4 cs[2][P], sn[2][P];
 #pragma unroll
-                for (int i = 0; i < 8; i++) u.x[i] = src[d + i];
-              if (ct != nullptr)
+            for (int k = 0; k < 2; k++) {
+              const int r = (warp & 3) * 32 + r0 + 4 * k + (lane >> 3), gr = first_row + r;
+              const int tk = quotient(gr, a.tiling.by_group), at_pos = p.r.len - p.r.n + tk;
+              const bool some = r < rows;
+              const T* src = static_cast<const T*>(a.q) + (p.r.first + tk) * a.q_stride +
+                             (int64_t)(p.h * group + gr - tk * group) * dim;
+              const int64_t tab = some && a.rope.cos != nullptr && at_pos >= 0
+                                      ? rope_row(a.rope, at_pos, a.batch.status) * (dim / 2) : -1;
 #pragma unroll
-                for (int i = 0; i < 8; i += 2) {
-                  float x0 = to_f32<T>(u.x[i]), x1 = to_f32<T>(u.x[i + 1]);
-                  rotate(x0, x1, __ldg(ct + (d + i) / 2), __ldg(st + (d + i) / 2));
-                  u.x[i] = from_f32<T>(x0);
-                  u.x[i + 1] = from_f32<T>(x1);
+              for (int i = 0; i < P; i++) {
+                const int d = 8 * ((lane & 7) + 8 * i);
+                u[k][i].v = make_uint4(0, 0, 0, 0);
+                cs[k][i] = make_float4(1.f, 1.f, 1.f, 1.f);
+                sn[k][i] = make_float4(0.f, 0.f, 0.f, 0.f);
+                if (some && d < dim) {
+                  if (q_vec) u[k][i].v = __ldg(reinterpret_cast<const uint4*>(src + d));
+                  else
+#pragma unroll
+                    for (int e = 0; e < 8; e++) u[k][i].x[e] = src[d + e];
+                  if (tab >= 0) {
+                    const float *ct = a.rope.cos + tab + d / 2, *st = a.rope.sin + tab + d / 2;
+                    if (rope_vec) {
+                      cs[k][i] = __ldg(reinterpret_cast<const float4*>(ct));
+                      sn[k][i] = __ldg(reinterpret_cast<const float4*>(st));
+                    } else {
+                      cs[k][i] = make_float4(__ldg(ct), __ldg(ct + 1), __ldg(ct + 2), __ldg(ct + 3));
+                      sn[k][i] = make_float4(__ldg(st), __ldg(st + 1), __ldg(st + 2), __ldg(st + 3));
+                    }
+                  }
                 }
+              }
             }
-            const uint32_t piece = (uint32_t)(d >> 3) & 7u;
-            const float4 f = *reinterpret_cast<const float4*>(&u.v);
-            sts128(q_row + (uint32_t)(d >> 6) * HALF * 128u + ((piece ^ (uint32_t)(row & 7)) << 4), f);
+#pragma unroll
+            for (int k = 0; k < 2; k++) {
+              const int r = (warp & 3) * 32 + r0 + 4 * k + (lane >> 3);
+#pragma unroll
+              for (int i = 0; i < P; i++) {
+                const int c = (lane & 7) + 8 * i;
+                if (a.rope.cos != nullptr) {
+                  const float cc[4] = {cs[k][i].x, cs[k][i].y, cs[k][i].z, cs[k][i].w};
+                  const float ss[4] = {sn[k][i].x, sn[k][i].y, sn[k][i].z, sn[k][i].w};
+#pragma unroll
+                  for (int e = 0; e < 4; e++) {
+                    float x0 = to_f32<T>(u[k][i].x[2 * e]), x1 = to_f32<T>(u[k][i].x[2 * e + 1]);
+                    rotate(x0, x1, cc[e], ss[e]);
+                    u[k][i].x[2 * e] = from_f32<T>(x0);
+                    u[k][i].x[2 * e + 1] = from_f32<T>(x1);
+                  }
+                }
+                sts128(tile + (uint32_t)(c >> 3) * HALF * 128u + (uint32_t)r * 128u +
+                           ((((uint32_t)c & 7u) ^ (uint32_t)(r & 7)) << 4),
+                       *reinterpret_cast<const float4*>(&u[k][i].v));
+              }
+            }
           }
           fence_async_smem();
           tc_fence_before();
