@@ -13,8 +13,8 @@
 //
 // A tile is 128 rows (TMEM lanes), a block 64 keys.  Warp 10 copies raw K and V
 // tiles by TMA, warps 4-7 turn them into pairs (a row by DH / 4 lanes: maximum,
-// exponent, split) in shared memory, warp 8 issues S = Q K^T of block j + 1,
-// then O += P V of block j, warps 0-3 (one row per thread) form the
+// exponent, split) in shared memory, warp 8 issues S = Q K^T up to a block ahead
+// of warp 9's O += P V, warps 0-3 (one row per thread) form the
 // probabilities, whose pair replaces the scores in TMEM.  P hi times
 // [V hi | V lo] is one product of N = 2 head_dim; the halves of O are added
 // when it is read.  The tensor pipe's f32 accumulation truncates, so every
@@ -74,7 +74,7 @@ paged_attention_f32_kernel(const __grid_constant__ CUtensorMap k_map,
   uint64_t* bars = reinterpret_cast<uint64_t*>(smem + L::BARS);
   enum {
     RAWFULL = 0, RAWEMPTY = 6, CONVFULL = 12, CONVEMPTY = 14, SFULL = 16, PREADY = 18, PVDONE = 20,
-    QREADY = 22, DRAIN = 23, NBARS
+    QREADY = 22, DRAIN = 23, NBARS = 25
   };
   const uint32_t bar0 = smem_u32(bars);
   auto B_ = [&](int i) { return bar0 + 8u * (uint32_t)i; };
@@ -151,60 +151,67 @@ paged_attention_f32_kernel(const __grid_constant__ CUtensorMap k_map,
       for (uint32_t c = count > L::RAWS ? count - L::RAWS : 0; c < count; c++)
         mbar_wait(B_(RAWFULL + c % L::RAWS), (c / L::RAWS) & 1u, &g_wait_error);
   } else if (warp == MMA_WARP) {
-    // ---- products
-    constexpr uint32_t idesc_s = idesc_f16_m128(BK, 0), idesc_o = idesc_f16_m128(DH, 1),
-                       idesc_o2 = idesc_f16_m128(2 * DH, 1);
+    // ---- S = Q K^T, up to a block ahead of P V
+    constexpr uint32_t idesc_s = idesc_f16_m128(BK, 0);
     uint32_t items = 0;
     bool ok = true;
-    auto scores = [&](uint32_t m) {
-      const uint32_t k = base + L::CONV + (m & 1u) * L::PAIRS, d = tmem + L::S0 + 64u * (m & 1u);
-#pragma unroll
-      for (int i = 0; i < DH / 16; i++) {
-        const uint64_t kh = kdesc16<BK>(k, i);
-        umma_f16(d, kdesc16<ROWS>(base + L::QLO, i), kh, idesc_s, i > 0 ? 1u : 0u);
-        umma_f16_ts(d, tmem + L::QH + 8u * i, kdesc16<BK>(k + L::KT, i), idesc_s, 1u);
-        umma_f16_ts(d, tmem + L::QH + 8u * i, kh, idesc_s, 1u);
-      }
-      umma_commit(B_(SFULL + (int)(m & 1u)));
-    };
     while (ok && left > 0) {
       const int nb = blocks_here();
-      ok = wait(QREADY, items);
-      if (ok) ok = wait(CONVFULL + (n & 1u), n >> 1);
-      ok = __all_sync(0xffffffffu, ok);
-      if (!ok) break;
-      tc_fence_after();
-      if (lane == 0) scores(n);
+      ok = wait(QREADY, items++);
       for (int j = 0; j < nb; j++, n++) {
-        const bool more = j + 1 < nb;
-        if (more) {
-          ok = __all_sync(0xffffffffu, wait(CONVFULL + ((n + 1) & 1u), (n + 1) >> 1));
-          if (!ok) break;
-          tc_fence_after();
-          if (lane == 0) scores(n + 1);
-        }
-        ok = __all_sync(0xffffffffu, wait(PREADY + (n & 1u), n >> 1));
+        const uint32_t slot = n & 1u;
+        if (ok) ok = wait(CONVFULL + slot, n >> 1);
+        if (ok && n >= 2) ok = wait(PVDONE + slot, (n >> 1) - 1);  // the slot held P of block n - 2
+        ok = __all_sync(0xffffffffu, ok);
         if (!ok) break;
         tc_fence_after();
         if (lane == 0) {
-          const uint32_t v = base + L::CONV + (n & 1u) * L::PAIRS + 2u * L::KT;
-          const uint32_t pa = tmem + L::S0 + 64u * (n & 1u);
+          const uint32_t k = base + L::CONV + slot * L::PAIRS, d = tmem + L::S0 + 64u * slot;
+#pragma unroll
+          for (int i = 0; i < DH / 16; i++) {
+            const uint64_t kh = kdesc16<BK>(k, i);
+            umma_f16(d, kdesc16<ROWS>(base + L::QLO, i), kh, idesc_s, i > 0 ? 1u : 0u);
+            umma_f16_ts(d, tmem + L::QH + 8u * i, kdesc16<BK>(k + L::KT, i), idesc_s, 1u);
+            umma_f16_ts(d, tmem + L::QH + 8u * i, kh, idesc_s, 1u);
+          }
+          umma_commit(B_(SFULL + (int)slot));
+        }
+      }
+      next_tile(nb);
+    }
+    if (lane == 0) {
+      umma_commit(B_(DRAIN));
+      mbar_wait(B_(DRAIN), 0u, &g_wait_error);
+    }
+  } else if (warp == MMA_WARP + 1) {
+    // ---- O += P V
+    constexpr uint32_t idesc_o = idesc_f16_m128(DH, 1), idesc_o2 = idesc_f16_m128(2 * DH, 1);
+    bool ok = true;
+    while (ok && left > 0) {
+      const int nb = blocks_here();
+      for (int j = 0; j < nb; j++, n++) {
+        const uint32_t slot = n & 1u;
+        ok = __all_sync(0xffffffffu, wait(PREADY + slot, n >> 1));
+        if (!ok) break;
+        tc_fence_after();
+        if (lane == 0) {
+          const uint32_t v = base + L::CONV + slot * L::PAIRS + 2u * L::KT;
+          const uint32_t pa = tmem + L::S0 + 64u * slot;
 #pragma unroll
           for (int i = 0; i < BK / 16; i++) {
             const uint64_t vd = mdesc16<BK>(v, i);  // V lo lies one chunk stride behind V hi
             umma_f16_ts(tmem + L::O, pa + 8u * i, vd, idesc_o2, (j % CHUNK != 0 || i > 0) ? 1u : 0u);
             umma_f16_ts(tmem + L::O, pa + 32u + 8u * i, vd, idesc_o, 1u);
           }
-          umma_commit(B_(PVDONE + (int)(n & 1u)));
-          umma_commit(B_(CONVEMPTY + (int)(n & 1u)));
+          umma_commit(B_(PVDONE + (int)slot));
+          umma_commit(B_(CONVEMPTY + (int)slot));
         }
       }
-      items++;
       next_tile(nb);
     }
     if (lane == 0) {
-      umma_commit(B_(DRAIN));
-      mbar_wait(B_(DRAIN), 0u, &g_wait_error);
+      umma_commit(B_(DRAIN + 1));
+      mbar_wait(B_(DRAIN + 1), 0u, &g_wait_error);
     }
   } else if (warp >= CONVERT_WARP && warp < MMA_WARP) {
     // ---- raw rows into pairs; warp w takes rows w RW, w RW + 1, ... of each 4 RW
@@ -219,42 +226,48 @@ paged_attention_f32_kernel(const __grid_constant__ CUtensorMap k_map,
         const uint32_t conv = base + L::CONV + (n & 1u) * L::PAIRS;
         float* f = factors + (n & 1u) * 3 * BK;
         if (n >= 2) ok = wait(CONVEMPTY + (n & 1u), (n >> 1) - 1);
-        for (int kv = 0; kv < 2 && ok; kv++) {
-          const uint32_t s = count % L::RAWS;
-          ok = wait(RAWFULL + s, count / L::RAWS);
-          if (!ok) break;
-          count++;
-          const uint32_t raw = base + s * L::RAW, hi = conv + (uint32_t)kv * 2u * L::KT;
-          // 8 rows of a lane group at once: loads, then maxima, then stores
-          constexpr int STEP = 4 * RW, AT_ONCE = 8;
+        const uint32_t sk = count % L::RAWS, sv = (count + 1) % L::RAWS;
+        if (ok) ok = wait(RAWFULL + sk, count / L::RAWS);
+        if (ok) ok = wait(RAWFULL + sv, (count + 1) / L::RAWS);
+        count += 2;
+        // rows of both tiles at once: loads, then maxima, then stores
+        constexpr int STEP = 4 * RW, AT_ONCE = 4;
+#pragma unroll 1
+        for (int r0 = 0; r0 < BK && ok; r0 += AT_ONCE * STEP) {
+          const int row0 = r0 + (warp - CONVERT_WARP) * RW + sub;
+          float4 x[2][AT_ONCE];
+          float m[2][AT_ONCE];
 #pragma unroll
-          for (int r0 = 0; r0 < BK; r0 += AT_ONCE * STEP) {
-            const int row0 = r0 + (warp - CONVERT_WARP) * RW + sub;
-            float4 x[AT_ONCE];
-            float m[AT_ONCE];
+          for (int kv = 0; kv < 2; kv++)
 #pragma unroll
             for (int k = 0; k < AT_ONCE; k++) {
               const int row = row0 + k * STEP;
-              x[k] = make_float4(0.f, 0.f, 0.f, 0.f);
-              if (row < valid) x[k] = lds128(raw + (uint32_t)(row * DH + 4 * col) * 4u);
-              m[k] = abs_max4(0.0f, x[k]);
+              x[kv][k] = make_float4(0.f, 0.f, 0.f, 0.f);
+              if (row < valid)
+                x[kv][k] = lds128(base + (kv == 0 ? sk : sv) * L::RAW + (uint32_t)(row * DH + 4 * col) * 4u);
+              m[kv][k] = abs_max4(0.0f, x[kv][k]);
             }
 #pragma unroll
-            for (int o = LANES / 2; o > 0; o >>= 1)
+          for (int o = LANES / 2; o > 0; o >>= 1)
 #pragma unroll
-              for (int k = 0; k < AT_ONCE; k++) m[k] = fmaxf(m[k], __shfl_xor_sync(0xffffffffu, m[k], o));
+            for (int i = 0; i < 2 * AT_ONCE; i++)
+              m[i & 1][i >> 1] = fmaxf(m[i & 1][i >> 1], __shfl_xor_sync(0xffffffffu, m[i & 1][i >> 1], o));
 #pragma unroll
-            for (int k = 0; k < AT_ONCE; k++) {
-              const int row = row0 + k * STEP, e = row_exponent(m[k]);
+          for (int k = 0; k < AT_ONCE; k++) {
+            const int row = row0 + k * STEP;
+            const uint32_t piece = ((uint32_t)col & 15u) >> 1;
+            const uint32_t at = conv + (uint32_t)(col >> 4) * BK * 128u + (uint32_t)row * 128u +
+                                ((piece ^ (uint32_t)(row & 7)) << 4) + (uint32_t)(col & 1) * 8u;
+#pragma unroll
+            for (int kv = 0; kv < 2; kv++) {
+              const int e = row_exponent(m[kv][k]);
               const float sc = exp2_int(e);
               float h0, l0, h1, l1;
-              pair2(x[k].x * sc, x[k].y * sc, h0, l0);
-              pair2(x[k].z * sc, x[k].w * sc, h1, l1);
-              const uint32_t piece = ((uint32_t)col & 15u) >> 1;
-              const uint32_t at = hi + (uint32_t)(col >> 4) * BK * 128u + (uint32_t)row * 128u +
-                                  ((piece ^ (uint32_t)(row & 7)) << 4) + (uint32_t)(col & 1) * 8u;
-              asm volatile("st.shared.v2.f32 [%0], {%1, %2};" ::"r"(at), "f"(h0), "f"(h1) : "memory");
-              asm volatile("st.shared.v2.f32 [%0], {%1, %2};" ::"r"(at + L::KT), "f"(l0), "f"(l1)
+              pair2(x[kv][k].x * sc, x[kv][k].y * sc, h0, l0);
+              pair2(x[kv][k].z * sc, x[kv][k].w * sc, h1, l1);
+              const uint32_t to = at + (uint32_t)kv * 2u * L::KT;
+              asm volatile("st.shared.v2.f32 [%0], {%1, %2};" ::"r"(to), "f"(h0), "f"(h1) : "memory");
+              asm volatile("st.shared.v2.f32 [%0], {%1, %2};" ::"r"(to + L::KT), "f"(l0), "f"(l1)
                            : "memory");
               if (col == 0) {
                 if (kv == 0) {
@@ -266,8 +279,11 @@ paged_attention_f32_kernel(const __grid_constant__ CUtensorMap k_map,
               }
             }
           }
-          __syncwarp();
-          if (lane == 0) mbar_arrive(B_(RAWEMPTY + s));
+        }
+        __syncwarp();
+        if (ok && lane == 0) {
+          mbar_arrive(B_(RAWEMPTY + sk));
+          mbar_arrive(B_(RAWEMPTY + sv));
         }
         ok = __all_sync(0xffffffffu, ok);
         if (!ok) break;
@@ -282,6 +298,7 @@ paged_attention_f32_kernel(const __grid_constant__ CUtensorMap k_map,
     const int row = tid;
     const uint32_t lanes = tmem + ((uint32_t)(warp * 32) << 16);
     const bool q_vec = ((reinterpret_cast<uintptr_t>(a.q) | (uintptr_t)(a.q_stride * 4)) & 15) == 0;
+    const bool rope_vec = ((reinterpret_cast<uintptr_t>(a.rope.cos) | reinterpret_cast<uintptr_t>(a.rope.sin)) & 7) == 0;
     const bool o_vec = ((reinterpret_cast<uintptr_t>(a.o) | (uintptr_t)(a.o_stride * 4)) & 15) == 0;
     bool ok = true;
     Cut cut{0, 0, 0, 0, 0};
@@ -304,73 +321,80 @@ paged_attention_f32_kernel(const __grid_constant__ CUtensorMap k_map,
       {
         constexpr int P = DH / 32;  // 16-byte pieces of a lane
         const uint32_t tile = base + L::QLO;
+        constexpr int G = DH == 128 ? 2 : 4;  // groups of 4 rows whose loads are in flight
+        auto unit_at = [&](int r, int i) {
+          const int c = (lane & 7) + 8 * i;  // 8-byte unit of the row
+          return tile + (uint32_t)(c >> 4) * ROWS * 128u + (uint32_t)r * 128u +
+                 (((((uint32_t)c & 15u) >> 1) ^ (uint32_t)(r & 7)) << 4) + (uint32_t)(c & 1) * 8u;
+        };
 #pragma unroll 1
-        for (int half = 0; half < 2; half++) {
-          for (int r0 = 0; r0 < 32; r0 += 8) {
-            float4 x[2][P], cs[2][P];
-            float sc[2];
+        for (int pass = 0; pass < 16; pass += G) {
+        const int g0 = pass & 7;
+        if (pass == 8) {  // hi is complete
+          __syncwarp();
+          tile_row16_to_tmem<DH>(tile, row, lanes, L::QH);
+          tmem_wait_st();
+          __syncwarp();
+        }
+          float4 x[G][P];
+          float2 cs[G][P], sn[G][P];
 #pragma unroll
-            for (int k = 0; k < 2; k++) {
-              const int r = warp * 32 + r0 + 4 * k + (lane >> 3), gr = p.tile * ROWS + r;
-              const int t = quotient(gr, a.tiling.by_group), at_pos = p.r.len - p.r.n + t;
-              const bool some = r < rows;
-              const float* src = static_cast<const float*>(a.q) + (p.r.first + t) * a.q_stride +
-                                 (int64_t)(p.h * group + gr - t * group) * dim;
-              const int64_t tab = some && a.rope.cos != nullptr && at_pos >= 0
-                                      ? rope_row(a.rope, at_pos, a.batch.status) * (dim / 2) : -1;
+          for (int k = 0; k < G; k++) {
+            const int r = warp * 32 + 4 * (g0 + k) + (lane >> 3), gr = p.tile * ROWS + r;
+            const int t = quotient(gr, a.tiling.by_group), at_pos = p.r.len - p.r.n + t;
+            const bool some = r < rows;
+            const float* src = static_cast<const float*>(a.q) + (p.r.first + t) * a.q_stride +
+                               (int64_t)(p.h * group + gr - t * group) * dim;
+            const int64_t tab = some && a.rope.cos != nullptr && at_pos >= 0
+                                    ? rope_row(a.rope, at_pos, a.batch.status) * (dim / 2) : -1;
 #pragma unroll
-              for (int i = 0; i < P; i++) {
-                const int d = 4 * ((lane & 7) + 8 * i);
-                x[k][i] = make_float4(0.f, 0.f, 0.f, 0.f);
-                cs[k][i] = make_float4(1.f, 0.f, 1.f, 0.f);
-                if (some && d < dim) {
-                  if (q_vec) x[k][i] = __ldg(reinterpret_cast<const float4*>(src + d));
-                  else x[k][i] = make_float4(__ldg(src + d), __ldg(src + d + 1), __ldg(src + d + 2), __ldg(src + d + 3));
-                  if (tab >= 0)
-                    cs[k][i] = make_float4(__ldg(a.rope.cos + tab + d / 2), __ldg(a.rope.sin + tab + d / 2),
-                                           __ldg(a.rope.cos + tab + d / 2 + 1), __ldg(a.rope.sin + tab + d / 2 + 1));
+            for (int i = 0; i < P; i++) {
+              const int d = 4 * ((lane & 7) + 8 * i);
+              x[k][i] = make_float4(0.f, 0.f, 0.f, 0.f);
+              cs[k][i] = make_float2(1.f, 1.f);
+              sn[k][i] = make_float2(0.f, 0.f);
+              if (some && d < dim) {
+                if (q_vec) x[k][i] = __ldg(reinterpret_cast<const float4*>(src + d));
+                else x[k][i] = make_float4(__ldg(src + d), __ldg(src + d + 1), __ldg(src + d + 2), __ldg(src + d + 3));
+                if (tab >= 0) {
+                  const float *ct = a.rope.cos + tab + d / 2, *st = a.rope.sin + tab + d / 2;
+                  if (rope_vec) {
+                    cs[k][i] = __ldg(reinterpret_cast<const float2*>(ct));
+                    sn[k][i] = __ldg(reinterpret_cast<const float2*>(st));
+                  } else {
+                    cs[k][i] = make_float2(__ldg(ct), __ldg(ct + 1));
+                    sn[k][i] = make_float2(__ldg(st), __ldg(st + 1));
+                  }
                 }
-              }
-            }
-#pragma unroll
-            for (int k = 0; k < 2; k++) {
-              float m = 0.0f;
-#pragma unroll
-              for (int i = 0; i < P; i++) m = abs_max4(m, x[k][i]);
-#pragma unroll
-              for (int o = 4; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
-              // a rotated pair is at most sqrt(2) times its larger element: below 2^14.5
-              const int e = row_exponent(m);
-              sc[k] = exp2_int(e);
-              const int mine = __shfl_sync(0xffffffffu, e, (lane & 3) * 8);
-              if ((lane >> 2) == (r0 >> 2) + k) cq = a.scale_log2 * exp2_int(-mine);
-            }
-#pragma unroll
-            for (int k = 0; k < 2; k++) {
-              const int r = warp * 32 + r0 + 4 * k + (lane >> 3);
-#pragma unroll
-              for (int i = 0; i < P; i++) {
-                float4 v = x[k][i];
-                if (a.rope.cos != nullptr) {
-                  rotate(v.x, v.y, cs[k][i].x, cs[k][i].y);
-                  rotate(v.z, v.w, cs[k][i].z, cs[k][i].w);
-                }
-                float h0, l0, h1, l1;
-                pair2(v.x * sc[k], v.y * sc[k], h0, l0);
-                pair2(v.z * sc[k], v.w * sc[k], h1, l1);
-                const int c = (lane & 7) + 8 * i;  // 8-byte unit of the row
-                const uint32_t at = tile + (uint32_t)(c >> 4) * ROWS * 128u + (uint32_t)r * 128u +
-                                    ((((uint32_t)c & 15u) >> 1 ^ (uint32_t)(r & 7)) << 4) + (uint32_t)(c & 1) * 8u;
-                asm volatile("st.shared.v2.f32 [%0], {%1, %2};" ::"r"(at), "f"(half ? l0 : h0),
-                             "f"(half ? l1 : h1) : "memory");
               }
             }
           }
-          __syncwarp();
-          if (half == 0) {
-            tile_row16_to_tmem<DH>(tile, row, lanes, L::QH);
-            tmem_wait_st();
-            __syncwarp();
+#pragma unroll
+          for (int k = 0; k < G; k++) {
+            const int r = warp * 32 + 4 * (g0 + k) + (lane >> 3);
+            float m = 0.0f;
+#pragma unroll
+            for (int i = 0; i < P; i++) m = abs_max4(m, x[k][i]);
+#pragma unroll
+            for (int o = 4; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
+            // a rotated pair is at most sqrt(2) times its larger element: below 2^14.5
+            const int e = row_exponent(m);
+            const float sc = exp2_int(e);
+            const int mine = __shfl_sync(0xffffffffu, e, (lane & 3) * 8);
+            if ((lane >> 2) == g0 + k) cq = a.scale_log2 * exp2_int(-mine);
+#pragma unroll
+            for (int i = 0; i < P; i++) {
+              float4 v = x[k][i];
+              if (a.rope.cos != nullptr) {
+                rotate(v.x, v.y, cs[k][i].x, sn[k][i].x);
+                rotate(v.z, v.w, cs[k][i].y, sn[k][i].y);
+              }
+              float h0, l0, h1, l1;
+              pair2(v.x * sc, v.y * sc, h0, l0);
+              pair2(v.z * sc, v.w * sc, h1, l1);
+              asm volatile("st.shared.v2.f32 [%0], {%1, %2};" ::"r"(unit_at(r, i)),
+                           "f"(pass < 8 ? h0 : l0), "f"(pass < 8 ? h1 : l1) : "memory");
+            }
           }
         }
         fence_async_smem();
@@ -406,7 +430,7 @@ paged_attention_f32_kernel(const __grid_constant__ CUtensorMap k_map,
           ok = __all_sync(0xffffffffu, wait(PVDONE + ((n - 1) & 1u), (n - 1) >> 1));
           if (!ok) break;
           tc_fence_after();
-#pragma unroll
+#pragma unroll 1
           for (int c = 0; c < DH / 32; c++) {
             float v[32];
             read_o(c, v);
@@ -421,30 +445,36 @@ paged_attention_f32_kernel(const __grid_constant__ CUtensorMap k_map,
         if (!ok) break;
         tc_fence_after();
         const uint32_t s_at = lanes + L::S0 + 64u * (n & 1u);
-        uint32_t r[2][32];
-        tmem_ld32_nowait(s_at, r[0]);
-        tmem_ld32_nowait(s_at + 32, r[1]);
-        tmem_wait_ld_pin<true>(r[0]);
-        tmem_wait_ld_pin<false>(r[1]);
         const int key0 = (p.blk + j) * BK;
         const bool masked = key0 + BK > vis_warp;
         const int seen = vis - key0;
         const uint32_t f_at = smem_u32(factors + (n & 1u) * 3 * BK);
-        float s[64], top[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+        // scores of 32 keys in base 2, exponents of their values added; computed for
+        // the maximum and again for the weights: half the code of keeping all 64
+        // (instruction fetches were a quarter of this kernel's stalls)
+        auto scores = [&](int c, float (&s)[32]) {
+          tmem_ld32(s_at + 32u * c, s);
 #pragma unroll
-        for (int i = 0; i < 64; i += 4) {
-          const float4 kf = lds128(f_at + 4u * i), ge = lds128(f_at + 4u * (BK + i));
-          s[i] = fmaf(__uint_as_float(r[i >> 5][i & 31]) * cq, kf.x, ge.x);
-          s[i + 1] = fmaf(__uint_as_float(r[i >> 5][(i & 31) + 1]) * cq, kf.y, ge.y);
-          s[i + 2] = fmaf(__uint_as_float(r[i >> 5][(i & 31) + 2]) * cq, kf.z, ge.z);
-          s[i + 3] = fmaf(__uint_as_float(r[i >> 5][(i & 31) + 3]) * cq, kf.w, ge.w);
+          for (int i = 0; i < 32; i += 4) {
+            const float4 kf = lds128(f_at + 4u * (32 * c + i)), ge = lds128(f_at + 4u * (BK + 32 * c + i));
+            s[i] = fmaf(s[i] * cq, kf.x, ge.x);
+            s[i + 1] = fmaf(s[i + 1] * cq, kf.y, ge.y);
+            s[i + 2] = fmaf(s[i + 2] * cq, kf.z, ge.z);
+            s[i + 3] = fmaf(s[i + 3] * cq, kf.w, ge.w);
+          }
           if (masked) {
 #pragma unroll
-            for (int k = 0; k < 4; k++)
-              if (i + k >= seen) s[i + k] = -INFINITY;
+            for (int i = 0; i < 32; i++)
+              if (32 * c + i >= seen) s[i] = -INFINITY;
           }
+        };
+        float top[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+#pragma unroll 1
+        for (int c = 0; c < 2; c++) {
+          float s[32];
+          scores(c, s);
 #pragma unroll
-          for (int k = 0; k < 4; k++) top[k] = fmaxf(top[k], s[i + k]);
+          for (int i = 0; i < 32; i++) top[i & 3] = fmaxf(top[i & 3], s[i]);
         }
         const float bmax = fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3]));
         const bool jump = bmax > m + kJump;
@@ -458,7 +488,7 @@ paged_attention_f32_kernel(const __grid_constant__ CUtensorMap k_map,
             ok = __all_sync(0xffffffffu, wait(PVDONE + ((n - 1) & 1u), (n - 1) >> 1));
             if (!ok) break;
             tc_fence_after();
-#pragma unroll
+#pragma unroll 1
             for (int c = 0; c < 2 * DH / 32; c++) {
               float o[32];
               tmem_ld32(lanes + L::O + 32u * c, o);
@@ -469,24 +499,38 @@ paged_attention_f32_kernel(const __grid_constant__ CUtensorMap k_map,
           }
         }
         const float from = (m == -INFINITY ? 0.0f : m) - kShift;
-#pragma unroll
+        float sum[4] = {0.f, 0.f, 0.f, 0.f};
+        // the pairs of the first 32 keys wait in registers: they replace scores that
+        // the second pass still reads
+        float hi[16], lo[16], hi0[16], lo0[16];
+#pragma unroll 1
         for (int c = 0; c < 2; c++) {
-          float hi[16], lo[16];
+          float s[32];
+          scores(c, s);
 #pragma unroll
           for (int i = 0; i < 32; i += 4) {
             const float4 vf = lds128(f_at + 4u * (2 * BK + 32 * c + i));
-            const float w0 = ex2(s[32 * c + i] - from), w1 = ex2(s[32 * c + i + 1] - from);
-            const float w2 = ex2(s[32 * c + i + 2] - from), w3 = ex2(s[32 * c + i + 3] - from);
-            l = fmaf(w0, vf.x, l);
-            l = fmaf(w1, vf.y, l);
-            l = fmaf(w2, vf.z, l);
-            l = fmaf(w3, vf.w, l);
+            const float w0 = ex2(s[i] - from), w1 = ex2(s[i + 1] - from);
+            const float w2 = ex2(s[i + 2] - from), w3 = ex2(s[i + 3] - from);
+            sum[0] = fmaf(w0, vf.x, sum[0]);
+            sum[1] = fmaf(w1, vf.y, sum[1]);
+            sum[2] = fmaf(w2, vf.z, sum[2]);
+            sum[3] = fmaf(w3, vf.w, sum[3]);
             pair2(w0, w1, hi[i / 2], lo[i / 2]);
             pair2(w2, w3, hi[i / 2 + 1], lo[i / 2 + 1]);
           }
-          tmem_st16(s_at + 16u * c, hi);
-          tmem_st16(s_at + 32u + 16u * c, lo);
+          if (c == 0)
+#pragma unroll
+            for (int i = 0; i < 16; i++) {
+              hi0[i] = hi[i];
+              lo0[i] = lo[i];
+            }
         }
+        tmem_st16(s_at, hi0);
+        tmem_st16(s_at + 32u, lo0);
+        tmem_st16(s_at + 16u, hi);
+        tmem_st16(s_at + 48u, lo);
+        l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
         tmem_wait_st();
         tc_fence_before();
         mbar_arrive(B_(PREADY + (n & 1u)));
@@ -497,7 +541,7 @@ paged_attention_f32_kernel(const __grid_constant__ CUtensorMap k_map,
         const float inv = l > 0.0f ? 1.0f / l : 0.0f;
         float* dst = static_cast<float*>(a.o) + (p.r.first + token) * a.o_stride + (int64_t)head * dim;
         const int slot = 2 * (int)blockIdx.x + (whole ? 1 : 0);
-#pragma unroll
+#pragma unroll 1
         for (int c = 0; c < DH / 32; c++) {
           float o[32];
           read_o(c, o);
