@@ -123,6 +123,11 @@ __device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
   asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
   return r;
 }
+__device__ __forceinline__ uint64_t mul2(uint64_t a, uint64_t b) {
+  uint64_t r;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
 __device__ __forceinline__ uint64_t twice(float a) { return pk(a, a); }
 
 // RoPE of the pair (x0, x1) in the reference's rounding order
@@ -209,10 +214,17 @@ struct Share {
 // This block's share of the units and where it begins; every thread of the
 // NT-thread block calls it and gets the same.
 template <int NT>
-__device__ Share divide(const Tiling& t, const Batch& B, int64_t least, Place& p) {
-  __shared__ int64_t warp_sum_s[NT / 32];
-  __shared__ int64_t found_s[2];
-  __shared__ Request request_s;
+struct DivideRoom {  // shared memory
+  int64_t warp_sum[NT / 32];
+  int64_t found[2];
+  Request request;
+};
+template <int NT>
+__device__ Share divide(const Tiling& t, const Batch& B, int64_t least, Place& p,
+                        DivideRoom<NT>& room) {
+  int64_t* warp_sum_s = room.warp_sum;
+  int64_t* found_s = room.found;
+  Request& request_s = room.request;
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   Request mine_r{0, 0, 0, 0};
   int64_t per_head = 0;

@@ -186,7 +186,8 @@ paged_attention_kernel(const __grid_constant__ CUtensorMap k_map,
   }
 
   Place p;
-  const Share share = divide<NT + (TMA ? 32 : 0)>(a.tiling, a.batch, a.least, p);
+  __shared__ DivideRoom<NT + (TMA ? 32 : 0)> room;
+  const Share share = divide(a.tiling, a.batch, a.least, p, room);
   __syncthreads();
   if (TMA && warp == NT / 32) {
     // ---- the copying warp

@@ -11,11 +11,13 @@
 // M the running maximum of s_j + g_j, so cached rows of any magnitude need no
 // pass of their own.
 //
-// A tile is 128 rows (TMEM lanes), a block 64 keys.  Warp 10 copies raw K and V
-// tiles by TMA, warps 4-7 turn them into pairs (a row by DH / 4 lanes: maximum,
-// exponent, split) in shared memory, warp 8 issues S = Q K^T up to a block ahead
-// of warp 9's O += P V, warps 0-3 (one row per thread) form the
-// probabilities, whose pair replaces the scores in TMEM.  P hi times
+// A tile is 128 rows (TMEM lanes), a block 64 keys.  Warp 18 copies raw K and V
+// tiles by TMA, warps 8-15 turn them into pairs (a row by DH / 4 lanes: maximum,
+// exponent, split) in shared memory, warp 16 issues S = Q K^T up to a block ahead
+// of warp 17's O += P V, warps 0-7 (two threads per row, 32 keys each) form the
+// probabilities, whose pair replaces the scores in TMEM.  A single warp per
+// scheduler issues an instruction of such code every five or six cycles, so both
+// kinds of arithmetic have two.  P hi times
 // [V hi | V lo] is one product of N = 2 head_dim; the halves of O are added
 // when it is read.  The tensor pipe's f32 accumulation truncates, so every
 // CHUNK blocks O moves to f32 sums in the workspace (each thread its row).
@@ -34,7 +36,10 @@ using namespace paged;
 using namespace f16att;
 
 constexpr int ROWS = 128, BK = 64;
-constexpr int CONVERT_WARP = 4, MMA_WARP = 8, LOAD_WARP = 10, THREADS = 384;
+constexpr int SOFT = 256, CONVERT_WARP = 8, MMA_WARP = 16, LOAD_WARP = 18, THREADS = 640;
+// registers of the warpgroups: probabilities, conversion, the rest
+constexpr int kSoftRegs = 120, kConvertRegs = 88, kLeanRegs = 64;
+static_assert(256 * kSoftRegs + 256 * kConvertRegs + 128 * kLeanRegs <= THREADS * 96, "registers at launch");
 constexpr float kJump = 8.0f;   // log2 of the largest P the standing maximum allows
 constexpr float kShift = 7.0f;  // P carries 2^7: at most 2^15
 constexpr int CHUNK = 8;        // blocks whose products one TMEM accumulator adds
@@ -50,8 +55,9 @@ struct Layout {
   static constexpr int CONV = RAWS * RAW;
   static constexpr int QLO = CONV + 2 * PAIRS;
   static constexpr int FACTORS = QLO + ROWS * DH * 2;  // [2][3][BK]: of K, exponents and factors of V
-  static constexpr int BARS = FACTORS + 2 * 3 * BK * 4;
-  static constexpr int SMEM = BARS + 256 + 1024;
+  static constexpr int SHARED_ROWS = FACTORS + 2 * 3 * BK * 4;  // what a row's threads exchange
+  static constexpr int BARS = SHARED_ROWS + 1024;
+  static constexpr int SMEM = BARS + 216;
   static constexpr uint32_t S0 = 0, QH = 128, O = 192, COLS = 512;
   static_assert(O + 2 * DH <= COLS && QH + DH / 2 <= O && SMEM <= 232448, "TMEM and shared memory");
 };
@@ -67,9 +73,7 @@ __global__ void __launch_bounds__(THREADS, 1)
 paged_attention_f32_kernel(const __grid_constant__ CUtensorMap k_map,
                            const __grid_constant__ CUtensorMap v_map, AttendArgs a, int box_rows) {
   using L = Layout<DH>;
-  extern __shared__ uint8_t smem_raw[];
-  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) &
-                                             ~(uintptr_t)1023);
+  extern __shared__ __align__(1024) uint8_t smem[];
   float* factors = reinterpret_cast<float*>(smem + L::FACTORS);
   uint64_t* bars = reinterpret_cast<uint64_t*>(smem + L::BARS);
   enum {
@@ -87,14 +91,15 @@ paged_attention_f32_kernel(const __grid_constant__ CUtensorMap k_map,
 
   if (tid == 0) {
     for (int i = 0; i < NBARS; i++)
-      mbar_init(B_(i), (i >= RAWEMPTY && i < CONVEMPTY) ? 4
-                       : (i == PREADY || i == PREADY + 1 || i == QREADY) ? ROWS : 1);
+      mbar_init(B_(i), (i >= RAWEMPTY && i < CONVEMPTY) ? MMA_WARP - CONVERT_WARP
+                       : (i == PREADY || i == PREADY + 1 || i == QREADY) ? SOFT : 1);
     *abort = 0;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
   if (warp == MMA_WARP) tmem_alloc(smem_u32(tslot), L::COLS);
   Place p;
-  const Share share = divide<THREADS>(a.tiling, a.batch, a.least, p);
+  const Share share = divide(a.tiling, a.batch, a.least, p,
+                             *reinterpret_cast<DivideRoom<THREADS>*>(smem + L::QLO));
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
@@ -111,6 +116,8 @@ paged_attention_f32_kernel(const __grid_constant__ CUtensorMap k_map,
   };
   uint32_t n = 0;  // blocks so far, of all tiles: slot n & 1, round n >> 1
 
+  if (warp >= MMA_WARP) {
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kLeanRegs));
   if (warp == LOAD_WARP) {
     // ---- raw tiles, page by page
     uint32_t count = 0;
@@ -200,8 +207,9 @@ paged_attention_f32_kernel(const __grid_constant__ CUtensorMap k_map,
 #pragma unroll
           for (int i = 0; i < BK / 16; i++) {
             const uint64_t vd = mdesc16<BK>(v, i);  // V lo lies one chunk stride behind V hi
-            umma_f16_ts(tmem + L::O, pa + 8u * i, vd, idesc_o2, (j % CHUNK != 0 || i > 0) ? 1u : 0u);
-            umma_f16_ts(tmem + L::O, pa + 32u + 8u * i, vd, idesc_o, 1u);
+            const uint32_t hi = pa + 32u * (i / 2) + 8u * (i % 2);
+            umma_f16_ts(tmem + L::O, hi, vd, idesc_o2, (j % CHUNK != 0 || i > 0) ? 1u : 0u);
+            umma_f16_ts(tmem + L::O, hi + 16u, vd, idesc_o, 1u);
           }
           umma_commit(B_(PVDONE + (int)slot));
           umma_commit(B_(CONVEMPTY + (int)slot));
@@ -213,8 +221,10 @@ paged_attention_f32_kernel(const __grid_constant__ CUtensorMap k_map,
       umma_commit(B_(DRAIN + 1));
       mbar_wait(B_(DRAIN + 1), 0u, &g_wait_error);
     }
-  } else if (warp >= CONVERT_WARP && warp < MMA_WARP) {
-    // ---- raw rows into pairs; warp w takes rows w RW, w RW + 1, ... of each 4 RW
+  }
+  } else if (warp >= CONVERT_WARP) {
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kConvertRegs));
+    // ---- raw rows into pairs; warp w takes rows w RW, w RW + 1, ... of each 8 RW
     constexpr int LANES = DH / 4, RW = 32 / LANES;  // lanes per row, rows of a warp at once
     const int sub = lane / LANES, col = lane % LANES;
     uint32_t count = 0;
@@ -231,7 +241,7 @@ paged_attention_f32_kernel(const __grid_constant__ CUtensorMap k_map,
         if (ok) ok = wait(RAWFULL + sv, (count + 1) / L::RAWS);
         count += 2;
         // rows of both tiles at once: loads, then maxima, then stores
-        constexpr int STEP = 4 * RW, AT_ONCE = 4;
+        constexpr int STEP = 8 * RW, AT_ONCE = 4;
 #pragma unroll 1
         for (int r0 = 0; r0 < BK && ok; r0 += AT_ONCE * STEP) {
           const int row0 = r0 + (warp - CONVERT_WARP) * RW + sub;
@@ -293,16 +303,22 @@ paged_attention_f32_kernel(const __grid_constant__ CUtensorMap k_map,
       }
       next_tile(nb);
     }
-  } else if (warp < CONVERT_WARP) {
-    // ---- probabilities, one row per thread
-    const int row = tid;
-    const uint32_t lanes = tmem + ((uint32_t)(warp * 32) << 16);
+  } else {
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kSoftRegs));
+    // ---- probabilities: two threads per row, keys 32 half .. 32 half + 31 of a block
+    const int quarter = warp & 3, half = warp >> 2, row = quarter * 32 + lane;
+    const uint32_t lanes = tmem + ((uint32_t)(quarter * 32) << 16);
+    __nv_bfloat16* row_max = reinterpret_cast<__nv_bfloat16*>(smem + L::SHARED_ROWS);  // [2][2][ROWS]
+    float* row_value = reinterpret_cast<float*>(smem + L::SHARED_ROWS);                // [ROWS], between tiles
+    auto pair_sync = [&]() { named_sync(1 + quarter, 64); };
     const bool q_vec = ((reinterpret_cast<uintptr_t>(a.q) | (uintptr_t)(a.q_stride * 4)) & 15) == 0;
     const bool rope_vec = ((reinterpret_cast<uintptr_t>(a.rope.cos) | reinterpret_cast<uintptr_t>(a.rope.sin)) & 7) == 0;
     const bool o_vec = ((reinterpret_cast<uintptr_t>(a.o) | (uintptr_t)(a.o_stride * 4)) & 15) == 0;
     bool ok = true;
     Cut cut{0, 0, 0, 0, 0};
-    while (ok && left > 0) {
+    // after a wait that ran out the loops still end, in step with the other thread
+    // of the row
+    while (left > 0) {
       const int nb = blocks_here(), rows = min(ROWS, p.r.n * group - p.tile * ROWS);
       const bool whole = p.blk == 0, ends = p.blk + nb == p.nblk, done = whole && ends;
       if (whole && !ends) {
@@ -315,77 +331,89 @@ paged_attention_f32_kernel(const __grid_constant__ CUtensorMap k_map,
       const int pos = p.r.len - p.r.n + token, vis = valid ? max(0, pos + 1) : 0;
       const int vis_warp = __shfl_sync(0xffffffffu, max(0, pos + 1), 0);
       float cq = 0.0f;
-      // ---- the warp's rows of Q, rotated: 8 lanes a row, whole lines.  hi passes
+      // ---- the warp's 16 rows of Q, rotated: 8 lanes a row, whole lines.  hi passes
       // through the tile of lo on its way into TMEM (a row per lane), then lo takes
       // the tile.
       {
         constexpr int P = DH / 32;  // 16-byte pieces of a lane
         const uint32_t tile = base + L::QLO;
-        constexpr int G = DH == 128 ? 2 : 4;  // groups of 4 rows whose loads are in flight
+        constexpr int G = 2;  // groups of 4 rows whose loads are in flight
         auto unit_at = [&](int r, int i) {
           const int c = (lane & 7) + 8 * i;  // 8-byte unit of the row
           return tile + (uint32_t)(c >> 4) * ROWS * 128u + (uint32_t)r * 128u +
                  (((((uint32_t)c & 15u) >> 1) ^ (uint32_t)(r & 7)) << 4) + (uint32_t)(c & 1) * 8u;
         };
 #pragma unroll 1
-        for (int pass = 0; pass < 16; pass += G) {
-        const int g0 = pass & 7;
-        if (pass == 8) {  // hi is complete
-          __syncwarp();
-          tile_row16_to_tmem<DH>(tile, row, lanes, L::QH);
-          tmem_wait_st();
-          __syncwarp();
-        }
+        for (int pass = 0; pass < 8; pass += G) {
+          const int g0 = pass & 3;
+          if (pass == 4) {  // hi is complete: this thread's half of its row
+            pair_sync();
+            cq = row_value[row];
+#pragma unroll
+            for (int w = 0; w < DH / 4; w += 16) {
+              float v[16];
+#pragma unroll
+              for (int i = 0; i < 4; i++) {
+                const uint32_t u = (uint32_t)(half * (DH / 4) + w) / 4u + (uint32_t)i;
+                const float4 f = lds128(tile + (u >> 3) * ROWS * 128u + (uint32_t)row * 128u +
+                                        (((u & 7u) ^ (uint32_t)(row & 7)) << 4));
+                v[4 * i] = f.x; v[4 * i + 1] = f.y; v[4 * i + 2] = f.z; v[4 * i + 3] = f.w;
+              }
+              tmem_st16(lanes + L::QH + (uint32_t)(half * (DH / 4) + w), v);
+            }
+            tmem_wait_st();
+            pair_sync();
+          }
+          // all loads first: rows and dims that are not there read the tensor's or
+          // the table's beginning
           float4 x[G][P];
           float2 cs[G][P], sn[G][P];
 #pragma unroll
           for (int k = 0; k < G; k++) {
-            const int r = warp * 32 + 4 * (g0 + k) + (lane >> 3), gr = p.tile * ROWS + r;
+            const int r = quarter * 32 + half * 16 + 4 * (g0 + k) + (lane >> 3), gr = p.tile * ROWS + r;
             const int t = quotient(gr, a.tiling.by_group), at_pos = p.r.len - p.r.n + t;
-            const bool some = r < rows;
-            const float* src = static_cast<const float*>(a.q) + (p.r.first + t) * a.q_stride +
-                               (int64_t)(p.h * group + gr - t * group) * dim;
-            const int64_t tab = some && a.rope.cos != nullptr && at_pos >= 0
-                                    ? rope_row(a.rope, at_pos, a.batch.status) * (dim / 2) : -1;
+            const float* src = static_cast<const float*>(a.q);
+            if (r < rows) src += (p.r.first + t) * a.q_stride + (int64_t)(p.h * group + gr - t * group) * dim;
+            const int64_t tab = r < rows && at_pos >= 0 ? min((int64_t)at_pos, a.rope.rows - 1) * (dim / 2) : 0;
 #pragma unroll
             for (int i = 0; i < P; i++) {
-              const int d = 4 * ((lane & 7) + 8 * i);
-              x[k][i] = make_float4(0.f, 0.f, 0.f, 0.f);
-              cs[k][i] = make_float2(1.f, 1.f);
-              sn[k][i] = make_float2(0.f, 0.f);
-              if (some && d < dim) {
-                if (q_vec) x[k][i] = __ldg(reinterpret_cast<const float4*>(src + d));
-                else x[k][i] = make_float4(__ldg(src + d), __ldg(src + d + 1), __ldg(src + d + 2), __ldg(src + d + 3));
-                if (tab >= 0) {
-                  const float *ct = a.rope.cos + tab + d / 2, *st = a.rope.sin + tab + d / 2;
-                  if (rope_vec) {
-                    cs[k][i] = __ldg(reinterpret_cast<const float2*>(ct));
-                    sn[k][i] = __ldg(reinterpret_cast<const float2*>(st));
-                  } else {
-                    cs[k][i] = make_float2(__ldg(ct), __ldg(ct + 1));
-                    sn[k][i] = make_float2(__ldg(st), __ldg(st + 1));
-                  }
+              const int d = 4 * ((lane & 7) + 8 * i), from = d < dim ? d : 0;
+              if (q_vec) x[k][i] = __ldg(reinterpret_cast<const float4*>(src + from));
+              else x[k][i] = make_float4(__ldg(src + from), __ldg(src + from + 1), __ldg(src + from + 2), __ldg(src + from + 3));
+              if (a.rope.cos != nullptr) {
+                const float *ct = a.rope.cos + tab + from / 2, *st = a.rope.sin + tab + from / 2;
+                if (rope_vec) {
+                  cs[k][i] = __ldg(reinterpret_cast<const float2*>(ct));
+                  sn[k][i] = __ldg(reinterpret_cast<const float2*>(st));
+                } else {
+                  cs[k][i] = make_float2(__ldg(ct), __ldg(ct + 1));
+                  sn[k][i] = make_float2(__ldg(st), __ldg(st + 1));
                 }
               }
             }
           }
 #pragma unroll
           for (int k = 0; k < G; k++) {
-            const int r = warp * 32 + 4 * (g0 + k) + (lane >> 3);
+            const int r = quarter * 32 + half * 16 + 4 * (g0 + k) + (lane >> 3);
+            const int at_pos = p.r.len - p.r.n + quotient(p.tile * ROWS + r, a.tiling.by_group);
+            const bool turned = r < rows && at_pos >= 0 && a.rope.cos != nullptr;
+            if (turned && at_pos >= a.rope.rows) report(a.batch.status, ET_B200_PAGED_BAD_ROPE);
             float m = 0.0f;
 #pragma unroll
-            for (int i = 0; i < P; i++) m = abs_max4(m, x[k][i]);
+            for (int i = 0; i < P; i++) {
+              if (r >= rows || 4 * ((lane & 7) + 8 * i) >= dim) x[k][i] = make_float4(0.f, 0.f, 0.f, 0.f);
+              m = abs_max4(m, x[k][i]);
+            }
 #pragma unroll
             for (int o = 4; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
             // a rotated pair is at most sqrt(2) times its larger element: below 2^14.5
             const int e = row_exponent(m);
             const float sc = exp2_int(e);
-            const int mine = __shfl_sync(0xffffffffu, e, (lane & 3) * 8);
-            if ((lane >> 2) == g0 + k) cq = a.scale_log2 * exp2_int(-mine);
+            if (pass < 4 && (lane & 7) == 0) row_value[r] = a.scale_log2 * exp2_int(-e);
 #pragma unroll
             for (int i = 0; i < P; i++) {
               float4 v = x[k][i];
-              if (a.rope.cos != nullptr) {
+              if (turned) {
                 rotate(v.x, v.y, cs[k][i].x, sn[k][i].x);
                 rotate(v.z, v.w, cs[k][i].y, sn[k][i].y);
               }
@@ -393,10 +421,12 @@ paged_attention_f32_kernel(const __grid_constant__ CUtensorMap k_map,
               pair2(v.x * sc, v.y * sc, h0, l0);
               pair2(v.z * sc, v.w * sc, h1, l1);
               asm volatile("st.shared.v2.f32 [%0], {%1, %2};" ::"r"(unit_at(r, i)),
-                           "f"(pass < 8 ? h0 : l0), "f"(pass < 8 ? h1 : l1) : "memory");
+                           "f"(pass < 4 ? h0 : l0), "f"(pass < 4 ? h1 : l1) : "memory");
             }
           }
         }
+      }
+      {
         fence_async_smem();
         tc_fence_before();
         mbar_arrive(B_(QREADY));
@@ -425,13 +455,12 @@ paged_attention_f32_kernel(const __grid_constant__ CUtensorMap k_map,
         for (int i = 0; i < 32; i += 4)
           *reinterpret_cast<float4*>(part + 32 * c + i) = make_float4(v[i], v[i + 1], v[i + 2], v[i + 3]);
       };
-      for (int j = 0; ok && j < nb; j++, n++) {
+      for (int j = 0; j < nb; j++, n++) {
         if (j > 0 && j % CHUNK == 0) {  // move O out: the next product starts a new accumulator
-          ok = __all_sync(0xffffffffu, wait(PVDONE + ((n - 1) & 1u), (n - 1) >> 1));
-          if (!ok) break;
+          if (ok) ok = __all_sync(0xffffffffu, wait(PVDONE + ((n - 1) & 1u), (n - 1) >> 1));
           tc_fence_after();
 #pragma unroll 1
-          for (int c = 0; c < DH / 32; c++) {
+          for (int c = half * (DH / 64); c < (half + 1) * (DH / 64); c++) {
             float v[32];
             read_o(c, v);
             write_part(c, v);
@@ -439,44 +468,47 @@ paged_attention_f32_kernel(const __grid_constant__ CUtensorMap k_map,
           have_part = true;
           m_part = m == -INFINITY ? 0.0f : m;
         }
-        ok = wait(CONVFULL + (n & 1u), n >> 1);  // the factors
+        if (ok) ok = wait(CONVFULL + (n & 1u), n >> 1);  // the factors
         if (ok) ok = wait(SFULL + (n & 1u), n >> 1);
         ok = __all_sync(0xffffffffu, ok);
-        if (!ok) break;
         tc_fence_after();
         const uint32_t s_at = lanes + L::S0 + 64u * (n & 1u);
         const int key0 = (p.blk + j) * BK;
         const bool masked = key0 + BK > vis_warp;
-        const int seen = vis - key0;
-        const uint32_t f_at = smem_u32(factors + (n & 1u) * 3 * BK);
-        // scores of 32 keys in base 2, exponents of their values added; computed for
-        // the maximum and again for the weights: half the code of keeping all 64
-        // (instruction fetches were a quarter of this kernel's stalls)
-        auto scores = [&](int c, float (&s)[32]) {
-          tmem_ld32(s_at + 32u * c, s);
+        const int seen = vis - key0 - 32 * half;
+        const uint32_t f_at = smem_u32(factors + (n & 1u) * 3 * BK) + 128u * (uint32_t)half;
+        // this thread's scores in base 2, exponents of their values added
+        uint64_t s2[16];
+        {
+          float s[32];
+          tmem_ld32(s_at + 32u * half, s);
+          const uint64_t cq2 = twice(cq);
 #pragma unroll
           for (int i = 0; i < 32; i += 4) {
-            const float4 kf = lds128(f_at + 4u * (32 * c + i)), ge = lds128(f_at + 4u * (BK + 32 * c + i));
-            s[i] = fmaf(s[i] * cq, kf.x, ge.x);
-            s[i + 1] = fmaf(s[i + 1] * cq, kf.y, ge.y);
-            s[i + 2] = fmaf(s[i + 2] * cq, kf.z, ge.z);
-            s[i + 3] = fmaf(s[i + 3] * cq, kf.w, ge.w);
+            const float4 kf = lds128(f_at + 4u * i), ge = lds128(f_at + 4u * (BK + i));
+            s2[i / 2] = fma2(mul2(pk(s[i], s[i + 1]), cq2), pk(kf.x, kf.y), pk(ge.x, ge.y));
+            s2[i / 2 + 1] = fma2(mul2(pk(s[i + 2], s[i + 3]), cq2), pk(kf.z, kf.w), pk(ge.z, ge.w));
           }
-          if (masked) {
-#pragma unroll
-            for (int i = 0; i < 32; i++)
-              if (32 * c + i >= seen) s[i] = -INFINITY;
-          }
-        };
-        float top[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
-#pragma unroll 1
-        for (int c = 0; c < 2; c++) {
-          float s[32];
-          scores(c, s);
-#pragma unroll
-          for (int i = 0; i < 32; i++) top[i & 3] = fmaxf(top[i & 3], s[i]);
         }
-        const float bmax = fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3]));
+        if (masked) {
+#pragma unroll
+          for (int i = 0; i < 16; i++) {
+            const float2 v = unpk(s2[i]);
+            s2[i] = pk(2 * i >= seen ? -INFINITY : v.x, 2 * i + 1 >= seen ? -INFINITY : v.y);
+          }
+        }
+        float top[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+#pragma unroll
+        for (int i = 0; i < 16; i++) {
+          const float2 v = unpk(s2[i]);
+          top[i & 3] = fmaxf(top[i & 3], fmaxf(v.x, v.y));
+        }
+        // the row's maximum over both threads, rounded up: any bound serves both
+        __nv_bfloat16* shared_max = row_max + (n & 1u) * 2 * ROWS;
+        const __nv_bfloat16 own = __float2bfloat16_ru(fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3])));
+        shared_max[half * ROWS + row] = own;
+        pair_sync();
+        const float bmax = fmaxf(__bfloat162float(own), __bfloat162float(shared_max[(1 - half) * ROWS + row]));
         const bool jump = bmax > m + kJump;
         if (__any_sync(0xffffffffu, jump)) {
           const float factor = jump ? ex2(m - bmax) : 1.0f;  // 0 while m is -inf
@@ -485,11 +517,10 @@ paged_attention_f32_kernel(const __grid_constant__ CUtensorMap k_map,
             l *= factor;
           }
           if (j % CHUNK != 0) {  // O holds products of this chunk: rescale it once they are complete
-            ok = __all_sync(0xffffffffu, wait(PVDONE + ((n - 1) & 1u), (n - 1) >> 1));
-            if (!ok) break;
+            if (ok) ok = __all_sync(0xffffffffu, wait(PVDONE + ((n - 1) & 1u), (n - 1) >> 1));
             tc_fence_after();
 #pragma unroll 1
-            for (int c = 0; c < 2 * DH / 32; c++) {
+            for (int c = half * (DH / 32); c < (half + 1) * (DH / 32); c++) {
               float o[32];
               tmem_ld32(lanes + L::O + 32u * c, o);
 #pragma unroll
@@ -499,50 +530,51 @@ paged_attention_f32_kernel(const __grid_constant__ CUtensorMap k_map,
           }
         }
         const float from = (m == -INFINITY ? 0.0f : m) - kShift;
-        float sum[4] = {0.f, 0.f, 0.f, 0.f};
-        // the pairs of the first 32 keys wait in registers: they replace scores that
-        // the second pass still reads
-        float hi[16], lo[16], hi0[16], lo0[16];
-#pragma unroll 1
-        for (int c = 0; c < 2; c++) {
-          float s[32];
-          scores(c, s);
+        uint64_t sum2[2] = {0, 0};
+        const uint64_t from2 = twice(-from);
+        float hi[16], lo[16];
 #pragma unroll
-          for (int i = 0; i < 32; i += 4) {
-            const float4 vf = lds128(f_at + 4u * (2 * BK + 32 * c + i));
-            const float w0 = ex2(s[i] - from), w1 = ex2(s[i + 1] - from);
-            const float w2 = ex2(s[i + 2] - from), w3 = ex2(s[i + 3] - from);
-            sum[0] = fmaf(w0, vf.x, sum[0]);
-            sum[1] = fmaf(w1, vf.y, sum[1]);
-            sum[2] = fmaf(w2, vf.z, sum[2]);
-            sum[3] = fmaf(w3, vf.w, sum[3]);
-            pair2(w0, w1, hi[i / 2], lo[i / 2]);
-            pair2(w2, w3, hi[i / 2 + 1], lo[i / 2 + 1]);
+        for (int i = 0; i < 16; i += 2) {
+          const float4 vf = lds128(f_at + 4u * (2 * BK + 2 * i));
+#pragma unroll
+          for (int k = 0; k < 2; k++) {
+            const float2 x = unpk(add2(s2[i + k], from2));
+            const uint64_t w = pk(ex2(x.x), ex2(x.y));
+            sum2[k] = fma2(w, k == 0 ? pk(vf.x, vf.y) : pk(vf.z, vf.w), sum2[k]);
+            const float2 w2 = unpk(w);
+            const __half2 h = __floats2half2_rn(w2.x, w2.y);
+            const float2 hf = __half22float2(h), rest = unpk(add2(w, pk(-hf.x, -hf.y)));
+            const __half2 l2 = __floats2half2_rn(rest.x, rest.y);
+            hi[i + k] = __uint_as_float(*reinterpret_cast<const uint32_t*>(&h));
+            lo[i + k] = __uint_as_float(*reinterpret_cast<const uint32_t*>(&l2));
           }
-          if (c == 0)
-#pragma unroll
-            for (int i = 0; i < 16; i++) {
-              hi0[i] = hi[i];
-              lo0[i] = lo[i];
-            }
         }
-        tmem_st16(s_at, hi0);
-        tmem_st16(s_at + 32u, lo0);
-        tmem_st16(s_at + 16u, hi);
-        tmem_st16(s_at + 48u, lo);
-        l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
+        // over the columns of these keys' scores: hi, then lo
+        tmem_st16(s_at + 32u * half, hi);
+        tmem_st16(s_at + 32u * half + 16u, lo);
+        const float2 all = unpk(add2(sum2[0], sum2[1]));
+        l += all.x + all.y;
         tmem_wait_st();
         tc_fence_before();
         mbar_arrive(B_(PREADY + (n & 1u)));
       }
       if (ok) ok = __all_sync(0xffffffffu, wait(PVDONE + ((n - 1) & 1u), (n - 1) >> 1));
+      pair_sync();  // the last maxima are read
+      if (half == 1) row_value[row] = l;
+      pair_sync();
+      if (half == 0) {
+        l += row_value[row];
+        row_value[row] = l;
+      }
+      pair_sync();
+      l = row_value[row];
       if (ok) {
         tc_fence_after();
         const float inv = l > 0.0f ? 1.0f / l : 0.0f;
         float* dst = static_cast<float*>(a.o) + (p.r.first + token) * a.o_stride + (int64_t)head * dim;
         const int slot = 2 * (int)blockIdx.x + (whole ? 1 : 0);
 #pragma unroll 1
-        for (int c = 0; c < DH / 32; c++) {
+        for (int c = half * (DH / 64); c < (half + 1) * (DH / 64); c++) {
           float o[32];
           read_o(c, o);
           if (!valid) continue;
@@ -562,7 +594,7 @@ paged_attention_f32_kernel(const __grid_constant__ CUtensorMap k_map,
             write_part(c, o);
           }
         }
-        if (valid) {
+        if (valid && half == 0) {
           // weights are relative to m - kShift
           if (!done) {
             a.joint.stats[(int64_t)slot * 2 * ROWS + row] = m - kShift;

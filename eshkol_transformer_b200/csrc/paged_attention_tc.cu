@@ -108,7 +108,8 @@ paged_attention_tc_kernel(const __grid_constant__ CUtensorMap k_map,
   }
   if (warp == MMA_WARP) tmem_alloc(smem_u32(tslot), L::COLS);
   Place p;
-  const Share share = divide<THREADS>(a.tiling, a.batch, a.least, p);
+  __shared__ DivideRoom<THREADS> room;
+  const Share share = divide(a.tiling, a.batch, a.least, p, room);
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
