@@ -38,7 +38,7 @@ using namespace f16att;
 constexpr int ROWS = 128, BK = 64;
 constexpr int SOFT = 256, CONVERT_WARP = 8, MMA_WARP = 16, LOAD_WARP = 18, THREADS = 640;
 // registers of the warpgroups: probabilities, conversion, the rest
-constexpr int kSoftRegs = 120, kConvertRegs = 88, kLeanRegs = 64;
+constexpr int kSoftRegs = 136, kConvertRegs = 72, kLeanRegs = 48;
 static_assert(256 * kSoftRegs + 256 * kConvertRegs + 128 * kLeanRegs <= THREADS * 96, "registers at launch");
 constexpr float kJump = 8.0f;   // log2 of the largest P the standing maximum allows
 constexpr float kShift = 7.0f;  // P carries 2^7: at most 2^15
@@ -241,7 +241,7 @@ paged_attention_f32_kernel(const __grid_constant__ CUtensorMap k_map,
         if (ok) ok = wait(RAWFULL + sv, (count + 1) / L::RAWS);
         count += 2;
         // rows of both tiles at once: loads, then maxima, then stores
-        constexpr int STEP = 8 * RW, AT_ONCE = 4;
+        constexpr int STEP = 8 * RW, AT_ONCE = 2;
 #pragma unroll 1
         for (int r0 = 0; r0 < BK && ok; r0 += AT_ONCE * STEP) {
           const int row0 = r0 + (warp - CONVERT_WARP) * RW + sub;
@@ -343,27 +343,9 @@ paged_attention_f32_kernel(const __grid_constant__ CUtensorMap k_map,
           return tile + (uint32_t)(c >> 4) * ROWS * 128u + (uint32_t)r * 128u +
                  (((((uint32_t)c & 15u) >> 1) ^ (uint32_t)(r & 7)) << 4) + (uint32_t)(c & 1) * 8u;
         };
-#pragma unroll 1
-        for (int pass = 0; pass < 8; pass += G) {
-          const int g0 = pass & 3;
-          if (pass == 4) {  // hi is complete: this thread's half of its row
-            pair_sync();
-            cq = row_value[row];
+        float low[4][P][2];
 #pragma unroll
-            for (int w = 0; w < DH / 4; w += 16) {
-              float v[16];
-#pragma unroll
-              for (int i = 0; i < 4; i++) {
-                const uint32_t u = (uint32_t)(half * (DH / 4) + w) / 4u + (uint32_t)i;
-                const float4 f = lds128(tile + (u >> 3) * ROWS * 128u + (uint32_t)row * 128u +
-                                        (((u & 7u) ^ (uint32_t)(row & 7)) << 4));
-                v[4 * i] = f.x; v[4 * i + 1] = f.y; v[4 * i + 2] = f.z; v[4 * i + 3] = f.w;
-              }
-              tmem_st16(lanes + L::QH + (uint32_t)(half * (DH / 4) + w), v);
-            }
-            tmem_wait_st();
-            pair_sync();
-          }
+        for (int g0 = 0; g0 < 4; g0 += G) {
           // all loads first: rows and dims that are not there read the tensor's or
           // the table's beginning
           float4 x[G][P];
@@ -409,7 +391,7 @@ paged_attention_f32_kernel(const __grid_constant__ CUtensorMap k_map,
             // a rotated pair is at most sqrt(2) times its larger element: below 2^14.5
             const int e = row_exponent(m);
             const float sc = exp2_int(e);
-            if (pass < 4 && (lane & 7) == 0) row_value[r] = a.scale_log2 * exp2_int(-e);
+            if ((lane & 7) == 0) row_value[r] = a.scale_log2 * exp2_int(-e);
 #pragma unroll
             for (int i = 0; i < P; i++) {
               float4 v = x[k][i];
@@ -417,14 +399,36 @@ paged_attention_f32_kernel(const __grid_constant__ CUtensorMap k_map,
                 rotate(v.x, v.y, cs[k][i].x, sn[k][i].x);
                 rotate(v.z, v.w, cs[k][i].y, sn[k][i].y);
               }
-              float h0, l0, h1, l1;
-              pair2(v.x * sc, v.y * sc, h0, l0);
-              pair2(v.z * sc, v.w * sc, h1, l1);
-              asm volatile("st.shared.v2.f32 [%0], {%1, %2};" ::"r"(unit_at(r, i)),
-                           "f"(pass < 4 ? h0 : l0), "f"(pass < 4 ? h1 : l1) : "memory");
+              float h0, h1;
+              pair2(v.x * sc, v.y * sc, h0, low[g0 + k][i][0]);
+              pair2(v.z * sc, v.w * sc, h1, low[g0 + k][i][1]);
+              asm volatile("st.shared.v2.f32 [%0], {%1, %2};" ::"r"(unit_at(r, i)), "f"(h0), "f"(h1) : "memory");
             }
           }
         }
+        // hi is complete: this thread's half of its row
+        pair_sync();
+        cq = row_value[row];
+#pragma unroll
+        for (int w = 0; w < DH / 4; w += 16) {
+          float v[16];
+#pragma unroll
+          for (int i = 0; i < 4; i++) {
+            const uint32_t u = (uint32_t)(half * (DH / 4) + w) / 4u + (uint32_t)i;
+            const float4 f = lds128(tile + (u >> 3) * ROWS * 128u + (uint32_t)row * 128u +
+                                    (((u & 7u) ^ (uint32_t)(row & 7)) << 4));
+            v[4 * i] = f.x; v[4 * i + 1] = f.y; v[4 * i + 2] = f.z; v[4 * i + 3] = f.w;
+          }
+          tmem_st16(lanes + L::QH + (uint32_t)(half * (DH / 4) + w), v);
+        }
+        tmem_wait_st();
+        pair_sync();
+#pragma unroll
+        for (int k = 0; k < 4; k++)
+#pragma unroll
+          for (int i = 0; i < P; i++)
+            asm volatile("st.shared.v2.f32 [%0], {%1, %2};" ::"r"(unit_at(quarter * 32 + half * 16 + 4 * k + (lane >> 3), i)),
+                         "f"(low[k][i][0]), "f"(low[k][i][1]) : "memory");
       }
       {
         fence_async_smem();
