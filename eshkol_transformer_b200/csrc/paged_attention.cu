@@ -868,7 +868,7 @@ int32_t et_b200_paged_attention_v1(const et_b200_paged_cache_v1* c,
     if ((reinterpret_cast<uintptr_t>(q) | reinterpret_cast<uintptr_t>(o)) % size != 0)
       return set_error(e, ET_KERNEL_ERROR_INVALID_ARGUMENT, ET_KERNEL_CODE_INVALID_BUFFER, op,
                        "q and o must be aligned to their elements");
-    if (b->tokens * q_heads > INT32_MAX)
+    if (b->tokens * q_heads > INT32_MAX - 4096)
       return set_error(e, ET_KERNEL_ERROR_SHAPE_MISMATCH, ET_KERNEL_CODE_INVALID_SHAPE, op,
                        "tokens times q_heads must stay below 2^31");
     if (workspace == nullptr || (reinterpret_cast<uintptr_t>(workspace) & 255) != 0 ||

@@ -8,7 +8,8 @@ rounded (u), so a score is off by at most delta = (u + DIM 2^-23) scale
 sum |q'||k| + 2^-22 |score| (f32 accumulation, the base-2 exponential); a
 weight by exp(2 delta) - 1 relative, plus u for its own rounding in the
 numerator, so o is off by at most (exp(2 delta) - 1 + u + KEYS 2^-23) sum p|v|
-+ u |o|.  At f32 the bar of the framework's other f32-grade attention tests:
++ u |o|; exponentials by polynomial are off by 2.7e-6, which numerator and
+denominator both carry (2^-17 together).  At f32 the bar of the framework's other f32-grade attention tests:
 2e-5 absolute plus relative.
 """
 import math
@@ -103,7 +104,7 @@ class Step:
                 lse_bound = 2e-5 + 2e-5 * lse.abs()
             else:
                 delta = (u + dim * 2.0 ** -23) * spread + 2.0 ** -22 * spread
-                wide = (2 * delta).expm1() + u + (m + 16) * 2.0 ** -23
+                wide = (2 * delta).expm1() + u + (m + 16) * 2.0 ** -23 + 2.0 ** -17
                 bound = wide[..., None] * weighted + u * o.abs() + 1e-30
                 lse_bound = delta + 2e-5 * (1 + lse.abs())
             empty = torch.isinf(lse)
@@ -138,7 +139,9 @@ def test_attention_vs_float64(lib, cuda, requests, q_heads, heads, dim, page, dt
     ([(1 + b % 3, 1 + 7 * b % 130) for b in range(300)], 2, 2, 64),  # more requests than threads
     ([(257, 600), (1, 2000), (129, 129), (16, 16)], 8, 2, 128),
     ([(200, 1000)], 3, 1, 64),                         # a group that straddles tiles
-], ids=["long", "ragged", "chunk", "many", "mixed", "odd group"])
+    ([(1, 3000), (2, 70)], 40, 1, 64),                 # more heads in a group than a small tile's rows
+    ([(140, 5000)], 2, 1, 96),                         # long accumulations, padded head_dim
+], ids=["long", "ragged", "chunk", "many", "mixed", "odd group", "wide group", "padded"])
 def test_attention_divided_work(lib, cuda, requests, q_heads, heads, dim, dtype):
     s = Step(requests, q_heads, heads, dim, 32, dtype, seed=len(requests))
     s.attend()
@@ -281,6 +284,39 @@ def test_far_pages(lib, cuda):
         delta = (U[F16] + 2.0 ** -16) * spread
         bound = ((2 * delta).expm1() + U[F16] + 2.0 ** -17)[..., None] * weighted
         assert ((o.double() - want).abs() <= bound + U[F16] * want.abs()).all()
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
+def test_empty_steps(lib, cuda, dtype):
+    """No request, no token, and requests that bring none."""
+    s = Step([(0, 30), (0, 0), (0, 9)], 2, 1, 64, 16, dtype, spare=3)
+    s.attend()
+    s.check()
+    keys = s.keys.clone().nan_to_num()
+    k = torch.ones(3, 1, 64, device="cuda", dtype=dtype)
+    s.cache.append(s.batch(), k, k)
+    assert torch.equal(s.keys.nan_to_num(), keys)
+    none = torch.zeros(0, 1, 64, device="cuda", dtype=dtype)
+    i64 = dict(dtype=torch.int64, device="cuda")
+    for batch in (paged.PagedBatch(s.offsets, s.lengths, s.table, 0),
+                  paged.PagedBatch(torch.zeros(1, **i64), torch.zeros(0, **i64),
+                                   torch.zeros(0, 4, dtype=torch.int32, device="cuda"), 0)):
+        s.cache.append(batch, none, none)
+        paged.PagedAttention(s.cache, 1).forward(batch, none, none.clone())
+    ids = torch.zeros(0, **i64)
+    sampling.Sampler(0, 5).sample(torch.zeros(0, 5, device="cuda"), torch.zeros(0, device="cuda"), ids)
+
+
+def test_one_workspace_serves_kernels_in_turn(lib, cuda):
+    """Chunks, single tokens and other caches' steps through one object, back to
+    back on one stream: nothing of a call is left for the next."""
+    s = Step([(90, 700), (1, 2000), (33, 40)], 4, 2, 64, 16, F16)
+    a = paged.PagedAttention(s.cache, 4)
+    for hint in (90, 1, 90, 4, 1):
+        b = paged.PagedBatch(s.offsets, s.lengths, s.table, s.tokens, hint, None, s.status)
+        a.forward(b, s.q, s.o, (s.cos, s.sin), s.lse)
+        s.check()
+        a.ws.fill_(255)  # NaNs
 
 
 def test_streams_graphs_and_workspaces(lib, cuda):
@@ -457,6 +493,48 @@ def test_sampling_special_values(lib, cuda):
     x = torch.zeros(4, 6, device="cuda")
     assert draw(x, np.array([-1.0, 1.0, 5.0, nan], np.float32))[0].tolist() == [0, 5, 5, 0]
     assert draw(x, 0.5, temperature=nan)[0].tolist() == [0] * 4
+
+
+@pytest.mark.parametrize("k", [16, 255, 256, 257, 512, 1024, 20000])
+def test_sampling_top_k_sizes(lib, cuda, k):
+    """Lists, histogram cuts and the borders between them."""
+    u = np.random.default_rng(k).random(6).astype(np.float32)
+    for vocab, dtype in ((30000, F32), (4097, BF16), (1500, F16)):
+        check_draw(logits_of(6, vocab, dtype, k), u, 1.0, top_k=k)
+        check_draw(logits_of(6, vocab, dtype, k + 1), u, 0.05, top_k=k, top_p=0.97)
+
+
+@pytest.mark.parametrize("scale,temperature", [(1e4, 1e4), (1e5, 1.0), (1.0, 1e-6), (1e-6, 1e-6),
+                                               (1e30, 1e30), (1.0, 1e4), (1e-3, 1e-3)])
+def test_sampling_extreme_scales(lib, cuda, scale, temperature):
+    """Large logits and temperatures of any size, and a row with one far outlier.
+    Weights beyond 2^-36 of the largest count as 0: of up to 5,000 tokens they
+    are 2^-23 of the mass, within the margin."""
+    x = logits_of(8, 5000, F32, 11) * scale
+    x[7, 17] = x[7, x[7] > -math.inf].max() + 200.0 * scale
+    u = np.random.default_rng(3).random(8).astype(np.float32)
+    for kw in (dict(), dict(top_k=30), dict(top_k=600), dict(top_p=0.9)):
+        check_draw(x, u, temperature, **kw)
+
+
+def test_sampling_vocabulary_beyond_a_cluster(lib, cuda):
+    """More logits than the shared memory of a cluster holds: read from memory."""
+    x = logits_of(2, 450001, F32, 5, sigma=1.0)
+    x[:, 1000:1010] += 14.0
+    u = np.array([0.3, 0.8], np.float32)
+    for kw in (dict(top_k=64), dict(top_k=5, top_p=0.5), dict(min_p=0.3), dict(temperature=0.0)):
+        check_draw(x, u, **kw)
+
+
+def test_sampling_is_the_same_whatever_the_rows(lib, cuda):
+    """A row's draw does not depend on how many rows (thread blocks per row) the
+    call has."""
+    x, u = logits_of(300, 20000, F32, 2), np.random.default_rng(5).random(300).astype(np.float32)
+    for kw in (dict(), dict(top_k=50), dict(top_p=0.9), dict(top_k=400, top_p=0.95, min_p=0.01)):
+        ids, lp = draw(x, u, 0.8, **kw)
+        for rows in (1, 7, 60):
+            a, b = draw(x[:rows], u[:rows], 0.8, **kw)
+            assert np.array_equal(a, ids[:rows]) and np.array_equal(b, lp[:rows])
 
 
 def test_sampling_strides_and_large_vocabulary(lib, cuda):
