@@ -346,7 +346,7 @@ struct AttendArgs {
   void* o;
   float* lse;
   int64_t q_stride, o_stride, least;
-  int q_heads;
+  int q_heads, sms;  // SMs of the device
   float scale_log2;  // log2(e) / sqrt(head_dim)
 };
 
@@ -384,7 +384,7 @@ inline int thread_blocks(const AttendArgs& a, int most, int rows, int keys) {
 }
 // The tcgen05 kernel (paged_attention_tc.cu): launches it and returns its
 // thread blocks, 0 where it does not take the cache (nothing is launched).
-size_t attend_tc_workspace(int dim_padded);
+size_t attend_tc_workspace(int dim_padded, int sms);
 int attend_tc(const et_b200_paged_cache_v1* c, AttendArgs& a, void* ws, cudaStream_t stream);
 // The same for f32 caches (paged_attention_f32.cu); its workspace is within
 // attend_tc_workspace.

@@ -757,7 +757,7 @@ void launch_join(const AttendArgs& a, int blocks, int64_t rows, cudaStream_t str
   cudaLaunchConfig_t cfg{};
   // a row per thread block for as many rows as a tile is likely to have (the
   // kernel walks any number)
-  cfg.gridDim = dim3(blocks < sm_count() ? blocks : sm_count(), rows < 1 ? 1 : rows < 16 ? rows : 16);
+  cfg.gridDim = dim3(blocks < a.sms ? blocks : a.sms, rows < 1 ? 1 : rows < 16 ? rows : 16);
   cfg.blockDim = dim3(32 * JOIN_WARPS);
   cfg.stream = stream;
   cudaLaunchAttribute attr{};
@@ -777,9 +777,10 @@ void launch_shape(const et_b200_paged_cache_v1* c, AttendArgs& a, int64_t max_ne
   CUtensorMap k_map, v_map;
   const bool tma = pool_map(&k_map, c->keys, c, S::WIDE, 1 << box_bits) &&
                    pool_map(&v_map, c->values, c, S::WIDE, 1 << box_bits);
+  const int sms = a.sms;
   const int resident = tma ? resident_blocks<paged_attention_kernel<T, S, true>>(S::NT + 32, S::SMEM)
                            : resident_blocks<paged_attention_kernel<T, S, false>>(S::NT, S::SMEM);
-  const int blocks = thread_blocks(a, resident * sm_count(), S::BM, S::BK);
+  const int blocks = thread_blocks(a, resident * sms, S::BM, S::BK);
   a.tiling = tiling_of(S::bits(S::BM), S::bits(S::BK), a.tiling.group, a.pools.kv_heads);
   a.least = 1;
   a.joint = joint_of(ws, blocks, S::BM, S::DH);
@@ -825,6 +826,12 @@ void launch_type(const et_b200_paged_cache_v1* c, AttendArgs& a, int64_t max_new
   }
 }
 
+size_t workspace_bytes(int64_t head_dim, int sms) {
+  const int dim = padded(head_dim);
+  const size_t plain = joint_bytes(kMostPerSm * sms, 64, dim), tc = attend_tc_workspace(dim, sms);
+  return plain > tc ? plain : tc;
+}
+
 }  // namespace
 }  // namespace etb
 
@@ -838,17 +845,15 @@ size_t et_b200_paged_attention_workspace_bytes_v1(const et_b200_paged_cache_v1* 
   if (check_cache(c, nullptr, "paged-attention-workspace") || q_heads < 1 ||
       q_heads % c->kv_heads != 0)
     return 0;
-  const size_t plain = joint_bytes(kMostPerSm * sm_count(), 64, padded(c->head_dim));
-  const size_t tc = attend_tc_workspace(padded(c->head_dim));
-  return plain > tc ? plain : tc;
+  return workspace_bytes(c->head_dim, sm_count());
 }
 
 int32_t et_b200_paged_attention_v1(const et_b200_paged_cache_v1* c,
                                    const et_b200_paged_batch_v1* b,
                                    const et_b200_paged_rope_v1* rope, int64_t q_heads,
                                    const void* q, int64_t q_stride, void* o, int64_t o_stride,
-                                   float* lse, void* workspace, size_t workspace_bytes,
-                                   void* stream, et_kernel_error* e) {
+                                   float* lse, void* workspace, size_t bytes, void* stream,
+                                   et_kernel_error* e) {
   const char* op = "paged-attention";
   if (int32_t r = check_cache(c, e, op)) return r;
   if (int32_t r = check_batch(b, c, e, op)) return r;
@@ -871,8 +876,9 @@ int32_t et_b200_paged_attention_v1(const et_b200_paged_cache_v1* c,
     if (b->tokens * q_heads > INT32_MAX - 4096)
       return set_error(e, ET_KERNEL_ERROR_SHAPE_MISMATCH, ET_KERNEL_CODE_INVALID_SHAPE, op,
                        "tokens times q_heads must stay below 2^31");
+    const int sms = sm_count();
     if (workspace == nullptr || (reinterpret_cast<uintptr_t>(workspace) & 255) != 0 ||
-        workspace_bytes < et_b200_paged_attention_workspace_bytes_v1(c, q_heads))
+        bytes < workspace_bytes(c->head_dim, sms))
       return set_error(e, ET_KERNEL_ERROR_INVALID_ARGUMENT, ET_KERNEL_CODE_BUFFER_TOO_SMALL, op,
                        "workspace is smaller than et_b200_paged_attention_workspace_bytes_v1 or "
                        "not 256-byte aligned");
@@ -889,6 +895,7 @@ int32_t et_b200_paged_attention_v1(const et_b200_paged_cache_v1* c,
     a.q_stride = q_stride;
     a.o_stride = o_stride;
     a.q_heads = (int)q_heads;
+    a.sms = sms;
     a.scale_log2 = kLog2e / sqrtf((float)c->head_dim);
     auto st = static_cast<cudaStream_t>(stream);
     if (c->dtype == ET_B200_DTYPE_F32) launch_type<float>(c, a, b->max_new, workspace, st);

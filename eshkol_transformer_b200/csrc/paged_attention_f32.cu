@@ -635,7 +635,7 @@ int launch_f32(const et_b200_paged_cache_v1* c, AttendArgs& a, void* ws, cudaStr
     return 0;
   a.tiling = tiling_of(7, 6, a.tiling.group, a.pools.kv_heads);
   static_assert(ROWS == 1 << 7 && BK == 1 << 6, "tiling");
-  const int blocks = thread_blocks(a, sm_count(), ROWS, BK);
+  const int blocks = thread_blocks(a, a.sms, ROWS, BK);
   a.least = 2;
   a.joint = joint_of(ws, blocks, ROWS, DH);
   cudaFuncSetAttribute(paged_attention_f32_kernel<DH>, cudaFuncAttributeMaxDynamicSharedMemorySize,

@@ -514,7 +514,7 @@ int launch_tc(const et_b200_paged_cache_v1* c, AttendArgs& a, void* ws, cudaStre
   CUtensorMap k_map, v_map;
   if (!pool_map(&k_map, c->keys, c, 64, box_rows) || !pool_map(&v_map, c->values, c, 64, box_rows))
     return 0;
-  const int blocks = thread_blocks(a, sm_count(), 2 * HALF, BK);
+  const int blocks = thread_blocks(a, a.sms, 2 * HALF, BK);
   a.tiling = tiling_of(8, 7, a.tiling.group, a.pools.kv_heads);
   static_assert(2 * HALF == 1 << 8 && BK == 1 << 7, "tiling");
   a.least = 2;
@@ -530,8 +530,8 @@ int launch_tc(const et_b200_paged_cache_v1* c, AttendArgs& a, void* ws, cudaStre
 
 namespace paged {
 
-size_t attend_tc_workspace(int dim_padded) {
-  return dim_padded > 128 ? 0 : joint_bytes(sm_count(), 2 * HALF, dim_padded < 64 ? 64 : dim_padded);
+size_t attend_tc_workspace(int dim_padded, int sms) {
+  return dim_padded > 128 ? 0 : joint_bytes(sms, 2 * HALF, dim_padded < 64 ? 64 : dim_padded);
 }
 
 int attend_tc(const et_b200_paged_cache_v1* c, AttendArgs& a, void* ws, cudaStream_t stream) {

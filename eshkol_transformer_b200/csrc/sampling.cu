@@ -10,13 +10,17 @@
 // A row is read from memory once, into the shared memory of a cluster of
 // thread blocks (each a contiguous slice; as many as the slices need, more
 // when there are few rows), while its maximum is formed.  Then
-//  - a small top-k (or a small vocabulary) becomes a list: each slice keeps
-//    what reaches a lower bound of its k-th largest logit (from the maxima of
-//    its threads), one block sorts the gathered list, cuts it by all filters,
-//    sorts what is left by index and draws;
-//  - otherwise a cut is found from a histogram (tokens or weights) over
-//    1,024 steps of the logit, the border's step is gathered and sorted, and
-//    the draw adds the kept weights slice by slice, warp by warp.
+//  - a small top-k (or a small vocabulary) becomes a list: every slice pushes
+//    what reaches a lower bound of the row's k-th largest logit (from the maxima
+//    of its threads) to one block, which ranks it, cuts it by all filters, adds
+//    up what is left in the order of the vocabulary and draws;
+//  - otherwise a cut is found from a histogram (tokens or weights) over 1,024
+//    steps of the logit, the border's step is gathered and ranked, and the draw
+//    adds the kept weights slice by slice, warp by warp.
+// Reading a row bounds the greedy case (256 rows of 128,259 bf16 logits: 30 us
+// with the thread blocks' set-up, 10 us at the copy rate); with filters it is the
+// arithmetic of the weights (some 25 instructions each) and the latency of the
+// steps that one thread block or cluster takes alone.
 // Rows for which the list or the border's step overflows (thousands of equal
 // logits) or the slices do not fit are selected by radix from memory.
 #include <math.h>
@@ -367,8 +371,15 @@ __device__ __forceinline__ void answer(const Args& a, int64_t row, int id, float
   a.ids[row] = id;
   if (a.logprobs == nullptr) return;
   const double d = sc.max == INFINITY ? 0.0 : (double)x - (double)sc.max;
-  a.logprobs[row] = (float)(d * f.per * 0.6931471805599453 -
-                            log((double)total / (double)weight_of(sc.max, sc)));
+  // ln(total / w(max)) of the ratio's exponent and mantissa: 1e-7 absolute
+  const float ratio = (float)total / (float)weight_of(sc.max, sc);
+  int k;
+  float m = frexpf(ratio, &k);
+  if (m < 0.70710678f) {  // around 1, so that a ratio of 1 is exactly 0
+    m *= 2.0f;
+    k--;
+  }
+  a.logprobs[row] = (float)((d * f.per - (double)k) * 0.6931471805599453 - (double)logf(m));
 }
 
 // One thread block draws for a row in global memory: radix selection.
@@ -762,9 +773,13 @@ struct Weights {
   __device__ __forceinline__ uint64_t operator()(float x) const { return weight_of(x, sc); }
   __device__ __forceinline__ void both(float x, float y, uint64_t (&w)[2]) const {
     if (sc.narrow) {
-      const float2 p = unpk(powers_of(x, y, sc));
-      w[0] = __float2ull_rn(p.x * 0x1p35f);
-      w[1] = __float2ull_rn(p.y * 0x1p35f);
+      // rounded as add_weights does; the integers lie in the sums' low bits
+      const uint64_t p = powers_of(x, y, sc), c = add2(p, twice(96.0f));
+      const uint64_t r = fma2(add2(c, twice(-96.0f)), twice(-1.0f), p);
+      const float2 cc = unpk(c), ff = unpk(add2(r, twice(0x1.8p-12f)));
+      const int base = __float_as_int(96.0f), fine = __float_as_int(0x1.8p-12f);
+      w[0] = ((uint64_t)(__float_as_int(cc.x) - base) << 18) + (int64_t)(__float_as_int(ff.x) - fine);
+      w[1] = ((uint64_t)(__float_as_int(cc.y) - base) << 18) + (int64_t)(__float_as_int(ff.y) - fine);
     } else {
       w[0] = weight_of(x, sc);
       w[1] = weight_of(y, sc);
