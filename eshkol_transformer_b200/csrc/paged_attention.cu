@@ -402,9 +402,13 @@ paged_attention_kernel(const __grid_constant__ CUtensorMap k_map,
             for (int i = 0; i < 4; i++) pair_tf32(kb[i], kh[i], kl[i]);
 #pragma unroll
             for (int i = 0; i < 2; i++) {
-              mma_tf32(s[2 * n + i], ql, kh[2 * i], kh[2 * i + 1]);
-              mma_tf32(s[2 * n + i], qh, kl[2 * i], kl[2 * i + 1]);
-              mma_tf32(s[2 * n + i], qh, kh[2 * i], kh[2 * i + 1]);
+              // the tensor pipe's accumulation truncates: eight dims at a time, added in f32
+              float part[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+              mma_tf32(part, ql, kh[2 * i], kh[2 * i + 1]);
+              mma_tf32(part, qh, kl[2 * i], kl[2 * i + 1]);
+              mma_tf32(part, qh, kh[2 * i], kh[2 * i + 1]);
+#pragma unroll
+              for (int e = 0; e < 4; e++) s[2 * n + i][e] += part[e];
             }
           } else {
             mma16<T>(s[2 * n], ql, kb[0], kb[1]);
@@ -471,7 +475,7 @@ paged_attention_kernel(const __grid_constant__ CUtensorMap k_map,
 #pragma unroll
             for (int i = 0; i < 2; i++)
               pair_tf32(lds32(vt + S::template at<BK>(row + i, d / 4) + 4 * (d & 3)), vh[i], vl[i]);
-            // the tensor pipe's accumulation truncates: eight keys at a time, added in f32
+            // eight keys at a time, as above
             float part[4] = {0.0f, 0.0f, 0.0f, 0.0f};
             mma_tf32(part, pl, vh[0], vh[1]);
             mma_tf32(part, ph, vl[0], vl[1]);
