@@ -235,9 +235,10 @@ int32_t et_b200_paged_append_v1(const et_b200_paged_cache_v1 *cache,
  * o_stride elements apart; q_heads a multiple of kv_heads, query head h reads
  * key head h / (q_heads / kv_heads).  A query that sees no key gets zeros.
  * lse (f32 [tokens, q_heads], or NULL) receives ln(sum of exp of the scaled
- * scores), -inf without keys.  Scores, statistics and sums are f32; q' and the
- * probabilities are rounded to the pools' type for the tensor cores at f16
- * and bf16, and carried as TF32 pairs (about 22 bits) at f32.  Keys and
+ * scores), -inf without keys.  Scores, statistics and sums are f32; for the
+ * tensor cores q' and the probabilities are rounded to the pools' type at f16
+ * and bf16 (q' with its residual up to 16 query rows per kv head), and all
+ * operands are carried as pairs of about 22 bits at f32.  Keys and
  * values of positions below a request's length must be finite; slots behind
  * may hold anything.  The workspace (any contents, overwritten; its size does
  * not depend on the batch) serves one call at a time: calls that may overlap,
