@@ -268,6 +268,8 @@ __device__ Share divide(const Tiling& t, const Batch& B, int64_t least, Place& p
   s.units = max((int64_t)0, min(total - u0, s.per));
   p.b = B.batch;
   if (s.units == 0) return s;
+  if (tid == 0) found_s[0] = B.batch;
+  __syncthreads();
   int64_t before = 0;
   for (int base = 0; base < B.batch; base += NT) {
     int64_t all;
@@ -291,6 +293,10 @@ __device__ Share divide(const Tiling& t, const Batch& B, int64_t least, Place& p
   }
   __syncthreads();
   p.b = (int)found_s[0];
+  if (p.b >= B.batch) {  // the lengths changed between the two passes: nothing is followed
+    s.units = 0;
+    return s;
+  }
   int64_t rest = found_s[1] & (((int64_t)1 << 48) - 1);
   p.h = (int)(found_s[1] >> 48);
   p.r = request_s;

@@ -805,12 +805,14 @@ __device__ bool cluster_cut(cg::cluster_group& cluster, Room& rm, unsigned rank,
     return t > 0.0f ? (int)fminf(t, (float)(LIST - 1)) : 0;
   };
   least = fmaxf(least, border.value);
-  cluster.sync();  // nobody reads this block's room any more
+  // (since the caller's last cluster.sync nobody reads or writes this block's
+  // histogram or list)
   for (int i = tid; i < LIST; i += NT) rm.low[i] = rm.high[i] = 0;
   __syncthreads();
+  const bool every = border.value == -INFINITY && least > -INFINITY;
   auto add = [&](float x, uint64_t w) {
-    if (w == 0) return;
-    const int step = step_of(x);
+    // `least` is finite for weights: steps need no bounds but the rounding's
+    const int step = COUNT ? step_of(x) : min((int)((max - x) * per), LIST - 1);
     if (COUNT) {
       atomicAdd(&rm.low[step], (uint32_t)w);
       return;
@@ -822,8 +824,8 @@ __device__ bool cluster_cut(cg::cluster_group& cluster, Room& rm, unsigned rank,
   slice.each_piece(least, [&](int i, const float (&v)[Slice<T>::N]) {
 #pragma unroll
     for (int k = 0; k < Slice<T>::N; k += 2) {
-      const bool a = v[k] >= least && kept(border, v[k], first + i + k);
-      const bool b = v[k + 1] >= least && kept(border, v[k + 1], first + i + k + 1);
+      const bool a = v[k] >= least && (every || kept(border, v[k], first + i + k));
+      const bool b = v[k + 1] >= least && (every || kept(border, v[k + 1], first + i + k + 1));
       if (a || b) {
         uint64_t w[2];
         unit.both(v[k], v[k + 1], w);
@@ -1150,7 +1152,8 @@ __global__ void __launch_bounds__(NT, 2) sample_cluster_kernel(const T* __restri
     if ((uint64_t)flt.top_k < cluster_total(cluster, rm, blocks))
       good = cluster_cut<T>(cluster, rm, rank, blocks, slice, first, max, kTopSteps, -INFINITY, border,
                             Tokens{}, (uint64_t)flt.top_k);
-    cluster.sync();
+    else
+      cluster.sync();  // the totals are read
   }
   if (good && flt.top_p < 1.0f) {
     const uint64_t here = block_weights(slice, first, border, sc, rm);
@@ -1170,9 +1173,9 @@ __global__ void __launch_bounds__(NT, 2) sample_cluster_kernel(const T* __restri
     const float per = fminf((float)(LIST - 1) / fmaxf(max - least, 0.0f), 1e30f);
     good = cluster_cut<T>(cluster, rm, rank, blocks, slice, first, max, per, least, border,
                           Weights{sc}, to);
-    cluster.sync();
   }
   if (!good) {
+    cluster.sync();  // the border is read: the others may leave
     if (rank == 0) sample_row<T>(x, a, row, flt, sc, rm.radix);
     return;
   }

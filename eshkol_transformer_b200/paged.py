@@ -10,7 +10,9 @@ and attention of new tokens over it (et_b200_paged_attention_v1).
 The descriptors hold the tensors they were built from and may be kept while
 their contents change (a decoding loop updates offsets, lengths and the page
 table in place).  Calls are enqueued on `stream` (a cudaStream_t address, 0 =
-the legacy default stream) of the current device.
+the legacy default stream) of the current device and return at once; on a
+stream other than torch's current one the caller orders the two and keeps the
+tensors (Tensor.record_stream) until the call has run.
 """
 from __future__ import annotations
 
