@@ -760,6 +760,7 @@ int resident_blocks(int threads, int smem) {
 
 template <typename T, int DH>
 void launch_join(const AttendArgs& a, int blocks, int64_t rows, cudaStream_t stream) {
+  if (cudaPeekAtLastError() != cudaSuccess) return;  // no parts were left to join
   cudaLaunchConfig_t cfg{};
   // a row per thread block for as many rows as a tile is likely to have (the
   // kernel walks any number)

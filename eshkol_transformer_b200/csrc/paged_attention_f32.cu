@@ -574,6 +574,7 @@ paged_attention_f32_kernel(const __grid_constant__ CUtensorMap k_map,
       }
       pair_sync();
       l = row_value[row];
+      pair_sync();  // read before the next tile's queries write there
       if (ok) {
         tc_fence_after();
         const float inv = l > 0.0f ? 1.0f / l : 0.0f;

@@ -518,7 +518,12 @@ def test_sampling_extreme_scales(lib, cuda, scale, temperature):
 
 
 def test_sampling_vocabulary_beyond_a_cluster(lib, cuda):
-    """More logits than the shared memory of a cluster holds: read from memory."""
+    """More logits than the shared memory of a cluster holds: read from memory.
+    300,001 fill most of it."""
+    x = logits_of(2, 300001, F32, 6, sigma=1.0)
+    x[:, 1000:1010] += 14.0
+    for kw in (dict(top_k=64), dict(top_p=0.5), dict(min_p=0.3), dict(top_k=1000, top_p=0.9)):
+        check_draw(x, np.array([0.3, 0.8], np.float32), **kw, least=0.0)
     x = logits_of(2, 450001, F32, 5, sigma=1.0)
     x[:, 1000:1010] += 14.0
     u = np.array([0.3, 0.8], np.float32)
