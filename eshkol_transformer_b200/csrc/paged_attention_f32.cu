@@ -56,8 +56,9 @@ struct Layout {
   static constexpr int PAIRS = 4 * KT;                // K hi, K lo, V hi, V lo
   static constexpr int CONV = RAWS * RAW;
   static constexpr int QLO = CONV + 2 * PAIRS;
-  static constexpr int FACTORS = QLO + ROWS * DH * 2;  // [2][3][BK]: of K, exponents and factors of V
-  static constexpr int SHARED_ROWS = FACTORS + 2 * 3 * BK * 4;  // what a row's threads exchange
+  static constexpr int V_FACTORS = QLO + ROWS * DH * 2;     // [2][2][BK]: exponents and factors
+  static constexpr int K_FACTORS = V_FACTORS + 2 * 2 * BK * 4;  // [3][BK]
+  static constexpr int SHARED_ROWS = K_FACTORS + 3 * BK * 4;  // what a row's threads exchange
   static constexpr int BARS = SHARED_ROWS + 1024;
   static constexpr int SMEM = BARS + 216;
   static constexpr uint32_t S0 = 0, QH = 128, O = 192, COLS = 512;
@@ -76,10 +77,11 @@ paged_attention_f32_kernel(const __grid_constant__ CUtensorMap k_map,
                            const __grid_constant__ CUtensorMap v_map, AttendArgs a, int box_rows) {
   using L = Layout<DH>;
   extern __shared__ __align__(1024) uint8_t smem[];
-  float* factors = reinterpret_cast<float*>(smem + L::FACTORS);
+  float* v_factors = reinterpret_cast<float*>(smem + L::V_FACTORS);
+  float* k_factors = reinterpret_cast<float*>(smem + L::K_FACTORS);
   uint64_t* bars = reinterpret_cast<uint64_t*>(smem + L::BARS);
   enum {
-    RAWFULL = 0, RAWEMPTY = 6, CONVFULL = 12, CONVEMPTY = 14, SFULL = 16, PREADY = 18, PVDONE = 20,
+    RAWFULL = 0, RAWEMPTY = 6, KFULL = 12, VFULL = 14, SFULL = 16, PREADY = 18, PVDONE = 20,
     QREADY = 22, DRAIN = 23, NBARS = 25
   };
   const uint32_t bar0 = smem_u32(bars);
@@ -93,7 +95,7 @@ paged_attention_f32_kernel(const __grid_constant__ CUtensorMap k_map,
 
   if (tid == 0) {
     for (int i = 0; i < NBARS; i++)
-      mbar_init(B_(i), (i >= RAWEMPTY && i < CONVEMPTY) ? MMA_WARP - CONVERT_WARP
+      mbar_init(B_(i), (i >= RAWEMPTY && i < SFULL) ? MMA_WARP - CONVERT_WARP
                        : (i == PREADY || i == PREADY + 1 || i == QREADY) ? SOFT : 1);
     *abort = 0;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
@@ -169,7 +171,7 @@ paged_attention_f32_kernel(const __grid_constant__ CUtensorMap k_map,
       ok = wait(QREADY, items++);
       for (int j = 0; j < nb; j++, n++) {
         const uint32_t slot = n & 1u;
-        if (ok) ok = wait(CONVFULL + slot, n >> 1);
+        if (ok) ok = wait(KFULL + slot, n >> 1);
         if (ok && n >= 2) ok = wait(PVDONE + slot, (n >> 1) - 1);  // the slot held P of block n - 2
         ok = __all_sync(0xffffffffu, ok);
         if (!ok) break;
@@ -214,7 +216,6 @@ paged_attention_f32_kernel(const __grid_constant__ CUtensorMap k_map,
             umma_f16_ts(tmem + L::O, hi + 16u, vd, idesc_o, 1u);
           }
           umma_commit(B_(PVDONE + (int)slot));
-          umma_commit(B_(CONVEMPTY + (int)slot));
         }
       }
       next_tile(nb);
@@ -226,82 +227,74 @@ paged_attention_f32_kernel(const __grid_constant__ CUtensorMap k_map,
   }
   } else if (warp >= CONVERT_WARP) {
     asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kConvertRegs));
-    // ---- raw rows into pairs; warp w takes rows w RW, w RW + 1, ... of each 8 RW
+    // ---- raw rows into pairs; warp w takes rows w RW, w RW + 1, ... of each 8 RW.  A
+    // slot of K is free once its scores are done, one of V (and of the scores) once
+    // its P V is: K is a block ahead by then and the next scores need not wait.  The
+    // factors of K outlive their slot by the probabilities, so they have three.
     constexpr int LANES = DH / 4, RW = 32 / LANES;  // lanes per row, rows of a warp at once
     const int sub = lane / LANES, col = lane % LANES;
-    uint32_t count = 0;
+    uint32_t count = 0;  // tiles: K, V, K, V, ...
     bool ok = true;
     while (ok && left > 0) {
       const int nb = blocks_here(), visible = tile_visible(a.tiling, p.r, p.tile);
-      for (int j = 0; j < nb; j++, n++) {
-        const int valid = visible - (p.blk + j) * BK;
-        const uint32_t conv = base + L::CONV + (n & 1u) * L::PAIRS;
-        float* f = factors + (n & 1u) * 3 * BK;
-        if (n >= 2) ok = wait(CONVEMPTY + (n & 1u), (n >> 1) - 1);
-        const uint32_t sk = count % L::RAWS, sv = (count + 1) % L::RAWS;
-        if (ok) ok = wait(RAWFULL + sk, count / L::RAWS);
-        if (ok) ok = wait(RAWFULL + sv, (count + 1) / L::RAWS);
-        count += 2;
-        // rows of both tiles at once: loads, then maxima, then stores
-        constexpr int STEP = 8 * RW, AT_ONCE = 2;
 #pragma unroll 1
-        for (int r0 = 0; r0 < BK && ok; r0 += AT_ONCE * STEP) {
+      for (int i = 0; i < 2 * nb; i++, count++) {
+        const int kv = i & 1, valid = visible - (p.blk + (i >> 1)) * BK;
+        const uint32_t s = count % L::RAWS, block = count >> 1;
+        const uint32_t conv = base + L::CONV + (block & 1u) * L::PAIRS + (uint32_t)kv * 2u * L::KT;
+        float* vf = v_factors + (block & 1u) * 2 * BK;
+        float* kf = k_factors + block % 3u * BK;
+        if (block >= 2) ok = wait((kv == 0 ? SFULL : PVDONE) + (block & 1u), (block >> 1) - 1);
+        if (ok) ok = wait(RAWFULL + s, count / L::RAWS);
+        ok = __all_sync(0xffffffffu, ok);
+        if (!ok) break;
+        // four rows at once: loads, then maxima, then stores
+        constexpr int STEP = 8 * RW, AT_ONCE = 4;
+#pragma unroll 1
+        for (int r0 = 0; r0 < BK; r0 += AT_ONCE * STEP) {
           const int row0 = r0 + (warp - CONVERT_WARP) * RW + sub;
-          float4 x[2][AT_ONCE];
-          float m[2][AT_ONCE];
+          float4 x[AT_ONCE];
+          float m[AT_ONCE];
 #pragma unroll
-          for (int kv = 0; kv < 2; kv++)
-#pragma unroll
-            for (int k = 0; k < AT_ONCE; k++) {
-              const int row = row0 + k * STEP;
-              x[kv][k] = make_float4(0.f, 0.f, 0.f, 0.f);
-              if (row < valid)
-                x[kv][k] = lds128(base + (kv == 0 ? sk : sv) * L::RAW + (uint32_t)(row * DH + 4 * col) * 4u);
-              m[kv][k] = abs_max4(0.0f, x[kv][k]);
-            }
+          for (int k = 0; k < AT_ONCE; k++) {
+            const int row = row0 + k * STEP;
+            x[k] = make_float4(0.f, 0.f, 0.f, 0.f);
+            if (row < valid) x[k] = lds128(base + s * L::RAW + (uint32_t)(row * DH + 4 * col) * 4u);
+            m[k] = abs_max4(0.0f, x[k]);
+          }
 #pragma unroll
           for (int o = LANES / 2; o > 0; o >>= 1)
 #pragma unroll
-            for (int i = 0; i < 2 * AT_ONCE; i++)
-              m[i & 1][i >> 1] = fmaxf(m[i & 1][i >> 1], __shfl_xor_sync(0xffffffffu, m[i & 1][i >> 1], o));
+            for (int k = 0; k < AT_ONCE; k++) m[k] = fmaxf(m[k], __shfl_xor_sync(0xffffffffu, m[k], o));
 #pragma unroll
           for (int k = 0; k < AT_ONCE; k++) {
             const int row = row0 + k * STEP;
             const uint32_t piece = ((uint32_t)col & 15u) >> 1;
-            const uint32_t at = conv + (uint32_t)(col >> 4) * BK * 128u + (uint32_t)row * 128u +
+            const uint32_t to = conv + (uint32_t)(col >> 4) * BK * 128u + (uint32_t)row * 128u +
                                 ((piece ^ (uint32_t)(row & 7)) << 4) + (uint32_t)(col & 1) * 8u;
-#pragma unroll
-            for (int kv = 0; kv < 2; kv++) {
-              const int e = row_exponent(m[kv][k]);
-              const float sc = exp2_int(e);
-              float h0, l0, h1, l1;
-              pair2(x[kv][k].x * sc, x[kv][k].y * sc, h0, l0);
-              pair2(x[kv][k].z * sc, x[kv][k].w * sc, h1, l1);
-              const uint32_t to = at + (uint32_t)kv * 2u * L::KT;
-              asm volatile("st.shared.v2.f32 [%0], {%1, %2};" ::"r"(to), "f"(h0), "f"(h1) : "memory");
-              asm volatile("st.shared.v2.f32 [%0], {%1, %2};" ::"r"(to + L::KT), "f"(l0), "f"(l1)
-                           : "memory");
-              if (col == 0) {
-                if (kv == 0) {
-                  f[row] = exp2_int(-e);
-                } else {
-                  f[BK + row] = (float)-e;
-                  f[2 * BK + row] = sc;
-                }
+            const int e = row_exponent(m[k]);
+            const float sc = exp2_int(e);
+            float h0, l0, h1, l1;
+            pair2(x[k].x * sc, x[k].y * sc, h0, l0);
+            pair2(x[k].z * sc, x[k].w * sc, h1, l1);
+            asm volatile("st.shared.v2.f32 [%0], {%1, %2};" ::"r"(to), "f"(h0), "f"(h1) : "memory");
+            asm volatile("st.shared.v2.f32 [%0], {%1, %2};" ::"r"(to + L::KT), "f"(l0), "f"(l1) : "memory");
+            if (col == 0) {
+              if (kv == 0) {
+                kf[row] = exp2_int(-e);
+              } else {
+                vf[row] = (float)-e;
+                vf[BK + row] = sc;
               }
             }
           }
         }
-        __syncwarp();
-        if (ok && lane == 0) {
-          mbar_arrive(B_(RAWEMPTY + sk));
-          mbar_arrive(B_(RAWEMPTY + sv));
-        }
-        ok = __all_sync(0xffffffffu, ok);
-        if (!ok) break;
         fence_async_smem();
         __syncwarp();
-        if (lane == 0) mbar_arrive(B_(CONVFULL + (n & 1u)));
+        if (lane == 0) {
+          mbar_arrive(B_(RAWEMPTY + s));
+          mbar_arrive(B_((kv == 0 ? KFULL : VFULL) + (block & 1u)));
+        }
       }
       next_tile(nb);
     }
@@ -474,7 +467,7 @@ paged_attention_f32_kernel(const __grid_constant__ CUtensorMap k_map,
           have_part = true;
           m_part = m == -INFINITY ? 0.0f : m;
         }
-        if (ok) ok = wait(CONVFULL + (n & 1u), n >> 1);  // the factors
+        if (ok) ok = wait(VFULL + (n & 1u), n >> 1);  // the factors of both: K's come first
         if (ok) ok = wait(SFULL + (n & 1u), n >> 1);
         ok = __all_sync(0xffffffffu, ok);
         tc_fence_after();
@@ -482,7 +475,8 @@ paged_attention_f32_kernel(const __grid_constant__ CUtensorMap k_map,
         const int key0 = (p.blk + j) * BK;
         const bool masked = key0 + BK > vis_warp;
         const int seen = vis - key0 - 32 * half;
-        const uint32_t f_at = smem_u32(factors + (n & 1u) * 3 * BK) + 128u * (uint32_t)half;
+        const uint32_t kf_at = smem_u32(k_factors + n % 3u * BK) + 128u * (uint32_t)half;
+        const uint32_t vf_at = smem_u32(v_factors + (n & 1u) * 2 * BK) + 128u * (uint32_t)half;
         // this thread's scores in base 2, exponents of their values added
         uint64_t s2[16];
         {
@@ -491,7 +485,7 @@ paged_attention_f32_kernel(const __grid_constant__ CUtensorMap k_map,
           const uint64_t cq2 = twice(cq);
 #pragma unroll
           for (int i = 0; i < 32; i += 4) {
-            const float4 kf = lds128(f_at + 4u * i), ge = lds128(f_at + 4u * (BK + i));
+            const float4 kf = lds128(kf_at + 4u * i), ge = lds128(vf_at + 4u * i);
             s2[i / 2] = fma2(mul2(pk(s[i], s[i + 1]), cq2), pk(kf.x, kf.y), pk(ge.x, ge.y));
             s2[i / 2 + 1] = fma2(mul2(pk(s[i + 2], s[i + 3]), cq2), pk(kf.z, kf.w), pk(ge.z, ge.w));
           }
@@ -541,7 +535,7 @@ paged_attention_f32_kernel(const __grid_constant__ CUtensorMap k_map,
         float hi[16], lo[16];
 #pragma unroll
         for (int i = 0; i < 16; i += 2) {
-          const float4 vf = lds128(f_at + 4u * (2 * BK + 2 * i));
+          const float4 vf = lds128(vf_at + 4u * (BK + 2 * i));
 #pragma unroll
           for (int k = 0; k < 2; k++) {
             const float2 x = unpk(add2(s2[i + k], from2));
