@@ -11,19 +11,25 @@
 // M the running maximum of s_j + g_j, so cached rows of any magnitude need no
 // pass of their own.
 //
-// A tile is 128 rows (TMEM lanes), a block 64 keys.  Warp 18 copies raw K and V
-// tiles by TMA, warps 8-15 turn them into pairs (a row by DH / 4 lanes: maximum,
-// exponent, split) in shared memory, warp 16 issues S = Q K^T up to a block ahead
-// of warp 17's O += P V, warps 0-7 (two threads per row, 32 keys each) form the
-// probabilities, whose pair replaces the scores in TMEM.  A single warp per
+// A tile is 128 rows (TMEM lanes), a block 64 keys.  One warp copies raw K and V
+// tiles by TMA, two teams of four warps turn them into pairs (a row by all lanes of
+// a warp: maximum, exponent, split) in shared memory, a team for K and one for V: K's
+// slot is free again when its scores are done, V's when its P V is, so the next
+// scores never wait for a conversion.  One warp issues S = Q K^T up to a block ahead
+// of another one's O += P V, and 2 threads per row (4 at more than 64 dims) form
+// the probabilities, whose pair replaces the scores in TMEM.  A single warp per
 // scheduler issues an instruction of such code every five or six cycles, so both
-// kinds of arithmetic have two.  P hi times
-// [V hi | V lo] is one product of N = 2 head_dim; the halves of O are added
-// when it is read.  The tensor pipe's f32 accumulation truncates, so every
-// CHUNK blocks O moves to f32 sums in the workspace (each thread its row).
-// Four ragged prompts of up to 1,024 tokens (16 heads x 64) take 113 us (307 us on
-// mma.sync): 3,700 cycles per block of 64 keys, bound by the probabilities'
-// instructions.  Waits are bounded as in paged_attention_tc.cu.
+// kinds of arithmetic have at least two.  P hi times [V hi | V lo] is one product of
+// N = 2 head_dim; the halves of O are added when it is read.  The tensor pipe's f32
+// accumulation truncates, so every CHUNK blocks O moves to f32 sums in the
+// workspace.
+// Four ragged prompts of up to 1,024 tokens (16 heads x 64) take 91 us (307 us on
+// mma.sync; 98 with one conversion of both tiles per block), the same with 9,000
+// keys of history 631 us (731).  3,000 to 3,500 cycles per block of 64 keys and
+// 11,000 per tile for its queries and output: instructions bound it, and their
+// cache, which the roles' code together overflows (100 KB; 10 % of its requests miss),
+// so what runs seldom or waits anyway is not unrolled.
+// Waits are bounded as in paged_attention_tc.cu.
 #include <math.h>
 
 #include <type_traits>
@@ -38,10 +44,7 @@ using namespace paged;
 using namespace f16att;
 
 constexpr int ROWS = 128, BK = 64;
-constexpr int SOFT = 256, CONVERT_WARP = 8, MMA_WARP = 16, LOAD_WARP = 18, THREADS = 640;
-// registers of the warpgroups: probabilities, conversion, the rest
-constexpr int kSoftRegs = 136, kConvertRegs = 72, kLeanRegs = 48;
-static_assert(256 * kSoftRegs + 256 * kConvertRegs + 128 * kLeanRegs <= THREADS * 96, "registers at launch");
+constexpr int TEAM = 4;  // warps that convert K, and as many for V
 constexpr float kJump = 8.0f;   // log2 of the largest P the standing maximum allows
 constexpr float kShift = 7.0f;  // P carries 2^7: at most 2^15
 constexpr int CHUNK = 8;        // blocks whose products one TMEM accumulator adds
@@ -50,17 +53,27 @@ __device__ int g_wait_error;  // bounded waits that gave up (the status word tel
 
 template <int DH>
 struct Layout {
+  static constexpr int PARTS = DH / 32, KEYS = BK / PARTS;  // threads of a row, keys of one
+  static constexpr int SOFT = ROWS * PARTS, CONVERT_WARP = SOFT / 32, MMA_WARP = CONVERT_WARP + 2 * TEAM,
+                       LOAD_WARP = MMA_WARP + 2, THREADS = 32 * (MMA_WARP + 4);
+  // registers of the warpgroups: probabilities, conversion, the rest
+  static constexpr int REGS = DH == 128 ? 72 : 96, SOFT_REGS = DH == 128 ? 88 : 136,
+                       CONVERT_REGS = DH == 128 ? 56 : 72, LEAN_REGS = DH == 128 ? 40 : 48;
+  static_assert(SOFT * SOFT_REGS + 256 * CONVERT_REGS + 128 * LEAN_REGS <= THREADS * REGS &&
+                    THREADS * REGS <= 65536, "registers at launch");
   static constexpr int RAW = BK * DH * 4;             // one raw tile of K or V
   static constexpr int RAWS = DH == 128 ? 2 : 6;      // tiles in the ring: K, V, K, V, ...
   static constexpr int KT = BK * DH * 2;              // one binary16 tile
-  static constexpr int PAIRS = 4 * KT;                // K hi, K lo, V hi, V lo
-  static constexpr int CONV = RAWS * RAW;
-  static constexpr int QLO = CONV + 2 * PAIRS;
-  static constexpr int V_FACTORS = QLO + ROWS * DH * 2;     // [2][2][BK]: exponents and factors
-  static constexpr int K_FACTORS = V_FACTORS + 2 * 2 * BK * 4;  // [3][BK]
+  static constexpr int PAIR = 2 * KT;                 // hi, lo
+  static constexpr int VS = DH == 128 ? 2 : 3;        // slots of V (of K: 2)
+  static constexpr int KP = RAWS * RAW, VP = KP + 2 * PAIR;
+  static constexpr int QLO = VP + VS * PAIR;
+  static constexpr int V_FACTORS = QLO + ROWS * DH * 2;     // [VS][2][BK]: exponents and factors
+  static constexpr int K_FACTORS = V_FACTORS + VS * 2 * BK * 4;  // [3][BK]
   static constexpr int SHARED_ROWS = K_FACTORS + 3 * BK * 4;  // what a row's threads exchange
-  static constexpr int BARS = SHARED_ROWS + 1024;
-  static constexpr int SMEM = BARS + 216;
+  static constexpr int MAXIMA = DH == 128 ? 1 : 2;            // buffers of the rows' maxima
+  static constexpr int BARS = SHARED_ROWS + MAXIMA * PARTS * ROWS * 2;
+  static constexpr int SMEM = BARS + 8 * (2 * RAWS + 2 * VS + 13) + 8;
   static constexpr uint32_t S0 = 0, QH = 128, O = 192, COLS = 512;
   static_assert(O + 2 * DH <= COLS && QH + DH / 2 <= O && SMEM <= 232448, "TMEM and shared memory");
 };
@@ -72,17 +85,19 @@ __device__ __forceinline__ int row_exponent(float amax) {
 }
 
 template <int DH>
-__global__ void __launch_bounds__(THREADS, 1)
+__global__ void __launch_bounds__(Layout<DH>::THREADS, 1)
 paged_attention_f32_kernel(const __grid_constant__ CUtensorMap k_map,
                            const __grid_constant__ CUtensorMap v_map, AttendArgs a, int box_rows) {
   using L = Layout<DH>;
+  constexpr int CONVERT_WARP = L::CONVERT_WARP, MMA_WARP = L::MMA_WARP;
   extern __shared__ __align__(1024) uint8_t smem[];
   float* v_factors = reinterpret_cast<float*>(smem + L::V_FACTORS);
   float* k_factors = reinterpret_cast<float*>(smem + L::K_FACTORS);
   uint64_t* bars = reinterpret_cast<uint64_t*>(smem + L::BARS);
   enum {
-    RAWFULL = 0, RAWEMPTY = 6, KFULL = 12, VFULL = 14, SFULL = 16, PREADY = 18, PVDONE = 20,
-    QREADY = 22, DRAIN = 23, NBARS = 25
+    RAWFULL = 0, RAWEMPTY = L::RAWS, KFULL = 2 * L::RAWS, VFULL = KFULL + 3, SFULL = VFULL + L::VS,
+    PREADY = SFULL + 2, PVDONE = PREADY + 2, KFREE = PVDONE + L::VS, QREADY = KFREE + 3,
+    DRAIN = QREADY + 1, NBARS = DRAIN + 2
   };
   const uint32_t bar0 = smem_u32(bars);
   auto B_ = [&](int i) { return bar0 + 8u * (uint32_t)i; };
@@ -95,15 +110,16 @@ paged_attention_f32_kernel(const __grid_constant__ CUtensorMap k_map,
 
   if (tid == 0) {
     for (int i = 0; i < NBARS; i++)
-      mbar_init(B_(i), (i >= RAWEMPTY && i < SFULL) ? MMA_WARP - CONVERT_WARP
-                       : (i == PREADY || i == PREADY + 1 || i == QREADY) ? SOFT : 1);
+      mbar_init(B_(i), (i >= RAWEMPTY && i < SFULL) ? TEAM
+                       : (i >= KFREE && i < QREADY) ? CONVERT_WARP
+                       : (i == PREADY || i == PREADY + 1 || i == QREADY) ? L::SOFT : 1);
     *abort = 0;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
   if (warp == MMA_WARP) tmem_alloc(smem_u32(tslot), L::COLS);
   Place p;
   const Share share = divide(a.tiling, a.batch, a.least, p,
-                             *reinterpret_cast<DivideRoom<THREADS>*>(smem + L::QLO));
+                             *reinterpret_cast<DivideRoom<L::THREADS>*>(smem + L::QLO));
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
@@ -118,11 +134,12 @@ paged_attention_f32_kernel(const __grid_constant__ CUtensorMap k_map,
   auto wait = [&](int i, uint32_t parity) {
     return role_wait(B_(i), parity & 1u, &g_wait_error, abort);
   };
+  auto pv_done = [&](uint32_t block) { return PVDONE + (int)(block % L::VS); };
   uint32_t n = 0;  // blocks so far, of all tiles: slot n & 1, round n >> 1
 
   if (warp >= MMA_WARP) {
-    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kLeanRegs));
-  if (warp == LOAD_WARP) {
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(L::LEAN_REGS));
+  if (warp == L::LOAD_WARP) {
     // ---- raw tiles, page by page
     uint32_t count = 0;
     bool ok = true;
@@ -141,7 +158,7 @@ paged_attention_f32_kernel(const __grid_constant__ CUtensorMap k_map,
             page = -1;  // outside the map: filled with zeros
           }
         }
-#pragma unroll
+#pragma unroll 1
         for (int kv = 0; kv < 2; kv++) {
           const uint32_t s = count % L::RAWS, round = count / L::RAWS;
           if (ok && round > 0) ok = wait(RAWEMPTY + s, round - 1);
@@ -171,14 +188,14 @@ paged_attention_f32_kernel(const __grid_constant__ CUtensorMap k_map,
       ok = wait(QREADY, items++);
       for (int j = 0; j < nb; j++, n++) {
         const uint32_t slot = n & 1u;
-        if (ok) ok = wait(KFULL + slot, n >> 1);
-        if (ok && n >= 2) ok = wait(PVDONE + slot, (n >> 1) - 1);  // the slot held P of block n - 2
+        if (ok) ok = wait(KFULL + n % 3u, n / 3u);
+        if (ok && n >= 2) ok = wait(pv_done(n - 2), (n - 2) / L::VS);  // the slot held P of block n - 2
         ok = __all_sync(0xffffffffu, ok);
         if (!ok) break;
         tc_fence_after();
         if (lane == 0) {
-          const uint32_t k = base + L::CONV + slot * L::PAIRS, d = tmem + L::S0 + 64u * slot;
-#pragma unroll
+          const uint32_t k = base + L::KP + slot * L::PAIR, d = tmem + L::S0 + 64u * slot;
+#pragma unroll 1
           for (int i = 0; i < DH / 16; i++) {
             const uint64_t kh = kdesc16<BK>(k, i);
             umma_f16(d, kdesc16<ROWS>(base + L::QLO, i), kh, idesc_s, i > 0 ? 1u : 0u);
@@ -206,16 +223,16 @@ paged_attention_f32_kernel(const __grid_constant__ CUtensorMap k_map,
         if (!ok) break;
         tc_fence_after();
         if (lane == 0) {
-          const uint32_t v = base + L::CONV + slot * L::PAIRS + 2u * L::KT;
+          const uint32_t v = base + L::VP + n % L::VS * L::PAIR;
           const uint32_t pa = tmem + L::S0 + 64u * slot;
-#pragma unroll
+#pragma unroll 1
           for (int i = 0; i < BK / 16; i++) {
             const uint64_t vd = mdesc16<BK>(v, i);  // V lo lies one chunk stride behind V hi
-            const uint32_t hi = pa + 32u * (i / 2) + 8u * (i % 2);
+            const uint32_t hi = pa + 16u * i;
             umma_f16_ts(tmem + L::O, hi, vd, idesc_o2, (j % CHUNK != 0 || i > 0) ? 1u : 0u);
-            umma_f16_ts(tmem + L::O, hi + 16u, vd, idesc_o, 1u);
+            umma_f16_ts(tmem + L::O, hi + 8u, vd, idesc_o, 1u);
           }
-          umma_commit(B_(PVDONE + (int)slot));
+          umma_commit(B_(pv_done(n)));
         }
       }
       next_tile(nb);
@@ -226,92 +243,126 @@ paged_attention_f32_kernel(const __grid_constant__ CUtensorMap k_map,
     }
   }
   } else if (warp >= CONVERT_WARP) {
-    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kConvertRegs));
-    // ---- raw rows into pairs; warp w takes rows w RW, w RW + 1, ... of each 8 RW.  A
-    // slot of K is free once its scores are done, one of V (and of the scores) once
-    // its P V is: K is a block ahead by then and the next scores need not wait.  The
-    // factors of K outlive their slot by the probabilities, so they have three.
-    constexpr int LANES = DH / 4, RW = 32 / LANES;  // lanes per row, rows of a warp at once
-    const int sub = lane / LANES, col = lane % LANES;
-    uint32_t count = 0;  // tiles: K, V, K, V, ...
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(L::CONVERT_REGS));
+    // ---- raw rows into pairs: a team of warps for K, one for V; a warp takes 16
+    // rows, a row at a time all its lanes.  A slot of K is free once its scores are
+    // done, one of V once its P V is.  The factors of K outlive their slot by the
+    // probabilities, so they have three.
+    constexpr int W = DH / 32, AT_ONCE = DH == 64 ? 8 : 4;  // dims of a lane, rows at once
+    const int kv = (warp - CONVERT_WARP) / TEAM, row0 = 16 * ((warp - CONVERT_WARP) % TEAM);
     bool ok = true;
     while (ok && left > 0) {
       const int nb = blocks_here(), visible = tile_visible(a.tiling, p.r, p.tile);
 #pragma unroll 1
-      for (int i = 0; i < 2 * nb; i++, count++) {
-        const int kv = i & 1, valid = visible - (p.blk + (i >> 1)) * BK;
-        const uint32_t s = count % L::RAWS, block = count >> 1;
-        const uint32_t conv = base + L::CONV + (block & 1u) * L::PAIRS + (uint32_t)kv * 2u * L::KT;
-        float* vf = v_factors + (block & 1u) * 2 * BK;
-        float* kf = k_factors + block % 3u * BK;
-        if (block >= 2) ok = wait((kv == 0 ? SFULL : PVDONE) + (block & 1u), (block >> 1) - 1);
-        if (ok) ok = wait(RAWFULL + s, count / L::RAWS);
+      for (int j = 0; j < nb; j++, n++) {
+        const int valid = visible - (p.blk + j) * BK;
+        const uint32_t s = (2 * n + kv) % L::RAWS, third = n % 3u;
+        const uint32_t v_slot = n % L::VS;
+        const uint32_t conv = base + (kv == 0 ? L::KP + (n & 1u) * L::PAIR : L::VP + v_slot * L::PAIR);
+        if (kv == 0) {
+          if (n >= 2) ok = wait(SFULL + (n & 1u), (n >> 1) - 1);
+          if (ok && n >= 3) ok = wait(KFREE + third, n / 3u - 1);
+        } else if (n >= L::VS) {
+          ok = wait(PVDONE + v_slot, n / L::VS - 1);
+        }
+        if (ok) ok = wait(RAWFULL + s, (2 * n + kv) / L::RAWS);
         ok = __all_sync(0xffffffffu, ok);
         if (!ok) break;
-        // four rows at once: loads, then maxima, then stores
-        constexpr int STEP = 8 * RW, AT_ONCE = 4;
+        // AT_ONCE rows at a time: loads, then maxima, then stores
+        const uint32_t raw = base + s * L::RAW + (uint32_t)(row0 * DH + W * lane) * 4u;
+        const uint32_t to = conv + (uint32_t)(lane * W / 64) * BK * 128u + (uint32_t)row0 * 128u;
+        int mine = 0;  // exponent of row row0 + lane
 #pragma unroll 1
-        for (int r0 = 0; r0 < BK; r0 += AT_ONCE * STEP) {
-          const int row0 = r0 + (warp - CONVERT_WARP) * RW + sub;
-          float4 x[AT_ONCE];
-          float m[AT_ONCE];
+        for (int r0 = 0; r0 < 16; r0 += AT_ONCE) {
+          float2 x[AT_ONCE][W / 2];
+          uint32_t m[AT_ONCE];
 #pragma unroll
           for (int k = 0; k < AT_ONCE; k++) {
-            const int row = row0 + k * STEP;
-            x[k] = make_float4(0.f, 0.f, 0.f, 0.f);
-            if (row < valid) x[k] = lds128(base + s * L::RAW + (uint32_t)(row * DH + 4 * col) * 4u);
-            m[k] = abs_max4(0.0f, x[k]);
+            const uint32_t from = raw + (uint32_t)((r0 + k) * DH) * 4u;
+            if constexpr (W == 4) {
+              const float4 y = lds128(from);
+              x[k][0] = make_float2(y.x, y.y);
+              x[k][1] = make_float2(y.z, y.w);
+            } else {
+              asm volatile("ld.shared.v2.f32 {%0, %1}, [%2];" : "=f"(x[k][0].x), "=f"(x[k][0].y) : "r"(from) : "memory");
+            }
+            if (row0 + r0 + k >= valid)  // slots behind may hold anything
+#pragma unroll
+              for (int i = 0; i < W / 2; i++) x[k][i] = make_float2(0.f, 0.f);
+            float top = 0.0f;
+#pragma unroll
+            for (int i = 0; i < W / 2; i++) top = fmaxf(top, fmaxf(fabsf(x[k][i].x), fabsf(x[k][i].y)));
+            m[k] = __float_as_uint(top);
           }
 #pragma unroll
-          for (int o = LANES / 2; o > 0; o >>= 1)
-#pragma unroll
-            for (int k = 0; k < AT_ONCE; k++) m[k] = fmaxf(m[k], __shfl_xor_sync(0xffffffffu, m[k], o));
+          for (int k = 0; k < AT_ONCE; k++) m[k] = __reduce_max_sync(0xffffffffu, m[k]);
 #pragma unroll
           for (int k = 0; k < AT_ONCE; k++) {
-            const int row = row0 + k * STEP;
-            const uint32_t piece = ((uint32_t)col & 15u) >> 1;
-            const uint32_t to = conv + (uint32_t)(col >> 4) * BK * 128u + (uint32_t)row * 128u +
-                                ((piece ^ (uint32_t)(row & 7)) << 4) + (uint32_t)(col & 1) * 8u;
-            const int e = row_exponent(m[k]);
-            const float sc = exp2_int(e);
-            float h0, l0, h1, l1;
-            pair2(x[k].x * sc, x[k].y * sc, h0, l0);
-            pair2(x[k].z * sc, x[k].w * sc, h1, l1);
-            asm volatile("st.shared.v2.f32 [%0], {%1, %2};" ::"r"(to), "f"(h0), "f"(h1) : "memory");
-            asm volatile("st.shared.v2.f32 [%0], {%1, %2};" ::"r"(to + L::KT), "f"(l0), "f"(l1) : "memory");
-            if (col == 0) {
-              if (kv == 0) {
-                kf[row] = exp2_int(-e);
-              } else {
-                vf[row] = (float)-e;
-                vf[BK + row] = sc;
-              }
+            const int r = r0 + k, e = row_exponent(__uint_as_float(m[k]));
+            const uint64_t sc = twice(exp2_int(e));
+            mine = lane == r ? e : mine;
+            uint32_t hi[W / 2], lo[W / 2];
+#pragma unroll
+            for (int i = 0; i < W / 2; i++) {
+              const uint64_t y = mul2(pk(x[k][i].x, x[k][i].y), sc);
+              const float2 f = unpk(y);
+              const __half2 h = __floats2half2_rn(f.x, f.y);
+              const float2 hf = __half22float2(h), rest = unpk(fma2(pk(hf.x, hf.y), twice(-1.0f), y));
+              const __half2 l = __floats2half2_rn(rest.x, rest.y);
+              hi[i] = *reinterpret_cast<const uint32_t*>(&h);
+              lo[i] = *reinterpret_cast<const uint32_t*>(&l);
             }
+            // byte 2 W lane of the row's 128 (of each 64 dims), 16-byte pieces swizzled
+            const uint32_t byte = 2u * W * ((uint32_t)lane % (64 / W)), at = to + 128u * r + (byte ^ (uint32_t)((AT_ONCE == 8 ? k : r & 7) << 4));
+            if constexpr (W == 4) {
+              asm volatile("st.shared.v2.b32 [%0], {%1, %2};" ::"r"(at), "r"(hi[0]), "r"(hi[W / 2 - 1]) : "memory");
+              asm volatile("st.shared.v2.b32 [%0], {%1, %2};" ::"r"(at + L::KT), "r"(lo[0]), "r"(lo[W / 2 - 1]) : "memory");
+            } else {
+              asm volatile("st.shared.b32 [%0], %1;" ::"r"(at), "r"(hi[0]) : "memory");
+              asm volatile("st.shared.b32 [%0], %1;" ::"r"(at + L::KT), "r"(lo[0]) : "memory");
+            }
+          }
+        }
+        if (lane < 16) {
+          if (kv == 0) {
+            k_factors[third * BK + row0 + lane] = exp2_int(-mine);
+          } else {
+            float* f = v_factors + v_slot * 2 * BK + row0 + lane;
+            f[0] = (float)-mine;
+            f[BK] = exp2_int(mine);
           }
         }
         fence_async_smem();
         __syncwarp();
         if (lane == 0) {
           mbar_arrive(B_(RAWEMPTY + s));
-          mbar_arrive(B_((kv == 0 ? KFULL : VFULL) + (block & 1u)));
+          mbar_arrive(B_(kv == 0 ? KFULL + third : VFULL + v_slot));
         }
       }
       next_tile(nb);
     }
   } else {
-    asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kSoftRegs));
-    // ---- probabilities: two threads per row, keys 32 half .. 32 half + 31 of a block
-    const int quarter = warp & 3, half = warp >> 2, row = quarter * 32 + lane;
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(L::SOFT_REGS));
+    // ---- probabilities: thread `which` of a row takes keys KEYS which .. of a block
+    constexpr int PARTS = L::PARTS, KEYS = L::KEYS;
+    const int quarter = warp & 3, which = warp >> 2, row = quarter * 32 + lane;
     const uint32_t lanes = tmem + ((uint32_t)(quarter * 32) << 16);
-    __nv_bfloat16* row_max = reinterpret_cast<__nv_bfloat16*>(smem + L::SHARED_ROWS);  // [2][2][ROWS]
-    float* row_value = reinterpret_cast<float*>(smem + L::SHARED_ROWS);                // [ROWS], between tiles
-    auto pair_sync = [&]() { named_sync(1 + quarter, 64); };
+    const uint32_t o_at = lanes + L::O;
+    uint8_t* q_lo = smem + L::QLO;
+    uint8_t* shared_rows = smem + L::SHARED_ROWS;
+    __nv_bfloat16* row_max = reinterpret_cast<__nv_bfloat16*>(shared_rows);  // [MAXIMA][PARTS][ROWS]
+    float* row_value = reinterpret_cast<float*>(shared_rows);                // [ROWS], before a tile
+    // behind a tile the memory of a quarter's queries passes on its row sums
+    // [PARTS][32], then its output, 16 columns of 32 rows per warp at a time
+    float* row_sums = reinterpret_cast<float*>(q_lo + quarter * 4096);
+    const uint32_t stage = smem_u32(q_lo + (which >> 1) * ROWS * 128 + quarter * 4096 + (which & 1) * 2048);
+    auto row_sync = [&]() { named_sync(1 + quarter, 32 * PARTS); };
     const bool q_vec = ((reinterpret_cast<uintptr_t>(a.q) | (uintptr_t)(a.q_stride * 4)) & 15) == 0;
     const bool rope_vec = ((reinterpret_cast<uintptr_t>(a.rope.cos) | reinterpret_cast<uintptr_t>(a.rope.sin)) & 7) == 0;
     const bool o_vec = ((reinterpret_cast<uintptr_t>(a.o) | (uintptr_t)(a.o_stride * 4)) & 15) == 0;
     bool ok = true;
     Cut cut{0, 0, 0, 0, 0};
-    // after a wait that ran out the loops still end, in step with the other thread
+    // after a wait that ran out the loops still end, in step with the other threads
     // of the row
     while (left > 0) {
       const int nb = blocks_here(), rows = min(ROWS, p.r.n * group - p.tile * ROWS);
@@ -326,28 +377,29 @@ paged_attention_f32_kernel(const __grid_constant__ CUtensorMap k_map,
       const int pos = p.r.len - p.r.n + token, vis = valid ? max(0, pos + 1) : 0;
       const int vis_warp = __shfl_sync(0xffffffffu, max(0, pos + 1), 0);
       float cq = 0.0f;
-      // ---- the warp's 16 rows of Q, rotated: 8 lanes a row, whole lines.  hi passes
+      // ---- the warp's rows of Q, rotated: 8 lanes a row, whole lines.  hi passes
       // through the tile of lo on its way into TMEM (a row per lane), then lo takes
       // the tile.
       {
         constexpr int P = DH / 32;  // 16-byte pieces of a lane
-        const uint32_t tile = base + L::QLO;
-        constexpr int G = 2;  // groups of 4 rows whose loads are in flight
+        const uint32_t tile = smem_u32(q_lo);
+        constexpr int FOURS = 32 / PARTS / 4, G = DH == 128 ? 1 : FOURS;  // groups of 4 rows; in flight
+        const int own = quarter * 32 + which * (32 / PARTS) + (lane >> 3);    // this lane's row of the first
         auto unit_at = [&](int r, int i) {
           const int c = (lane & 7) + 8 * i;  // 8-byte unit of the row
           return tile + (uint32_t)(c >> 4) * ROWS * 128u + (uint32_t)r * 128u +
                  (((((uint32_t)c & 15u) >> 1) ^ (uint32_t)(r & 7)) << 4) + (uint32_t)(c & 1) * 8u;
         };
-        float low[4][P][2];
+        float low[FOURS][P][2];
 #pragma unroll
-        for (int g0 = 0; g0 < 4; g0 += G) {
+        for (int g0 = 0; g0 < FOURS; g0 += G) {
           // all loads first: rows and dims that are not there read the tensor's or
           // the table's beginning
           float4 x[G][P];
           float2 cs[G][P], sn[G][P];
 #pragma unroll
           for (int k = 0; k < G; k++) {
-            const int r = quarter * 32 + half * 16 + 4 * (g0 + k) + (lane >> 3), gr = p.tile * ROWS + r;
+            const int r = own + 4 * (g0 + k), gr = p.tile * ROWS + r;
             const int t = quotient(gr, a.tiling.by_group), at_pos = p.r.len - p.r.n + t;
             const float* src = static_cast<const float*>(a.q);
             if (r < rows) src += (p.r.first + t) * a.q_stride + (int64_t)(p.h * group + gr - t * group) * dim;
@@ -371,7 +423,7 @@ paged_attention_f32_kernel(const __grid_constant__ CUtensorMap k_map,
           }
 #pragma unroll
           for (int k = 0; k < G; k++) {
-            const int r = quarter * 32 + half * 16 + 4 * (g0 + k) + (lane >> 3);
+            const int r = own + 4 * (g0 + k);
             const int at_pos = p.r.len - p.r.n + quotient(p.tile * ROWS + r, a.tiling.by_group);
             const bool turned = r < rows && at_pos >= 0 && a.rope.cos != nullptr;
             if (turned && at_pos >= a.rope.rows) report(a.batch.status, ET_B200_PAGED_BAD_ROPE);
@@ -401,28 +453,28 @@ paged_attention_f32_kernel(const __grid_constant__ CUtensorMap k_map,
             }
           }
         }
-        // hi is complete: this thread's half of its row
-        pair_sync();
+        // hi is complete: this thread's 16 columns of its row
+        row_sync();
         cq = row_value[row];
-#pragma unroll
-        for (int w = 0; w < DH / 4; w += 16) {
+        static_assert(16 * PARTS == DH / 2, "columns of a thread");
+        {
           float v[16];
 #pragma unroll
           for (int i = 0; i < 4; i++) {
-            const uint32_t u = (uint32_t)(half * (DH / 4) + w) / 4u + (uint32_t)i;
+            const uint32_t u = 4u * which + (uint32_t)i;
             const float4 f = lds128(tile + (u >> 3) * ROWS * 128u + (uint32_t)row * 128u +
                                     (((u & 7u) ^ (uint32_t)(row & 7)) << 4));
             v[4 * i] = f.x; v[4 * i + 1] = f.y; v[4 * i + 2] = f.z; v[4 * i + 3] = f.w;
           }
-          tmem_st16(lanes + L::QH + (uint32_t)(half * (DH / 4) + w), v);
+          tmem_st16(lanes + L::QH + (uint32_t)(16 * which), v);
         }
         tmem_wait_st();
-        pair_sync();
+        row_sync();
 #pragma unroll
-        for (int k = 0; k < 4; k++)
+        for (int k = 0; k < FOURS; k++)
 #pragma unroll
           for (int i = 0; i < P; i++)
-            asm volatile("st.shared.v2.f32 [%0], {%1, %2};" ::"r"(unit_at(quarter * 32 + half * 16 + 4 * k + (lane >> 3), i)),
+            asm volatile("st.shared.v2.f32 [%0], {%1, %2};" ::"r"(unit_at(own + 4 * k, i)),
                          "f"(low[k][i][0]), "f"(low[k][i][1]) : "memory");
       }
       {
@@ -430,85 +482,93 @@ paged_attention_f32_kernel(const __grid_constant__ CUtensorMap k_map,
         tc_fence_before();
         mbar_arrive(B_(QREADY));
       }
-      float* part = a.joint.sums + ((int64_t)(2 * (int)blockIdx.x + (whole ? 1 : 0)) * ROWS + row) * DH;
+      // What leaves TMEM between chunks, 32 columns from o_col of a row per thread:
+      // piece by piece, the threads side by side.  (A row per thread in place, every
+      // store reaches 32 lines and keeps the other warps from shared memory.)
+      constexpr int SIDE = 4 * ROWS * PARTS;
+      float* scratch = a.joint.stats + (int64_t)gridDim.x * 4 * ROWS +
+                       (int64_t)blockIdx.x * ROWS * DH + 4 * (which * ROWS + row);
       float m = -INFINITY, l = 0.0f, m_part = -INFINITY;
       bool have_part = false;
-      // O so far, relative to m, into v (32 columns from 32 c), with what the workspace holds
-      auto read_o = [&](int c, float (&v)[32]) {
+      static_assert(DH / PARTS == 32, "columns of a thread");
+      const int o_col = 32 * which;
+      // O so far, relative to m, with what the scratch holds
+      auto read_o = [&](float (&v)[32]) {
         float v2[32];
-        tmem_ld32(lanes + L::O + 32u * c, v);
-        tmem_ld32(lanes + L::O + (uint32_t)DH + 32u * c, v2);
+        tmem_ld32(o_at + (uint32_t)o_col, v);
+        tmem_ld32(o_at + (uint32_t)(DH + o_col), v2);
         const float f = have_part ? ex2(m_part - (m == -INFINITY ? 0.0f : m)) : 0.0f;
 #pragma unroll
         for (int i = 0; i < 32; i += 4) {
           float4 y = make_float4(0.f, 0.f, 0.f, 0.f);
-          if (have_part) y = *reinterpret_cast<const float4*>(part + 32 * c + i);
+          if (have_part) y = *reinterpret_cast<const float4*>(scratch + i / 4 * SIDE);
           v[i] = (v[i] + v2[i]) + f * y.x;
           v[i + 1] = (v[i + 1] + v2[i + 1]) + f * y.y;
           v[i + 2] = (v[i + 2] + v2[i + 2]) + f * y.z;
           v[i + 3] = (v[i + 3] + v2[i + 3]) + f * y.w;
         }
       };
-      auto write_part = [&](int c, const float (&v)[32]) {
-#pragma unroll
-        for (int i = 0; i < 32; i += 4)
-          *reinterpret_cast<float4*>(part + 32 * c + i) = make_float4(v[i], v[i + 1], v[i + 2], v[i + 3]);
-      };
       for (int j = 0; j < nb; j++, n++) {
         if (j > 0 && j % CHUNK == 0) {  // move O out: the next product starts a new accumulator
-          if (ok) ok = __all_sync(0xffffffffu, wait(PVDONE + ((n - 1) & 1u), (n - 1) >> 1));
+          if (ok) ok = __all_sync(0xffffffffu, wait(pv_done(n - 1), (n - 1) / L::VS));
           tc_fence_after();
-#pragma unroll 1
-          for (int c = half * (DH / 64); c < (half + 1) * (DH / 64); c++) {
-            float v[32];
-            read_o(c, v);
-            write_part(c, v);
-          }
+          float v[32];
+          read_o(v);
+#pragma unroll
+          for (int i = 0; i < 32; i += 4)
+            *reinterpret_cast<float4*>(scratch + i / 4 * SIDE) = make_float4(v[i], v[i + 1], v[i + 2], v[i + 3]);
           have_part = true;
           m_part = m == -INFINITY ? 0.0f : m;
         }
-        if (ok) ok = wait(VFULL + (n & 1u), n >> 1);  // the factors of both: K's come first
+        if (ok) ok = wait(KFULL + n % 3u, n / 3u) && wait(VFULL + n % L::VS, n / L::VS);  // the factors
         if (ok) ok = wait(SFULL + (n & 1u), n >> 1);
         ok = __all_sync(0xffffffffu, ok);
         tc_fence_after();
         const uint32_t s_at = lanes + L::S0 + 64u * (n & 1u);
         const int key0 = (p.blk + j) * BK;
         const bool masked = key0 + BK > vis_warp;
-        const int seen = vis - key0 - 32 * half;
-        const uint32_t kf_at = smem_u32(k_factors + n % 3u * BK) + 128u * (uint32_t)half;
-        const uint32_t vf_at = smem_u32(v_factors + (n & 1u) * 2 * BK) + 128u * (uint32_t)half;
+        const int seen = vis - key0 - KEYS * which;
+        const uint32_t kf_at = smem_u32(k_factors + n % 3u * BK + KEYS * which);
+        const uint32_t vf_at = smem_u32(v_factors + n % L::VS * 2 * BK + KEYS * which);
         // this thread's scores in base 2, exponents of their values added
-        uint64_t s2[16];
+        uint64_t s2[KEYS / 2];
         {
-          float s[32];
-          tmem_ld32(s_at + 32u * half, s);
           const uint64_t cq2 = twice(cq);
 #pragma unroll
-          for (int i = 0; i < 32; i += 4) {
-            const float4 kf = lds128(kf_at + 4u * i), ge = lds128(vf_at + 4u * i);
-            s2[i / 2] = fma2(mul2(pk(s[i], s[i + 1]), cq2), pk(kf.x, kf.y), pk(ge.x, ge.y));
-            s2[i / 2 + 1] = fma2(mul2(pk(s[i + 2], s[i + 3]), cq2), pk(kf.z, kf.w), pk(ge.z, ge.w));
+          for (int h = 0; h < KEYS; h += 16) {
+            float s[16];
+            tmem_ld16(s_at + (uint32_t)(KEYS * which + h), s);
+#pragma unroll
+            for (int i = 0; i < 16; i += 4) {
+              const float4 kf = lds128(kf_at + 4u * (h + i)), ge = lds128(vf_at + 4u * (h + i));
+              s2[(h + i) / 2] = fma2(mul2(pk(s[i], s[i + 1]), cq2), pk(kf.x, kf.y), pk(ge.x, ge.y));
+              s2[(h + i) / 2 + 1] = fma2(mul2(pk(s[i + 2], s[i + 3]), cq2), pk(kf.z, kf.w), pk(ge.z, ge.w));
+            }
           }
         }
+        __syncwarp();
+        if (lane == 0) mbar_arrive(B_(KFREE + n % 3u));
         if (masked) {
 #pragma unroll
-          for (int i = 0; i < 16; i++) {
+          for (int i = 0; i < KEYS / 2; i++) {
             const float2 v = unpk(s2[i]);
             s2[i] = pk(2 * i >= seen ? -INFINITY : v.x, 2 * i + 1 >= seen ? -INFINITY : v.y);
           }
         }
         float top[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll
-        for (int i = 0; i < 16; i++) {
+        for (int i = 0; i < KEYS / 2; i++) {
           const float2 v = unpk(s2[i]);
           top[i & 3] = fmaxf(top[i & 3], fmaxf(v.x, v.y));
         }
-        // the row's maximum over both threads, rounded up: any bound serves both
-        __nv_bfloat16* shared_max = row_max + (n & 1u) * 2 * ROWS;
-        const __nv_bfloat16 own = __float2bfloat16_ru(fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3])));
-        shared_max[half * ROWS + row] = own;
-        pair_sync();
-        const float bmax = fmaxf(__bfloat162float(own), __bfloat162float(shared_max[(1 - half) * ROWS + row]));
+        // the row's maximum over its threads, rounded up: any bound serves them
+        __nv_bfloat16* shared_max = row_max + (n & (uint32_t)(L::MAXIMA - 1)) * PARTS * ROWS + row;
+        if (L::MAXIMA == 1 && j > 0) row_sync();  // the last block's are read
+        shared_max[which * ROWS] = __float2bfloat16_ru(fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3])));
+        row_sync();
+        float bmax = -INFINITY;
+#pragma unroll
+        for (int i = 0; i < PARTS; i++) bmax = fmaxf(bmax, __bfloat162float(shared_max[i * ROWS]));
         const bool jump = bmax > m + kJump;
         if (__any_sync(0xffffffffu, jump)) {
           const float factor = jump ? ex2(m - bmax) : 1.0f;  // 0 while m is -inf
@@ -517,85 +577,97 @@ paged_attention_f32_kernel(const __grid_constant__ CUtensorMap k_map,
             l *= factor;
           }
           if (j % CHUNK != 0) {  // O holds products of this chunk: rescale it once they are complete
-            if (ok) ok = __all_sync(0xffffffffu, wait(PVDONE + ((n - 1) & 1u), (n - 1) >> 1));
+            if (ok) ok = __all_sync(0xffffffffu, wait(pv_done(n - 1), (n - 1) / L::VS));
             tc_fence_after();
 #pragma unroll 1
-            for (int c = half * (DH / 32); c < (half + 1) * (DH / 32); c++) {
+            for (int c = 2 * which; c < 2 * which + 2; c++) {
               float o[32];
-              tmem_ld32(lanes + L::O + 32u * c, o);
+              tmem_ld32(o_at + 32u * c, o);
 #pragma unroll
               for (int i = 0; i < 32; i++) o[i] *= factor;
-              tmem_st32(lanes + L::O + 32u * c, o);
+              tmem_st32(o_at + 32u * c, o);
             }
           }
         }
         const float from = (m == -INFINITY ? 0.0f : m) - kShift;
         uint64_t sum2[2] = {0, 0};
         const uint64_t from2 = twice(-from);
-        float hi[16], lo[16];
 #pragma unroll
-        for (int i = 0; i < 16; i += 2) {
-          const float4 vf = lds128(vf_at + 4u * (BK + 2 * i));
+        for (int h = 0; h < KEYS; h += 16) {
+          float pair[16];  // hi of 16 keys, then lo
 #pragma unroll
-          for (int k = 0; k < 2; k++) {
-            const float2 x = unpk(add2(s2[i + k], from2));
-            const uint64_t w = pk(ex2(x.x), ex2(x.y));
-            sum2[k] = fma2(w, k == 0 ? pk(vf.x, vf.y) : pk(vf.z, vf.w), sum2[k]);
-            const float2 w2 = unpk(w);
-            const __half2 h = __floats2half2_rn(w2.x, w2.y);
-            const float2 hf = __half22float2(h), rest = unpk(add2(w, pk(-hf.x, -hf.y)));
-            const __half2 l2 = __floats2half2_rn(rest.x, rest.y);
-            hi[i + k] = __uint_as_float(*reinterpret_cast<const uint32_t*>(&h));
-            lo[i + k] = __uint_as_float(*reinterpret_cast<const uint32_t*>(&l2));
+          for (int i = 0; i < 8; i += 2) {
+            const float4 vf = lds128(vf_at + 4u * (BK + h + 2 * i));
+#pragma unroll
+            for (int k = 0; k < 2; k++) {
+              const float2 x = unpk(add2(s2[h / 2 + i + k], from2));
+              const uint64_t w = pk(ex2(x.x), ex2(x.y));
+              sum2[k] = fma2(w, k == 0 ? pk(vf.x, vf.y) : pk(vf.z, vf.w), sum2[k]);
+              const float2 w2 = unpk(w);
+              const __half2 h2 = __floats2half2_rn(w2.x, w2.y);
+              const float2 hf = __half22float2(h2), rest = unpk(add2(w, pk(-hf.x, -hf.y)));
+              const __half2 l2 = __floats2half2_rn(rest.x, rest.y);
+              pair[i + k] = __uint_as_float(*reinterpret_cast<const uint32_t*>(&h2));
+              pair[8 + i + k] = __uint_as_float(*reinterpret_cast<const uint32_t*>(&l2));
+            }
           }
+          tmem_st16(s_at + (uint32_t)(KEYS * which + h), pair);  // over these keys' scores
         }
-        // over the columns of these keys' scores: hi, then lo
-        tmem_st16(s_at + 32u * half, hi);
-        tmem_st16(s_at + 32u * half + 16u, lo);
         const float2 all = unpk(add2(sum2[0], sum2[1]));
         l += all.x + all.y;
         tmem_wait_st();
         tc_fence_before();
         mbar_arrive(B_(PREADY + (n & 1u)));
       }
-      if (ok) ok = __all_sync(0xffffffffu, wait(PVDONE + ((n - 1) & 1u), (n - 1) >> 1));
-      pair_sync();  // the last maxima are read
-      if (half == 1) row_value[row] = l;
-      pair_sync();
-      if (half == 0) {
-        l += row_value[row];
-        row_value[row] = l;
-      }
-      pair_sync();
-      l = row_value[row];
-      pair_sync();  // read before the next tile's queries write there
+      // the row's sum, over the queries: the scores are done with them
+      row_sums[which * 32 + lane] = l;
+      row_sync();
+      l = 0.0f;
+#pragma unroll
+      for (int i = 0; i < PARTS; i++) l += row_sums[i * 32 + lane];
+      row_sync();  // read before the outputs are written there
+      if (ok) ok = __all_sync(0xffffffffu, wait(pv_done(n - 1), (n - 1) / L::VS));
       if (ok) {
         tc_fence_after();
-        const float inv = l > 0.0f ? 1.0f / l : 0.0f;
-        float* dst = static_cast<float*>(a.o) + (p.r.first + token) * a.o_stride + (int64_t)head * dim;
+        const float inv = !done ? 1.0f : l > 0.0f ? 1.0f / l : 0.0f;
         const int slot = 2 * (int)blockIdx.x + (whole ? 1 : 0);
-#pragma unroll 1
-        for (int c = half * (DH / 64); c < (half + 1) * (DH / 64); c++) {
-          float o[32];
-          read_o(c, o);
-          if (!valid) continue;
-          if (done) {
+        float* mine = done ? static_cast<float*>(a.o) + (p.r.first + token) * a.o_stride + (int64_t)head * dim
+                           : a.joint.sums + ((int64_t)slot * ROWS + row) * DH;
+        float* to[4];  // rows lane / 4 + 8 k of the warp: four lanes write 16 columns of one
 #pragma unroll
-            for (int i = 0; i < 32; i += 4) {
-              const int d = 32 * c + i;
-              if (d >= dim) break;
-              if (o_vec)
-                *reinterpret_cast<float4*>(dst + d) =
-                    make_float4(o[i] * inv, o[i + 1] * inv, o[i + 2] * inv, o[i + 3] * inv);
-              else
+        for (int k = 0; k < 4; k++)
+          to[k] = reinterpret_cast<float*>(
+              __shfl_sync(0xffffffffu, reinterpret_cast<unsigned long long>(mine), 8 * k + (lane >> 2)));
+        const int width = done ? dim : DH;
+        const bool vec = !done || o_vec;
+        float o[32];
+        read_o(o);
 #pragma unroll
-                for (int k = 0; k < 4; k++) dst[d + k] = o[i + k] * inv;
+        for (int h = 0; h < 32; h += 16) {
+#pragma unroll
+          for (int i = 0; i < 4; i++)
+            sts128(stage + 64u * lane + ((i ^ ((uint32_t)lane >> 1 & 3u)) << 4),
+                   make_float4(o[h + 4 * i] * inv, o[h + 4 * i + 1] * inv, o[h + 4 * i + 2] * inv, o[h + 4 * i + 3] * inv));
+          __syncwarp();
+          const int d = o_col + h + 4 * (lane & 3);
+#pragma unroll
+          for (int k = 0; k < 4; k++) {
+            const uint32_t r = 8u * k + ((uint32_t)lane >> 2);
+            const float4 v = lds128(stage + 64u * r + ((((uint32_t)lane & 3u) ^ (r >> 1 & 3u)) << 4));
+            if (quarter * 32 + (int)r < rows && d < width) {
+              if (vec) {
+                *reinterpret_cast<float4*>(to[k] + d) = v;
+              } else {
+                to[k][d] = v.x;
+                to[k][d + 1] = v.y;
+                to[k][d + 2] = v.z;
+                to[k][d + 3] = v.w;
+              }
             }
-          } else {
-            write_part(c, o);
           }
+          __syncwarp();
         }
-        if (valid && half == 0) {
+        if (valid && which == 0) {
           // weights are relative to m - kShift
           if (!done) {
             a.joint.stats[(int64_t)slot * 2 * ROWS + row] = m - kShift;
@@ -607,6 +679,7 @@ paged_attention_f32_kernel(const __grid_constant__ CUtensorMap k_map,
         }
         tc_fence_before();  // O is read before the next tile's QREADY
       }
+      row_sync();  // the stage is read before the next tile's queries are written there
       next_tile(nb);
     }
     if (tid == 0) {
@@ -637,7 +710,7 @@ int launch_f32(const et_b200_paged_cache_v1* c, AttendArgs& a, void* ws, cudaStr
   a.joint = joint_of(ws, blocks, ROWS, DH);
   cudaFuncSetAttribute(paged_attention_f32_kernel<DH>, cudaFuncAttributeMaxDynamicSharedMemorySize,
                        L::SMEM);
-  paged_attention_f32_kernel<DH><<<blocks, THREADS, L::SMEM, stream>>>(k_map, v_map, a, box_rows);
+  paged_attention_f32_kernel<DH><<<blocks, L::THREADS, L::SMEM, stream>>>(k_map, v_map, a, box_rows);
   count_launch();
   return blocks;
 }
