@@ -905,9 +905,10 @@ int32_t et_b200_paged_attention_v1(const et_b200_paged_cache_v1* c,
     a.sms = sms;
     a.scale_log2 = kLog2e / sqrtf((float)c->head_dim);
     auto st = static_cast<cudaStream_t>(stream);
-    if (c->dtype == ET_B200_DTYPE_F32) launch_type<float>(c, a, b->max_new, workspace, st);
-    else if (c->dtype == ET_B200_DTYPE_F16) launch_type<__half>(c, a, b->max_new, workspace, st);
-    else launch_type<__nv_bfloat16>(c, a, b->max_new, workspace, st);
+    const int64_t max_new = least_of(b->max_new, (int64_t)INT32_MAX);  // times group fits
+    if (c->dtype == ET_B200_DTYPE_F32) launch_type<float>(c, a, max_new, workspace, st);
+    else if (c->dtype == ET_B200_DTYPE_F16) launch_type<__half>(c, a, max_new, workspace, st);
+    else launch_type<__nv_bfloat16>(c, a, max_new, workspace, st);
     const cudaError_t status = cudaGetLastError();
     if (status != cudaSuccess) return cuda_error(e, status, op);
   }

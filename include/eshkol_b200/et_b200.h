@@ -240,7 +240,7 @@ int32_t et_b200_paged_append_v1(const et_b200_paged_cache_v1 *cache,
  * and bf16 (q' with its residual up to 16 query rows per kv head), and all
  * operands are carried as pairs of about 22 bits at f32.  Keys and
  * values of positions below a request's length must be finite; slots behind
- * may hold anything.  The workspace (any contents, overwritten; its size does
+ * may hold anything.  o must overlap neither q nor the pools.  The workspace (any contents, overwritten; its size does
  * not depend on the batch) serves one call at a time: calls that may overlap,
  * and graphs that may, need one each. */
 size_t et_b200_paged_attention_workspace_bytes_v1(

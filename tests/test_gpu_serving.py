@@ -180,6 +180,19 @@ def test_attention_kernels_agree_whatever_the_hint(lib, cuda):
         s.check()
 
 
+def test_attention_largest_hint(lib, cuda):
+    """The largest max_new is a large one: it picks the kernel of many rows."""
+    s = Step([(40, 200)], 4, 2, 64, 16, F16)
+    a = paged.PagedAttention(s.cache, 4)
+    out = []
+    for hint in (40, (1 << 63) - 1):
+        b = paged.PagedBatch(s.offsets, s.lengths, s.table, s.tokens, hint, 0, s.status)
+        a.forward(b, s.q, s.o, (s.cos, s.sin), s.lse)
+        s.check()
+        out.append((s.o[:s.used].clone(), s.lse[:s.used].clone()))
+    assert torch.equal(out[0][0], out[1][0]) and torch.equal(out[0][1], out[1][1])
+
+
 @pytest.mark.parametrize("dtype", [F32, F16, BF16])
 @pytest.mark.parametrize("heads,dim,page,layout,shift", [
     (1, 8, 1, "heads", 0), (2, 64, 16, "heads", 0), (8, 128, 24, "slots", 0),
