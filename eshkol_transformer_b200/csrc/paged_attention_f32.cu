@@ -70,9 +70,8 @@ struct Layout {
   static constexpr int QLO = VP + VS * PAIR;
   static constexpr int V_FACTORS = QLO + ROWS * DH * 2;     // [VS][2][BK]: exponents and factors
   static constexpr int K_FACTORS = V_FACTORS + VS * 2 * BK * 4;  // [3][BK]
-  static constexpr int SHARED_ROWS = K_FACTORS + 3 * BK * 4;  // what a row's threads exchange
-  static constexpr int MAXIMA = DH == 128 ? 1 : 2;            // buffers of the rows' maxima
-  static constexpr int BARS = SHARED_ROWS + MAXIMA * PARTS * ROWS * 2;
+  static constexpr int SHARED_ROWS = K_FACTORS + 3 * BK * 4;  // [2][ROWS]: what a row's threads exchange
+  static constexpr int BARS = SHARED_ROWS + 2 * ROWS * 4;
   static constexpr int SMEM = BARS + 8 * (2 * RAWS + 2 * VS + 13) + 8;
   static constexpr uint32_t S0 = 0, QH = 128, O = 192, COLS = 512;
   static_assert(O + 2 * DH <= COLS && QH + DH / 2 <= O && SMEM <= 232448, "TMEM and shared memory");
@@ -82,6 +81,15 @@ struct Layout {
 // and a large one keeps it out of the maximum) and for rows below 2^-87.
 __device__ __forceinline__ int row_exponent(float amax) {
   return min(100, 13 - ((int)(__float_as_uint(amax) >> 23) - 127));
+}
+
+// A float's bits in an order of integers, and back.
+__device__ __forceinline__ int ordered_bits(float x) {
+  const int i = __float_as_int(x);
+  return i ^ ((i >> 31) & 0x7fffffff);
+}
+__device__ __forceinline__ float from_ordered(int i) {
+  return __int_as_float(i ^ ((i >> 31) & 0x7fffffff));
 }
 
 template <int DH>
@@ -350,8 +358,8 @@ paged_attention_f32_kernel(const __grid_constant__ CUtensorMap k_map,
     const uint32_t o_at = lanes + L::O;
     uint8_t* q_lo = smem + L::QLO;
     uint8_t* shared_rows = smem + L::SHARED_ROWS;
-    __nv_bfloat16* row_max = reinterpret_cast<__nv_bfloat16*>(shared_rows);  // [MAXIMA][PARTS][ROWS]
-    float* row_value = reinterpret_cast<float*>(shared_rows);                // [ROWS], before a tile
+    int* row_max = reinterpret_cast<int*>(shared_rows);        // [2][ROWS], of ordered_bits
+    float* row_value = reinterpret_cast<float*>(shared_rows);  // [ROWS], before a tile
     // behind a tile the memory of a quarter's queries passes on its row sums
     // [PARTS][32], then its output, 16 columns of 32 rows per warp at a time
     float* row_sums = reinterpret_cast<float*>(q_lo + quarter * 4096);
@@ -470,6 +478,7 @@ paged_attention_f32_kernel(const __grid_constant__ CUtensorMap k_map,
         }
         tmem_wait_st();
         row_sync();
+        if (which == 0) row_max[row] = row_max[ROWS + row] = ordered_bits(-INFINITY);
 #pragma unroll
         for (int k = 0; k < FOURS; k++)
 #pragma unroll
@@ -481,6 +490,7 @@ paged_attention_f32_kernel(const __grid_constant__ CUtensorMap k_map,
         fence_async_smem();
         tc_fence_before();
         mbar_arrive(B_(QREADY));
+        row_sync();  // row_max is set
       }
       // What leaves TMEM between chunks, 32 columns from o_col of a row per thread:
       // piece by piece, the threads side by side.  (A row per thread in place, every
@@ -488,7 +498,7 @@ paged_attention_f32_kernel(const __grid_constant__ CUtensorMap k_map,
       constexpr int SIDE = 4 * ROWS * PARTS;
       float* scratch = a.joint.stats + (int64_t)gridDim.x * 4 * ROWS +
                        (int64_t)blockIdx.x * ROWS * DH + 4 * (which * ROWS + row);
-      float m = -INFINITY, l = 0.0f, m_part = -INFINITY;
+      float m = -INFINITY, l = 0.0f, m_part = -INFINITY, far = -INFINITY;
       bool have_part = false;
       static_assert(DH / PARTS == 32, "columns of a thread");
       const int o_col = 32 * which;
@@ -561,14 +571,16 @@ paged_attention_f32_kernel(const __grid_constant__ CUtensorMap k_map,
           const float2 v = unpk(s2[i]);
           top[i & 3] = fmaxf(top[i & 3], fmaxf(v.x, v.y));
         }
-        // the row's maximum over its threads, rounded up: any bound serves them
-        __nv_bfloat16* shared_max = row_max + (n & (uint32_t)(L::MAXIMA - 1)) * PARTS * ROWS + row;
-        if (L::MAXIMA == 1 && j > 0) row_sync();  // the last block's are read
-        shared_max[which * ROWS] = __float2bfloat16_ru(fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3])));
+        // the row's maximum over its threads, in f32: probabilities relative to a
+        // bound above it would leave binary16.  Each thread adds the largest of all
+        // its blocks so far to one of two places in turn, so what block n - 2 left
+        // there is no larger than block n's; block n - 1's is in the other, and who
+        // reads that is here before anyone writes it again.
+        far = fmaxf(far, fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3])));
+        int* shared_max = row_max + (n & 1u) * ROWS + row;
+        atomicMax(shared_max, ordered_bits(far));
         row_sync();
-        float bmax = -INFINITY;
-#pragma unroll
-        for (int i = 0; i < PARTS; i++) bmax = fmaxf(bmax, __bfloat162float(shared_max[i * ROWS]));
+        const float bmax = from_ordered(*reinterpret_cast<volatile int*>(shared_max));
         const bool jump = bmax > m + kJump;
         if (__any_sync(0xffffffffu, jump)) {
           const float factor = jump ? ex2(m - bmax) : 1.0f;  // 0 while m is -inf
