@@ -95,6 +95,11 @@ __device__ __forceinline__ float ex2(float x) {
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
   return y;
 }
+// l 2^d for a sum of weights l, which may lie far from 1: in two steps where 2^d alone
+// would be flushed to zero.
+__device__ __forceinline__ float scaled(float l, float d) {
+  return d < -120.0f ? l * ex2(-120.0f) * ex2(d + 120.0f) : l * ex2(d);
+}
 
 // kind::tf32 instruction descriptor: f32 accumulate, M = 128, N = n, A
 // K-major, B K-major (b_mn = 0) or MN-major (b_mn = 1).

@@ -645,7 +645,7 @@ __global__ void __launch_bounds__(32 * JOIN_WARPS) paged_join_kernel(AttendArgs 
         const float m1 = mine ? a.joint.stats[s * 2 * rows + r] : -INFINITY;
         const float l1 = mine ? a.joint.stats[(s * 2 + 1) * rows + r] : 0.0f;
         const float m = warp_max(m1), ref = m == -INFINITY ? 0.0f : m;
-        const float f1 = ex2(m1 - ref);
+        const float f1 = ex2(m1 - ref), lf = scaled(l1, m1 - ref);
         // in the order of the parts, as below
         float l = 0.0f, x[W];
 #pragma unroll
@@ -653,7 +653,7 @@ __global__ void __launch_bounds__(32 * JOIN_WARPS) paged_join_kernel(AttendArgs 
 #pragma unroll 2
         for (int i = 0; i < cut.parts; i++) {
           const float f = __shfl_sync(0xffffffffu, f1, i);
-          l += f * __shfl_sync(0xffffffffu, l1, i);
+          l += __shfl_sync(0xffffffffu, lf, i);
           const float* src = a.joint.sums + ((int64_t)slot_of(i) * rows + r) * DH + lane * W;
           if constexpr (W >= 4) {
 #pragma unroll
@@ -696,8 +696,8 @@ __global__ void __launch_bounds__(32 * JOIN_WARPS) paged_join_kernel(AttendArgs 
 #pragma unroll 4
       for (int i = warp; i < cut.parts; i += JOIN_WARPS) {
         const int64_t s = slot_of(i);
-        const float f = ex2(a.joint.stats[s * 2 * rows + r] - ref);
-        l += f * a.joint.stats[(s * 2 + 1) * rows + r];
+        const float below = a.joint.stats[s * 2 * rows + r] - ref, f = ex2(below);
+        l += scaled(a.joint.stats[(s * 2 + 1) * rows + r], below);
         if (lane < LANES) {
           const float* src = a.joint.sums + (s * rows + r) * DH + lane * V;
 #pragma unroll

@@ -9,7 +9,9 @@
 // a value row, which moves into the weight: with v_j = v^_j 2^g_j,
 //   o = sum_j 2^(s_j + g_j - M) v^_j / sum_j 2^(s_j + g_j - M) 2^-g_j,
 // M the running maximum of s_j + g_j, so cached rows of any magnitude need no
-// pass of their own.
+// pass of their own.  Where values of 2^24 and more stand beside far smaller ones,
+// a key whose 2^(s_j + g_j - M) is flushed to zero may still have a share of the
+// denominator: such keys are added to it by themselves (kFar below).
 //
 // A tile is 128 rows (TMEM lanes), a block 64 keys.  One warp copies raw K and V
 // tiles by TMA, two teams of four warps turn them into pairs (a row by all lanes of
@@ -70,17 +72,33 @@ struct Layout {
   static constexpr int QLO = VP + VS * PAIR;
   static constexpr int V_FACTORS = QLO + ROWS * DH * 2;     // [VS][2][BK]: exponents and factors
   static constexpr int K_FACTORS = V_FACTORS + VS * 2 * BK * 4;  // [3][BK]
-  static constexpr int SHARED_ROWS = K_FACTORS + 3 * BK * 4;  // [2][ROWS]: what a row's threads exchange
+  static constexpr int V_LEAST = K_FACTORS + 3 * BK * 4;      // [VS][TEAM]: least exponents so far
+  static constexpr int SHARED_ROWS = V_LEAST + VS * TEAM * 4;  // [2][ROWS]: what a row's threads exchange
   static constexpr int BARS = SHARED_ROWS + 2 * ROWS * 4;
   static constexpr int SMEM = BARS + 8 * (2 * RAWS + 2 * VS + 13) + 8;
   static constexpr uint32_t S0 = 0, QH = 128, O = 192, COLS = 512;
   static_assert(O + 2 * DH <= COLS && QH + DH / 2 <= O && SMEM <= 232448, "TMEM and shared memory");
 };
 
-// e with 2^13 <= amax 2^e < 2^14; 100 for a row of zeros (any e describes it,
-// and a large one keeps it out of the maximum) and for rows below 2^-87.
-__device__ __forceinline__ int row_exponent(float amax) {
-  return min(100, 13 - ((int)(__float_as_uint(amax) >> 23) - 127));
+// e with 2^13 <= amax 2^e < 2^14; `most` for a row of zeros (any e describes it,
+// and a large one keeps it out of the maximum) and for rows below 2^(13 - most).
+__device__ __forceinline__ int row_exponent(float amax, int most = 100) {
+  return min(most, 13 - ((int)(__float_as_uint(amax) >> 23) - 127));
+}
+// Of values: a key adds at most 2^(kShift + kJump + 80) to its row's sum of weights,
+// so 2^31 keys stay inside f32.
+constexpr int kMostOfV = 80;
+// A weight 2^(s_j + g_j - M + kShift) that f32 flushes to zero adds nothing to the
+// numerator, but 2^-g_j of it belongs to the sum of weights.  Beside the row k that
+// M stands for it is below 2^(-133 - g_j + g_k), so below 2^-44 while g_k < 10 (values
+// under 2^24); from there on (kFar: exponents e = -g) such keys are added by themselves.
+constexpr int kFar = -10;
+
+__device__ __forceinline__ float tmem_ld1(uint32_t addr) {
+  uint32_t v;
+  asm volatile("tcgen05.ld.sync.aligned.32x32b.x1.b32 {%0}, [%1];\n\ttcgen05.wait::ld.sync.aligned;"
+               : "=r"(v) : "r"(addr) : "memory");
+  return __uint_as_float(v);
 }
 
 // A float's bits in an order of integers, and back.
@@ -101,6 +119,7 @@ paged_attention_f32_kernel(const __grid_constant__ CUtensorMap k_map,
   extern __shared__ __align__(1024) uint8_t smem[];
   float* v_factors = reinterpret_cast<float*>(smem + L::V_FACTORS);
   float* k_factors = reinterpret_cast<float*>(smem + L::K_FACTORS);
+  int* v_least = reinterpret_cast<int*>(smem + L::V_LEAST);
   uint64_t* bars = reinterpret_cast<uint64_t*>(smem + L::BARS);
   enum {
     RAWFULL = 0, RAWEMPTY = L::RAWS, KFULL = 2 * L::RAWS, VFULL = KFULL + 3, SFULL = VFULL + L::VS,
@@ -258,9 +277,11 @@ paged_attention_f32_kernel(const __grid_constant__ CUtensorMap k_map,
     // probabilities, so they have three.
     constexpr int W = DH / 32, AT_ONCE = DH == 64 ? 8 : 4;  // dims of a lane, rows at once
     const int kv = (warp - CONVERT_WARP) / TEAM, row0 = 16 * ((warp - CONVERT_WARP) % TEAM);
+    const int most = kv == 0 ? 100 : kMostOfV;
     bool ok = true;
     while (ok && left > 0) {
       const int nb = blocks_here(), visible = tile_visible(a.tiling, p.r, p.tile);
+      int least = most;  // exponent of this warp's rows of the tile so far
 #pragma unroll 1
       for (int j = 0; j < nb; j++, n++) {
         const int valid = visible - (p.blk + j) * BK;
@@ -306,7 +327,7 @@ paged_attention_f32_kernel(const __grid_constant__ CUtensorMap k_map,
           for (int k = 0; k < AT_ONCE; k++) m[k] = __reduce_max_sync(0xffffffffu, m[k]);
 #pragma unroll
           for (int k = 0; k < AT_ONCE; k++) {
-            const int r = r0 + k, e = row_exponent(__uint_as_float(m[k]));
+            const int r = r0 + k, e = row_exponent(__uint_as_float(m[k]), most);
             const uint64_t sc = twice(exp2_int(e));
             mine = lane == r ? e : mine;
             uint32_t hi[W / 2], lo[W / 2];
@@ -339,6 +360,10 @@ paged_attention_f32_kernel(const __grid_constant__ CUtensorMap k_map,
             f[0] = (float)-mine;
             f[BK] = exp2_int(mine);
           }
+        }
+        if (kv == 1) {
+          least = min(least, __reduce_min_sync(0xffffffffu, lane < 16 ? mine : most));
+          if (lane == 0) v_least[v_slot * TEAM + row0 / 16] = least;
         }
         fence_async_smem();
         __syncwarp();
@@ -498,7 +523,7 @@ paged_attention_f32_kernel(const __grid_constant__ CUtensorMap k_map,
       constexpr int SIDE = 4 * ROWS * PARTS;
       float* scratch = a.joint.stats + (int64_t)gridDim.x * 4 * ROWS +
                        (int64_t)blockIdx.x * ROWS * DH + 4 * (which * ROWS + row);
-      float m = -INFINITY, l = 0.0f, m_part = -INFINITY, far = -INFINITY;
+      float m = -INFINITY, l = 0.0f, m_part = -INFINITY, most = -INFINITY;
       bool have_part = false;
       static_assert(DH / PARTS == 32, "columns of a thread");
       const int o_col = 32 * which;
@@ -556,8 +581,6 @@ paged_attention_f32_kernel(const __grid_constant__ CUtensorMap k_map,
             }
           }
         }
-        __syncwarp();
-        if (lane == 0) mbar_arrive(B_(KFREE + n % 3u));
         if (masked) {
 #pragma unroll
           for (int i = 0; i < KEYS / 2; i++) {
@@ -576,17 +599,19 @@ paged_attention_f32_kernel(const __grid_constant__ CUtensorMap k_map,
         // its blocks so far to one of two places in turn, so what block n - 2 left
         // there is no larger than block n's; block n - 1's is in the other, and who
         // reads that is here before anyone writes it again.
-        far = fmaxf(far, fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3])));
+        most = fmaxf(most, fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3])));
         int* shared_max = row_max + (n & 1u) * ROWS + row;
-        atomicMax(shared_max, ordered_bits(far));
+        atomicMax(shared_max, ordered_bits(most));
         row_sync();
         const float bmax = from_ordered(*reinterpret_cast<volatile int*>(shared_max));
         const bool jump = bmax > m + kJump;
-        if (__any_sync(0xffffffffu, jump)) {
+        const int4 far_v = *reinterpret_cast<const int4*>(v_least + n % L::VS * TEAM);
+        const bool far = min(min(far_v.x, far_v.y), min(far_v.z, far_v.w)) <= kFar;
+        if (__any_sync(0xffffffffu, jump || far)) {
           const float factor = jump ? ex2(m - bmax) : 1.0f;  // 0 while m is -inf
           if (jump) {
+            l = scaled(l, m - bmax);
             m = bmax;
-            l *= factor;
           }
           if (j % CHUNK != 0) {  // O holds products of this chunk: rescale it once they are complete
             if (ok) ok = __all_sync(0xffffffffu, wait(pv_done(n - 1), (n - 1) / L::VS));
@@ -600,7 +625,19 @@ paged_attention_f32_kernel(const __grid_constant__ CUtensorMap k_map,
               tmem_st32(o_at + 32u * c, o);
             }
           }
+          if (far) {  // the sum of weights of the keys that the loop below flushes to zero
+            const float* kf = k_factors + n % 3u * BK + KEYS * which;
+            const float* ge = v_factors + n % L::VS * 2 * BK + KEYS * which;
+            const float below = (m == -INFINITY ? 0.0f : m) - kShift;
+#pragma unroll 1
+            for (int i = 0; i < KEYS; i++) {
+              const float x = fmaf(tmem_ld1(s_at + (uint32_t)(KEYS * which + i)) * cq, kf[i], ge[i]) - below;
+              if (i < seen && x < -126.0f) l += ex2(x - ge[i]);
+            }
+          }
         }
+        __syncwarp();
+        if (lane == 0) mbar_arrive(B_(KFREE + n % 3u));
         const float from = (m == -INFINITY ? 0.0f : m) - kShift;
         uint64_t sum2[2] = {0, 0};
         const uint64_t from2 = twice(-from);

@@ -69,3 +69,89 @@ def test_f32_scores_in_the_thousands(lib, cuda, hint, dim, scale):
     s.q *= scale
     run(s, hint)
     check(s)
+
+
+ZERO, HUGE = -1000, 47
+
+
+def value_rows(pattern, m, g):
+    """Exponents of the m rows of values."""
+    at = torch.arange(m, device="cuda")
+    some = torch.randint(0, 3, (m,), device="cuda", generator=g) == 0
+    if pattern == "one huge":
+        return torch.where(at == 3, HUGE, ZERO)
+    if pattern == "half huge":
+        return torch.where(some, HUGE, ZERO)
+    if pattern == "late huge":
+        return torch.where((at > m // 2) & some, HUGE, ZERO)
+    if pattern == "early huge":
+        return torch.where((at < m // 4) & some, HUGE, ZERO)
+    if pattern == "largest and ones":
+        return torch.where(some, 110, torch.where(at % 5 == 0, ZERO, 0))
+    if pattern == "any":
+        return torch.randint(-100, 101, (m,), device="cuda", generator=g)
+    if pattern == "small":
+        return torch.where(some, -70, ZERO)
+    return torch.full((m,), ZERO, device="cuda")  # "zeros"
+
+
+@pytest.mark.parametrize("requests", [[(40, 700), (150, 150)], [(20, 9001)]], ids=["blocks", "joined"])
+@pytest.mark.parametrize("dim", [64, 128])
+@pytest.mark.parametrize("scores", ["equal", "normal"])
+@pytest.mark.parametrize("pattern", ["one huge", "half huge", "late huge", "early huge",
+                                     "largest and ones", "any", "small", "zeros"])
+def test_f32_value_rows_of_any_magnitude(lib, cuda, pattern, scores, dim, requests):
+    """Rows of zeros and rows up to 2^110 next to one another: each keeps its share
+    of the denominator.  (With rows of 0 and 2^47 at equal scores the output is their
+    mean.)"""
+    s = Step(requests, 2, 1, dim, 16, F32, seed=dim)
+    g = torch.Generator(device="cuda").manual_seed(dim)
+    if scores == "equal":
+        s.q.zero_()
+    for b, (_, m) in enumerate(requests):
+        e = value_rows(pattern, m, g)
+        s.v[b] *= torch.where(e == ZERO, 0.0, torch.exp2(e.float()))[:, None, None]
+        s.store(b, s.k[b], s.v[b])
+    for hint in (1, 100):
+        run(s, hint)
+        for rows, m, o, lse, weighted, _ in expected(s):
+            room = 2e-5 * weighted.amax(-1, keepdim=True)
+            assert ((s.o[rows].double() - o).abs() <= room).all(), hint
+            assert ((s.lse[rows].double() - lse).abs() <= 2e-5 * (1 + lse.abs())).all(), hint
+
+
+@pytest.mark.parametrize("dim", [64, 128])
+def test_f32_far_value_behind_a_low_score(lib, cuda, dim):
+    """A key whose value is 2^100 and whose weight is below 2^-400 changes nothing."""
+    s = Step([(40, 700)], 2, 1, dim, 16, F32, seed=dim)
+    s.q.copy_(s.q[:1, :1].expand_as(s.q).clone())
+    s.k[0][5] = -40.0 * s.q[0, :1]
+    s.v[0][5] *= 2.0 ** 100
+    s.store(0, s.k[0], s.v[0])
+    for hint in (1, 100):
+        run(s, hint, rope=False)
+        for rows, m, o, lse, _, _ in expected(s, rope=False):
+            assert ((s.o[rows].double() - o).abs() <= 2e-5 * (1 + o.abs())).all(), hint
+            assert ((s.lse[rows].double() - lse).abs() <= 2e-5 * (1 + lse.abs())).all(), hint
+
+
+@pytest.mark.parametrize("dim", [64, 128])
+def test_f32_many_zero_values(lib, cuda, dim):
+    """20,000 keys with values of zero, the first ones a little less likely: the sum
+    of weights stays inside f32.  150 requests share the pages, so that a thread
+    block has all keys of one."""
+    new, length, page, batch = 20, 20000, 16, 150
+    keys = torch.zeros(length // page, 1, page, dim, device="cuda")
+    keys[:4] = -5.4 / math.sqrt(dim)  # e^-5.4 of the others' weight
+    cache = paged.PagedCache(keys, torch.zeros_like(keys))
+    table = torch.arange(length // page, device="cuda").int().expand(batch, -1).contiguous()
+    offsets = torch.arange(batch + 1, device="cuda") * new
+    q = torch.ones(batch * new, 1, dim, device="cuda")
+    seen = length - new + 1 + torch.arange(new, device="cuda").double()
+    want = torch.log((seen - 64) + 64 * math.exp(-5.4)).repeat(batch)
+    for hint in (1, new):
+        o, lse = torch.full_like(q, 7.0), torch.full((batch * new, 1), 7.0, device="cuda")
+        b = paged.PagedBatch(offsets, torch.full((batch,), length, device="cuda"), table, batch * new, hint)
+        paged.PagedAttention(cache, 1).forward(b, q, o, None, lse)
+        torch.cuda.synchronize()
+        assert (o == 0).all() and ((lse[:, 0].double() - want).abs() <= 2e-4).all(), hint
