@@ -159,6 +159,8 @@ paged_attention_kernel(const __grid_constant__ CUtensorMap k_map,
   constexpr int DH = S::DH, BM = S::BM, BK = S::BK, KW = S::KW, NT = S::NT, WK = S::WK;
   constexpr bool F32 = sizeof(T) == 4;
   constexpr int KSTEP = F32 ? 8 : 16;  // dims (or keys) per matrix instruction
+  // f16 probabilities carry 2^15: their least normal number is then 2^-29 of the largest
+  constexpr float kShift = std::is_same_v<T, __half> ? 15.0f : 0.0f;
   extern __shared__ __align__(1024) uint8_t smem[];
   int64_t* koff = reinterpret_cast<int64_t*>(smem + S::KOFF);
   float* join_m = reinterpret_cast<float*>(smem + S::JOIN);
@@ -447,7 +449,7 @@ paged_attention_kernel(const __grid_constant__ CUtensorMap k_map,
       for (int i = 0; i < KW / 8; i++)
 #pragma unroll
         for (int e = 0; e < 4; e++) {
-          s[i][e] = ex2(s[i][e] - from[e >> 1]);
+          s[i][e] = ex2(s[i][e] - (from[e >> 1] - kShift));
           l[e >> 1] += s[i][e];
         }
       if (__any_sync(0xffffffffu, factor[0] != 1.0f || factor[1] != 1.0f)) {
@@ -579,7 +581,7 @@ paged_attention_kernel(const __grid_constant__ CUtensorMap k_map,
                   if (d < dim) store2<T>(dst + d, o[n][2 * i] * inv, o[n][2 * i + 1] * inv);
                 }
                 if (a.lse != nullptr && (lane & 3) == 0)
-                  a.lse[t * a.q_heads + h] = l[i] > 0.0f ? m[i] * kLn2 + logf(l[i]) : -INFINITY;
+                  a.lse[t * a.q_heads + h] = l[i] > 0.0f ? (m[i] - kShift) * kLn2 + logf(l[i]) : -INFINITY;
               }
             } else {
               float* dst = a.joint.sums + ((int64_t)slot * BM + r) * DH;
@@ -588,7 +590,7 @@ paged_attention_kernel(const __grid_constant__ CUtensorMap k_map,
                 *reinterpret_cast<float2*>(dst + 8 * n + 2 * (lane & 3)) =
                     make_float2(o[n][2 * i], o[n][2 * i + 1]);
               if ((lane & 3) == 0) {
-                a.joint.stats[(int64_t)slot * 2 * BM + r] = m[i];
+                a.joint.stats[(int64_t)slot * 2 * BM + r] = m[i] - kShift;
                 a.joint.stats[((int64_t)slot * 2 + 1) * BM + r] = l[i];
               }
             }

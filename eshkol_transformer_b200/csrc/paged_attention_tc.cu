@@ -12,7 +12,7 @@
 // turns, which keeps the halves out of step: while the pipe works on one half, the other half's four warps (one row per thread, no exchange between
 // threads) turn scores into probabilities, written over the scores in TMEM as
 // the A operand of P V.  The row maximum stands until a block exceeds it by
-// 2^8 (the sums stay far inside f32), so O is rescaled in TMEM only then.
+// 2^8 (2^4 at f16; the sums stay far inside f32), so O is rescaled in TMEM only then.
 // A 4,096-token chunk over 12,000 keys (32 / 8 heads x 128, bf16) takes 720 us, 927
 // TFLOP/s; a pair of half-blocks 3,520 cycles, 1,550 of them probabilities, whose
 // hand-off bounds it (the products alone take 2,750).
@@ -37,7 +37,6 @@ constexpr int HALF = 128, BK = 128;
 constexpr int MMA_WARP = 8, LOAD_WARP = 10, THREADS = 384;
 constexpr int kWideRegs = 208, kLeanRegs = 88;
 static_assert(256 * kWideRegs + 128 * kLeanRegs <= THREADS * 168, "registers at launch");
-constexpr float kJump = 8.0f;  // log2 of the largest P the standing maximum allows
 
 __device__ int g_wait_error;  // bounded waits that gave up (the status word tells the caller)
 
@@ -52,7 +51,7 @@ __device__ __forceinline__ uint32_t pack2(float a, float b) {
   }
 }
 
-// 2^x of two finite values on the FMA pipe (x <= 8, under -126 as -126): x =
+// 2^x of two finite values on the FMA pipe (x <= 15, under -126 as -126): x =
 // n + f with n rounded to nearest, 2^f by its polynomial of degree 4 of least
 // relative error on |f| <= 1/2 (2.7e-6), n added to the exponent.
 __device__ __forceinline__ uint64_t power2(uint64_t x) {
@@ -88,6 +87,11 @@ paged_attention_tc_kernel(const __grid_constant__ CUtensorMap k_map,
                           const __grid_constant__ CUtensorMap v_map, AttendArgs a, int box_rows) {
   using L = Layout<DH>;
   constexpr int SLOTS = L::SLOTS;
+  // log2 of the largest P the standing maximum allows, and what P carries on top: at
+  // f16 at most 2^15 together, so that its least normal number is 2^-25 of the standing
+  // maximum (without it many unlikely keys behind a likely one lost their bits)
+  constexpr float kJump = std::is_same_v<T, __half> ? 4.0f : 8.0f;
+  constexpr float kShift = std::is_same_v<T, __half> ? 11.0f : 0.0f;
   constexpr uint32_t kType = std::is_same_v<T, __nv_bfloat16> ? (1u << 7) | (1u << 10) : 0u;
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) &
@@ -414,7 +418,7 @@ paged_attention_tc_kernel(const __grid_constant__ CUtensorMap k_map,
               }
             }
           }
-          const float from = m == -INFINITY ? 0.0f : m;
+          const float from = (m == -INFINITY ? 0.0f : m) - kShift;
           // a quarter of the exponentials on the FMA pipe, the others on the special
           // function unit (8 cycles per warp; the 4,096-token chunk: 783 us with all
           // of them there, 757 with a quarter on the FMA pipe, 800 with half);
@@ -486,10 +490,10 @@ paged_attention_tc_kernel(const __grid_constant__ CUtensorMap k_map,
           }
           if (valid) {
             if (!done) {
-              a.joint.stats[(int64_t)slot * 4 * HALF + r] = m;
+              a.joint.stats[(int64_t)slot * 4 * HALF + r] = m - kShift;
               a.joint.stats[((int64_t)slot * 2 + 1) * 2 * HALF + r] = l;
             } else if (a.lse != nullptr) {
-              a.lse[(p.r.first + token) * a.q_heads + head] = l > 0.0f ? m * kLn2 + logf(l) : -INFINITY;
+              a.lse[(p.r.first + token) * a.q_heads + head] = l > 0.0f ? (m - kShift) * kLn2 + logf(l) : -INFINITY;
             }
           }
           tc_fence_before();  // O is read before the next tile's QREADY

@@ -155,3 +155,30 @@ def test_f32_many_zero_values(lib, cuda, dim):
         paged.PagedAttention(cache, 1).forward(b, q, o, None, lse)
         torch.cuda.synchronize()
         assert (o == 0).all() and ((lse[:, 0].double() - want).abs() <= 2e-4).all(), hint
+
+
+@pytest.mark.parametrize("dtype", [F16, BF16])
+@pytest.mark.parametrize("dim", [64, 128, 256])
+@pytest.mark.parametrize("hint", [1, 100])
+@pytest.mark.parametrize("gap", [12.0, 16.5])
+def test_many_unlikely_keys_behind_a_likely_one(lib, cuda, gap, hint, dim, dtype):
+    """One key without a value takes nearly all weight (an attention sink), 4,000
+    others, e^-gap each, carry the output: their weights keep their bits.  (32 heads, so
+    that a thread block walks many keys behind the likely one.)  The scores' products
+    are exact: what is left are the weights' rounding u, the exponentials' 2^-18 (by
+    polynomial; 2^-20 of f32 scores of 24) and sums' (KEYS + 16) 2^-23, and the
+    output's rounding, absolute below the normal range."""
+    s = Step([(20, 4001)], 32, 32, dim, 16, dtype, seed=dim)
+    s.q.fill_(1.0)
+    s.k[0].zero_()
+    s.k[0][7] = gap / math.sqrt(dim)
+    s.v[0] += 1.0
+    s.v[0][7] = 0.0
+    s.store(0, s.k[0], s.v[0])
+    run(s, hint, rope=False)
+    u = U[dtype]
+    for rows, m, o, lse, weighted, _ in expected(s, rope=False):
+        bound = (u + 2.0 ** -17 + (m + 16) * 2.0 ** -23) * weighted + u * o.abs()
+        bound += torch.finfo(dtype).smallest_normal * u
+        assert ((s.o[rows].double() - o).abs() <= 1.01 * bound).all()
+        assert ((s.lse[rows].double() - lse).abs() <= 2e-5 * (1 + lse.abs())).all()
