@@ -353,7 +353,10 @@ struct AttendArgs {
   float* lse;
   int64_t q_stride, o_stride, least;
   int q_heads, sms;  // SMs of the device
-  float scale_log2;  // log2(e) / sqrt(head_dim)
+  float scale_log2;  // log2(e) / sqrt(head_dim), and 1 / q_factor
+  // 1/2 for rotated f16 queries, whose elements reach sqrt(2) times the largest f16;
+  // else 1
+  float q_factor;
 };
 
 // ---- TMA from the pools ---------------------------------------------------------------

@@ -313,6 +313,10 @@ paged_attention_kernel(const __grid_constant__ CUtensorMap k_map,
           if (i >= PAIRS) break;
           float x0 = to_f32<T>(x[k][0]), x1 = to_f32<T>(x[k][1]);
           if (a.rope.cos != nullptr) rotate(x0, x1, cs[k], sn[k]);
+          if constexpr (std::is_same_v<T, __half>) {
+            x0 *= a.q_factor;
+            x1 *= a.q_factor;
+          }
           const uint32_t at = S::template at<BM>(r, d * (int)sizeof(T) / 16) + (d * (int)sizeof(T)) % 16;
           T* dst = reinterpret_cast<T*>(smem + S::STAGES * S::STAGE + at);
           dst[0] = from_f32<T>(x0);
@@ -905,7 +909,8 @@ int32_t et_b200_paged_attention_v1(const et_b200_paged_cache_v1* c,
     a.o_stride = o_stride;
     a.q_heads = (int)q_heads;
     a.sms = sms;
-    a.scale_log2 = kLog2e / sqrtf((float)c->head_dim);
+    a.q_factor = c->dtype == ET_B200_DTYPE_F16 && a.rope.cos != nullptr ? 0.5f : 1.0f;
+    a.scale_log2 = kLog2e / sqrtf((float)c->head_dim) / a.q_factor;
     auto st = static_cast<cudaStream_t>(stream);
     const int64_t max_new = least_of(b->max_new, (int64_t)INT32_MAX);  // times group fits
     if (c->dtype == ET_B200_DTYPE_F32) launch_type<float>(c, a, max_new, workspace, st);

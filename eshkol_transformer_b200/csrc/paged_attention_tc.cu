@@ -356,6 +356,10 @@ paged_attention_tc_kernel(const __grid_constant__ CUtensorMap k_map,
                   for (int e = 0; e < 4; e++) {
                     float x0 = to_f32<T>(u[k][i].x[2 * e]), x1 = to_f32<T>(u[k][i].x[2 * e + 1]);
                     rotate(x0, x1, cc[e], ss[e]);
+                    if constexpr (std::is_same_v<T, __half>) {
+                      x0 *= a.q_factor;
+                      x1 *= a.q_factor;
+                    }
                     u[k][i].x[2 * e] = from_f32<T>(x0);
                     u[k][i].x[2 * e + 1] = from_f32<T>(x1);
                   }

@@ -182,3 +182,17 @@ def test_many_unlikely_keys_behind_a_likely_one(lib, cuda, gap, hint, dim, dtype
         bound += torch.finfo(dtype).smallest_normal * u
         assert ((s.o[rows].double() - o).abs() <= 1.01 * bound).all()
         assert ((s.lse[rows].double() - lse).abs() <= 2e-5 * (1 + lse.abs())).all()
+
+
+@pytest.mark.parametrize("dim", [64, 128, 256])
+@pytest.mark.parametrize("hint", [1, 100])
+def test_f16_queries_near_the_largest(lib, cuda, hint, dim):
+    """Queries of up to 65,000 whose rotation passes 65,504, the largest f16."""
+    s = Step([(30, 200), (1, 77)], 2, 1, dim, 16, F16, seed=dim)
+    s.q.copy_(65000.0 * (1.0 - 0.2 * s.q.float().abs().clamp(max=4.0)))
+    assert float(turn(s.q[29:30].double(), s.cos[[199]], s.sin[[199]]).abs().max()) > 70000.0
+    for b in range(2):
+        s.k[b] *= 2.0 ** -13
+        s.store(b, s.k[b], s.v[b])
+    run(s, hint)
+    check(s)
