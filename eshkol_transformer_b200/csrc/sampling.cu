@@ -345,7 +345,10 @@ __device__ __forceinline__ Filters filters_of(const Args& a, int64_t row) {
   f.min_p = a.min_p != nullptr ? a.min_p[row] : 0.0f;
   f.uniform = (double)a.uniform[row];
   f.per = 1.4426950408889634 / (double)f.temperature;
-  f.fall = f.min_p > 0.0f ? (double)f.temperature * log((double)fminf(f.min_p, 1.0f)) : 0.0;
+  // at an infinite temperature every logit weighs 1, which is no less than min_p
+  f.fall = !(f.min_p > 0.0f) ? 0.0
+           : f.temperature == INFINITY ? -(double)INFINITY
+                                       : (double)f.temperature * log((double)fminf(f.min_p, 1.0f));
   return f;
 }
 // What the running sum has to reach: the first integer above u total, inside

@@ -196,3 +196,22 @@ def test_f16_queries_near_the_largest(lib, cuda, hint, dim):
         s.store(b, s.k[b], s.v[b])
     run(s, hint)
     check(s)
+
+
+@pytest.mark.parametrize("vocab", [7, 900, 4099, 30011])
+def test_sampling_infinite_temperature(lib, cuda, vocab):
+    """Every logit above -inf weighs the same, and every row gets an answer."""
+    x = torch.randn(16, vocab, device="cuda")
+    x[:, 1::3] = -math.inf
+    some = np.nonzero((x[0] > -math.inf).cpu().numpy())[0]
+    u = ((np.arange(16) + 0.5) / 16).astype(np.float32)
+    for kw in (dict(), dict(min_p=1.0), dict(min_p=0.3), dict(min_p=5.0), dict(top_p=1.0, min_p=1.0)):
+        ids, lp = draw(x, u, math.inf, **kw)
+        assert np.array_equal(ids, some[np.floor(u.astype(np.float64) * some.size).astype(int)]), kw
+        assert np.allclose(lp, -math.log(some.size), atol=2e-6), kw
+    for kw, left in ((dict(top_k=4), 4), (dict(top_k=4, min_p=1.0), 4),
+                     (dict(top_k=4, top_p=0.75, min_p=0.5), 3)):
+        ids, lp = draw(x, u, math.inf, **kw)
+        for r in range(16):
+            kept = np.sort(np.argsort(-x[r].double().cpu().numpy(), kind="stable")[:left])
+            assert ids[r] == kept[int(u[r] * left)] and abs(lp[r] + math.log(left)) <= 2e-6, kw
