@@ -91,11 +91,18 @@ __device__ __forceinline__ float power_of(float x, const Scale& s) {
   } else {
     if (!(x > -INFINITY)) return 0.0f;
     if (s.max == INFINITY) return x == INFINITY ? 1.0f : 0.0f;
-    const float d = x - s.max, t = d * s.hi;
-    if (!(t >= -64.0f)) return 0.0f;
-    const float bb = d - x, e = (x - (d - bb)) - (s.max + bb);
-    n = rintf(t);
-    f = (t - n) + (fmaf(d, s.hi, -t) + fmaf(d, s.lo, e * s.hi));
+    const float d = x - s.max;
+    if (d == -INFINITY) {  // further apart than the largest f32: of weight at such temperatures only
+      const float t = fmaf(x, s.hi, -s.max * s.hi);
+      n = rintf(fmaxf(t, -64.0f));
+      f = t < -64.0f ? 0.0f : t - n;
+    } else {
+      const float t = d * s.hi;
+      if (!(t >= -64.0f)) return 0.0f;
+      const float bb = d - x, e = (x - (d - bb)) - (s.max + bb);
+      n = rintf(t);
+      f = (t - n) + (fmaf(d, s.hi, -t) + fmaf(d, s.lo, e * s.hi));
+    }
   }
   float y = 1.5252734e-5f;
   y = fmaf(y, f, 1.5403530e-4f);

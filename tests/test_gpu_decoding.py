@@ -215,3 +215,22 @@ def test_sampling_infinite_temperature(lib, cuda, vocab):
         for r in range(16):
             kept = np.sort(np.argsort(-x[r].double().cpu().numpy(), kind="stable")[:left])
             assert ids[r] == kept[int(u[r] * left)] and abs(lp[r] + math.log(left)) <= 2e-6, kw
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("vocab", [5, 2000])
+def test_sampling_logits_further_apart_than_the_largest_f32(lib, cuda, vocab, dtype):
+    """max x - x overflows f32, the weight exp((x - max x) / temperature) does not."""
+    x = torch.full((3, vocab), -3.3e38, device="cuda")
+    x[:, 1], x[:, 3] = 3.3e38, 0.0
+    x = x.to(dtype)
+    host = x[0].double().cpu().numpy()
+    for t in (math.inf, 3e38, 1e37, 1.0):
+        for kw in (dict(), dict(top_p=0.9), dict(min_p=0.3), dict(top_k=3)):
+            u = np.array([0.0, 0.37, 0.93], np.float32)
+            ids, lp = draw(x, u, t, **kw)
+            for r in range(3):
+                i, want, room = sample(host, float(u[r]), float(np.float32(t)), kw.get("top_k", 0),
+                                       float(np.float32(kw.get("top_p", 1.0))),
+                                       float(np.float32(kw.get("min_p", 0.0))))
+                assert room <= 2.5e-7 or (ids[r] == i and abs(lp[r] - want) <= 2e-6), (t, kw, r)
