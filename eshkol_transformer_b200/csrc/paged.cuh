@@ -57,6 +57,13 @@ __device__ __forceinline__ void report(int* status, int bit) {
   if (status != nullptr) atomicOr(status, bit);
 }
 
+// A block's abort word is also the error word of its bounded waits (role_wait,
+// mbar_wait): the one that runs out sets it, whichever role waits, the other roles'
+// waits then give up, and who comes last tells the caller.
+__device__ __forceinline__ void report_abort(int* status, volatile int* abort) {
+  if (*abort != 0) report(status, ET_B200_PAGED_TIMEOUT);
+}
+
 // A request's new tokens (rows first .. first + n - 1 of the tensors) and its
 // length, clamped to the tensors and the page table; `bad` holds the status
 // bits of what had to be clamped.

@@ -150,8 +150,6 @@ struct Shape {
   }
 };
 
-__device__ int g_wait_error;  // bounded waits that gave up (the status word tells the caller)
-
 template <typename T, typename S, bool TMA>
 __global__ void __launch_bounds__(S::NT + (TMA ? 32 : 0), S::PER_SM)
 paged_attention_kernel(const __grid_constant__ CUtensorMap k_map,
@@ -179,7 +177,8 @@ paged_attention_kernel(const __grid_constant__ CUtensorMap k_map,
   const uint32_t bars = base + S::BARS;
   auto full_bar = [&](int st) { return bars + 8u * (uint32_t)st; };
   auto empty_bar = [&](int st) { return bars + 8u * (uint32_t)(S::STAGES + st); };
-  volatile int* abort = reinterpret_cast<volatile int*>(smem + S::BARS + 2 * S::STAGES * 8);
+  int* abort_word = reinterpret_cast<int*>(smem + S::BARS + 2 * S::STAGES * 8);
+  volatile int* abort = abort_word;
   if (TMA && tid == 0) {
     for (int i = 0; i < S::STAGES; i++) {
       mbar_init(full_bar(i), 1);
@@ -209,7 +208,7 @@ paged_attention_kernel(const __grid_constant__ CUtensorMap k_map,
     for (int u = 0; u < (int)share.units; u++) {
       const int st = u % S::STAGES, key0 = p.blk * BK, h = p.h, now = page;
       if (u >= S::STAGES && !__all_sync(0xffffffffu, role_wait(empty_bar(st), (uint32_t)((u / S::STAGES - 1) & 1),
-                                                               &g_wait_error, abort)))
+                                                               abort_word, abort)))
         break;
       const int boxes = __popc(__ballot_sync(0xffffffffu, now != -2));
       if (lane == 0) mbar_expect_tx(full_bar(st), (uint32_t)((boxes << box_bits) * S::ROW * 2));
@@ -233,7 +232,8 @@ paged_attention_kernel(const __grid_constant__ CUtensorMap k_map,
     }
     // every copy has landed before the block releases its memory
     for (int u = max(0, fetched - S::STAGES); u < fetched; u++)
-      mbar_wait(full_bar(u % S::STAGES), (uint32_t)((u / S::STAGES) & 1), &g_wait_error);
+      mbar_wait(full_bar(u % S::STAGES), (uint32_t)((u / S::STAGES) & 1), abort_word);
+    if (lane == 0) report_abort(a.batch.status, abort);
     return;
   }
   Cut cut{0, 0, 0, 0, 0};
@@ -343,7 +343,7 @@ paged_attention_kernel(const __grid_constant__ CUtensorMap k_map,
         // after a wait that ran out the loop still ends, in step with the other warps
         if (ok)
           ok = __all_sync(0xffffffffu, role_wait(full_bar(st), (uint32_t)((u / S::STAGES) & 1),
-                                                 &g_wait_error, abort));
+                                                 abort_word, abort));
       } else {
         cp_wait<S::STAGES - 2>();
         __syncthreads();  // stage u is complete; stage u - 1 and its addresses are free
@@ -613,7 +613,7 @@ paged_attention_kernel(const __grid_constant__ CUtensorMap k_map,
       advance(a.tiling, a.batch, p);
     }
     if constexpr (TMA) {
-      if (!ok && tid == 0) report(a.batch.status, ET_B200_PAGED_TIMEOUT);
+      if (!ok && lane == 0) report_abort(a.batch.status, abort);
     } else {
       cp_wait<0>();
     }

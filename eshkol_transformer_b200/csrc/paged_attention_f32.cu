@@ -51,8 +51,6 @@ constexpr float kJump = 8.0f;   // log2 of the largest P the standing maximum al
 constexpr float kShift = 7.0f;  // P carries 2^7: at most 2^15
 constexpr int CHUNK = 8;        // blocks whose products one TMEM accumulator adds
 
-__device__ int g_wait_error;  // bounded waits that gave up (the status word tells the caller)
-
 template <int DH>
 struct Layout {
   static constexpr int PARTS = DH / 32, KEYS = BK / PARTS;  // threads of a row, keys of one
@@ -129,7 +127,8 @@ paged_attention_f32_kernel(const __grid_constant__ CUtensorMap k_map,
   const uint32_t bar0 = smem_u32(bars);
   auto B_ = [&](int i) { return bar0 + 8u * (uint32_t)i; };
   uint32_t* tslot = reinterpret_cast<uint32_t*>(bars + NBARS);
-  volatile int* abort = reinterpret_cast<volatile int*>(tslot + 1);
+  int* abort_word = reinterpret_cast<int*>(tslot + 1);
+  volatile int* abort = abort_word;
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const uint32_t base = smem_u32(smem);
   const int group = a.tiling.group, dim = a.pools.head_dim;
@@ -159,7 +158,7 @@ paged_attention_f32_kernel(const __grid_constant__ CUtensorMap k_map,
     advance(a.tiling, a.batch, p);
   };
   auto wait = [&](int i, uint32_t parity) {
-    return role_wait(B_(i), parity & 1u, &g_wait_error, abort);
+    return role_wait(B_(i), parity & 1u, abort_word, abort);
   };
   auto pv_done = [&](uint32_t block) { return PVDONE + (int)(block % L::VS); };
   uint32_t n = 0;  // blocks so far, of all tiles: slot n & 1, round n >> 1
@@ -204,7 +203,7 @@ paged_attention_f32_kernel(const __grid_constant__ CUtensorMap k_map,
     // every copy has landed before the CTA releases its memory
     if (lane == 0)
       for (uint32_t c = count > L::RAWS ? count - L::RAWS : 0; c < count; c++)
-        mbar_wait(B_(RAWFULL + c % L::RAWS), (c / L::RAWS) & 1u, &g_wait_error);
+        mbar_wait(B_(RAWFULL + c % L::RAWS), (c / L::RAWS) & 1u, abort_word);
   } else if (warp == MMA_WARP) {
     // ---- S = Q K^T, up to a block ahead of P V
     constexpr uint32_t idesc_s = idesc_f16_m128(BK, 0);
@@ -236,7 +235,7 @@ paged_attention_f32_kernel(const __grid_constant__ CUtensorMap k_map,
     }
     if (lane == 0) {
       umma_commit(B_(DRAIN));
-      mbar_wait(B_(DRAIN), 0u, &g_wait_error);
+      mbar_wait(B_(DRAIN), 0u, abort_word);
     }
   } else if (warp == MMA_WARP + 1) {
     // ---- O += P V
@@ -266,7 +265,7 @@ paged_attention_f32_kernel(const __grid_constant__ CUtensorMap k_map,
     }
     if (lane == 0) {
       umma_commit(B_(DRAIN + 1));
-      mbar_wait(B_(DRAIN + 1), 0u, &g_wait_error);
+      mbar_wait(B_(DRAIN + 1), 0u, abort_word);
     }
   }
   } else if (warp >= CONVERT_WARP) {
@@ -731,16 +730,14 @@ paged_attention_f32_kernel(const __grid_constant__ CUtensorMap k_map,
       row_sync();  // the stage is read before the next tile's queries are written there
       next_tile(nb);
     }
-    if (tid == 0) {
-      if (!ok) report(a.batch.status, ET_B200_PAGED_TIMEOUT);
-      a.joint.cuts[blockIdx.x] = cut;
-    }
+    if (tid == 0) a.joint.cuts[blockIdx.x] = cut;
   }
   tc_fence_before();
   __syncthreads();
   if (warp == MMA_WARP) {
     tc_fence_after();
     tmem_dealloc(tmem, L::COLS);
+    if (lane == 0) report_abort(a.batch.status, abort);
   }
 }
 

@@ -38,8 +38,6 @@ constexpr int MMA_WARP = 8, LOAD_WARP = 10, THREADS = 384;
 constexpr int kWideRegs = 208, kLeanRegs = 88;
 static_assert(256 * kWideRegs + 128 * kLeanRegs <= THREADS * 168, "registers at launch");
 
-__device__ int g_wait_error;  // bounded waits that gave up (the status word tells the caller)
-
 template <typename T>
 __device__ __forceinline__ uint32_t pack2(float a, float b) {
   if constexpr (std::is_same_v<T, __half>) {
@@ -101,7 +99,8 @@ paged_attention_tc_kernel(const __grid_constant__ CUtensorMap k_map,
   const uint32_t bar0 = smem_u32(bars);
   auto B_ = [&](int i) { return bar0 + 8u * (uint32_t)i; };
   uint32_t* tslot = reinterpret_cast<uint32_t*>(bars + NBARS);
-  volatile int* abort = reinterpret_cast<volatile int*>(tslot + 1);
+  int* abort_word = reinterpret_cast<int*>(tslot + 1);
+  volatile int* abort = abort_word;
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const uint32_t base = smem_u32(smem);
   const int group = a.tiling.group, dim = a.pools.head_dim;
@@ -134,7 +133,7 @@ paged_attention_tc_kernel(const __grid_constant__ CUtensorMap k_map,
     advance(a.tiling, a.batch, p);
   };
   auto wait = [&](int i, uint32_t parity) {
-    return role_wait(B_(i), parity & 1u, &g_wait_error, abort);
+    return role_wait(B_(i), parity & 1u, abort_word, abort);
   };
 
   if (warp >= MMA_WARP) {
@@ -181,7 +180,7 @@ paged_attention_tc_kernel(const __grid_constant__ CUtensorMap k_map,
     // every copy has landed before the CTA releases its memory
     if (lane == 0)
       for (uint32_t c = count > SLOTS ? count - SLOTS : 0; c < count; c++)
-        mbar_wait(B_(FULL + c % SLOTS), (c / SLOTS) & 1u, &g_wait_error);
+        mbar_wait(B_(FULL + c % SLOTS), (c / SLOTS) & 1u, abort_word);
   } else if (warp < LOAD_WARP) {
     // ---- products of half t.  A half without rows goes along with the slots.
     const int t = warp - MMA_WARP;
@@ -269,7 +268,7 @@ paged_attention_tc_kernel(const __grid_constant__ CUtensorMap k_map,
     }
     if (lane == 0) {
       umma_commit(B_(DRAIN + t));
-      mbar_wait(B_(DRAIN + t), 0u, &g_wait_error);
+      mbar_wait(B_(DRAIN + t), 0u, abort_word);
     }
   }
   } else {
@@ -505,16 +504,14 @@ paged_attention_tc_kernel(const __grid_constant__ CUtensorMap k_map,
       }
       next_tile(nb);
     }
-    if (tid == 0) {
-      if (!ok) report(a.batch.status, ET_B200_PAGED_TIMEOUT);
-      a.joint.cuts[blockIdx.x] = cut;
-    }
+    if (tid == 0) a.joint.cuts[blockIdx.x] = cut;
   }
   tc_fence_before();
   __syncthreads();
   if (warp == MMA_WARP) {
     tc_fence_after();
     tmem_dealloc(tmem, L::COLS);
+    if (lane == 0) report_abort(a.batch.status, abort);
   }
 }
 

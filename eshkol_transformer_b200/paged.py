@@ -28,7 +28,7 @@ BAD_PAGE = 1    # a page outside the pool: reads as zeros, writes are dropped
 BAD_LENGTH = 2  # a length below 0 or beyond the table's columns: clamped
 BAD_OFFSET = 4  # offsets that fall or leave the tensors: clamped
 BAD_ROPE = 8    # a position beyond the RoPE tables: the last row is used
-TIMEOUT = 16    # a kernel gave up waiting: o is not valid
+TIMEOUT = 16    # a kernel gave up waiting: o is not valid (only status tells)
 
 
 class CacheDescriptor(C.Structure):
@@ -116,7 +116,8 @@ class PagedBatch:
     page_table [batch, columns] (i32) on the device, rows of the token-major
     tensors; max_new and max_length (new tokens and length of the largest
     request as far as the host knows) only pick the kernel.  status: an i32
-    tensor of one element that collects BAD_* bits, or None."""
+    tensor of one element that collects BAD_* and TIMEOUT bits, or None: then
+    nothing tells of either."""
 
     def __init__(self, offsets, lengths, page_table, tokens: int, max_new: int | None = None,
                  max_length: int | None = None, status=None):

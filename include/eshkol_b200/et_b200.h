@@ -197,8 +197,9 @@ enum {
                                    clamped */
   ET_B200_PAGED_BAD_ROPE = 8,   /* a position beyond the RoPE tables: the last
                                    row is used */
-  ET_B200_PAGED_TIMEOUT = 16    /* a kernel gave up waiting for its own copies
-                                   or products: o is not valid */
+  ET_B200_PAGED_TIMEOUT = 16    /* a kernel gave up waiting (some 2 s) for its
+                                   own copies or products: o is not valid.
+                                   Only the status word tells */
 };
 typedef struct et_b200_paged_batch_v1 {
   size_t struct_size;
@@ -207,7 +208,8 @@ typedef struct et_b200_paged_batch_v1 {
   const int64_t *offsets;    /* [batch + 1], ascending from 0 */
   const int64_t *lengths;    /* [batch] */
   const int32_t *page_table; /* [batch, table_columns] */
-  int32_t *status;           /* one word, or NULL */
+  int32_t *status;           /* one word, or NULL (then nothing of the above
+                                is recorded, a timeout included) */
 } et_b200_paged_batch_v1;
 
 /* RoPE tables as et_b200_rope_tables_v1 lays them out: device f32 [rows,

@@ -234,3 +234,13 @@ def test_sampling_logits_further_apart_than_the_largest_f32(lib, cuda, vocab, dt
                                        float(np.float32(kw.get("top_p", 1.0))),
                                        float(np.float32(kw.get("min_p", 0.0))))
                 assert room <= 2.5e-7 or (ids[r] == i and abs(lp[r] - want) <= 2e-6), (t, kw, r)
+
+
+def test_waits_that_run_out_are_reported(cuda, tmp_path):
+    """From any warp, with and without a status word (see paged_wait.cu)."""
+    root, out = Path(__file__).resolve().parents[1], tmp_path / "paged_wait"
+    subprocess.run([build.nvcc(), *build.ARCH, "-std=c++17", "--expt-relaxed-constexpr",
+                    f"-I{build.INCLUDE}", f"-I{build.CSRC}", str(root / "tests" / "paged_wait.cu"),
+                    "-o", str(out)], check=True)
+    done = subprocess.run([str(out)], capture_output=True, text=True, timeout=120)
+    assert done.returncode == 0 and done.stdout.strip() == "ok", done.stdout
