@@ -39,6 +39,9 @@ struct Pools {
   int page_size, kv_heads, head_dim;
   Divisor by_page;
 };
+// Most keys of a page table: positions, rounded up to whole blocks of keys and of
+// look-ups, stay 32-bit numbers.
+constexpr int64_t kMostCapacity = INT32_MAX - 4096;
 struct Batch {
   const int64_t* offsets;
   const int64_t* lengths;

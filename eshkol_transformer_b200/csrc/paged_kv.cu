@@ -164,10 +164,11 @@ int32_t check_batch(const et_b200_paged_batch_v1* b, const et_b200_paged_cache_v
     return set_error(e, ET_KERNEL_ERROR_VERSION_MISMATCH, ET_KERNEL_CODE_INVALID_STRUCT_SIZE, op,
                      "paged batch descriptor is missing or truncated");
   if (b->batch < 0 || b->batch > (1 << 20) || b->tokens < 0 || b->tokens > (1 << 26) ||
-      b->table_columns < 1 || b->table_columns > INT32_MAX / c->page_size || b->max_new < 0 ||
+      b->table_columns < 1 || b->table_columns > kMostCapacity / c->page_size || b->max_new < 0 ||
       b->max_length < 0)
     return set_error(e, ET_KERNEL_ERROR_SHAPE_MISMATCH, ET_KERNEL_CODE_INVALID_SHAPE, op,
-                     "paged batch is outside its limits");
+                     "paged batch is outside its limits (a page table holds fewer than 2^31 - "
+                     "4096 keys)");
   if (b->batch > 0 && (b->offsets == nullptr || b->lengths == nullptr || b->page_table == nullptr))
     return set_error(e, ET_KERNEL_ERROR_INVALID_ARGUMENT, ET_KERNEL_CODE_NULL_ARGUMENT, op,
                      "offsets, lengths and the page table are required");

@@ -207,7 +207,8 @@ typedef struct et_b200_paged_batch_v1 {
   int64_t max_new, max_length;
   const int64_t *offsets;    /* [batch + 1], ascending from 0 */
   const int64_t *lengths;    /* [batch] */
-  const int32_t *page_table; /* [batch, table_columns] */
+  const int32_t *page_table; /* [batch, table_columns]; table_columns *
+                                page_size < 2^31 - 4096 */
   int32_t *status;           /* one word, or NULL (then nothing of the above
                                 is recorded, a timeout included) */
 } et_b200_paged_batch_v1;

@@ -1,0 +1,32 @@
+"""The serving operators' host side at the ends of its ranges, without a GPU."""
+import ctypes as C
+import subprocess
+from pathlib import Path
+
+import pytest
+
+from eshkol_transformer_b200 import build
+from test_serving_host import append, attend, batch, cache
+
+ROOT = Path(__file__).resolve().parents[1]
+
+
+@pytest.mark.parametrize("page", [1, 16, 64, 1 << 20])
+def test_page_tables_of_nearly_2_31_keys_are_refused(lib, page):
+    """Rounded up to blocks of keys, their positions would leave 32 bits."""
+    pool = cache(page_size=page, head_stride=64 * page, page_stride=128 * page)
+    for columns in {(2 ** 31 - 1) // page, (2 ** 31 - 4097) // page + 1}:
+        if columns * page < 2 ** 31 - 4096:  # the last whole page lies below
+            continue
+        for call in (append, attend):
+            rc, err = call(lib, pool, batch(table_columns=columns))
+            assert rc != 0 and b"limits" in err.message, (page, columns)
+
+
+def test_arithmetic_at_the_largest_page_table(tmp_path):
+    out = tmp_path / "paged_limits"
+    subprocess.run([build.nvcc(), *build.ARCH, "-std=c++17", "--expt-relaxed-constexpr",
+                    f"-I{build.INCLUDE}", f"-I{build.CSRC}", str(ROOT / "tests" / "paged_limits.cu"),
+                    "-o", str(out)], check=True)
+    done = subprocess.run([str(out)], capture_output=True, text=True)
+    assert done.returncode == 0 and done.stdout.strip() == "ok", done.stdout
