@@ -45,7 +45,14 @@ paged_append_kernel(Pools P, Batch B, Rope R, T* __restrict__ keys, T* __restric
   constexpr int N = 16 / sizeof(T);
   const int lane = threadIdx.x & 31;
   const int64_t token = (int64_t)blockIdx.x * WARPS + (threadIdx.x >> 5);
-  if (token >= B.tokens) return;
+  if (token >= B.tokens) {
+    // a block behind the last token (there is one where there is a status word)
+    // looks at the metadata of every request, also of those that store nothing
+    if ((int64_t)blockIdx.x * WARPS >= B.tokens && blockIdx.y == 0)
+      for (int b = threadIdx.x; b < B.batch; b += 32 * WARPS)
+        if (const int bad = load_request(B, b).bad) report(B.status, bad);
+    return;
+  }
   const int row_pieces = P.kv_heads * P.head_dim / N;
   const int piece0 = blockIdx.y * 32 * VPL + lane;
   uint4 kp[VPL], vp[VPL];
@@ -107,7 +114,8 @@ void launch_append(const et_b200_paged_cache_v1* c, const Pools& P, const Batch&
   const uintptr_t bits = reinterpret_cast<uintptr_t>(k) | reinterpret_cast<uintptr_t>(v) |
                          (uintptr_t)(ks * (int64_t)sizeof(T)) | (uintptr_t)(vs * (int64_t)sizeof(T));
   const int pieces = P.kv_heads * P.head_dim / (int)(16 / sizeof(T));
-  const dim3 grid((unsigned)((B.tokens + WARPS - 1) / WARPS), (unsigned)((pieces + 32 * VPL - 1) / (32 * VPL)));
+  const unsigned check = B.status != nullptr ? 1 : 0;  // a block behind the last token
+  const dim3 grid((unsigned)((B.tokens + WARPS - 1) / WARPS) + check, (unsigned)((pieces + 32 * VPL - 1) / (32 * VPL)));
   auto go = [&](auto vec) {
     paged_append_kernel<T, decltype(vec)::value><<<grid, 32 * WARPS, 0, stream>>>(
         P, B, R, static_cast<T*>(c->keys), static_cast<T*>(c->values), static_cast<const T*>(k), ks,

@@ -183,8 +183,8 @@ typedef struct et_b200_paged_cache_v1 {
  * its tokens with them, so its token i of n stands at position lengths[b] - n
  * + i, in slot position % page_size of page page_table[b][position /
  * page_size].  A request may bring no token; a token at a negative position
- * is not stored and sees no key.  Rows of no request are neither read nor
- * written.  max_new and max_length (the host's idea of the largest request)
+ * is not stored and sees no key.  Rows of no request are not written,
+ * and nothing depends on them.  max_new and max_length (the host's idea of the largest request)
  * only pick the kernel.  The arrays are device memory, read when the kernels
  * run; what in them leads outside the pools or tensors is not followed but
  * recorded in *status (never cleared here): */

@@ -244,3 +244,23 @@ def test_waits_that_run_out_are_reported(cuda, tmp_path):
                     "-o", str(out)], check=True)
     done = subprocess.run([str(out)], capture_output=True, text=True, timeout=120)
     assert done.returncode == 0 and done.stdout.strip() == "ok", done.stdout
+
+
+def test_append_records_every_request(lib, cuda):
+    """What is wrong with a request is recorded whether or not a token of it is
+    stored, as the attention does."""
+    for change, bit in (((("offsets", 2, 99),), paged.BAD_OFFSET), ((("offsets", 0, -3),), paged.BAD_OFFSET),
+                        ((("lengths", 1, 1 << 40),), paged.BAD_LENGTH),
+                        ((("lengths", 1, -1),), paged.BAD_LENGTH), ((), 0)):
+        for many in (0, 3000):  # requests behind the two, without tokens
+            s = Step([(2, 20), (0, 9)] + [(0, 0)] * many, 2, 1, 64, 16, F16, spare=0)
+            for name, i, x in change:
+                getattr(s, name)[i if i < 2 else -1] = x
+            k = torch.zeros(2, 1, 64, dtype=F16, device="cuda")
+            s.cache.append(s.batch(), k, k)
+            torch.cuda.synchronize()
+            assert int(s.status) == bit, (change, many)
+            s.status.zero_()
+            s.attend()
+            torch.cuda.synchronize()
+            assert int(s.status) == bit, (change, many)
