@@ -9,10 +9,11 @@ and attention of new tokens over it (et_b200_paged_attention_v1).
 
 The descriptors hold the tensors they were built from and may be kept while
 their contents change (a decoding loop updates offsets, lengths and the page
-table in place).  Calls are enqueued on `stream` (a cudaStream_t address, 0 =
-the legacy default stream) of the current device and return at once; on a
-stream other than torch's current one the caller orders the two and keeps the
-tensors (Tensor.record_stream) until the call has run.
+table in place).  Calls are enqueued on `stream` of the current device and
+return at once: None is torch's current stream, as for torch's own operations;
+else a cudaStream_t address (0 = the legacy default stream), and on a stream
+other than torch's current one the caller orders the two and keeps the tensors
+(Tensor.record_stream) until the call has run.
 """
 from __future__ import annotations
 
@@ -50,6 +51,12 @@ class BatchDescriptor(C.Structure):
 class RopeDescriptor(C.Structure):
     """et_b200_paged_rope_v1"""
     _fields_ = [("cos", C.c_void_p), ("sin", C.c_void_p), ("rows", C.c_int64)]
+
+
+def stream_of(stream: int | None, index: int) -> int:
+    """A call's stream: torch's current one unless given.  (The raw handle:
+    torch.cuda.current_stream builds an object, 1.3 us of a call's 8.)"""
+    return torch._C._cuda_getCurrentRawStream(index) if stream is None else stream
 
 
 def _need(condition: bool, message: str) -> None:
@@ -98,7 +105,7 @@ class PagedCache:
             page = max(slots * token, heads * head)
         return page, head, token
 
-    def append(self, batch: "PagedBatch", k, v, rope=None, stream: int = 0) -> None:
+    def append(self, batch: "PagedBatch", k, v, rope=None, stream: int | None = None) -> None:
         """Stores k (rotated by rope = (cos, sin), [positions, head_dim / 2]
         each) and v, [tokens, kv_heads, head_dim] with dense heads."""
         err = k1.KernelError()
@@ -106,7 +113,7 @@ class PagedCache:
         v_stride = _rows(v, batch, self, self.kv_heads, "v")
         rc = self.lib.et_b200_paged_append_v1(
             self._ref, batch.bind(self), batch.rope(rope, self), k.data_ptr(), k_stride,
-            v.data_ptr(), v_stride, stream, C.byref(err))
+            v.data_ptr(), v_stride, stream_of(stream, self.index), C.byref(err))
         if rc != 0:
             _check(rc, err)
 
@@ -193,7 +200,8 @@ class PagedAttention:
         self.ws = torch.empty(self.ws_bytes + 256, dtype=torch.uint8, device=cache.device)
         self.ws_ptr = (self.ws.data_ptr() + 255) & ~255
 
-    def forward(self, batch: PagedBatch, q, o, rope=None, lse=None, stream: int = 0) -> None:
+    def forward(self, batch: PagedBatch, q, o, rope=None, lse=None,
+                stream: int | None = None) -> None:
         """o = attention of q (rotated by rope) over the keys each token sees;
         q, o [tokens, q_heads, head_dim]; lse f32 [tokens, q_heads] or None."""
         err = k1.KernelError()
@@ -207,4 +215,4 @@ class PagedAttention:
         _check(self.lib.et_b200_paged_attention_v1(
             cache._ref, batch.bind(cache), batch.rope(rope, cache), self.q_heads, q.data_ptr(),
             q_stride, o.data_ptr(), o_stride, lse.data_ptr() if lse is not None else None,
-            self.ws_ptr, self.ws_bytes, stream, C.byref(err)), err)
+            self.ws_ptr, self.ws_bytes, stream_of(stream, cache.index), C.byref(err)), err)

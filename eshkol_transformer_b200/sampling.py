@@ -6,7 +6,7 @@ import ctypes as C
 import torch
 
 from . import _check, k1, load
-from .paged import DTYPES
+from .paged import DTYPES, stream_of
 
 
 class SamplingDescriptor(C.Structure):
@@ -35,11 +35,11 @@ class Sampler:
         return t.data_ptr()
 
     def sample(self, logits, uniform, ids, logprobs=None, temperature=None, top_k=None, top_p=None,
-               min_p=None, stream: int = 0) -> None:
+               min_p=None, stream: int | None = None) -> None:
         """ids (i64 [rows]) and logprobs (f32 [rows], or None) receive the
         drawn tokens and their log-probabilities; uniform f32 [rows] in
         [0, 1); temperature, top_p, min_p f32 [rows], top_k i64 [rows], or
-        None."""
+        None.  stream: as in `paged`."""
         device = logits.get_device()
         if device < 0 or torch.cuda.current_device() != device:
             raise ValueError("the logits must be on the current CUDA device")
@@ -60,6 +60,7 @@ class Sampler:
         rc = self.lib.et_b200_sample_v1(
             C.byref(d), logits.data_ptr(), self._row_values(uniform, f32, device, "uniform"),
             self._row_values(ids, torch.int64, device, "ids"),
-            self._row_values(logprobs, f32, device, "logprobs"), stream, C.byref(err))
+            self._row_values(logprobs, f32, device, "logprobs"), stream_of(stream, device),
+            C.byref(err))
         if rc != 0:
             _check(rc, err)

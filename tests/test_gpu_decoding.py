@@ -264,3 +264,52 @@ def test_append_records_every_request(lib, cuda):
             s.attend()
             torch.cuda.synchronize()
             assert int(s.status) == bit, (change, many)
+
+
+def test_calls_follow_the_current_stream(lib, cuda):
+    """Without `stream` a call takes torch's current one: it comes after what was
+    enqueued there, and into a capture."""
+    s = Step([(1, 40), (3, 30)], 2, 1, 64, 16, F16, spare=0)
+    a = paged.PagedAttention(s.cache, 2)
+    sampler = sampling.Sampler(4, 5000)
+    logits, ids = torch.zeros(4, 5000, device="cuda"), torch.zeros(4, dtype=torch.int64, device="cuda")
+    u = torch.zeros(4, device="cuda")
+    k, v = torch.randn(2, s.tokens, 1, 64, device="cuda").half()
+    q, batch = torch.zeros_like(s.q), s.batch()
+    keys, values = s.keys.clone().nan_to_num(), s.values.clone().nan_to_num()
+    s.keys.nan_to_num_()
+    s.values.nan_to_num_()
+
+    def step():
+        s.cache.append(batch, k, v, rope=(s.cos, s.sin))
+        a.forward(batch, q, s.o, (s.cos, s.sin), s.lse)
+        sampler.sample(logits, u, ids)
+
+    q.copy_(s.q)
+    logits[:, 77] = 100.0
+    step()
+    torch.cuda.synchronize()
+    want = [t.clone() for t in (s.o, s.keys, ids)]
+    for t in (q, s.o, s.lse, logits, ids):
+        t.zero_()
+    s.keys.copy_(keys)
+    s.values.copy_(values)
+    torch.cuda.synchronize()
+    side = torch.cuda.Stream()
+    with torch.cuda.stream(side):
+        torch.cuda._sleep(20_000_000)  # what follows has to wait for this
+        q.copy_(s.q)
+        logits[:, 77] = 100.0
+        step()
+    side.synchronize()
+    for now, then in zip((s.o, s.keys, ids), want):
+        assert torch.equal(now, then)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        step()
+    s.o.zero_()
+    ids.zero_()
+    torch.cuda.synchronize()
+    graph.replay()
+    torch.cuda.synchronize()
+    assert torch.equal(s.o, want[0]) and torch.equal(ids, want[2])
