@@ -839,6 +839,10 @@ void launch_type(const et_b200_paged_cache_v1* c, AttendArgs& a, int64_t max_new
   }
 }
 
+bool heads_fit(const et_b200_paged_cache_v1* c, int64_t q_heads) {
+  return q_heads >= 1 && q_heads <= 65536 && q_heads % c->kv_heads == 0;
+}
+
 size_t workspace_bytes(int64_t head_dim, int sms) {
   const int dim = padded(head_dim);
   const size_t plain = joint_bytes(kMostPerSm * sms, 64, dim), tc = attend_tc_workspace(dim, sms);
@@ -855,9 +859,7 @@ extern "C" {
 
 size_t et_b200_paged_attention_workspace_bytes_v1(const et_b200_paged_cache_v1* c,
                                                   int64_t q_heads) {
-  if (check_cache(c, nullptr, "paged-attention-workspace") || q_heads < 1 ||
-      q_heads % c->kv_heads != 0)
-    return 0;
+  if (check_cache(c, nullptr, "paged-attention-workspace") || !heads_fit(c, q_heads)) return 0;
   return workspace_bytes(c->head_dim, sm_count());
 }
 
@@ -871,9 +873,9 @@ int32_t et_b200_paged_attention_v1(const et_b200_paged_cache_v1* c,
   if (int32_t r = check_cache(c, e, op)) return r;
   if (int32_t r = check_batch(b, c, e, op)) return r;
   if (int32_t r = check_rope(rope, e, op)) return r;
-  if (q_heads < 1 || q_heads > 65536 || q_heads % c->kv_heads != 0)
+  if (!heads_fit(c, q_heads))
     return set_error(e, ET_KERNEL_ERROR_SHAPE_MISMATCH, ET_KERNEL_CODE_INVALID_SHAPE, op,
-                     "q_heads must be a multiple of the cache's kv_heads");
+                     "q_heads must be a multiple of the cache's kv_heads, up to 65536");
   if (b->tokens > 0 && b->batch > 0) {
     const int64_t row = q_heads * c->head_dim, size = c->dtype == ET_B200_DTYPE_F32 ? 4 : 2;
     if (q == nullptr || o == nullptr)

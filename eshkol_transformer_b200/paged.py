@@ -121,8 +121,10 @@ class PagedCache:
 class PagedBatch:
     """One step's requests: offsets [batch + 1] and lengths [batch] (i64),
     page_table [batch, columns] (i32) on the device, rows of the token-major
-    tensors; max_new and max_length (new tokens and length of the largest
-    request as far as the host knows) only pick the kernel.  status: an i32
+    tensors; max_new (new tokens of the largest request as far as the host
+    knows; None counts all tokens as one request's, which for many single
+    tokens is the slower kernel) only picks the kernel, max_length is not used
+    so far.  status: an i32
     tensor of one element that collects BAD_* and TIMEOUT bits, or None: then
     nothing tells of either."""
 

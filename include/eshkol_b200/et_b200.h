@@ -183,9 +183,9 @@ typedef struct et_b200_paged_cache_v1 {
  * its tokens with them, so its token i of n stands at position lengths[b] - n
  * + i, in slot position % page_size of page page_table[b][position /
  * page_size].  A request may bring no token; a token at a negative position
- * is not stored and sees no key.  Rows of no request are not written,
- * and nothing depends on them.  max_new and max_length (the host's idea of the largest request)
- * only pick the kernel.  The arrays are device memory, read when the kernels
+ * is not stored and sees no key.  Rows of no request are not written, and
+ * nothing depends on them.  max_new (the host's idea of the largest request)
+ * only picks the kernel; max_length is not used so far.  The arrays are device memory, read when the kernels
  * run; what in them leads outside the pools or tensors is not followed but
  * recorded in *status (never cleared here): */
 enum {
@@ -235,17 +235,18 @@ int32_t et_b200_paged_append_v1(const et_b200_paged_cache_v1 *cache,
 /* o = softmax(q' k^T / sqrt(head_dim)) v over the keys at positions up to the
  * query's own (the new tokens' keys are in the cache already), q' = q rotated
  * in f32.  q and o: [tokens, q_heads, head_dim], heads dense, rows q_stride /
- * o_stride elements apart; q_heads a multiple of kv_heads, query head h reads
- * key head h / (q_heads / kv_heads).  A query that sees no key gets zeros.
+ * o_stride elements apart; q_heads a multiple of kv_heads up to 65,536, query
+ * head h reads key head h / (q_heads / kv_heads).  A query that sees no key gets
+ * zeros.
  * lse (f32 [tokens, q_heads], or NULL) receives ln(sum of exp of the scaled
  * scores), -inf without keys.  Scores, statistics and sums are f32; for the
  * tensor cores q' and the probabilities are rounded to the pools' type at f16
  * and bf16 (q' with its residual up to 16 query rows per kv head), and all
  * operands are carried as pairs of about 22 bits at f32.  Keys and
  * values of positions below a request's length must be finite; slots behind
- * may hold anything.  o must overlap neither q nor the pools.  The workspace (any contents, overwritten; its size does
- * not depend on the batch) serves one call at a time: calls that may overlap,
- * and graphs that may, need one each. */
+ * may hold anything.  o must overlap neither q nor the pools.  The workspace
+ * (any contents, overwritten; its size does not depend on the batch) serves one
+ * call at a time: calls that may overlap, and graphs that may, need one each. */
 size_t et_b200_paged_attention_workspace_bytes_v1(
     const et_b200_paged_cache_v1 *cache, int64_t q_heads);
 int32_t et_b200_paged_attention_v1(const et_b200_paged_cache_v1 *cache,

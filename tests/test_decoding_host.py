@@ -30,3 +30,12 @@ def test_arithmetic_at_the_largest_page_table(tmp_path):
                     "-o", str(out)], check=True)
     done = subprocess.run([str(out)], capture_output=True, text=True)
     assert done.returncode == 0 and done.stdout.strip() == "ok", done.stdout
+
+
+def test_workspace_of_a_refused_number_of_heads(lib):
+    """No workspace where the call itself is refused (65,536 query heads at most)."""
+    size = lambda heads: lib.et_b200_paged_attention_workspace_bytes_v1(C.byref(cache()), heads)
+    assert size(65536) > 0
+    for heads in (65538, 1 << 40, 3, 0, -2):
+        assert size(heads) == 0, heads
+        assert attend(lib, cache(), batch(), heads=heads, qs=1 << 31, os=1 << 31)[0] != 0
