@@ -11,7 +11,6 @@ sum p|v|, plus its last rounding u |o|.
 """
 import math
 import subprocess
-import sys
 from pathlib import Path
 
 import numpy as np
@@ -236,6 +235,65 @@ def test_sampling_logits_further_apart_than_the_largest_f32(lib, cuda, vocab, dt
                 assert room <= 2.5e-7 or (ids[r] == i and abs(lp[r] - want) <= 2e-6), (t, kw, r)
 
 
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("vocab", [900, 5000, 30011, 300001])
+def test_sampling_infinite_logits_among_many(lib, cuda, vocab, dtype):
+    """+inf logits share all weight whatever the filters, also where cuts come from
+    histograms over the logits."""
+    g = torch.Generator(device="cuda").manual_seed(vocab)
+    x = torch.randn(4, vocab, device="cuda", generator=g).to(dtype)
+    x[:, 5:9] = math.nan
+    x[:, 20:40] = -math.inf
+    where = [3, 17, vocab // 2, vocab - 2, vocab - 1]
+    for r in range(4):
+        x[r, where[:r + 1]] = math.inf
+    u = np.array([0.7, 0.45, 0.6, 0.95], np.float32)
+    for kw in (dict(), dict(top_p=0.9), dict(top_p=0.5), dict(min_p=0.2), dict(top_k=2),
+               dict(top_k=600), dict(top_k=600, top_p=0.8, min_p=0.1)):
+        ids, lp = draw(x, u, 0.7, **kw)
+        for r in range(4):
+            i, want, _ = sample(x[r].double().cpu().numpy(), float(u[r]), 0.7, kw.get("top_k", 0),
+                                kw.get("top_p", 1.0), kw.get("min_p", 0.0))
+            assert ids[r] == i and abs(lp[r] - want) <= 2e-6, (r, kw)
+
+
+@pytest.mark.parametrize("dtype", [F32, F16])
+@pytest.mark.parametrize("vocab", [200001, 300001, 425968, 450001])
+def test_sampling_draws_inside_a_likely_token(lib, cuda, vocab, dtype):
+    """Slices that fill a cluster's shared memory and vocabularies beyond them, each
+    draw in the middle of a likely token's share."""
+    g = torch.Generator(device="cuda").manual_seed(vocab)
+    x = torch.randn(6, vocab, device="cuda", generator=g)
+    likely = torch.randint(vocab, (6, 8), device="cuda", generator=g)
+    x.scatter_(1, likely, 15.0 + 0.25 * torch.arange(8, device="cuda").expand(6, 8))
+    x = x.to(dtype)
+    host = x.double().cpu().numpy()
+    for kw in (dict(), dict(top_k=64), dict(top_p=0.5), dict(min_p=0.3), dict(top_k=1000, top_p=0.9),
+               dict(top_p=0.97)):
+        u, want = np.zeros(6, np.float32), []
+        for r in range(6):
+            args = kw.get("top_k", 0), kw.get("top_p", 1.0), kw.get("min_p", 0.0)
+            # the middle of the likeliest token's share of what the filters keep
+            best = int(host[r].argmax())
+            order = np.lexsort((np.arange(vocab), -host[r]))
+            w = np.exp(host[r][order] - host[r].max())
+            if args[0]:
+                w[args[0]:] = 0.0
+            before = np.cumsum(w) - w
+            w[(before >= args[1] * w.sum()) & (args[1] < 1.0)] = 0.0
+            w[w < args[2]] = 0.0
+            run_sum = np.zeros(vocab)
+            run_sum[order] = w
+            run_sum = np.cumsum(run_sum)
+            u[r] = (run_sum[best] - 0.5) / run_sum[-1]  # its weight is 1
+            i, lp, _ = sample(host[r], float(u[r]), 1.0, *args)
+            assert i == best
+            want.append(lp)
+        ids, lp = draw(x, u, 1.0, **kw)
+        assert np.array_equal(ids, host.argmax(1)), kw
+        assert np.allclose(lp, want, atol=2e-6), kw
+
+
 def test_waits_that_run_out_are_reported(cuda, tmp_path):
     """From any warp, with and without a status word (see paged_wait.cu)."""
     root, out = Path(__file__).resolve().parents[1], tmp_path / "paged_wait"
@@ -313,3 +371,84 @@ def test_calls_follow_the_current_stream(lib, cuda):
     graph.replay()
     torch.cuda.synchronize()
     assert torch.equal(s.o, want[0]) and torch.equal(ids, want[2])
+
+
+@pytest.mark.parametrize("dtype", [F32, F16, BF16])
+@pytest.mark.parametrize("dim,page", [(64, 16), (128, 64), (64, 24), (80, 7), (256, 8)])
+@pytest.mark.parametrize("hint", [1, 100])
+def test_bad_metadata_of_every_kernel(lib, cuda, hint, dim, page, dtype):
+    """Pages outside the pool read as zeros; lengths, offsets and positions beyond
+    the tables are clamped: in the kernels of few and of many rows, with pages
+    copied by TMA and one by one."""
+    s = Step([(1, 40), (20, 400), (1, 20)], 2, 1, dim, page, dtype)
+    s.keys.nan_to_num_()
+    s.values.nan_to_num_()
+    for what, bit in (("page", paged.BAD_PAGE), ("length", paged.BAD_LENGTH),
+                      ("offset", paged.BAD_OFFSET), ("rope", paged.BAD_ROPE)):
+        keep = [t.clone() for t in (s.table, s.lengths, s.offsets)]
+        rope = (s.cos, s.sin)
+        if what == "page":
+            s.table[0, 0], s.table[1, 1], s.table[2, 0] = -1, s.keys.shape[0], 2 ** 31 - 1
+        elif what == "length":
+            s.lengths[0], s.lengths[1] = -(2 ** 40), 2 ** 40
+        elif what == "offset":
+            s.offsets[1], s.offsets[3] = 2 ** 40, -9
+        else:
+            rope = (s.cos[:3].contiguous(), s.sin[:3].contiguous())
+        s.status.zero_()
+        s.o.fill_(7.0)
+        b = paged.PagedBatch(s.offsets, s.lengths, s.table, s.tokens, hint, None, s.status)
+        paged.PagedAttention(s.cache, 2).forward(b, s.q, s.o, rope, s.lse)
+        torch.cuda.synchronize()
+        assert int(s.status) & bit, what
+        assert torch.isfinite(s.o.float()).all()
+        if what == "page":  # as with pages of zeros in their place
+            s.status.zero_()
+            for r, c in ((0, 0), (1, 1), (2, 0)):
+                s.table[r, c] = keep[0][r, c]
+                for b_, t in ((r, s.k), (r, s.v)):
+                    t[b_][c * page:(c + 1) * page] = 0.0
+                s.store(r, s.k[r], s.v[r])
+            got = s.o.clone()
+            run(s, hint)
+            assert torch.equal(s.o[:s.used], got[:s.used])
+        for t, old in zip((s.table, s.lengths, s.offsets), keep):
+            t.copy_(old)
+
+
+@pytest.mark.parametrize("dtype", [F32, F16])
+@pytest.mark.parametrize("page", [16, 24])
+def test_captured_chunks(lib, cuda, page, dtype):
+    """Captured steps of many rows, two graphs with their own workspaces side by
+    side: the same bits as the eager call, replay after replay."""
+    steps = [Step([(70, 700), (1, 90), (33, 2000)], 4, 2, 64, page, dtype, seed=i) for i in range(2)]
+    objects = [paged.PagedAttention(s.cache, 4) for s in steps]
+    graphs, streams, batches = [], [torch.cuda.Stream() for _ in steps], [s.batch() for s in steps]
+    for s, a, b, stream in zip(steps, objects, batches, streams):
+        s.attend(attention_object=a)
+        s.check()
+        s.first = s.o.clone()
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph, stream=stream):
+            a.forward(b, s.q, s.o, (s.cos, s.sin), s.lse, stream=stream.cuda_stream)
+        graphs.append(graph)
+        s.o.fill_(7.0)
+    torch.cuda.synchronize()
+    for _ in range(5):
+        for graph, stream in zip(graphs, streams):
+            with torch.cuda.stream(stream):
+                graph.replay()
+    torch.cuda.synchronize()
+    for s in steps:
+        assert torch.equal(s.o, s.first)
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
+def test_more_requests_than_threads(lib, cuda, dtype):
+    """700 requests, a few of them with many rows: the division takes several
+    passes in the kernels of many rows too."""
+    s = Step([(40 if b % 300 == 7 else b % 2, 1 + 7 * b % 130 + 40) for b in range(700)], 2, 1, 64, 16,
+             dtype, seed=4)
+    for hint in (1, 100):
+        run(s, hint)
+        s.check()
