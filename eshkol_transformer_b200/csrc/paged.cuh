@@ -388,6 +388,10 @@ bool pool_map(CUtensorMap* map, void* pool, const et_b200_paged_cache_v1* c, int
               bool swizzled = true);
 
 // Host pieces of the entry points.
+template <typename... P>
+inline bool aligned_to(uintptr_t bytes, P... pointers) {
+  return ((reinterpret_cast<uintptr_t>(pointers) | ...) & (bytes - 1)) == 0;
+}
 int32_t check_cache(const et_b200_paged_cache_v1* c, et_kernel_error* e, const char* op);
 int32_t check_batch(const et_b200_paged_batch_v1* b, const et_b200_paged_cache_v1* c,
                     et_kernel_error* e, const char* op);

@@ -885,9 +885,9 @@ int32_t et_b200_paged_attention_v1(const et_b200_paged_cache_v1* c,
         o_stride > (int64_t)1 << 31)
       return set_error(e, ET_KERNEL_ERROR_NONCONTIGUOUS, ET_KERNEL_CODE_INVALID_BUFFER, op,
                        "rows of q or o overlap or lie too far apart");
-    if ((reinterpret_cast<uintptr_t>(q) | reinterpret_cast<uintptr_t>(o)) % size != 0)
+    if (!aligned_to(size, q, o) || !aligned_to(4, lse))
       return set_error(e, ET_KERNEL_ERROR_INVALID_ARGUMENT, ET_KERNEL_CODE_INVALID_BUFFER, op,
-                       "q and o must be aligned to their elements");
+                       "q, o and lse must be aligned to their elements");
     if (b->tokens * q_heads > INT32_MAX - 4096)
       return set_error(e, ET_KERNEL_ERROR_SHAPE_MISMATCH, ET_KERNEL_CODE_INVALID_SHAPE, op,
                        "tokens times q_heads must stay below 2^31");

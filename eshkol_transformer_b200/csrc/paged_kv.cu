@@ -180,6 +180,10 @@ int32_t check_batch(const et_b200_paged_batch_v1* b, const et_b200_paged_cache_v
   if (b->batch > 0 && (b->offsets == nullptr || b->lengths == nullptr || b->page_table == nullptr))
     return set_error(e, ET_KERNEL_ERROR_INVALID_ARGUMENT, ET_KERNEL_CODE_NULL_ARGUMENT, op,
                      "offsets, lengths and the page table are required");
+  if (!aligned_to(8, b->offsets, b->lengths) || !aligned_to(4, b->page_table, b->status))
+    return set_error(e, ET_KERNEL_ERROR_INVALID_ARGUMENT, ET_KERNEL_CODE_INVALID_BUFFER, op,
+                     "offsets, lengths, the page table and the status word must be aligned to "
+                     "their elements");
   return 0;
 }
 
@@ -191,6 +195,9 @@ int32_t check_rope(const et_b200_paged_rope_v1* r, et_kernel_error* e, const cha
   if (r->rows < 1)
     return set_error(e, ET_KERNEL_ERROR_SHAPE_MISMATCH, ET_KERNEL_CODE_INVALID_SHAPE, op,
                      "RoPE tables have no rows");
+  if (!aligned_to(4, r->cos, r->sin))
+    return set_error(e, ET_KERNEL_ERROR_INVALID_ARGUMENT, ET_KERNEL_CODE_INVALID_BUFFER, op,
+                     "RoPE tables must be aligned to their elements");
   return 0;
 }
 

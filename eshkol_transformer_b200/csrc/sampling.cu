@@ -1317,9 +1317,11 @@ extern "C" int32_t et_b200_sample_v1(const et_b200_sampling_v1* s, const void* l
       return set_error(e, ET_KERNEL_ERROR_INVALID_ARGUMENT, ET_KERNEL_CODE_NULL_ARGUMENT, op,
                        "logits, uniform numbers and ids are required");
     const uintptr_t size = s->dtype == ET_B200_DTYPE_F32 ? 4 : 2;
-    if (reinterpret_cast<uintptr_t>(logits) % size != 0)
+    using paged::aligned_to;
+    if (!aligned_to(size, logits) || !aligned_to(8, ids, s->top_k) ||
+        !aligned_to(4, uniform, logprobs, s->temperature, s->top_p, s->min_p))
       return set_error(e, ET_KERNEL_ERROR_INVALID_ARGUMENT, ET_KERNEL_CODE_INVALID_BUFFER, op,
-                       "logits must be aligned to their elements");
+                       "logits and the rows' values must be aligned to their elements");
     auto st = static_cast<cudaStream_t>(stream);
     const Args a{uniform, s->temperature, s->top_k, s->top_p, s->min_p, ids, logprobs,
                  s->row_stride, (int)s->vocabulary, 0};
