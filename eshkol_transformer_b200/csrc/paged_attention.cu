@@ -16,8 +16,9 @@
 // hi hi + hi lo + lo hi of operands rounded to TF32 pairs), which are joined
 // where a tile ends.  With few rows (a decoding step) reading the cache
 // bounds it: one tile of 16 rows, warps split along the keys.  Measured: 64 requests
-// of up to 8,192 keys (32 / 8 heads x 128, bf16, 1.35 GB) 231 us, 5.8 TB/s (274 us
-// with cp.async); one token over 300 f32 keys 9.6 us with the joining kernel.
+// of up to 8,192 keys (32 / 8 heads x 128, bf16, 1.35 GB) 230 to 248 us by machine,
+// 5.4 to 5.8 TB/s (274 us with cp.async where it took 231); one token over 300 f32
+// keys 9.6 us with the joining kernel.
 #include <math.h>
 
 #include <type_traits>

@@ -25,12 +25,12 @@
 // N = 2 head_dim; the halves of O are added when it is read.  The tensor pipe's f32
 // accumulation truncates, so every CHUNK blocks O moves to f32 sums in the
 // workspace.
-// Four ragged prompts of up to 1,024 tokens (16 heads x 64) take 92 us (307 us on
-// mma.sync; 99 with one conversion of both tiles per block), the same with 9,000
-// keys of history 625 us (730).  3,000 to 3,500 cycles per block of 64 keys and
-// 11,000 per tile for its queries and output: instructions bound it, and their
-// cache, which the roles' code together overflows (100 KB; 10 % of its requests miss),
-// so what runs seldom or waits anyway is not unrolled.
+// Four ragged prompts of up to 1,024 tokens (16 heads x 64) take 96 to 102 us by
+// machine (307 us on mma.sync), the same with 9,000 keys of history 600 us.  3,000 to
+// 3,500 cycles per block of 64 keys and 11,000 per tile for its queries and output:
+// instructions bound it, and their cache, which the roles' code together overflows
+// (100 KB; 8 % of its requests miss), so what runs seldom or waits anyway is not
+// unrolled, and a few instructions more or less move the time by some per cent.
 // Waits are bounded as in paged_attention_tc.cu.
 #include <math.h>
 

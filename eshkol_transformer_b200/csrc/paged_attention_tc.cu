@@ -9,13 +9,15 @@
 // traffic per product.  Each half has a thread that issues P V of a block and
 // the next Q K^T behind it (one thread for both left the tensor pipe idle for
 // 1,100 of 3,950 cycles per pair of blocks between barriers); the two take
-// turns, which keeps the halves out of step: while the pipe works on one half, the other half's four warps (one row per thread, no exchange between
-// threads) turn scores into probabilities, written over the scores in TMEM as
-// the A operand of P V.  The row maximum stands until a block exceeds it by
+// turns, which keeps the halves out of step: while the pipe works on one half, the
+// other half's four warps (one row per thread, no exchange between threads) turn
+// scores into probabilities, written over the scores in TMEM as the A operand of P V.  The row maximum stands until a block exceeds it by
 // 2^8 (2^4 at f16; the sums stay far inside f32), so O is rescaled in TMEM only then.
-// A 4,096-token chunk over 12,000 keys (32 / 8 heads x 128, bf16) takes 720 us, 927
-// TFLOP/s; a pair of half-blocks 3,520 cycles, 1,550 of them probabilities, whose
-// hand-off bounds it (the products alone take 2,750).
+// A 4,096-token chunk over 12,000 keys (32 / 8 heads x 128, bf16) takes 725 us, 920
+// TFLOP/s; a pair of half-blocks 3,520 cycles, 1,550 of them probabilities.  The
+// products alone take 2,750 (the pipe's rate would allow some 2,050: Q K^T reads both
+// 128-row operands from shared memory), the hand-off of scores and probabilities the
+// rest.
 // Waits are bounded; one that runs out raises a CTA-wide abort, copies and
 // products in flight are waited for and TMEM is released.
 #include <math.h>

@@ -242,9 +242,10 @@ int32_t et_b200_paged_append_v1(const et_b200_paged_cache_v1 *cache,
  * scores), -inf without keys.  Scores, statistics and sums are f32; for the
  * tensor cores q' and the probabilities are rounded to the pools' type at f16
  * and bf16 (q' with its residual up to 16 query rows per kv head), and all
- * operands are carried as pairs of about 22 bits at f32.  Keys and
- * values of positions below a request's length must be finite; slots behind
- * may hold anything.  o must overlap neither q nor the pools.  The workspace
+ * operands are carried as pairs of about 22 bits at f32 (above 16 query rows per
+ * kv head elements more than 2^16 below their row's largest only to 2^-38 of
+ * it).  Keys and values of positions below a request's length must be
+ * finite, those hidden from a query included; slots behind may hold anything.  o must overlap neither q nor the pools.  The workspace
  * (any contents, overwritten; its size does not depend on the batch) serves one
  * call at a time: calls that may overlap, and graphs that may, need one each. */
 size_t et_b200_paged_attention_workspace_bytes_v1(
@@ -270,8 +271,9 @@ int32_t et_b200_paged_attention_v1(const et_b200_paged_cache_v1 *cache,
  *                       left ranked before them;
  *   min_p  (<= 0: off)  w >= min_p (w of the most likely token is 1).
  * temperature NULL means 1; a row whose temperature is not above 2^-100 takes
- * the most likely token, with log-probability 0.  Weights are 2^-35 fixed
- * point, so results depend on no order of summation.  -inf and NaN logits are
+ * the most likely token, with log-probability 0; at an infinite one every logit
+ * above -inf weighs 1.  Weights are 2^-35 fixed point, so results depend on no
+ * order of summation and tokens below 2^-36 of the likeliest weigh nothing.  -inf and NaN logits are
  * never drawn; a row without others gets id -1 and log-probability -inf;
  * +inf logits share all weight.  vocabulary <= 2^22.  uniform is meant in
  * [0, 1); other values act as the nearest end. */
