@@ -11,13 +11,20 @@
 // 1,100 of 3,950 cycles per pair of blocks between barriers); the two take
 // turns, which keeps the halves out of step: while the pipe works on one half, the
 // other half's four warps (one row per thread, no exchange between threads) turn
-// scores into probabilities, written over the scores in TMEM as the A operand of P V.  The row maximum stands until a block exceeds it by
-// 2^8 (2^4 at f16; the sums stay far inside f32), so O is rescaled in TMEM only then.
+// scores into probabilities, written over the scores in TMEM as the A operand of P V.
+// The row maximum stands until a block exceeds it by 2^8 (2^4 at f16; the sums stay far
+// inside f32), so O is rescaled in TMEM only then.
 // A 4,096-token chunk over 12,000 keys (32 / 8 heads x 128, bf16) takes 725 us, 920
 // TFLOP/s; a pair of half-blocks 3,520 cycles, 1,550 of them probabilities.  The
 // products alone take 2,750 (the pipe's rate would allow some 2,050: Q K^T reads both
 // 128-row operands from shared memory), the hand-off of scores and probabilities the
 // rest.
+// Fewer bits, by choice: the rotated queries and the probabilities are rounded to the
+// cache's type (sums of weights are not).  The queries' residual would take 64 KB of
+// shared memory (two of the five slots at head_dim 128) and half as many score products
+// again.  Error of that chunk against 64 bits 2.9e-3 of the result, 1.7e-3 of it the
+// rounding of the output alone; each of the two roundings adds some 1.5e-3 to 1.9e-3 in
+// squares.
 // Waits are bounded; one that runs out raises a CTA-wide abort, copies and
 // products in flight are waited for and TMEM is released.
 #include <math.h>

@@ -4,12 +4,13 @@
 // written with v to slot pos % page_size of the request's page.  Pure data
 // movement: every byte is read once and written once.  The latency of its loads
 // bounds it: of the data in large steps (four 16-byte pieces of K and V in flight a
-// lane), of the chain offsets, length, page, tables in small ones.  One warp takes one token and 32 VPL 16-byte pieces of its
-// keys and values; the pieces are requested before the chain is followed,
-// so the two latencies overlap, and the request is found by a 32-ary search
-// of the whole warp (two load rounds up to 1,024 requests).  Measured: 27.5 us for
-// 32 MB of keys and values from 11 prompts (4.7 TB/s read and written, the writes to
-// L2), 2.8 us for one token; fewer pieces per lane with more resident warps took 28 to 30 us.
+// lane), of the chain offsets, length, page, tables in small ones.  One warp takes
+// one token and 32 VPL 16-byte pieces of its keys and values; the pieces are
+// requested before the chain is followed, so the two latencies overlap, and the
+// request is found by a 32-ary search of the whole warp (two load rounds up to 1,024
+// requests).  Measured: 27.5 us for 32 MB of keys and values from 11 prompts (4.7
+// TB/s read and written, the writes to L2), 2.8 us for one token; fewer pieces per
+// lane with more resident warps took 28 to 30 us.
 #include <type_traits>
 
 #include "attention_tc.cuh"

@@ -124,9 +124,8 @@ class PagedBatch:
     tensors; max_new (new tokens of the largest request as far as the host
     knows; None counts all tokens as one request's, which for many single
     tokens is the slower kernel) only picks the kernel, max_length is not used
-    so far.  status: an i32
-    tensor of one element that collects BAD_* and TIMEOUT bits, or None: then
-    nothing tells of either."""
+    so far.  status: an i32 tensor of one element that collects BAD_* and
+    TIMEOUT bits, or None: then nothing tells of either."""
 
     def __init__(self, offsets, lengths, page_table, tokens: int, max_new: int | None = None,
                  max_length: int | None = None, status=None):

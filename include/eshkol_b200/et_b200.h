@@ -185,9 +185,9 @@ typedef struct et_b200_paged_cache_v1 {
  * page_size].  A request may bring no token; a token at a negative position
  * is not stored and sees no key.  Rows of no request are not written, and
  * nothing depends on them.  max_new (the host's idea of the largest request)
- * only picks the kernel; max_length is not used so far.  The arrays are device memory, read when the kernels
- * run; what in them leads outside the pools or tensors is not followed but
- * recorded in *status (never cleared here): */
+ * only picks the kernel; max_length is not used so far.  The arrays are device
+ * memory, read when the kernels run; what in them leads outside the pools or
+ * tensors is not followed but recorded in *status (never cleared here): */
 enum {
   ET_B200_PAGED_BAD_PAGE = 1,   /* a page outside the pool: reads as zeros,
                                    writes are dropped */
@@ -244,10 +244,11 @@ int32_t et_b200_paged_append_v1(const et_b200_paged_cache_v1 *cache,
  * and bf16 (q' with its residual up to 16 query rows per kv head), and all
  * operands are carried as pairs of about 22 bits at f32 (above 16 query rows per
  * kv head elements more than 2^16 below their row's largest only to 2^-38 of
- * it).  Keys and values of positions below a request's length must be
- * finite, those hidden from a query included; slots behind may hold anything.  o must overlap neither q nor the pools.  The workspace
- * (any contents, overwritten; its size does not depend on the batch) serves one
- * call at a time: calls that may overlap, and graphs that may, need one each. */
+ * it).  Keys and values of positions below a request's length must be finite,
+ * those hidden from a query included; slots behind may hold anything.  o must
+ * overlap neither q nor the pools.  The workspace (any contents, overwritten; its
+ * size does not depend on the batch) serves one call at a time: calls that may
+ * overlap, and graphs that may, need one each. */
 size_t et_b200_paged_attention_workspace_bytes_v1(
     const et_b200_paged_cache_v1 *cache, int64_t q_heads);
 int32_t et_b200_paged_attention_v1(const et_b200_paged_cache_v1 *cache,
@@ -273,10 +274,10 @@ int32_t et_b200_paged_attention_v1(const et_b200_paged_cache_v1 *cache,
  * temperature NULL means 1; a row whose temperature is not above 2^-100 takes
  * the most likely token, with log-probability 0; at an infinite one every logit
  * above -inf weighs 1.  Weights are 2^-35 fixed point, so results depend on no
- * order of summation and tokens below 2^-36 of the likeliest weigh nothing.  -inf and NaN logits are
- * never drawn; a row without others gets id -1 and log-probability -inf;
- * +inf logits share all weight.  vocabulary <= 2^22.  uniform is meant in
- * [0, 1); other values act as the nearest end. */
+ * order of summation and tokens below 2^-36 of the likeliest weigh nothing.
+ * -inf and NaN logits are never drawn; a row without others gets id -1 and
+ * log-probability -inf; +inf logits share all weight.  vocabulary <= 2^22.
+ * uniform is meant in [0, 1); other values act as the nearest end. */
 typedef struct et_b200_sampling_v1 {
   size_t struct_size;
   int64_t rows, vocabulary, row_stride;

@@ -452,3 +452,64 @@ def test_more_requests_than_threads(lib, cuda, dtype):
     for hint in (1, 100):
         run(s, hint)
         s.check()
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("heads,page,dim", [(2, 16, 64), (1, 8, 128), (3, 1, 64), (1, 1, 32), (2, 24, 40)])
+@pytest.mark.parametrize("hint", [1, 100])
+def test_pools_inside_a_larger_tensor(lib, cuda, hint, heads, page, dim, dtype):
+    """Keys and values of one layer of a [pages, layers, 2, ...] tensor, appended and
+    attended in place; the other layers stay as they are."""
+    s = Step([(1, 40), (20, 90), (3, 3)], 2 * heads, heads, dim, page, dtype)
+    pages = s.keys.shape[0]
+    for layout in ("heads", "slots"):
+        shape = (heads, page, dim) if layout == "heads" else (page, heads, dim)
+        whole = torch.full((pages, 3, 2, *shape), 5.0, dtype=dtype, device="cuda")
+        s.keys, s.values = whole[:, 1, 0], whole[:, 1, 1]
+        if layout == "slots":
+            s.keys, s.values = s.keys.transpose(1, 2), s.values.transpose(1, 2)
+        s.cache = paged.PagedCache(s.keys, s.values)
+        new = [torch.cat([t[b][m - n:] for b, (n, m) in enumerate(s.requests)] + [t[0][:2]])
+               for t in (s.k, s.v)]
+        for b, (n, m) in enumerate(s.requests):  # what was cached before this step
+            s.store(b, s.k[b][:m - n], s.v[b][:m - n])
+        s.cache.append(s.batch(), *new)
+        run(s, hint)
+        check(s)
+        assert (whole[:, 0] == 5.0).all() and (whole[:, 2] == 5.0).all()
+
+
+def test_two_host_threads(lib, cuda):
+    """Steps issued from two threads on streams of their own, each with its own
+    objects, give the bits that they give alone."""
+    import threading
+    steps = [Step([(1, 900), (30, 300)], 4, 2, 64, 16, t, seed=i) for i, t in enumerate((F16, F32))]
+    want, streams, errors = [], [torch.cuda.Stream() for _ in steps], []
+    for s in steps:
+        s.attend()
+        s.check()
+        want.append(s.o.clone())
+        s.o.fill_(7.0)
+    torch.cuda.synchronize()
+
+    def work(s, stream, first):
+        try:
+            a = paged.PagedAttention(s.cache, s.q_heads)
+            x = torch.zeros(2, 5000, device="cuda")
+            ids = torch.full((2,), -7, dtype=torch.int64, device="cuda")
+            torch.cuda.synchronize()
+            with torch.cuda.stream(stream):
+                for _ in range(50):
+                    s.attend(attention_object=a, stream=None)
+                    sampling.Sampler(2, 5000).sample(x, x[:, 0].contiguous(), ids)
+            stream.synchronize()
+            assert torch.equal(s.o, first) and (ids == 0).all()
+        except BaseException as e:
+            errors.append(e)
+
+    threads = [threading.Thread(target=work, args=a) for a in zip(steps, streams, want)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert not errors, errors
