@@ -10,17 +10,17 @@
 // of at least 8 slots by TMA from a warp of its own, which keeps copies,
 // look-ups and block-wide barriers out of the arithmetic warps; any other page
 // size by 16-byte cp.async, the key addresses of a block looked up one block
-// ahead of its copies.  Warp
-// (wm, wk) takes 16 rows and BK / WK keys of each block with its own maxima,
-// sums and accumulators (mma.sync m16n8k16, or for f32 m16n8k8 as 3xTF32:
-// hi hi + hi lo + lo hi of operands rounded to TF32 pairs), which are joined
-// where a tile ends.  At f16 and bf16 the queries carry their rounding's residual (the
-// products are not what bounds it); the probabilities are rounded to the cache's type,
-// which adds a third to the error of the output's own rounding.  With few rows (a decoding step) reading the cache
-// bounds it: one tile of 16 rows, warps split along the keys.  Measured: 64 requests
-// of up to 8,192 keys (32 / 8 heads x 128, bf16, 1.35 GB) 230 to 248 us by machine,
-// 5.4 to 5.8 TB/s (274 us with cp.async where it took 231); one token over 300 f32
-// keys 9.6 us with the joining kernel.
+// ahead of its copies.  Warp (wm, wk) takes 16 rows and BK / WK keys of each block
+// with its own maxima, sums and accumulators (mma.sync m16n8k16, or for f32 m16n8k8
+// as 3xTF32: hi hi + hi lo + lo hi of operands rounded to TF32 pairs), which are
+// joined where a tile ends.  At f16 and bf16 the queries carry their rounding's
+// residual (the products are not what bounds it); the probabilities are rounded to
+// the cache's type, which adds a third to the error of the output's own rounding.
+// With few rows (a decoding step) reading the cache bounds it: one tile of 16 rows,
+// warps split along the keys.  Measured: 64 requests of up to 8,192 keys (32 / 8
+// heads x 128, bf16, 1.35 GB) 230 to 248 us by machine, 5.4 to 5.8 TB/s (274 us with
+// cp.async where it took 231); one token over 300 f32 keys 9.6 us with the joining
+// kernel.
 #include <math.h>
 
 #include <type_traits>
