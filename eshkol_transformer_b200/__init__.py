@@ -8,7 +8,8 @@ Python handles over its entry points:
 * ``LanguageModel`` -- the native training step (et_b200_lm_*);
 * ``Optimizer`` -- the O2-shaped device AdamW (et_b200_o2_*);
 * ``paged``, ``sampling`` -- the serving operators on torch tensors
-  (et_b200_paged_*, et_b200_sample_v1).
+  (et_b200_paged_*, et_b200_sample_v1, et_b200_probabilities_v1,
+  et_b200_verify_v1).
 
 There is no fallback: loading fails loudly when the library is missing.
 """
@@ -96,6 +97,14 @@ def load() -> C.CDLL:
         "et_b200_paged_attention_v1": (C.c_int32, [C.c_void_p] * 3 +
                                        [C.c_int64, C.c_void_p, C.c_int64, C.c_void_p, C.c_int64,
                                         C.c_void_p, C.c_void_p, C.c_size_t, C.c_void_p, E]),
+        "et_b200_paged_append8_v1": (C.c_int32, [C.c_void_p] * 4 + [C.c_int64, C.c_void_p,
+                                                                    C.c_int64, C.c_void_p, E]),
+        "et_b200_paged_attention8_workspace_bytes_v1": (C.c_size_t, [C.c_void_p, C.c_int64]),
+        "et_b200_paged_attention8_v1": (C.c_int32, [C.c_void_p] * 3 +
+                                        [C.c_int64, C.c_void_p, C.c_int64, C.c_void_p, C.c_int64,
+                                         C.c_void_p, C.c_void_p, C.c_size_t, C.c_void_p, E]),
+        "et_b200_probabilities_v1": (C.c_int32, [C.c_void_p] * 3 + [C.c_int64, C.c_void_p, E]),
+        "et_b200_verify_v1": (C.c_int32, [C.c_void_p] * 6 + [E]),
         "et_b200_sample_v1": (C.c_int32, [C.c_void_p] * 6 + [E]),
         "et_b200_o2_optimizer_create_v1": (C.c_int32, [C.c_size_t, C.c_void_p, C.c_uint32,
                                                        C.c_uint32, C.c_uint32, C.c_uint64,

@@ -393,11 +393,16 @@ inline bool aligned_to(uintptr_t bytes, P... pointers) {
   return ((reinterpret_cast<uintptr_t>(pointers) | ...) & (bytes - 1)) == 0;
 }
 int32_t check_cache(const et_b200_paged_cache_v1* c, et_kernel_error* e, const char* op);
-int32_t check_batch(const et_b200_paged_batch_v1* b, const et_b200_paged_cache_v1* c,
-                    et_kernel_error* e, const char* op);
+int32_t check_batch(const et_b200_paged_batch_v1* b, int64_t page_size, et_kernel_error* e,
+                    const char* op);
+bool strides_nest(int64_t page_size, int64_t kv_heads, int64_t row, int64_t pages, int64_t ps,
+                  int64_t hs, int64_t ts);
 int32_t check_rope(const et_b200_paged_rope_v1* r, et_kernel_error* e, const char* op);
+// The append's rows of k and v: `row` elements of `size` bytes.
+int32_t check_new_rows(const void* k, int64_t k_stride, const void* v, int64_t v_stride, int64_t row,
+                       int64_t size, et_kernel_error* e, const char* op);
 Pools pools_of(const et_b200_paged_cache_v1* c);
-Batch batch_of(const et_b200_paged_batch_v1* b, const et_b200_paged_cache_v1* c);
+Batch batch_of(const et_b200_paged_batch_v1* b, int64_t page_size);
 Rope rope_of(const et_b200_paged_rope_v1* r);
 // `most` thread blocks, or fewer where the host's sizes leave fewer units.
 inline int thread_blocks(const AttendArgs& a, int most, int rows, int keys) {
@@ -405,6 +410,18 @@ inline int thread_blocks(const AttendArgs& a, int most, int rows, int keys) {
   const int64_t blocks = (a.batch.capacity + keys - 1) / keys;
   return blocks < most && tiles * blocks < most ? (int)(tiles * blocks) : most;
 }
+// What the attention's entry points check alike (`size`: bytes of an element of q and o),
+// and the workspace of both.
+bool heads_fit(int64_t kv_heads, int64_t q_heads);
+size_t attention_workspace(int64_t head_dim, int sms);
+int32_t check_attention(const et_b200_paged_batch_v1* b, int64_t head_dim, int64_t size,
+                        int64_t q_heads, const void* q, int64_t q_stride, const void* o,
+                        int64_t o_stride, const float* lse, const void* workspace, size_t bytes,
+                        size_t need, et_kernel_error* e, const char* op);
+// Joins the parts of cut tiles (paged_attention.cu): `blocks` thread blocks' of the launch
+// before, about `rows` rows a tile; dtype that of o, dim_padded that of the sums (64 to 256).
+void join_parts(const AttendArgs& a, uint32_t dtype, int dim_padded, int blocks, int64_t rows,
+                cudaStream_t stream);
 // The tcgen05 kernel (paged_attention_tc.cu): launches it and returns its
 // thread blocks, 0 where it does not take the cache (nothing is launched).
 size_t attend_tc_workspace(int dim_padded, int sms);

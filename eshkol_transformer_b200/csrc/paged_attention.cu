@@ -25,97 +25,12 @@
 
 #include <type_traits>
 
-#include "attention_tc.cuh"
-#include "paged.cuh"
+#include "paged_mma.cuh"
 
 namespace etb {
 namespace {
 
 using namespace paged;
-
-// ---- warp matrix pieces -----------------------------------------------------------------
-
-__device__ __forceinline__ void ldsm4(uint32_t (&r)[4], uint32_t addr) {
-  asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0,%1,%2,%3}, [%4];"
-               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
-               : "r"(addr)
-               : "memory");
-}
-__device__ __forceinline__ void ldsm4t(uint32_t (&r)[4], uint32_t addr) {
-  asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0,%1,%2,%3}, [%4];"
-               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
-               : "r"(addr)
-               : "memory");
-}
-__device__ __forceinline__ uint32_t lds32(uint32_t addr) {
-  uint32_t v;
-  asm volatile("ld.shared.b32 %0, [%1];" : "=r"(v) : "r"(addr) : "memory");
-  return v;
-}
-template <typename T>
-__device__ __forceinline__ void mma16(float (&d)[4], const uint32_t (&a)[4], uint32_t b0,
-                                      uint32_t b1) {
-  if constexpr (std::is_same_v<T, __half>)
-    asm volatile(
-        "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, "
-        "{%8,%9}, {%0,%1,%2,%3};"
-        : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
-        : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
-  else
-    asm volatile(
-        "mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, "
-        "{%8,%9}, {%0,%1,%2,%3};"
-        : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
-        : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
-}
-__device__ __forceinline__ void mma_tf32(float (&d)[4], const uint32_t (&a)[4], uint32_t b0,
-                                         uint32_t b1) {
-  asm volatile(
-      "mma.sync.aligned.m16n8k8.row.col.f32.tf32.tf32.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, "
-      "{%8,%9}, {%0,%1,%2,%3};"
-      : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
-      : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
-}
-// x = hi + lo + r with hi, lo TF32 values, |r| <= 2^-22 |x|
-__device__ __forceinline__ void pair_tf32(uint32_t x, uint32_t& hi, uint32_t& lo) {
-  asm("cvt.rna.tf32.f32 %0, %1;" : "=r"(hi) : "f"(__uint_as_float(x)));
-  const float rest = __uint_as_float(x) - __uint_as_float(hi);
-  asm("cvt.rna.tf32.f32 %0, %1;" : "=r"(lo) : "f"(rest));
-}
-template <typename T>
-__device__ __forceinline__ uint32_t pack2(float a, float b) {
-  if constexpr (std::is_same_v<T, __half>) {
-    const __half2 h = __floats2half2_rn(a, b);
-    return *reinterpret_cast<const uint32_t*>(&h);
-  } else {
-    const __nv_bfloat162 h = __floats2bfloat162_rn(a, b);
-    return *reinterpret_cast<const uint32_t*>(&h);
-  }
-}
-__device__ __forceinline__ void cp16(uint32_t dst, const void* src, bool full) {
-  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src),
-               "r"(full ? 16 : 0)
-               : "memory");
-}
-__device__ __forceinline__ void cp_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
-template <int N>
-__device__ __forceinline__ void cp_wait() {
-  asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
-}
-
-// Two neighbouring outputs; one store where the address allows it.
-template <typename T>
-__device__ __forceinline__ void store2(T* dst, float a, float b) {
-  if ((reinterpret_cast<uintptr_t>(dst) & (2 * sizeof(T) - 1)) == 0) {
-    if constexpr (sizeof(T) == 4)
-      *reinterpret_cast<float2*>(dst) = make_float2(a, b);
-    else
-      *reinterpret_cast<uint32_t*>(dst) = pack2<T>(a, b);
-  } else {
-    dst[0] = from_f32<T>(a);
-    dst[1] = from_f32<T>(b);
-  }
-}
 
 // ---- the kernel -------------------------------------------------------------------------
 
@@ -743,30 +658,6 @@ __global__ void __launch_bounds__(32 * JOIN_WARPS) paged_join_kernel(AttendArgs 
 
 // ---- launching --------------------------------------------------------------------------
 
-// Padded head_dim of the kernels: 32, 64, 128 or 256.
-int padded(int64_t dim) { return dim <= 32 ? 32 : dim <= 64 ? 64 : dim <= 128 ? 128 : 256; }
-
-constexpr int kMostPerSm = 4;  // resident thread blocks per SM that the workspace allows for
-
-// Resident thread blocks of a kernel per SM (at most kMostPerSm), per device
-// (the attribute that admits its shared memory is set on the way).
-template <auto Kernel>
-int resident_blocks(int threads, int smem) {
-  static std::atomic<int> known[64];
-  int dev = 0;
-  cudaGetDevice(&dev);
-  if (dev >= 0 && dev < 64) {
-    const int n = known[dev].load(std::memory_order_relaxed);
-    if (n > 0) return n;
-  }
-  cudaFuncSetAttribute(Kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
-  int n = 0;
-  cudaOccupancyMaxActiveBlocksPerMultiprocessor(&n, Kernel, threads, smem);
-  n = n < 1 ? 1 : n > kMostPerSm ? kMostPerSm : n;
-  if (dev >= 0 && dev < 64) known[dev].store(n, std::memory_order_relaxed);
-  return n;
-}
-
 template <typename T, int DH>
 void launch_join(const AttendArgs& a, int blocks, int64_t rows, cudaStream_t stream) {
   if (cudaPeekAtLastError() != cudaSuccess) return;  // no parts were left to join
@@ -842,17 +733,63 @@ void launch_type(const et_b200_paged_cache_v1* c, AttendArgs& a, int64_t max_new
   }
 }
 
-bool heads_fit(const et_b200_paged_cache_v1* c, int64_t q_heads) {
-  return q_heads >= 1 && q_heads <= 65536 && q_heads % c->kv_heads == 0;
+template <typename T>
+void join_type(const AttendArgs& a, int dim_padded, int blocks, int64_t rows, cudaStream_t stream) {
+  switch (dim_padded) {
+    case 64: return launch_join<T, 64>(a, blocks, rows, stream);
+    case 128: return launch_join<T, 128>(a, blocks, rows, stream);
+    default: return launch_join<T, 256>(a, blocks, rows, stream);
+  }
 }
 
-size_t workspace_bytes(int64_t head_dim, int sms) {
+}  // namespace
+
+namespace paged {
+
+size_t attention_workspace(int64_t head_dim, int sms) {
   const int dim = padded(head_dim);
   const size_t plain = joint_bytes(kMostPerSm * sms, 64, dim), tc = attend_tc_workspace(dim, sms);
   return plain > tc ? plain : tc;
 }
 
-}  // namespace
+bool heads_fit(int64_t kv_heads, int64_t q_heads) {
+  return q_heads >= 1 && q_heads <= 65536 && q_heads % kv_heads == 0;
+}
+
+int32_t check_attention(const et_b200_paged_batch_v1* b, int64_t head_dim, int64_t size,
+                        int64_t q_heads, const void* q, int64_t q_stride, const void* o,
+                        int64_t o_stride, const float* lse, const void* workspace, size_t bytes,
+                        size_t need, et_kernel_error* e, const char* op) {
+  const int64_t row = q_heads * head_dim;
+  if (q == nullptr || o == nullptr)
+    return set_error(e, ET_KERNEL_ERROR_INVALID_ARGUMENT, ET_KERNEL_CODE_NULL_ARGUMENT, op,
+                     "q and o are required");
+  if (q_stride < row || o_stride < row || q_stride > (int64_t)1 << 31 ||
+      o_stride > (int64_t)1 << 31)
+    return set_error(e, ET_KERNEL_ERROR_NONCONTIGUOUS, ET_KERNEL_CODE_INVALID_BUFFER, op,
+                     "rows of q or o overlap or lie too far apart");
+  if (!aligned_to(size, q, o) || !aligned_to(4, lse))
+    return set_error(e, ET_KERNEL_ERROR_INVALID_ARGUMENT, ET_KERNEL_CODE_INVALID_BUFFER, op,
+                     "q, o and lse must be aligned to their elements");
+  if (b->tokens * q_heads > INT32_MAX - 4096)
+    return set_error(e, ET_KERNEL_ERROR_SHAPE_MISMATCH, ET_KERNEL_CODE_INVALID_SHAPE, op,
+                     "tokens times q_heads must stay below 2^31");
+  if (workspace == nullptr || (reinterpret_cast<uintptr_t>(workspace) & 255) != 0 ||
+      bytes < need)
+    return set_error(e, ET_KERNEL_ERROR_INVALID_ARGUMENT, ET_KERNEL_CODE_BUFFER_TOO_SMALL, op,
+                     "workspace is smaller than et_b200_paged_attention_workspace_bytes_v1 or "
+                     "not 256-byte aligned");
+  return 0;
+}
+
+void join_parts(const AttendArgs& a, uint32_t dtype, int dim_padded, int blocks, int64_t rows,
+                cudaStream_t stream) {
+  if (dtype == ET_B200_DTYPE_F32) join_type<float>(a, dim_padded, blocks, rows, stream);
+  else if (dtype == ET_B200_DTYPE_F16) join_type<__half>(a, dim_padded, blocks, rows, stream);
+  else join_type<__nv_bfloat16>(a, dim_padded, blocks, rows, stream);
+}
+
+}  // namespace paged
 }  // namespace etb
 
 using namespace etb;
@@ -862,8 +799,8 @@ extern "C" {
 
 size_t et_b200_paged_attention_workspace_bytes_v1(const et_b200_paged_cache_v1* c,
                                                   int64_t q_heads) {
-  if (check_cache(c, nullptr, "paged-attention-workspace") || !heads_fit(c, q_heads)) return 0;
-  return workspace_bytes(c->head_dim, sm_count());
+  if (check_cache(c, nullptr, "paged-attention-workspace") || !heads_fit(c->kv_heads, q_heads)) return 0;
+  return attention_workspace(c->head_dim, sm_count());
 }
 
 int32_t et_b200_paged_attention_v1(const et_b200_paged_cache_v1* c,
@@ -874,35 +811,20 @@ int32_t et_b200_paged_attention_v1(const et_b200_paged_cache_v1* c,
                                    et_kernel_error* e) {
   const char* op = "paged-attention";
   if (int32_t r = check_cache(c, e, op)) return r;
-  if (int32_t r = check_batch(b, c, e, op)) return r;
+  if (int32_t r = check_batch(b, c->page_size, e, op)) return r;
   if (int32_t r = check_rope(rope, e, op)) return r;
-  if (!heads_fit(c, q_heads))
+  if (!heads_fit(c->kv_heads, q_heads))
     return set_error(e, ET_KERNEL_ERROR_SHAPE_MISMATCH, ET_KERNEL_CODE_INVALID_SHAPE, op,
                      "q_heads must be a multiple of the cache's kv_heads, up to 65536");
   if (b->tokens > 0 && b->batch > 0) {
-    const int64_t row = q_heads * c->head_dim, size = c->dtype == ET_B200_DTYPE_F32 ? 4 : 2;
-    if (q == nullptr || o == nullptr)
-      return set_error(e, ET_KERNEL_ERROR_INVALID_ARGUMENT, ET_KERNEL_CODE_NULL_ARGUMENT, op,
-                       "q and o are required");
-    if (q_stride < row || o_stride < row || q_stride > (int64_t)1 << 31 ||
-        o_stride > (int64_t)1 << 31)
-      return set_error(e, ET_KERNEL_ERROR_NONCONTIGUOUS, ET_KERNEL_CODE_INVALID_BUFFER, op,
-                       "rows of q or o overlap or lie too far apart");
-    if (!aligned_to(size, q, o) || !aligned_to(4, lse))
-      return set_error(e, ET_KERNEL_ERROR_INVALID_ARGUMENT, ET_KERNEL_CODE_INVALID_BUFFER, op,
-                       "q, o and lse must be aligned to their elements");
-    if (b->tokens * q_heads > INT32_MAX - 4096)
-      return set_error(e, ET_KERNEL_ERROR_SHAPE_MISMATCH, ET_KERNEL_CODE_INVALID_SHAPE, op,
-                       "tokens times q_heads must stay below 2^31");
     const int sms = sm_count();
-    if (workspace == nullptr || (reinterpret_cast<uintptr_t>(workspace) & 255) != 0 ||
-        bytes < workspace_bytes(c->head_dim, sms))
-      return set_error(e, ET_KERNEL_ERROR_INVALID_ARGUMENT, ET_KERNEL_CODE_BUFFER_TOO_SMALL, op,
-                       "workspace is smaller than et_b200_paged_attention_workspace_bytes_v1 or "
-                       "not 256-byte aligned");
+    if (int32_t r = check_attention(b, c->head_dim, c->dtype == ET_B200_DTYPE_F32 ? 4 : 2, q_heads,
+                                    q, q_stride, o, o_stride, lse, workspace, bytes,
+                                    attention_workspace(c->head_dim, sms), e, op))
+      return r;
     AttendArgs a{};
     a.pools = pools_of(c);
-    a.batch = batch_of(b, c);
+    a.batch = batch_of(b, c->page_size);
     a.rope = rope_of(rope);
     a.tiling.group = (int)(q_heads / c->kv_heads);
     a.keys = c->keys;

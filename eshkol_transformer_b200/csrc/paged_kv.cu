@@ -130,6 +130,19 @@ void launch_append(const et_b200_paged_cache_v1* c, const Pools& P, const Batch&
 
 namespace paged {
 
+// Whether no stride lets two rows of a pool share a place: the smallest nesting is
+// token < head < page or head < token < page.  Far strides are refused too.
+bool strides_nest(int64_t page_size, int64_t kv_heads, int64_t row, int64_t pages, int64_t ps,
+                  int64_t hs, int64_t ts) {
+  if (ts < 1 || hs < 1 || ps < 1 || ts > (int64_t)1 << 31 || hs > (int64_t)1 << 36 ||
+      ps > INT64_MAX / 8 / pages)
+    return false;
+  return (ts >= row && hs >= (page_size - 1) * ts + row &&
+          ps >= (kv_heads - 1) * hs + (page_size - 1) * ts + row) ||
+         (hs >= row && ts >= (kv_heads - 1) * hs + row &&
+          ps >= (page_size - 1) * ts + (kv_heads - 1) * hs + row);
+}
+
 int32_t check_cache(const et_b200_paged_cache_v1* c, et_kernel_error* e, const char* op) {
   if (c == nullptr || c->struct_size < sizeof(et_b200_paged_cache_v1))
     return set_error(e, ET_KERNEL_ERROR_VERSION_MISMATCH, ET_KERNEL_CODE_INVALID_STRUCT_SIZE, op,
@@ -144,17 +157,8 @@ int32_t check_cache(const et_b200_paged_cache_v1* c, et_kernel_error* e, const c
                      "paged cache shape is outside its limits (head_dim: a multiple of 8 up to "
                      "256)");
   const int64_t size = c->dtype == ET_B200_DTYPE_F32 ? 4 : 2;
-  const int64_t most = INT64_MAX / 8;
-  // no stride may let two elements of the pools share a place: the smallest
-  // nesting is token < head < page or head < token < page
   const int64_t hs = c->head_stride, ts = c->token_stride, ps = c->page_stride;
-  const bool nested =
-      (ts >= c->head_dim && hs >= (c->page_size - 1) * ts + c->head_dim &&
-       ps >= (c->kv_heads - 1) * hs + (c->page_size - 1) * ts + c->head_dim) ||
-      (hs >= c->head_dim && ts >= (c->kv_heads - 1) * hs + c->head_dim &&
-       ps >= (c->page_size - 1) * ts + (c->kv_heads - 1) * hs + c->head_dim);
-  if (ts < 1 || hs < 1 || ps < 1 || ts > (int64_t)1 << 31 || hs > (int64_t)1 << 36 ||
-      ps > most / c->pages || !nested)
+  if (!strides_nest(c->page_size, c->kv_heads, c->head_dim, c->pages, ps, hs, ts))
     return set_error(e, ET_KERNEL_ERROR_NONCONTIGUOUS, ET_KERNEL_CODE_INVALID_BUFFER, op,
                      "paged cache strides overlap or are out of range");
   if (c->keys == nullptr || c->values == nullptr)
@@ -167,13 +171,13 @@ int32_t check_cache(const et_b200_paged_cache_v1* c, et_kernel_error* e, const c
   return 0;
 }
 
-int32_t check_batch(const et_b200_paged_batch_v1* b, const et_b200_paged_cache_v1* c,
-                    et_kernel_error* e, const char* op) {
+int32_t check_batch(const et_b200_paged_batch_v1* b, int64_t page_size, et_kernel_error* e,
+                    const char* op) {
   if (b == nullptr || b->struct_size < sizeof(et_b200_paged_batch_v1))
     return set_error(e, ET_KERNEL_ERROR_VERSION_MISMATCH, ET_KERNEL_CODE_INVALID_STRUCT_SIZE, op,
                      "paged batch descriptor is missing or truncated");
   if (b->batch < 0 || b->batch > (1 << 20) || b->tokens < 0 || b->tokens > (1 << 26) ||
-      b->table_columns < 1 || b->table_columns > kMostCapacity / c->page_size || b->max_new < 0 ||
+      b->table_columns < 1 || b->table_columns > kMostCapacity / page_size || b->max_new < 0 ||
       b->max_length < 0)
     return set_error(e, ET_KERNEL_ERROR_SHAPE_MISMATCH, ET_KERNEL_CODE_INVALID_SHAPE, op,
                      "paged batch is outside its limits (a page table holds fewer than 2^31 - "
@@ -185,6 +189,21 @@ int32_t check_batch(const et_b200_paged_batch_v1* b, const et_b200_paged_cache_v
     return set_error(e, ET_KERNEL_ERROR_INVALID_ARGUMENT, ET_KERNEL_CODE_INVALID_BUFFER, op,
                      "offsets, lengths, the page table and the status word must be aligned to "
                      "their elements");
+  return 0;
+}
+
+int32_t check_new_rows(const void* k, int64_t k_stride, const void* v, int64_t v_stride, int64_t row,
+                       int64_t size, et_kernel_error* e, const char* op) {
+  if (k == nullptr || v == nullptr)
+    return set_error(e, ET_KERNEL_ERROR_INVALID_ARGUMENT, ET_KERNEL_CODE_NULL_ARGUMENT, op,
+                     "k and v are required");
+  if (k_stride < row || v_stride < row || k_stride > (int64_t)1 << 31 ||
+      v_stride > (int64_t)1 << 31)
+    return set_error(e, ET_KERNEL_ERROR_NONCONTIGUOUS, ET_KERNEL_CODE_INVALID_BUFFER, op,
+                     "rows of k and v overlap or lie too far apart");
+  if ((reinterpret_cast<uintptr_t>(k) | reinterpret_cast<uintptr_t>(v)) % size != 0)
+    return set_error(e, ET_KERNEL_ERROR_INVALID_ARGUMENT, ET_KERNEL_CODE_INVALID_BUFFER, op,
+                     "k and v must be aligned to their elements");
   return 0;
 }
 
@@ -229,9 +248,9 @@ Pools pools_of(const et_b200_paged_cache_v1* c) {
   return Pools{c->pages, c->page_stride, c->head_stride, c->token_stride, (int)c->page_size,
                (int)c->kv_heads, (int)c->head_dim, divisor_of((uint32_t)c->page_size)};
 }
-Batch batch_of(const et_b200_paged_batch_v1* b, const et_b200_paged_cache_v1* c) {
+Batch batch_of(const et_b200_paged_batch_v1* b, int64_t page_size) {
   return Batch{b->offsets, b->lengths, b->page_table, b->status, b->tokens, b->table_columns,
-               (int)b->batch, (int)(b->table_columns * c->page_size)};
+               (int)b->batch, (int)(b->table_columns * page_size)};
 }
 Rope rope_of(const et_b200_paged_rope_v1* r) {
   return r == nullptr ? Rope{nullptr, nullptr, 0} : Rope{r->cos, r->sin, r->rows};
@@ -250,22 +269,13 @@ extern "C" int32_t et_b200_paged_append_v1(const et_b200_paged_cache_v1* c,
                                            void* stream, et_kernel_error* e) {
   const char* op = "paged-append";
   if (int32_t r = check_cache(c, e, op)) return r;
-  if (int32_t r = check_batch(b, c, e, op)) return r;
+  if (int32_t r = check_batch(b, c->page_size, e, op)) return r;
   if (int32_t r = check_rope(rope, e, op)) return r;
   const int64_t row = c->kv_heads * c->head_dim, size = c->dtype == ET_B200_DTYPE_F32 ? 4 : 2;
   if (b->tokens > 0 && b->batch > 0) {
-    if (k == nullptr || v == nullptr)
-      return set_error(e, ET_KERNEL_ERROR_INVALID_ARGUMENT, ET_KERNEL_CODE_NULL_ARGUMENT, op,
-                       "k and v are required");
-    if (k_stride < row || v_stride < row || k_stride > (int64_t)1 << 31 ||
-        v_stride > (int64_t)1 << 31)
-      return set_error(e, ET_KERNEL_ERROR_NONCONTIGUOUS, ET_KERNEL_CODE_INVALID_BUFFER, op,
-                       "rows of k and v overlap or lie too far apart");
-    if ((reinterpret_cast<uintptr_t>(k) | reinterpret_cast<uintptr_t>(v)) % size != 0)
-      return set_error(e, ET_KERNEL_ERROR_INVALID_ARGUMENT, ET_KERNEL_CODE_INVALID_BUFFER, op,
-                       "k and v must be aligned to their elements");
+    if (int32_t r = check_new_rows(k, k_stride, v, v_stride, row, size, e, op)) return r;
     const Pools P = pools_of(c);
-    const Batch B = batch_of(b, c);
+    const Batch B = batch_of(b, c->page_size);
     const Rope R = rope_of(rope);
     auto st = static_cast<cudaStream_t>(stream);
     if (c->dtype == ET_B200_DTYPE_F32) launch_append<float>(c, P, B, R, k, k_stride, v, v_stride, st);

@@ -1,4 +1,5 @@
-// Sampling one token per row of logits (et_b200_sample_v1).
+// Sampling one token per row of logits (et_b200_sample_v1), and the distributions that it
+// draws from (et_b200_probabilities_v1).
 //
 // Weights w(x) = exp((x - M) / temperature), M the row's maximum, as 2^-35
 // fixed point: integer sums are the same in every order, so cumulative sums,
@@ -343,7 +344,8 @@ struct Args {
   const float* min_p;
   int64_t* ids;
   float* logprobs;
-  int64_t row_stride;
+  float* probs;  // et_b200_probabilities_v1: no draw, the rows' distributions
+  int64_t row_stride, probs_stride;
   int n, slice;  // tokens of a row, of a slice
 };
 __device__ __forceinline__ Filters filters_of(const Args& a, int64_t row) {
@@ -352,7 +354,7 @@ __device__ __forceinline__ Filters filters_of(const Args& a, int64_t row) {
   f.top_k = a.top_k != nullptr ? a.top_k[row] : 0;
   f.top_p = a.top_p != nullptr ? a.top_p[row] : 1.0f;
   f.min_p = a.min_p != nullptr ? a.min_p[row] : 0.0f;
-  f.uniform = (double)a.uniform[row];
+  f.uniform = a.uniform != nullptr ? (double)a.uniform[row] : 0.0;
   f.per = 1.4426950408889634 / (double)f.temperature;
   // at an infinite temperature every logit weighs 1, which is no less than min_p
   f.fall = !(f.min_p > 0.0f) ? 0.0
@@ -394,8 +396,19 @@ __device__ __forceinline__ void answer(const Args& a, int64_t row, int id, float
   a.logprobs[row] = (float)((d * f.per - (double)k) * 0.6931471805599453 - (double)logf(m));
 }
 
+// What a token's weight is divided by: the total in units of the weight 1.
+__device__ __forceinline__ float per_total(uint64_t total) {
+  return (float)(0x1p35 / (double)total);
+}
+// The probability of a kept token: its weight as f32 (a fixed-point one has few bits
+// where it is small), 0 where the fixed-point one is 0.
+__device__ __forceinline__ float share_of(float x, const Scale& s, float inv) {
+  const float w = power_of(x, s);
+  return w > 0x1p-36f ? w * inv : 0.0f;
+}
+
 // One thread block draws for a row in global memory: radix selection.
-template <typename T>
+template <typename T, bool PROBS>
 __device__ void sample_row(const T* x, const Args& a, int64_t row, const Filters& flt,
                            const Scale& sc, Shared& sm) {
   const int n = a.n;
@@ -420,7 +433,16 @@ __device__ void sample_row(const T* x, const Args& a, int64_t row, const Filters
         total = all;
         return draw_aim(flt.uniform, all);
       });
-  if (threadIdx.x == 0) answer(a, row, id, to_f32<T>(x[id]), flt, sc, total);
+  if constexpr (PROBS) {
+    const float inv = per_total(total);
+    float* out = a.probs + row * a.probs_stride;
+    for (int i = threadIdx.x; i < n; i += NT) {
+      const float v = to_f32<T>(x[i]);
+      out[i] = kept(cut, key_of(v), i) ? share_of(v, sc, inv) : 0.0f;
+    }
+  } else {
+    if (threadIdx.x == 0) answer(a, row, id, to_f32<T>(x[id]), flt, sc, total);
+  }
 }
 
 // ---- rows in the shared memory of a cluster ------------------------------------------------
@@ -677,7 +699,9 @@ __device__ __forceinline__ void count_before(const Ranking& r, int n, const Room
   *mass = m;
 }
 
-// Rank 0: cuts the list of n entries by all filters and draws (n <= NT).
+// Rank 0: cuts the list of n entries by all filters and draws (n <= NT), or, for
+// distributions, leaves the last kept entry in rm.border and what is kept in rm.total.
+template <bool PROBS>
 __device__ void draw_from_short_list(int n, const Args& a, int64_t row, const Filters& flt,
                                      const Scale& sc, Room& rm) {
   const int tid = threadIdx.x;
@@ -695,6 +719,15 @@ __device__ void draw_from_short_list(int n, const Args& a, int64_t row, const Fi
   const uint64_t aim = flt.top_p < 1.0f ? share_aim(flt.top_p, all) : all;
   const bool keep = first && rank < k && (before < aim || rank == 0) && x >= least_logit(flt, sc.max);
   room_scan(keep ? w : 0, rm, &all);  // its barriers also end the reading of the weights
+  if constexpr (PROBS) {
+    // what is kept is a prefix of the ranking
+    const int count = __syncthreads_count(keep);
+    if (keep && rank == count - 1) {
+      rm.border = Border{x, entry_index(e)};
+      rm.total = all;
+    }
+    return;
+  }
   if (first && !keep) rm.list[r.entry] = 0;
   __syncthreads();
   const uint64_t to = draw_aim(flt.uniform, all);
@@ -705,9 +738,10 @@ __device__ void draw_from_short_list(int n, const Args& a, int64_t row, const Fi
 }
 
 // The same for any list, by sorting.
+template <bool PROBS>
 __device__ void draw_from_list(int n, const Args& a, int64_t row, const Filters& flt,
                                const Scale& sc, Room& rm) {
-  if (n <= NT) return draw_from_short_list(n, a, row, flt, sc, rm);
+  if (n <= NT) return draw_from_short_list<PROBS>(n, a, row, flt, sc, rm);
   constexpr int PER = LIST / NT;
   const int tid = threadIdx.x;
   const int size = pad_list(rm.all, n);
@@ -736,6 +770,17 @@ __device__ void draw_from_list(int n, const Args& a, int64_t row, const Filters&
   if ((tid & 31) == 0 && keep) atomicAdd(&rm.keep, keep);
   __syncthreads();
   n = rm.keep;  // what is kept is a prefix of the ranking
+  if constexpr (PROBS) {
+    mine = 0;
+#pragma unroll
+    for (int j = 0; j < PER; j++) mine += tid * PER + j < n ? w[j] : 0;
+    room_scan(mine, rm, &all);
+    if (tid == 0) {
+      rm.border = Border{entry_value(rm.all[n - 1]), entry_index(rm.all[n - 1])};
+      rm.total = all;
+    }
+    return;
+  }
   __syncthreads();
   // by index, ascending: entries (~index, logit bits), descending
   for (int i = tid; i < n; i += NT) {
@@ -1002,7 +1047,44 @@ __device__ uint64_t block_weights(const Slice<T>& s, int first, const Border& bo
   return here;
 }
 
+// The distribution of a slice: f(x, i) for every token; out: the row's output at the
+// slice's first token.  Pieces without a token that reaches `least` are zeros.
+template <typename T, typename F>
+__device__ __forceinline__ void write_slice(const Slice<T>& s, float* out, float least, F f) {
+  constexpr int N = Slice<T>::N;
+  const bool vec = (reinterpret_cast<uintptr_t>(out + s.head) & 15) == 0;
+  for (int p = threadIdx.x; p < s.pieces; p += NT) {
+    union { uint4 v; T x[N]; } u;
+    const int i = s.head + p * N;
+    u.v = *reinterpret_cast<const uint4*>(s.x + i);
+    float y[N];
+#pragma unroll
+    for (int k = 0; k < N; k++) y[k] = 0.0f;
+    if (piece_max<T>(u.v) >= least)
+#pragma unroll
+      for (int k = 0; k < N; k++) y[k] = f(to_f32<T>(u.x[k]), i + k);
+#pragma unroll
+    for (int k = 0; k < N; k += 4) {
+      if (vec) __stcs(reinterpret_cast<float4*>(out + i + k), make_float4(y[k], y[k + 1], y[k + 2], y[k + 3]));
+      else
+#pragma unroll
+        for (int j = 0; j < 4; j++) out[i + k + j] = y[k + j];
+    }
+  }
+  const int t = threadIdx.x, tail = s.head + s.pieces * N;
+  if (t < s.head) out[t] = f(to_f32<T>(s.x[t]), t);
+  else if (t >= 32 && tail + t - 32 < s.n) out[tail + t - 32] = f(to_f32<T>(s.x[tail + t - 32]), tail + t - 32);
+}
 template <typename T>
+__device__ __forceinline__ void write_shares(const Slice<T>& s, float* out, int first,
+                                             const Border& border, const Scale& sc, uint64_t total) {
+  const float inv = per_total(total);
+  write_slice(s, out, border.value, [&](float x, int i) {
+    return kept(border, x, first + i) ? share_of(x, sc, inv) : 0.0f;
+  });
+}
+
+template <typename T, bool PROBS>
 __global__ void __launch_bounds__(NT, 2) sample_cluster_kernel(const T* __restrict__ logits, Args a) {
   extern __shared__ __align__(16) uint8_t slice_smem[];
   __shared__ Room rm;
@@ -1072,8 +1154,10 @@ __global__ void __launch_bounds__(NT, 2) sample_cluster_kernel(const T* __restri
   for (unsigned b = 0; b < blocks; b++) max = fmaxf(max, cluster.map_shared_rank(&rm, b)->top);
 
   // no block leaves while another may read or write its shared memory
+  float* out = PROBS ? a.probs + row * a.probs_stride + first : nullptr;
   if (max == -INFINITY) {
-    if (rank == 0 && tid == 0) {
+    if constexpr (PROBS) write_slice(slice, out, INFINITY, [](float, int) { return 0.0f; });
+    if (!PROBS && rank == 0 && tid == 0) {
       a.ids[row] = -1;
       if (a.logprobs != nullptr) a.logprobs[row] = -INFINITY;
     }
@@ -1088,7 +1172,12 @@ __global__ void __launch_bounds__(NT, 2) sample_cluster_kernel(const T* __restri
     __syncthreads();
     if (lane == 0) rm.warp[warp] = (uint64_t)best;
     cluster.sync();
-    if (rank == 0 && warp == 0) {
+    if constexpr (PROBS) {  // every warp finds it
+      for (unsigned i = lane; i < blocks * WARPS; i += 32)
+        best = min(best, (int)cluster.map_shared_rank(&rm, i / WARPS)->warp[i % WARPS]);
+      best = __reduce_min_sync(0xffffffffu, best);
+      write_slice(slice, out, max, [&](float, int i) { return first + i == best ? 1.0f : 0.0f; });
+    } else if (rank == 0 && warp == 0) {
       for (unsigned i = lane; i < blocks * WARPS; i += 32)
         best = min(best, (int)cluster.map_shared_rank(&rm, i / WARPS)->warp[i % WARPS]);
       best = __reduce_min_sync(0xffffffffu, best);
@@ -1139,7 +1228,14 @@ __global__ void __launch_bounds__(NT, 2) sample_cluster_kernel(const T* __restri
       // only rank 0 has work left, in its own memory; it waits until the others
       // have read its count
       cluster.sync();
-      if (rank == 0) draw_from_list(n, a, row, flt, sc, rm);
+      if (rank == 0) draw_from_list<PROBS>(n, a, row, flt, sc, rm);
+      if constexpr (PROBS) {
+        cluster.sync();
+        const Border border = head->border;
+        const uint64_t total = head->total;
+        cluster.sync();  // read: rank 0 may leave
+        write_shares(slice, out, first, border, sc, total);
+      }
       return;
     }
   }
@@ -1188,7 +1284,7 @@ __global__ void __launch_bounds__(NT, 2) sample_cluster_kernel(const T* __restri
   }
   if (!good) {
     cluster.sync();  // the border is read: the others may leave
-    if (rank == 0) sample_row<T>(x, a, row, flt, sc, rm.radix);
+    if (rank == 0) sample_row<T, PROBS>(x, a, row, flt, sc, rm.radix);
     return;
   }
   const float least = least_logit(flt, sc.max);
@@ -1199,6 +1295,11 @@ __global__ void __launch_bounds__(NT, 2) sample_cluster_kernel(const T* __restri
   if (tid == 0) rm.total = here;
   cluster.sync();
   const uint64_t all = cluster_total(cluster, rm, blocks);
+  if constexpr (PROBS) {
+    cluster.sync();  // nothing of another block is read any more
+    write_shares(slice, out, first, border, sc, all);
+    return;
+  }
   uint64_t before = 0;
   for (unsigned b = 0; b < rank; b++) before += cluster.map_shared_rank(&rm, b)->total;
   cluster.sync();  // nothing of another block is read any more
@@ -1230,7 +1331,7 @@ __global__ void __launch_bounds__(NT, 2) sample_cluster_kernel(const T* __restri
 }
 
 // Vocabularies beyond the shared memory of a cluster.
-template <typename T>
+template <typename T, bool PROBS>
 __global__ void __launch_bounds__(NT) sample_kernel(const T* __restrict__ logits, Args a) {
   __shared__ Shared sm;
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, n = a.n;
@@ -1250,32 +1351,35 @@ __global__ void __launch_bounds__(NT) sample_kernel(const T* __restrict__ logits
   const uint32_t best_key = (uint32_t)(best >> 32);
   const bool none = best_key <= kKeyMinusInf;
   if (none || !(flt.temperature > 0x1p-100f)) {
-    if (tid == 0) {
+    if constexpr (PROBS) {
+      const int one = none ? -1 : (int)(0xffffffffu - (uint32_t)best);
+      for (int i = tid; i < n; i += NT) a.probs[row * a.probs_stride + i] = i == one ? 1.0f : 0.0f;
+    } else if (tid == 0) {
       a.ids[row] = none ? -1 : (int64_t)(0xffffffffu - (uint32_t)best);
       if (a.logprobs != nullptr) a.logprobs[row] = none ? -INFINITY : 0.0f;
     }
     return;
   }
-  sample_row<T>(x, a, row, flt, scale_of(value_of(best_key), flt.per), sm);
+  sample_row<T, PROBS>(x, a, row, flt, scale_of(value_of(best_key), flt.per), sm);
 }
 
 // Clusters of as few thread blocks as hold a row (two of them per SM), and of
 // up to 8 while that leaves SMs idle and a slice keeps 4,096 logits.
-template <typename T>
+template <typename T, bool PROBS>
 cudaError_t launch(const T* logits, Args a, int64_t rows, cudaStream_t stream) {
   constexpr int kSliceBytes = 96 * 1024;
   int blocks = 1;
   auto slice_of = [&](int b) { return ((a.n + b - 1) / b + 15) / 16 * 16; };
   while (blocks < 8 && (int64_t)slice_of(blocks) * (int)sizeof(T) > kSliceBytes) blocks *= 2;
   if ((int64_t)slice_of(blocks) * (int)sizeof(T) > 208 * 1024 || rows * blocks > INT32_MAX) {
-    sample_kernel<T><<<(unsigned)rows, NT, 0, stream>>>(logits, a);
+    sample_kernel<T, PROBS><<<(unsigned)rows, NT, 0, stream>>>(logits, a);
     count_launch();
     return cudaGetLastError();
   }
   while (blocks < 8 && rows * blocks * 2 <= 2 * sm_count() && slice_of(2 * blocks) >= 4096) blocks *= 2;
   a.slice = slice_of(blocks);
   const int smem = a.slice * (int)sizeof(T) + 32;
-  cudaError_t st = cudaFuncSetAttribute(sample_cluster_kernel<T>,
+  cudaError_t st = cudaFuncSetAttribute(sample_cluster_kernel<T, PROBS>,
                                         cudaFuncAttributeMaxDynamicSharedMemorySize, 209 * 1024);
   if (st != cudaSuccess) return st;
   cudaLaunchConfig_t cfg{};
@@ -1290,9 +1394,40 @@ cudaError_t launch(const T* logits, Args a, int64_t rows, cudaStream_t stream) {
   attr.val.clusterDim.z = 1;
   cfg.attrs = &attr;
   cfg.numAttrs = 1;
-  st = cudaLaunchKernelEx(&cfg, sample_cluster_kernel<T>, logits, a);
+  st = cudaLaunchKernelEx(&cfg, sample_cluster_kernel<T, PROBS>, logits, a);
   count_launch();
   return st;
+}
+
+template <bool PROBS>
+cudaError_t launch_type(uint32_t dtype, const void* logits, const Args& a, int64_t rows,
+                        cudaStream_t stream) {
+  if (dtype == ET_B200_DTYPE_F32) return launch<float, PROBS>(static_cast<const float*>(logits), a, rows, stream);
+  if (dtype == ET_B200_DTYPE_F16) return launch<__half, PROBS>(static_cast<const __half*>(logits), a, rows, stream);
+  return launch<__nv_bfloat16, PROBS>(static_cast<const __nv_bfloat16*>(logits), a, rows, stream);
+}
+
+// What both entry points check of their shape and its filters.
+int32_t check_shape(const et_b200_sampling_v1* s, et_kernel_error* e, const char* op) {
+  if (s == nullptr || s->struct_size < sizeof(et_b200_sampling_v1))
+    return set_error(e, ET_KERNEL_ERROR_VERSION_MISMATCH, ET_KERNEL_CODE_INVALID_STRUCT_SIZE, op,
+                     "sampling descriptor is missing or truncated");
+  if (s->dtype > ET_B200_DTYPE_BF16)
+    return set_error(e, ET_KERNEL_ERROR_DTYPE_MISMATCH, ET_KERNEL_CODE_INVALID_ENUM, op,
+                     "unknown element type of the logits");
+  if (s->rows < 0 || s->rows > INT32_MAX || s->vocabulary < 1 || s->vocabulary > (1 << 22) ||
+      s->row_stride < s->vocabulary || s->row_stride > (int64_t)1 << 31)
+    return set_error(e, ET_KERNEL_ERROR_SHAPE_MISMATCH, ET_KERNEL_CODE_INVALID_SHAPE, op,
+                     "rows, vocabulary or row stride are outside their limits");
+  return 0;
+}
+int32_t check_rows(const et_b200_sampling_v1* s, const void* logits, et_kernel_error* e,
+                   const char* op) {
+  if (!paged::aligned_to(s->dtype == ET_B200_DTYPE_F32 ? 4 : 2, logits) ||
+      !paged::aligned_to(8, s->top_k) || !paged::aligned_to(4, s->temperature, s->top_p, s->min_p))
+    return set_error(e, ET_KERNEL_ERROR_INVALID_ARGUMENT, ET_KERNEL_CODE_INVALID_BUFFER, op,
+                     "logits and the rows' values must be aligned to their elements");
+  return 0;
 }
 
 }  // namespace
@@ -1304,36 +1439,45 @@ extern "C" int32_t et_b200_sample_v1(const et_b200_sampling_v1* s, const void* l
                                      const float* uniform, int64_t* ids, float* logprobs,
                                      void* stream, et_kernel_error* e) {
   const char* op = "sample";
-  if (s == nullptr || s->struct_size < sizeof(et_b200_sampling_v1))
-    return set_error(e, ET_KERNEL_ERROR_VERSION_MISMATCH, ET_KERNEL_CODE_INVALID_STRUCT_SIZE, op,
-                     "sampling descriptor is missing or truncated");
-  if (s->dtype > ET_B200_DTYPE_BF16)
-    return set_error(e, ET_KERNEL_ERROR_DTYPE_MISMATCH, ET_KERNEL_CODE_INVALID_ENUM, op,
-                     "unknown element type of the logits");
-  if (s->rows < 0 || s->rows > INT32_MAX || s->vocabulary < 1 || s->vocabulary > (1 << 22) ||
-      s->row_stride < s->vocabulary || s->row_stride > (int64_t)1 << 31)
-    return set_error(e, ET_KERNEL_ERROR_SHAPE_MISMATCH, ET_KERNEL_CODE_INVALID_SHAPE, op,
-                     "rows, vocabulary or row stride are outside their limits");
+  if (int32_t r = check_shape(s, e, op)) return r;
   if (s->rows > 0) {
     if (logits == nullptr || uniform == nullptr || ids == nullptr)
       return set_error(e, ET_KERNEL_ERROR_INVALID_ARGUMENT, ET_KERNEL_CODE_NULL_ARGUMENT, op,
                        "logits, uniform numbers and ids are required");
-    const uintptr_t size = s->dtype == ET_B200_DTYPE_F32 ? 4 : 2;
-    using paged::aligned_to;
-    if (!aligned_to(size, logits) || !aligned_to(8, ids, s->top_k) ||
-        !aligned_to(4, uniform, logprobs, s->temperature, s->top_p, s->min_p))
+    if (int32_t r = check_rows(s, logits, e, op)) return r;
+    if (!paged::aligned_to(8, ids) || !paged::aligned_to(4, uniform, logprobs))
       return set_error(e, ET_KERNEL_ERROR_INVALID_ARGUMENT, ET_KERNEL_CODE_INVALID_BUFFER, op,
                        "logits and the rows' values must be aligned to their elements");
-    auto st = static_cast<cudaStream_t>(stream);
-    const Args a{uniform, s->temperature, s->top_k, s->top_p, s->min_p, ids, logprobs,
-                 s->row_stride, (int)s->vocabulary, 0};
-    cudaError_t status;
-    if (s->dtype == ET_B200_DTYPE_F32)
-      status = launch(static_cast<const float*>(logits), a, s->rows, st);
-    else if (s->dtype == ET_B200_DTYPE_F16)
-      status = launch(static_cast<const __half*>(logits), a, s->rows, st);
-    else
-      status = launch(static_cast<const __nv_bfloat16*>(logits), a, s->rows, st);
+    const Args a{uniform, s->temperature, s->top_k, s->top_p, s->min_p, ids, logprobs, nullptr,
+                 s->row_stride, 0, (int)s->vocabulary, 0};
+    const cudaError_t status =
+        launch_type<false>(s->dtype, logits, a, s->rows, static_cast<cudaStream_t>(stream));
+    if (status != cudaSuccess) return cuda_error(e, status, op);
+  }
+  if (e) memset(e, 0, sizeof(*e));
+  return 0;
+}
+
+extern "C" int32_t et_b200_probabilities_v1(const et_b200_sampling_v1* s, const void* logits,
+                                            float* probs, int64_t probs_stride, void* stream,
+                                            et_kernel_error* e) {
+  const char* op = "probabilities";
+  if (int32_t r = check_shape(s, e, op)) return r;
+  if (probs_stride < s->vocabulary || probs_stride > (int64_t)1 << 31)
+    return set_error(e, ET_KERNEL_ERROR_SHAPE_MISMATCH, ET_KERNEL_CODE_INVALID_SHAPE, op,
+                     "the probabilities' row stride is outside its limits");
+  if (s->rows > 0) {
+    if (logits == nullptr || probs == nullptr)
+      return set_error(e, ET_KERNEL_ERROR_INVALID_ARGUMENT, ET_KERNEL_CODE_NULL_ARGUMENT, op,
+                       "logits and probabilities are required");
+    if (int32_t r = check_rows(s, logits, e, op)) return r;
+    if (!paged::aligned_to(4, probs))
+      return set_error(e, ET_KERNEL_ERROR_INVALID_ARGUMENT, ET_KERNEL_CODE_INVALID_BUFFER, op,
+                       "probabilities must be aligned to their elements");
+    const Args a{nullptr, s->temperature, s->top_k, s->top_p, s->min_p, nullptr, nullptr, probs,
+                 s->row_stride, probs_stride, (int)s->vocabulary, 0};
+    const cudaError_t status =
+        launch_type<true>(s->dtype, logits, a, s->rows, static_cast<cudaStream_t>(stream));
     if (status != cudaSuccess) return cuda_error(e, status, op);
   }
   if (e) memset(e, 0, sizeof(*e));

@@ -1,7 +1,9 @@
 """Paged KV cache on torch CUDA tensors: appending (et_b200_paged_append_v1)
-and attention of new tokens over it (et_b200_paged_attention_v1).
+and attention of new tokens over it (et_b200_paged_attention_v1); the same over a
+cache of 8 bits an element (et_b200_paged_append8_v1, et_b200_paged_attention8_v1).
 
     cache = PagedCache(keys, values)             # one layer's pools
+    # or PagedCache8(keys, values, key_scales, value_scales, dtype)
     batch = PagedBatch(offsets, lengths, table, tokens, max_new, max_length)
     cache.append(batch, k, v, rope=(cos, sin))
     attention = PagedAttention(cache, q_heads)
@@ -38,6 +40,17 @@ class CacheDescriptor(C.Structure):
                 ("pages", C.c_int64), ("page_size", C.c_int64), ("kv_heads", C.c_int64),
                 ("head_dim", C.c_int64), ("page_stride", C.c_int64), ("head_stride", C.c_int64),
                 ("token_stride", C.c_int64), ("dtype", C.c_uint32), ("reserved", C.c_uint32)]
+
+
+class Cache8Descriptor(C.Structure):
+    """et_b200_paged_cache8_v1"""
+    _fields_ = [("struct_size", C.c_size_t), ("keys", C.c_void_p), ("values", C.c_void_p),
+                ("key_scales", C.c_void_p), ("value_scales", C.c_void_p),
+                ("pages", C.c_int64), ("page_size", C.c_int64), ("kv_heads", C.c_int64),
+                ("head_dim", C.c_int64), ("page_stride", C.c_int64), ("head_stride", C.c_int64),
+                ("token_stride", C.c_int64), ("scale_page_stride", C.c_int64),
+                ("scale_head_stride", C.c_int64), ("scale_token_stride", C.c_int64),
+                ("dtype", C.c_uint32), ("reserved", C.c_uint32)]
 
 
 class BatchDescriptor(C.Structure):
@@ -108,14 +121,59 @@ class PagedCache:
     def append(self, batch: "PagedBatch", k, v, rope=None, stream: int | None = None) -> None:
         """Stores k (rotated by rope = (cos, sin), [positions, head_dim / 2]
         each) and v, [tokens, kv_heads, head_dim] with dense heads."""
-        err = k1.KernelError()
-        k_stride = _rows(k, batch, self, self.kv_heads, "k")
-        v_stride = _rows(v, batch, self, self.kv_heads, "v")
-        rc = self.lib.et_b200_paged_append_v1(
-            self._ref, batch.bind(self), batch.rope(rope, self), k.data_ptr(), k_stride,
-            v.data_ptr(), v_stride, stream_of(stream, self.index), C.byref(err))
-        if rc != 0:
-            _check(rc, err)
+        _append(self.lib.et_b200_paged_append_v1, self, batch, k, v, rope, stream)
+
+
+def _append(call, cache, batch: "PagedBatch", k, v, rope, stream) -> None:
+    err = k1.KernelError()
+    k_stride = _rows(k, batch, cache, cache.kv_heads, "k")
+    v_stride = _rows(v, batch, cache, cache.kv_heads, "v")
+    rc = call(cache._ref, batch.bind(cache), batch.rope(rope, cache), k.data_ptr(), k_stride,
+              v.data_ptr(), v_stride, stream_of(stream, cache.index), C.byref(err))
+    if rc != 0:
+        _check(rc, err)
+
+
+class PagedCache8:
+    """One layer's pools of pages in 8 bits: keys and values torch tensors [pages,
+    kv_heads, page_size, head_dim] (float8_e4m3fn, or uint8 that holds its bytes) with
+    a dense last dimension and strides of whole 16-byte pieces, the same for both;
+    key_scales and value_scales f32 [pages, kv_heads, page_size], of any strides, the
+    same for both.  A cached row stands for its elements times its scale.  dtype (f32,
+    f16 or bf16) is that of k, v, q and o.  append and PagedAttention are used as with
+    a PagedCache; dense scales of neighbouring slots take the faster kernels."""
+
+    def __init__(self, keys, values, key_scales, value_scales, dtype):
+        tensors = (keys, values, key_scales, value_scales)
+        _need(all(t.is_cuda and t.device == keys.device for t in tensors),
+              "the pools and scales must be CUDA tensors of one device")
+        _need(keys.dim() == 4 and keys.shape == values.shape and keys.dtype == values.dtype,
+              "the pools must be [pages, kv_heads, page_size, head_dim] tensors of one type")
+        _need(keys.dtype in (torch.float8_e4m3fn, torch.uint8), "the pools must be float8_e4m3fn or uint8")
+        _need(key_scales.shape == keys.shape[:3] and value_scales.shape == keys.shape[:3] and
+              key_scales.dtype == torch.float32 and value_scales.dtype == torch.float32,
+              "the scales must be f32 [pages, kv_heads, page_size]")
+        _need(dtype in DTYPES, "the tensors beside the cache must be f32, f16 or bf16")
+        _need(keys.numel() > 0, "the pools are empty")
+        strides = [PagedCache._strides(t) for t in tensors[:2]]
+        scale_strides = [PagedCache._strides(t[..., None]) for t in tensors[2:]]
+        _need(strides[0] == strides[1] and scale_strides[0] == scale_strides[1],
+              "both pools must have the same strides, both scales too")
+        self.lib = load()
+        self.keys, self.values, self.key_scales, self.value_scales = tensors
+        self.device, self.index, self.dtype = keys.device, keys.get_device(), dtype
+        self.pages, self.kv_heads, self.page_size, self.head_dim = keys.shape
+        self.descriptor = Cache8Descriptor(
+            C.sizeof(Cache8Descriptor), keys.data_ptr(), values.data_ptr(), key_scales.data_ptr(),
+            value_scales.data_ptr(), self.pages, self.page_size, self.kv_heads, self.head_dim,
+            *strides[0], *scale_strides[0], DTYPES[dtype], 0)
+        self._ref = C.byref(self.descriptor)
+
+    def append(self, batch: "PagedBatch", k, v, rope=None, stream: int | None = None) -> None:
+        """Stores k (rotated by rope = (cos, sin), [positions, head_dim / 2]
+        each) and v, [tokens, kv_heads, head_dim] with dense heads, with the scales of
+        their rows."""
+        _append(self.lib.et_b200_paged_append8_v1, self, batch, k, v, rope, stream)
 
 
 class PagedBatch:
@@ -189,14 +247,20 @@ def _rows(t, batch: PagedBatch, cache: PagedCache, heads: int, name: str) -> int
 
 
 class PagedAttention:
-    """Attention of query heads over a paged cache, with its workspace (one
-    call at a time: objects whose calls may overlap need their own)."""
+    """Attention of query heads over a paged cache (PagedCache or PagedCache8), with
+    its workspace (one call at a time: objects whose calls may overlap need their
+    own)."""
 
-    def __init__(self, cache: PagedCache, q_heads: int):
+    def __init__(self, cache: PagedCache | PagedCache8, q_heads: int):
         self.lib = load()
         self.cache, self.q_heads = cache, q_heads
+        eight = isinstance(cache, PagedCache8)
+        self.call = (self.lib.et_b200_paged_attention8_v1 if eight else
+                     self.lib.et_b200_paged_attention_v1)
+        size = (self.lib.et_b200_paged_attention8_workspace_bytes_v1 if eight else
+                self.lib.et_b200_paged_attention_workspace_bytes_v1)
         with torch.cuda.device(cache.device):
-            self.ws_bytes = self.lib.et_b200_paged_attention_workspace_bytes_v1(cache._ref, q_heads)
+            self.ws_bytes = size(cache._ref, q_heads)
         _need(self.ws_bytes > 0, "paged attention shape rejected")
         self.ws = torch.empty(self.ws_bytes + 256, dtype=torch.uint8, device=cache.device)
         self.ws_ptr = (self.ws.data_ptr() + 255) & ~255
@@ -213,7 +277,7 @@ class PagedAttention:
             _need(lse.shape == (batch.tokens, self.q_heads) and lse.dtype == torch.float32 and
                   lse.is_contiguous() and lse.device == cache.device,
                   "lse must be dense f32 [tokens, q_heads] on the cache's device")
-        _check(self.lib.et_b200_paged_attention_v1(
+        _check(self.call(
             cache._ref, batch.bind(cache), batch.rope(rope, cache), self.q_heads, q.data_ptr(),
             q_stride, o.data_ptr(), o_stride, lse.data_ptr() if lse is not None else None,
             self.ws_ptr, self.ws_bytes, stream_of(stream, cache.index), C.byref(err)), err)

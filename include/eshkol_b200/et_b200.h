@@ -260,6 +260,59 @@ int32_t et_b200_paged_attention_v1(const et_b200_paged_cache_v1 *cache,
                                    size_t workspace_bytes, void *stream,
                                    et_kernel_error *error);
 
+/* A paged cache of 8 bits: as et_b200_paged_cache_v1, but an element is a byte of
+ * type e4m3 (sign, 4 bits of exponent, 3 of fraction, largest 448; strides count
+ * bytes and are multiples of 16, head_dim a multiple of 16 up to 256), and each
+ * row of head_dim elements stands for its values times one f32 scale, at page *
+ * scale_page_stride + head * scale_head_stride + slot * scale_token_stride of the
+ * scale pools (in floats).  dtype is that of k, v, q and o.  A cached token and
+ * head takes head_dim + 4 bytes of keys and as many of values. */
+typedef struct et_b200_paged_cache8_v1 {
+  size_t struct_size;
+  void *keys;
+  void *values;
+  float *key_scales;
+  float *value_scales;
+  int64_t pages, page_size, kv_heads, head_dim;
+  int64_t page_stride, head_stride, token_stride;
+  int64_t scale_page_stride, scale_head_stride, scale_token_stride;
+  uint32_t dtype; /* ET_B200_DTYPE_*, of k, v, q and o */
+  uint32_t reserved;
+} et_b200_paged_cache8_v1;
+
+/* et_b200_paged_append_v1 into a cache of 8 bits: of each row x (a token's head; of
+ * the keys rotated in f32) the scale s is the least power of two with |x| <= 448 s
+ * for every element (no less than 2^-126; 0 for a row of zeros), and the stored
+ * elements are x / s rounded to the nearest, ties to even.  A row that holds an
+ * infinity or a NaN gets the scale NaN, which the attention hands on to every query
+ * that sees the row. */
+int32_t et_b200_paged_append8_v1(const et_b200_paged_cache8_v1 *cache,
+                                 const et_b200_paged_batch_v1 *batch,
+                                 const et_b200_paged_rope_v1 *rope,
+                                 const void *k, int64_t k_stride, const void *v,
+                                 int64_t v_stride, void *stream,
+                                 et_kernel_error *error);
+
+/* et_b200_paged_attention_v1 over a cache of 8 bits.  Elements and products with
+ * scales that are powers of two (or 0), as the append writes them, are exact;
+ * other finite scales round rows to 11 bits where a chunk of f16 or bf16 queries is
+ * computed (more than 16 query rows per kv head).  q' is carried as binary16 of a
+ * scale per row: at f32 and, up to 16 rows, at f16 with its residual (about 22
+ * bits); the probabilities as binary16, at f32 with their residual.  Above 16 rows
+ * at f16 and bf16, rows of a block of 128 keys (of the keys), or behind the
+ * largest so far (of the values), whose scale is less than 2^-21 of the largest
+ * one's lose bits. */
+size_t et_b200_paged_attention8_workspace_bytes_v1(
+    const et_b200_paged_cache8_v1 *cache, int64_t q_heads);
+int32_t et_b200_paged_attention8_v1(const et_b200_paged_cache8_v1 *cache,
+                                    const et_b200_paged_batch_v1 *batch,
+                                    const et_b200_paged_rope_v1 *rope,
+                                    int64_t q_heads, const void *q,
+                                    int64_t q_stride, void *o, int64_t o_stride,
+                                    float *lse, void *workspace,
+                                    size_t workspace_bytes, void *stream,
+                                    et_kernel_error *error);
+
 /* Draws one token per row of logits [rows, vocabulary] (row_stride elements
  * apart) by inversion: with the weights w = exp((x - max x) / temperature) of
  * the tokens that the filters keep, ids[r] is the first token, in vocabulary
@@ -291,6 +344,56 @@ typedef struct et_b200_sampling_v1 {
 int32_t et_b200_sample_v1(const et_b200_sampling_v1 *shape, const void *logits,
                           const float *uniform, int64_t *ids, float *logprobs,
                           void *stream, et_kernel_error *error);
+
+/* The distribution that et_b200_sample_v1 draws from, with the same shape and
+ * filters: probs (f32 [rows, vocabulary], rows probs_stride floats apart) receives
+ * w / total of every token that the filters keep and 0 for all others.  Weights
+ * below 2^-36 of the likeliest count as 0, as there; others are f32 (not fixed
+ * point), so probabilities are right to some 2^-22 of themselves however small.  A
+ * row that takes the most likely token gets a single 1, a row without a token to
+ * draw only zeros. */
+int32_t et_b200_probabilities_v1(const et_b200_sampling_v1 *shape,
+                                 const void *logits, float *probs,
+                                 int64_t probs_stride, void *stream,
+                                 et_kernel_error *error);
+
+/* Verification of drafted tokens (speculative decoding).  Request b's rows
+ * offsets[b] .. offsets[b + 1] - 1 are the positions that one pass of the target
+ * model gave: its last accepted token and the tokens drafted behind it, so row r
+ * holds the target's distribution p_r (target [tokens, vocabulary], f32) of the
+ * token that drafts[r] proposes; the last row of a request has no proposal
+ * (drafts[r] is not read there).  draft (f32, rows as in target, or NULL) holds the
+ * distributions q_r that the drafts were drawn from; NULL means drafts made without
+ * chance (q_r is 1 at drafts[r]).  In order, a proposal x is accepted if
+ * accept_uniform[r] q_r(x) < p_r(x); at the first that is not, the request's token
+ * is drawn from max(p_r - q_r, 0), and behind its last accepted proposal from p_r of
+ * the last row: the first token, in vocabulary order, whose running sum exceeds
+ * draw_uniform[b] times the total.  Products, differences and sums are formed in 64
+ * bits, in an order that depends on the vocabulary alone.  ids[r] receives the
+ * accepted proposals, then the drawn token, then -1; accepted[b] the number of
+ * accepted proposals (0 for a request without rows).
+ * Probabilities count as 0 where they are NaN or negative and as 1 above 1;
+ * accept_uniform is meant in [0, 1) (a NaN accepts nothing), draw_uniform too
+ * (other values act as the nearest end).  A proposal outside the vocabulary is
+ * not accepted, and its q_r counts as 0 everywhere.  Where max(p - q, 0) is 0
+ * everywhere the token is drawn from p; where that is too, it is -1.  Rows of no
+ * request are not written.  offsets that fall or leave the tensors are clamped and
+ * ET_B200_PAGED_BAD_OFFSET is recorded in *status.  Device memory throughout, read
+ * when the kernel runs. */
+typedef struct et_b200_verification_v1 {
+  size_t struct_size;
+  int64_t batch, tokens, vocabulary;
+  int64_t target_stride, draft_stride; /* floats between rows */
+  const int64_t *offsets;              /* [batch + 1], ascending from 0 */
+  const int64_t *drafts;               /* [tokens] */
+  const float *accept_uniform;         /* [tokens] */
+  const float *draw_uniform;           /* [batch] */
+  int32_t *status;                     /* one word, or NULL */
+} et_b200_verification_v1;
+int32_t et_b200_verify_v1(const et_b200_verification_v1 *shape,
+                          const float *target, const float *draft, int64_t *ids,
+                          int64_t *accepted, void *stream,
+                          et_kernel_error *error);
 
 /* ------------------------------------------------------------ synthetic data
  * Seeded inputs shared with the tests: value i of (seed, stream) is a pure
