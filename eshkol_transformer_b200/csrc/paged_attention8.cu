@@ -75,13 +75,6 @@ struct Shape8 {
   }
 };
 
-// 2^e of a row of queries: the largest magnitude times it lies in [2^14, 2^15) (1 for
-// rows of zeros and rows that are not finite).
-__device__ __forceinline__ int query_exponent(float top) {
-  const int b = (int)(__float_as_uint(top) >> 23);
-  return b == 255 || top == 0.0f ? 0 : min(141 - b, 126);
-}
-
 template <typename T, typename S, bool TMA>
 __global__ void __launch_bounds__(S::NT + (TMA ? 32 : 0), S::PER_SM)
 paged_attention8_kernel(const __grid_constant__ CUtensorMap k_map,
@@ -725,6 +718,8 @@ int launch_dim8(const et_b200_paged_cache8_v1* c, Attend8Args& x, bool few, void
 template <typename T>
 int launch_type8(const et_b200_paged_cache8_v1* c, Attend8Args& x, bool few, void* ws,
                  cudaStream_t stream) {
+  if (!few && sizeof(T) == 2)
+    if (const int blocks = attend8_tc(c, x, ws, stream)) return blocks;
   switch (padded8(c->head_dim)) {
     case 64: return launch_dim8<T, 64>(c, x, few, ws, stream);
     case 128: return launch_dim8<T, 128>(c, x, few, ws, stream);

@@ -1,0 +1,667 @@
+// Attention of chunks of new tokens over an 8-bit paged cache on tcgen05: f16 / bf16
+// queries, head_dim up to 128, pages of a power of two of at least 8 slots.
+//
+// The mathematics are those of paged_attention8.cu, tiles and roles those of
+// paged_attention_tc.cu (256 rows as two halves, blocks of 128 keys, a warpgroup of
+// probabilities and a product warp a half), with four more warps that turn each
+// block's bytes into the binary16 tiles that the products read.  They also apply the
+// scales, so the probabilities' loop knows nothing of them: rows of K times 2^(6 - E)
+// with E the largest exponent of the block's scales, a constant of the block's scores;
+// rows of V times 2^(6 - F) with F the largest exponent of the tile's blocks so far, by
+// whose growth O is rescaled together with a new maximum.  With scales that are
+// powers of two that is exact down to 2^-21 of the largest (binary16 holds 2^-24 to
+// 2^15, an element 2^-9 to 448); other scales round each element to 11 bits.
+// Queries are binary16 times 2^-e of their row, weights binary16 times 2^11 below a
+// standing maximum that allows 2^4: 11 bits, more than a bf16 result keeps.
+// Waits are bounded; one that runs out raises a CTA-wide abort, copies and
+// products in flight are waited for and TMEM is released.
+#include <math.h>
+
+#include <type_traits>
+
+#include "attention_f16.cuh"
+#include "paged8.cuh"
+#include "paged_mma.cuh"
+
+namespace etb {
+namespace {
+
+using namespace paged;
+using namespace f16att;
+
+constexpr int HALF = 128, BK = 128;
+// warps 0-7 probabilities; 8, 9 products, 10 copies; 12-15 conversion.  Registers of
+// the warpgroups out of 512 x 128.
+constexpr int MMA_WARP = 8, LOAD_WARP = 10, CONVERT_WARP = 12, THREADS = 512;
+constexpr int kWideRegs = 208, kLeanRegs = 40, kConvertRegs = 56;
+static_assert(256 * kWideRegs + 128 * (kLeanRegs + kConvertRegs) <= THREADS * 128, "registers at launch");
+constexpr float kJump = 4.0f, kShift = 11.0f;  // weights reach 2^15
+constexpr int RING = 8;  // blocks whose exponents are kept: more than conversion runs ahead
+constexpr int kNone = -1000;  // the exponent of no scale
+
+template <int DH>
+struct Layout {
+  static constexpr int SLOT = BK * DH * 2;  // one block of K or V in binary16
+  static constexpr int SLOTS = DH == 128 ? 3 : 6;
+  static constexpr int RAW = BK * DH;       // one block of K or V in bytes
+  static constexpr int RAWS = DH == 128 ? 2 : 4;
+  static constexpr int Q = SLOTS * SLOT;    // two halves of 128 rows
+  static constexpr int BYTES = Q + 2 * HALF * DH * 2;
+  static constexpr int SCALES = BYTES + RAWS * 2 * RAW;  // [RAWS][keys, values][BK]
+  static constexpr int BARS = SCALES + RAWS * 2 * BK * 4;
+  static constexpr int SMEM = BARS + 512;
+  // TMEM: scores of the halves (P over the first 64 columns), outputs
+  static constexpr uint32_t S0 = 0, O0 = 256, COLS = 512;
+  static_assert(O0 + 2 * DH <= COLS && SMEM <= 232448, "TMEM and shared memory");
+};
+
+// Whether `v` holds for all `threads` threads of a named barrier.
+__device__ __forceinline__ bool named_all(int id, int threads, bool v) {
+  uint32_t all;
+  asm volatile(
+      "{\n\t.reg .pred p, q;\n\t"
+      "setp.ne.u32 q, %3, 0;\n\t"
+      "bar.red.and.pred p, %1, %2, q;\n\t"
+      "selp.u32 %0, 1, 0, p;\n\t}\n"
+      : "=r"(all)
+      : "r"(id), "r"(threads), "r"((uint32_t)v)
+      : "memory");
+  return all != 0;
+}
+
+// x 2^e in two steps, e from -252 to 252
+__device__ __forceinline__ float times_power(float x, int e) {
+  const int h = e / 2;
+  return x * exp2_int(h) * exp2_int(e - h);
+}
+
+template <typename T, int DH>
+__global__ void __launch_bounds__(THREADS, 1)
+paged_attention8_tc_kernel(const __grid_constant__ CUtensorMap k_map,
+                           const __grid_constant__ CUtensorMap v_map, Attend8Args args, int box_rows) {
+  using L = Layout<DH>;
+  constexpr int SLOTS = L::SLOTS, RAWS = L::RAWS;
+  const AttendArgs& a = args.a;
+  extern __shared__ __align__(1024) uint8_t smem[];
+  float* scales_s = reinterpret_cast<float*>(smem + L::SCALES);
+  uint64_t* bars = reinterpret_cast<uint64_t*>(smem + L::BARS);
+  enum { FULL = 0, EMPTY = FULL + SLOTS, RAWFULL = EMPTY + SLOTS, RAWEMPTY = RAWFULL + RAWS,
+         SFULL = RAWEMPTY + RAWS, PREADY = SFULL + 2, QREADY = PREADY + 2, ODONE = QREADY + 2,
+         DRAIN = ODONE + 2, TURN = DRAIN + 2, EXPS = TURN + 2, NBARS = EXPS + RING };
+  const uint32_t bar0 = smem_u32(bars);
+  auto B_ = [&](int i) { return bar0 + 8u * (uint32_t)i; };
+  int* exps = reinterpret_cast<int*>(bars + NBARS);  // [RING][E, F]
+  int* found = exps + 2 * RING;                      // [E, F][4 warps]
+  uint32_t* tslot = reinterpret_cast<uint32_t*>(found + 8);
+  int* abort_word = reinterpret_cast<int*>(tslot + 1);
+  static_assert(NBARS * 8 + (2 * RING + 8 + 2) * 4 <= 512, "room behind the tiles");
+  volatile int* abort = abort_word;
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  const uint32_t base = smem_u32(smem);
+  const int group = a.tiling.group, dim = a.pools.head_dim;
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+
+  if (tid == 0) {
+    for (int i = 0; i < NBARS; i++)
+      mbar_init(B_(i), i < EMPTY                       ? 128
+                       : i < RAWFULL                   ? 2
+                       : i >= RAWEMPTY && i < SFULL    ? 4
+                       : i >= PREADY && i < ODONE      ? HALF
+                                                       : 1);
+    *abort = 0;
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+  }
+  if (warp == MMA_WARP) tmem_alloc(smem_u32(tslot), L::COLS);
+  Place p;
+  // the rows of Q are written behind the barrier below
+  const Share share = divide(a.tiling, a.batch, a.least, p,
+                             *reinterpret_cast<DivideRoom<THREADS>*>(smem + L::Q));
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = *tslot;
+  // blocks of the tile at p that fall into this share, and its rows
+  int64_t left = share.units;
+  auto blocks_here = [&]() { return (int)min((int64_t)(p.nblk - p.blk), left); };
+  auto rows_here = [&]() {
+    return min(2 * HALF, p.r.n * group - p.tile * 2 * HALF);
+  };
+  auto next_tile = [&](int done) {
+    left -= done;
+    p.blk += done - 1;
+    advance(a.tiling, a.batch, p);
+  };
+  auto wait = [&](int i, uint32_t parity) {
+    return role_wait(B_(i), parity & 1u, abort_word, abort);
+  };
+
+  if (warp >= CONVERT_WARP) {
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kConvertRegs));
+    // ---- bytes into binary16, rows times their scales
+    const int c = tid - 32 * CONVERT_WARP;  // this thread's key of a block's scales
+    uint32_t n = 0;
+    // a wait of one warp that runs out ends the four together, at their next barrier
+    bool ok = true, live = true;
+    while (live && left > 0) {
+      const int nb = blocks_here(), visible = tile_visible(a.tiling, p.r, p.tile);
+      int high = kNone;  // F
+      for (int j = 0; j < nb; j++, n++) {
+        const uint32_t st = n % RAWS;
+        if (ok) ok = __all_sync(0xffffffffu, wait(RAWFULL + st, n / RAWS));
+        const int valid = visible - (p.blk + j) * BK;
+        uint32_t* factors = reinterpret_cast<uint32_t*>(scales_s + st * 2 * BK);
+        int e[2];
+        float s[2];
+#pragma unroll
+        for (int i = 0; i < 2; i++) {
+          s[i] = c < valid ? __uint_as_float(factors[i * BK + c]) : 0.0f;
+          const int x = (int)(__float_as_uint(s[i]) >> 23) & 255;
+          e[i] = s[i] == 0.0f ? kNone : min(max(x, 1) - 127, 126);
+          const int top = __reduce_max_sync(0xffffffffu, e[i]);
+          if (lane == 0) found[4 * i + (warp & 3)] = top;
+        }
+        live = named_all(1, 128, ok);
+        if (!live) break;
+#pragma unroll
+        for (int i = 0; i < 2; i++) e[i] = max(max(found[4 * i], found[4 * i + 1]), max(found[4 * i + 2], found[4 * i + 3]));
+        if (e[0] == kNone) e[0] = 0;
+        high = max(high, e[1]);
+        e[1] = high == kNone ? 0 : high;
+        // in place of the scales: their products, as pairs of binary16
+#pragma unroll
+        for (int i = 0; i < 2; i++) {
+          const __half2 f = __float2half2_rn(s[i] * exp2_int(-e[i]) * 64.0f);
+          factors[i * BK + c] = *reinterpret_cast<const uint32_t*>(&f);
+        }
+        if (c == 0) {
+          exps[2 * (n % RING)] = e[0];
+          exps[2 * (n % RING) + 1] = e[1];
+          mbar_arrive(B_(EXPS + n % RING));
+        }
+        named_sync(1, 128);
+#pragma unroll 1
+        for (int kv = 0; kv < 2; kv++) {
+          const uint32_t count = 2 * n + kv, slot = count % SLOTS, round = count / SLOTS;
+          if (round > 0) ok = __all_sync(0xffffffffu, wait(EMPTY + slot, round - 1));
+          if (!ok) break;  // live until the next barrier
+          // a thread takes a 16-byte piece of every fourth (second) row
+          constexpr int P = DH / 16, STEP = 128 / P, UNROLL = 4;
+          const int piece = c % P;
+          const uint32_t raw = base + L::BYTES + (st * 2 + kv) * L::RAW;
+          const uint32_t to = base + slot * L::SLOT + (uint32_t)(piece / 4) * BK * 128u;
+          // lanes of one row that write the same banks take their halves in turn
+          const int turn = piece / 4 & 1;
+#pragma unroll 1
+          for (int r0 = c / P; r0 < BK; r0 += STEP * UNROLL) {
+            float4 x[UNROLL];
+            uint32_t f[UNROLL];
+#pragma unroll
+            for (int i = 0; i < UNROLL; i++) {
+              const int r = r0 + i * STEP;
+              const uint32_t swizzled = DH == 128 ? (uint32_t)(piece ^ (r & 7)) : (uint32_t)(piece ^ ((r >> 1) & 3));
+              x[i] = lds128(raw + (uint32_t)r * DH + (swizzled << 4));
+              f[i] = factors[kv * BK + r];
+            }
+#pragma unroll
+            for (int i = 0; i < UNROLL; i++) {
+              const int r = r0 + i * STEP;
+              uint32_t h[8];
+              halves_of(__float_as_uint(x[i].x), h[0], h[1]);
+              halves_of(__float_as_uint(x[i].y), h[2], h[3]);
+              halves_of(__float_as_uint(x[i].z), h[4], h[5]);
+              halves_of(__float_as_uint(x[i].w), h[6], h[7]);
+#pragma unroll
+              for (int k = 0; k < 8; k++) {
+                asm("mul.rn.f16x2 %0, %0, %1;" : "+r"(h[k]) : "r"(f[i]));
+                if (r >= valid) h[k] = 0;  // slots behind the keys may hold anything
+              }
+              const float4 lower = make_float4(__uint_as_float(h[0]), __uint_as_float(h[1]),
+                                               __uint_as_float(h[2]), __uint_as_float(h[3]));
+              const float4 upper = make_float4(__uint_as_float(h[4]), __uint_as_float(h[5]),
+                                               __uint_as_float(h[6]), __uint_as_float(h[7]));
+              const uint32_t row = to + (uint32_t)r * 128u, at = (uint32_t)(2 * (piece & 3));
+              sts128(row + (((at + turn) ^ (uint32_t)(r & 7)) << 4), turn ? upper : lower);
+              sts128(row + (((at + 1 - turn) ^ (uint32_t)(r & 7)) << 4), turn ? lower : upper);
+            }
+          }
+          fence_async_smem();
+          mbar_arrive(B_(FULL + slot));
+        }
+        __syncwarp();
+        if (ok && lane == 0) mbar_arrive(B_(RAWEMPTY + st));
+      }
+      next_tile(nb);
+    }
+  } else if (warp >= MMA_WARP) {
+  asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kLeanRegs));
+  if (warp == LOAD_WARP) {
+    // ---- bytes and scales of K and V, page by page: lanes 0 to 15 K, the others V
+    uint32_t n = 0;
+    bool ok = true;
+    while (ok && left > 0) {
+      const int nb = blocks_here(), visible = tile_visible(a.tiling, p.r, p.tile);
+      for (int j = 0; j < nb; j++) {
+        const int key0 = (p.blk + j) * BK;
+        const int boxes = max(0, (min(visible - key0, BK) + box_rows - 1) / box_rows);
+        // each lane looks up the box it will load (at most 16 pages of 8 keys)
+        const int mine = lane % 16, v = lane / 16;
+        int page = -1, slot = 0;
+        if (mine < boxes) {
+          const int key = key0 + mine * box_rows, column = quotient(key, a.pools.by_page);
+          slot = key - column * a.pools.page_size;
+          page = a.batch.table[(int64_t)p.b * a.batch.columns + column];
+          if (page < 0 || page >= a.pools.pages) {
+            report(a.batch.status, ET_B200_PAGED_BAD_PAGE);
+            page = -1;  // outside the map: filled with zeros
+          }
+        }
+        const uint32_t st = n % RAWS, round = n / RAWS;
+        if (round > 0) ok = wait(RAWEMPTY + st, round - 1);
+        ok = __all_sync(0xffffffffu, ok);
+        if (!ok) break;
+        float* scales = scales_s + (st * 2 + v) * BK + mine * box_rows;
+        if (mine < boxes && page < 0)
+          for (int i = 0; i < box_rows; i++) scales[i] = 0.0f;
+        const int sound = __popc(__ballot_sync(0xffffffffu, page >= 0));
+        __syncwarp();
+        const uint32_t bar = B_(RAWFULL + st);
+        if (lane == 0)
+          mbar_expect_tx(bar, (uint32_t)(boxes * box_rows * DH * 2 + sound * box_rows * 4));
+        __syncwarp();
+        if (mine < boxes) {
+          tma_load_4d(base + L::BYTES + (st * 2 + v) * L::RAW + (uint32_t)(mine * box_rows) * DH,
+                      v ? &v_map : &k_map, bar, 0, slot, p.h, page);
+          if (page >= 0)
+            bulk_load(smem_u32(scales),
+                      (v ? args.scales.values : args.scales.keys) + page * args.scales.page_stride +
+                          p.h * args.scales.head_stride + slot,
+                      4u * box_rows, bar);
+        }
+        n++;
+      }
+      next_tile(nb);
+    }
+    // every copy has landed before the CTA releases its memory
+    if (lane == 0)
+      for (uint32_t i = n > RAWS ? n - RAWS : 0; i < n; i++)
+        mbar_wait(B_(RAWFULL + i % RAWS), (i / RAWS) & 1u, abort_word);
+  } else if (warp < LOAD_WARP) {
+    // ---- products of half t.  A half without rows goes along with the slots.
+    const int t = warp - MMA_WARP;
+    constexpr uint32_t idesc_s = idesc_f16_m128(BK, 0);
+    constexpr uint32_t idesc_o = idesc_f16_m128(DH, 1);
+    const uint32_t q = base + L::Q + (uint32_t)t * (HALF * DH * 2);
+    const uint32_t s_at = tmem + L::S0 + 128u * t, o_at = tmem + L::O0 + (uint32_t)(DH * t);
+    uint32_t count = 0, items = 0, steps = 0, turns = 0;
+    bool ok = true;
+    // the halves' products go out in turns while both have rows
+    auto my_turn = [&](bool both) { return !both || (t == 0 && turns == 0) || wait(TURN + t, turns - 1 + t); };
+    auto pass_on = [&](bool both) {
+      if (both) {
+        mbar_arrive(B_(TURN + 1 - t));
+        turns++;
+      }
+    };
+    auto scores = [&](uint32_t slot) {
+      const uint32_t k = base + slot * L::SLOT;
+#pragma unroll
+      for (int i = 0; i < DH / 16; i++)
+        umma_f16(s_at, kdesc16<HALF>(q, i), kdesc16<BK>(k, i), idesc_s, i > 0 ? 1u : 0u);
+      umma_commit(B_(SFULL + t));
+    };
+    while (ok && left > 0) {
+      const int nb = blocks_here();
+      const bool rows = rows_here() > HALF * t, both = rows_here() > HALF;
+      uint32_t ks = count % SLOTS;
+      ok = wait(FULL + ks, count / SLOTS);
+      count++;
+      if (ok && rows) ok = wait(QREADY + t, items);
+      if (ok) ok = my_turn(both);
+      ok = __all_sync(0xffffffffu, ok);
+      if (!ok) break;
+      tc_fence_after();
+      if (lane == 0) {
+        if (rows) scores(ks);
+        pass_on(both);
+        umma_commit(B_(EMPTY + ks));
+      }
+      turns = __shfl_sync(0xffffffffu, turns, 0);
+      for (int j = 0; j < nb; j++) {
+        const uint32_t vs = count % SLOTS, vt = base + vs * L::SLOT;
+        ok = __all_sync(0xffffffffu, wait(FULL + vs, count / SLOTS));
+        if (!ok) break;
+        count++;
+        const bool more = j + 1 < nb;
+        if (more) {
+          ks = count % SLOTS;
+          ok = wait(FULL + ks, count / SLOTS);
+          count++;
+        }
+        if (ok && rows) ok = wait(PREADY + t, steps);
+        if (ok) ok = my_turn(both);
+        ok = __all_sync(0xffffffffu, ok);
+        if (!ok) break;
+        tc_fence_after();
+        if (lane == 0) {
+          if (rows) {
+#pragma unroll
+            for (int i = 0; i < BK / 16; i++)
+              umma_f16_ts(o_at, s_at + 8u * i, mdesc16<BK>(vt, i), idesc_o, (j > 0 || i > 0) ? 1u : 0u);
+            if (more) scores(ks);
+            else umma_commit(B_(ODONE + t));
+          }
+          pass_on(both);
+          umma_commit(B_(EMPTY + vs));
+          if (more) umma_commit(B_(EMPTY + ks));
+        }
+        turns = __shfl_sync(0xffffffffu, turns, 0);
+        steps += rows ? 1 : 0;
+      }
+      items += rows ? 1 : 0;
+      next_tile(nb);
+    }
+    if (lane == 0) {
+      umma_commit(B_(DRAIN + t));
+      mbar_wait(B_(DRAIN + t), 0u, abort_word);
+    }
+  }
+  } else {
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kWideRegs));
+    // ---- probabilities: half t, one row per thread
+    const int t = warp >> 2, row = tid & (HALF - 1);
+    const uint32_t lanes = tmem + ((uint32_t)((warp & 3) * 32) << 16);
+    const uint32_t s_at = lanes + L::S0 + 128u * t, o_at = lanes + L::O0 + (uint32_t)(DH * t);
+    const bool q_vec = ((reinterpret_cast<uintptr_t>(a.q) | (uintptr_t)(a.q_stride * 2)) & 15) == 0;
+    const bool rope_vec = ((reinterpret_cast<uintptr_t>(a.rope.cos) | reinterpret_cast<uintptr_t>(a.rope.sin)) & 15) == 0;
+    const bool o_vec = ((reinterpret_cast<uintptr_t>(a.o) | (uintptr_t)(a.o_stride * 2)) & 15) == 0;
+    uint32_t items = 0, steps = 0, n = 0;
+    bool ok = true;
+    Cut cut{0, 0, 0, 0, 0};
+    while (ok && left > 0) {
+      const int nb = blocks_here(), rows = rows_here() - HALF * t;
+      const bool whole = p.blk == 0, ends = p.blk + nb == p.nblk;
+      if (whole && !ends) {
+        const int64_t rest = p.nblk - nb;
+        cut = Cut{p.r.first, p.r.n, p.h, p.tile, 1 + (int)((rest + share.per - 1) / share.per)};
+      }
+      if (rows > 0) {
+        const int g = p.tile * 2 * HALF + HALF * t + row;
+        const bool valid = row < rows;
+        const int token = quotient(g, a.tiling.by_group), head = p.h * group + g - token * group;
+        const int pos = p.r.len - p.r.n + token;
+        const int vis = valid ? max(0, pos + 1) : 0;
+        // keys that every row of this warp sees (invalid rows follow the last valid one)
+        const int vis_warp = __shfl_sync(0xffffffffu, max(0, pos + 1), 0);
+        // ---- the warp's rows of Q, rotated and times 2^e, into the swizzled tile: 8
+        // lanes a row, whole lines, 8 rows' loads in flight
+        float row_scale = 0.0f;
+        {
+          constexpr int P = DH / 64;  // 16-byte pieces of a lane
+          const int first_row = p.tile * 2 * HALF + HALF * t;
+          const uint32_t tile = base + L::Q + (uint32_t)t * (HALF * DH * 2);
+          for (int r0 = 0; r0 < 32; r0 += 8) {
+            union Piece { uint4 v; T x[8]; };
+            Piece u[2][P];
+            float4 cs[2][P], sn[2][P];
+#pragma unroll
+            for (int k = 0; k < 2; k++) {
+              const int r = (warp & 3) * 32 + r0 + 4 * k + (lane >> 3), gr = first_row + r;
+              const int tk = quotient(gr, a.tiling.by_group), at_pos = p.r.len - p.r.n + tk;
+              const bool some = r < rows;
+              const T* src = static_cast<const T*>(a.q) + (p.r.first + tk) * a.q_stride +
+                             (int64_t)(p.h * group + gr - tk * group) * dim;
+              const int64_t tab = some && a.rope.cos != nullptr && at_pos >= 0
+                                      ? rope_row(a.rope, at_pos, a.batch.status) * (dim / 2) : -1;
+#pragma unroll
+              for (int i = 0; i < P; i++) {
+                const int d = 8 * ((lane & 7) + 8 * i);
+                u[k][i].v = make_uint4(0, 0, 0, 0);
+                cs[k][i] = make_float4(1.f, 1.f, 1.f, 1.f);
+                sn[k][i] = make_float4(0.f, 0.f, 0.f, 0.f);
+                if (some && d < dim) {
+                  if (q_vec) u[k][i].v = __ldg(reinterpret_cast<const uint4*>(src + d));
+                  else
+#pragma unroll
+                    for (int e = 0; e < 8; e++) u[k][i].x[e] = src[d + e];
+                  if (tab >= 0) {
+                    const float *ct = a.rope.cos + tab + d / 2, *st = a.rope.sin + tab + d / 2;
+                    if (rope_vec) {
+                      cs[k][i] = __ldg(reinterpret_cast<const float4*>(ct));
+                      sn[k][i] = __ldg(reinterpret_cast<const float4*>(st));
+                    } else {
+                      cs[k][i] = make_float4(__ldg(ct), __ldg(ct + 1), __ldg(ct + 2), __ldg(ct + 3));
+                      sn[k][i] = make_float4(__ldg(st), __ldg(st + 1), __ldg(st + 2), __ldg(st + 3));
+                    }
+                  }
+                }
+              }
+            }
+#pragma unroll
+            for (int k = 0; k < 2; k++) {
+              const int r = (warp & 3) * 32 + r0 + 4 * k + (lane >> 3);
+              float y[P][8], top = 0.0f;
+#pragma unroll
+              for (int i = 0; i < P; i++) {
+                const float cc[4] = {cs[k][i].x, cs[k][i].y, cs[k][i].z, cs[k][i].w};
+                const float ss[4] = {sn[k][i].x, sn[k][i].y, sn[k][i].z, sn[k][i].w};
+#pragma unroll
+                for (int e = 0; e < 4; e++) {
+                  y[i][2 * e] = to_f32<T>(u[k][i].x[2 * e]);
+                  y[i][2 * e + 1] = to_f32<T>(u[k][i].x[2 * e + 1]);
+                  if (a.rope.cos != nullptr) rotate(y[i][2 * e], y[i][2 * e + 1], cc[e], ss[e]);
+                  top = fmaxf(top, fmaxf(fabsf(y[i][2 * e]), fabsf(y[i][2 * e + 1])));
+                }
+              }
+#pragma unroll
+              for (int o = 1; o < 8; o <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+              const int e = query_exponent(top);
+              const float by = exp2_int(e);
+              // to the thread that owns the row
+              const float back = __shfl_sync(0xffffffffu, a.scale_log2 * exp2_int(-e), 8 * (lane & 3));
+              if (lane / 4 == r0 / 4 + k) row_scale = back;
+#pragma unroll
+              for (int i = 0; i < P; i++) {
+                const int c = (lane & 7) + 8 * i;
+                sts128(tile + (uint32_t)(c >> 3) * HALF * 128u + (uint32_t)r * 128u +
+                           ((((uint32_t)c & 7u) ^ (uint32_t)(r & 7)) << 4),
+                       make_float4(__uint_as_float(pack2<__half>(y[i][0] * by, y[i][1] * by)),
+                                   __uint_as_float(pack2<__half>(y[i][2] * by, y[i][3] * by)),
+                                   __uint_as_float(pack2<__half>(y[i][4] * by, y[i][5] * by)),
+                                   __uint_as_float(pack2<__half>(y[i][6] * by, y[i][7] * by))));
+              }
+            }
+          }
+          fence_async_smem();
+          tc_fence_before();
+          mbar_arrive(B_(QREADY + t));
+        }
+        float m = -INFINITY, l = 0.0f;
+        int high = 0;  // F
+        for (int j = 0; ok && j < nb; j++) {
+          const uint32_t at = (n + j) % RING;
+          ok = wait(SFULL + t, steps);
+          if (ok) ok = wait(EXPS + at, (n + j) / RING);
+          ok = __all_sync(0xffffffffu, ok);
+          if (!ok) break;
+          steps++;
+          tc_fence_after();
+          uint32_t r[4][32];
+#pragma unroll
+          for (int c = 0; c < 4; c++) tmem_ld32_nowait(s_at + 32 * c, r[c]);
+          // no less than the least normal number: 0 times a masked score is NaN
+          const float scale = fmaxf(times_power(row_scale, exps[2 * at] - 6), 0x1p-126f);
+          const int now = exps[2 * at + 1], grown = j > 0 ? now - high : 0;
+          high = now;
+          tmem_wait_ld_pin<true>(r[0]);
+          tmem_wait_ld_pin<false>(r[1]);
+          tmem_wait_ld_pin<false>(r[2]);
+          tmem_wait_ld_pin<false>(r[3]);
+          const int key0 = (p.blk + j) * BK;
+          const bool masked = key0 + BK > vis_warp;
+          if (masked) {
+            const int seen = vis - key0;
+#pragma unroll
+            for (int c = 0; c < 4; c++)
+#pragma unroll
+              for (int i = 0; i < 32; i++)
+                if (32 * c + i >= seen) r[c][i] = 0xff800000u;  // -inf
+          }
+          float top[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+#pragma unroll
+          for (int c = 0; c < 4; c++)
+#pragma unroll
+            for (int i = 0; i < 32; i++) top[i & 3] = fmaxf(top[i & 3], __uint_as_float(r[c][i]));
+          const float bmax = fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3])) * scale;
+          const bool jump = bmax > m + kJump || (m == -INFINITY && bmax > -INFINITY);
+          if (__any_sync(0xffffffffu, jump) || grown != 0) {
+            float factor = jump ? ex2(m - bmax) : 1.0f;  // 0 while m is -inf
+            if (jump) {
+              m = bmax;
+              l *= factor;
+            }
+            if (j > 0) {
+              factor *= ex2((float)-grown);
+              // the scores' barrier also says that the last P V is complete
+#pragma unroll
+              for (int c = 0; c < DH / 32; c++) {
+                float o[32];
+                tmem_ld32(o_at + 32 * c, o);
+#pragma unroll
+                for (int i = 0; i < 32; i++) o[i] *= factor;
+                tmem_st32(o_at + 32 * c, o);
+              }
+            }
+          }
+          const float from = (m == -INFINITY ? 0.0f : m) - kShift;
+          // a quarter of the exponentials on the FMA pipe (as in paged_attention_tc.cu);
+          // blocks with masked scores (-inf) all on the special function unit
+          uint64_t sum[2] = {0, 0};
+          auto powers = [&](int c, auto some_masked) {
+            float w[16];
+#pragma unroll
+            for (int i = 0; i < 16; i++) {
+              uint64_t x = fma2(pk(__uint_as_float(r[c][2 * i]), __uint_as_float(r[c][2 * i + 1])),
+                                twice(scale), twice(-from));
+              if (!decltype(some_masked)::value && (i & 3) == 3) {
+                x = power2(x);
+              } else {
+                const float2 v = unpk(x);
+                x = pk(ex2(v.x), ex2(v.y));
+              }
+              sum[i & 1] = add2(sum[i & 1], x);
+              const float2 v = unpk(x);
+              w[i] = __uint_as_float(pack2<__half>(v.x, v.y));
+            }
+            tmem_st16(s_at + 16 * c, w);
+          };
+          if (masked) {
+#pragma unroll
+            for (int c = 0; c < 4; c++) powers(c, std::true_type{});
+          } else {
+#pragma unroll
+            for (int c = 0; c < 4; c++) powers(c, std::false_type{});
+          }
+          const float2 all = unpk(add2(sum[0], sum[1]));
+          l += all.x + all.y;
+          tmem_wait_st();
+          tc_fence_before();
+          mbar_arrive(B_(PREADY + t));
+        }
+        if (ok) ok = __all_sync(0xffffffffu, wait(ODONE + t, items));
+        items++;
+        if (ok) {
+          tc_fence_after();
+          const bool done = whole && ends;
+          const int h2 = (high - 6) / 2;
+          const float f0 = exp2_int(h2), f1 = exp2_int(high - 6 - h2);
+          const float inv = (l > 0.0f ? 1.0f / l : 0.0f) * f0;
+          T* dst = static_cast<T*>(a.o) + (p.r.first + token) * a.o_stride + (int64_t)head * dim;
+          const int slot = 2 * (int)blockIdx.x + (whole ? 1 : 0), r = HALF * t + row;
+          float* part = a.joint.sums + ((int64_t)slot * 2 * HALF + r) * DH;
+#pragma unroll
+          for (int c = 0; c < DH / 32; c++) {
+            float o[32];
+            tmem_ld32(o_at + 32 * c, o);
+            if (!valid) continue;
+            if (done) {
+#pragma unroll
+              for (int i = 0; i < 32; i += 8) {
+                const int d = 32 * c + i;
+                if (d >= dim) break;
+                union { uint4 v; uint32_t w[4]; T x[8]; } u;
+#pragma unroll
+                for (int k = 0; k < 4; k++)
+                  u.w[k] = pack2<T>(o[i + 2 * k] * inv * f1, o[i + 2 * k + 1] * inv * f1);
+                if (o_vec) *reinterpret_cast<uint4*>(dst + d) = u.v;
+                else
+#pragma unroll
+                  for (int k = 0; k < 8; k++) dst[d + k] = u.x[k];
+              }
+            } else {
+#pragma unroll
+              for (int i = 0; i < 32; i += 4)
+                *reinterpret_cast<float4*>(part + 32 * c + i) =
+                    make_float4(o[i] * f0 * f1, o[i + 1] * f0 * f1, o[i + 2] * f0 * f1, o[i + 3] * f0 * f1);
+            }
+          }
+          if (valid) {
+            if (!done) {
+              a.joint.stats[(int64_t)slot * 4 * HALF + r] = m - kShift;
+              a.joint.stats[((int64_t)slot * 2 + 1) * 2 * HALF + r] = l;
+            } else if (a.lse != nullptr) {
+              a.lse[(p.r.first + token) * a.q_heads + head] = l > 0.0f ? (m - kShift) * kLn2 + logf(l) : -INFINITY;
+            }
+          }
+          tc_fence_before();  // O is read before the next tile's QREADY
+        }
+      }
+      n += nb;
+      next_tile(nb);
+    }
+    if (tid == 0) a.joint.cuts[blockIdx.x] = cut;
+  }
+  tc_fence_before();
+  __syncthreads();
+  if (warp == MMA_WARP) {
+    tc_fence_after();
+    tmem_dealloc(tmem, L::COLS);
+    if (lane == 0) report_abort(a.batch.status, abort);
+  }
+}
+
+template <typename T, int DH>
+int launch_tc8(const et_b200_paged_cache8_v1* c, Attend8Args& x, void* ws, cudaStream_t stream) {
+  using L = Layout<DH>;
+  AttendArgs& a = x.a;
+  const int box_rows = (int)(c->page_size < BK ? c->page_size : BK);
+  CUtensorMap k_map, v_map;
+  if (!scales_copy(c) || !pool8_map(&k_map, c->keys, c, DH, box_rows) ||
+      !pool8_map(&v_map, c->values, c, DH, box_rows))
+    return 0;
+  const int blocks = thread_blocks(a, a.sms, 2 * HALF, BK);
+  a.tiling = tiling_of(8, 7, a.tiling.group, a.pools.kv_heads);
+  static_assert(2 * HALF == 1 << 8 && BK == 1 << 7, "tiling");
+  a.least = 2;
+  a.joint = joint_of(ws, blocks, 2 * HALF, DH);
+  cudaFuncSetAttribute(paged_attention8_tc_kernel<T, DH>,
+                       cudaFuncAttributeMaxDynamicSharedMemorySize, L::SMEM);
+  paged_attention8_tc_kernel<T, DH><<<blocks, THREADS, L::SMEM, stream>>>(k_map, v_map, x, box_rows);
+  count_launch();
+  return blocks;
+}
+
+}  // namespace
+
+namespace paged {
+
+int attend8_tc(const et_b200_paged_cache8_v1* c, Attend8Args& x, void* ws, cudaStream_t stream) {
+  if (c->dtype == ET_B200_DTYPE_F32 || c->head_dim > 128) return 0;
+  if (c->dtype == ET_B200_DTYPE_F16)
+    return c->head_dim <= 64 ? launch_tc8<__half, 64>(c, x, ws, stream)
+                             : launch_tc8<__half, 128>(c, x, ws, stream);
+  return c->head_dim <= 64 ? launch_tc8<__nv_bfloat16, 64>(c, x, ws, stream)
+                           : launch_tc8<__nv_bfloat16, 128>(c, x, ws, stream);
+}
+
+}  // namespace paged
+}  // namespace etb

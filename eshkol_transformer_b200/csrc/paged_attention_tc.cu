@@ -32,7 +32,7 @@
 #include <type_traits>
 
 #include "attention_f16.cuh"
-#include "paged.cuh"
+#include "paged_mma.cuh"
 
 namespace etb {
 namespace {
@@ -46,35 +46,6 @@ constexpr int HALF = 128, BK = 128;
 constexpr int MMA_WARP = 8, LOAD_WARP = 10, THREADS = 384;
 constexpr int kWideRegs = 208, kLeanRegs = 88;
 static_assert(256 * kWideRegs + 128 * kLeanRegs <= THREADS * 168, "registers at launch");
-
-template <typename T>
-__device__ __forceinline__ uint32_t pack2(float a, float b) {
-  if constexpr (std::is_same_v<T, __half>) {
-    const __half2 h = __floats2half2_rn(a, b);
-    return *reinterpret_cast<const uint32_t*>(&h);
-  } else {
-    const __nv_bfloat162 h = __floats2bfloat162_rn(a, b);
-    return *reinterpret_cast<const uint32_t*>(&h);
-  }
-}
-
-// 2^x of two finite values on the FMA pipe (x <= 15, under -126 as -126): x =
-// n + f with n rounded to nearest, 2^f by its polynomial of degree 4 of least
-// relative error on |f| <= 1/2 (2.7e-6), n added to the exponent.
-__device__ __forceinline__ uint64_t power2(uint64_t x) {
-  const float2 v = unpk(x);
-  x = pk(fmaxf(v.x, -126.0f), fmaxf(v.y, -126.0f));
-  const uint64_t m = add2(x, twice(12582912.0f));  // 1.5 2^23: n in the low bits
-  const uint64_t f = fma2(add2(m, twice(-12582912.0f)), twice(-1.0f), x);
-  uint64_t y = twice(9.5701013e-3f);
-  y = fma2(y, f, twice(5.5917859e-2f));
-  y = fma2(y, f, twice(2.4024744e-1f));
-  y = fma2(y, f, twice(6.9312179e-1f));
-  y = fma2(y, f, twice(9.9999928e-1f));
-  const float2 mm = unpk(m), yy = unpk(y);
-  return pk(__int_as_float(__float_as_int(yy.x) + (__float_as_int(mm.x) << 23)),
-            __int_as_float(__float_as_int(yy.y) + (__float_as_int(mm.y) << 23)));
-}
 
 template <int DH>
 struct Layout {

@@ -1,6 +1,5 @@
-// Warp matrix pieces, copies and stores that the mma.sync kernels of the paged
-// attention share (paged_attention.cu, paged_attention8.cu), and what launches
-// them.
+// Warp matrix pieces, copies, exponentials and stores that the kernels of the paged
+// attention share, and what launches those on mma.sync.
 #pragma once
 
 #include <type_traits>
@@ -93,6 +92,26 @@ __device__ __forceinline__ void store2(T* dst, float a, float b) {
     dst[0] = from_f32<T>(a);
     dst[1] = from_f32<T>(b);
   }
+}
+
+// ---- exponentials -----------------------------------------------------------------------
+
+// 2^x of two finite values on the FMA pipe (x <= 15, under -126 as -126): x =
+// n + f with n rounded to nearest, 2^f by its polynomial of degree 4 of least
+// relative error on |f| <= 1/2 (2.7e-6), n added to the exponent.
+__device__ __forceinline__ uint64_t power2(uint64_t x) {
+  const float2 v = unpk(x);
+  x = pk(fmaxf(v.x, -126.0f), fmaxf(v.y, -126.0f));
+  const uint64_t m = add2(x, twice(12582912.0f));  // 1.5 2^23: n in the low bits
+  const uint64_t f = fma2(add2(m, twice(-12582912.0f)), twice(-1.0f), x);
+  uint64_t y = twice(9.5701013e-3f);
+  y = fma2(y, f, twice(5.5917859e-2f));
+  y = fma2(y, f, twice(2.4024744e-1f));
+  y = fma2(y, f, twice(6.9312179e-1f));
+  y = fma2(y, f, twice(9.9999928e-1f));
+  const float2 mm = unpk(m), yy = unpk(y);
+  return pk(__int_as_float(__float_as_int(yy.x) + (__float_as_int(mm.x) << 23)),
+            __int_as_float(__float_as_int(yy.y) + (__float_as_int(mm.y) << 23)));
 }
 
 // ---- launching --------------------------------------------------------------------------
