@@ -33,7 +33,7 @@ constexpr int HALF = 128, BK = 128;
 // warps 0-7 probabilities; 8, 9 products, 10 copies; 12-15 conversion.  Registers of
 // the warpgroups out of 512 x 128.
 constexpr int MMA_WARP = 8, LOAD_WARP = 10, CONVERT_WARP = 12, THREADS = 512;
-constexpr int kWideRegs = 208, kLeanRegs = 40, kConvertRegs = 56;
+constexpr int kWideRegs = 200, kLeanRegs = 56, kConvertRegs = 56;
 static_assert(256 * kWideRegs + 128 * (kLeanRegs + kConvertRegs) <= THREADS * 128, "registers at launch");
 constexpr float kJump = 4.0f, kShift = 11.0f;  // weights reach 2^15
 constexpr int RING = 8;  // blocks whose exponents are kept: more than conversion runs ahead
@@ -42,13 +42,13 @@ constexpr int kNone = -1000;  // the exponent of no scale
 template <int DH>
 struct Layout {
   static constexpr int SLOT = BK * DH * 2;  // one block of K or V in binary16
-  static constexpr int SLOTS = DH == 128 ? 3 : 6;
+  static constexpr int SLOTS = DH == 128 ? 4 : 6;
   static constexpr int RAW = BK * DH;       // one block of K or V in bytes
   static constexpr int RAWS = DH == 128 ? 2 : 4;
   static constexpr int Q = SLOTS * SLOT;    // two halves of 128 rows
   static constexpr int BYTES = Q + 2 * HALF * DH * 2;
-  static constexpr int SCALES = BYTES + RAWS * 2 * RAW;  // [RAWS][keys, values][BK]
-  static constexpr int BARS = SCALES + RAWS * 2 * BK * 4;
+  static constexpr int SCALES = BYTES + RAWS * RAW;  // [block % 2][keys, values][BK]
+  static constexpr int BARS = SCALES + 2 * 2 * BK * 4;
   static constexpr int SMEM = BARS + 512;
   // TMEM: scores of the halves (P over the first 64 columns), outputs
   static constexpr uint32_t S0 = 0, O0 = 256, COLS = 512;
@@ -146,10 +146,10 @@ paged_attention8_tc_kernel(const __grid_constant__ CUtensorMap k_map,
       const int nb = blocks_here(), visible = tile_visible(a.tiling, p.r, p.tile);
       int high = kNone;  // F
       for (int j = 0; j < nb; j++, n++) {
-        const uint32_t st = n % RAWS;
-        if (ok) ok = __all_sync(0xffffffffu, wait(RAWFULL + st, n / RAWS));
+        // the scales of both come with K
+        if (ok) ok = __all_sync(0xffffffffu, wait(RAWFULL + 2 * n % RAWS, 2 * n / RAWS));
         const int valid = visible - (p.blk + j) * BK;
-        uint32_t* factors = reinterpret_cast<uint32_t*>(scales_s + st * 2 * BK);
+        uint32_t* factors = reinterpret_cast<uint32_t*>(scales_s + n % 2 * 2 * BK);
         int e[2];
         float s[2];
 #pragma unroll
@@ -182,12 +182,14 @@ paged_attention8_tc_kernel(const __grid_constant__ CUtensorMap k_map,
 #pragma unroll 1
         for (int kv = 0; kv < 2; kv++) {
           const uint32_t count = 2 * n + kv, slot = count % SLOTS, round = count / SLOTS;
-          if (round > 0) ok = __all_sync(0xffffffffu, wait(EMPTY + slot, round - 1));
+          const uint32_t st = count % RAWS;
+          if (kv == 1) ok = __all_sync(0xffffffffu, wait(RAWFULL + st, count / RAWS));
+          if (ok && round > 0) ok = __all_sync(0xffffffffu, wait(EMPTY + slot, round - 1));
           if (!ok) break;  // live until the next barrier
           // a thread takes a 16-byte piece of every fourth (second) row
-          constexpr int P = DH / 16, STEP = 128 / P, UNROLL = 4;
+          constexpr int P = DH / 16, STEP = 128 / P, UNROLL = 2;
           const int piece = c % P;
-          const uint32_t raw = base + L::BYTES + (st * 2 + kv) * L::RAW;
+          const uint32_t raw = base + L::BYTES + st * L::RAW;
           const uint32_t to = base + slot * L::SLOT + (uint32_t)(piece / 4) * BK * 128u;
           // lanes of one row that write the same banks take their halves in turn
           const int turn = piece / 4 & 1;
@@ -213,8 +215,10 @@ paged_attention8_tc_kernel(const __grid_constant__ CUtensorMap k_map,
 #pragma unroll
               for (int k = 0; k < 8; k++) {
                 asm("mul.rn.f16x2 %0, %0, %1;" : "+r"(h[k]) : "r"(f[i]));
-                if (r >= valid) h[k] = 0;  // slots behind the keys may hold anything
               }
+              if (valid < BK && r >= valid)  // slots behind the keys may hold anything
+#pragma unroll
+                for (int k = 0; k < 8; k++) h[k] = 0;
               const float4 lower = make_float4(__uint_as_float(h[0]), __uint_as_float(h[1]),
                                                __uint_as_float(h[2]), __uint_as_float(h[3]));
               const float4 upper = make_float4(__uint_as_float(h[4]), __uint_as_float(h[5]),
@@ -226,9 +230,9 @@ paged_attention8_tc_kernel(const __grid_constant__ CUtensorMap k_map,
           }
           fence_async_smem();
           mbar_arrive(B_(FULL + slot));
+          __syncwarp();
+          if (lane == 0) mbar_arrive(B_(RAWEMPTY + st));
         }
-        __syncwarp();
-        if (ok && lane == 0) mbar_arrive(B_(RAWEMPTY + st));
       }
       next_tile(nb);
     }
@@ -236,7 +240,7 @@ paged_attention8_tc_kernel(const __grid_constant__ CUtensorMap k_map,
   asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kLeanRegs));
   if (warp == LOAD_WARP) {
     // ---- bytes and scales of K and V, page by page: lanes 0 to 15 K, the others V
-    uint32_t n = 0;
+    uint32_t n = 0, count = 0;
     bool ok = true;
     while (ok && left > 0) {
       const int nb = blocks_here(), visible = tile_visible(a.tiling, p.r, p.tile);
@@ -255,35 +259,39 @@ paged_attention8_tc_kernel(const __grid_constant__ CUtensorMap k_map,
             page = -1;  // outside the map: filled with zeros
           }
         }
-        const uint32_t st = n % RAWS, round = n / RAWS;
-        if (round > 0) ok = wait(RAWEMPTY + st, round - 1);
-        ok = __all_sync(0xffffffffu, ok);
-        if (!ok) break;
-        float* scales = scales_s + (st * 2 + v) * BK + mine * box_rows;
-        if (mine < boxes && page < 0)
-          for (int i = 0; i < box_rows; i++) scales[i] = 0.0f;
-        const int sound = __popc(__ballot_sync(0xffffffffu, page >= 0));
-        __syncwarp();
-        const uint32_t bar = B_(RAWFULL + st);
-        if (lane == 0)
-          mbar_expect_tx(bar, (uint32_t)(boxes * box_rows * DH * 2 + sound * box_rows * 4));
-        __syncwarp();
-        if (mine < boxes) {
-          tma_load_4d(base + L::BYTES + (st * 2 + v) * L::RAW + (uint32_t)(mine * box_rows) * DH,
-                      v ? &v_map : &k_map, bar, 0, slot, p.h, page);
-          if (page >= 0)
+#pragma unroll
+        for (int kv = 0; kv < 2; kv++, count++) {
+          const uint32_t st = count % RAWS, round = count / RAWS, bar = B_(RAWFULL + st);
+          if (round > 0) ok = wait(RAWEMPTY + st, round - 1);
+          ok = __all_sync(0xffffffffu, ok);
+          if (!ok) break;
+          uint32_t bytes = (uint32_t)(boxes * box_rows * DH);
+          float* scales = scales_s + (n % 2 * 2 + v) * BK + mine * box_rows;
+          if (kv == 0) {
+            if (mine < boxes && page < 0)
+              for (int i = 0; i < box_rows; i++) scales[i] = 0.0f;
+            bytes += (uint32_t)(__popc(__ballot_sync(0xffffffffu, page >= 0)) * box_rows * 4);
+            __syncwarp();
+          }
+          if (lane == 0) mbar_expect_tx(bar, bytes);
+          __syncwarp();
+          if (kv == 0 && page >= 0)
             bulk_load(smem_u32(scales),
                       (v ? args.scales.values : args.scales.keys) + page * args.scales.page_stride +
                           p.h * args.scales.head_stride + slot,
                       4u * box_rows, bar);
+          if (v == kv && mine < boxes)
+            tma_load_4d(base + L::BYTES + st * L::RAW + (uint32_t)(mine * box_rows) * DH,
+                        v ? &v_map : &k_map, bar, 0, slot, p.h, page);
         }
+        if (!ok) break;
         n++;
       }
       next_tile(nb);
     }
     // every copy has landed before the CTA releases its memory
     if (lane == 0)
-      for (uint32_t i = n > RAWS ? n - RAWS : 0; i < n; i++)
+      for (uint32_t i = count > RAWS ? count - RAWS : 0; i < count; i++)
         mbar_wait(B_(RAWFULL + i % RAWS), (i / RAWS) & 1u, abort_word);
   } else if (warp < LOAD_WARP) {
     // ---- products of half t.  A half without rows goes along with the slots.
@@ -479,8 +487,13 @@ paged_attention8_tc_kernel(const __grid_constant__ CUtensorMap k_map,
         int high = 0;  // F
         for (int j = 0; ok && j < nb; j++) {
           const uint32_t at = (n + j) % RING;
-          ok = wait(SFULL + t, steps);
-          if (ok) ok = wait(EXPS + at, (n + j) / RING);
+          // the exponents, which are there before the scores
+          ok = wait(EXPS + at, (n + j) / RING);
+          // no less than the least normal number: 0 times a masked score is NaN
+          const float scale = fmaxf(times_power(row_scale, exps[2 * at] - 6), 0x1p-126f);
+          const int now = exps[2 * at + 1], grown = j > 0 ? now - high : 0;
+          high = now;
+          if (ok) ok = wait(SFULL + t, steps);
           ok = __all_sync(0xffffffffu, ok);
           if (!ok) break;
           steps++;
@@ -488,10 +501,6 @@ paged_attention8_tc_kernel(const __grid_constant__ CUtensorMap k_map,
           uint32_t r[4][32];
 #pragma unroll
           for (int c = 0; c < 4; c++) tmem_ld32_nowait(s_at + 32 * c, r[c]);
-          // no less than the least normal number: 0 times a masked score is NaN
-          const float scale = fmaxf(times_power(row_scale, exps[2 * at] - 6), 0x1p-126f);
-          const int now = exps[2 * at + 1], grown = j > 0 ? now - high : 0;
-          high = now;
           tmem_wait_ld_pin<true>(r[0]);
           tmem_wait_ld_pin<false>(r[1]);
           tmem_wait_ld_pin<false>(r[2]);
