@@ -42,13 +42,13 @@ constexpr int kNone = -1000;  // the exponent of no scale
 template <int DH>
 struct Layout {
   static constexpr int SLOT = BK * DH * 2;  // one block of K or V in binary16
-  static constexpr int SLOTS = DH == 128 ? 4 : 6;
+  static constexpr int SLOTS = DH == 128 ? 3 : 6;
   static constexpr int RAW = BK * DH;       // one block of K or V in bytes
-  static constexpr int RAWS = DH == 128 ? 2 : 4;
+  static constexpr int RAWS = DH == 128 ? 4 : 8;
   static constexpr int Q = SLOTS * SLOT;    // two halves of 128 rows
   static constexpr int BYTES = Q + 2 * HALF * DH * 2;
-  static constexpr int SCALES = BYTES + RAWS * RAW;  // [block % 2][keys, values][BK]
-  static constexpr int BARS = SCALES + 2 * 2 * BK * 4;
+  static constexpr int SCALES = BYTES + RAWS * RAW;  // [block % (RAWS / 2)][keys, values][BK]
+  static constexpr int BARS = SCALES + RAWS * BK * 4;
   static constexpr int SMEM = BARS + 512;
   // TMEM: scores of the halves (P over the first 64 columns), outputs
   static constexpr uint32_t S0 = 0, O0 = 256, COLS = 512;
@@ -75,12 +75,12 @@ __device__ __forceinline__ float times_power(float x, int e) {
   return x * exp2_int(h) * exp2_int(e - h);
 }
 
-template <typename T, int DH>
+template <typename T, int DH, bool SPLIT>
 __global__ void __launch_bounds__(THREADS, 1)
 paged_attention8_tc_kernel(const __grid_constant__ CUtensorMap k_map,
                            const __grid_constant__ CUtensorMap v_map, Attend8Args args, int box_rows) {
   using L = Layout<DH>;
-  constexpr int SLOTS = L::SLOTS, RAWS = L::RAWS;
+  constexpr int SLOTS = L::SLOTS, RAWS = L::RAWS, TILE = SPLIT ? HALF : 2 * HALF;
   const AttendArgs& a = args.a;
   extern __shared__ __align__(1024) uint8_t smem[];
   float* scales_s = reinterpret_cast<float*>(smem + L::SCALES);
@@ -104,7 +104,7 @@ paged_attention8_tc_kernel(const __grid_constant__ CUtensorMap k_map,
   if (tid == 0) {
     for (int i = 0; i < NBARS; i++)
       mbar_init(B_(i), i < EMPTY                       ? 128
-                       : i < RAWFULL                   ? 2
+                       : i < RAWFULL                   ? (SPLIT ? 1 : 2)
                        : i >= RAWEMPTY && i < SFULL    ? 4
                        : i >= PREADY && i < ODONE      ? HALF
                                                        : 1);
@@ -124,7 +124,7 @@ paged_attention8_tc_kernel(const __grid_constant__ CUtensorMap k_map,
   int64_t left = share.units;
   auto blocks_here = [&]() { return (int)min((int64_t)(p.nblk - p.blk), left); };
   auto rows_here = [&]() {
-    return min(2 * HALF, p.r.n * group - p.tile * 2 * HALF);
+    return min(TILE, p.r.n * group - p.tile * TILE);
   };
   auto next_tile = [&](int done) {
     left -= done;
@@ -146,10 +146,12 @@ paged_attention8_tc_kernel(const __grid_constant__ CUtensorMap k_map,
       const int nb = blocks_here(), visible = tile_visible(a.tiling, p.r, p.tile);
       int high = kNone;  // F
       for (int j = 0; j < nb; j++, n++) {
-        // the scales of both come with K
-        if (ok) ok = __all_sync(0xffffffffu, wait(RAWFULL + 2 * n % RAWS, 2 * n / RAWS));
+        // the scales of both come with V, whose slot says when theirs is free
+        if (ok) ok = wait(RAWFULL + 2 * n % RAWS, 2 * n / RAWS);
+        if (ok) ok = wait(RAWFULL + (2 * n + 1) % RAWS, (2 * n + 1) / RAWS);
+        ok = __all_sync(0xffffffffu, ok);
         const int valid = visible - (p.blk + j) * BK;
-        uint32_t* factors = reinterpret_cast<uint32_t*>(scales_s + n % 2 * 2 * BK);
+        uint32_t* factors = reinterpret_cast<uint32_t*>(scales_s + n % (RAWS / 2) * 2 * BK);
         int e[2];
         float s[2];
 #pragma unroll
@@ -183,8 +185,7 @@ paged_attention8_tc_kernel(const __grid_constant__ CUtensorMap k_map,
         for (int kv = 0; kv < 2; kv++) {
           const uint32_t count = 2 * n + kv, slot = count % SLOTS, round = count / SLOTS;
           const uint32_t st = count % RAWS;
-          if (kv == 1) ok = __all_sync(0xffffffffu, wait(RAWFULL + st, count / RAWS));
-          if (ok && round > 0) ok = __all_sync(0xffffffffu, wait(EMPTY + slot, round - 1));
+          if (round > 0) ok = __all_sync(0xffffffffu, wait(EMPTY + slot, round - 1));
           if (!ok) break;  // live until the next barrier
           // a thread takes a 16-byte piece of every fourth (second) row
           constexpr int P = DH / 16, STEP = 128 / P, UNROLL = 2;
@@ -266,8 +267,8 @@ paged_attention8_tc_kernel(const __grid_constant__ CUtensorMap k_map,
           ok = __all_sync(0xffffffffu, ok);
           if (!ok) break;
           uint32_t bytes = (uint32_t)(boxes * box_rows * DH);
-          float* scales = scales_s + (n % 2 * 2 + v) * BK + mine * box_rows;
-          if (kv == 0) {
+          float* scales = scales_s + (n % (RAWS / 2) * 2 + v) * BK + mine * box_rows;
+          if (kv == 1) {
             if (mine < boxes && page < 0)
               for (int i = 0; i < box_rows; i++) scales[i] = 0.0f;
             bytes += (uint32_t)(__popc(__ballot_sync(0xffffffffu, page >= 0)) * box_rows * 4);
@@ -275,7 +276,7 @@ paged_attention8_tc_kernel(const __grid_constant__ CUtensorMap k_map,
           }
           if (lane == 0) mbar_expect_tx(bar, bytes);
           __syncwarp();
-          if (kv == 0 && page >= 0)
+          if (kv == 1 && page >= 0)
             bulk_load(smem_u32(scales),
                       (v ? args.scales.values : args.scales.keys) + page * args.scales.page_stride +
                           p.h * args.scales.head_stride + slot,
@@ -317,7 +318,51 @@ paged_attention8_tc_kernel(const __grid_constant__ CUtensorMap k_map,
         umma_f16(s_at, kdesc16<HALF>(q, i), kdesc16<BK>(k, i), idesc_s, i > 0 ? 1u : 0u);
       umma_commit(B_(SFULL + t));
     };
-    while (ok && left > 0) {
+    // halves along the keys: each takes every second block of a tile, by itself
+    while (SPLIT && ok && left > 0) {
+      const int nb = blocks_here();
+      ok = __all_sync(0xffffffffu, wait(QREADY + t, items++));
+      for (int j = t; ok && j < nb; j += 2) {
+        const uint32_t k0 = 2 * (count + j), v0 = k0 + 1, k2 = k0 + 4;
+        const uint32_t vt = base + v0 % SLOTS * L::SLOT;
+        if (j == t) {
+          ok = __all_sync(0xffffffffu, wait(FULL + k0 % SLOTS, k0 / SLOTS));
+          if (!ok) break;
+          tc_fence_after();
+          if (lane == 0) {
+            scores(k0 % SLOTS);
+            umma_commit(B_(EMPTY + k0 % SLOTS));
+          }
+        }
+        ok = wait(FULL + v0 % SLOTS, v0 / SLOTS);
+        if (ok) ok = wait(PREADY + t, steps++);
+        ok = __all_sync(0xffffffffu, ok);
+        if (!ok) break;
+        tc_fence_after();
+        const bool more = j + 2 < nb;
+        if (lane == 0) {
+#pragma unroll
+          for (int i = 0; i < BK / 16; i++)
+            umma_f16_ts(o_at, s_at + 8u * i, mdesc16<BK>(vt, i), idesc_o, (j > t || i > 0) ? 1u : 0u);
+          umma_commit(B_(EMPTY + v0 % SLOTS));
+          if (!more) umma_commit(B_(ODONE + t));
+        }
+        __syncwarp();
+        if (more) {  // its slot may be the one that was just given back
+          ok = __all_sync(0xffffffffu, wait(FULL + k2 % SLOTS, k2 / SLOTS));
+          if (!ok) break;
+          tc_fence_after();
+          if (lane == 0) {
+            scores(k2 % SLOTS);
+            umma_commit(B_(EMPTY + k2 % SLOTS));
+          }
+          __syncwarp();
+        }
+      }
+      count += (uint32_t)nb;
+      next_tile(nb);
+    }
+    while (!SPLIT && ok && left > 0) {
       const int nb = blocks_here();
       const bool rows = rows_here() > HALF * t, both = rows_here() > HALF;
       uint32_t ks = count % SLOTS;
@@ -385,15 +430,17 @@ paged_attention8_tc_kernel(const __grid_constant__ CUtensorMap k_map,
     uint32_t items = 0, steps = 0, n = 0;
     bool ok = true;
     Cut cut{0, 0, 0, 0, 0};
+    constexpr int STEP = SPLIT ? 2 : 1;  // blocks from one of this half's to its next
+    const int j0 = SPLIT ? t : 0;
     while (ok && left > 0) {
-      const int nb = blocks_here(), rows = rows_here() - HALF * t;
+      const int nb = blocks_here(), rows = SPLIT ? rows_here() : rows_here() - HALF * t;
       const bool whole = p.blk == 0, ends = p.blk + nb == p.nblk;
       if (whole && !ends) {
         const int64_t rest = p.nblk - nb;
         cut = Cut{p.r.first, p.r.n, p.h, p.tile, 1 + (int)((rest + share.per - 1) / share.per)};
       }
       if (rows > 0) {
-        const int g = p.tile * 2 * HALF + HALF * t + row;
+        const int first_row = p.tile * TILE + (SPLIT ? 0 : HALF * t), g = first_row + row;
         const bool valid = row < rows;
         const int token = quotient(g, a.tiling.by_group), head = p.h * group + g - token * group;
         const int pos = p.r.len - p.r.n + token;
@@ -405,7 +452,6 @@ paged_attention8_tc_kernel(const __grid_constant__ CUtensorMap k_map,
         float row_scale = 0.0f;
         {
           constexpr int P = DH / 64;  // 16-byte pieces of a lane
-          const int first_row = p.tile * 2 * HALF + HALF * t;
           const uint32_t tile = base + L::Q + (uint32_t)t * (HALF * DH * 2);
           for (int r0 = 0; r0 < 32; r0 += 8) {
             union Piece { uint4 v; T x[8]; };
@@ -485,15 +531,16 @@ paged_attention8_tc_kernel(const __grid_constant__ CUtensorMap k_map,
         }
         float m = -INFINITY, l = 0.0f;
         int high = 0;  // F
-        for (int j = 0; ok && j < nb; j++) {
+        for (int j = j0; ok && j < nb; j += STEP) {
           const uint32_t at = (n + j) % RING;
-          // the exponents, which are there before the scores
-          ok = wait(EXPS + at, (n + j) / RING);
+          // the exponents are there before the scores, but only these keep in step with a half
+          // that had no rows for a while
+          ok = wait(SFULL + t, steps);
+          if (ok) ok = wait(EXPS + at, (n + j) / RING);
           // no less than the least normal number: 0 times a masked score is NaN
           const float scale = fmaxf(times_power(row_scale, exps[2 * at] - 6), 0x1p-126f);
-          const int now = exps[2 * at + 1], grown = j > 0 ? now - high : 0;
+          const int now = exps[2 * at + 1], grown = j > j0 ? now - high : 0;
           high = now;
-          if (ok) ok = wait(SFULL + t, steps);
           ok = __all_sync(0xffffffffu, ok);
           if (!ok) break;
           steps++;
@@ -528,7 +575,7 @@ paged_attention8_tc_kernel(const __grid_constant__ CUtensorMap k_map,
               m = bmax;
               l *= factor;
             }
-            if (j > 0) {
+            if (j > j0) {
               factor *= ex2((float)-grown);
               // the scores' barrier also says that the last P V is complete
 #pragma unroll
@@ -576,52 +623,94 @@ paged_attention8_tc_kernel(const __grid_constant__ CUtensorMap k_map,
           tc_fence_before();
           mbar_arrive(B_(PREADY + t));
         }
-        if (ok) ok = __all_sync(0xffffffffu, wait(ODONE + t, items));
-        items++;
-        if (ok) {
-          tc_fence_after();
-          const bool done = whole && ends;
-          const int h2 = (high - 6) / 2;
-          const float f0 = exp2_int(h2), f1 = exp2_int(high - 6 - h2);
-          const float inv = (l > 0.0f ? 1.0f / l : 0.0f) * f0;
-          T* dst = static_cast<T*>(a.o) + (p.r.first + token) * a.o_stride + (int64_t)head * dim;
-          const int slot = 2 * (int)blockIdx.x + (whole ? 1 : 0), r = HALF * t + row;
-          float* part = a.joint.sums + ((int64_t)slot * 2 * HALF + r) * DH;
+        const bool done = whole && ends;
+        T* dst = static_cast<T*>(a.o) + (p.r.first + token) * a.o_stride + (int64_t)head * dim;
+        const int slot = 2 * (int)blockIdx.x + (whole ? 1 : 0), r = first_row - p.tile * TILE + row;
+        float* part = a.joint.sums + ((int64_t)slot * TILE + r) * DH;
+        // 32 sums of the row from dim d, into the result or the parts
+        auto put = [&](int d, const float (&o)[32]) {
+          if (!valid) return;
+          if (done) {
 #pragma unroll
-          for (int c = 0; c < DH / 32; c++) {
-            float o[32];
-            tmem_ld32(o_at + 32 * c, o);
-            if (!valid) continue;
-            if (done) {
+            for (int i = 0; i < 32; i += 8) {
+              if (d + i >= dim) break;
+              union { uint4 v; uint32_t w[4]; T x[8]; } u;
 #pragma unroll
-              for (int i = 0; i < 32; i += 8) {
-                const int d = 32 * c + i;
-                if (d >= dim) break;
-                union { uint4 v; uint32_t w[4]; T x[8]; } u;
+              for (int k = 0; k < 4; k++) u.w[k] = pack2<T>(o[i + 2 * k], o[i + 2 * k + 1]);
+              if (o_vec) *reinterpret_cast<uint4*>(dst + d + i) = u.v;
+              else
 #pragma unroll
-                for (int k = 0; k < 4; k++)
-                  u.w[k] = pack2<T>(o[i + 2 * k] * inv * f1, o[i + 2 * k + 1] * inv * f1);
-                if (o_vec) *reinterpret_cast<uint4*>(dst + d) = u.v;
-                else
-#pragma unroll
-                  for (int k = 0; k < 8; k++) dst[d + k] = u.x[k];
-              }
-            } else {
-#pragma unroll
-              for (int i = 0; i < 32; i += 4)
-                *reinterpret_cast<float4*>(part + 32 * c + i) =
-                    make_float4(o[i] * f0 * f1, o[i + 1] * f0 * f1, o[i + 2] * f0 * f1, o[i + 3] * f0 * f1);
+                for (int k = 0; k < 8; k++) dst[d + i + k] = u.x[k];
             }
+          } else {
+#pragma unroll
+            for (int i = 0; i < 32; i += 4)
+              *reinterpret_cast<float4*>(part + d + i) = make_float4(o[i], o[i + 1], o[i + 2], o[i + 3]);
           }
-          if (valid) {
-            if (!done) {
-              a.joint.stats[(int64_t)slot * 4 * HALF + r] = m - kShift;
-              a.joint.stats[((int64_t)slot * 2 + 1) * 2 * HALF + r] = l;
-            } else if (a.lse != nullptr) {
-              a.lse[(p.r.first + token) * a.q_heads + head] = l > 0.0f ? (m - kShift) * kLn2 + logf(l) : -INFINITY;
+        };
+        auto put_row = [&](float m_all, float l_all) {
+          if (!valid) return;
+          if (!done) {
+            a.joint.stats[(int64_t)slot * 2 * TILE + r] = m_all - kShift;
+            a.joint.stats[((int64_t)slot * 2 + 1) * TILE + r] = l_all;
+          } else if (a.lse != nullptr) {
+            a.lse[(p.r.first + token) * a.q_heads + head] =
+                l_all > 0.0f ? (m_all - kShift) * kLn2 + logf(l_all) : -INFINITY;
+          }
+        };
+        if constexpr (!SPLIT) {
+          if (ok) ok = __all_sync(0xffffffffu, wait(ODONE + t, items));
+          items++;
+          if (ok) {
+            tc_fence_after();
+            const int h2 = (high - 6) / 2;
+            const float f0 = (done ? l > 0.0f ? 1.0f / l : 0.0f : 1.0f) * exp2_int(h2), f1 = exp2_int(high - 6 - h2);
+#pragma unroll
+            for (int c = 0; c < DH / 32; c++) {
+              float o[32];
+              tmem_ld32(o_at + 32 * c, o);
+#pragma unroll
+              for (int i = 0; i < 32; i++) o[i] = o[i] * f0 * f1;
+              put(32 * c, o);
             }
+            put_row(m, l);
+            tc_fence_before();  // O is read before the next tile's QREADY
           }
-          tc_fence_before();  // O is read before the next tile's QREADY
+        } else {
+          // the halves exchange their rows' statistics where their queries were (their
+          // scores are complete), then each writes half of the dims of both sums together
+          const bool mine = nb > t, theirs = nb > 1 - t;
+          if (ok && mine) ok = __all_sync(0xffffffffu, wait(ODONE + t, items++));
+          float4* stats = reinterpret_cast<float4*>(smem + L::Q);
+          constexpr int APART = HALF * DH * 2 / 16;  // float4s from one half's queries to the other's
+          if (ok) stats[t * APART + row] = make_float4(m, l, __int_as_float(high), 0.0f);
+          tc_fence_before();
+          // a wait that ran out ends both together
+          ok = named_all(3, 2 * HALF, ok);
+          if (ok) {
+            tc_fence_after();
+            const float4 other = stats[(1 - t) * APART + row];
+            const float all = fmaxf(m, other.x), ref = all == -INFINITY ? 0.0f : all;
+            const float g0 = ex2(m - ref), g1 = ex2(other.x - ref), sum = l * g0 + other.y * g1;
+            const float inv = done ? sum > 0.0f ? 1.0f / sum : 0.0f : 1.0f;
+            const uint32_t other_at = lanes + L::O0 + (uint32_t)(DH * (1 - t));
+            const int e0 = high - 6, e1 = __float_as_int(other.z) - 6;
+#pragma unroll
+            for (int c = t * (DH / 64); c < (t + 1) * (DH / 64); c++) {
+              float o[32], x[32];
+#pragma unroll
+              for (int i = 0; i < 32; i++) o[i] = x[i] = 0.0f;
+              if (mine) tmem_ld32(o_at + 32 * c, o);
+              if (theirs) tmem_ld32(other_at + 32 * c, x);
+#pragma unroll
+              for (int i = 0; i < 32; i++)
+                o[i] = (times_power(o[i] * g0, e0) + times_power(x[i] * g1, e1)) * inv;
+              put(32 * c, o);
+            }
+            if (t == 0) put_row(all, sum);
+            tc_fence_before();
+            named_sync(3, 2 * HALF);  // O and the statistics are read
+          }
         }
       }
       n += nb;
@@ -639,7 +728,8 @@ paged_attention8_tc_kernel(const __grid_constant__ CUtensorMap k_map,
 }
 
 template <typename T, int DH>
-int launch_tc8(const et_b200_paged_cache8_v1* c, Attend8Args& x, void* ws, cudaStream_t stream) {
+int launch_tc8(const et_b200_paged_cache8_v1* c, Attend8Args& x, int64_t rows, void* ws,
+               cudaStream_t stream) {
   using L = Layout<DH>;
   AttendArgs& a = x.a;
   const int box_rows = (int)(c->page_size < BK ? c->page_size : BK);
@@ -647,29 +737,34 @@ int launch_tc8(const et_b200_paged_cache8_v1* c, Attend8Args& x, void* ws, cudaS
   if (!scales_copy(c) || !pool8_map(&k_map, c->keys, c, DH, box_rows) ||
       !pool8_map(&v_map, c->values, c, DH, box_rows))
     return 0;
-  const int blocks = thread_blocks(a, a.sms, 2 * HALF, BK);
-  a.tiling = tiling_of(8, 7, a.tiling.group, a.pools.kv_heads);
-  static_assert(2 * HALF == 1 << 8 && BK == 1 << 7, "tiling");
-  a.least = 2;
-  a.joint = joint_of(ws, blocks, 2 * HALF, DH);
-  cudaFuncSetAttribute(paged_attention8_tc_kernel<T, DH>,
-                       cudaFuncAttributeMaxDynamicSharedMemorySize, L::SMEM);
-  paged_attention8_tc_kernel<T, DH><<<blocks, THREADS, L::SMEM, stream>>>(k_map, v_map, x, box_rows);
-  count_launch();
-  return blocks;
+  auto go = [&](auto split) {
+    constexpr int TILE = decltype(split)::value ? HALF : 2 * HALF;
+    const auto kernel = paged_attention8_tc_kernel<T, DH, decltype(split)::value>;
+    const int blocks = thread_blocks(a, a.sms, TILE, BK);
+    a.tiling = tiling_of(TILE == HALF ? 7 : 8, 7, a.tiling.group, a.pools.kv_heads);
+    static_assert(HALF == 1 << 7 && BK == 1 << 7, "tiling");
+    a.least = 2;
+    a.joint = joint_of(ws, blocks, TILE, DH);
+    cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, L::SMEM);
+    kernel<<<blocks, THREADS, L::SMEM, stream>>>(k_map, v_map, x, box_rows);
+    count_launch();
+    return blocks;
+  };
+  return rows <= HALF ? go(std::true_type{}) : go(std::false_type{});
 }
 
 }  // namespace
 
 namespace paged {
 
-int attend8_tc(const et_b200_paged_cache8_v1* c, Attend8Args& x, void* ws, cudaStream_t stream) {
+int attend8_tc(const et_b200_paged_cache8_v1* c, Attend8Args& x, int64_t rows, void* ws,
+               cudaStream_t stream) {
   if (c->dtype == ET_B200_DTYPE_F32 || c->head_dim > 128) return 0;
   if (c->dtype == ET_B200_DTYPE_F16)
-    return c->head_dim <= 64 ? launch_tc8<__half, 64>(c, x, ws, stream)
-                             : launch_tc8<__half, 128>(c, x, ws, stream);
-  return c->head_dim <= 64 ? launch_tc8<__nv_bfloat16, 64>(c, x, ws, stream)
-                           : launch_tc8<__nv_bfloat16, 128>(c, x, ws, stream);
+    return c->head_dim <= 64 ? launch_tc8<__half, 64>(c, x, rows, ws, stream)
+                             : launch_tc8<__half, 128>(c, x, rows, ws, stream);
+  return c->head_dim <= 64 ? launch_tc8<__nv_bfloat16, 64>(c, x, rows, ws, stream)
+                           : launch_tc8<__nv_bfloat16, 128>(c, x, rows, ws, stream);
 }
 
 }  // namespace paged
