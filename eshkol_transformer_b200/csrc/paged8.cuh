@@ -51,11 +51,9 @@ bool pool8_map(CUtensorMap* map, void* pool, const et_b200_paged_cache8_v1* c, i
                int box_rows);
 // Whether the scales of neighbouring slots can be copied in whole 16-byte pieces.
 bool scales_copy(const et_b200_paged_cache8_v1* c);
-// The tcgen05 kernel (paged_attention8_tc.cu), for about `rows` query rows per kv head:
-// its thread blocks, 0 where it does not take the cache (nothing is launched).  Its
-// workspace is within attend_tc_workspace.
-int attend8_tc(const et_b200_paged_cache8_v1* c, Attend8Args& a, int64_t rows, void* ws,
-               cudaStream_t stream);
+// The tcgen05 kernel (paged_attention8_tc.cu): its thread blocks, 0 where it does not
+// take the cache (nothing is launched).  Its workspace is within attend_tc_workspace.
+int attend8_tc(const et_b200_paged_cache8_v1* c, Attend8Args& a, void* ws, cudaStream_t stream);
 
 // 2^e of a row of queries: the largest magnitude times it lies in [2^14, 2^15) (1 for
 // rows of zeros and rows that are not finite).

@@ -1009,6 +1009,13 @@ int launch_shape8(const et_b200_paged_cache8_v1* c, Attend8Args& x, void* ws, cu
   return tma ? go(std::true_type{}) : go(std::false_type{});
 }
 
+// How a step's rows per kv head are taken.  One or two columns of 8 queries: few8_kernel
+// alone.  More: tiles of 16, each of which reads the cache (from the L2 after the
+// first), against one pass of attend8_tc (16-bit types) or many8_kernel, whose time is that
+// of its conversion whatever the rows.  32 requests of up to 4,000 keys, 32 / 8 heads x 128,
+// us for 20, 32, 48, 64, 96, 128 rows: bf16 70, 98, 134, 166, 230, 295 in tiles of 16 and 134,
+// 141, 151, 156, 167, 175 by attend8_tc; f32 104, 145, 212, 251, 358, 467 and 272, 274, 275,
+// 277, -, 467 by many8_kernel.
 template <typename T, int DH>
 int launch_dim8(const et_b200_paged_cache8_v1* c, Attend8Args& x, int64_t rows, void* ws,
                 cudaStream_t stream) {
@@ -1018,9 +1025,10 @@ int launch_dim8(const et_b200_paged_cache8_v1* c, Attend8Args& x, int64_t rows, 
     return launch_shape8<T, Shape8<T, DH, 64, 4, 1, 64, 2, 1>>(c, x, ws, stream);
   } else {
     if (rows <= 8) return launch_shape8<T, Shape8<T, DH, 8, 4, 4, 128, 2, 3>>(c, x, ws, stream);
-    if (rows <= 16) return launch_shape8<T, Shape8<T, DH, 16, 4, 4, 128, 3, 2>>(c, x, ws, stream);
+    if (rows <= (sizeof(T) == 2 ? 48 : 64))
+      return launch_shape8<T, Shape8<T, DH, 16, 4, 4, 128, 3, 2>>(c, x, ws, stream);
     if constexpr (sizeof(T) == 2)
-      if (const int blocks = attend8_tc(c, x, rows, ws, stream)) return blocks;
+      if (const int blocks = attend8_tc(c, x, ws, stream)) return blocks;
     return launch_shape8<T, Shape8<T, DH, 64, 4, 1, 64, 2, 2>>(c, x, ws, stream);
   }
 }

@@ -75,12 +75,12 @@ __device__ __forceinline__ float times_power(float x, int e) {
   return x * exp2_int(h) * exp2_int(e - h);
 }
 
-template <typename T, int DH, bool SPLIT>
+template <typename T, int DH>
 __global__ void __launch_bounds__(THREADS, 1)
 paged_attention8_tc_kernel(const __grid_constant__ CUtensorMap k_map,
                            const __grid_constant__ CUtensorMap v_map, Attend8Args args, int box_rows) {
   using L = Layout<DH>;
-  constexpr int SLOTS = L::SLOTS, RAWS = L::RAWS, TILE = SPLIT ? HALF : 2 * HALF;
+  constexpr int SLOTS = L::SLOTS, RAWS = L::RAWS, TILE = 2 * HALF;
   const AttendArgs& a = args.a;
   extern __shared__ __align__(1024) uint8_t smem[];
   float* scales_s = reinterpret_cast<float*>(smem + L::SCALES);
@@ -104,7 +104,7 @@ paged_attention8_tc_kernel(const __grid_constant__ CUtensorMap k_map,
   if (tid == 0) {
     for (int i = 0; i < NBARS; i++)
       mbar_init(B_(i), i < EMPTY                       ? 128
-                       : i < RAWFULL                   ? (SPLIT ? 1 : 2)
+                       : i < RAWFULL                   ? 2
                        : i >= RAWEMPTY && i < SFULL    ? 4
                        : i >= PREADY && i < ODONE      ? HALF
                                                        : 1);
@@ -139,6 +139,19 @@ paged_attention8_tc_kernel(const __grid_constant__ CUtensorMap k_map,
     asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kConvertRegs));
     // ---- bytes into binary16, rows times their scales
     const int c = tid - 32 * CONVERT_WARP;  // this thread's key of a block's scales
+    // A thread takes 16-byte pieces of rows that share their place among 8, so its addresses
+    // differ by constants; lanes 4 apart take rows r and r ^ 5, whose pieces lie in
+    // different banks, both of the bytes and of what is written.
+    constexpr int GROUPS = DH / 64;                                  // of 4 pieces
+    constexpr int APART = DH == 128 ? 16 : 32, ROUNDS = BK / APART;  // rows from one to the next
+    const int quarter = DH == 128 ? (lane >> 4) + 2 * (warp & 1) : lane >> 3 & 3;
+    const int r0 = 8 * (DH == 128 ? warp >> 1 & 1 : warp & 3) + ((lane & 4) ? quarter ^ 5 : quarter);
+    const int in = lane & 3, piece = in + 4 * (GROUPS > 1 ? lane >> 3 & 1 : 0);
+    const uint32_t from = base + L::BYTES + (uint32_t)r0 * DH +
+                          (uint32_t)((DH == 128 ? piece ^ (r0 & 7) : piece ^ (r0 >> 1 & 3)) << 4);
+    const uint32_t to = base + (uint32_t)(piece / 4) * BK * 128u + (uint32_t)r0 * 128u;
+    const uint32_t to0 = to + (uint32_t)(((2 * in) ^ (r0 & 7)) << 4);
+    const uint32_t to1 = to + (uint32_t)(((2 * in + 1) ^ (r0 & 7)) << 4);
     uint32_t n = 0;
     // a wait of one warp that runs out ends the four together, at their next barrier
     bool ok = true, live = true;
@@ -187,46 +200,35 @@ paged_attention8_tc_kernel(const __grid_constant__ CUtensorMap k_map,
           const uint32_t st = count % RAWS;
           if (round > 0) ok = __all_sync(0xffffffffu, wait(EMPTY + slot, round - 1));
           if (!ok) break;  // live until the next barrier
-          // a thread takes a 16-byte piece of every fourth (second) row
-          constexpr int P = DH / 16, STEP = 128 / P, UNROLL = 2;
-          const int piece = c % P;
-          const uint32_t raw = base + L::BYTES + st * L::RAW;
-          const uint32_t to = base + slot * L::SLOT + (uint32_t)(piece / 4) * BK * 128u;
-          // lanes of one row that write the same banks take their halves in turn
-          const int turn = piece / 4 & 1;
+          const uint32_t raw = from + st * L::RAW, out = slot * L::SLOT;
+          const uint32_t* factor = factors + kv * BK + r0;
+          constexpr int BATCH = 2;  // rows whose loads go out together
 #pragma unroll 1
-          for (int r0 = c / P; r0 < BK; r0 += STEP * UNROLL) {
-            float4 x[UNROLL];
-            uint32_t f[UNROLL];
+          for (int i0 = 0; i0 < ROUNDS; i0 += BATCH) {
+            float4 x[BATCH];
+            uint32_t f[BATCH];
 #pragma unroll
-            for (int i = 0; i < UNROLL; i++) {
-              const int r = r0 + i * STEP;
-              const uint32_t swizzled = DH == 128 ? (uint32_t)(piece ^ (r & 7)) : (uint32_t)(piece ^ ((r >> 1) & 3));
-              x[i] = lds128(raw + (uint32_t)r * DH + (swizzled << 4));
-              f[i] = factors[kv * BK + r];
+            for (int k = 0; k < BATCH; k++) {
+              x[k] = lds128(raw + (uint32_t)((i0 + k) * APART * DH));
+              f[k] = factor[(i0 + k) * APART];
             }
 #pragma unroll
-            for (int i = 0; i < UNROLL; i++) {
-              const int r = r0 + i * STEP;
+            for (int k = 0; k < BATCH; k++) {
               uint32_t h[8];
-              halves_of(__float_as_uint(x[i].x), h[0], h[1]);
-              halves_of(__float_as_uint(x[i].y), h[2], h[3]);
-              halves_of(__float_as_uint(x[i].z), h[4], h[5]);
-              halves_of(__float_as_uint(x[i].w), h[6], h[7]);
+              halves_of(__float_as_uint(x[k].x), h[0], h[1]);
+              halves_of(__float_as_uint(x[k].y), h[2], h[3]);
+              halves_of(__float_as_uint(x[k].z), h[4], h[5]);
+              halves_of(__float_as_uint(x[k].w), h[6], h[7]);
 #pragma unroll
-              for (int k = 0; k < 8; k++) {
-                asm("mul.rn.f16x2 %0, %0, %1;" : "+r"(h[k]) : "r"(f[i]));
-              }
-              if (valid < BK && r >= valid)  // slots behind the keys may hold anything
+              for (int e = 0; e < 8; e++) asm("mul.rn.f16x2 %0, %0, %1;" : "+r"(h[e]) : "r"(f[k]));
+              if (valid < BK && r0 + (i0 + k) * APART >= valid)  // slots behind the keys may hold anything
 #pragma unroll
-                for (int k = 0; k < 8; k++) h[k] = 0;
-              const float4 lower = make_float4(__uint_as_float(h[0]), __uint_as_float(h[1]),
-                                               __uint_as_float(h[2]), __uint_as_float(h[3]));
-              const float4 upper = make_float4(__uint_as_float(h[4]), __uint_as_float(h[5]),
-                                               __uint_as_float(h[6]), __uint_as_float(h[7]));
-              const uint32_t row = to + (uint32_t)r * 128u, at = (uint32_t)(2 * (piece & 3));
-              sts128(row + (((at + turn) ^ (uint32_t)(r & 7)) << 4), turn ? upper : lower);
-              sts128(row + (((at + 1 - turn) ^ (uint32_t)(r & 7)) << 4), turn ? lower : upper);
+                for (int e = 0; e < 8; e++) h[e] = 0;
+              const uint32_t at = out + (uint32_t)((i0 + k) * APART * 128);
+              sts128(to0 + at, make_float4(__uint_as_float(h[0]), __uint_as_float(h[1]),
+                                           __uint_as_float(h[2]), __uint_as_float(h[3])));
+              sts128(to1 + at, make_float4(__uint_as_float(h[4]), __uint_as_float(h[5]),
+                                           __uint_as_float(h[6]), __uint_as_float(h[7])));
             }
           }
           fence_async_smem();
@@ -318,51 +320,7 @@ paged_attention8_tc_kernel(const __grid_constant__ CUtensorMap k_map,
         umma_f16(s_at, kdesc16<HALF>(q, i), kdesc16<BK>(k, i), idesc_s, i > 0 ? 1u : 0u);
       umma_commit(B_(SFULL + t));
     };
-    // halves along the keys: each takes every second block of a tile, by itself
-    while (SPLIT && ok && left > 0) {
-      const int nb = blocks_here();
-      ok = __all_sync(0xffffffffu, wait(QREADY + t, items++));
-      for (int j = t; ok && j < nb; j += 2) {
-        const uint32_t k0 = 2 * (count + j), v0 = k0 + 1, k2 = k0 + 4;
-        const uint32_t vt = base + v0 % SLOTS * L::SLOT;
-        if (j == t) {
-          ok = __all_sync(0xffffffffu, wait(FULL + k0 % SLOTS, k0 / SLOTS));
-          if (!ok) break;
-          tc_fence_after();
-          if (lane == 0) {
-            scores(k0 % SLOTS);
-            umma_commit(B_(EMPTY + k0 % SLOTS));
-          }
-        }
-        ok = wait(FULL + v0 % SLOTS, v0 / SLOTS);
-        if (ok) ok = wait(PREADY + t, steps++);
-        ok = __all_sync(0xffffffffu, ok);
-        if (!ok) break;
-        tc_fence_after();
-        const bool more = j + 2 < nb;
-        if (lane == 0) {
-#pragma unroll
-          for (int i = 0; i < BK / 16; i++)
-            umma_f16_ts(o_at, s_at + 8u * i, mdesc16<BK>(vt, i), idesc_o, (j > t || i > 0) ? 1u : 0u);
-          umma_commit(B_(EMPTY + v0 % SLOTS));
-          if (!more) umma_commit(B_(ODONE + t));
-        }
-        __syncwarp();
-        if (more) {  // its slot may be the one that was just given back
-          ok = __all_sync(0xffffffffu, wait(FULL + k2 % SLOTS, k2 / SLOTS));
-          if (!ok) break;
-          tc_fence_after();
-          if (lane == 0) {
-            scores(k2 % SLOTS);
-            umma_commit(B_(EMPTY + k2 % SLOTS));
-          }
-          __syncwarp();
-        }
-      }
-      count += (uint32_t)nb;
-      next_tile(nb);
-    }
-    while (!SPLIT && ok && left > 0) {
+    while (ok && left > 0) {
       const int nb = blocks_here();
       const bool rows = rows_here() > HALF * t, both = rows_here() > HALF;
       uint32_t ks = count % SLOTS;
@@ -430,108 +388,115 @@ paged_attention8_tc_kernel(const __grid_constant__ CUtensorMap k_map,
     uint32_t items = 0, steps = 0, n = 0;
     bool ok = true;
     Cut cut{0, 0, 0, 0, 0};
-    constexpr int STEP = SPLIT ? 2 : 1;  // blocks from one of this half's to its next
-    const int j0 = SPLIT ? t : 0;
     while (ok && left > 0) {
-      const int nb = blocks_here(), rows = SPLIT ? rows_here() : rows_here() - HALF * t;
+      const int nb = blocks_here(), rows = rows_here() - HALF * t;
       const bool whole = p.blk == 0, ends = p.blk + nb == p.nblk;
       if (whole && !ends) {
         const int64_t rest = p.nblk - nb;
         cut = Cut{p.r.first, p.r.n, p.h, p.tile, 1 + (int)((rest + share.per - 1) / share.per)};
       }
       if (rows > 0) {
-        const int first_row = p.tile * TILE + (SPLIT ? 0 : HALF * t), g = first_row + row;
+        const int first_row = p.tile * TILE + HALF * t, g = first_row + row;
         const bool valid = row < rows;
         const int token = quotient(g, a.tiling.by_group), head = p.h * group + g - token * group;
         const int pos = p.r.len - p.r.n + token;
         const int vis = valid ? max(0, pos + 1) : 0;
         // keys that every row of this warp sees (invalid rows follow the last valid one)
         const int vis_warp = __shfl_sync(0xffffffffu, max(0, pos + 1), 0);
-        // ---- the warp's rows of Q, rotated and times 2^e, into the swizzled tile: 8
-        // lanes a row, whole lines, 8 rows' loads in flight
+        // a warp without rows only keeps its barriers; its lanes of the products hold anything
+        const bool live = (warp & 3) * 32 < rows;
+        // ---- the warp's rows of Q, rotated and times 2^e, into the swizzled tile: 8 lanes a
+        // row, whole lines, 4 rows' loads ahead of their use.  Rolled, as whatever runs once a
+        // tile is: its instructions have to be fetched each time.
         float row_scale = 0.0f;
-        {
+        if (live) {
           constexpr int P = DH / 64;  // 16-byte pieces of a lane
           const uint32_t tile = base + L::Q + (uint32_t)t * (HALF * DH * 2);
-          for (int r0 = 0; r0 < 32; r0 += 8) {
-            union Piece { uint4 v; T x[8]; };
-            Piece u[2][P];
-            float4 cs[2][P], sn[2][P];
+          union Piece { uint4 v; T x[8]; };
+          Piece u[P], u_next[P];
+          float4 cs[P], sn[P], cs_next[P], sn_next[P];
+          auto load = [&](int r, Piece (&u)[P], float4 (&cs)[P], float4 (&sn)[P]) {
+            const int gr = first_row + r;
+            const int tk = quotient(gr, a.tiling.by_group), at_pos = p.r.len - p.r.n + tk;
+            const bool some = r < rows;
+            const T* src = static_cast<const T*>(a.q) + (p.r.first + tk) * a.q_stride +
+                           (int64_t)(p.h * group + gr - tk * group) * dim;
+            const int64_t tab = some && a.rope.cos != nullptr && at_pos >= 0
+                                    ? rope_row(a.rope, at_pos, a.batch.status) * (dim / 2) : -1;
 #pragma unroll
-            for (int k = 0; k < 2; k++) {
-              const int r = (warp & 3) * 32 + r0 + 4 * k + (lane >> 3), gr = first_row + r;
-              const int tk = quotient(gr, a.tiling.by_group), at_pos = p.r.len - p.r.n + tk;
-              const bool some = r < rows;
-              const T* src = static_cast<const T*>(a.q) + (p.r.first + tk) * a.q_stride +
-                             (int64_t)(p.h * group + gr - tk * group) * dim;
-              const int64_t tab = some && a.rope.cos != nullptr && at_pos >= 0
-                                      ? rope_row(a.rope, at_pos, a.batch.status) * (dim / 2) : -1;
+            for (int i = 0; i < P; i++) {
+              const int d = 8 * ((lane & 7) + 8 * i);
+              u[i].v = make_uint4(0, 0, 0, 0);
+              cs[i] = make_float4(1.f, 1.f, 1.f, 1.f);
+              sn[i] = make_float4(0.f, 0.f, 0.f, 0.f);
+              if (some && d < dim) {
+                if (q_vec) u[i].v = __ldg(reinterpret_cast<const uint4*>(src + d));
+                else
 #pragma unroll
-              for (int i = 0; i < P; i++) {
-                const int d = 8 * ((lane & 7) + 8 * i);
-                u[k][i].v = make_uint4(0, 0, 0, 0);
-                cs[k][i] = make_float4(1.f, 1.f, 1.f, 1.f);
-                sn[k][i] = make_float4(0.f, 0.f, 0.f, 0.f);
-                if (some && d < dim) {
-                  if (q_vec) u[k][i].v = __ldg(reinterpret_cast<const uint4*>(src + d));
-                  else
-#pragma unroll
-                    for (int e = 0; e < 8; e++) u[k][i].x[e] = src[d + e];
-                  if (tab >= 0) {
-                    const float *ct = a.rope.cos + tab + d / 2, *st = a.rope.sin + tab + d / 2;
-                    if (rope_vec) {
-                      cs[k][i] = __ldg(reinterpret_cast<const float4*>(ct));
-                      sn[k][i] = __ldg(reinterpret_cast<const float4*>(st));
-                    } else {
-                      cs[k][i] = make_float4(__ldg(ct), __ldg(ct + 1), __ldg(ct + 2), __ldg(ct + 3));
-                      sn[k][i] = make_float4(__ldg(st), __ldg(st + 1), __ldg(st + 2), __ldg(st + 3));
-                    }
+                  for (int e = 0; e < 8; e++) u[i].x[e] = src[d + e];
+                if (tab >= 0) {
+                  const float *ct = a.rope.cos + tab + d / 2, *st = a.rope.sin + tab + d / 2;
+                  if (rope_vec) {
+                    cs[i] = __ldg(reinterpret_cast<const float4*>(ct));
+                    sn[i] = __ldg(reinterpret_cast<const float4*>(st));
+                  } else {
+                    cs[i] = make_float4(__ldg(ct), __ldg(ct + 1), __ldg(ct + 2), __ldg(ct + 3));
+                    sn[i] = make_float4(__ldg(st), __ldg(st + 1), __ldg(st + 2), __ldg(st + 3));
                   }
                 }
               }
             }
+          };
+          const int row0 = (warp & 3) * 32 + (lane >> 3);
+          load(row0, u_next, cs_next, sn_next);
+#pragma unroll 1
+          for (int r0 = 0; r0 < 32 && (warp & 3) * 32 + r0 < rows; r0 += 4) {
 #pragma unroll
-            for (int k = 0; k < 2; k++) {
-              const int r = (warp & 3) * 32 + r0 + 4 * k + (lane >> 3);
-              float y[P][8], top = 0.0f;
+            for (int i = 0; i < P; i++) {
+              u[i] = u_next[i];
+              cs[i] = cs_next[i];
+              sn[i] = sn_next[i];
+            }
+            const int r = row0 + r0;
+            load(r + 4, u_next, cs_next, sn_next);  // rows past the last read nothing
+            float y[P][8], top = 0.0f;
 #pragma unroll
-              for (int i = 0; i < P; i++) {
-                const float cc[4] = {cs[k][i].x, cs[k][i].y, cs[k][i].z, cs[k][i].w};
-                const float ss[4] = {sn[k][i].x, sn[k][i].y, sn[k][i].z, sn[k][i].w};
+            for (int i = 0; i < P; i++) {
+              const float cc[4] = {cs[i].x, cs[i].y, cs[i].z, cs[i].w};
+              const float ss[4] = {sn[i].x, sn[i].y, sn[i].z, sn[i].w};
 #pragma unroll
-                for (int e = 0; e < 4; e++) {
-                  y[i][2 * e] = to_f32<T>(u[k][i].x[2 * e]);
-                  y[i][2 * e + 1] = to_f32<T>(u[k][i].x[2 * e + 1]);
-                  if (a.rope.cos != nullptr) rotate(y[i][2 * e], y[i][2 * e + 1], cc[e], ss[e]);
-                  top = fmaxf(top, fmaxf(fabsf(y[i][2 * e]), fabsf(y[i][2 * e + 1])));
-                }
+              for (int e = 0; e < 4; e++) {
+                y[i][2 * e] = to_f32<T>(u[i].x[2 * e]);
+                y[i][2 * e + 1] = to_f32<T>(u[i].x[2 * e + 1]);
+                if (a.rope.cos != nullptr) rotate(y[i][2 * e], y[i][2 * e + 1], cc[e], ss[e]);
+                top = fmaxf(top, fmaxf(fabsf(y[i][2 * e]), fabsf(y[i][2 * e + 1])));
               }
+            }
 #pragma unroll
-              for (int o = 1; o < 8; o <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
-              const int e = query_exponent(top);
-              const float by = exp2_int(e);
-              // to the thread that owns the row
-              const float back = __shfl_sync(0xffffffffu, a.scale_log2 * exp2_int(-e), 8 * (lane & 3));
-              if (lane / 4 == r0 / 4 + k) row_scale = back;
+            for (int o = 1; o < 8; o <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+            const int e = query_exponent(top);
+            const float by = exp2_int(e);
+            // to the thread that owns the row
+            const float back = __shfl_sync(0xffffffffu, a.scale_log2 * exp2_int(-e), 8 * (lane & 3));
+            if (lane / 4 == r0 / 4) row_scale = back;
 #pragma unroll
-              for (int i = 0; i < P; i++) {
-                const int c = (lane & 7) + 8 * i;
-                sts128(tile + (uint32_t)(c >> 3) * HALF * 128u + (uint32_t)r * 128u +
-                           ((((uint32_t)c & 7u) ^ (uint32_t)(r & 7)) << 4),
-                       make_float4(__uint_as_float(pack2<__half>(y[i][0] * by, y[i][1] * by)),
-                                   __uint_as_float(pack2<__half>(y[i][2] * by, y[i][3] * by)),
-                                   __uint_as_float(pack2<__half>(y[i][4] * by, y[i][5] * by)),
-                                   __uint_as_float(pack2<__half>(y[i][6] * by, y[i][7] * by))));
-              }
+            for (int i = 0; i < P; i++) {
+              const int c = (lane & 7) + 8 * i;
+              sts128(tile + (uint32_t)(c >> 3) * HALF * 128u + (uint32_t)r * 128u +
+                         ((((uint32_t)c & 7u) ^ (uint32_t)(r & 7)) << 4),
+                     make_float4(__uint_as_float(pack2<__half>(y[i][0] * by, y[i][1] * by)),
+                                 __uint_as_float(pack2<__half>(y[i][2] * by, y[i][3] * by)),
+                                 __uint_as_float(pack2<__half>(y[i][4] * by, y[i][5] * by)),
+                                 __uint_as_float(pack2<__half>(y[i][6] * by, y[i][7] * by))));
             }
           }
           fence_async_smem();
           tc_fence_before();
-          mbar_arrive(B_(QREADY + t));
         }
+        mbar_arrive(B_(QREADY + t));
         float m = -INFINITY, l = 0.0f;
         int high = 0;  // F
-        for (int j = j0; ok && j < nb; j += STEP) {
+        for (int j = 0; ok && j < nb; j++) {
           const uint32_t at = (n + j) % RING;
           // the exponents are there before the scores, but only these keep in step with a half
           // that had no rows for a while
@@ -539,11 +504,15 @@ paged_attention8_tc_kernel(const __grid_constant__ CUtensorMap k_map,
           if (ok) ok = wait(EXPS + at, (n + j) / RING);
           // no less than the least normal number: 0 times a masked score is NaN
           const float scale = fmaxf(times_power(row_scale, exps[2 * at] - 6), 0x1p-126f);
-          const int now = exps[2 * at + 1], grown = j > j0 ? now - high : 0;
+          const int now = exps[2 * at + 1], grown = j > 0 ? now - high : 0;
           high = now;
           ok = __all_sync(0xffffffffu, ok);
           if (!ok) break;
           steps++;
+          if (!live) {
+            mbar_arrive(B_(PREADY + t));
+            continue;
+          }
           tc_fence_after();
           uint32_t r[4][32];
 #pragma unroll
@@ -575,7 +544,7 @@ paged_attention8_tc_kernel(const __grid_constant__ CUtensorMap k_map,
               m = bmax;
               l *= factor;
             }
-            if (j > j0) {
+            if (j > 0) {
               factor *= ex2((float)-grown);
               // the scores' barrier also says that the last P V is complete
 #pragma unroll
@@ -623,94 +592,50 @@ paged_attention8_tc_kernel(const __grid_constant__ CUtensorMap k_map,
           tc_fence_before();
           mbar_arrive(B_(PREADY + t));
         }
-        const bool done = whole && ends;
-        T* dst = static_cast<T*>(a.o) + (p.r.first + token) * a.o_stride + (int64_t)head * dim;
-        const int slot = 2 * (int)blockIdx.x + (whole ? 1 : 0), r = first_row - p.tile * TILE + row;
-        float* part = a.joint.sums + ((int64_t)slot * TILE + r) * DH;
-        // 32 sums of the row from dim d, into the result or the parts
-        auto put = [&](int d, const float (&o)[32]) {
-          if (!valid) return;
-          if (done) {
+        if (ok) ok = __all_sync(0xffffffffu, wait(ODONE + t, items));
+        items++;
+        if (ok && live) {
+          tc_fence_after();
+          const bool done = whole && ends;
+          const int h2 = (high - 6) / 2;
+          const float f0 = (done ? l > 0.0f ? 1.0f / l : 0.0f : 1.0f) * exp2_int(h2), f1 = exp2_int(high - 6 - h2);
+          T* dst = static_cast<T*>(a.o) + (p.r.first + token) * a.o_stride + (int64_t)head * dim;
+          const int slot = 2 * (int)blockIdx.x + (whole ? 1 : 0), r = HALF * t + row;
+          float* part = a.joint.sums + ((int64_t)slot * TILE + r) * DH;
+#pragma unroll 1
+          for (int c = 0; c < DH; c += 32) {
+            float o[32];
+            tmem_ld32(o_at + c, o);
+            if (!valid) continue;
 #pragma unroll
-            for (int i = 0; i < 32; i += 8) {
-              if (d + i >= dim) break;
-              union { uint4 v; uint32_t w[4]; T x[8]; } u;
+            for (int i = 0; i < 32; i++) o[i] = o[i] * f0 * f1;
+            if (done) {
 #pragma unroll
-              for (int k = 0; k < 4; k++) u.w[k] = pack2<T>(o[i + 2 * k], o[i + 2 * k + 1]);
-              if (o_vec) *reinterpret_cast<uint4*>(dst + d + i) = u.v;
-              else
+              for (int i = 0; i < 32; i += 8) {
+                if (c + i >= dim) break;
+                union { uint4 v; uint32_t w[4]; T x[8]; } u;
 #pragma unroll
-                for (int k = 0; k < 8; k++) dst[d + i + k] = u.x[k];
+                for (int k = 0; k < 4; k++) u.w[k] = pack2<T>(o[i + 2 * k], o[i + 2 * k + 1]);
+                if (o_vec) *reinterpret_cast<uint4*>(dst + c + i) = u.v;
+                else
+#pragma unroll
+                  for (int k = 0; k < 8; k++) dst[c + i + k] = u.x[k];
+              }
+            } else {
+#pragma unroll
+              for (int i = 0; i < 32; i += 4)
+                *reinterpret_cast<float4*>(part + c + i) = make_float4(o[i], o[i + 1], o[i + 2], o[i + 3]);
             }
-          } else {
-#pragma unroll
-            for (int i = 0; i < 32; i += 4)
-              *reinterpret_cast<float4*>(part + d + i) = make_float4(o[i], o[i + 1], o[i + 2], o[i + 3]);
           }
-        };
-        auto put_row = [&](float m_all, float l_all) {
-          if (!valid) return;
-          if (!done) {
-            a.joint.stats[(int64_t)slot * 2 * TILE + r] = m_all - kShift;
-            a.joint.stats[((int64_t)slot * 2 + 1) * TILE + r] = l_all;
-          } else if (a.lse != nullptr) {
-            a.lse[(p.r.first + token) * a.q_heads + head] =
-                l_all > 0.0f ? (m_all - kShift) * kLn2 + logf(l_all) : -INFINITY;
-          }
-        };
-        if constexpr (!SPLIT) {
-          if (ok) ok = __all_sync(0xffffffffu, wait(ODONE + t, items));
-          items++;
-          if (ok) {
-            tc_fence_after();
-            const int h2 = (high - 6) / 2;
-            const float f0 = (done ? l > 0.0f ? 1.0f / l : 0.0f : 1.0f) * exp2_int(h2), f1 = exp2_int(high - 6 - h2);
-#pragma unroll
-            for (int c = 0; c < DH / 32; c++) {
-              float o[32];
-              tmem_ld32(o_at + 32 * c, o);
-#pragma unroll
-              for (int i = 0; i < 32; i++) o[i] = o[i] * f0 * f1;
-              put(32 * c, o);
+          if (valid) {
+            if (!done) {
+              a.joint.stats[(int64_t)slot * 2 * TILE + r] = m - kShift;
+              a.joint.stats[((int64_t)slot * 2 + 1) * TILE + r] = l;
+            } else if (a.lse != nullptr) {
+              a.lse[(p.r.first + token) * a.q_heads + head] = l > 0.0f ? (m - kShift) * kLn2 + logf(l) : -INFINITY;
             }
-            put_row(m, l);
-            tc_fence_before();  // O is read before the next tile's QREADY
           }
-        } else {
-          // the halves exchange their rows' statistics where their queries were (their
-          // scores are complete), then each writes half of the dims of both sums together
-          const bool mine = nb > t, theirs = nb > 1 - t;
-          if (ok && mine) ok = __all_sync(0xffffffffu, wait(ODONE + t, items++));
-          float4* stats = reinterpret_cast<float4*>(smem + L::Q);
-          constexpr int APART = HALF * DH * 2 / 16;  // float4s from one half's queries to the other's
-          if (ok) stats[t * APART + row] = make_float4(m, l, __int_as_float(high), 0.0f);
-          tc_fence_before();
-          // a wait that ran out ends both together
-          ok = named_all(3, 2 * HALF, ok);
-          if (ok) {
-            tc_fence_after();
-            const float4 other = stats[(1 - t) * APART + row];
-            const float all = fmaxf(m, other.x), ref = all == -INFINITY ? 0.0f : all;
-            const float g0 = ex2(m - ref), g1 = ex2(other.x - ref), sum = l * g0 + other.y * g1;
-            const float inv = done ? sum > 0.0f ? 1.0f / sum : 0.0f : 1.0f;
-            const uint32_t other_at = lanes + L::O0 + (uint32_t)(DH * (1 - t));
-            const int e0 = high - 6, e1 = __float_as_int(other.z) - 6;
-#pragma unroll
-            for (int c = t * (DH / 64); c < (t + 1) * (DH / 64); c++) {
-              float o[32], x[32];
-#pragma unroll
-              for (int i = 0; i < 32; i++) o[i] = x[i] = 0.0f;
-              if (mine) tmem_ld32(o_at + 32 * c, o);
-              if (theirs) tmem_ld32(other_at + 32 * c, x);
-#pragma unroll
-              for (int i = 0; i < 32; i++)
-                o[i] = (times_power(o[i] * g0, e0) + times_power(x[i] * g1, e1)) * inv;
-              put(32 * c, o);
-            }
-            if (t == 0) put_row(all, sum);
-            tc_fence_before();
-            named_sync(3, 2 * HALF);  // O and the statistics are read
-          }
+          tc_fence_before();  // O is read before the next tile's QREADY
         }
       }
       n += nb;
@@ -728,8 +653,7 @@ paged_attention8_tc_kernel(const __grid_constant__ CUtensorMap k_map,
 }
 
 template <typename T, int DH>
-int launch_tc8(const et_b200_paged_cache8_v1* c, Attend8Args& x, int64_t rows, void* ws,
-               cudaStream_t stream) {
+int launch_tc8(const et_b200_paged_cache8_v1* c, Attend8Args& x, void* ws, cudaStream_t stream) {
   using L = Layout<DH>;
   AttendArgs& a = x.a;
   const int box_rows = (int)(c->page_size < BK ? c->page_size : BK);
@@ -737,34 +661,29 @@ int launch_tc8(const et_b200_paged_cache8_v1* c, Attend8Args& x, int64_t rows, v
   if (!scales_copy(c) || !pool8_map(&k_map, c->keys, c, DH, box_rows) ||
       !pool8_map(&v_map, c->values, c, DH, box_rows))
     return 0;
-  auto go = [&](auto split) {
-    constexpr int TILE = decltype(split)::value ? HALF : 2 * HALF;
-    const auto kernel = paged_attention8_tc_kernel<T, DH, decltype(split)::value>;
-    const int blocks = thread_blocks(a, a.sms, TILE, BK);
-    a.tiling = tiling_of(TILE == HALF ? 7 : 8, 7, a.tiling.group, a.pools.kv_heads);
-    static_assert(HALF == 1 << 7 && BK == 1 << 7, "tiling");
-    a.least = 2;
-    a.joint = joint_of(ws, blocks, TILE, DH);
-    cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, L::SMEM);
-    kernel<<<blocks, THREADS, L::SMEM, stream>>>(k_map, v_map, x, box_rows);
-    count_launch();
-    return blocks;
-  };
-  return rows <= HALF ? go(std::true_type{}) : go(std::false_type{});
+  const int blocks = thread_blocks(a, a.sms, 2 * HALF, BK);
+  a.tiling = tiling_of(8, 7, a.tiling.group, a.pools.kv_heads);
+  static_assert(2 * HALF == 1 << 8 && BK == 1 << 7, "tiling");
+  a.least = 2;
+  a.joint = joint_of(ws, blocks, 2 * HALF, DH);
+  cudaFuncSetAttribute(paged_attention8_tc_kernel<T, DH>,
+                       cudaFuncAttributeMaxDynamicSharedMemorySize, L::SMEM);
+  paged_attention8_tc_kernel<T, DH><<<blocks, THREADS, L::SMEM, stream>>>(k_map, v_map, x, box_rows);
+  count_launch();
+  return blocks;
 }
 
 }  // namespace
 
 namespace paged {
 
-int attend8_tc(const et_b200_paged_cache8_v1* c, Attend8Args& x, int64_t rows, void* ws,
-               cudaStream_t stream) {
+int attend8_tc(const et_b200_paged_cache8_v1* c, Attend8Args& x, void* ws, cudaStream_t stream) {
   if (c->dtype == ET_B200_DTYPE_F32 || c->head_dim > 128) return 0;
   if (c->dtype == ET_B200_DTYPE_F16)
-    return c->head_dim <= 64 ? launch_tc8<__half, 64>(c, x, rows, ws, stream)
-                             : launch_tc8<__half, 128>(c, x, rows, ws, stream);
-  return c->head_dim <= 64 ? launch_tc8<__nv_bfloat16, 64>(c, x, rows, ws, stream)
-                           : launch_tc8<__nv_bfloat16, 128>(c, x, rows, ws, stream);
+    return c->head_dim <= 64 ? launch_tc8<__half, 64>(c, x, ws, stream)
+                             : launch_tc8<__half, 128>(c, x, ws, stream);
+  return c->head_dim <= 64 ? launch_tc8<__nv_bfloat16, 64>(c, x, ws, stream)
+                           : launch_tc8<__nv_bfloat16, 128>(c, x, ws, stream);
 }
 
 }  // namespace paged
