@@ -699,8 +699,8 @@ __device__ __forceinline__ void count_before(const Ranking& r, int n, const Room
   *mass = m;
 }
 
-// Rank 0: cuts the list of n entries by all filters and draws (n <= NT), or, for
-// distributions, leaves the last kept entry in rm.border and what is kept in rm.total.
+// Rank 0: cuts the list of n entries by all filters and draws (n <= NT), or writes the
+// kept tokens' probabilities into a row of zeros.
 template <bool PROBS>
 __device__ void draw_from_short_list(int n, const Args& a, int64_t row, const Filters& flt,
                                      const Scale& sc, Room& rm) {
@@ -720,12 +720,7 @@ __device__ void draw_from_short_list(int n, const Args& a, int64_t row, const Fi
   const bool keep = first && rank < k && (before < aim || rank == 0) && x >= least_logit(flt, sc.max);
   room_scan(keep ? w : 0, rm, &all);  // its barriers also end the reading of the weights
   if constexpr (PROBS) {
-    // what is kept is a prefix of the ranking
-    const int count = __syncthreads_count(keep);
-    if (keep && rank == count - 1) {
-      rm.border = Border{x, entry_index(e)};
-      rm.total = all;
-    }
+    if (keep) a.probs[row * a.probs_stride + entry_index(e)] = share_of(x, sc, per_total(all));
     return;
   }
   if (first && !keep) rm.list[r.entry] = 0;
@@ -775,10 +770,9 @@ __device__ void draw_from_list(int n, const Args& a, int64_t row, const Filters&
 #pragma unroll
     for (int j = 0; j < PER; j++) mine += tid * PER + j < n ? w[j] : 0;
     room_scan(mine, rm, &all);
-    if (tid == 0) {
-      rm.border = Border{entry_value(rm.all[n - 1]), entry_index(rm.all[n - 1])};
-      rm.total = all;
-    }
+    const float inv = per_total(all);
+    for (int i = tid; i < n; i += NT)
+      a.probs[row * a.probs_stride + entry_index(rm.all[i])] = share_of(entry_value(rm.all[i]), sc, inv);
     return;
   }
   __syncthreads();
@@ -1084,6 +1078,33 @@ __device__ __forceinline__ void write_shares(const Slice<T>& s, float* out, int 
   });
 }
 
+// Zeros for n floats from out, as copies that run by themselves until zeros_done; `zeros` is
+// ZEROS floats of shared memory.
+constexpr int ZEROS = 1024;
+__device__ void begin_zeros(float* out, int n, float* zeros) {
+  const int tid = threadIdx.x;
+  for (int i = tid; i < ZEROS; i += NT) zeros[i] = 0.0f;
+  const int head = min(n, (int)((16 - (reinterpret_cast<uintptr_t>(out) & 15)) & 15) / 4);
+  const int whole = (n - head) & ~3, tail = head + whole;
+  if (tid < head) out[tid] = 0.0f;
+  else if (tid >= 32 && tail + tid - 32 < n) out[tail + tid - 32] = 0.0f;
+  asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+  __syncthreads();
+  if (tid == 0) {
+    const uint32_t from = (uint32_t)__cvta_generic_to_shared(zeros);
+    for (int i = 0; i < whole; i += ZEROS)
+      asm volatile("cp.async.bulk.global.shared::cta.bulk_group [%0], [%1], %2;" ::"l"(out + head + i),
+                   "r"(from), "r"(4 * min(ZEROS, whole - i)) : "memory");
+    asm volatile("cp.async.bulk.commit_group;" ::: "memory");
+  }
+}
+__device__ __forceinline__ void zeros_done() {  // by the thread that began them
+  if (threadIdx.x == 0) {
+    asm volatile("cp.async.bulk.wait_group 0;" ::: "memory");
+    asm volatile("fence.proxy.async.global;" ::: "memory");
+  }
+}
+
 template <typename T, bool PROBS>
 __global__ void __launch_bounds__(NT, 2) sample_cluster_kernel(const T* __restrict__ logits, Args a) {
   extern __shared__ __align__(16) uint8_t slice_smem[];
@@ -1115,6 +1136,15 @@ __global__ void __launch_bounds__(NT, 2) sample_cluster_kernel(const T* __restri
     for (int p = g * part + tid; p < end; p += NT) cp16(dst + 16u * p, src + p * Slice<T>::N);
     asm volatile("cp.async.commit_group;" ::: "memory");
   }
+  // A row that keeps few tokens is zeros but for those, which go out while it is read: a
+  // greedy one, and one that becomes a list.
+  const bool greedy = !(flt.temperature > 0x1p-100f);
+  const bool top_k = flt.top_k > 0 && flt.top_k < a.n;
+  bool listed = a.n <= LIST || (top_k && flt.top_k <= NT / 2);
+  float* out = PROBS ? a.probs + row * a.probs_stride + first : nullptr;
+  __shared__ __align__(16) float zeros[PROBS ? ZEROS : 4];
+  if constexpr (PROBS)
+    if (greedy || listed) begin_zeros(out, slice.n, zeros);
   float top = -INFINITY;
   {
     const int tail = slice.head + slice.pieces * Slice<T>::N;
@@ -1154,9 +1184,11 @@ __global__ void __launch_bounds__(NT, 2) sample_cluster_kernel(const T* __restri
   for (unsigned b = 0; b < blocks; b++) max = fmaxf(max, cluster.map_shared_rank(&rm, b)->top);
 
   // no block leaves while another may read or write its shared memory
-  float* out = PROBS ? a.probs + row * a.probs_stride + first : nullptr;
   if (max == -INFINITY) {
-    if constexpr (PROBS) write_slice(slice, out, INFINITY, [](float, int) { return 0.0f; });
+    if constexpr (PROBS) {
+      if (greedy || listed) zeros_done();
+      else write_slice(slice, out, INFINITY, [](float, int) { return 0.0f; });
+    }
     if (!PROBS && rank == 0 && tid == 0) {
       a.ids[row] = -1;
       if (a.logprobs != nullptr) a.logprobs[row] = -INFINITY;
@@ -1164,38 +1196,36 @@ __global__ void __launch_bounds__(NT, 2) sample_cluster_kernel(const T* __restri
     cluster.sync();
     return;
   }
-  if (!(flt.temperature > 0x1p-100f)) {  // the first of the largest
+  if (greedy) {  // the first of the largest
     int best = INT32_MAX;
     if (block_top == max)
       slice.each([&](int i, float v) { if (v == max) best = min(best, first + i); });
     best = __reduce_min_sync(0xffffffffu, best);
     __syncthreads();
     if (lane == 0) rm.warp[warp] = (uint64_t)best;
+    if constexpr (PROBS) zeros_done();
     cluster.sync();
-    if constexpr (PROBS) {  // every warp finds it
-      for (unsigned i = lane; i < blocks * WARPS; i += 32)
-        best = min(best, (int)cluster.map_shared_rank(&rm, i / WARPS)->warp[i % WARPS]);
-      best = __reduce_min_sync(0xffffffffu, best);
-      write_slice(slice, out, max, [&](float, int i) { return first + i == best ? 1.0f : 0.0f; });
-    } else if (rank == 0 && warp == 0) {
+    if (rank == 0 && warp == 0) {
       for (unsigned i = lane; i < blocks * WARPS; i += 32)
         best = min(best, (int)cluster.map_shared_rank(&rm, i / WARPS)->warp[i % WARPS]);
       best = __reduce_min_sync(0xffffffffu, best);
       if (lane == 0) {
-        a.ids[row] = best;
-        if (a.logprobs != nullptr) a.logprobs[row] = 0.0f;
+        if constexpr (PROBS) {
+          a.probs[row * a.probs_stride + best] = 1.0f;
+        } else {
+          a.ids[row] = best;
+          if (a.logprobs != nullptr) a.logprobs[row] = 0.0f;
+        }
       }
     }
     cluster.sync();
     return;
   }
   const Scale sc = scale_of(max, flt.per);
-  const bool top_k = flt.top_k > 0 && flt.top_k < a.n;
 
   // ---- a list
-  bool listed = a.n <= LIST;
   float bound = -INFINITY;
-  if (!listed && top_k && flt.top_k <= NT / 2) {
+  if (listed && a.n > LIST) {
     // What k / blocks tokens of every slice reach, k tokens of the row reach;
     // where a slice has fewer, what k tokens of one slice reach.
     bound = top_bound(thread_top, block_top, ((int)flt.top_k + (int)blocks - 1) / (int)blocks, rm);
@@ -1215,13 +1245,13 @@ __global__ void __launch_bounds__(NT, 2) sample_cluster_kernel(const T* __restri
       cluster.sync();  // the first bounds are read
       exchange(false);
     }
-    listed = true;
   }
   if (listed) {
     Room* head = cluster.map_shared_rank(&rm, 0);
     slice.each_from(bound, [&](int i, float v) {
       if (v > -INFINITY && v >= bound) push(head, entry_of(v, first + i));
     });
+    if constexpr (PROBS) zeros_done();
     cluster.sync();
     const int n = head->count;
     if (n <= LIST) {
@@ -1229,13 +1259,6 @@ __global__ void __launch_bounds__(NT, 2) sample_cluster_kernel(const T* __restri
       // have read its count
       cluster.sync();
       if (rank == 0) draw_from_list<PROBS>(n, a, row, flt, sc, rm);
-      if constexpr (PROBS) {
-        cluster.sync();
-        const Border border = head->border;
-        const uint64_t total = head->total;
-        cluster.sync();  // read: rank 0 may leave
-        write_shares(slice, out, first, border, sc, total);
-      }
       return;
     }
   }
@@ -1367,11 +1390,13 @@ __global__ void __launch_bounds__(NT) sample_kernel(const T* __restrict__ logits
 // up to 8 while that leaves SMs idle and a slice keeps 4,096 logits.
 template <typename T, bool PROBS>
 cudaError_t launch(const T* logits, Args a, int64_t rows, cudaStream_t stream) {
-  constexpr int kSliceBytes = 96 * 1024;
+  // two thread blocks of the largest slice fit an SM, distributions with their zeros too
+  constexpr int kSliceBytes = (PROBS ? 88 : 96) * 1024;
   int blocks = 1;
   auto slice_of = [&](int b) { return ((a.n + b - 1) / b + 15) / 16 * 16; };
   while (blocks < 8 && (int64_t)slice_of(blocks) * (int)sizeof(T) > kSliceBytes) blocks *= 2;
-  if ((int64_t)slice_of(blocks) * (int)sizeof(T) > 208 * 1024 || rows * blocks > INT32_MAX) {
+  constexpr int kMost = (PROBS ? 204 : 208) * 1024;  // of one thread block
+  if ((int64_t)slice_of(blocks) * (int)sizeof(T) > kMost || rows * blocks > INT32_MAX) {
     sample_kernel<T, PROBS><<<(unsigned)rows, NT, 0, stream>>>(logits, a);
     count_launch();
     return cudaGetLastError();
@@ -1380,7 +1405,7 @@ cudaError_t launch(const T* logits, Args a, int64_t rows, cudaStream_t stream) {
   a.slice = slice_of(blocks);
   const int smem = a.slice * (int)sizeof(T) + 32;
   cudaError_t st = cudaFuncSetAttribute(sample_cluster_kernel<T, PROBS>,
-                                        cudaFuncAttributeMaxDynamicSharedMemorySize, 209 * 1024);
+                                        cudaFuncAttributeMaxDynamicSharedMemorySize, kMost + 1024);
   if (st != cudaSuccess) return st;
   cudaLaunchConfig_t cfg{};
   cfg.gridDim = dim3((unsigned)(rows * blocks));

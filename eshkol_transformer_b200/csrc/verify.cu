@@ -164,7 +164,8 @@ __global__ void __launch_bounds__(NT, 2) verify_kernel(VerifyArgs a) {
       const unsigned from = (unsigned)(s / each);
       if (from != rank) sums[s] = cluster.map_shared_rank(sums, from)[s];
     }
-    cluster.sync();  // read by all: blocks may leave or begin again
+    // every block waits for this before it leaves or begins again; the first draws meanwhile
+    cluster.barrier_arrive();
     // running sums of `per` segments a thread
     const int per = (a.segs + NT - 1) / NT, t0 = min(a.segs, tid * per), t1 = min(a.segs, t0 + per);
     double own = 0.0;
@@ -184,7 +185,7 @@ __global__ void __launch_bounds__(NT, 2) verify_kernel(VerifyArgs a) {
       total += warp_s[w];
     }
     if (total > 0.0) {
-      if (rank != 0) return;
+      if (rank != 0) break;
       const double u = a.draw[b], aim = u > 0.0 ? u * total : 0.0;
       // the first segment whose running sum exceeds the aim; rounding, or an aim of the
       // total, may leave none: then the last that weighs something
@@ -215,30 +216,44 @@ __global__ void __launch_bounds__(NT, 2) verify_kernel(VerifyArgs a) {
       }
       __syncthreads();
       if (warp == 0) {
-        // 32 neighbouring tokens a lane
+        // the tokens in order: rounds of 128, 4 neighbours a lane
         const double left = none ? INFINITY : aim - before_s;
-        const int i0 = seg * SEG + lane * (SEG / 32), i1 = min(a.n, i0 + SEG / 32);
-        double sum = 0.0;
-        int some = -1;
-        for (int i = i0; i < i1; i++) {
-          const double w = rest.at(i);
-          sum += w;
-          if (w > 0.0) some = i;
-        }
-        double upto = sum;
+        constexpr int J = 4;  // rounds whose loads go out together
+        double go = 0.0;
+        int hit = INT32_MAX, some = -1;
+#pragma unroll 1
+        for (int i0 = seg * SEG + 4 * lane; i0 < (seg + 1) * SEG + 4 * lane; i0 += 128 * J) {
+          float x[J][4], y[J][4];
 #pragma unroll
-        for (int o = 1; o < 32; o <<= 1) {
-          const double v = __shfl_up_sync(0xffffffffu, upto, o);
-          if (lane >= o) upto += v;
-        }
-        double go = upto - sum;
-        int hit = INT32_MAX;
-        for (int i = i0; i < i1; i++) {
-          const double w = rest.at(i);
-          go += w;
-          if (w > 0.0 && go > left) {
-            hit = i;
-            break;
+          for (int j = 0; j < J; j++)
+#pragma unroll
+            for (int k = 0; k < 4; k++) {
+              const int i = i0 + 128 * j + k;
+              x[j][k] = i < a.n && i != rest.without ? rest.p[i] : 0.0f;
+              y[j][k] = i < a.n && rest.q != nullptr ? rest.q[i] : 0.0f;
+            }
+#pragma unroll
+          for (int j = 0; j < J; j++) {
+            double w[4], sum = 0.0;
+#pragma unroll
+            for (int k = 0; k < 4; k++) {
+              w[k] = fmax(probability(x[j][k]) - probability(y[j][k]), 0.0);
+              sum += w[k];
+              if (w[k] > 0.0) some = i0 + 128 * j + k;
+            }
+            double upto = sum;
+#pragma unroll
+            for (int o = 1; o < 32; o <<= 1) {
+              const double v = __shfl_up_sync(0xffffffffu, upto, o);
+              if (lane >= o) upto += v;
+            }
+            double run_in = go + (upto - sum);
+#pragma unroll
+            for (int k = 0; k < 4; k++) {
+              run_in += w[k];
+              if (w[k] > 0.0 && run_in > left) hit = min(hit, i0 + 128 * j + k);
+            }
+            go += __shfl_sync(0xffffffffu, upto, 31);
           }
         }
         hit = __reduce_min_sync(0xffffffffu, hit);
@@ -252,8 +267,9 @@ __global__ void __launch_bounds__(NT, 2) verify_kernel(VerifyArgs a) {
     if (rest.q == nullptr && rest.without < 0) break;  // p has no mass either
     rest.q = nullptr;
     rest.without = -1;
-    __syncthreads();
+    cluster.barrier_wait();
   }
+  cluster.barrier_wait();
   if (rank != 0) return;
   for (int i = tid; i < n; i += NT)
     a.ids[first + i] = i < stop ? a.drafts[first + i] : i == stop ? id : -1;
@@ -261,10 +277,10 @@ __global__ void __launch_bounds__(NT, 2) verify_kernel(VerifyArgs a) {
 }
 
 cudaError_t launch_verify(const VerifyArgs& a, int64_t batch, cudaStream_t stream) {
-  // up to 8 thread blocks a request while they fit the device at once (4 of 512 threads
-  // an SM) and each warp keeps a segment
+  // up to 8 thread blocks a request while they fit the device at once (two an SM) and each
+  // warp keeps a segment
   int blocks = 1;
-  while (blocks < 8 && batch * blocks * 2 <= 4 * sm_count() && a.segs >= 2 * blocks * WARPS) blocks *= 2;
+  while (blocks < 8 && batch * blocks * 2 <= 2 * sm_count() && a.segs >= 2 * blocks * WARPS) blocks *= 2;
   cudaLaunchConfig_t cfg{};
   cfg.gridDim = dim3((unsigned)(batch * blocks));
   cfg.blockDim = dim3(NT);
