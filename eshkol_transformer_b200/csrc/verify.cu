@@ -43,8 +43,11 @@ struct VerifyArgs {
 };
 
 // A probability as the rules read it: NaN and negative ones are 0, the largest is 1.
-__device__ __forceinline__ double probability(float p) {
-  return p > 0.0f ? (double)fminf(p, 1.0f) : 0.0;
+__device__ __forceinline__ float probability(float p) { return p > 0.0f ? fminf(p, 1.0f) : 0.0f; }
+// max(p - q, 0), in 32 bits: a conversion to 64 costs four times a difference, and its
+// rounding moves a draw's border by less than 2^-24 of one token's weight.
+__device__ __forceinline__ double weight(float p, float q) {
+  return (double)fmaxf(probability(p) - probability(q), 0.0f);
 }
 
 // The weights that the request's token is drawn from.
@@ -53,9 +56,7 @@ struct Rest {
   const float* q;  // or null
   int without;     // a token of weight 0 (a proposal made without chance), or -1
   __device__ __forceinline__ double at(int i) const {
-    const double x = probability(p[i]);
-    if (q != nullptr) return fmax(x - probability(q[i]), 0.0);
-    return i == without ? 0.0 : x;
+    return weight(i == without ? 0.0f : p[i], q != nullptr ? q[i] : 0.0f);
   }
 };
 
@@ -79,19 +80,19 @@ __device__ double segment(const VerifyArgs& a, const Rest& rest, int s) {
       for (int j = 0; j < J; j++) y[j] = __ldcs(reinterpret_cast<const float4*>(rest.q + i0) + lane + 32 * j);
 #pragma unroll
       for (int j = 0; j < J; j++) {
-        sum += fmax(probability(x[j].x) - probability(y[j].x), 0.0);
-        sum += fmax(probability(x[j].y) - probability(y[j].y), 0.0);
-        sum += fmax(probability(x[j].z) - probability(y[j].z), 0.0);
-        sum += fmax(probability(x[j].w) - probability(y[j].w), 0.0);
+        sum += weight(x[j].x, y[j].x);
+        sum += weight(x[j].y, y[j].y);
+        sum += weight(x[j].z, y[j].z);
+        sum += weight(x[j].w, y[j].w);
       }
     } else {
 #pragma unroll
       for (int j = 0; j < J; j++) {
         const int i = i0 + 4 * (lane + 32 * j);
-        sum += i == rest.without ? 0.0 : probability(x[j].x);
-        sum += i + 1 == rest.without ? 0.0 : probability(x[j].y);
-        sum += i + 2 == rest.without ? 0.0 : probability(x[j].z);
-        sum += i + 3 == rest.without ? 0.0 : probability(x[j].w);
+        sum += weight(i == rest.without ? 0.0f : x[j].x, 0.0f);
+        sum += weight(i + 1 == rest.without ? 0.0f : x[j].y, 0.0f);
+        sum += weight(i + 2 == rest.without ? 0.0f : x[j].z, 0.0f);
+        sum += weight(i + 3 == rest.without ? 0.0f : x[j].w, 0.0f);
       }
     }
   } else {
@@ -134,7 +135,7 @@ __global__ void __launch_bounds__(NT, 2) verify_kernel(VerifyArgs a) {
     bool good = false;
     if (sound(x)) {
       const double p = probability(a.target[r * a.target_stride + x]);
-      const double q = a.draft != nullptr ? probability(a.draft[r * a.draft_stride + x]) : 1.0;
+      const double q = a.draft != nullptr ? probability(a.draft[r * a.draft_stride + x]) : 1.0f;
       good = (double)a.accept[r] * q < p;
     }
     if (!good) mine = i;
@@ -237,7 +238,7 @@ __global__ void __launch_bounds__(NT, 2) verify_kernel(VerifyArgs a) {
             double w[4], sum = 0.0;
 #pragma unroll
             for (int k = 0; k < 4; k++) {
-              w[k] = fmax(probability(x[j][k]) - probability(y[j][k]), 0.0);
+              w[k] = weight(x[j][k], y[j][k]);
               sum += w[k];
               if (w[k] > 0.0) some = i0 + 128 * j + k;
             }
