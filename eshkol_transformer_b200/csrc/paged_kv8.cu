@@ -39,23 +39,29 @@ struct Eight {
   }
 };
 
-// The scale of a row whose largest magnitude is `top`: 448 = 1.75 2^8.
-__device__ __forceinline__ float scale_of_row(float top) {
-  if (top == 0.0f) return 0.0f;
+// The larger magnitude; NaN if either is.
+__device__ __forceinline__ float larger(float a, float b) {
+  float r;
+  asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(fabsf(a)), "f"(fabsf(b)));
+  return r;
+}
+// The scale of a row whose largest magnitude is `top` (448 = 1.75 2^8), and its inverse: a
+// power of two between 2^-126 and 2^120, so exact, and in range; 0 for rows of zeros and
+// rows that are not finite.
+__device__ __forceinline__ float scale_of_row(float top, float& inverse) {
   const uint32_t u = __float_as_uint(top);
-  if (u >= 0x7f800000u) return NAN;
-  const int e = (int)(u >> 23) - 8 + ((u & 0x7fffffu) > 0x600000u ? 1 : 0);  // biased
-  return __uint_as_float((uint32_t)max(e, 1) << 23);
+  const int e = max((int)((u + 0x1fffffu) >> 23) - 8, 1);  // biased; + 1 above 1.75
+  const bool some = top > 0.0f && u < 0x7f800000u;
+  inverse = some ? __uint_as_float((uint32_t)(254 - e) << 23) : 0.0f;
+  return some ? __uint_as_float((uint32_t)e << 23) : top == 0.0f ? 0.0f : NAN;
 }
 __device__ __forceinline__ uint32_t two_e4m3(float low, float high) {
   uint16_t r;
   asm("cvt.rn.satfinite.e4m3x2.f32 %0, %1, %2;" : "=h"(r) : "f"(high), "f"(low));
   return r;
 }
-// The stored elements of 8 values: x / s with s a power of two of at least 2^-126, its
-// inverse exact (2^-120 and less: in range as 448 s is below the largest f32).
-__device__ __forceinline__ uint2 quantised(const float (&x)[8], float scale) {
-  const float inv = scale > 0.0f ? 1.0f / scale : 0.0f;
+// The stored elements of 8 values: x / s.
+__device__ __forceinline__ uint2 quantised(const float (&x)[8], float inv) {
   return make_uint2(two_e4m3(x[0] * inv, x[1] * inv) | two_e4m3(x[2] * inv, x[3] * inv) << 16,
                     two_e4m3(x[4] * inv, x[5] * inv) | two_e4m3(x[6] * inv, x[7] * inv) << 16);
 }
@@ -105,10 +111,17 @@ paged_append8_kernel(Pools P, Scales S, Batch B, Rope R, uint8_t* __restrict__ k
   float cs[4] = {1.0f, 1.0f, 1.0f, 1.0f}, sn[4] = {0.0f, 0.0f, 0.0f, 0.0f};
   if (R.cos != nullptr && d < P.head_dim) {
     const int64_t row = rope_row(R, pos, B.status) * (P.head_dim / 2) + d / 2;
+    if (((reinterpret_cast<uintptr_t>(R.cos) | reinterpret_cast<uintptr_t>(R.sin)) & 15) == 0) {
+      const float4 c = __ldg(reinterpret_cast<const float4*>(R.cos + row));
+      const float4 s = __ldg(reinterpret_cast<const float4*>(R.sin + row));
+      cs[0] = c.x, cs[1] = c.y, cs[2] = c.z, cs[3] = c.w;
+      sn[0] = s.x, sn[1] = s.y, sn[2] = s.z, sn[3] = s.w;
+    } else {
 #pragma unroll
-    for (int j = 0; j < 4; j++) {
-      cs[j] = __ldg(R.cos + row + j);
-      sn[j] = __ldg(R.sin + row + j);
+      for (int j = 0; j < 4; j++) {
+        cs[j] = __ldg(R.cos + row + j);
+        sn[j] = __ldg(R.sin + row + j);
+      }
     }
   }
 #pragma unroll
@@ -116,6 +129,7 @@ paged_append8_kernel(Pools P, Scales S, Batch B, Rope R, uint8_t* __restrict__ k
     const int h = h0 + i * at_once;
     const bool some = h < P.kv_heads && d < P.head_dim;
     float x[8], y[8], top[2] = {0.0f, 0.0f};
+    if (h0 - (lane >> lane_bits) + i * at_once >= P.kv_heads) break;  // for the whole warp
     if (some) {
 #pragma unroll
       for (int j = 0; j < 8; j++) {
@@ -126,28 +140,22 @@ paged_append8_kernel(Pools P, Scales S, Batch B, Rope R, uint8_t* __restrict__ k
 #pragma unroll
         for (int j = 0; j < 4; j++) rotate(x[2 * j], x[2 * j + 1], cs[j], sn[j]);
       }
-      // magnitudes as integers: a NaN is the largest
-      uint32_t m0 = 0, m1 = 0;
 #pragma unroll
       for (int j = 0; j < 8; j++) {
-        m0 = max(m0, __float_as_uint(x[j]) & 0x7fffffffu);
-        m1 = max(m1, __float_as_uint(y[j]) & 0x7fffffffu);
+        top[0] = larger(top[0], x[j]);
+        top[1] = larger(top[1], y[j]);
       }
-      top[0] = __uint_as_float(m0);
-      top[1] = __uint_as_float(m1);
     }
     for (int o = 1; o < lanes; o <<= 1) {
 #pragma unroll
-      for (int j = 0; j < 2; j++) {
-        const uint32_t other = __float_as_uint(__shfl_xor_sync(0xffffffffu, top[j], o));
-        top[j] = __uint_as_float(max(__float_as_uint(top[j]), other));
-      }
+      for (int j = 0; j < 2; j++) top[j] = larger(top[j], __shfl_xor_sync(0xffffffffu, top[j], o));
     }
     if (some) {
-      const float ks = scale_of_row(top[0]), vs = scale_of_row(top[1]);
+      float ki, vi;
+      const float ks = scale_of_row(top[0], ki), vs = scale_of_row(top[1], vi);
       const int64_t e = at.element + h * P.head_stride + d;
-      *reinterpret_cast<uint2*>(keys + e) = quantised(x, ks);
-      *reinterpret_cast<uint2*>(values + e) = quantised(y, vs);
+      *reinterpret_cast<uint2*>(keys + e) = quantised(x, ki);
+      *reinterpret_cast<uint2*>(values + e) = quantised(y, vi);
       if (d == 0) {
         S.keys[at.scale + h * S.head_stride] = ks;
         S.values[at.scale + h * S.head_stride] = vs;
