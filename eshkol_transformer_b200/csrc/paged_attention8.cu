@@ -1027,8 +1027,7 @@ int launch_dim8(const et_b200_paged_cache8_v1* c, Attend8Args& x, int64_t rows, 
     if (rows <= 8) return launch_shape8<T, Shape8<T, DH, 8, 4, 4, 128, 2, 3>>(c, x, ws, stream);
     if (rows <= (sizeof(T) == 2 ? 48 : 64))
       return launch_shape8<T, Shape8<T, DH, 16, 4, 4, 128, 3, 2>>(c, x, ws, stream);
-    if constexpr (sizeof(T) == 2)
-      if (const int blocks = attend8_tc(c, x, ws, stream)) return blocks;
+    if (const int blocks = attend8_tc(c, x, ws, stream)) return blocks;
     return launch_shape8<T, Shape8<T, DH, 64, 4, 1, 64, 2, 2>>(c, x, ws, stream);
   }
 }

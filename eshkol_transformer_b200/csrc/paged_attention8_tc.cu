@@ -39,20 +39,23 @@ constexpr float kJump = 4.0f, kShift = 11.0f;  // weights reach 2^15
 constexpr int RING = 8;  // blocks whose exponents are kept: more than conversion runs ahead
 constexpr int kNone = -1000;  // the exponent of no scale
 
-template <int DH>
+// PAIRS: queries and weights with their residuals (f32)
+template <int DH, bool PAIRS>
 struct Layout {
   static constexpr int SLOT = BK * DH * 2;  // one block of K or V in binary16
   static constexpr int SLOTS = DH == 128 ? 3 : 6;
   static constexpr int RAW = BK * DH;       // one block of K or V in bytes
-  static constexpr int RAWS = DH == 128 ? 4 : 8;
+  static constexpr int RAWS = DH == 128 ? 4 : PAIRS ? 6 : 8;
+  static constexpr int TILE_Q = HALF * DH * 2 * (PAIRS ? 2 : 1);
   static constexpr int Q = SLOTS * SLOT;    // two halves of 128 rows
-  static constexpr int BYTES = Q + 2 * HALF * DH * 2;
+  static constexpr int BYTES = Q + 2 * TILE_Q;
   static constexpr int SCALES = BYTES + RAWS * RAW;  // [block % (RAWS / 2)][keys, values][BK]
   static constexpr int BARS = SCALES + RAWS * BK * 4;
   static constexpr int SMEM = BARS + 512;
-  // TMEM: scores of the halves (P over the first 64 columns), outputs
-  static constexpr uint32_t S0 = 0, O0 = 256, COLS = 512;
-  static_assert(O0 + 2 * DH <= COLS && SMEM <= 232448, "TMEM and shared memory");
+  // TMEM: scores of the halves (P over the first 64 columns, its residual over the others),
+  // outputs, with PAIRS their sums over blocks
+  static constexpr uint32_t S0 = 0, O0 = 256, SUM0 = O0 + 2 * DH, COLS = 512;
+  static_assert(SUM0 + (PAIRS ? 2 * DH : 0) <= COLS && SMEM <= 232448, "TMEM and shared memory");
 };
 
 // Whether `v` holds for all `threads` threads of a named barrier.
@@ -79,7 +82,8 @@ template <typename T, int DH>
 __global__ void __launch_bounds__(THREADS, 1)
 paged_attention8_tc_kernel(const __grid_constant__ CUtensorMap k_map,
                            const __grid_constant__ CUtensorMap v_map, Attend8Args args, int box_rows) {
-  using L = Layout<DH>;
+  constexpr bool PAIRS = sizeof(T) == 4;
+  using L = Layout<DH, PAIRS>;
   constexpr int SLOTS = L::SLOTS, RAWS = L::RAWS, TILE = 2 * HALF;
   const AttendArgs& a = args.a;
   extern __shared__ __align__(1024) uint8_t smem[];
@@ -301,7 +305,7 @@ paged_attention8_tc_kernel(const __grid_constant__ CUtensorMap k_map,
     const int t = warp - MMA_WARP;
     constexpr uint32_t idesc_s = idesc_f16_m128(BK, 0);
     constexpr uint32_t idesc_o = idesc_f16_m128(DH, 1);
-    const uint32_t q = base + L::Q + (uint32_t)t * (HALF * DH * 2);
+    const uint32_t q = base + L::Q + (uint32_t)t * L::TILE_Q;
     const uint32_t s_at = tmem + L::S0 + 128u * t, o_at = tmem + L::O0 + (uint32_t)(DH * t);
     uint32_t count = 0, items = 0, steps = 0, turns = 0;
     bool ok = true;
@@ -316,8 +320,11 @@ paged_attention8_tc_kernel(const __grid_constant__ CUtensorMap k_map,
     auto scores = [&](uint32_t slot) {
       const uint32_t k = base + slot * L::SLOT;
 #pragma unroll
-      for (int i = 0; i < DH / 16; i++)
-        umma_f16(s_at, kdesc16<HALF>(q, i), kdesc16<BK>(k, i), idesc_s, i > 0 ? 1u : 0u);
+      for (int i = 0; i < DH / 16; i++) {
+        if constexpr (PAIRS)
+          umma_f16(s_at, kdesc16<HALF>(q + HALF * DH * 2, i), kdesc16<BK>(k, i), idesc_s, i > 0 ? 1u : 0u);
+        umma_f16(s_at, kdesc16<HALF>(q, i), kdesc16<BK>(k, i), idesc_s, PAIRS || i > 0 ? 1u : 0u);
+      }
       umma_commit(B_(SFULL + t));
     };
     while (ok && left > 0) {
@@ -356,8 +363,15 @@ paged_attention8_tc_kernel(const __grid_constant__ CUtensorMap k_map,
         if (lane == 0) {
           if (rows) {
 #pragma unroll
-            for (int i = 0; i < BK / 16; i++)
-              umma_f16_ts(o_at, s_at + 8u * i, mdesc16<BK>(vt, i), idesc_o, (j > 0 || i > 0) ? 1u : 0u);
+            for (int i = 0; i < BK / 16; i++) {
+              const uint32_t more_of_it = (!PAIRS && j > 0) || i > 0 ? 1u : 0u;
+              if constexpr (PAIRS) {
+                umma_f16_ts(o_at, s_at + 64u + 8u * i, mdesc16<BK>(vt, i), idesc_o, more_of_it);
+                umma_f16_ts(o_at, s_at + 8u * i, mdesc16<BK>(vt, i), idesc_o, 1u);
+              } else {
+                umma_f16_ts(o_at, s_at + 8u * i, mdesc16<BK>(vt, i), idesc_o, more_of_it);
+              }
+            }
             if (more) scores(ks);
             else umma_commit(B_(ODONE + t));
           }
@@ -382,9 +396,11 @@ paged_attention8_tc_kernel(const __grid_constant__ CUtensorMap k_map,
     const int t = warp >> 2, row = tid & (HALF - 1);
     const uint32_t lanes = tmem + ((uint32_t)((warp & 3) * 32) << 16);
     const uint32_t s_at = lanes + L::S0 + 128u * t, o_at = lanes + L::O0 + (uint32_t)(DH * t);
-    const bool q_vec = ((reinterpret_cast<uintptr_t>(a.q) | (uintptr_t)(a.q_stride * 2)) & 15) == 0;
+    const uint32_t sum_at = lanes + L::SUM0 + (uint32_t)(DH * t);
+    constexpr int SIZE = (int)sizeof(T);
+    const bool q_vec = ((reinterpret_cast<uintptr_t>(a.q) | (uintptr_t)(a.q_stride * SIZE)) & 15) == 0;
     const bool rope_vec = ((reinterpret_cast<uintptr_t>(a.rope.cos) | reinterpret_cast<uintptr_t>(a.rope.sin)) & 15) == 0;
-    const bool o_vec = ((reinterpret_cast<uintptr_t>(a.o) | (uintptr_t)(a.o_stride * 2)) & 15) == 0;
+    const bool o_vec = ((reinterpret_cast<uintptr_t>(a.o) | (uintptr_t)(a.o_stride * SIZE)) & 15) == 0;
     uint32_t items = 0, steps = 0, n = 0;
     bool ok = true;
     Cut cut{0, 0, 0, 0, 0};
@@ -410,9 +426,9 @@ paged_attention8_tc_kernel(const __grid_constant__ CUtensorMap k_map,
         // tile is: its instructions have to be fetched each time.
         float row_scale = 0.0f;
         if (live) {
-          constexpr int P = DH / 64;  // 16-byte pieces of a lane
-          const uint32_t tile = base + L::Q + (uint32_t)t * (HALF * DH * 2);
-          union Piece { uint4 v; T x[8]; };
+          constexpr int P = DH / 64;  // 8 dims of a lane
+          const uint32_t tile = base + L::Q + (uint32_t)t * L::TILE_Q;
+          union Piece { uint4 v[SIZE / 2]; T x[8]; };
           Piece u[P], u_next[P];
           float4 cs[P], sn[P], cs_next[P], sn_next[P];
           auto load = [&](int r, Piece (&u)[P], float4 (&cs)[P], float4 (&sn)[P]) {
@@ -426,14 +442,18 @@ paged_attention8_tc_kernel(const __grid_constant__ CUtensorMap k_map,
 #pragma unroll
             for (int i = 0; i < P; i++) {
               const int d = 8 * ((lane & 7) + 8 * i);
-              u[i].v = make_uint4(0, 0, 0, 0);
+#pragma unroll
+              for (int e = 0; e < SIZE / 2; e++) u[i].v[e] = make_uint4(0, 0, 0, 0);
               cs[i] = make_float4(1.f, 1.f, 1.f, 1.f);
               sn[i] = make_float4(0.f, 0.f, 0.f, 0.f);
               if (some && d < dim) {
-                if (q_vec) u[i].v = __ldg(reinterpret_cast<const uint4*>(src + d));
-                else
+                if (q_vec) {
+#pragma unroll
+                  for (int e = 0; e < SIZE / 2; e++) u[i].v[e] = __ldg(reinterpret_cast<const uint4*>(src + d) + e);
+                } else {
 #pragma unroll
                   for (int e = 0; e < 8; e++) u[i].x[e] = src[d + e];
+                }
                 if (tab >= 0) {
                   const float *ct = a.rope.cos + tab + d / 2, *st = a.rope.sin + tab + d / 2;
                   if (rope_vec) {
@@ -482,12 +502,13 @@ paged_attention8_tc_kernel(const __grid_constant__ CUtensorMap k_map,
 #pragma unroll
             for (int i = 0; i < P; i++) {
               const int c = (lane & 7) + 8 * i;
-              sts128(tile + (uint32_t)(c >> 3) * HALF * 128u + (uint32_t)r * 128u +
-                         ((((uint32_t)c & 7u) ^ (uint32_t)(r & 7)) << 4),
-                     make_float4(__uint_as_float(pack2<__half>(y[i][0] * by, y[i][1] * by)),
-                                 __uint_as_float(pack2<__half>(y[i][2] * by, y[i][3] * by)),
-                                 __uint_as_float(pack2<__half>(y[i][4] * by, y[i][5] * by)),
-                                 __uint_as_float(pack2<__half>(y[i][6] * by, y[i][7] * by))));
+              const uint32_t at = tile + (uint32_t)(c >> 3) * HALF * 128u + (uint32_t)r * 128u +
+                                  ((((uint32_t)c & 7u) ^ (uint32_t)(r & 7)) << 4);
+              float hi[4], lo[4];
+#pragma unroll
+              for (int k = 0; k < 4; k++) pair2(y[i][2 * k] * by, y[i][2 * k + 1] * by, hi[k], lo[k]);
+              sts128(at, make_float4(hi[0], hi[1], hi[2], hi[3]));
+              if constexpr (PAIRS) sts128(at + HALF * DH * 2, make_float4(lo[0], lo[1], lo[2], lo[3]));
             }
           }
           fence_async_smem();
@@ -538,23 +559,41 @@ paged_attention8_tc_kernel(const __grid_constant__ CUtensorMap k_map,
             for (int i = 0; i < 32; i++) top[i & 3] = fmaxf(top[i & 3], __uint_as_float(r[c][i]));
           const float bmax = fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3])) * scale;
           const bool jump = bmax > m + kJump || (m == -INFINITY && bmax > -INFINITY);
-          if (__any_sync(0xffffffffu, jump) || grown != 0) {
-            float factor = jump ? ex2(m - bmax) : 1.0f;  // 0 while m is -inf
-            if (jump) {
-              m = bmax;
-              l *= factor;
-            }
+          float factor = jump ? ex2(m - bmax) : 1.0f;  // 0 while m is -inf
+          if (jump) {
+            m = bmax;
+            l *= factor;
+          }
+          factor *= ex2((float)-grown);
+          // the scores' barrier also says that the last P V is complete
+          if constexpr (PAIRS) {
+            // the tensor pipe's f32 accumulation truncates: the products of a block are added to
+            // the sums here (no slower than one accumulator of many blocks; error of prompts of
+            // up to 1,024 tokens 1.0e-6 with eight blocks, 0.6e-6 with one)
             if (j > 0) {
-              factor *= ex2((float)-grown);
-              // the scores' barrier also says that the last P V is complete
+#pragma unroll 1
+              for (int c = 0; c < DH; c += 32) {
+                float o[32], x[32];
+                tmem_ld32(o_at + c, o);
+                if (j > 1) {
+                  tmem_ld32(sum_at + c, x);
 #pragma unroll
-              for (int c = 0; c < DH / 32; c++) {
-                float o[32];
-                tmem_ld32(o_at + 32 * c, o);
+                  for (int i = 0; i < 32; i++) o[i] += x[i];
+                }
 #pragma unroll
                 for (int i = 0; i < 32; i++) o[i] *= factor;
-                tmem_st32(o_at + 32 * c, o);
+                tmem_st32(sum_at + c, o);
               }
+              tmem_wait_st();
+            }
+          } else if (j > 0 && (__any_sync(0xffffffffu, jump) || grown != 0)) {
+#pragma unroll
+            for (int c = 0; c < DH / 32; c++) {
+              float o[32];
+              tmem_ld32(o_at + 32 * c, o);
+#pragma unroll
+              for (int i = 0; i < 32; i++) o[i] *= factor;
+              tmem_st32(o_at + 32 * c, o);
             }
           }
           const float from = (m == -INFINITY ? 0.0f : m) - kShift;
@@ -563,11 +602,12 @@ paged_attention8_tc_kernel(const __grid_constant__ CUtensorMap k_map,
           uint64_t sum[2] = {0, 0};
           auto powers = [&](int c, auto some_masked) {
             float w[16];
+            [[maybe_unused]] float w_lo[16];
 #pragma unroll
             for (int i = 0; i < 16; i++) {
               uint64_t x = fma2(pk(__uint_as_float(r[c][2 * i]), __uint_as_float(r[c][2 * i + 1])),
                                 twice(scale), twice(-from));
-              if (!decltype(some_masked)::value && (i & 3) == 3) {
+              if (!PAIRS && !decltype(some_masked)::value && (i & 3) == 3) {
                 x = power2(x);
               } else {
                 const float2 v = unpk(x);
@@ -575,11 +615,13 @@ paged_attention8_tc_kernel(const __grid_constant__ CUtensorMap k_map,
               }
               sum[i & 1] = add2(sum[i & 1], x);
               const float2 v = unpk(x);
-              w[i] = __uint_as_float(pack2<__half>(v.x, v.y));
+              if constexpr (PAIRS) pair2(v.x, v.y, w[i], w_lo[i]);
+              else w[i] = __uint_as_float(pack2<__half>(v.x, v.y));
             }
             tmem_st16(s_at + 16 * c, w);
+            if constexpr (PAIRS) tmem_st16(s_at + 64 + 16 * c, w_lo);
           };
-          if (masked) {
+          if (masked || PAIRS) {
 #pragma unroll
             for (int c = 0; c < 4; c++) powers(c, std::true_type{});
           } else {
@@ -606,6 +648,12 @@ paged_attention8_tc_kernel(const __grid_constant__ CUtensorMap k_map,
           for (int c = 0; c < DH; c += 32) {
             float o[32];
             tmem_ld32(o_at + c, o);
+            if (PAIRS && nb > 1) {
+              float x[32];
+              tmem_ld32(sum_at + c, x);
+#pragma unroll
+              for (int i = 0; i < 32; i++) o[i] += x[i];
+            }
             if (!valid) continue;
 #pragma unroll
             for (int i = 0; i < 32; i++) o[i] = o[i] * f0 * f1;
@@ -613,13 +661,16 @@ paged_attention8_tc_kernel(const __grid_constant__ CUtensorMap k_map,
 #pragma unroll
               for (int i = 0; i < 32; i += 8) {
                 if (c + i >= dim) break;
-                union { uint4 v; uint32_t w[4]; T x[8]; } u;
+                union { uint4 v[SIZE / 2]; T x[8]; } u;
 #pragma unroll
-                for (int k = 0; k < 4; k++) u.w[k] = pack2<T>(o[i + 2 * k], o[i + 2 * k + 1]);
-                if (o_vec) *reinterpret_cast<uint4*>(dst + c + i) = u.v;
-                else
+                for (int k = 0; k < 8; k++) u.x[k] = from_f32<T>(o[i + k]);
+                if (o_vec) {
+#pragma unroll
+                  for (int k = 0; k < SIZE / 2; k++) reinterpret_cast<uint4*>(dst + c + i)[k] = u.v[k];
+                } else {
 #pragma unroll
                   for (int k = 0; k < 8; k++) dst[c + i + k] = u.x[k];
+                }
               }
             } else {
 #pragma unroll
@@ -654,7 +705,7 @@ paged_attention8_tc_kernel(const __grid_constant__ CUtensorMap k_map,
 
 template <typename T, int DH>
 int launch_tc8(const et_b200_paged_cache8_v1* c, Attend8Args& x, void* ws, cudaStream_t stream) {
-  using L = Layout<DH>;
+  using L = Layout<DH, sizeof(T) == 4>;
   AttendArgs& a = x.a;
   const int box_rows = (int)(c->page_size < BK ? c->page_size : BK);
   CUtensorMap k_map, v_map;
@@ -678,7 +729,9 @@ int launch_tc8(const et_b200_paged_cache8_v1* c, Attend8Args& x, void* ws, cudaS
 namespace paged {
 
 int attend8_tc(const et_b200_paged_cache8_v1* c, Attend8Args& x, void* ws, cudaStream_t stream) {
-  if (c->dtype == ET_B200_DTYPE_F32 || c->head_dim > 128) return 0;
+  // at f32 the sums over blocks need the tensor memory that 128 dims would take
+  if (c->head_dim > (c->dtype == ET_B200_DTYPE_F32 ? 64 : 128)) return 0;
+  if (c->dtype == ET_B200_DTYPE_F32) return launch_tc8<float, 64>(c, x, ws, stream);
   if (c->dtype == ET_B200_DTYPE_F16)
     return c->head_dim <= 64 ? launch_tc8<__half, 64>(c, x, ws, stream)
                              : launch_tc8<__half, 128>(c, x, ws, stream);
