@@ -39,7 +39,6 @@ struct VerifyArgs {
   int* status;
   int64_t tokens, target_stride, draft_stride;
   int n, segs;  // tokens of the vocabulary, its segments
-  bool vec;     // rows can be read in 16-byte pieces
 };
 
 // A probability as the rules read it: NaN and negative ones are 0, the largest is 1.
@@ -55,9 +54,6 @@ struct Rest {
   const float* p;
   const float* q;  // or null
   int without;     // a token of weight 0 (a proposal made without chance), or -1
-  __device__ __forceinline__ double at(int i) const {
-    return weight(i == without ? 0.0f : p[i], q != nullptr ? q[i] : 0.0f);
-  }
 };
 
 __device__ __forceinline__ double warp_total(double v) {
@@ -66,43 +62,28 @@ __device__ __forceinline__ double warp_total(double v) {
   return v;
 }
 
-// The weights of segment s, added up by a warp.
+// The weights of segment s, added up by a warp: whole lines whatever the rows' alignment
+// (an odd vocabulary has rows at every multiple of 4 bytes), 16 loads of a lane and row out
+// together.
 __device__ double segment(const VerifyArgs& a, const Rest& rest, int s) {
-  const int lane = threadIdx.x & 31, i0 = s * SEG;
+  constexpr int J = 16;
+  const int lane = threadIdx.x & 31;
   double sum = 0.0;
-  if (a.vec && i0 + SEG <= a.n) {
-    constexpr int J = SEG / 128;
-    float4 x[J], y[J];
+#pragma unroll 1
+  for (int i0 = s * SEG + lane; i0 < (s + 1) * SEG && i0 - lane < a.n; i0 += 32 * J) {
+    float x[J], y[J];
 #pragma unroll
-    for (int j = 0; j < J; j++) x[j] = __ldcs(reinterpret_cast<const float4*>(rest.p + i0) + lane + 32 * j);
-    if (rest.q != nullptr) {
-#pragma unroll
-      for (int j = 0; j < J; j++) y[j] = __ldcs(reinterpret_cast<const float4*>(rest.q + i0) + lane + 32 * j);
-#pragma unroll
-      for (int j = 0; j < J; j++) {
-        sum += weight(x[j].x, y[j].x);
-        sum += weight(x[j].y, y[j].y);
-        sum += weight(x[j].z, y[j].z);
-        sum += weight(x[j].w, y[j].w);
-      }
-    } else {
-#pragma unroll
-      for (int j = 0; j < J; j++) {
-        const int i = i0 + 4 * (lane + 32 * j);
-        sum += weight(i == rest.without ? 0.0f : x[j].x, 0.0f);
-        sum += weight(i + 1 == rest.without ? 0.0f : x[j].y, 0.0f);
-        sum += weight(i + 2 == rest.without ? 0.0f : x[j].z, 0.0f);
-        sum += weight(i + 3 == rest.without ? 0.0f : x[j].w, 0.0f);
-      }
+    for (int j = 0; j < J; j++) {
+      const int i = i0 + 32 * j;
+      x[j] = i < a.n && i != rest.without ? __ldcs(rest.p + i) : 0.0f;
     }
-  } else {
-    // the same tokens per lane in the same order, so that sums do not depend on alignment
-    for (int j = 0; j < SEG / 128; j++)
 #pragma unroll
-      for (int k = 0; k < 4; k++) {
-        const int i = i0 + 4 * (lane + 32 * j) + k;
-        if (i < a.n) sum += rest.at(i);
-      }
+    for (int j = 0; j < J; j++) {
+      const int i = i0 + 32 * j;
+      y[j] = rest.q != nullptr && i < a.n ? __ldcs(rest.q + i) : 0.0f;
+    }
+#pragma unroll
+    for (int j = 0; j < J; j++) sum += weight(x[j], y[j]);
   }
   return warp_total(sum);
 }
@@ -329,11 +310,9 @@ extern "C" int32_t et_b200_verify_v1(const et_b200_verification_v1* s, const flo
         !aligned_to(4, s->accept_uniform, s->draw_uniform, s->status, target, draft))
       return set_error(e, ET_KERNEL_ERROR_INVALID_ARGUMENT, ET_KERNEL_CODE_INVALID_BUFFER, op,
                        "arrays must be aligned to their elements");
-    VerifyArgs a{target, draft, s->offsets, s->drafts, s->accept_uniform, s->draw_uniform, ids,
+    const VerifyArgs a{target, draft, s->offsets, s->drafts, s->accept_uniform, s->draw_uniform, ids,
                  accepted, s->status, s->tokens, s->target_stride, s->draft_stride,
-                 (int)s->vocabulary, (int)((s->vocabulary + SEG - 1) / SEG), false};
-    a.vec = aligned_to(16, target, draft) && s->target_stride % 4 == 0 &&
-            (draft == nullptr || s->draft_stride % 4 == 0);
+                 (int)s->vocabulary, (int)((s->vocabulary + SEG - 1) / SEG)};
     const cudaError_t status = launch_verify(a, s->batch, static_cast<cudaStream_t>(stream));
     if (status != cudaSuccess) return cuda_error(e, status, op);
   }
