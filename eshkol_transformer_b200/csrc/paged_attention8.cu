@@ -319,12 +319,15 @@ __device__ void load_queries(const AttendArgs& a, const Place& p, uint8_t* smem)
   }
 }
 
-// A value's scale b = 2^x c as (x, c), c below 2.
+// A value's scale b = 2^x c as (x, c), c below 2 (0 for a scale that is not finite).
 __device__ __forceinline__ void scale_parts(float b, float& x, float& c) {
-  const int e = min((int)(__float_as_uint(b) >> 23) & 255, 253);
-  x = (float)(e - 127);
-  c = b * __uint_as_float((uint32_t)(254 - e) << 23);
+  const int e = (int)(__float_as_uint(b) >> 23) & 255, top = min(e, 253);
+  x = (float)(top - 127);
+  c = e == 255 ? 0.0f : b * __uint_as_float((uint32_t)(254 - top) << 23);
 }
+// The scale of a key's scores: NaN if either of its scales is not finite, so that the row
+// makes NaN of the queries that see it, and of no other.
+__device__ __forceinline__ float key_scale(float k, float v) { return fmaf(k + v, 0.0f, k); }
 // The running maximum m of s, `big` of s + x, sum l and exponent D of a row of queries, and
 // their change by a block whose maxima are top and tob.
 struct RowState {
@@ -517,7 +520,7 @@ few8_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_constant__ C
         for (int h = 0; h < 2; h++) {  // key g, key g + 8
           const int in = wk * KW + 16 * k + 8 * h + g;
           scale_parts(in < valid ? vs_s[in] : 0.0f, xv[k][h], cv[k][h]);
-          const float ks = ks_s[in];
+          const float ks = key_scale(ks_s[in], vs_s[in]);
 #pragma unroll
           for (int n = 0; n < NQ; n++)
 #pragma unroll
@@ -853,8 +856,9 @@ many8_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_constant__ 
 #pragma unroll
       for (int i = 0; i < BK / 8; i++) {
         const int in = 8 * i + 2 * (lane & 3);
-        const float2 ks = *reinterpret_cast<const float2*>(ks_s + in);
+        float2 ks = *reinterpret_cast<const float2*>(ks_s + in);
         const float2 vb = *reinterpret_cast<const float2*>(vs_s + in);
+        ks = make_float2(key_scale(ks.x, vb.x), key_scale(ks.y, vb.y));
         float xv[2], c;
         scale_parts(in < valid ? vb.x : 0.0f, xv[0], c);
         scale_parts(in + 1 < valid ? vb.y : 0.0f, xv[1], c);

@@ -38,6 +38,7 @@ static_assert(256 * kWideRegs + 128 * (kLeanRegs + kConvertRegs) <= THREADS * 12
 constexpr float kJump = 4.0f, kShift = 11.0f;  // weights reach 2^15
 constexpr int RING = 8;  // blocks whose exponents are kept: more than conversion runs ahead
 constexpr int kNone = -1000;  // the exponent of no scale
+constexpr int kMarked = 4096;  // added to E of a block with keys that make NaN
 
 // PAIRS: queries and weights with their residuals (f32)
 template <int DH, bool PAIRS>
@@ -95,10 +96,10 @@ paged_attention8_tc_kernel(const __grid_constant__ CUtensorMap k_map,
   const uint32_t bar0 = smem_u32(bars);
   auto B_ = [&](int i) { return bar0 + 8u * (uint32_t)i; };
   int* exps = reinterpret_cast<int*>(bars + NBARS);  // [RING][E, F]
-  int* found = exps + 2 * RING;                      // [E, F][4 warps]
-  uint32_t* tslot = reinterpret_cast<uint32_t*>(found + 8);
+  int* found = exps + 2 * RING;                      // [E, F, NaN][4 warps]
+  uint32_t* tslot = reinterpret_cast<uint32_t*>(found + 12);
   int* abort_word = reinterpret_cast<int*>(tslot + 1);
-  static_assert(NBARS * 8 + (2 * RING + 8 + 2) * 4 <= 512, "room behind the tiles");
+  static_assert(NBARS * 8 + (2 * RING + 12 + 2) * 4 <= 512, "room behind the tiles");
   volatile int* abort = abort_word;
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const uint32_t base = smem_u32(smem);
@@ -171,14 +172,18 @@ paged_attention8_tc_kernel(const __grid_constant__ CUtensorMap k_map,
         uint32_t* factors = reinterpret_cast<uint32_t*>(scales_s + n % (RAWS / 2) * 2 * BK);
         int e[2];
         float s[2];
+        bool bad = false;
 #pragma unroll
         for (int i = 0; i < 2; i++) {
           s[i] = c < valid ? __uint_as_float(factors[i * BK + c]) : 0.0f;
           const int x = (int)(__float_as_uint(s[i]) >> 23) & 255;
-          e[i] = s[i] == 0.0f ? kNone : min(max(x, 1) - 127, 126);
+          bad |= x == 255;
+          e[i] = s[i] == 0.0f || x == 255 ? kNone : min(max(x, 1) - 127, 126);
           const int top = __reduce_max_sync(0xffffffffu, e[i]);
           if (lane == 0) found[4 * i + (warp & 3)] = top;
         }
+        const bool any = __any_sync(0xffffffffu, bad);
+        if (lane == 0) found[8 + (warp & 3)] = any;
         live = named_all(1, 128, ok);
         if (!live) break;
 #pragma unroll
@@ -186,14 +191,15 @@ paged_attention8_tc_kernel(const __grid_constant__ CUtensorMap k_map,
         if (e[0] == kNone) e[0] = 0;
         high = max(high, e[1]);
         e[1] = high == kNone ? 0 : high;
-        // in place of the scales: their products, as pairs of binary16
+        // in place of the scales: their products, as pairs of binary16.  A key with a scale that
+        // is not finite makes NaN of its scores, which those that do not see it drop.
 #pragma unroll
         for (int i = 0; i < 2; i++) {
-          const __half2 f = __float2half2_rn(s[i] * exp2_int(-e[i]) * 64.0f);
+          const __half2 f = __float2half2_rn(bad ? (i == 0 ? NAN : 0.0f) : s[i] * exp2_int(-e[i]) * 64.0f);
           factors[i * BK + c] = *reinterpret_cast<const uint32_t*>(&f);
         }
         if (c == 0) {
-          exps[2 * (n % RING)] = e[0];
+          exps[2 * (n % RING)] = e[0] + ((found[8] | found[9] | found[10] | found[11]) ? kMarked : 0);
           exps[2 * (n % RING) + 1] = e[1];
           mbar_arrive(B_(EXPS + n % RING));
         }
@@ -524,7 +530,9 @@ paged_attention8_tc_kernel(const __grid_constant__ CUtensorMap k_map,
           ok = wait(SFULL + t, steps);
           if (ok) ok = wait(EXPS + at, (n + j) / RING);
           // no less than the least normal number: 0 times a masked score is NaN
-          const float scale = fmaxf(times_power(row_scale, exps[2 * at] - 6), 0x1p-126f);
+          const int e = exps[2 * at];
+          const bool marked = e > kMarked / 2;
+          const float scale = fmaxf(times_power(row_scale, e - 6 - (marked ? kMarked : 0)), 0x1p-126f);
           const int now = exps[2 * at + 1], grown = j > 0 ? now - high : 0;
           high = now;
           ok = __all_sync(0xffffffffu, ok);
@@ -598,7 +606,7 @@ paged_attention8_tc_kernel(const __grid_constant__ CUtensorMap k_map,
           }
           const float from = (m == -INFINITY ? 0.0f : m) - kShift;
           // a quarter of the exponentials on the FMA pipe (as in paged_attention_tc.cu);
-          // blocks with masked scores (-inf) all on the special function unit
+          // blocks with masked scores (-inf) or NaN all on the special function unit
           uint64_t sum[2] = {0, 0};
           auto powers = [&](int c, auto some_masked) {
             float w[16];
@@ -621,7 +629,7 @@ paged_attention8_tc_kernel(const __grid_constant__ CUtensorMap k_map,
             tmem_st16(s_at + 16 * c, w);
             if constexpr (PAIRS) tmem_st16(s_at + 64 + 16 * c, w_lo);
           };
-          if (masked || PAIRS) {
+          if (masked || marked || PAIRS) {
 #pragma unroll
             for (int c = 0; c < 4; c++) powers(c, std::true_type{});
           } else {
@@ -647,6 +655,7 @@ paged_attention8_tc_kernel(const __grid_constant__ CUtensorMap k_map,
 #pragma unroll 1
           for (int c = 0; c < DH; c += 32) {
             float o[32];
+            __syncwarp();
             tmem_ld32(o_at + c, o);
             if (PAIRS && nb > 1) {
               float x[32];

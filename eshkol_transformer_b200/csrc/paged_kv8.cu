@@ -60,8 +60,9 @@ __device__ __forceinline__ uint32_t two_e4m3(float low, float high) {
   asm("cvt.rn.satfinite.e4m3x2.f32 %0, %1, %2;" : "=h"(r) : "f"(high), "f"(low));
   return r;
 }
-// The stored elements of 8 values: x / s.
-__device__ __forceinline__ uint2 quantised(const float (&x)[8], float inv) {
+// The stored elements of 8 values: x / s; zeros under the scale NaN.
+__device__ __forceinline__ uint2 quantised(const float (&x)[8], float s, float inv) {
+  if (s != s) return make_uint2(0, 0);
   return make_uint2(two_e4m3(x[0] * inv, x[1] * inv) | two_e4m3(x[2] * inv, x[3] * inv) << 16,
                     two_e4m3(x[4] * inv, x[5] * inv) | two_e4m3(x[6] * inv, x[7] * inv) << 16);
 }
@@ -154,8 +155,8 @@ paged_append8_kernel(Pools P, Scales S, Batch B, Rope R, uint8_t* __restrict__ k
       float ki, vi;
       const float ks = scale_of_row(top[0], ki), vs = scale_of_row(top[1], vi);
       const int64_t e = at.element + h * P.head_stride + d;
-      *reinterpret_cast<uint2*>(keys + e) = quantised(x, ki);
-      *reinterpret_cast<uint2*>(values + e) = quantised(y, vi);
+      *reinterpret_cast<uint2*>(keys + e) = quantised(x, ks, ki);
+      *reinterpret_cast<uint2*>(values + e) = quantised(y, vs, vi);
       if (d == 0) {
         S.keys[at.scale + h * S.head_stride] = ks;
         S.values[at.scale + h * S.head_stride] = vs;

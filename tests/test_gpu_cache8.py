@@ -205,6 +205,50 @@ def test_append_of_extreme_rows(lib, cuda, dtype):
     assert torch.isnan(s.o[39].float()).any()
 
 
+@pytest.mark.parametrize("dtype,n,m,q_heads,heads,dim,page", [
+    (F32, 1, 300, 4, 2, 64, 16), (BF16, 1, 5000, 16, 2, 128, 64), (F16, 5, 700, 6, 2, 80, 24),
+    (BF16, 12, 900, 4, 2, 256, 16), (F16, 40, 900, 6, 3, 256, 16), (F32, 60, 400, 4, 2, 128, 16),
+    (BF16, 200, 1500, 4, 2, 128, 16), (F16, 300, 300, 8, 2, 64, 8), (F32, 150, 700, 4, 2, 64, 32),
+    (BF16, 200, 500, 4, 2, 128, 24)])
+@pytest.mark.parametrize("where", ["new", "old"])
+def test_rows_that_are_not_finite_reach_the_queries_that_see_them_alone(lib, cuda, dtype, n, m, q_heads,
+                                                                        heads, dim, page, where):
+    """One row of keys, another of values, of head 0 that hold an infinity or a NaN: NaN for the
+    queries of that head from the first of their positions on, nothing for all others."""
+    s = Step8([(n, m)], q_heads, heads, dim, page, dtype, spare=0)
+    s.attend()
+    sound = s.o.clone().double()
+    # positions 6 and 7 of eight, where exponentials may take another pipe
+    first = m - 1 if where == "new" and n == 1 else m - n // 2 if where == "new" else (m - n) // 2 // 8 * 8 + 6
+    if where == "old" and m == n:
+        first = 6
+    bad = Step8([(n, m)], q_heads, heads, dim, page, dtype, spare=0)
+    # a step that stores non-finite rows at `first` and behind it
+    x = torch.ones(2, heads, dim, device="cuda").to(dtype)
+    for i, at in enumerate((first, min(first + 1, m - 1))):
+        k, v = x[:1].clone(), x[:1].clone()
+        (k if i == 0 else v)[0, 0, 3] = math.inf if i == 0 else math.nan
+        keep = [p.clone() for p in pools_of(bad)]
+        one = paged.PagedBatch(torch.tensor([0, 1], device="cuda"), torch.tensor([at + 1], device="cuda"),
+                               bad.table, 1, 1, None, bad.status)
+        bad.cache.append(one, k, v)
+        page_at, slot = bad.slots(0, at, at + 1)
+        for p, q in zip(pools_of(bad), keep):  # the other heads keep their rows
+            p[page_at, 1:, slot] = q[page_at, 1:, slot]
+    bad.attend()
+    torch.cuda.synchronize()
+    assert int(bad.status) == 0
+    seen = max(0, first - (m - n))
+    group = q_heads // heads
+    got = bad.o.double()
+    assert torch.isnan(got[seen:, :group]).all()
+    # a weight is rounded to 11 bits at most, from exponentials of either pipe (2^-18), the
+    # output to its type: two runs differ by twice that
+    most = max(float(r.abs().max()) for r in s.v)
+    for a, b in ((got[:seen], sound[:seen]), (got[:, group:], sound[:, group:])):
+        assert ((a - b).abs() <= (2.0 ** -10 + 2.0 ** -17) * most + 2 * U[dtype] * b.abs()).all()
+
+
 def test_append_records_bad_metadata(lib, cuda):
     for change, bit in (("length", paged.BAD_LENGTH), ("offset", paged.BAD_OFFSET), ("page", paged.BAD_PAGE),
                         ("rope", paged.BAD_ROPE)):
