@@ -1446,6 +1446,15 @@ int32_t check_shape(const et_b200_sampling_v1* s, et_kernel_error* e, const char
                      "rows, vocabulary or row stride are outside their limits");
   return 0;
 }
+// Whether rows of a and of b share memory (rows of different steps: whether their spans do).
+bool rows_meet(const void* a, int64_t a_step, int64_t a_bytes, const void* b, int64_t b_step,
+               int64_t b_bytes, int64_t rows) {
+  const int64_t x = (int64_t)reinterpret_cast<uintptr_t>(a), y = (int64_t)reinterpret_cast<uintptr_t>(b);
+  if (x + (rows - 1) * a_step + a_bytes <= y || y + (rows - 1) * b_step + b_bytes <= x) return false;
+  if (rows == 1 || a_step != b_step) return true;
+  const int64_t apart = ((y - x) % a_step + a_step) % a_step;
+  return apart < a_bytes || apart + b_bytes > a_step;
+}
 int32_t check_rows(const et_b200_sampling_v1* s, const void* logits, et_kernel_error* e,
                    const char* op) {
   if (!paged::aligned_to(s->dtype == ET_B200_DTYPE_F32 ? 4 : 2, logits) ||
@@ -1499,6 +1508,11 @@ extern "C" int32_t et_b200_probabilities_v1(const et_b200_sampling_v1* s, const 
     if (!paged::aligned_to(4, probs))
       return set_error(e, ET_KERNEL_ERROR_INVALID_ARGUMENT, ET_KERNEL_CODE_INVALID_BUFFER, op,
                        "probabilities must be aligned to their elements");
+    const int64_t size = s->dtype == ET_B200_DTYPE_F32 ? 4 : 2;
+    if (rows_meet(logits, s->row_stride * size, s->vocabulary * size, probs, probs_stride * 4,
+                  s->vocabulary * 4, s->rows))
+      return set_error(e, ET_KERNEL_ERROR_INVALID_ARGUMENT, ET_KERNEL_CODE_INVALID_BUFFER, op,
+                       "probabilities are written while logits are read: they must not overlap");
     const Args a{nullptr, s->temperature, s->top_k, s->top_p, s->min_p, nullptr, nullptr, probs,
                  s->row_stride, probs_stride, (int)s->vocabulary, 0};
     const cudaError_t status =

@@ -284,8 +284,8 @@ typedef struct et_b200_paged_cache8_v1 {
  * the keys rotated in f32) the scale s is the least power of two with |x| <= 448 s
  * for every element (no less than 2^-126; 0 for a row of zeros), and the stored
  * elements are x / s rounded to the nearest, ties to even.  A row that holds an
- * infinity or a NaN gets the scale NaN, which the attention hands on to every query
- * that sees the row. */
+ * infinity or a NaN gets the scale NaN and elements of 0.  Two requests that own the
+ * same slot race. */
 int32_t et_b200_paged_append8_v1(const et_b200_paged_cache8_v1 *cache,
                                  const et_b200_paged_batch_v1 *batch,
                                  const et_b200_paged_rope_v1 *rope,
@@ -293,15 +293,21 @@ int32_t et_b200_paged_append8_v1(const et_b200_paged_cache8_v1 *cache,
                                  int64_t v_stride, void *stream,
                                  et_kernel_error *error);
 
-/* et_b200_paged_attention_v1 over a cache of 8 bits.  Elements and products with
- * scales that are powers of two (or 0), as the append writes them, are exact;
- * other finite scales round rows to 11 bits where a chunk of f16 or bf16 queries is
- * computed (more than 16 query rows per kv head).  q' is carried as binary16 of a
- * scale per row: at f32 and, up to 16 rows, at f16 with its residual (about 22
- * bits); the probabilities as binary16, at f32 with their residual.  Above 16 rows
- * at f16 and bf16, rows of a block of 128 keys (of the keys), or behind the
- * largest so far (of the values), whose scale is less than 2^-21 of the largest
- * one's lose bits. */
+/* et_b200_paged_attention_v1 over a cache of 8 bits, by the same rules but for these.
+ * Finite scales are at most 2^126.  A row whose keys' or values' scale is not
+ * finite makes NaN of o for every query that sees it (whose lse is then
+ * unspecified) and of no other; elements must not be NaN, those hidden from a query
+ * included.
+ * Precision: scores, statistics and sums are f32.  q' is carried as binary16 of a
+ * scale per row, at f32 and f16 with its residual (about 22 bits; at f16 not in the
+ * chunks below); the probabilities as binary16, at f32 with their residual.
+ * Elements and their products with scales that are powers of two (or 0), as the
+ * append writes them, are exact.  Chunks (more than 48 query rows per kv head, as
+ * max_new tells, and head_dim up to 128 at f16 and bf16, more than 64 rows and
+ * head_dim up to 64 at f32) over pages of a power of two of at least 8 slots whose scales lie side by
+ * side round other scales' products to 11 bits; there, rows of a block of 128 keys (of the
+ * keys), or behind the largest so far (of the values), whose scale is less than
+ * 2^-21 of the largest one's lose bits. */
 size_t et_b200_paged_attention8_workspace_bytes_v1(
     const et_b200_paged_cache8_v1 *cache, int64_t q_heads);
 int32_t et_b200_paged_attention8_v1(const et_b200_paged_cache8_v1 *cache,
@@ -351,7 +357,7 @@ int32_t et_b200_sample_v1(const et_b200_sampling_v1 *shape, const void *logits,
  * below 2^-36 of the likeliest count as 0, as there; others are f32 (not fixed
  * point), so probabilities are right to some 2^-22 of themselves however small.  A
  * row that takes the most likely token gets a single 1, a row without a token to
- * draw only zeros. */
+ * draw only zeros.  probs must not overlap the logits. */
 int32_t et_b200_probabilities_v1(const et_b200_sampling_v1 *shape,
                                  const void *logits, float *probs,
                                  int64_t probs_stride, void *stream,
@@ -368,10 +374,11 @@ int32_t et_b200_probabilities_v1(const et_b200_sampling_v1 *shape,
  * accept_uniform[r] q_r(x) < p_r(x); at the first that is not, the request's token
  * is drawn from max(p_r - q_r, 0), and behind its last accepted proposal from p_r of
  * the last row: the first token, in vocabulary order, whose running sum exceeds
- * draw_uniform[b] times the total.  Products, differences and sums are formed in 64
- * bits, in an order that depends on the vocabulary alone.  ids[r] receives the
- * accepted proposals, then the drawn token, then -1; accepted[b] the number of
- * accepted proposals (0 for a request without rows).
+ * draw_uniform[b] times the total.  Differences are f32, products
+ * and sums are formed in 64 bits, in an order that depends on the vocabulary alone.
+ * ids[r] receives the accepted proposals, then the drawn token, then -1 (ids may be
+ * drafts); accepted[b] the number of accepted proposals (0 for a request without
+ * rows).
  * Probabilities count as 0 where they are NaN or negative and as 1 above 1;
  * accept_uniform is meant in [0, 1) (a NaN accepts nothing), draw_uniform too
  * (other values act as the nearest end).  A proposal outside the vocabulary is

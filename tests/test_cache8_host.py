@@ -85,7 +85,7 @@ def test_empty_steps_do_nothing(lib):
         assert attend(lib, cache(), b, q=None, o=None, ws=None, size=0)[0] == 0
 
 
-def probabilities(lib, logits=FAKE, probs=FAKE, stride=100, **change):
+def probabilities(lib, logits=FAKE, probs=FAKE + (1 << 20), stride=100, **change):
     d = dict(struct_size=C.sizeof(sampling.SamplingDescriptor), rows=2, vocabulary=100,
              row_stride=100, dtype=0, reserved=0, temperature=None, top_k=None, top_p=None,
              min_p=None)
@@ -104,6 +104,15 @@ def test_bad_distributions_are_refused(lib):
         assert rc != 0 and err.message, kw
     assert lib.et_b200_probabilities_v1(None, FAKE, FAKE, 100, None, None) != 0
     assert probabilities(lib, rows=0, logits=None, probs=None)[0] == 0
+
+
+def test_distributions_over_their_logits_are_refused(lib):
+    """Zeros go out while logits are read: no byte of a row may belong to both."""
+    for kw in (dict(probs=FAKE), dict(probs=FAKE + 4), dict(probs=FAKE + 4 * 199), dict(probs=FAKE - 4 * 99),
+               dict(probs=FAKE + 400, row_stride=150, stride=150), dict(probs=FAKE + 400, row_stride=200),
+               dict(probs=FAKE, dtype=1), dict(probs=FAKE, rows=1)):
+        rc, err = probabilities(lib, **kw)
+        assert rc != 0 and b"overlap" in err.message, kw
 
 
 def verify(lib, target=FAKE, draft=FAKE, ids=FAKE, accepted=FAKE, **change):

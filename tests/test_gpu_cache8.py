@@ -460,6 +460,64 @@ def test_attention_beyond_32_bits(lib, cuda):
     assert torch.equal(pool[0][where, :, slot], bits) and torch.equal(scale[0][where, :, slot], sc)
 
 
+@pytest.mark.parametrize("dtype,n", [(F32, 1), (BF16, 7), (F16, 90), (F32, 90)])
+def test_pools_inside_one_tensor(lib, cuda, dtype, n):
+    """Keys and values of all layers side by side in one tensor, as views of torch's own type:
+    the same bits as in pools of their own, nothing else touched."""
+    s = Step8([(n, 200), (n, n), (0, 9)], 4, 2, 64, 16, dtype)
+    k, v = [torch.randn(s.tokens, 2, 64, device="cuda").to(dtype) for _ in range(2)]
+    pages = s.keys.shape[0]
+    every = torch.full((pages, 3, 2, 2, 16, 64), 0x11, device="cuda", dtype=torch.uint8)
+    scales = torch.full((pages, 3, 2, 2, 16), 5.0, device="cuda")
+    every[:, 1, 0], every[:, 1, 1], scales[:, 1, 0], scales[:, 1, 1] = pools_of(s)
+    inside = paged.PagedCache8(*every.view(torch.float8_e4m3fn)[:, 1].unbind(1), *scales[:, 1].unbind(1), dtype)
+    o, lse = s.o.clone(), s.lse.clone()
+    rope = (s.cos, s.sin)
+    inside.append(s.batch(), k, v, rope)
+    paged.PagedAttention(inside, 4).forward(s.batch(), s.q, o, rope, lse)
+    s.cache.append(s.batch(), k, v, rope)
+    s.attend()
+    torch.cuda.synchronize()
+    assert int(s.status) == 0
+    for a, b in zip((every[:, 1, 0], every[:, 1, 1], scales[:, 1, 0], scales[:, 1, 1]), pools_of(s)):
+        assert same(a, b)
+    assert torch.equal(o, s.o) and torch.equal(lse, s.lse)
+    for layer in (0, 2):
+        assert (every[:, layer] == 0x11).all() and (scales[:, layer] == 5.0).all()
+
+
+@pytest.mark.parametrize("dtype,group,new", [(BF16, 1, 1), (F32, 4, 3), (F16, 2, 30), (F32, 2, 40)])
+def test_many_requests_of_all_lengths(lib, cuda, dtype, group, new):
+    """More requests than thread blocks, some without tokens, some without keys, some with more
+    new tokens than they keep."""
+    lengths = [(i * 37) % 131 for i in range(700)]
+    requests = [(0 if i % 11 == 3 else 1 + i % new, m) for i, m in enumerate(lengths)]
+    s = Step8(requests, 2 * group, 2, 32, 8, dtype)
+    s.attend()
+    torch.cuda.synchronize()
+    assert int(s.status) == 0
+    whole, lse = s.o.clone(), s.lse.clone()
+    # some of them against 64 bits and against steps of their own
+    first = 0
+    for b, (n, m) in enumerate(requests):
+        if b % 29 == 0 and n:
+            at = torch.arange(m - n, m, device="cuda").clamp_min(0)
+            o, want, _, _ = attention(turn(s.q[first:first + n].double(), s.cos[at], s.sin[at]), s.k[b], s.v[b], m - n)
+            most = float(s.v[b].abs().max()) if m else 0.0
+            assert torch.equal(torch.isinf(lse[first:first + n]), torch.isinf(want))
+            assert ((whole[first:first + n].double() - o).abs() <= 2.0 ** -6 * (most + 1e-3)).all()
+            one = paged.PagedBatch(torch.tensor([0, n], device="cuda"), s.lengths[b:b + 1], s.table[b:b + 1], n,
+                                   new, None, s.status)
+            part, part_lse = torch.empty_like(whole[first:first + n]), torch.empty_like(lse[first:first + n])
+            paged.PagedAttention(s.cache, s.q_heads).forward(one, s.q[first:first + n], part, (s.cos, s.sin), part_lse)
+            torch.cuda.synchronize()
+            # the same products in other divisions: weights rounded to 11 bits at worst
+            assert ((part.double() - whole[first:first + n].double()).abs() <=
+                    2.0 ** -9 * most + 2 * U[dtype] * part.double().abs()).all()
+        first += n
+    assert (whole[s.used:] == 7.0).all()
+
+
 def test_graphs_streams_and_workspaces(lib, cuda):
     """Captured steps follow the contents of their buffers, two graphs with their own
     workspaces replay side by side, and a workspace may hold anything."""

@@ -125,6 +125,22 @@ def test_distributions_strides(lib, cuda, kw):
             assert (out == 7.0).all()
 
 
+@pytest.mark.parametrize("kw", [dict(), dict(top_k=20), dict(temperature=0.0)], ids=str)
+def test_distributions_beside_their_logits(lib, cuda, kw):
+    """Rows of logits and of probabilities that alternate in one tensor share no byte; in place
+    they would, and are refused."""
+    x = logits_of(5, 1003, F32, 3)
+    both = torch.full((5, 2 * 1003), 7.0, device="cuda")
+    both[:, :1003] = x
+    got = distributions(both[:, :1003], both[:, 1003:], **kw)
+    want = distributions(x, **kw)
+    torch.cuda.synchronize()
+    assert torch.equal(got, want) and torch.equal(both[:, :1003], x)
+    for at in (0, 1002):
+        with pytest.raises(RuntimeError):
+            distributions(both[:, :1003], both[:, at:at + 1003], **kw)
+
+
 def test_draws_have_their_probability(lib, cuda):
     """What sample draws from the same logits is kept, with this probability."""
     x, rows = logits_of(64, 20000, BF16, 3), 64
