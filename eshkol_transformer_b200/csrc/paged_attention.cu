@@ -541,9 +541,10 @@ paged_attention_kernel(const __grid_constant__ CUtensorMap k_map,
 
 // Joins the parts of the tiles that the thread blocks blockIdx.x, blockIdx.x +
 // gridDim.x, ... (of `blocks`) of the attention began and did not finish;
-// blockIdx.y takes its share of the rows.  A large tile of up to 8 parts takes a warp
-// per row (with the tcgen05 kernels' many rows and two or three parts, rows in
-// turn took 35 us of the f32 prompts' 154); more parts take the block: warp w
+// blockIdx.y takes its share of the rows.  A large tile of up to 8 parts takes the lanes
+// that read a row in 16-byte pieces per row (with the tcgen05 kernels' many rows and two
+// or three parts, rows in turn took 35 us of the f32 prompts' 154; a warp a row of 64 dims
+// 15 us where this takes 11); more parts take the block: warp w
 // parts w, w + 8, ..., 4 dims per lane, several parts' loads in flight, and
 // shared memory adds the warps up in order.
 constexpr int JOIN_WARPS = 8;
@@ -560,15 +561,20 @@ __global__ void __launch_bounds__(32 * JOIN_WARPS) paged_join_kernel(AttendArgs 
     if (cut.parts == 0) continue;
     auto slot_of = [&](int part) { return part == 0 ? 2 * c + 1 : 2 * (c + part); };
     if (rows > 16 && cut.parts <= JOIN_WARPS) {
-      constexpr int W = DH / 32;  // dims per lane
-      for (int r = blockIdx.y * JOIN_WARPS + warp; r < rows; r += gridDim.y * JOIN_WARPS) {
-        const int g = (cut.tile << a.tiling.row_bits) + r;
-        if (g >= cut.n * group) break;
-        const bool mine = lane < cut.parts;
-        const int64_t s = mine ? slot_of(lane) : 0;
+      // 16 bytes of a part at a time, so as many rows as the warp has lanes for at once
+      constexpr int W = DH / 32 > 4 ? DH / 32 : 4, LANES_ROW = DH / W, AT_ONCE = 32 / LANES_ROW;
+      const int sub = lane / LANES_ROW, in = lane % LANES_ROW;
+      for (int r0 = (blockIdx.y * JOIN_WARPS + warp) * AT_ONCE; r0 < rows; r0 += gridDim.y * JOIN_WARPS * AT_ONCE) {
+        const int r = r0 + sub, g = (cut.tile << a.tiling.row_bits) + r;
+        if (g - sub >= cut.n * group) break;
+        const bool mine = in < cut.parts;
+        const int64_t s = mine ? slot_of(in) : 0;
         const float m1 = mine ? a.joint.stats[s * 2 * rows + r] : -INFINITY;
         const float l1 = mine ? a.joint.stats[(s * 2 + 1) * rows + r] : 0.0f;
-        const float m = warp_max(m1), ref = m == -INFINITY ? 0.0f : m;
+        float m = m1;
+#pragma unroll
+        for (int o = 1; o < LANES_ROW; o <<= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
+        const float ref = m == -INFINITY ? 0.0f : m;
         const float f1 = ex2(m1 - ref), lf = scaled(l1, m1 - ref);
         // in the order of the parts, as below
         float l = 0.0f, x[W];
@@ -576,32 +582,24 @@ __global__ void __launch_bounds__(32 * JOIN_WARPS) paged_join_kernel(AttendArgs 
         for (int k = 0; k < W; k++) x[k] = 0.0f;
 #pragma unroll 2
         for (int i = 0; i < cut.parts; i++) {
-          const float f = __shfl_sync(0xffffffffu, f1, i);
-          l += __shfl_sync(0xffffffffu, lf, i);
-          const float* src = a.joint.sums + ((int64_t)slot_of(i) * rows + r) * DH + lane * W;
-          if constexpr (W >= 4) {
+          const float f = __shfl_sync(0xffffffffu, f1, sub * LANES_ROW + i);
+          l += __shfl_sync(0xffffffffu, lf, sub * LANES_ROW + i);
+          const float* src = a.joint.sums + ((int64_t)slot_of(i) * rows + r) * DH + in * W;
 #pragma unroll
-            for (int k = 0; k < W; k += 4) {
-              const float4 y = *reinterpret_cast<const float4*>(src + k);
-              x[k] += f * y.x; x[k + 1] += f * y.y; x[k + 2] += f * y.z; x[k + 3] += f * y.w;
-            }
-          } else {
-#pragma unroll
-            for (int k = 0; k < W; k++) x[k] += f * src[k];
+          for (int k = 0; k < W; k += 4) {
+            const float4 y = *reinterpret_cast<const float4*>(src + k);
+            x[k] += f * y.x; x[k + 1] += f * y.y; x[k + 2] += f * y.z; x[k + 3] += f * y.w;
           }
         }
+        if (g >= cut.n * group) continue;
         const int by = quotient(g, a.tiling.by_group), h = cut.h * group + g - by * group;
         const int64_t t = cut.first + by;
         const float inv = l > 0.0f ? 1.0f / l : 0.0f;
-        T* dst = static_cast<T*>(a.o) + t * a.o_stride + (int64_t)h * dim + lane * W;
-        if constexpr (W == 1) {
-          if (lane < dim) dst[0] = from_f32<T>(x[0] * inv);
-        } else {
+        T* dst = static_cast<T*>(a.o) + t * a.o_stride + (int64_t)h * dim + in * W;
 #pragma unroll
-          for (int k = 0; k < W; k += 2)
-            if (lane * W + k < dim) store2<T>(dst + k, x[k] * inv, x[k + 1] * inv);
-        }
-        if (a.lse != nullptr && lane == 0)
+        for (int k = 0; k < W; k += 2)
+          if (in * W + k < dim) store2<T>(dst + k, x[k] * inv, x[k + 1] * inv);
+        if (a.lse != nullptr && in == 0)
           a.lse[t * a.q_heads + h] = l > 0.0f ? m * kLn2 + logf(l) : -INFINITY;
       }
       continue;
