@@ -13,17 +13,29 @@
 // their row.  At f32 queries and weights carry the residual of that rounding (22 bits), at
 // f16 the queries do.
 //
-// Up to 32 rows (few8_kernel) products have the keys as rows, S^T = K Q^T and O^T = V^T
-// P^T with the queries as 8 to 32 columns, and warps split the keys of a block: what is
-// converted (every byte once, by the warp that uses it) is the operand of 16 rows, a
-// step of few queries has no idle rows, and o takes dim x 8 sums.  A thread's four
+// Tiles of 8 or 16 rows (few8_kernel): products have the keys as rows, S^T = K Q^T and
+// O^T = V^T P^T with the queries as 8 or 16 columns, and warps split the keys of a block:
+// what is converted (every byte once, by the warp that uses it) is the operand of all
+// rows, a step of few queries has no idle rows, and o takes dim x 8 sums.  A thread's four
 // neighbouring bytes of a key are the two register pairs that a 16-deep product wants
 // if dims are numbered that way, which the queries' layout follows; of V the transposed
 // load brings two dims of two keys, which one byte permutation turns into two pairs of
 // keys, rows of an even and an odd dim.  Weights change from a result's to an operand's
 // layout by 8 x 8 transposes of the register files.
-// More rows (many8_kernel): four warps convert a block together to binary16 tiles first,
-// then take 16 rows and all keys each.
+// Tiles of 64 rows (many8_kernel, chunks that the tcgen05 kernel does not take): four warps
+// convert a block together to binary16 tiles first, then take 16 rows and all keys each.
+//
+// Single tokens are read at 5.0 TB/s (64 requests of up to 8,192 keys, 32 / 8 heads x 128,
+// bf16, 697 MB: 140 us, 76 % of the copy rate); a block of 128 keys then waits for bytes
+// (2.7 of the 6.7 cycles between two instructions of a warp), issue slots are 41 % busy.  Three
+// thread blocks an SM with two stages each hide that best: two with three stages 177 us,
+// four of 64 keys 151.  Drafts (32 requests of 5 tokens, 20 rows a head, to 4,000 keys:
+// 71 us, 2.5 TB/s) read the cache twice, from the L2 the second time, and are bound by
+// the latency of a step's chain (conversion, products, exponentials, products; issue
+// slots 41 %, tensor pipe 19 %): tiles of 8 rows 76 us, of 32 rows as two warps' halves 107.
+// many8_kernel: 512 tokens over 6,000 keys, 32 / 8 heads x 128 bf16, pages of 24: 344 us,
+// 140 TFLOP/s; two blocks an SM (254 registers), whose conversion, products and
+// exponentials follow one another (issue slots 47 %, tensor pipe 27 %).
 #include <math.h>
 
 #include <type_traits>
@@ -39,8 +51,9 @@ using namespace paged;
 // log2 of the largest weight: D is within 1/2 of the largest exponent, c below 2
 constexpr float kShift = 13.0f;
 
-// ROWS queries of a tile, WARPS warps, WK of them along the keys of a block (WK == 1:
-// many8_kernel, tiles of binary16 in shared memory); PER_SM thread blocks whose registers have to fit an SM.
+// ROWS queries of a tile, WARPS warps, all (WK == WARPS: few8_kernel) or one of them (many8_kernel,
+// tiles of binary16 in shared memory) along the BK keys of a block; PER_SM thread blocks whose
+// registers have to fit an SM.
 template <typename T, int DH_, int ROWS_, int WARPS_, int WK_, int BK_, int STAGES_, int PER_SM_>
 struct Shape8 {
   static constexpr int DH = DH_, BM = ROWS_, WARPS = WARPS_, WK = WK_, BK = BK_, STAGES = STAGES_,
@@ -384,8 +397,8 @@ __global__ void __launch_bounds__(S::NT + (TMA ? 32 : 0), S::PER_SM)
 few8_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_constant__ CUtensorMap v_map,
             const __grid_constant__ Attend8Args args, int box_bits) {
   constexpr int DH = S::DH, BM = S::BM, BK = S::BK, KW = S::KW, NT = S::NT, WK = S::WK;
-  constexpr int WM = S::WARPS / WK, MINE = BM / WM;  // parts of the rows, rows of a warp
-  constexpr int NQ = MINE / 8, KG = KW / 16;         // columns of 8 queries, rows of 16 keys
+  static_assert(WK == S::WARPS, "every warp takes all rows");
+  constexpr int NQ = BM / 8, KG = KW / 16;  // columns of 8 queries, rows of 16 keys
   constexpr bool QLO = S::QLO, PLO = S::PLO;
   const AttendArgs& a = args.a;
   extern __shared__ __align__(1024) uint8_t smem[];
@@ -394,7 +407,7 @@ few8_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_constant__ C
   float* join_m = reinterpret_cast<float*>(smem + S::JOIN);
   float* join_l = join_m + WK * BM;
   const uint32_t base = smem_u32(smem);
-  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, wk = warp % WK, q0 = warp / WK * MINE;
+  const int tid = threadIdx.x, lane = tid & 31, wk = tid >> 5;
   const int dim = a.pools.head_dim, group = a.tiling.group;
   const int g = lane >> 2, t2 = 2 * (lane & 3);  // a result's row (and row + 8), its columns
   // lets the joining kernel start its launch; it waits for this one's results
@@ -409,7 +422,7 @@ few8_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_constant__ C
   const Share share = divide(a.tiling, a.batch, a.least, p, room);
   __syncthreads();
   const int units = (int)share.units;
-  if (TMA && warp == S::WARPS) {
+  if (TMA && wk == WK) {
     copy_blocks<S>(k_map, v_map, args, box_bits, p, units, smem);
     return;
   }
@@ -452,7 +465,7 @@ few8_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_constant__ C
         for (int n = 0; n < NQ; n++)
 #pragma unroll
           for (int c = 0; c < 2; c++) {
-            const int r = q0 + 8 * n + t2 + c;
+            const int r = 8 * n + t2 + c;
             row[n][c].clear();
             mul[n][c] = qmul[r];
             vis[n][c] = r < rows ? max(0, p.r.len - p.r.n + quotient(first_row + r, a.tiling.by_group) + 1) : 0;
@@ -484,7 +497,7 @@ few8_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_constant__ C
         uint32_t qh[NQ][4], ql[NQ][4];     // pairs of two 16-deep products
 #pragma unroll
         for (int n = 0; n < NQ; n++) {
-          const uint32_t at = base + S::Q + S::template at16<BM>(q0 + 8 * n + (lane & 7), 4 * d + (lane >> 3));
+          const uint32_t at = base + S::Q + S::template at16<BM>(8 * n + (lane & 7), 4 * d + (lane >> 3));
           ldsm4(qh[n], at);
           if constexpr (QLO) ldsm4(ql[n], at + S::TILE_Q);
         }
@@ -609,8 +622,8 @@ few8_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_constant__ C
 #pragma unroll
             for (int x = 4; x < 32; x <<= 1) v += __shfl_xor_sync(0xffffffffu, v, x);
             if (g == 0) {
-              join_m[wk * BM + q0 + 8 * n + t2 + c] = row[n][c].m;
-              join_l[wk * BM + q0 + 8 * n + t2 + c] = v;
+              join_m[wk * BM + 8 * n + t2 + c] = row[n][c].m;
+              join_l[wk * BM + 8 * n + t2 + c] = v;
             }
           }
         named_sync(1, NT);  // every warp is done with the stage, too
@@ -618,7 +631,7 @@ few8_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_constant__ C
         for (int n = 0; n < NQ; n++)
 #pragma unroll
           for (int c = 0; c < 2; c++) {
-            const int r = q0 + 8 * n + t2 + c;
+            const int r = 8 * n + t2 + c;
             float all = -INFINITY;
 #pragma unroll
             for (int w = 0; w < WK; w++) all = fmaxf(all, join_m[w * BM + r]);
@@ -636,7 +649,7 @@ few8_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_constant__ C
               o[i][n][2 + c] = o[i][n][2 + c] * f0 * f1;
             }
           }
-        float4* merge = reinterpret_cast<float4*>(smem + st * S::STAGE + q0 * (WK / 2 * DH * 4));
+        float4* merge = reinterpret_cast<float4*>(smem + st * S::STAGE);
 #pragma unroll
         for (int half = WK / 2; half > 0; half >>= 1) {
           if (half < WK / 2) named_sync(1, NT);
@@ -669,7 +682,7 @@ few8_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_constant__ C
           for (int n = 0; n < NQ; n++)
 #pragma unroll
             for (int c = 0; c < 2; c++) {
-              const int r = q0 + 8 * n + t2 + c, at = (p.tile << a.tiling.row_bits) + r;
+              const int r = 8 * n + t2 + c, at = (p.tile << a.tiling.row_bits) + r;
               if (done) {
                 if (at < p.r.n * group) {
                   const int by = quotient(at, a.tiling.by_group), h = p.h * group + at - by * group;
@@ -1019,7 +1032,9 @@ int launch_shape8(const et_b200_paged_cache8_v1* c, Attend8Args& x, void* ws, cu
 // of its conversion whatever the rows.  32 requests of up to 4,000 keys, 32 / 8 heads x 128,
 // us for 20, 32, 48, 64, 96, 128 rows: bf16 70, 98, 134, 166, 230, 295 in tiles of 16 and 134,
 // 141, 151, 156, 167, 175 by attend8_tc; f32 104, 145, 212, 251, 358, 467 and 272, 274, 275,
-// 277, -, 467 by many8_kernel.
+// 277, -, 467 by many8_kernel.  With 16 heads x 64 of group 1 f32 takes 139, 171, 239, 297
+// us for the first four in tiles of 16 and 315, 318, 333, 346 by attend8_tc (366 and 371 for 96 and
+// 128).
 template <typename T, int DH>
 int launch_dim8(const et_b200_paged_cache8_v1* c, Attend8Args& x, int64_t rows, void* ws,
                 cudaStream_t stream) {

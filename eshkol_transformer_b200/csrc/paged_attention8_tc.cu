@@ -1,5 +1,5 @@
 // Attention of chunks of new tokens over an 8-bit paged cache on tcgen05: f16 / bf16
-// queries, head_dim up to 128, pages of a power of two of at least 8 slots.
+// queries of head_dim up to 128, f32 of up to 64, pages of a power of two of at least 8 slots.
 //
 // The mathematics are those of paged_attention8.cu, tiles and roles those of
 // paged_attention_tc.cu (256 rows as two halves, blocks of 128 keys, a warpgroup of
@@ -12,7 +12,21 @@
 // powers of two that is exact down to 2^-21 of the largest (binary16 holds 2^-24 to
 // 2^15, an element 2^-9 to 448); other scales round each element to 11 bits.
 // Queries are binary16 times 2^-e of their row, weights binary16 times 2^11 below a
-// standing maximum that allows 2^4: 11 bits, more than a bf16 result keeps.
+// standing maximum that allows 2^4: 11 bits, more than a bf16 result keeps.  At f32 both carry
+// the residual of that rounding (22 bits, two products instead of one), and the products of a
+// block are added to f32 sums in tensor memory.
+//
+// 4,096 tokens over 12,000 keys (32 / 8 heads x 128, bf16): 930 us, 720 TFLOP/s, 43 % of the
+// matrix rate (810 to 840 with the conversion's arithmetic left out).  Bound by the chain
+// of a block (scores to probabilities 3,000 to 3,500 cycles, conversion 1,250 beside it), with
+// issue slots 46 % and the tensor pipe 34 % busy, the roles' code beyond the instruction cache
+// (stalls for it 0.5 a warp's instruction; placement moves the time by 5 %).  Four ragged f32
+// prompts to 1,024 (16 heads x 64): 78 us with the joining, of 7 blocks in two tiles a thread
+// block half in queries (6.5 us a tile) and outputs (4 us), issue slots 28 % busy.
+// Measured and not kept: a warp that computes the scales' factors ahead (978 to 1,130 us),
+// probabilities in rolled loops (1,216 to 1,327), the halves along the keys for few rows (140 to
+// 180 us for 20 to 128 rows where this takes 135 to 175), loads of the queries two or three
+// steps ahead (prompts 83 and 85 us) or prefetched into the L2 (83).
 // Waits are bounded; one that runs out raises a CTA-wide abort, copies and
 // products in flight are waited for and TMEM is released.
 #include <math.h>

@@ -26,6 +26,15 @@
 // of the steps that one thread block or cluster takes alone.
 // Rows for which the list or the border's step overflows (thousands of equal
 // logits) or the slices do not fit are selected by radix from memory.
+//
+// Distributions take the same steps up to the draw, then write w / total with w in f32 and
+// the fixed-point total.  A row that keeps few tokens (greedy, or a list) is zeros but for
+// those: bulk copies write them from 4 KB of shared memory while the row is read; other
+// rows are written from shared memory once their cut is known.  320 rows of 128,259 bf16 with
+// top-k 40 (246 MB, two thirds of it written): 77.7 us, 3.2 TB/s, of which the set-up of four
+// waves of thread blocks and their barriers (6.8 of the 16 cycles between two instructions
+// of a warp) take half; with the zeros written by the threads behind the list 111 us.  One
+// row of 32,768: 12.3 us, the latency of the steps.
 #include <math.h>
 
 #include <cooperative_groups.h>
