@@ -775,8 +775,8 @@ int32_t check_attention(const et_b200_paged_batch_v1* b, int64_t head_dim, int64
   if (workspace == nullptr || (reinterpret_cast<uintptr_t>(workspace) & 255) != 0 ||
       bytes < need)
     return set_error(e, ET_KERNEL_ERROR_INVALID_ARGUMENT, ET_KERNEL_CODE_BUFFER_TOO_SMALL, op,
-                     "workspace is smaller than et_b200_paged_attention_workspace_bytes_v1 or "
-                     "not 256-byte aligned");
+                     "workspace is smaller than the call's workspace_bytes_v1 asks for or not "
+                     "256-byte aligned");
   return 0;
 }
 
