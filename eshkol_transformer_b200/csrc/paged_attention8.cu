@@ -1028,13 +1028,13 @@ int launch_shape8(const et_b200_paged_cache8_v1* c, Attend8Args& x, void* ws, cu
 
 // How a step's rows per kv head are taken.  One or two columns of 8 queries: few8_kernel
 // alone.  More: tiles of 16, each of which reads the cache (from the L2 after the
-// first), against one pass of attend8_tc (16-bit types) or many8_kernel, whose time is that
-// of its conversion whatever the rows.  32 requests of up to 4,000 keys, 32 / 8 heads x 128,
-// us for 20, 32, 48, 64, 96, 128 rows: bf16 70, 98, 134, 166, 230, 295 in tiles of 16 and 134,
-// 141, 151, 156, 167, 175 by attend8_tc; f32 104, 145, 212, 251, 358, 467 and 272, 274, 275,
-// 277, -, 467 by many8_kernel.  With 16 heads x 64 of group 1 f32 takes 139, 171, 239, 297
-// us for the first four in tiles of 16 and 315, 318, 333, 346 by attend8_tc (366 and 371 for 96 and
-// 128).
+// first), against one pass of attend8_tc, whose time is that of its conversion whatever the
+// rows (or of many8_kernel, where that does not take the cache).  32 requests of up to 4,000
+// keys, 32 / 8 heads x 128, us for 20, 32, 48, 64, 96, 128 rows: bf16 70, 98, 134, 166, 230,
+// 295 in tiles of 16 and 134, 141, 151, 156, 167, 175 by attend8_tc; f32 104, 145, 206, 248,
+// 358, 467 and, from 48 rows on, 211, 218, 225, 236 by attend8_tc.  With 16 heads x 64 of
+// group 1 f32 takes 139, 171, 239, 297 us for the first four in tiles of 16 and 315, 318, 333,
+// 346 by attend8_tc (366 and 371 for 96 and 128).
 template <typename T, int DH>
 int launch_dim8(const et_b200_paged_cache8_v1* c, Attend8Args& x, int64_t rows, void* ws,
                 cudaStream_t stream) {
@@ -1044,7 +1044,7 @@ int launch_dim8(const et_b200_paged_cache8_v1* c, Attend8Args& x, int64_t rows, 
     return launch_shape8<T, Shape8<T, DH, 64, 4, 1, 64, 2, 1>>(c, x, ws, stream);
   } else {
     if (rows <= 8) return launch_shape8<T, Shape8<T, DH, 8, 4, 4, 128, 2, 3>>(c, x, ws, stream);
-    if (rows <= (sizeof(T) == 2 ? 48 : 64))
+    if (rows <= (sizeof(T) == 4 && DH == 64 ? 64 : 48))
       return launch_shape8<T, Shape8<T, DH, 16, 4, 4, 128, 3, 2>>(c, x, ws, stream);
     if (const int blocks = attend8_tc(c, x, ws, stream)) return blocks;
     return launch_shape8<T, Shape8<T, DH, 64, 4, 1, 64, 2, 2>>(c, x, ws, stream);

@@ -1,5 +1,5 @@
-// Attention of chunks of new tokens over an 8-bit paged cache on tcgen05: f16 / bf16
-// queries of head_dim up to 128, f32 of up to 64, pages of a power of two of at least 8 slots.
+// Attention of chunks of new tokens over an 8-bit paged cache on tcgen05: head_dim up to
+// 128, pages of a power of two of at least 8 slots.
 //
 // The mathematics are those of paged_attention8.cu, tiles and roles those of
 // paged_attention_tc.cu (256 rows as two halves, blocks of 128 keys, a warpgroup of
@@ -22,7 +22,9 @@
 // issue slots 46 % and the tensor pipe 34 % busy, the roles' code beyond the instruction cache
 // (stalls for it 0.5 a warp's instruction; placement moves the time by 5 %).  Four ragged f32
 // prompts to 1,024 (16 heads x 64): 78 us with the joining, of 7 blocks in two tiles a thread
-// block half in queries (6.5 us a tile) and outputs (4 us), issue slots 28 % busy.
+// block half in queries (6.5 us a tile) and outputs (4 us), issue slots 28 % busy.  f32 at 128
+// dims: 2,048 tokens over 6,000 keys (32 / 8 heads) 635 us, tiles of one half (1,771 us by
+// mma.sync).
 // Measured and not kept: a warp that computes the scales' factors ahead (978 to 1,130 us),
 // probabilities in rolled loops (1,216 to 1,327), the halves along the keys for few rows (140 to
 // 180 us for 20 to 128 rows where this takes 135 to 175), loads of the queries two or three
@@ -57,20 +59,22 @@ constexpr int kMarked = 4096;  // added to E of a block with keys that make NaN
 // PAIRS: queries and weights with their residuals (f32)
 template <int DH, bool PAIRS>
 struct Layout {
+  // halves of 128 rows; f32 at 128 dims has one, as its sums take the other's tensor memory
+  static constexpr int HALVES = PAIRS && DH == 128 ? 1 : 2;
   static constexpr int SLOT = BK * DH * 2;  // one block of K or V in binary16
   static constexpr int SLOTS = DH == 128 ? 3 : 6;
   static constexpr int RAW = BK * DH;       // one block of K or V in bytes
   static constexpr int RAWS = DH == 128 ? 4 : PAIRS ? 6 : 8;
   static constexpr int TILE_Q = HALF * DH * 2 * (PAIRS ? 2 : 1);
-  static constexpr int Q = SLOTS * SLOT;    // two halves of 128 rows
-  static constexpr int BYTES = Q + 2 * TILE_Q;
+  static constexpr int Q = SLOTS * SLOT;
+  static constexpr int BYTES = Q + HALVES * TILE_Q;
   static constexpr int SCALES = BYTES + RAWS * RAW;  // [block % (RAWS / 2)][keys, values][BK]
   static constexpr int BARS = SCALES + RAWS * BK * 4;
   static constexpr int SMEM = BARS + 512;
   // TMEM: scores of the halves (P over the first 64 columns, its residual over the others),
   // outputs, with PAIRS their sums over blocks
-  static constexpr uint32_t S0 = 0, O0 = 256, SUM0 = O0 + 2 * DH, COLS = 512;
-  static_assert(SUM0 + (PAIRS ? 2 * DH : 0) <= COLS && SMEM <= 232448, "TMEM and shared memory");
+  static constexpr uint32_t S0 = 0, O0 = 256, SUM0 = O0 + HALVES * DH, COLS = 512;
+  static_assert(SUM0 + (PAIRS ? HALVES * DH : 0) <= COLS && SMEM <= 232448, "TMEM and shared memory");
 };
 
 // Whether `v` holds for all `threads` threads of a named barrier.
@@ -99,7 +103,7 @@ paged_attention8_tc_kernel(const __grid_constant__ CUtensorMap k_map,
                            const __grid_constant__ CUtensorMap v_map, Attend8Args args, int box_rows) {
   constexpr bool PAIRS = sizeof(T) == 4;
   using L = Layout<DH, PAIRS>;
-  constexpr int SLOTS = L::SLOTS, RAWS = L::RAWS, TILE = 2 * HALF;
+  constexpr int SLOTS = L::SLOTS, RAWS = L::RAWS, TILE = L::HALVES * HALF;
   const AttendArgs& a = args.a;
   extern __shared__ __align__(1024) uint8_t smem[];
   float* scales_s = reinterpret_cast<float*>(smem + L::SCALES);
@@ -735,11 +739,12 @@ int launch_tc8(const et_b200_paged_cache8_v1* c, Attend8Args& x, void* ws, cudaS
   if (!scales_copy(c) || !pool8_map(&k_map, c->keys, c, DH, box_rows) ||
       !pool8_map(&v_map, c->values, c, DH, box_rows))
     return 0;
-  const int blocks = thread_blocks(a, a.sms, 2 * HALF, BK);
-  a.tiling = tiling_of(8, 7, a.tiling.group, a.pools.kv_heads);
-  static_assert(2 * HALF == 1 << 8 && BK == 1 << 7, "tiling");
+  constexpr int TILE = L::HALVES * HALF;
+  const int blocks = thread_blocks(a, a.sms, TILE, BK);
+  a.tiling = tiling_of(L::HALVES == 2 ? 8 : 7, 7, a.tiling.group, a.pools.kv_heads);
+  static_assert(HALF == 1 << 7 && BK == 1 << 7, "tiling");
   a.least = 2;
-  a.joint = joint_of(ws, blocks, 2 * HALF, DH);
+  a.joint = joint_of(ws, blocks, TILE, DH);
   cudaFuncSetAttribute(paged_attention8_tc_kernel<T, DH>,
                        cudaFuncAttributeMaxDynamicSharedMemorySize, L::SMEM);
   paged_attention8_tc_kernel<T, DH><<<blocks, THREADS, L::SMEM, stream>>>(k_map, v_map, x, box_rows);
@@ -752,9 +757,10 @@ int launch_tc8(const et_b200_paged_cache8_v1* c, Attend8Args& x, void* ws, cudaS
 namespace paged {
 
 int attend8_tc(const et_b200_paged_cache8_v1* c, Attend8Args& x, void* ws, cudaStream_t stream) {
-  // at f32 the sums over blocks need the tensor memory that 128 dims would take
-  if (c->head_dim > (c->dtype == ET_B200_DTYPE_F32 ? 64 : 128)) return 0;
-  if (c->dtype == ET_B200_DTYPE_F32) return launch_tc8<float, 64>(c, x, ws, stream);
+  if (c->head_dim > 128) return 0;
+  if (c->dtype == ET_B200_DTYPE_F32)
+    return c->head_dim <= 64 ? launch_tc8<float, 64>(c, x, ws, stream)
+                             : launch_tc8<float, 128>(c, x, ws, stream);
   if (c->dtype == ET_B200_DTYPE_F16)
     return c->head_dim <= 64 ? launch_tc8<__half, 64>(c, x, ws, stream)
                              : launch_tc8<__half, 128>(c, x, ws, stream);

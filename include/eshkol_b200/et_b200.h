@@ -303,11 +303,11 @@ int32_t et_b200_paged_append8_v1(const et_b200_paged_cache8_v1 *cache,
  * chunks below); the probabilities as binary16, at f32 with their residual.
  * Elements and their products with scales that are powers of two (or 0), as the
  * append writes them, are exact.  Chunks (more than 48 query rows per kv head, as
- * max_new tells, and head_dim up to 128 at f16 and bf16, more than 64 rows and
- * head_dim up to 64 at f32) over pages of a power of two of at least 8 slots whose scales lie side by
- * side round other scales' products to 11 bits; there, rows of a block of 128 keys (of the
- * keys), or behind the largest so far (of the values), whose scale is less than
- * 2^-21 of the largest one's lose bits. */
+ * max_new tells, at f32 up to 64 dims more than 64; head_dim up to 128) over pages of a
+ * power of two of at least 8 slots whose scales lie side by side round other scales'
+ * products to 11 bits; there, rows of a block of 128 keys (of the keys), or behind the
+ * largest so far (of the values), whose scale is less than 2^-21 of the largest one's
+ * lose bits. */
 size_t et_b200_paged_attention8_workspace_bytes_v1(
     const et_b200_paged_cache8_v1 *cache, int64_t q_heads);
 int32_t et_b200_paged_attention8_v1(const et_b200_paged_cache8_v1 *cache,

@@ -335,13 +335,24 @@ def test_attention_layouts(lib, cuda, requests, layout, strided, loose, dtype):
     s.check(rope=False)
 
 
+@pytest.mark.parametrize("q_heads,heads,dim,page", [(4, 2, 128, 16), (6, 1, 80, 8), (3, 3, 96, 64), (16, 2, 128, 128)])
+@pytest.mark.parametrize("strided", [False, True])
+def test_f32_chunks_above_64_dims(lib, cuda, q_heads, heads, dim, page, strided):
+    """Tiles of 128 rows with sums of their own, whole and cut into parts."""
+    s = Step8([(300, 2000), (130, 130), (70, 5000), (0, 7), (1, 900), (64, 3)], q_heads, heads, dim, page, F32,
+              seed=dim + page, strided=strided)
+    s.attend()
+    s.check()
+
+
 @pytest.mark.parametrize("dtype", [F32, F16, BF16])
 @pytest.mark.parametrize("hint,dim", [(1, 64), (1, 128), (1, 256), (100, 64), (100, 128), (100, 256)])
 def test_rows_of_any_size(lib, cuda, hint, dim, dtype):
     """Rows whose scales differ by many powers of two and rows of zeros: with up to 16 rows
     a head and where mma.sync takes the chunk, of any size; in the tcgen05 kernel (chunks up
-    to 128 dims, f32 up to 64) down to 2^-21 of the largest, of the values 2^-10 here for the
-    weights' own rounding of 2^-38."""
+    to 128 dims) down to 2^-21 of the largest, of the values 2^-10 here for the weights' own
+    rounding of 2^-38; f32 of 128 dims there has 2^-30 here, where what is lost of such rows
+    is 2^-11 of them and less than 2^-40 of the largest."""
     near = hint > 16 and dim <= (64 if dtype == F32 else 128)
     low = -10 if near else -30
 
