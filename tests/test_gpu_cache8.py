@@ -13,6 +13,7 @@ up to 2^-25 whatever the value).  At f32 the bar of the framework's
 other f32-grade attention tests: 2e-5 absolute plus relative.
 """
 import math
+import threading
 
 import pytest
 import torch
@@ -567,6 +568,42 @@ def test_graphs_streams_and_workspaces(lib, cuda):
     torch.cuda.synchronize()
     graphs[0].replay()
     s.check()
+
+
+def test_calls_from_several_threads(lib, cuda):
+    """Host threads with streams and workspaces of their own, kernels of every kind at once."""
+    made = [Step8(r, 8, 2, d, p, t, seed=i) for i, (r, d, p, t) in enumerate((
+        ([(1, 3000)] * 5, 128, 16, BF16), ([(6, 500), (40, 40)], 64, 24, F16), ([(90, 700)], 128, 64, F32),
+        ([(200, 300), (3, 900)], 128, 16, BF16)))]
+    for s in made:
+        s.attend()
+    torch.cuda.synchronize()
+    alone = [(s.o.clone(), s.lse.clone()) for s in made]
+    for s in made:
+        s.o.zero_(), s.lse.zero_()
+    torch.cuda.synchronize()
+    failed = []
+
+    def work(s):
+        try:
+            stream = torch.cuda.Stream()
+            attention_object = paged.PagedAttention(s.cache, s.q_heads)
+            for _ in range(20):
+                s.attend(stream=stream.cuda_stream, attention_object=attention_object)
+            stream.synchronize()
+        except Exception as e:  # reported by the test's own thread
+            failed.append(e)
+
+    threads = [threading.Thread(target=work, args=(s,)) for s in made]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    torch.cuda.synchronize()
+    assert not failed
+    for s, (o, lse) in zip(made, alone):
+        rows = slice(0, s.used)
+        assert torch.equal(s.o[rows], o[rows]) and torch.equal(s.lse[rows], lse[rows]) and int(s.status) == 0
 
 
 def test_calls_follow_the_current_stream(lib, cuda):
