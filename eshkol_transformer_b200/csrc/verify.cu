@@ -152,6 +152,8 @@ __global__ void __launch_bounds__(NT, 2) verify_kernel(VerifyArgs a) {
     }
     // every block waits for this before it leaves or begins again; the first draws meanwhile
     cluster.barrier_arrive();
+    // the sums that a thread scans are neighbours, gathered by others once they are more than NT
+    __syncthreads();
     // running sums of `per` segments a thread
     const int per = (a.segs + NT - 1) / NT, t0 = min(a.segs, tid * per), t1 = min(a.segs, t0 + per);
     double own = 0.0;
