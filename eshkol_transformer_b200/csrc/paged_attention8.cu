@@ -146,8 +146,10 @@ __device__ void copy_blocks(const CUtensorMap& k_map, const CUtensorMap& v_map, 
     const int boxes = __popc(__ballot_sync(0xffffffffu, now != -2));
     const int sound = __popc(__ballot_sync(0xffffffffu, now >= 0));
     float* sc = scales_s + st * 2 * BK + (lane << box_bits);
-    if (now == -1)
+    if (now == -1) {
       for (int i = 0; i < 1 << box_bits; i++) sc[i] = sc[BK + i] = 0.0f;
+      fence_async_smem();  // before a later block's copy to these places
+    }
     __syncwarp();
     if (lane == 0)
       mbar_expect_tx(bars.full(st), (uint32_t)((boxes << box_bits) * S::ROW * 2 + (sound << box_bits) * 8));
