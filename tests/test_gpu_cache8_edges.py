@@ -2,6 +2,7 @@
 import pytest
 import torch
 
+from cache8_f64 import rows_of
 from test_gpu_cache8 import BF16, F16, F32, Step8
 from eshkol_transformer_b200 import paged
 
@@ -36,3 +37,57 @@ def test_bad_pages_among_sound_ones(lib, cuda, hint, dim, page, dtype):
         torch.cuda.synchronize()
         assert int(s.status) == paged.BAD_PAGE
         assert torch.equal(s.o, want) and torch.equal(s.lse, lse)
+
+
+@pytest.mark.parametrize("dtype", [F32, F16, BF16])
+@pytest.mark.parametrize("dim", [64, 128, 256])
+@pytest.mark.parametrize("hint", [1, 4, 100])
+def test_small_rows_beside_large_ones(lib, cuda, hint, dim, dtype):
+    """Rows of keys and of values whose scales are 2^-21 of the largest of their block keep every
+    bit, in every kernel: the large keys lie where no query looks (their scores are below -1,000), so
+    the outputs are means of the small values alone.
+
+    With u = 2^-11 (f32: 2^-22) for queries and weights, a score of a small key is off by delta =
+    (u + dim 2^-23 + 2^-22) sum |q||k|, its weight by exp(2 delta) - 1 and by u relative and by 2^-36 of
+    the largest, sums over m keys by (m + 16) 2^-23 and exponentials by 2^-17 where the type is of 16
+    bits, by 2e-5 at f32; the output by half a step."""
+    s = Step8([(100, 700), (64, 300), (70, 170)], 4, 2, dim, 16, dtype, seed=dim)
+    g = torch.Generator(device="cuda").manual_seed(dim + hint)
+    s.q.copy_(torch.randn(s.q.shape, device="cuda", generator=g) * 2.0 ** 8)
+    s.q[..., 0] = (s.q[..., 0].abs() + 2.0 ** 8).to(dtype)
+    u, step = (2.0 ** -22, 2.0 ** -24) if dtype == F32 else (2.0 ** -11, 2.0 ** (-11 if dtype == F16 else -8))
+    large = []
+    for b, (_, m) in enumerate(s.requests):
+        where, slot = s.slots(b, 0, m)
+        large.append(torch.rand(m, 2, device="cuda", generator=g) < 0.3)
+        bits = s.keys[where, :, slot]
+        bits[large[b]] = 0
+        bits[..., 0] = torch.where(large[b], 0xc8, bits[..., 0].int()).byte()  # -4
+        s.keys[where, :, slot] = bits
+        s.key_scales[where, :, slot] = torch.where(large[b], 2.0 ** 5, 2.0 ** -16)
+        s.value_scales[where, :, slot] = torch.where(large[b], 2.0 ** 6, 2.0 ** -15)
+        s.k[b] = rows_of(s.keys[where, :, slot], s.key_scales[where, :, slot])
+        s.v[b] = rows_of(s.values[where, :, slot], s.value_scales[where, :, slot])
+    s.attend(rope=False, max_new=hint)
+    torch.cuda.synchronize()
+    assert int(s.status) == 0
+    first = 0
+    for b, (n, m) in enumerate(s.requests):
+        q, got = s.q[first:first + n].double(), s.o[first:first + n].double()
+        lse = s.lse[first:first + n].double()
+        first += n
+        hidden = torch.arange(m, device="cuda") > torch.arange(m - n, m, device="cuda")[:, None]
+        for h in range(4):
+            k, v, far = s.k[b][:, h // 2], s.v[b][:, h // 2], large[b][:, h // 2]
+            x = (q[:, h] @ k.T / dim ** 0.5).masked_fill(hidden, -torch.inf)
+            assert (x[:, far] < -1000).all() and x[:, ~far].abs().nan_to_num(posinf=0.0).amax() < 256
+            p, small = torch.softmax(x, 1)[:, ~far], v[~far]
+            want, weighted = p @ small, p @ small.abs()
+            spread = (q[:, h].abs() @ k[~far].abs().T / dim ** 0.5).amax(1, keepdim=True)
+            delta = (u + dim * 2.0 ** -23 + 2.0 ** -22) * spread
+            sums = 2e-5 if dtype == F32 else (m + 16) * 2.0 ** -23 + 2.0 ** -17
+            bound = ((2 * delta).expm1() + u + sums) * weighted + m * 2.0 ** -36 * small.abs().max()
+            bound = bound + step * want.abs() + (2.0 ** -25 if dtype == F16 else 0.0)
+            assert ((got[:, h] - want).abs() <= bound).all()
+            room = delta[:, 0] + 2e-5 * (1 + torch.logsumexp(x, 1).abs())
+            assert ((lse[:, h] - torch.logsumexp(x, 1)).abs() <= room).all()
