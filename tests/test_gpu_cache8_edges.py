@@ -3,7 +3,7 @@ import pytest
 import torch
 
 from cache8_f64 import rows_of
-from test_gpu_cache8 import BF16, F16, F32, Step8
+from test_gpu_cache8 import BF16, F16, F32, Step8, appended, pools_of, same
 from eshkol_transformer_b200 import paged
 
 pytestmark = pytest.mark.gpu
@@ -91,3 +91,38 @@ def test_small_rows_beside_large_ones(lib, cuda, hint, dim, dtype):
             assert ((got[:, h] - want).abs() <= bound).all()
             room = delta[:, 0] + 2e-5 * (1 + torch.logsumexp(x, 1).abs())
             assert ((lse[:, h] - torch.logsumexp(x, 1)).abs() <= room).all()
+
+
+@pytest.mark.parametrize("dtype", [F32, F16, BF16])
+def test_append_leaves_zeros_under_scales_that_are_nan(lib, cuda, dtype):
+    """Every byte of the pools, those of rows that are not finite included: zeros, which a query that does
+    not see them multiplies by 0."""
+    s = Step8([(40, 40), (3, 50)], 2, 2, 64, 16, dtype)
+    g = torch.Generator(device="cuda").manual_seed(3)
+    k, v = (torch.randn(s.tokens, 2, 64, device="cuda", generator=g).to(dtype) for _ in range(2))
+    for x in (k, v):
+        for i, bad in enumerate((torch.inf, -torch.inf, torch.nan)):
+            x[5 + 4 * i, i % 2, 7 * i] = bad
+            x[41, i % 2, 63] = bad
+    for rope in (True, False):
+        want = appended(s, k, v, rope)
+        s.cache.append(s.batch(), k, v, (s.cos, s.sin) if rope else None)
+        torch.cuda.synchronize()
+        assert int(s.status) == 0
+        for got, w in zip(pools_of(s), want):
+            assert same(got, w)
+        where, slot = s.slots(0, 0, 40)
+        none = torch.isnan(s.value_scales[where, :, slot])
+        assert int(none.sum()) == 3 and (s.values[where, :, slot][none] == 0).all()
+
+
+@pytest.mark.parametrize("dtype", [F32, F16, BF16])
+@pytest.mark.parametrize("group,dim,page,new", [(4, 32, 8, 3), (2, 32, 8, 40), (4, 64, 16, 9), (1, 128, 24, 5),
+                                                (8, 128, 16, 12)])
+def test_hundreds_of_requests_against_float64(lib, cuda, group, dim, page, new, dtype):
+    """More requests than thread blocks, some without tokens, some without keys, some with more new tokens
+    than they keep; every one of them by the bounds of the few."""
+    requests = [(0 if i % 11 == 3 else 1 + i % new, (i * 37) % 131) for i in range(400)]
+    s = Step8(requests, 2 * group, 2, dim, page, dtype, seed=new)
+    s.attend()
+    s.check()
