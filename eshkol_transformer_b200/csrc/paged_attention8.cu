@@ -1031,24 +1031,32 @@ int launch_shape8(const et_b200_paged_cache8_v1* c, Attend8Args& x, void* ws, cu
 // How a step's rows per kv head are taken.  One or two columns of 8 queries: few8_kernel
 // alone.  More: tiles of 16, each of which reads the cache (from the L2 after the
 // first), against one pass of attend8_tc, whose time is that of its conversion whatever the
-// rows (or of many8_kernel, where that does not take the cache).  32 requests of up to 4,000
-// keys, 32 / 8 heads x 128, us for 20, 32, 48, 64, 96, 128 rows: bf16 70, 98, 134, 166, 230,
-// 295 in tiles of 16 and 134, 141, 151, 156, 167, 175 by attend8_tc; f32 104, 145, 206, 248,
-// 358, 467 and, from 48 rows on, 211, 218, 225, 236 by attend8_tc.  With 16 heads x 64 of
-// group 1 f32 takes 139, 171, 239, 297 us for the first four in tiles of 16 and 315, 318, 333,
-// 346 by attend8_tc (366 and 371 for 96 and 128).
+// rows, or of many8_kernel, where that does not take the cache.  us for 20, 32, 48, 64, 96, 128 rows,
+// 32 requests of up to 4,000 keys:
+//   32 / 8 heads x 128, bf16: tiles of 16 rows 75, 104, 141, 174, 239, 308; attend8_tc 142, 148,
+//     159, 164, 175, 180.  f32: 104, 145, 207, 248, 352, 466 and 198, 203, 213, 220, 229, 242.
+//   16 heads x 64 of group 1, f32: 148, 181, 248, 308, 428, 544 and 311, 318, 327, 336, 349, 357.
+// Against many8_kernel:
+//   32 / 8 x 128, pages of 24, bf16: 86, 123, 173, 212, 297, 382 and 169, 170, 172, 174, 255, 289.
+//     f32: 103, 148, 208, 255, 362, 468 (192 rows: 680) and 280, 281, 284, 286, 415, 480 (684).
+//   32 / 8 x 64, pages of 24, f32: 71, 101, 136, 169, 234, 300 and 156, 156, 157, 159, 234, 265.
+//   32 / 8 x 256, bf16: 134, 196, 280, 348, 505, 652 and 327, 329, 341, 341, 499, 573.  f32: 204, 300, 427,
+//     539, 801, 1,016 (192 rows: 1,528; 256: 2,033) and 618, 621, 638, 640, 955, 1,101 (1,599; 1,958).
 template <typename T, int DH>
 int launch_dim8(const et_b200_paged_cache8_v1* c, Attend8Args& x, int64_t rows, void* ws,
                 cudaStream_t stream) {
+  constexpr bool F32 = sizeof(T) == 4;
   if constexpr (DH == 256) {
     if (rows <= 8) return launch_shape8<T, Shape8<T, DH, 8, 4, 4, 64, 3, 2>>(c, x, ws, stream);
-    if (rows <= 16) return launch_shape8<T, Shape8<T, DH, 16, 4, 4, 128, 3, 1>>(c, x, ws, stream);
+    if (rows <= (F32 ? 192 : 48))
+      return launch_shape8<T, Shape8<T, DH, 16, 4, 4, 128, 3, 1>>(c, x, ws, stream);
     return launch_shape8<T, Shape8<T, DH, 64, 4, 1, 64, 2, 1>>(c, x, ws, stream);
   } else {
     if (rows <= 8) return launch_shape8<T, Shape8<T, DH, 8, 4, 4, 128, 2, 3>>(c, x, ws, stream);
-    if (rows <= (sizeof(T) == 4 && DH == 64 ? 64 : 48))
-      return launch_shape8<T, Shape8<T, DH, 16, 4, 4, 128, 3, 2>>(c, x, ws, stream);
+    using Sixteen = Shape8<T, DH, 16, 4, 4, 128, 3, 2>;
+    if (rows <= (F32 && DH == 64 ? 64 : 48)) return launch_shape8<T, Sixteen>(c, x, ws, stream);
     if (const int blocks = attend8_tc(c, x, ws, stream)) return blocks;
+    if (F32 && DH == 128 && rows <= 192) return launch_shape8<T, Sixteen>(c, x, ws, stream);
     return launch_shape8<T, Shape8<T, DH, 64, 4, 1, 64, 2, 2>>(c, x, ws, stream);
   }
 }

@@ -126,3 +126,17 @@ def test_hundreds_of_requests_against_float64(lib, cuda, group, dim, page, new, 
     s = Step8(requests, 2 * group, 2, dim, page, dtype, seed=new)
     s.attend()
     s.check()
+
+
+@pytest.mark.parametrize("dtype", [F32, F16, BF16])
+@pytest.mark.parametrize("dim,page", [(256, 16), (128, 24), (112, 7), (64, 24)])
+@pytest.mark.parametrize("new", [5, 12, 13, 48, 49])
+def test_rows_around_the_kernels_borders(lib, cuda, new, dim, page, dtype):
+    """20 to 196 rows per kv head where no tcgen05 kernel takes the cache."""
+    s = Step8([(new, 900), (new // 2, 40), (1, 2000), (new, new)], 8, 2, dim, page, dtype, seed=new)
+    s.attend()
+    s.check()
+    first = s.o.clone()
+    s.attend()
+    torch.cuda.synchronize()
+    assert torch.equal(first, s.o)
