@@ -18,6 +18,14 @@ def pytest_configure(config):
     config.addinivalue_line("markers", "gpu: needs a B200 (sm_100a) GPU")
 
 
+def pytest_collection_modifyitems(items):
+    """Where the reference's library is not built, the tests that compare with it (`apis`) come
+    last: a run that stops at the first failure has run all others by then."""
+    from oracle import oracle as orc
+    if orc.ref() is None:
+        items.sort(key=lambda item: "apis" in getattr(item, "fixturenames", ()))
+
+
 @pytest.fixture(scope="session")
 def lib():
     import eshkol_transformer_b200 as etb
