@@ -47,8 +47,9 @@ struct VerifyArgs {
 
 // A probability as the rules read it: NaN and negative ones are 0, the largest is 1.
 __device__ __forceinline__ float probability(float p) { return p > 0.0f ? fminf(p, 1.0f) : 0.0f; }
-// max(p - q, 0), in 32 bits: a conversion to 64 costs four times a difference, and its
-// rounding moves a draw's border by less than 2^-24 of one token's weight.
+// max(p - q, 0), in 32 bits: a conversion to 64 costs four times a difference (64 requests 28 us
+// with two, 22 with one).  Each is off by at most 2^-24 of itself, a draw's border by 2^-24 of the
+// running sum before it.
 __device__ __forceinline__ double weight(float p, float q) {
   return (double)fmaxf(probability(p) - probability(q), 0.0f);
 }

@@ -185,7 +185,8 @@ typedef struct et_b200_paged_cache_v1 {
  * page_size].  A request may bring no token; a token at a negative position
  * is not stored and sees no key.  Rows of no request are not written, and
  * nothing depends on them.  max_new (the host's idea of the largest request)
- * only picks the kernel; max_length is not used so far.  The arrays are device
+ * only picks the kernel, and with it the roundings that the calls state for
+ * few query rows and for many; max_length is not used so far.  The arrays are device
  * memory, read when the kernels run; what in them leads outside the pools or
  * tensors is not followed but recorded in *status (never cleared here): */
 enum {
@@ -300,7 +301,9 @@ int32_t et_b200_paged_append8_v1(const et_b200_paged_cache8_v1 *cache,
  * included.
  * Precision: scores, statistics and sums are f32.  q' is carried as binary16 of a
  * scale per row, at f32 and f16 with its residual (about 22 bits; at f16 not in the
- * chunks below); the probabilities as binary16, at f32 with their residual.
+ * chunks below); the probabilities as binary16, at f32 with their residual, in the
+ * chunks below to no less than 2^-36 of a row's largest, else times their values'
+ * scales and to no less than 2^-37 of the largest such product.
  * Elements and their products with scales that are powers of two (or 0), as the
  * append writes them, are exact.  Chunks (more than 48 query rows per kv head, as
  * max_new tells, at f32 up to 64 dims more than 64; head_dim up to 128) over pages of a
@@ -355,7 +358,8 @@ int32_t et_b200_sample_v1(const et_b200_sampling_v1 *shape, const void *logits,
  * filters: probs (f32 [rows, vocabulary], rows probs_stride floats apart) receives
  * w / total of every token that the filters keep and 0 for all others.  Weights
  * below 2^-36 of the likeliest count as 0, as there; others are f32 (not fixed
- * point), so probabilities are right to some 2^-22 of themselves however small.  A
+ * point) over a fixed-point total, so a probability, however small, is right to
+ * 2^-21 + n 2^-36 of itself, n the number of kept tokens (the latter is 6e-5 where 2^22 are).  A
  * row that takes the most likely token gets a single 1, a row without a token to
  * draw only zeros.  probs must not overlap the logits. */
 int32_t et_b200_probabilities_v1(const et_b200_sampling_v1 *shape,
