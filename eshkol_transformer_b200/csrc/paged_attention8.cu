@@ -11,7 +11,10 @@
 // s_j - m + x_j so far, so that value rows of any magnitudes stand side by side, and
 // o's sums are multiplied by 2^D where a tile ends.  Queries are binary16 times 2^-e of
 // their row.  At f32 queries and weights carry the residual of that rounding (22 bits), at
-// f16 the queries do.
+// f16 the queries do.  At bf16 11 bits of a query stand beside results of 8: over 64 requests to 8,192
+// keys the output is 1.68e-3 off 64 bits (norms), with sums in 32 bits throughout 1.64e-3, both the
+// output's own rounding; the residual would bring the two from 1.1e-3 to 2e-4 of each other for
+// 2 % of single tokens' time and 21 % of drafts' (72 us to 87).
 //
 // Tiles of 8 or 16 rows (few8_kernel): products have the keys as rows, S^T = K Q^T and
 // O^T = V^T P^T with the queries as 8 or 16 columns, and warps split the keys of a block:
@@ -29,7 +32,11 @@
 // bf16, 697 MB: 140 us, 76 % of the copy rate); a block of 128 keys then waits for bytes
 // (2.7 of the 6.7 cycles between two instructions of a warp), issue slots are 41 % busy.  Three
 // thread blocks an SM with two stages each hide that best: two with three stages 177 us,
-// four of 64 keys 151.  Drafts (32 requests of 5 tokens, 20 rows a head, to 4,000 keys:
+// four of 64 keys 151.  Rows of 64 dims take 69 us for 64 requests of up to 4,000 keys (174 MB, 2.5
+// TB/s): the work of a key is that of 128 dims (78 us) for half its bytes, and a stage holds half as
+// many (a warp waits 3.9 of its 7.8 cycles an instruction for memory, issue slots 41 %).  f32 of 128
+// dims takes 87 us, its residuals' products and conversions (issue slots 51 %); 256 dims 147 us, two
+// thread blocks an SM (35 %); without TMA 97 us, copies in the arithmetic warps (54 %).  Drafts (32 requests of 5 tokens, 20 rows a head, to 4,000 keys:
 // 71 us, 2.5 TB/s) read the cache twice, from the L2 the second time, and are bound by
 // the latency of a step's chain (conversion, products, exponentials, products; issue
 // slots 41 %, tensor pipe 19 %): tiles of 8 rows 76 us, of 32 rows as two warps' halves 107.

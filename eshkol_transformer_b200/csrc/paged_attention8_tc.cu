@@ -12,7 +12,8 @@
 // powers of two that is exact down to 2^-21 of the largest (binary16 holds 2^-24 to
 // 2^15, an element 2^-9 to 448); other scales round each element to 11 bits.
 // Queries are binary16 times 2^-e of their row, weights binary16 times 2^11 below a
-// standing maximum that allows 2^4: 11 bits, more than a bf16 result keeps.  At f32 both carry
+// standing maximum that allows 2^4: 11 bits, more than a bf16 result keeps (queries with their residual do not
+// fit shared memory beside two halves of 128 dims).  At f32 both carry
 // the residual of that rounding (22 bits, two products instead of one), and the products of a
 // block are added to f32 sums in tensor memory.
 //

@@ -7,10 +7,12 @@
 // many as a row has (a power of two up to 32) a row of K and the row of V beside it,
 // whose maxima they exchange by shuffles.  The rows are requested before the chain
 // offsets, length, page, tables is followed, as in the append of wider types (paged_kv.cu).
-// 11 ragged prompts (15,600 tokens, 8 heads x 128, bf16, 98 MB): 23.6 us on the device, 4.2 TB/s;
-// issue slots 65 % busy (rotation, maxima, conversion) while a warp waits 2 of its 7
-// cycles an instruction for its loads.  A warp a token of 4 rows a lane; four tokens a warp
-// 30.6 us, two rows or one a lane 28 to 34.  One token: 7.4 us, the call on the host.
+// 11 ragged prompts (15,600 tokens, 8 heads x 128, bf16 or f16, 98 MB): 28.2 us on the device where
+// the inputs come from memory, 3.5 TB/s (24.7 us where the L2 holds a part of them from the call
+// before); f32 (162 MB) 40.5 us, 4.0 TB/s.  Issue slots are 65 % busy (rotation, maxima, conversion)
+// while a warp waits 2 of its 7 cycles an instruction for its loads.  A warp a token of 4 rows a
+// lane; with the L2's help, four tokens a warp 30.6 us, two rows or one a lane 28 to 34.  One token:
+// 7.4 us a call (the host), 3.9 us on the device.
 #include <type_traits>
 
 #include "attention_tc.cuh"

@@ -8,10 +8,11 @@
 // segments' sums come together in every block, whose scan finds the segment of the
 // draw, and one warp walks it.  Segments, and with them all orders of summation, depend
 // on the vocabulary alone.
-// 64 requests of 5 rows of 128,259 (66 MB): 20.7 us, 3.2 TB/s; a thread block an SM holds two
-// segments a warp, so the start, the cluster's barriers (3.5 of the 13 cycles between two
-// instructions of a warp) and the conversions to f64 stand beside the reading.  One request
-// of 32,768: 10.5 us, the latency of those steps.
+// 64 requests of 5 rows of 128,259 (66 MB): 19.3 us on the device, other inputs each time, 3.4 TB/s;
+// without draft distributions (33 MB) 17.5 us.  A thread block an SM holds two segments a warp,
+// so the start, the cluster's barriers (3.5 of the 13 cycles between two instructions of a warp)
+// and the conversions to f64 stand beside the reading, and take as long for half the bytes.  One
+// request of 32,768: 9.5 us, the latency of those steps.
 #include <math.h>
 
 #include <cooperative_groups.h>
